@@ -77,11 +77,18 @@ class Hop(ctypes.Structure):
                 ("coo_row", ctypes.c_void_p), ("coo_col", ctypes.c_void_p), ("frontier", ctypes.c_void_p)]
 
 
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("copy", ctypes.c_void_p), ("n", ctypes.c_int64),
+                ("at", ctypes.c_int64), ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32),
+                ("copy_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/dgs_b200.h declares
 _I32, _I64, _U64, _VP, _SZ = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_size_t
 _DP, _SP = ctypes.POINTER(ChunkDesc), ctypes.POINTER(Segments)
 _I64P = ctypes.POINTER(ctypes.c_int64)
 _HP = ctypes.POINTER(Hop)
+_AP, _F32, _F64 = ctypes.POINTER(AdamWTensor), ctypes.c_float, ctypes.c_double
 ABI_SIGNATURES = {
     "dgs_last_error": (ctypes.c_char_p, []),
     "dgs_device_check": (ctypes.c_int, []),
@@ -133,6 +140,20 @@ ABI_SIGNATURES = {
     "dgs_cache_table_slots": (_I64, [_I64]),
     "dgs_cache_build": (ctypes.c_int, [_VP, _VP, _I32, _I64, _VP, _VP, _I64, _VP, _VP]),
     "dgs_cache_fetch": (ctypes.c_int, [_VP, _I64, _DP, _VP, _I32, _I64, _I64, _VP, _VP, _I64, _VP, _VP, _VP]),
+    "dgs_layer_norm": (ctypes.c_int, [_VP, _I64, _I32, _VP, _VP, _I32, _I64, _I64, _F32, _VP, _VP, _VP, _VP]),
+    "dgs_layer_norm_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "dgs_layer_norm_backward": (ctypes.c_int, [_VP, _I64, _VP, _I64, _I32, _VP, _I32, _VP, _VP, _I64, _I64, _VP, _VP, _VP, _VP,
+                                               _SZ, _VP]),
+    "dgs_linear_cross_entropy_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
+    "dgs_linear_cross_entropy": (ctypes.c_int, [_VP, _I64, _VP, _I64, _I32, _VP, _I32, _I64, _I64, _I64, _I64, _VP, _VP, _VP,
+                                                _SZ, _VP, _VP]),
+    "dgs_linear_cross_entropy_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
+    "dgs_linear_cross_entropy_backward": (ctypes.c_int, [_VP, _VP, _I64, _VP, _I64, _I32, _VP, _I32, _VP, _I64, _I64, _I64, _I64,
+                                                         _VP, _VP, _VP, _SZ, _VP, _VP]),
+    "dgs_adamw_slot_elems": (_I64, [_I64]),
+    "dgs_adamw_step": (ctypes.c_int, [_AP, _I32, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _VP]),
+    "dgs_adamw_step_8bit": (ctypes.c_int, [_AP, _I32, _VP, _VP, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _VP]),
+    "dgs_adamw_state_values": (ctypes.c_int, [_VP, _I32, _VP, _I64, _VP, _VP]),
 }
 
 
@@ -335,3 +356,5 @@ def block_csc(coo_row, coo_col, n_dst, rows_sorted=True):
 # placement policy (capacity planning in the reference's priority order, free-memory rule, renumbering by degree)
 from .placement import (CACHE_PRIORITY, get_available_memory, permute_edge_tensor, plan_capacities,  # noqa: E402,F401
                         reduce_min_over_ranks, renumber_by_degree)
+# the training step behind the samplers
+from .training import AdamW, layer_norm, linear_cross_entropy  # noqa: E402,F401

@@ -25,6 +25,9 @@ ABI_SOURCES = [
     "kernels/sample.cu",
     "kernels/relabel.cu",
     "kernels/blocks.cu",
+    "kernels/norm.cu",
+    "kernels/cross_entropy.cu",
+    "kernels/adamw.cu",
     "host/error.cc",
     "host/comm.cc",
     "host/store.cc",
@@ -37,6 +40,7 @@ HEADERS = [
     "kernels/launchers.h",
     "kernels/relabel_device.cuh",
     "kernels/sample_device.cuh",
+    "kernels/train_common.cuh",
     "host/comm.h",
     "../../include/dgs_b200.h",
 ]
@@ -113,7 +117,7 @@ def build_binding(force=False, verbose=False):
 
     src = os.path.join(CSRC, "binding", "ops.cc")
     hdrs = [os.path.join(ROOT, "include", "dgs_b200.h")] + \
-        [os.path.join(CSRC, "binding", h) for h in ("chunk_tensor.h", "host_words.h", "pipeline.h")]
+        [os.path.join(CSRC, "binding", h) for h in ("chunk_tensor.h", "host_words.h", "pipeline.h", "training.h")]
     out = binding_path()
     stamp = out + ".sha"
     dig = _digest([src] + hdrs, torch.__version__)

@@ -4,7 +4,7 @@
 // of include/dgs_b200.h.  Only this directory (binding/) sees torch types; every
 // kernel launch goes through an extern "C" entry point.  chunk_tensor.h holds the
 // ChunkTensor class, host_words.h the pinned size / status words leased per call,
-// pipeline.h the BlockPipeline class (several mini-batches in flight).
+// pipeline.h the BlockPipeline class (several mini-batches in flight), training.h the operators of a training step.
 //
 // Conventions kept from the reference: one process per GPU, tensors returned
 // on the current CUDA device, ChunkTensor construction/destruction collective
@@ -30,6 +30,7 @@
 #include "chunk_tensor.h"
 #include "host_words.h"
 #include "pipeline.h"
+#include "training.h"
 
 namespace dgs {
 namespace {
@@ -566,5 +567,13 @@ TORCH_LIBRARY(dgs_ops, m) {
       .def("_CAPI_fetch_data_chunk_tensor", &FetchDataWithChunkTensorCUDA)
       .def("_CAPI_get_unique_id", &GetUniqueId)
       .def("_CAPI_set_nccl", &SetNCCL)
-      .def("_CAPI_get_current_allocated", &GetCurrAllocated);
+      .def("_CAPI_get_current_allocated", &GetCurrAllocated)
+      // additions: a training step on what the samplers deliver, see training.h
+      .def("_CAPI_layer_norm", &LayerNormCUDA)
+      .def("_CAPI_layer_norm_backward", &LayerNormBackwardCUDA)
+      .def("_CAPI_linear_cross_entropy", &LinearCrossEntropyCUDA)
+      .def("_CAPI_linear_cross_entropy_backward", &LinearCrossEntropyBackwardCUDA)
+      .def("_CAPI_adamw_step", &AdamWStepCUDA)
+      .def("_CAPI_adamw_step_8bit", &AdamWStep8bitCUDA)
+      .def("_CAPI_adamw_state_values", &AdamWStateValuesCUDA);
 }

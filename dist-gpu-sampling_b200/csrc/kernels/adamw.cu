@@ -1,0 +1,308 @@
+// One AdamW step over a list of tensors, moments in 32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+//   p = (1 - lr wd) p - (m / (sqrt(v) / sqrt(1 - b2^t) + eps)) (lr / (1 - b1^t)),  copy = p in the copy's type
+//
+// Every element is read and written once: bound by HBM.  The moments lie in flat buffers in which every tensor has a slot
+// of whole 256-element blocks, so a warp's 256 elements are one block of the 8-bit form and the list needs three pointers
+// a tensor.  The list travels in the kernel's parameters (nothing is copied to the device and nothing is kept), a CTA finds
+// its tensor by bisecting the list's chunk numbers.
+//
+// 8 bits, per block: m = a sgn(c) (c / 127)^2 with a = max |m|, and sqrt(v) = a (c / 255)^2 with a = max sqrt(v).  The
+// squares give small values finer steps; the second moment is held as its root because that is what divides, and a root
+// that is not zero never gets the code zero, which would make its element's step arbitrarily large.
+//
+// The arithmetic is 32-bit, operation by operation as written above: no contraction to fused multiply-add, IEEE division
+// and square root.  A moment that falls between two codes is then rounded the same way wherever the formula is evaluated
+// in 32 bits; the kernel waits for HBM, so the longer instructions are hidden.
+#include <cmath>
+#include <type_traits>
+
+#include "train_common.cuh"
+
+namespace dgs {
+namespace {
+
+constexpr int AW_THREADS = 256;
+constexpr int AW_BLOCK = 256;                                // elements that share a scale: 8 a lane
+constexpr int AW_VALUES = 8;
+constexpr int64_t AW_CHUNK = AW_THREADS * AW_VALUES;         // elements a CTA takes at a time: 8 blocks
+constexpr int AW_SMALL_LIST = 64, AW_LARGE_LIST = 512;       // tensors of one launch (parameters of 3.6 and 28 KB)
+
+struct Entry {
+  void* param;
+  const void* grad;
+  void* copy;
+  int64_t n;
+  int64_t at;          // first element of the slot in the moments
+  int64_t first_chunk;
+  int8_t param_dtype, grad_dtype, copy_dtype;
+  int8_t whole;        // every pointer allows accesses of 8 elements
+};
+template <int N>
+struct List {
+  Entry e[N];
+};
+struct Scalars {
+  float keep, b1, c1, b2, c2, root2, eps, step;
+};
+
+struct Moments32 {
+  float* m;
+  float* v;
+};
+struct Moments8 {
+  int8_t* m;
+  float* m_scale;
+  uint8_t* v;
+  float* v_scale;
+};
+
+__device__ __forceinline__ float update(float p, float g, float& m, float& v, const Scalars& k) {
+  m = __fadd_rn(__fmul_rn(m, k.b1), __fmul_rn(g, k.c1));
+  v = __fadd_rn(__fmul_rn(v, k.b2), __fmul_rn(__fmul_rn(g, g), k.c2));
+  const float under = __fadd_rn(__fmul_rn(__fsqrt_rn(v), k.root2), k.eps);
+  return __fsub_rn(__fmul_rn(p, k.keep), __fmul_rn(__fdiv_rn(m, under), k.step));
+}
+
+// the largest of the warp's non-negative values; a NaN counts as larger than any (its bits are)
+__device__ __forceinline__ float warp_max_bits(uint32_t bits) { return __uint_as_float(__reduce_max_sync(FULL_MASK, bits)); }
+
+__device__ __forceinline__ float first_moment(int c, float scale) {
+  const float u = __fmul_rn(static_cast<float>(c), 1.0f / 127.0f);
+  return __fmul_rn(__fmul_rn(u, fabsf(u)), scale);
+}
+__device__ __forceinline__ float second_moment(int c, float scale) {
+  const float u = __fmul_rn(static_cast<float>(c), 1.0f / 255.0f);
+  const float r = __fmul_rn(__fmul_rn(u, u), scale);
+  return __fmul_rn(r, r);
+}
+
+template <int N, typename Moments>
+__global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant__ List<N> list, const int count,
+                                                           const int64_t chunks, const Moments mo,
+                                                           const __grid_constant__ Scalars k) {
+  constexpr bool kEight = std::is_same<Moments, Moments8>::value;
+  pdl_enter();
+  for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (list.e[mid].first_chunk <= chunk) lo = mid;
+      else hi = mid - 1;
+    }
+    const Entry& e = list.e[lo];
+    const int64_t i = (chunk - e.first_chunk) * AW_CHUNK + static_cast<int64_t>(threadIdx.x) * AW_VALUES;
+    const int64_t left = e.n - i;  // elements of the tensor from this thread's first on
+    // whole warps leave together: a warp that has any element takes part with all its lanes (the scales of a block)
+    if (e.n - (i - static_cast<int64_t>(threadIdx.x & 31) * AW_VALUES) <= 0) continue;
+    float p[AW_VALUES], g[AW_VALUES], m[AW_VALUES], v[AW_VALUES];
+    const bool full = e.whole && left >= AW_VALUES;
+    if (full) {
+      load_vec_as_float<AW_VALUES>(e.param, e.param_dtype, i, p);
+      load_vec_as_float<AW_VALUES>(e.grad, e.grad_dtype, i, g);
+    } else {
+#pragma unroll
+      for (int j = 0; j < AW_VALUES; ++j) {
+        p[j] = j < left ? load_as_float(e.param, e.param_dtype, i + j) : 0.0f;
+        g[j] = j < left ? load_as_float(e.grad, e.grad_dtype, i + j) : 0.0f;
+      }
+    }
+    const int64_t at = e.at + i;
+    if constexpr (kEight) {
+      Vec<int8_t, AW_VALUES> mc;
+      Vec<uint8_t, AW_VALUES> vc;
+      // a slot is whole blocks, so all eight codes are there; those beyond the tensor's end count as zero
+      mc = *reinterpret_cast<const Vec<int8_t, AW_VALUES>*>(mo.m + at);
+      vc = *reinterpret_cast<const Vec<uint8_t, AW_VALUES>*>(mo.v + at);
+      const float ma = mo.m_scale[at / AW_BLOCK], va = mo.v_scale[at / AW_BLOCK];
+#pragma unroll
+      for (int j = 0; j < AW_VALUES; ++j) {
+        m[j] = j < left ? first_moment(mc.v[j], ma) : 0.0f;
+        v[j] = j < left ? second_moment(vc.v[j], va) : 0.0f;
+      }
+    } else {
+      load_vec<float, AW_VALUES>(mo.m + at, m);
+      load_vec<float, AW_VALUES>(mo.v + at, v);
+    }
+#pragma unroll
+    for (int j = 0; j < AW_VALUES; ++j) p[j] = update(p[j], g[j], m[j], v[j], k);
+    if (full) {
+      store_vec_from_float<AW_VALUES>(e.param, e.param_dtype, i, p);
+      if (e.copy != nullptr) store_vec_from_float<AW_VALUES>(e.copy, e.copy_dtype, i, p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < AW_VALUES; ++j) {
+        if (j < left) {
+          store_from_float(e.param, e.param_dtype, i + j, p[j]);
+          if (e.copy != nullptr) store_from_float(e.copy, e.copy_dtype, i + j, p[j]);
+        }
+      }
+    }
+    if constexpr (kEight) {
+      uint32_t mb = 0, vb = 0;
+#pragma unroll
+      for (int j = 0; j < AW_VALUES; ++j) {
+        if (j >= left) m[j] = v[j] = 0.0f;
+        v[j] = __fsqrt_rn(v[j]);
+        mb = max(mb, __float_as_uint(fabsf(m[j])));
+        vb = max(vb, __float_as_uint(fabsf(v[j])));
+      }
+      const float ma = warp_max_bits(mb), va = warp_max_bits(vb);
+      Vec<int8_t, AW_VALUES> mc;
+      Vec<uint8_t, AW_VALUES> vc;
+#pragma unroll
+      for (int j = 0; j < AW_VALUES; ++j) {
+        // a scale of zero, or one that is no number, leaves the code zero
+        const float tm = ma > 0.0f ? __fsqrt_rn(__fdiv_rn(fabsf(m[j]), ma)) : 0.0f;
+        const float tv = va > 0.0f ? __fsqrt_rn(__fdiv_rn(v[j], va)) : 0.0f;
+        const int cm = __float2int_rn(__fmul_rn(tm, 127.0f));
+        int cv = __float2int_rn(__fmul_rn(tv, 255.0f));
+        if (v[j] > 0.0f && cv < 1) cv = 1;
+        mc.v[j] = static_cast<int8_t>(m[j] < 0.0f ? -cm : cm);
+        vc.v[j] = static_cast<uint8_t>(cv);
+      }
+      *reinterpret_cast<Vec<int8_t, AW_VALUES>*>(mo.m + at) = mc;
+      *reinterpret_cast<Vec<uint8_t, AW_VALUES>*>(mo.v + at) = vc;
+      if ((threadIdx.x & 31) == 0) {
+        mo.m_scale[at / AW_BLOCK] = ma;
+        mo.v_scale[at / AW_BLOCK] = va;
+      }
+    } else {
+      if (left >= AW_VALUES) {
+        store_vec<float, AW_VALUES>(mo.m + at, m);
+        store_vec<float, AW_VALUES>(mo.v + at, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < AW_VALUES; ++j) {
+          if (j < left) {
+            mo.m[at + j] = m[j];
+            mo.v[at + j] = v[j];
+          }
+        }
+      }
+    }
+  }
+}
+
+template <typename Code>
+__global__ void __launch_bounds__(AW_THREADS) adamw_values_kernel(const Code* __restrict__ codes, const float* __restrict__ scales,
+                                                                  const int64_t n, float* __restrict__ out) {
+  pdl_enter();
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * AW_THREADS + threadIdx.x) * AW_VALUES; i < n;
+       i += static_cast<int64_t>(gridDim.x) * AW_CHUNK) {
+    const Vec<Code, AW_VALUES> c = *reinterpret_cast<const Vec<Code, AW_VALUES>*>(codes + i);
+    const float scale = scales[i / AW_BLOCK];
+    float v[AW_VALUES];
+#pragma unroll
+    for (int j = 0; j < AW_VALUES; ++j)
+      v[j] = std::is_signed<Code>::value ? first_moment(c.v[j], scale) : second_moment(c.v[j], scale);
+    store_vec<float, AW_VALUES>(out + i, v);
+  }
+}
+
+int make_scalars(const char* who, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step, Scalars* k) {
+  DGS_REQUIRE(lr >= 0.0 && eps >= 0.0 && weight_decay >= 0.0, DGS_ERR_INVALID, "%s: lr, eps and weight_decay must be >= 0", who);
+  DGS_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, DGS_ERR_INVALID, "%s: betas must lie in [0, 1)", who);
+  DGS_REQUIRE(step >= 1, DGS_ERR_INVALID, "%s: steps count from 1", who);
+  const double t = static_cast<double>(step);
+  k->keep = static_cast<float>(1.0 - lr * weight_decay);
+  k->b1 = static_cast<float>(beta1);
+  k->c1 = static_cast<float>(1.0 - beta1);
+  k->b2 = static_cast<float>(beta2);
+  k->c2 = static_cast<float>(1.0 - beta2);
+  k->root2 = static_cast<float>(1.0 / sqrt(1.0 - pow(beta2, t)));
+  k->eps = static_cast<float>(eps);
+  k->step = static_cast<float>(lr / (1.0 - pow(beta1, t)));
+  return DGS_OK;
+}
+
+int check_tensor(const char* who, const dgs_adamw_tensor& t) {
+  DGS_REQUIRE(t.n >= 0, DGS_ERR_INVALID, "%s: a tensor of %lld elements", who, static_cast<long long>(t.n));
+  DGS_REQUIRE(t.at >= 0 && t.at % AW_BLOCK == 0, DGS_ERR_INVALID, "%s: a slot begins at a multiple of %d elements", who, AW_BLOCK);
+  DGS_REQUIRE(t.n == 0 || (t.param != nullptr && t.grad != nullptr), DGS_ERR_INVALID, "%s: null tensor", who);
+  DGS_REQUIRE(dtype_bytes(t.param_dtype) != 0 && dtype_bytes(t.grad_dtype) != 0 &&
+                  (t.copy == nullptr || dtype_bytes(t.copy_dtype) != 0),
+              DGS_ERR_UNSUPPORTED, "%s: element type", who);
+  return DGS_OK;
+}
+
+template <int N, typename Moments>
+int launch_list(const dgs_adamw_tensor* ts, int32_t count, const Moments& mo, const Scalars& k, cudaStream_t s) {
+  List<N> list;
+  int used = 0;
+  int64_t chunks = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    const dgs_adamw_tensor& t = ts[i];
+    if (t.n == 0) continue;
+    const bool whole = aligned_to(t.param, 16) && aligned_to(t.grad, 16) && aligned_to(t.copy, 16);
+    list.e[used++] = Entry{t.param, t.grad, t.copy, t.n, t.at, chunks, static_cast<int8_t>(t.param_dtype),
+                           static_cast<int8_t>(t.grad_dtype), static_cast<int8_t>(t.copy_dtype), static_cast<int8_t>(whole)};
+    chunks += (t.n + AW_CHUNK - 1) / AW_CHUNK;
+  }
+  if (used == 0) return DGS_OK;
+  const int64_t most = static_cast<int64_t>(sm_count()) * 8;
+  DGS_CUDA_TRY(launch_training(adamw_kernel<N, Moments>, dim3(static_cast<unsigned>(chunks < most ? chunks : most)), AW_THREADS, 0,
+                               s, list, used, chunks, mo, k));
+  return DGS_OK;
+}
+
+template <typename Moments>
+int step_all(const char* who, const dgs_adamw_tensor* ts, int32_t count, const Moments& mo, const Scalars& k, cudaStream_t s) {
+  DGS_REQUIRE(count >= 0 && (count == 0 || ts != nullptr), DGS_ERR_INVALID, "%s: %d tensors", who, count);
+  for (int32_t i = 0; i < count; ++i)
+    if (int rc = check_tensor(who, ts[i])) return rc;
+  for (int32_t done = 0; done < count;) {
+    const int32_t left = count - done;
+    const int32_t now = left < AW_LARGE_LIST ? left : AW_LARGE_LIST;
+    const int rc = now <= AW_SMALL_LIST ? launch_list<AW_SMALL_LIST>(ts + done, now, mo, k, s)
+                                        : launch_list<AW_LARGE_LIST>(ts + done, now, mo, k, s);
+    if (rc != DGS_OK) return rc;
+    done += now;
+  }
+  return DGS_OK;
+}
+
+}  // namespace
+}  // namespace dgs
+
+using namespace dgs;
+
+extern "C" int64_t dgs_adamw_slot_elems(int64_t n) { return n <= 0 ? 0 : (n + AW_BLOCK - 1) / AW_BLOCK * AW_BLOCK; }
+
+extern "C" int dgs_adamw_step(const dgs_adamw_tensor* tensors, int32_t count, float* exp_avg, float* exp_avg_sq, double lr,
+                              double beta1, double beta2, double eps, double weight_decay, int64_t step, dgs_stream_t stream) {
+  Scalars k;
+  if (int rc = make_scalars("adamw_step", lr, beta1, beta2, eps, weight_decay, step, &k)) return rc;
+  DGS_REQUIRE(count <= 0 || (exp_avg != nullptr && exp_avg_sq != nullptr && aligned_to(exp_avg, 16) && aligned_to(exp_avg_sq, 16)),
+              DGS_ERR_INVALID, "adamw_step: moments that are null or not 16-byte aligned");
+  return step_all("adamw_step", tensors, count, Moments32{exp_avg, exp_avg_sq}, k, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dgs_adamw_step_8bit(const dgs_adamw_tensor* tensors, int32_t count, int8_t* exp_avg, float* exp_avg_scale,
+                                   uint8_t* exp_avg_sq, float* exp_avg_sq_scale, double lr, double beta1, double beta2,
+                                   double eps, double weight_decay, int64_t step, dgs_stream_t stream) {
+  Scalars k;
+  if (int rc = make_scalars("adamw_step_8bit", lr, beta1, beta2, eps, weight_decay, step, &k)) return rc;
+  DGS_REQUIRE(count <= 0 || (exp_avg != nullptr && exp_avg_sq != nullptr && exp_avg_scale != nullptr &&
+                             exp_avg_sq_scale != nullptr && aligned_to(exp_avg, 8) && aligned_to(exp_avg_sq, 8)),
+              DGS_ERR_INVALID, "adamw_step_8bit: moments that are null or not 8-byte aligned");
+  return step_all("adamw_step_8bit", tensors, count, Moments8{exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale}, k,
+                  static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dgs_adamw_state_values(const void* codes, int32_t second, const float* scales, int64_t n, float* out,
+                                      dgs_stream_t stream) {
+  DGS_REQUIRE(n >= 0 && n % AW_BLOCK == 0, DGS_ERR_INVALID, "adamw_state_values: whole blocks of %d codes", AW_BLOCK);
+  if (n == 0) return DGS_OK;
+  DGS_REQUIRE(codes != nullptr && scales != nullptr && out != nullptr && aligned_to(codes, 8) && aligned_to(out, 16), DGS_ERR_INVALID,
+              "adamw_state_values: null or unaligned argument");
+  const int64_t need = (n + AW_CHUNK - 1) / AW_CHUNK, most = static_cast<int64_t>(sm_count()) * 8;
+  const dim3 grid(static_cast<unsigned>(need < most ? need : most));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (second != 0)
+    DGS_CUDA_TRY(launch_training(adamw_values_kernel<uint8_t>, grid, AW_THREADS, 0, s, static_cast<const uint8_t*>(codes), scales, n, out));
+  else
+    DGS_CUDA_TRY(launch_training(adamw_values_kernel<int8_t>, grid, AW_THREADS, 0, s, static_cast<const int8_t*>(codes), scales, n, out));
+  return DGS_OK;
+}

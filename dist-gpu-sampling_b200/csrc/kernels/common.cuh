@@ -81,7 +81,7 @@ __device__ __forceinline__ void pdl_enter() {
 }
 
 // which launch this is; DGS_NO_PDL=1 turns the attribute off everywhere, DGS_PDL_OFF_MASK=<hex> per site
-enum LaunchSite { SITE_INIT = 0, SITE_PLAN, SITE_SAMPLE, SITE_INSERT, SITE_NUMBER = 5, SITE_LOOKUP, SITE_GATHER };
+enum LaunchSite { SITE_INIT = 0, SITE_PLAN, SITE_SAMPLE, SITE_INSERT, SITE_NUMBER = 5, SITE_LOOKUP, SITE_GATHER, SITE_TRAINING };
 bool chained_launches_enabled(int site);  // host/error.cc
 
 template <typename... KArgs, typename... Args>

@@ -386,6 +386,83 @@ DGS_API int dgs_cache_fetch(const void* cpu_data, int64_t cpu_rows, const dgs_ch
                     const void* key_buf, const void* value_buf, int64_t slots,
                     void* out, int32_t* status, dgs_stream_t stream);
 
+/* ---- operators of a training step --------------------------------------- */
+/* What a consumer of the batches runs on them: layer norm, softmax cross entropy
+ * against a large vocabulary, an AdamW step.  No counterparts in the reference,
+ * whose trainers take these from torch.  Sums, statistics and moments are in 32
+ * bits whatever the element type; results are rounded once.  Nothing is kept from
+ * one call for the next, and the same inputs give the same bits. */
+enum { DGS_F32 = 0, DGS_BF16 = 1, DGS_F16 = 2 };
+
+/* y = (x - mean) * rstd * weight + bias over rows of D elements, x_stride elements
+ * apart; y is contiguous.  weight and bias are of type param_dtype; weight == NULL:
+ * 1, bias == NULL: 0 (a bias needs a weight).  mean[n], rstd[n] are what the
+ * backward pass takes. */
+DGS_API int dgs_layer_norm(const void* x, int64_t x_stride, int32_t dtype, const void* weight, const void* bias,
+                           int32_t param_dtype, int64_t n, int64_t D, float eps, void* y, float* mean, float* rstd,
+                           dgs_stream_t stream);
+/* dx[n, D] (may be NULL), dweight[D] and dbias[D] (both or neither; of type
+ * param_dtype).  workspace: for the parameters' gradients alone, 16-byte aligned. */
+DGS_API size_t dgs_layer_norm_backward_workspace_bytes(int64_t n, int64_t D);
+DGS_API int dgs_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int32_t dtype,
+                                    const void* weight, int32_t param_dtype, const float* mean, const float* rstd,
+                                    int64_t n, int64_t D, void* dx, void* dweight, void* dbias, void* workspace,
+                                    size_t workspace_bytes, dgs_stream_t stream);
+
+/* Softmax cross entropy of the logits s_iv = hidden_i . weight_v, which are never
+ * all held at once:
+ *   lse_i = log sum_v exp(s_iv),  loss_i = lse_i - s_i,target_i
+ * hidden [n, D] and weight [V, D] have rows hidden_stride / weight_stride elements
+ * apart.  targets (int64 when ids64, else int32) equal to ignore_index give loss
+ * and lse 0, whatever stands in their rows; any other target outside [0, V) too,
+ * and DGS_ERR_RANGE in *status. */
+DGS_API size_t dgs_linear_cross_entropy_workspace_bytes(int64_t n, int64_t D, int64_t V, int32_t dtype);
+DGS_API int dgs_linear_cross_entropy(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
+                                     int32_t dtype, const void* target, int32_t ids64, int64_t n, int64_t D, int64_t V,
+                                     int64_t ignore_index, float* loss, float* lse, void* workspace, size_t workspace_bytes,
+                                     int32_t* status, dgs_stream_t stream);
+/* With G_iv = dloss_i (exp(s_iv - lse_i) - [v = target_i]), 0 in ignored rows:
+ *   dhidden = G weight [n, D],  dweight = G^T hidden [V, D]   (either may be NULL)
+ * lse as the forward call gave it.  The logits are computed again, piece by piece. */
+DGS_API size_t dgs_linear_cross_entropy_backward_workspace_bytes(int64_t n, int64_t D, int64_t V, int32_t dtype);
+DGS_API int dgs_linear_cross_entropy_backward(const float* dloss, const void* hidden, int64_t hidden_stride, const void* weight,
+                                              int64_t weight_stride, int32_t dtype, const void* target, int32_t ids64,
+                                              const float* lse, int64_t n, int64_t D, int64_t V, int64_t ignore_index,
+                                              void* dhidden, void* dweight, void* workspace, size_t workspace_bytes,
+                                              int32_t* status, dgs_stream_t stream);
+
+/* One AdamW step (decoupled weight decay, bias correction) over `count` tensors:
+ *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,
+ *   p = (1 - lr wd) p - lr / (1-b1^t) * m / (sqrt(v) / sqrt(1-b2^t) + eps)
+ * The moments of all tensors lie in flat buffers; a tensor's slot begins at element
+ * `at`, a multiple of 256, and is dgs_adamw_slot_elems(n) long (zero it at the
+ * start).  copy (may be NULL) receives the new parameters in copy_dtype.  The list
+ * is read during the call only.  Parameters, copies and slots of one list must not
+ * overlap. */
+typedef struct dgs_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* copy;
+  int64_t n;
+  int64_t at;
+  int32_t param_dtype, grad_dtype, copy_dtype;
+  int32_t reserved;
+} dgs_adamw_tensor;
+DGS_API int64_t dgs_adamw_slot_elems(int64_t n);
+DGS_API int dgs_adamw_step(const dgs_adamw_tensor* tensors, int32_t count, float* exp_avg, float* exp_avg_sq, double lr,
+                           double beta1, double beta2, double eps, double weight_decay, int64_t step, dgs_stream_t stream);
+/* The same with moments in 8 bits and a scale for every 256-element block:
+ * m = scale * sgn(c) * (c/127)^2 and sqrt(v) = scale * (c/255)^2, each code the
+ * nearest one (a second moment that is not zero keeps a code that is not), the scale
+ * the block's largest |m| / sqrt(v).  A gradient that is no finite number leaves
+ * the scale of its block no finite number. */
+DGS_API int dgs_adamw_step_8bit(const dgs_adamw_tensor* tensors, int32_t count, int8_t* exp_avg, float* exp_avg_scale,
+                                uint8_t* exp_avg_sq, float* exp_avg_sq_scale, double lr, double beta1, double beta2, double eps,
+                                double weight_decay, int64_t step, dgs_stream_t stream);
+/* The moments that n codes (whole blocks) stand for; second != 0: codes of v. */
+DGS_API int dgs_adamw_state_values(const void* codes, int32_t second, const float* scales, int64_t n, float* out,
+                                   dgs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
