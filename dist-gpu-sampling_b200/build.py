@@ -27,6 +27,7 @@ ABI_SOURCES = [
     "kernels/blocks.cu",
     "kernels/norm.cu",
     "kernels/cross_entropy.cu",
+    "kernels/cross_entropy_mma.cu",
     "kernels/adamw.cu",
     "host/error.cc",
     "host/comm.cc",
@@ -41,6 +42,8 @@ HEADERS = [
     "kernels/relabel_device.cuh",
     "kernels/sample_device.cuh",
     "kernels/train_common.cuh",
+    "kernels/tensor_core.cuh",
+    "kernels/cross_entropy.h",
     "host/comm.h",
     "../../include/dgs_b200.h",
 ]

@@ -135,6 +135,12 @@ inline CrossEntropyInputs cross_entropy_inputs(const char* op, const torch::Tens
 inline void lay_out(CrossEntropyInputs& in, const torch::Tensor& hidden, const torch::Tensor& weight, const torch::Tensor& target) {
   in.hidden = as_rows(hidden, in.D);
   in.weight = as_rows(weight, in.D);
+  // 16-bit rows of a multiple of 8 elements are fetched where they lie, which needs 16-byte boundaries
+  if (in.dtype != DGS_F32 && in.D % 8 == 0 && (in.weight.stride % 8 != 0 || reinterpret_cast<uintptr_t>(in.weight.t.data_ptr()) % 16 != 0)) {
+    in.weight.t = device_empty({in.V, in.D}, weight.scalar_type(), weight.device());
+    in.weight.t.copy_(weight);
+    in.weight.stride = in.D;
+  }
   in.target = target.contiguous();
 }
 }  // namespace

@@ -11,10 +11,13 @@
 // complete.  That is 8 n V D operations for a training step instead of 6 with the logits kept (n V values, 2.1 GB at
 // 8 192 rows and 65 537 classes).
 //
+// This file: the entry points, and the products of 32-bit operands on the CUDA cores (fused multiply-adds in 32 bits, which
+// the tensor cores do not have).  16-bit operands: cross_entropy_mma.cu.
+//
 // A first launch copies the hidden rows into packed rows and the targets into 32-bit words: rows without a valid target
 // become zero there, so that what stands in an ignored row (an infinity, say) reaches neither dh nor dW, and alignment
 // and strides no longer matter.
-#include "train_common.cuh"
+#include "cross_entropy.h"
 
 namespace dgs {
 namespace {
@@ -24,23 +27,6 @@ constexpr int CE_COLS = 128;            // classes of a tile
 constexpr int CE_K = 16;
 constexpr int CE_THREADS = 256;
 constexpr int64_t CE_PIECE_BYTES = int64_t(96) << 20;  // of G: what L2 (126 MB) holds beside the operands
-
-inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-inline int64_t tiles(int64_t v, int64_t per) { return (v + per - 1) / per; }
-
-// Slices of `cols` column tiles for `rows` row blocks on `slots` CTAs that run at once: the cut with the fewest tiles in
-// the busiest slot.
-inline int64_t slices_for(int64_t rows, int64_t cols, int64_t slots) {
-  int64_t best = 1, least = tiles(rows, slots) * cols;
-  for (int64_t s = 2; s <= cols && s <= slots; ++s) {
-    const int64_t cost = tiles(rows * s, slots) * tiles(cols, s);
-    if (cost < least) {
-      least = cost;
-      best = s;
-    }
-  }
-  return best;
-}
 
 // ---- packing -----------------------------------------------------------------------------------------------------
 template <typename T, typename IdT>
@@ -69,14 +55,14 @@ __global__ void __launch_bounds__(CE_THREADS) ce_pack_kernel(const T* __restrict
 // ---- products on the CUDA cores ------------------------------------------------------------------------------------
 // A tile of CE_ROWS x CE_COLS, eight by eight values a thread, operands staged through shared memory CE_K at a time.
 // KMAJOR: element (r, k) at p[r * stride + k]; else at p[k * stride + r].
-template <typename T, bool KMAJOR>
+template <bool KMAJOR>
 struct Operand {
-  const T* p;
+  const float* p;
   int64_t stride;
   int64_t rows;
   __device__ __forceinline__ float at(int64_t r, int64_t k, int64_t k_end) const {
     if (r >= rows || k >= k_end) return 0.0f;
-    return to_float<T>(KMAJOR ? p[r * stride + k] : p[k * stride + r]);
+    return KMAJOR ? p[r * stride + k] : p[k * stride + r];
   }
 };
 
@@ -85,8 +71,8 @@ struct Stage {
   float b[CE_K][CE_COLS + 4];
 };
 
-template <typename T, bool KMAJOR>
-__device__ __forceinline__ void fetch(const Operand<T, KMAJOR>& o, int64_t r0, int64_t k0, int64_t k_end, float (&v)[8]) {
+template <bool KMAJOR>
+__device__ __forceinline__ void fetch(const Operand<KMAJOR>& o, int64_t r0, int64_t k0, int64_t k_end, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int e = threadIdx.x + i * CE_THREADS;
@@ -106,8 +92,8 @@ __device__ __forceinline__ void stage(float (*s)[CE_ROWS + 4], const float (&v)[
 // rows (i < 4 ? i : 60 + i) + 4 * (thread / 16) of the tile, columns likewise with thread % 16
 __device__ __forceinline__ int tile_at(int who, int i) { return who * 4 + (i < 4 ? i : 60 + i); }
 
-template <typename TA, bool AK, typename TB, bool BK>
-__device__ __forceinline__ void tile_product(const Operand<TA, AK>& a, int64_t m0, const Operand<TB, BK>& b, int64_t n0, int64_t k0,
+template <bool AK, bool BK>
+__device__ __forceinline__ void tile_product(const Operand<AK>& a, int64_t m0, const Operand<BK>& b, int64_t n0, int64_t k0,
                                              int64_t k_end, Stage& sm, float (&acc)[8][8]) {
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
 #pragma unroll
@@ -151,8 +137,9 @@ struct StatsArgs {
   float* total;  // [slices][n]
 };
 
-template <typename T>
-__global__ void __launch_bounds__(CE_THREADS, 2) ce_stats_kernel(const Operand<T, true> h, const Operand<T, true> w,
+
+
+__global__ void __launch_bounds__(CE_THREADS, 2) ce_stats_kernel(const Operand<true> h, const Operand<true> w,
                                                                  const __grid_constant__ StatsArgs a) {
   __shared__ __align__(16) Stage sm;
   pdl_enter();
@@ -185,7 +172,8 @@ __global__ void __launch_bounds__(CE_THREADS, 2) ce_stats_kernel(const Operand<T
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
-      const float base = m == -INFINITY ? 0.0f : m;  // nothing but minus infinity so far: exp must not see their difference
+      // nothing but minus infinity so far: the exponential must not see their difference
+      const float base = m == -INFINITY ? 0.0f : m;
       float s = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += expf(acc[i][j] - base);
@@ -218,10 +206,10 @@ __global__ void __launch_bounds__(CE_THREADS) ce_join_kernel(const float* __rest
   const float base = m == -INFINITY ? 0.0f : m;
   float s = 0.0f;
   for (int64_t p = 0; p < parts; ++p) s += total[p * n + row] * expf(top[p * n + row] - base);
-  const float l = base + logf(s);
+  const float l = logf(s);
   const bool live = word[row] >= 0;
-  lse[row] = live ? l : 0.0f;
-  loss[row] = live ? l - target_logit[row] : 0.0f;
+  lse[row] = live ? base + l : 0.0f;
+  loss[row] = live ? (base - target_logit[row]) + l : 0.0f;  // logits of one size meet first: exact, or nearly
 }
 
 struct GradArgs {
@@ -235,8 +223,7 @@ struct GradArgs {
   float* g;  // [n][pitch]
 };
 
-template <typename T>
-__global__ void __launch_bounds__(CE_THREADS, 2) ce_grad_kernel(const Operand<T, true> h, const Operand<T, true> w,
+__global__ void __launch_bounds__(CE_THREADS, 2) ce_grad_kernel(const Operand<true> h, const Operand<true> w,
                                                                 const __grid_constant__ GradArgs a) {
   __shared__ __align__(16) Stage sm;
   pdl_enter();
@@ -260,10 +247,10 @@ __global__ void __launch_bounds__(CE_THREADS, 2) ce_grad_kernel(const Operand<T,
   }
 }
 
-// out (32 bits, [splits][rows][cols], grown over the calls unless `first`) or, `last`-typed, T [rows][cols]
-template <typename TA, bool AK, typename TB, bool BK, typename OUT>
-__global__ void __launch_bounds__(CE_THREADS, 2) ce_product_kernel(const Operand<TA, AK> a, const Operand<TB, BK> b, const int64_t K,
-                                                                   OUT* __restrict__ out, const bool grow) {
+// out [splits][rows of a][rows of b]; grow: added to what is there
+template <bool AK>
+__global__ void __launch_bounds__(CE_THREADS, 2) ce_product_kernel(const Operand<AK> a, const Operand<false> b, const int64_t K,
+                                                                   float* __restrict__ out, const bool grow) {
   __shared__ __align__(16) Stage sm;
   pdl_enter();
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
@@ -272,7 +259,7 @@ __global__ void __launch_bounds__(CE_THREADS, 2) ce_product_kernel(const Operand
   const int64_t k0 = kt * blockIdx.z / gridDim.z * CE_K, k1 = kt * (blockIdx.z + 1) / gridDim.z * CE_K;
   float acc[8][8];
   tile_product(a, m0, b, n0, k0, k1 < K ? k1 : K, sm, acc);
-  OUT* to = out + static_cast<int64_t>(blockIdx.z) * a.rows * b.rows;
+  float* to = out + static_cast<int64_t>(blockIdx.z) * a.rows * b.rows;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t r = m0 + tile_at(ty, i);
@@ -280,21 +267,23 @@ __global__ void __launch_bounds__(CE_THREADS, 2) ce_product_kernel(const Operand
     for (int j = 0; j < 8; ++j) {
       const int64_t c = n0 + tile_at(tx, j);
       if (r < a.rows && c < b.rows) {
-        float v = acc[i][j];
-        if (grow) v += to_float<OUT>(to[r * b.rows + c]);
-        to[r * b.rows + c] = from_float<OUT>(v);
+        float* at = to + r * b.rows + c;
+        *at = grow ? *at + acc[i][j] : acc[i][j];
       }
     }
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(CE_THREADS) ce_sum_kernel(const float* __restrict__ parts, const int64_t splits, const int64_t n,
-                                                            T* __restrict__ out) {
+__global__ void __launch_bounds__(CE_THREADS) ce_sum_kernel(const float* __restrict__ parts, const int64_t splits, const int64_t split_elems,
+                                                            const int64_t n, const int D, const int pitch, T* __restrict__ out) {
   pdl_enter();
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(CE_THREADS) + threadIdx.x; i < n; i += gridDim.x * static_cast<int64_t>(CE_THREADS)) {
+  const int64_t count = n * D;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(CE_THREADS) + threadIdx.x; i < count; i += gridDim.x * static_cast<int64_t>(CE_THREADS)) {
+    const int64_t row = i / D;
+    const float* p = parts + row * pitch + (i - row * D);
     float s = 0.0f;
-    for (int64_t p = 0; p < splits; ++p) s += parts[p * n + i];
+    for (int64_t k = 0; k < splits; ++k) s += p[k * split_elems];
     out[i] = from_float<T>(s);
   }
 }
@@ -305,15 +294,14 @@ struct Plan {
   int64_t row_blocks, col_tiles, slices;
   int64_t piece;                       // classes of a piece
   int64_t splits;                      // of a piece's classes in dh's product
-  // offsets in the workspace
   size_t packed, word, target_logit, top, total, g, dh;
   size_t forward_bytes, backward_bytes;
 };
 
-Plan make_plan(int64_t n, int64_t D, int64_t V, int32_t dtype) {
+Plan make_plan(int64_t n, int64_t D, int64_t V) {
   Plan p{};
   const int64_t slots = static_cast<int64_t>(sm_count()) * 2;
-  p.pitch = up(D, 8);
+  p.pitch = D;
   p.row_blocks = tiles(n, CE_ROWS);
   p.col_tiles = tiles(V, CE_COLS);
   p.slices = slices_for(p.row_blocks, p.col_tiles, slots);
@@ -323,101 +311,75 @@ Plan make_plan(int64_t n, int64_t D, int64_t V, int32_t dtype) {
   const int64_t dh_tiles = p.row_blocks * tiles(D, CE_COLS);
   p.splits = dh_tiles < slots ? slots / dh_tiles : 1;
   if (p.splits > tiles(p.piece, 512)) p.splits = tiles(p.piece, 512);
-  size_t at = 0;
-  auto take = [&](int64_t bytes) {
-    const size_t here = at;
-    at += static_cast<size_t>(up(bytes, 256));
-    return here;
-  };
-  p.packed = take(n * p.pitch * dtype_bytes(dtype));
-  p.word = take(n * 4);
-  const size_t common = at;
-  p.target_logit = take(n * 4);
-  p.top = take(p.slices * n * 4);
-  p.total = take(p.slices * n * 4);
-  p.forward_bytes = at;
-  at = common;
-  p.g = take(n * p.piece * 4);
-  p.dh = take(p.splits * n * D * 4);
-  p.backward_bytes = at;
+  Layout l;
+  p.packed = l.take(n * p.pitch * 4);
+  p.word = l.take(n * 4);
+  const Layout common = l;
+  p.target_logit = l.take(n * 4);
+  p.top = l.take(p.slices * n * 4);
+  p.total = l.take(p.slices * n * 4);
+  p.forward_bytes = l.bytes;
+  l = common;
+  p.g = l.take(n * p.piece * 4);
+  p.dh = l.take(p.splits * n * D * 4);
+  p.backward_bytes = l.bytes;
   return p;
 }
 
-struct Problem {
-  const void* hidden;
-  int64_t hidden_stride;
-  const void* weight;
-  int64_t weight_stride;
-  const void* target;
-  bool ids64;
-  int64_t n, D, V, ignore_index;
-  char* ws;
-  int32_t* status;
-};
-
 template <typename T>
-int pack(const Problem& q, const Plan& p, bool logits, cudaStream_t s) {
-  T* packed = reinterpret_cast<T*>(q.ws + p.packed);
-  int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
-  float* tl = logits ? reinterpret_cast<float*>(q.ws + p.target_logit) : nullptr;
+int pack(const CeProblem& q, void* packed, int64_t pitch, int32_t* word, float* target_logit, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(tiles(q.n, CE_THREADS / 32)));
   const T* h = static_cast<const T*>(q.hidden);
+  T* to = static_cast<T*>(packed);
+  const int D = static_cast<int>(q.D), pt = static_cast<int>(pitch);
   if (q.ids64)
     DGS_CUDA_TRY(launch_training(ce_pack_kernel<T, int64_t>, grid, CE_THREADS, 0, s, h, q.hidden_stride, static_cast<const int64_t*>(q.target),
-                                 q.n, static_cast<int>(q.D), static_cast<int>(p.pitch), q.V, q.ignore_index, packed, word, tl, q.status));
+                                 q.n, D, pt, q.V, q.ignore_index, to, word, target_logit, q.status));
   else
     DGS_CUDA_TRY(launch_training(ce_pack_kernel<T, int32_t>, grid, CE_THREADS, 0, s, h, q.hidden_stride, static_cast<const int32_t*>(q.target),
-                                 q.n, static_cast<int>(q.D), static_cast<int>(p.pitch), q.V, q.ignore_index, packed, word, tl, q.status));
+                                 q.n, D, pt, q.V, q.ignore_index, to, word, target_logit, q.status));
   return DGS_OK;
 }
 
-template <typename T>
-int forward(const Problem& q, const Plan& p, float* loss, float* lse, cudaStream_t s) {
-  if (int rc = pack<T>(q, p, true, s)) return rc;
-  const int32_t* word = reinterpret_cast<const int32_t*>(q.ws + p.word);
+int forward32(const CeProblem& q, float* loss, float* lse, cudaStream_t s) {
+  const Plan p = make_plan(q.n, q.D, q.V);
+  const float* packed = reinterpret_cast<const float*>(q.ws + p.packed);
+  int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
   float* tl = reinterpret_cast<float*>(q.ws + p.target_logit);
+  if (int rc = ce_pack(q, q.ws + p.packed, p.pitch, word, tl, s)) return rc;
   float *top = reinterpret_cast<float*>(q.ws + p.top), *total = reinterpret_cast<float*>(q.ws + p.total);
-  const Operand<T, true> h{reinterpret_cast<const T*>(q.ws + p.packed), p.pitch, q.n};
-  const Operand<T, true> w{static_cast<const T*>(q.weight), q.weight_stride, q.V};
   const StatsArgs a{q.n, q.V, static_cast<int>(q.D), p.row_blocks, p.col_tiles, p.slices, word, tl, top, total};
-  DGS_CUDA_TRY(launch_training(ce_stats_kernel<T>, dim3(static_cast<unsigned>(p.row_blocks * p.slices)), CE_THREADS, 0, s, h, w, a));
-  DGS_CUDA_TRY(launch_training(ce_join_kernel, dim3(static_cast<unsigned>(tiles(q.n, CE_THREADS))), CE_THREADS, 0, s, top, total, p.slices,
-                               q.n, word, tl, loss, lse));
-  return DGS_OK;
+  DGS_CUDA_TRY(launch_training(ce_stats_kernel, dim3(static_cast<unsigned>(p.row_blocks * p.slices)), CE_THREADS, 0, s,
+                               Operand<true>{packed, p.pitch, q.n}, Operand<true>{static_cast<const float*>(q.weight), q.weight_stride, q.V}, a));
+  return ce_join(q, top, total, p.slices, word, tl, loss, lse, s);
 }
 
-template <typename T>
-int backward(const Problem& q, const Plan& p, const float* dloss, const float* lse, T* dhidden, T* dweight, cudaStream_t s) {
-  if (int rc = pack<T>(q, p, false, s)) return rc;
-  const int32_t* word = reinterpret_cast<const int32_t*>(q.ws + p.word);
-  const T* packed = reinterpret_cast<const T*>(q.ws + p.packed);
+int backward32(const CeProblem& q, const float* dloss, const float* lse, float* dhidden, float* dweight, cudaStream_t s) {
+  const Plan p = make_plan(q.n, q.D, q.V);
+  int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
+  const float* packed = reinterpret_cast<const float*>(q.ws + p.packed);
+  if (int rc = ce_pack(q, q.ws + p.packed, p.pitch, word, nullptr, s)) return rc;
   float *g = reinterpret_cast<float*>(q.ws + p.g), *dh = reinterpret_cast<float*>(q.ws + p.dh);
+  const unsigned dtiles = static_cast<unsigned>(tiles(q.D, CE_COLS));
   for (int64_t v0 = 0; v0 < q.V; v0 += p.piece) {
     const int64_t width = q.V - v0 < p.piece ? q.V - v0 : p.piece;
-    const T* wp = static_cast<const T*>(q.weight) + v0 * q.weight_stride;
+    const float* wp = static_cast<const float*>(q.weight) + v0 * q.weight_stride;
     const GradArgs a{q.n, q.V, v0, p.piece, p.row_blocks, static_cast<int>(q.D), word, dloss, lse, g};
-    DGS_CUDA_TRY(launch_training(ce_grad_kernel<T>, dim3(static_cast<unsigned>(p.row_blocks * tiles(width, CE_COLS))), CE_THREADS, 0, s,
-                                 Operand<T, true>{packed, p.pitch, q.n}, Operand<T, true>{wp, q.weight_stride, width}, a));
-    const unsigned dtiles = static_cast<unsigned>(tiles(q.D, CE_COLS));
+    DGS_CUDA_TRY(launch_training(ce_grad_kernel, dim3(static_cast<unsigned>(p.row_blocks * tiles(width, CE_COLS))), CE_THREADS, 0, s,
+                                 Operand<true>{packed, p.pitch, q.n}, Operand<true>{wp, q.weight_stride, width}, a));
     if (dhidden != nullptr)
-      DGS_CUDA_TRY(launch_training(ce_product_kernel<float, true, T, false, float>,
-                                   dim3(static_cast<unsigned>(p.row_blocks), dtiles, static_cast<unsigned>(p.splits)), CE_THREADS, 0, s,
-                                   Operand<float, true>{g, p.piece, q.n}, Operand<T, false>{wp, q.weight_stride, q.D}, width, dh, v0 > 0));
+      DGS_CUDA_TRY(launch_training(ce_product_kernel<true>, dim3(static_cast<unsigned>(p.row_blocks), dtiles, static_cast<unsigned>(p.splits)),
+                                   CE_THREADS, 0, s, Operand<true>{g, p.piece, q.n}, Operand<false>{wp, q.weight_stride, q.D}, width, dh, v0 > 0));
     if (dweight != nullptr)
-      DGS_CUDA_TRY(launch_training(ce_product_kernel<float, false, T, false, T>,
-                                   dim3(static_cast<unsigned>(tiles(width, CE_ROWS)), dtiles), CE_THREADS, 0, s,
-                                   Operand<float, false>{g, p.piece, width}, Operand<T, false>{packed, p.pitch, q.D}, q.n,
-                                   dweight + v0 * q.D, false));
+      DGS_CUDA_TRY(launch_training(ce_product_kernel<false>, dim3(static_cast<unsigned>(tiles(width, CE_ROWS)), dtiles), CE_THREADS, 0, s,
+                                   Operand<false>{g, p.piece, width}, Operand<false>{packed, p.pitch, q.D}, q.n, dweight + v0 * q.D, false));
   }
-  if (dhidden != nullptr) {
-    const int64_t count = q.n * q.D, need = tiles(count, CE_THREADS), most = static_cast<int64_t>(sm_count()) * 16;
-    DGS_CUDA_TRY(launch_training(ce_sum_kernel<T>, dim3(static_cast<unsigned>(need < most ? need : most)), CE_THREADS, 0, s, dh, p.splits, count, dhidden));
-  }
+  if (dhidden != nullptr) return ce_sum(dh, p.splits, q.n, q.D, q.n, q.D, dhidden, DGS_F32, s);
   return DGS_OK;
 }
 
-int check(const char* who, const Problem& q, int32_t dtype) {
-  DGS_REQUIRE(dtype_bytes(dtype) != 0, DGS_ERR_UNSUPPORTED, "%s: element type %d", who, dtype);
+int check(const char* who, const CeProblem& q) {
+  DGS_REQUIRE(dtype_bytes(q.dtype) != 0, DGS_ERR_UNSUPPORTED, "%s: element type %d", who, q.dtype);
   DGS_REQUIRE(q.n >= 0 && q.D >= 1 && q.V >= 1, DGS_ERR_INVALID, "%s: %lld rows of %lld elements, %lld classes", who,
               static_cast<long long>(q.n), static_cast<long long>(q.D), static_cast<long long>(q.V));
   DGS_REQUIRE(q.n < (int64_t(1) << 30) && q.V < (int64_t(1) << 30) && q.D <= (int64_t(1) << 20), DGS_ERR_UNSUPPORTED,
@@ -429,36 +391,61 @@ int check(const char* who, const Problem& q, int32_t dtype) {
 }
 
 }  // namespace
+
+int ce_pack(const CeProblem& q, void* packed, int64_t pitch, int32_t* word, float* target_logit, cudaStream_t s) {
+  // (16-bit elements are moved as they are, whichever of the two types they have)
+  return q.dtype == DGS_F32 ? pack<float>(q, packed, pitch, word, target_logit, s) : pack<__half>(q, packed, pitch, word, target_logit, s);
+}
+
+int ce_join(const CeProblem& q, const float* top, const float* total, int64_t parts, const int32_t* word, const float* target_logit,
+            float* loss, float* lse, cudaStream_t s) {
+  DGS_CUDA_TRY(launch_training(ce_join_kernel, dim3(static_cast<unsigned>(tiles(q.n, CE_THREADS))), CE_THREADS, 0, s, top, total, parts, q.n,
+                               word, target_logit, loss, lse));
+  return DGS_OK;
+}
+
+int ce_sum(const float* parts, int64_t splits, int64_t n, int64_t D, int64_t rows, int64_t pitch, void* out, int32_t dtype, cudaStream_t s) {
+  const int64_t need = tiles(n * D, CE_THREADS), most = static_cast<int64_t>(sm_count()) * 16;
+  const dim3 grid(static_cast<unsigned>(need < most ? need : most));
+  const int d = static_cast<int>(D), pt = static_cast<int>(pitch);
+  if (dtype == DGS_F32)
+    DGS_CUDA_TRY(launch_training(ce_sum_kernel<float>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, static_cast<float*>(out)));
+  else if (dtype == DGS_BF16)
+    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__nv_bfloat16>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt,
+                                 static_cast<__nv_bfloat16*>(out)));
+  else
+    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__half>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, static_cast<__half*>(out)));
+  return DGS_OK;
+}
+
 }  // namespace dgs
 
 using namespace dgs;
 
 extern "C" size_t dgs_linear_cross_entropy_workspace_bytes(int64_t n, int64_t D, int64_t V, int32_t dtype) {
   if (n <= 0 || D <= 0 || V <= 0 || dtype_bytes(dtype) == 0) return 0;
-  return make_plan(n, D, V, dtype).forward_bytes;
+  return dtype == DGS_F32 ? make_plan(n, D, V).forward_bytes : ce_mma_forward_bytes(n, D, V);
 }
 
 extern "C" int dgs_linear_cross_entropy(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
                                         int32_t dtype, const void* target, int32_t ids64, int64_t n, int64_t D, int64_t V,
                                         int64_t ignore_index, float* loss, float* lse, void* workspace, size_t workspace_bytes,
                                         int32_t* status, dgs_stream_t stream) {
-  const Problem q{hidden, hidden_stride, weight, weight_stride, target, ids64 != 0, n, D, V, ignore_index, static_cast<char*>(workspace), status};
-  if (int rc = check("linear_cross_entropy", q, dtype)) return rc;
+  const CeProblem q{hidden, hidden_stride, weight, weight_stride, dtype, target, ids64 != 0, n, D, V, ignore_index, static_cast<char*>(workspace), status};
+  if (int rc = check("linear_cross_entropy", q)) return rc;
   if (n == 0) return DGS_OK;
   DGS_REQUIRE(hidden != nullptr && weight != nullptr && target != nullptr && loss != nullptr && lse != nullptr, DGS_ERR_INVALID,
               "linear_cross_entropy: null argument");
-  const Plan p = make_plan(n, D, V, dtype);
-  DGS_REQUIRE(workspace != nullptr && workspace_bytes >= p.forward_bytes && aligned_to(workspace, 256), DGS_ERR_INVALID,
-              "linear_cross_entropy: workspace of %zu bytes, 256-byte aligned, is needed", p.forward_bytes);
+  const size_t need = dgs_linear_cross_entropy_workspace_bytes(n, D, V, dtype);
+  DGS_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned_to(workspace, 256), DGS_ERR_INVALID,
+              "linear_cross_entropy: workspace of %zu bytes, 256-byte aligned, is needed", need);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == DGS_F32    ? forward<float>(q, p, loss, lse, s)
-         : dtype == DGS_BF16 ? forward<__nv_bfloat16>(q, p, loss, lse, s)
-                             : forward<__half>(q, p, loss, lse, s);
+  return dtype == DGS_F32 ? forward32(q, loss, lse, s) : ce_mma_forward(q, loss, lse, s);
 }
 
 extern "C" size_t dgs_linear_cross_entropy_backward_workspace_bytes(int64_t n, int64_t D, int64_t V, int32_t dtype) {
   if (n <= 0 || D <= 0 || V <= 0 || dtype_bytes(dtype) == 0) return 0;
-  return make_plan(n, D, V, dtype).backward_bytes;
+  return dtype == DGS_F32 ? make_plan(n, D, V).backward_bytes : ce_mma_backward_bytes(n, D, V);
 }
 
 extern "C" int dgs_linear_cross_entropy_backward(const float* dloss, const void* hidden, int64_t hidden_stride, const void* weight,
@@ -466,8 +453,8 @@ extern "C" int dgs_linear_cross_entropy_backward(const float* dloss, const void*
                                                  const float* lse, int64_t n, int64_t D, int64_t V, int64_t ignore_index, void* dhidden,
                                                  void* dweight, void* workspace, size_t workspace_bytes, int32_t* status,
                                                  dgs_stream_t stream) {
-  const Problem q{hidden, hidden_stride, weight, weight_stride, target, ids64 != 0, n, D, V, ignore_index, static_cast<char*>(workspace), status};
-  if (int rc = check("linear_cross_entropy_backward", q, dtype)) return rc;
+  const CeProblem q{hidden, hidden_stride, weight, weight_stride, dtype, target, ids64 != 0, n, D, V, ignore_index, static_cast<char*>(workspace), status};
+  if (int rc = check("linear_cross_entropy_backward", q)) return rc;
   if (dhidden == nullptr && dweight == nullptr) return DGS_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (n == 0) {
@@ -476,11 +463,9 @@ extern "C" int dgs_linear_cross_entropy_backward(const float* dloss, const void*
   }
   DGS_REQUIRE(dloss != nullptr && hidden != nullptr && weight != nullptr && target != nullptr && lse != nullptr, DGS_ERR_INVALID,
               "linear_cross_entropy_backward: null argument");
-  const Plan p = make_plan(n, D, V, dtype);
-  DGS_REQUIRE(workspace != nullptr && workspace_bytes >= p.backward_bytes && aligned_to(workspace, 256), DGS_ERR_INVALID,
-              "linear_cross_entropy_backward: workspace of %zu bytes, 256-byte aligned, is needed", p.backward_bytes);
-  return dtype == DGS_F32 ? backward<float>(q, p, dloss, lse, static_cast<float*>(dhidden), static_cast<float*>(dweight), s)
-         : dtype == DGS_BF16
-             ? backward<__nv_bfloat16>(q, p, dloss, lse, static_cast<__nv_bfloat16*>(dhidden), static_cast<__nv_bfloat16*>(dweight), s)
-             : backward<__half>(q, p, dloss, lse, static_cast<__half*>(dhidden), static_cast<__half*>(dweight), s);
+  const size_t need = dgs_linear_cross_entropy_backward_workspace_bytes(n, D, V, dtype);
+  DGS_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned_to(workspace, 256), DGS_ERR_INVALID,
+              "linear_cross_entropy_backward: workspace of %zu bytes, 256-byte aligned, is needed", need);
+  return dtype == DGS_F32 ? backward32(q, dloss, lse, static_cast<float*>(dhidden), static_cast<float*>(dweight), s)
+                          : ce_mma_backward(q, dloss, lse, dhidden, dweight, s);
 }

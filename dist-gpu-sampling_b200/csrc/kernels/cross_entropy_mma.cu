@@ -1,0 +1,737 @@
+// The cross entropy of 16-bit operands on the tensor cores.  The mathematics and the order of the launches are those of
+// cross_entropy.cu; this file holds the products.
+//
+// One kernel in three forms, all of them persistent over pairs of CTAs (cta_group::2):
+//   STATS    logits of a row block against a slice of the vocabulary; running maximum and sum of every row in registers
+//   GRAD     logits of a piece again, left as G in 16 bits
+//   PRODUCT  dh += G W and dW = G^T h of a piece, the tiles of both in one launch
+// A pair's tile is 256 x 256: each CTA of the pair holds 128 rows of it in its TMEM, fetches its 128 rows of A and its half
+// of B, so an operand element crosses from L2 once per pair.  Roles: warp 0 fetches (TMA, five or six stages of 64 along k),
+// warp 1 of the pair's first CTA issues the products, warps 4 to 11 work on finished accumulators.  TMEM holds two
+// accumulators, so the products of the next tile run beside the exponentials of the last one.
+//
+// What bounds it: the products, 2 n V D operations each, at D >= 256; below that the exponentials, 16 a clock and SM.
+// exp(s - m) = 2^(s log2(e) - m log2(e)): one fused multiply-add and one ex2 an element.  The rounding of m log2(e) changes a
+// row's lse by less than the rounding of the lse itself.
+//
+// Every wait is bounded.  One that runs out marks the CTA's words as dead, all roles leave, the status word gets
+// DGS_ERR_CUDA, and the pair frees its TMEM as usual.
+#include "cross_entropy.h"
+#include "tensor_core.cuh"
+
+namespace dgs {
+namespace tc {
+
+int make_map(CUtensorMap* map, const void* base, int32_t dtype, int64_t cols, int64_t rows, int64_t pitch, uint32_t box_cols,
+             uint32_t box_rows) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                              CUtensorMapFloatOOBfill);
+  static std::atomic<void*> known{nullptr};
+  void* fn = known.load(std::memory_order_acquire);
+  if (fn == nullptr) {
+    cudaDriverEntryPointQueryResult found;
+    DGS_CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+    DGS_REQUIRE(found == cudaDriverEntryPointSuccess && fn != nullptr, DGS_ERR_CUDA, "the driver has no tensor maps");
+    known.store(fn, std::memory_order_release);
+  }
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * dtype_bytes(dtype)};
+  const cuuint32_t box[2] = {box_cols, box_rows}, step[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == DGS_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == DGS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult rc = reinterpret_cast<Encode>(fn)(map, type, 2, const_cast<void*>(base), dims, strides, box, step,
+                                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  DGS_REQUIRE(rc == CUDA_SUCCESS, DGS_ERR_CUDA, "tensor map of %lld x %lld elements, %lld apart: error %d", static_cast<long long>(rows),
+              static_cast<long long>(cols), static_cast<long long>(pitch), static_cast<int>(rc));
+  return DGS_OK;
+}
+
+}  // namespace tc
+
+namespace {
+using namespace tc;
+
+constexpr int M_TILE = 256, N_TILE = 256, K_TILE = 64;  // of a pair
+constexpr int M_CTA = M_TILE / 2;
+constexpr int MMA_THREADS = 384, EPILOGUE_WARPS = 8, FIRST_EPILOGUE_WARP = 4;
+constexpr uint32_t A_BYTES = M_CTA * K_TILE * 2, STAGE_BYTES = 2 * A_BYTES;
+constexpr uint32_t BOX_BYTES = 64 * K_TILE * 2;  // 64 of m (or n) by 64 of k, MN-major
+constexpr uint32_t STAGING_BYTES = 4096;         // 32 rows of 128 bytes: one store of a warp
+constexpr uint32_t TMEM_COLS = 512;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int64_t PIECE_BYTES = int64_t(96) << 20;  // of G
+
+enum Mode { STATS, GRAD, PRODUCT };
+template <int MODE>
+constexpr int stages() {
+  return MODE == STATS ? 6 : 5;
+}
+template <int MODE>
+constexpr uint32_t smem_bytes() {  // alignment, stages, two staging buffers a warp, barriers
+  return 1024 + stages<MODE>() * STAGE_BYTES + (MODE == STATS ? 0 : EPILOGUE_WARPS * 2 * STAGING_BYTES) + 256;
+}
+
+enum OutKind { OUT_F32_STORE, OUT_F32_ADD, OUT_TYPED, OUT_TYPED_ODD };
+
+// One of the two products of a PRODUCT launch
+struct Part {
+  int32_t a_mn;     // A is held with m contiguous
+  int32_t items, n_tiles, splits;
+  int32_t k_blocks;
+  int32_t n_total;  // columns of the result
+  int32_t m_total;
+  int32_t out_kind;
+  int64_t split_rows;  // rows between the splits' partial results
+  void* odd;           // OUT_TYPED_ODD: the result itself, rows of n_total elements
+};
+
+struct alignas(64) MmaArgs {
+  CUtensorMap a[2], b[2], out[2];
+  Part part[2];
+  int32_t items, parts;
+  int32_t row_blocks, col_tiles, slices, k_blocks;
+  int64_t n, V;  // GRAD: V is the width of the piece
+  int32_t v0;    // GRAD: first class of the piece
+  const int32_t* word;
+  float* target_logit;
+  float* top;
+  float* total;
+  const float* dloss;
+  const float* lse;
+  const float* scale;  // 16-bit floats: the factor of G and its inverse; null: 1
+  int32_t* status;
+};
+
+struct Tile {
+  int32_t m0, n0;      // of the pair
+  int32_t k0, k1;      // blocks of K_TILE
+  int32_t n;           // columns: N_TILE or half of it
+  int32_t which;       // part
+  int32_t split;
+};
+
+template <int MODE>
+__device__ __forceinline__ Tile tile_of(const MmaArgs& a, int item, int t) {
+  Tile x;
+  x.which = 0;
+  x.split = 0;
+  x.n = N_TILE;
+  if constexpr (MODE == PRODUCT) {
+    x.which = item >= a.part[0].items;
+    const Part& p = a.part[x.which];
+    const int i = item - (x.which ? a.part[0].items : 0);
+    const int nt = i % p.n_tiles, rest = i / p.n_tiles;
+    x.split = rest % p.splits;
+    x.m0 = rest / p.splits * M_TILE;
+    x.n0 = nt * N_TILE;
+    if (p.n_total - x.n0 <= N_TILE / 2) x.n = N_TILE / 2;
+    x.k0 = static_cast<int32_t>(static_cast<int64_t>(p.k_blocks) * x.split / p.splits);
+    x.k1 = static_cast<int32_t>(static_cast<int64_t>(p.k_blocks) * (x.split + 1) / p.splits);
+  } else {
+    x.m0 = item % a.row_blocks * M_TILE;
+    x.n0 = t * N_TILE;
+    x.k0 = 0;
+    x.k1 = a.k_blocks;
+  }
+  return x;
+}
+// the column tiles [t0, t1) of an item
+template <int MODE>
+__device__ __forceinline__ void range_of(const MmaArgs& a, int item, int* t0, int* t1) {
+  if constexpr (MODE == STATS) {
+    const int slice = item / a.row_blocks;
+    *t0 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * slice / a.slices);
+    *t1 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * (slice + 1) / a.slices);
+  } else if constexpr (MODE == GRAD) {
+    *t0 = item / a.row_blocks;
+    *t1 = *t0 + 1;
+  } else {
+    *t0 = 0;
+    *t1 = 1;
+  }
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// A logit (or lse) so large that its product with log2(e) may leave the range of 32-bit floats: the type's lowest value as a
+// mask, infinities
+__device__ __forceinline__ bool far(float x) { return !(fabsf(x) < 1e38f); }
+
+// Running maximum of one row and the sum of e^(s - top)
+struct RowSum {
+  float top = -INFINITY, total = 0.0f;
+  __device__ __forceinline__ void add(const uint32_t (&bits)[32], int valid) {
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(bits[i]);
+    if (valid < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i >= valid) v[i] = -INFINITY;
+    }
+    float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
+#pragma unroll
+    for (int i = 4; i < 32; i += 4) {
+      m0 = fmaxf(m0, fmaxf(v[i], v[i + 1]));
+      m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3]));
+    }
+    m0 = fmaxf(m0, m1);
+    if (m0 > top) {
+      total *= top == -INFINITY ? 0.0f : ex2((top - m0) * LOG2E);  // (a NaN stays one)
+      top = m0;
+    }
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!far(top)) {
+      const float base = top * LOG2E;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) s[i & 3] += ex2(fmaf(v[i], LOG2E, -base));
+    } else {
+      const float base = top == -INFINITY ? 0.0f : top;  // nothing but minus infinity so far
+#pragma unroll
+      for (int i = 0; i < 32; ++i) s[i & 3] += ex2((v[i] - base) * LOG2E);
+    }
+    total += (s[0] + s[1]) + (s[2] + s[3]);
+  }
+};
+
+__device__ __forceinline__ float pick(const uint32_t (&bits)[32], int at) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (i == at) r = bits[i];
+  return __uint_as_float(r);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  } else {
+    const __half2 t = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  }
+}
+__device__ __forceinline__ void st_shared(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+template <int MODE, bool BF16>
+__global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_mma_kernel(const __grid_constant__ MmaArgs a) {
+  constexpr int STAGES = stages<MODE>();
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t staging = smem + STAGES * STAGE_BYTES;
+  const uint32_t words = staging + (MODE == STATS ? 0 : EPILOGUE_WARPS * 2 * STAGING_BYTES);
+  const uint32_t full = words, empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16, tmem_word = acc_empty + 16;
+  volatile int32_t* dead = reinterpret_cast<volatile int32_t*>(smem_raw + (tmem_word + 8 - smem_addr(smem_raw)));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      bar_init(full + 8 * i, 1);
+      bar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(acc_full + 8 * i, 1);
+      bar_init(acc_empty + 8 * i, 2 * EPILOGUE_WARPS);
+    }
+    *dead = 0;
+    bar_init_fence();
+  }
+  if (warp == 2) tmem_alloc(tmem_word, TMEM_COLS);
+  fence_before();
+  __syncthreads();
+  cluster_sync();
+  fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_word) : "memory");
+  pdl_enter();
+
+  bool ok = true;  // this thread's waits have all ended well
+  if (warp == 0 && lane == 0) {
+    // ---- fetch: this CTA's rows of A and its half of B
+    fence_async_global();  // operands that ordinary stores of an earlier launch wrote
+    int st = 0;
+    uint32_t phase = 0;
+    for (int item = pair; ok && item < a.items; item += pairs) {
+      int t0, t1;
+      range_of<MODE>(a, item, &t0, &t1);
+      for (int t = t0; ok && t < t1; ++t) {
+        const Tile x = tile_of<MODE>(a, item, t);
+        const CUtensorMap *ma = &a.a[x.which], *mb = &a.b[x.which];
+        const bool a_mn = MODE == PRODUCT && a.part[x.which].a_mn;
+        const uint32_t bytes = 2 * A_BYTES + x.n * (K_TILE * 2);  // of both CTAs
+        const int32_t m = x.m0 + static_cast<int32_t>(rank) * M_CTA, n = x.n0 + static_cast<int32_t>(rank) * (x.n / 2);
+        for (int kb = x.k0; kb < x.k1; ++kb) {
+          if (!(ok = !*dead && bar_wait(empty + 8 * st, phase ^ 1))) break;
+          const uint32_t to = smem + st * STAGE_BYTES, bar = in_cta(full + 8 * st, 0);
+          if (rank == 0) bar_expect(full + 8 * st, bytes);
+          const int32_t k = kb * K_TILE;
+          if (a_mn) {
+            load_box(to, ma, m, k, bar);
+            load_box(to + BOX_BYTES, ma, m + 64, k, bar);
+          } else {
+            load_box(to, ma, k, m, bar);
+          }
+          if (MODE == PRODUCT) {
+            load_box(to + A_BYTES, mb, n, k, bar);
+            if (x.n == N_TILE) load_box(to + A_BYTES + BOX_BYTES, mb, n + 64, k, bar);
+          } else {
+            load_box(to + A_BYTES, mb, k, n, bar);
+          }
+          if (++st == STAGES) st = 0, phase ^= 1;
+        }
+      }
+    }
+    if (!ok) {
+      // this CTA's copies still in flight land within microseconds; nobody will read them, but they must not outlive the CTA
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---- products
+    int st = 0, buf = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    for (int item = pair; ok && item < a.items; item += pairs) {
+      int t0, t1;
+      range_of<MODE>(a, item, &t0, &t1);
+      for (int t = t0; ok && t < t1; ++t) {
+        const Tile x = tile_of<MODE>(a, item, t);
+        const bool a_mn = MODE == PRODUCT && a.part[x.which].a_mn;
+        constexpr bool b_mn = MODE == PRODUCT;
+        const uint32_t idesc = mma_desc(BF16, a_mn, b_mn, M_TILE, x.n);
+        const uint32_t d = tmem + buf * N_TILE;
+        if (!(ok = !*dead && bar_wait(acc_empty + 8 * buf, acc_phase ^ 1))) break;
+        fence_after();
+        for (int kb = x.k0; kb < x.k1; ++kb) {
+          if (!(ok = !*dead && bar_wait(full + 8 * st, phase))) break;
+          fence_after();
+          const uint32_t sa = smem + st * STAGE_BYTES, sb = sa + A_BYTES;
+          const uint64_t da = smem_desc(sa, a_mn ? BOX_BYTES : 16, 1024), db = smem_desc(sb, b_mn ? BOX_BYTES : 16, 1024);
+          // 16 of k: 32 bytes of every row (K-major) or 16 rows of 128 bytes (MN-major), in units of 16 bytes
+          const uint32_t step_a = a_mn ? 128 : 2, step_b = b_mn ? 128 : 2;
+#pragma unroll
+          for (int k = 0; k < K_TILE / 16; ++k) mma(d, da + k * step_a, db + k * step_b, idesc, kb > x.k0 || k > 0);
+          mma_commit(empty + 8 * st);
+          if (++st == STAGES) st = 0, phase ^= 1;
+        }
+        if (!ok) break;
+        mma_commit(acc_full + 8 * buf);
+        buf ^= 1;
+        if (buf == 0) acc_phase ^= 1;
+      }
+    }
+  } else if (warp >= FIRST_EPILOGUE_WARP) {
+    // ---- finished accumulators: a warp reads the 32 lanes (rows) that its number allows, and half of the columns
+    const int w = warp - FIRST_EPILOGUE_WARP, quarter = warp & 3, half = w >> 2;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    uint32_t stage_at = staging + w * 2 * STAGING_BYTES;  // this warp's two buffers in turn
+    const uint32_t stage_sum = 2 * stage_at + STAGING_BYTES;
+    const uint32_t free_bar0 = in_cta(acc_empty, 0);
+    int buf = 0;
+    uint32_t acc_phase = 0;
+    const float factor = MODE != STATS && a.scale != nullptr ? a.scale[MODE == PRODUCT] : 1.0f;
+    for (int item = pair; ok && item < a.items; item += pairs) {
+      int t0, t1;
+      range_of<MODE>(a, item, &t0, &t1);
+      RowSum sum;
+      for (int t = t0; t < t1; ++t) {
+        const Tile x = tile_of<MODE>(a, item, t);
+        const int32_t row = x.m0 + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
+        const int32_t cols = x.n / 2, c0 = half * cols;
+        int32_t word = -1;
+        float grad = 0.0f, lse = 0.0f;
+        if (MODE != PRODUCT && row < a.n) {
+          word = a.word[row];
+          if (MODE == GRAD && word >= 0) {
+            grad = a.dloss[row] * factor;
+            lse = a.lse[row];
+          }
+        }
+        ok = !*dead && bar_wait(acc_full + 8 * buf, acc_phase);
+        ok = __all_sync(FULL_MASK, ok);
+        if (!ok) break;
+        fence_after();
+        const uint32_t from = tmem + buf * N_TILE + lanes + c0;
+        uint32_t v[2][32];
+        tmem_load32(from, v[0]);
+        const int chunks = cols / 32;  // 4, or 2
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c < chunks) {
+            uint32_t(&now)[32] = v[c & 1];
+            tmem_wait(now);
+            if (c + 1 < chunks) {
+              tmem_load32(from + (c + 1) * 32, v[(c + 1) & 1]);
+            } else {
+              fence_before();
+              __syncwarp();
+              if (lane == 0) bar_arrive_in(free_bar0 + 8 * buf);
+            }
+            const int32_t col = x.n0 + c0 + c * 32;  // first of the 32
+            if constexpr (MODE == STATS) {
+              const int64_t left = a.V - col;
+              const uint32_t at = static_cast<uint32_t>(word - col);
+              if (at < 32u && word >= 0) a.target_logit[row] = pick(now, static_cast<int>(at));
+              if (left > 0) sum.add(now, left < 32 ? static_cast<int>(left) : 32);
+            } else if constexpr (MODE == GRAD) {
+              if (!far(lse)) {
+                const float base = lse * LOG2E;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) now[i] = __float_as_uint(grad * ex2(fmaf(__uint_as_float(now[i]), LOG2E, -base)));
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) now[i] = __float_as_uint(grad * ex2((__uint_as_float(now[i]) - lse) * LOG2E));
+              }
+              const uint32_t at = static_cast<uint32_t>(word - a.v0 - col);
+              if (at < 32u && word >= 0) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (i == static_cast<int>(at)) now[i] = __float_as_uint(__uint_as_float(now[i]) - grad);
+              }
+              if (word < 0) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) now[i] = 0;
+              }
+            }
+            if constexpr (MODE != STATS) {
+              const int kind = MODE == GRAD ? static_cast<int>(OUT_TYPED) : a.part[x.which].out_kind;
+              const bool typed = kind == OUT_TYPED || kind == OUT_TYPED_ODD;
+              if (MODE == PRODUCT) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) now[i] = __float_as_uint(__uint_as_float(now[i]) * factor);
+              }
+              // two chunks of 16-bit values fill a buffer, one of 32-bit values does
+              if (!typed || (c & 1) == 0) {
+                if (lane == 0) store_wait_read<1>();
+                __syncwarp();
+              }
+              const uint32_t at_row = stage_at + lane * 128;
+              if (typed) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  uint32_t p[4];
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    p[i] = pack2<BF16>(__uint_as_float(now[j * 8 + i * 2]), __uint_as_float(now[j * 8 + i * 2 + 1]));
+                  st_shared(at_row + (((c & 1) * 4 + j) ^ (lane & 7)) * 16, p[0], p[1], p[2], p[3]);
+                }
+              } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  st_shared(at_row + (j ^ (lane & 7)) * 16, now[j * 4], now[j * 4 + 1], now[j * 4 + 2], now[j * 4 + 3]);
+              }
+              if (!typed || (c & 1) == 1) {
+                const int32_t first = typed ? col - 32 : col, row0 = row - lane;
+                if (kind == OUT_TYPED_ODD) {
+                  // rows that do not begin at 16-byte boundaries: element by element, a row at a time
+                  __syncwarp();
+                  const Part& p = a.part[x.which];
+                  for (int r = 0; r < 32 && row0 + r < p.m_total; ++r) {
+#pragma unroll
+                    for (int e = lane; e < 64; e += 32) {
+                      uint16_t bits;
+                      asm volatile("ld.shared.b16 %0, [%1];"
+                                   : "=h"(bits)
+                                   : "r"(stage_at + r * 128 + (((e >> 3) ^ (r & 7)) * 16) + (e & 7) * 2)
+                                   : "memory");
+                      if (first + e < p.n_total)
+                        static_cast<uint16_t*>(p.odd)[static_cast<int64_t>(row0 + r) * p.n_total + first + e] = bits;
+                    }
+                  }
+                  __syncwarp();
+                } else {
+                  fence_async_smem();
+                  __syncwarp();
+                  if (lane == 0) {
+                    const CUtensorMap* to = &a.out[x.which];
+                    const int32_t y = MODE == PRODUCT && !typed ? static_cast<int32_t>(x.split * a.part[x.which].split_rows) + row0 : row0;
+                    if (kind == OUT_F32_ADD) add_box(to, first, y, stage_at);
+                    else store_box(to, first, y, stage_at);
+                    store_commit();
+                  }
+                  stage_at = stage_sum - stage_at;
+                }
+              }
+            }
+          }
+        }
+        buf ^= 1;
+        if (buf == 0) acc_phase ^= 1;
+      }
+      if (MODE == STATS && ok) {
+        const int32_t row = item % a.row_blocks * M_TILE + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
+        const int64_t part = item / a.row_blocks * 2 + half;
+        if (row < a.n) {
+          a.top[part * a.n + row] = sum.top;
+          a.total[part * a.n + row] = sum.total;
+        }
+      }
+    }
+    if (MODE != STATS && lane == 0) store_wait_all();
+  }
+  if (!ok) {
+    *dead = 1;
+    raise_status(a.status, DGS_ERR_CUDA);
+  }
+  __syncwarp();
+  __syncthreads();
+  fence_before();
+  cluster_sync();  // the pair's products, copies and arrivals are over
+  fence_after();
+  if (warp == 2) tmem_free(tmem, TMEM_COLS);
+}
+
+// float16: G is scaled by a power of two that brings its largest possible value, max |dloss|, to just below 2^15, so that
+// probabilities down to 2^-29 of it stay normal numbers.  scale = {factor, its inverse}.
+__global__ void __launch_bounds__(1024) ce_scale_kernel(const float* __restrict__ dloss, const int32_t* __restrict__ word,
+                                                        const int64_t n, float* __restrict__ scale) {
+  __shared__ float top[32];
+  pdl_enter();
+  float m = 0.0f;
+  for (int64_t i = threadIdx.x; i < n; i += 1024)
+    if (word[i] >= 0) m = fmaxf(m, fabsf(dloss[i]));
+  m = __uint_as_float(__reduce_max_sync(FULL_MASK, __float_as_uint(m)));
+  if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    m = __uint_as_float(__reduce_max_sync(FULL_MASK, __float_as_uint(top[threadIdx.x])));
+    if (threadIdx.x == 0) {
+      int e = 0;
+      if (m > 0.0f && m < INFINITY) frexpf(m, &e);  // m = f 2^e, f in [1/2, 1)
+      e = e < -100 ? -100 : e > 100 ? 100 : e;
+      scale[0] = ldexpf(1.0f, 15 - e);
+      scale[1] = ldexpf(1.0f, e - 15);
+    }
+  }
+}
+
+// The weight's rows, `pitch` elements apart (rows of an odd length cannot be fetched by TMA where they lie)
+__global__ void __launch_bounds__(256) ce_pack_weight_kernel(const uint16_t* __restrict__ weight, const int64_t stride, const int64_t V,
+                                                             const int D, const int pitch, uint16_t* __restrict__ packed) {
+  pdl_enter();
+  const int64_t count = V * pitch;
+  for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < count; i += gridDim.x * int64_t(256)) {
+    const int64_t row = i / pitch;
+    const int j = static_cast<int>(i - row * pitch);
+    packed[i] = j < D ? weight[row * stride + j] : uint16_t(0);
+  }
+}
+
+// ---- host side -----------------------------------------------------------------------------------------------------
+struct MmaPlan {
+  int64_t pitch, row_blocks, col_tiles, slices, pairs;
+  int64_t piece, splits, dpitch;
+  bool one_piece;
+  size_t packed, word, weight, target_logit, top, total, scale, g, dh;
+  size_t forward_bytes, backward_bytes;
+};
+
+MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
+  MmaPlan p{};
+  p.pairs = sm_count() / 2;
+  p.pitch = up(D, 8);
+  p.row_blocks = tiles(n, M_TILE);
+  p.col_tiles = tiles(V, N_TILE);
+  p.slices = slices_for(p.row_blocks, p.col_tiles, p.pairs);
+  p.piece = PIECE_BYTES / 2 / (n > 0 ? n : 1) / N_TILE * N_TILE;
+  if (p.piece < N_TILE) p.piece = N_TILE;
+  if (p.piece > p.col_tiles * N_TILE) p.piece = p.col_tiles * N_TILE;
+  p.one_piece = p.piece >= V;
+  p.dpitch = up(D, 4);
+  // dh's tiles are cut along the classes until none is longer than half of what each pair has to do
+  const int64_t d_tiles = tiles(D, N_TILE), dh_tiles = p.row_blocks * d_tiles, dh_k = tiles(p.piece, K_TILE);
+  const int64_t dw_k = tiles(n, K_TILE), all = dh_tiles * dh_k + tiles(p.piece, M_TILE) * d_tiles * dw_k;
+  int64_t most = all / p.pairs / 2;
+  if (most < 16) most = 16;
+  p.splits = tiles(dh_k, most);
+  if (p.splits > 32) p.splits = 32;
+  Layout l;
+  p.packed = l.take(n * p.pitch * 2);
+  p.word = l.take(n * 4);
+  if (D % 8 != 0) p.weight = l.take(V * p.pitch * 2);
+  const Layout common = l;
+  p.target_logit = l.take(n * 4);
+  p.top = l.take(2 * p.slices * n * 4);
+  p.total = l.take(2 * p.slices * n * 4);
+  p.forward_bytes = l.bytes;
+  l = common;
+  p.scale = l.take(8);
+  p.g = l.take(n * p.piece * 2);
+  if (!(p.one_piece && p.splits == 1)) p.dh = l.take(p.splits * p.row_blocks * M_TILE * p.dpitch * 4);
+  p.backward_bytes = l.bytes;
+  return p;
+}
+
+template <int MODE, bool BF16>
+int launch(const MmaArgs& a, int64_t pairs, cudaStream_t s) {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<bool> allowed[kMaxDevices] = {};
+  auto kernel = ce_mma_kernel<MODE, BF16>;
+  int dev = 0;
+  DGS_CUDA_TRY(cudaGetDevice(&dev));
+  DGS_REQUIRE(dev >= 0 && dev < kMaxDevices, DGS_ERR_UNSUPPORTED, "cross entropy: device ordinal %d", dev);
+  if (!allowed[dev].load(std::memory_order_acquire)) {
+    DGS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<MODE>())));
+    allowed[dev].store(true, std::memory_order_release);
+  }
+  const int64_t used = a.items < pairs ? a.items : pairs;
+  DGS_CUDA_TRY(launch_training(kernel, dim3(static_cast<unsigned>(2 * used)), MMA_THREADS, smem_bytes<MODE>(), s, a));
+  return DGS_OK;
+}
+template <int MODE>
+int launch(const MmaArgs& a, int64_t pairs, int32_t dtype, cudaStream_t s) {
+  return dtype == DGS_BF16 ? launch<MODE, true>(a, pairs, s) : launch<MODE, false>(a, pairs, s);
+}
+
+// the weight as TMA can fetch it
+struct Weight {
+  const uint16_t* p;
+  int64_t stride;
+};
+int fetchable_weight(const CeProblem& q, const MmaPlan& p, Weight* w, cudaStream_t s) {
+  *w = Weight{static_cast<const uint16_t*>(q.weight), q.V == 1 ? p.pitch : q.weight_stride};
+  if (aligned_to(w->p, 16) && w->stride % 8 == 0) return DGS_OK;
+  DGS_REQUIRE(q.D % 8 != 0, DGS_ERR_INVALID, "linear_cross_entropy: rows of %lld 16-bit elements must begin at 16-byte boundaries",
+              static_cast<long long>(q.D));
+  uint16_t* packed = reinterpret_cast<uint16_t*>(q.ws + p.weight);
+  const int64_t need = tiles(q.V * p.pitch, 256 * 4), most = static_cast<int64_t>(sm_count()) * 8;
+  DGS_CUDA_TRY(launch_training(ce_pack_weight_kernel, dim3(static_cast<unsigned>(need < most ? need : most)), 256, 0, s, w->p,
+                               q.weight_stride, q.V, static_cast<int>(q.D), static_cast<int>(p.pitch), packed));
+  *w = Weight{packed, p.pitch};
+  return DGS_OK;
+}
+
+}  // namespace
+
+size_t ce_mma_forward_bytes(int64_t n, int64_t D, int64_t V) { return make_plan(n, D, V).forward_bytes; }
+size_t ce_mma_backward_bytes(int64_t n, int64_t D, int64_t V) { return make_plan(n, D, V).backward_bytes; }
+
+int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) {
+  const MmaPlan p = make_plan(q.n, q.D, q.V);
+  void* packed = q.ws + p.packed;
+  int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
+  float* tl = reinterpret_cast<float*>(q.ws + p.target_logit);
+  if (int rc = ce_pack(q, packed, p.pitch, word, tl, s)) return rc;
+  Weight w;
+  if (int rc = fetchable_weight(q, p, &w, s)) return rc;
+  MmaArgs a{};
+  if (int rc = make_map(&a.a[0], packed, q.dtype, q.D, q.n, p.pitch, K_TILE, M_CTA)) return rc;
+  if (int rc = make_map(&a.b[0], w.p, q.dtype, q.D, q.V, w.stride, K_TILE, N_TILE / 2)) return rc;
+  a.items = static_cast<int32_t>(p.row_blocks * p.slices);
+  a.row_blocks = static_cast<int32_t>(p.row_blocks);
+  a.col_tiles = static_cast<int32_t>(p.col_tiles);
+  a.slices = static_cast<int32_t>(p.slices);
+  a.k_blocks = static_cast<int32_t>(tiles(q.D, K_TILE));
+  a.n = q.n;
+  a.V = q.V;
+  a.word = word;
+  a.target_logit = tl;
+  a.top = reinterpret_cast<float*>(q.ws + p.top);
+  a.total = reinterpret_cast<float*>(q.ws + p.total);
+  a.status = q.status;
+  if (int rc = launch<STATS>(a, p.pairs, q.dtype, s)) return rc;
+  return ce_join(q, a.top, a.total, 2 * p.slices, word, tl, loss, lse, s);
+}
+
+int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, void* dhidden, void* dweight, cudaStream_t s) {
+  const MmaPlan p = make_plan(q.n, q.D, q.V);
+  void* packed = q.ws + p.packed;
+  int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
+  if (int rc = ce_pack(q, packed, p.pitch, word, nullptr, s)) return rc;
+  float* scale = nullptr;
+  if (q.dtype == DGS_F16) {
+    scale = reinterpret_cast<float*>(q.ws + p.scale);
+    DGS_CUDA_TRY(launch_training(ce_scale_kernel, dim3(1), 1024, 0, s, dloss, word, q.n, scale));
+  }
+  Weight w;
+  if (int rc = fetchable_weight(q, p, &w, s)) return rc;
+  uint16_t* g = reinterpret_cast<uint16_t*>(q.ws + p.g);
+  float* dh = reinterpret_cast<float*>(q.ws + p.dh);
+  // results whose rows begin at 16-byte boundaries leave by TMA
+  const bool dh_direct = p.one_piece && p.splits == 1, even = q.D % 8 == 0;
+  const int32_t d_tiles = static_cast<int32_t>(tiles(q.D, N_TILE));
+  for (int64_t v0 = 0; v0 < q.V; v0 += p.piece) {
+    const int64_t width = q.V - v0 < p.piece ? q.V - v0 : p.piece;
+    const uint16_t* wp = w.p + v0 * w.stride;
+    MmaArgs a{};
+    if (int rc = make_map(&a.a[0], packed, q.dtype, q.D, q.n, p.pitch, K_TILE, M_CTA)) return rc;
+    if (int rc = make_map(&a.b[0], wp, q.dtype, q.D, width, w.stride, K_TILE, N_TILE / 2)) return rc;
+    if (int rc = make_map(&a.out[0], g, q.dtype, width, q.n, p.piece, 64, 32)) return rc;
+    a.row_blocks = static_cast<int32_t>(p.row_blocks);
+    a.col_tiles = static_cast<int32_t>(tiles(width, N_TILE));
+    a.items = a.row_blocks * a.col_tiles;
+    a.k_blocks = static_cast<int32_t>(tiles(q.D, K_TILE));
+    a.n = q.n;
+    a.V = width;
+    a.v0 = static_cast<int32_t>(v0);
+    a.word = word;
+    a.dloss = dloss;
+    a.lse = lse;
+    a.scale = scale;
+    a.status = q.status;
+    if (int rc = launch<GRAD>(a, p.pairs, q.dtype, s)) return rc;
+
+    MmaArgs m{};
+    int parts = 0;
+    if (dhidden != nullptr) {
+      Part& t = m.part[parts];
+      t.a_mn = 0;
+      t.n_tiles = d_tiles;
+      t.k_blocks = static_cast<int32_t>(tiles(width, K_TILE));
+      // (the first piece has work for every split; a narrow last one adds to as many as it has)
+      t.splits = static_cast<int32_t>(p.splits < t.k_blocks ? p.splits : t.k_blocks);
+      t.items = static_cast<int32_t>(p.row_blocks * d_tiles * t.splits);
+      t.n_total = static_cast<int32_t>(q.D);
+      t.m_total = static_cast<int32_t>(q.n);
+      t.split_rows = p.row_blocks * M_TILE;
+      t.out_kind = !dh_direct ? (v0 > 0 ? OUT_F32_ADD : OUT_F32_STORE) : even && aligned_to(dhidden, 16) ? OUT_TYPED : OUT_TYPED_ODD;
+      t.odd = dhidden;
+      if (int rc = make_map(&m.a[parts], g, q.dtype, width, q.n, p.piece, K_TILE, M_CTA)) return rc;
+      if (int rc = make_map(&m.b[parts], wp, q.dtype, q.D, width, w.stride, 64, K_TILE)) return rc;
+      if (t.out_kind == OUT_TYPED) {
+        if (int rc = make_map(&m.out[parts], dhidden, q.dtype, q.D, q.n, q.D, 64, 32)) return rc;
+      } else if (t.out_kind != OUT_TYPED_ODD) {
+        if (int rc = make_map(&m.out[parts], dh, DGS_F32, q.D, p.splits * t.split_rows, p.dpitch, 32, 32)) return rc;
+      }
+      ++parts;
+    }
+    if (dweight != nullptr) {
+      Part& t = m.part[parts];
+      t.a_mn = 1;
+      t.n_tiles = d_tiles;
+      t.splits = 1;
+      t.k_blocks = static_cast<int32_t>(tiles(q.n, K_TILE));
+      t.items = static_cast<int32_t>(tiles(width, M_TILE)) * d_tiles;
+      t.n_total = static_cast<int32_t>(q.D);
+      t.m_total = static_cast<int32_t>(width);
+      uint16_t* to = static_cast<uint16_t*>(dweight) + v0 * q.D;
+      t.out_kind = even && aligned_to(dweight, 16) ? OUT_TYPED : OUT_TYPED_ODD;
+      t.odd = to;
+      if (int rc = make_map(&m.a[parts], g, q.dtype, width, q.n, p.piece, 64, K_TILE)) return rc;
+      if (int rc = make_map(&m.b[parts], packed, q.dtype, q.D, q.n, p.pitch, 64, K_TILE)) return rc;
+      if (t.out_kind == OUT_TYPED) {
+        if (int rc = make_map(&m.out[parts], to, q.dtype, q.D, width, q.D, 64, 32)) return rc;
+      }
+      ++parts;
+    }
+    m.parts = parts;
+    m.items = m.part[0].items + m.part[1].items;
+    m.scale = scale;
+    m.status = q.status;
+    if (int rc = launch<PRODUCT>(m, p.pairs, q.dtype, s)) return rc;
+  }
+  if (dhidden != nullptr && !dh_direct) return ce_sum(dh, p.splits, q.n, q.D, p.row_blocks * M_TILE, p.dpitch, dhidden, q.dtype, s);
+  return DGS_OK;
+}
+
+}  // namespace dgs

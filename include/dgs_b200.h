@@ -415,7 +415,8 @@ DGS_API int dgs_layer_norm_backward(const void* dy, int64_t dy_stride, const voi
  * hidden [n, D] and weight [V, D] have rows hidden_stride / weight_stride elements
  * apart.  targets (int64 when ids64, else int32) equal to ignore_index give loss
  * and lse 0, whatever stands in their rows; any other target outside [0, V) too,
- * and DGS_ERR_RANGE in *status. */
+ * and DGS_ERR_RANGE in *status.  16-bit types with D a multiple of 8: the weight's
+ * rows must begin at 16-byte boundaries.  workspace: 256-byte aligned. */
 DGS_API size_t dgs_linear_cross_entropy_workspace_bytes(int64_t n, int64_t D, int64_t V, int32_t dtype);
 DGS_API int dgs_linear_cross_entropy(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
                                      int32_t dtype, const void* target, int32_t ids64, int64_t n, int64_t D, int64_t V,
