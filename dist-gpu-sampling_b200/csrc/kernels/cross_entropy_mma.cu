@@ -7,7 +7,7 @@
 //   PRODUCT  dh += G W and dW = G^T h of a piece, the tiles of both in one launch
 // A pair's tile is 256 x 256: each CTA of the pair holds 128 rows of it in its TMEM, fetches its 128 rows of A and its half
 // of B, so an operand element crosses from L2 once per pair.  Roles: warp 0 fetches (TMA, five or six stages of 64 along k),
-// warp 1 of the pair's first CTA issues the products, warps 4 to 11 work on finished accumulators.  TMEM holds two
+// warp 1 of the pair's first CTA issues the products, sixteen more work on finished accumulators.  TMEM holds two
 // accumulators, so the products of the next tile run beside the exponentials of the last one.
 //
 // What bounds it: the products, 2 n V D operations each, at D >= 256; below that the exponentials, 16 a clock and SM.
@@ -56,7 +56,8 @@ using namespace tc;
 
 constexpr int M_TILE = 256, N_TILE = 256, K_TILE = 64;  // of a pair
 constexpr int M_CTA = M_TILE / 2;
-constexpr int MMA_THREADS = 384, EPILOGUE_WARPS = 8, FIRST_EPILOGUE_WARP = 4;
+constexpr int MMA_THREADS = 640, EPILOGUE_WARPS = 16, FIRST_EPILOGUE_WARP = 4;
+constexpr int COL_GROUPS = EPILOGUE_WARPS / 4, GROUP_COLS = N_TILE / COL_GROUPS;  // the columns of a tile that a warp works on
 constexpr uint32_t A_BYTES = M_CTA * K_TILE * 2, STAGE_BYTES = 2 * A_BYTES;
 constexpr uint32_t BOX_BYTES = 64 * K_TILE * 2;  // 64 of m (or n) by 64 of k, MN-major
 constexpr uint32_t STAGING_BYTES = 4096;         // 32 rows of 128 bytes: one store of a warp
@@ -70,8 +71,8 @@ constexpr int stages() {
   return MODE == STATS ? 6 : 5;
 }
 template <int MODE>
-constexpr uint32_t smem_bytes() {  // alignment, stages, two staging buffers a warp, barriers
-  return 1024 + stages<MODE>() * STAGE_BYTES + (MODE == STATS ? 0 : EPILOGUE_WARPS * 2 * STAGING_BYTES) + 256;
+constexpr uint32_t smem_bytes() {  // alignment, stages, a staging buffer for each warp, barriers
+  return 1024 + stages<MODE>() * STAGE_BYTES + (MODE == STATS ? 0 : EPILOGUE_WARPS * STAGING_BYTES) + 256;
 }
 
 enum OutKind { OUT_F32_STORE, OUT_F32_ADD, OUT_TYPED, OUT_TYPED_ODD };
@@ -167,38 +168,34 @@ __device__ __forceinline__ bool far(float x) { return !(fabsf(x) < 1e38f); }
 // Running maximum of one row and the sum of e^(s - top)
 struct RowSum {
   float top = -INFINITY, total = 0.0f;
-  __device__ __forceinline__ void add(const uint32_t (&bits)[32], int valid) {
-    float v[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(bits[i]);
+  __device__ __forceinline__ void add(uint32_t (&v)[32], int valid) {
     if (valid < 32) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (i >= valid) v[i] = -INFINITY;
+        if (i >= valid) v[i] = __float_as_uint(-INFINITY);
     }
-    float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
+    float m[4];
 #pragma unroll
-    for (int i = 4; i < 32; i += 4) {
-      m0 = fmaxf(m0, fmaxf(v[i], v[i + 1]));
-      m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3]));
-    }
-    m0 = fmaxf(m0, m1);
-    if (m0 > top) {
-      total *= top == -INFINITY ? 0.0f : ex2((top - m0) * LOG2E);  // (a NaN stays one)
-      top = m0;
-    }
+    for (int i = 0; i < 4; ++i) m[i] = fmaxf(at(v, i), at(v, i + 4));
+#pragma unroll
+    for (int i = 8; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], at(v, i));
+    const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (!far(top)) {
-      const float base = top * LOG2E;
+    if (!far(now)) {
+      const float base = now * LOG2E;
+      total *= ex2((top - now) * LOG2E);  // (0 while top is minus infinity; a NaN stays one)
 #pragma unroll
-      for (int i = 0; i < 32; ++i) s[i & 3] += ex2(fmaf(v[i], LOG2E, -base));
+      for (int i = 0; i < 32; ++i) s[i & 3] += ex2(fmaf(at(v, i), LOG2E, -base));
     } else {
-      const float base = top == -INFINITY ? 0.0f : top;  // nothing but minus infinity so far
+      const float base = now == -INFINITY ? 0.0f : now;  // nothing but minus infinity so far
+      total *= ex2((top - base) * LOG2E);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) s[i & 3] += ex2((v[i] - base) * LOG2E);
+      for (int i = 0; i < 32; ++i) s[i & 3] += ex2((at(v, i) - base) * LOG2E);
     }
+    top = now;
     total += (s[0] + s[1]) + (s[2] + s[3]);
   }
+  static __device__ __forceinline__ float at(const uint32_t (&v)[32], int i) { return __uint_as_float(v[i]); }
 };
 
 __device__ __forceinline__ float pick(const uint32_t (&bits)[32], int at) {
@@ -229,7 +226,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
   extern __shared__ unsigned char smem_raw[];
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = smem + STAGES * STAGE_BYTES;
-  const uint32_t words = staging + (MODE == STATS ? 0 : EPILOGUE_WARPS * 2 * STAGING_BYTES);
+  const uint32_t words = staging + (MODE == STATS ? 0 : EPILOGUE_WARPS * STAGING_BYTES);
   const uint32_t full = words, empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16, tmem_word = acc_empty + 16;
   volatile int32_t* dead = reinterpret_cast<volatile int32_t*>(smem_raw + (tmem_word + 8 - smem_addr(smem_raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -331,12 +328,11 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
       }
     }
   } else if (warp >= FIRST_EPILOGUE_WARP) {
-    // ---- finished accumulators: a warp reads the 32 lanes (rows) that its number allows, and half of the columns
-    const int w = warp - FIRST_EPILOGUE_WARP, quarter = warp & 3, half = w >> 2;
-    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    uint32_t stage_at = staging + w * 2 * STAGING_BYTES;  // this warp's two buffers in turn
-    const uint32_t stage_sum = 2 * stage_at + STAGING_BYTES;
-    const uint32_t free_bar0 = in_cta(acc_empty, 0);
+    // ---- finished accumulators: a warp reads the 32 lanes (rows) that its number allows, and a quarter of the columns
+    const int quarter = warp & 3, group = (warp - FIRST_EPILOGUE_WARP) >> 2, c0 = group * GROUP_COLS;
+    const uint32_t from0 = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
+    const uint32_t stage_at = staging + (warp - FIRST_EPILOGUE_WARP) * STAGING_BYTES;
+    const uint32_t free_bar = in_cta(acc_empty, 0);
     int buf = 0;
     uint32_t acc_phase = 0;
     const float factor = MODE != STATS && a.scale != nullptr ? a.scale[MODE == PRODUCT] : 1.0f;
@@ -347,7 +343,6 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
       for (int t = t0; t < t1; ++t) {
         const Tile x = tile_of<MODE>(a, item, t);
         const int32_t row = x.m0 + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
-        const int32_t cols = x.n / 2, c0 = half * cols;
         int32_t word = -1;
         float grad = 0.0f, lse = 0.0f;
         if (MODE != PRODUCT && row < a.n) {
@@ -361,28 +356,24 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
         ok = __all_sync(FULL_MASK, ok);
         if (!ok) break;
         fence_after();
-        const uint32_t from = tmem + buf * N_TILE + lanes + c0;
-        uint32_t v[2][32];
-        tmem_load32(from, v[0]);
-        const int chunks = cols / 32;  // 4, or 2
+        const int chunks = c0 < x.n ? GROUP_COLS / 32 : 0;  // a narrow tile has nothing for half of the warps
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < GROUP_COLS / 32; ++c) {
           if (c < chunks) {
-            uint32_t(&now)[32] = v[c & 1];
+            uint32_t now[32];
+            tmem_load32(from0 + buf * N_TILE + c * 32, now);
             tmem_wait(now);
-            if (c + 1 < chunks) {
-              tmem_load32(from + (c + 1) * 32, v[(c + 1) & 1]);
-            } else {
+            if (c + 1 == chunks) {
               fence_before();
               __syncwarp();
-              if (lane == 0) bar_arrive_in(free_bar0 + 8 * buf);
+              if (lane == 0) bar_arrive_in(free_bar + 8 * buf);
             }
             const int32_t col = x.n0 + c0 + c * 32;  // first of the 32
             if constexpr (MODE == STATS) {
-              const int64_t left = a.V - col;
+              const int32_t left = static_cast<int32_t>(a.V) - col;
               const uint32_t at = static_cast<uint32_t>(word - col);
               if (at < 32u && word >= 0) a.target_logit[row] = pick(now, static_cast<int>(at));
-              if (left > 0) sum.add(now, left < 32 ? static_cast<int>(left) : 32);
+              if (left > 0) sum.add(now, left);
             } else if constexpr (MODE == GRAD) {
               if (!far(lse)) {
                 const float base = lse * LOG2E;
@@ -410,9 +401,9 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
 #pragma unroll
                 for (int i = 0; i < 32; ++i) now[i] = __float_as_uint(__uint_as_float(now[i]) * factor);
               }
-              // two chunks of 16-bit values fill a buffer, one of 32-bit values does
+              // two chunks of 16-bit values fill the buffer, one of 32-bit values does
               if (!typed || (c & 1) == 0) {
-                if (lane == 0) store_wait_read<1>();
+                if (lane == 0) store_wait_read<0>();
                 __syncwarp();
               }
               const uint32_t at_row = stage_at + lane * 128;
@@ -459,18 +450,18 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
                     else store_box(to, first, y, stage_at);
                     store_commit();
                   }
-                  stage_at = stage_sum - stage_at;
                 }
               }
             }
           }
         }
+        if (chunks == 0 && lane == 0) bar_arrive_in(free_bar + 8 * buf);
         buf ^= 1;
         if (buf == 0) acc_phase ^= 1;
       }
       if (MODE == STATS && ok) {
         const int32_t row = item % a.row_blocks * M_TILE + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
-        const int64_t part = item / a.row_blocks * 2 + half;
+        const int64_t part = item / a.row_blocks * COL_GROUPS + group;
         if (row < a.n) {
           a.top[part * a.n + row] = sum.top;
           a.total[part * a.n + row] = sum.total;
@@ -561,8 +552,8 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   if (D % 8 != 0) p.weight = l.take(V * p.pitch * 2);
   const Layout common = l;
   p.target_logit = l.take(n * 4);
-  p.top = l.take(2 * p.slices * n * 4);
-  p.total = l.take(2 * p.slices * n * 4);
+  p.top = l.take(COL_GROUPS * p.slices * n * 4);
+  p.total = l.take(COL_GROUPS * p.slices * n * 4);
   p.forward_bytes = l.bytes;
   l = common;
   p.scale = l.take(8);
@@ -640,7 +631,7 @@ int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) 
   a.total = reinterpret_cast<float*>(q.ws + p.total);
   a.status = q.status;
   if (int rc = launch<STATS>(a, p.pairs, q.dtype, s)) return rc;
-  return ce_join(q, a.top, a.total, 2 * p.slices, word, tl, loss, lse, s);
+  return ce_join(q, a.top, a.total, COL_GROUPS * p.slices, word, tl, loss, lse, s);
 }
 
 int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, void* dhidden, void* dweight, cudaStream_t s) {
