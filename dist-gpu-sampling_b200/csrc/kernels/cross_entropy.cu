@@ -29,27 +29,133 @@ constexpr int CE_THREADS = 256;
 constexpr int64_t CE_PIECE_BYTES = int64_t(96) << 20;  // of G: what L2 (126 MB) holds beside the operands
 
 // ---- packing -----------------------------------------------------------------------------------------------------
-template <typename T, typename IdT>
-__global__ void __launch_bounds__(CE_THREADS) ce_pack_kernel(const T* __restrict__ hidden, const int64_t stride,
-                                                             const IdT* __restrict__ target, const int64_t n, const int D,
-                                                             const int pitch, const int64_t V, const int64_t ignore_index,
-                                                             T* __restrict__ packed, int32_t* __restrict__ word,
-                                                             float* __restrict__ target_logit, int32_t* status) {
+struct PackArgs {
+  const void* hidden;
+  int64_t stride;
+  const void* target;
+  int32_t ids64, vectors;  // vectors: rows are moved 16 bytes at a time
+  int64_t n, V, ignore_index;
+  int32_t D, pitch;
+  CePacked to;
+  const float *dloss, *lse;
+  int32_t* status;
+};
+
+// Rows with a valid target in each CE_COUNT_ROWS
+__global__ void __launch_bounds__(CE_THREADS) ce_count_kernel(const __grid_constant__ PackArgs a) {
   pdl_enter();
-  const int64_t row = blockIdx.x * static_cast<int64_t>(CE_THREADS / 32) + (threadIdx.x >> 5);
-  if (row >= n) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t t = static_cast<int64_t>(target[row]);
-  const bool ignored = t == ignore_index;
-  const bool live = !ignored && t >= 0 && t < V;
-  if (lane == 0) {
-    word[row] = live ? static_cast<int32_t>(t) : -1;
-    if (target_logit != nullptr) target_logit[row] = 0.0f;
-    if (!ignored && !live) raise_status(status, DGS_ERR_RANGE);
+  int mine = 0;
+#pragma unroll
+  for (int k = 0; k < CE_COUNT_ROWS / CE_THREADS; ++k) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * CE_COUNT_ROWS + k * CE_THREADS + threadIdx.x;
+    bool wrong;
+    if (row < a.n) mine += target_word(a.target, a.ids64, row, a.V, a.ignore_index, &wrong) >= 0;
   }
-  const T* from = hidden + row * stride;
-  T* to = packed + row * pitch;
-  for (int j = lane; j < pitch; j += 32) to[j] = live && j < D ? from[j] : from_float<T>(0.0f);
+  __shared__ int sums[CE_THREADS / 32];
+  mine = __reduce_add_sync(FULL_MASK, mine);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int s = 0;
+    for (int w = 0; w < CE_THREADS / 32; ++w) s += sums[w];
+    a.to.counts[blockIdx.x] = s;
+  }
+}
+
+__device__ __forceinline__ int cta_sum_int(int v, int* smem) {
+  v = __reduce_add_sync(FULL_MASK, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int s = 0;
+#pragma unroll
+  for (int w = 0; w < CE_THREADS / 32; ++w) s += smem[w];
+  return s;
+}
+
+// A warp moves two rows.  Compact: a CTA's rows go behind all valid rows before them, counted from the chunks' numbers and the
+// targets of its own chunk.
+template <typename T>
+__global__ void __launch_bounds__(CE_THREADS) ce_pack_kernel(const __grid_constant__ PackArgs a) {
+  constexpr int VEC = 16 / sizeof(T), WARPS = CE_THREADS / 32;
+  __shared__ int sums[WARPS];
+  __shared__ int32_t words[CE_PACK_ROWS];
+  __shared__ float peak[WARPS];
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * CE_PACK_ROWS;
+  if (threadIdx.x < CE_PACK_ROWS && row0 + threadIdx.x < a.n) {
+    bool wrong;
+    words[threadIdx.x] = target_word(a.target, a.ids64, row0 + threadIdx.x, a.V, a.ignore_index, &wrong);
+    if (wrong) raise_status(a.status, DGS_ERR_RANGE);
+  }
+  int before = 0, live = 0;
+  if (a.to.compact) {
+    const int64_t chunk = row0 / CE_COUNT_ROWS, chunks = (a.n + CE_COUNT_ROWS - 1) / CE_COUNT_ROWS;
+    for (int64_t c = threadIdx.x; c < chunks; c += CE_THREADS) {
+      const int k = a.to.counts[c];
+      live += k;
+      if (c < chunk) before += k;
+    }
+    for (int64_t r = chunk * CE_COUNT_ROWS + threadIdx.x; r < row0; r += CE_THREADS) {
+      bool wrong;
+      before += target_word(a.target, a.ids64, r, a.V, a.ignore_index, &wrong) >= 0;
+    }
+    before = cta_sum_int(before, sums);
+    live = cta_sum_int(live, sums);
+  }
+  __syncthreads();
+  float most = 0.0f;
+#pragma unroll
+  for (int k = 0; k < CE_PACK_ROWS / WARPS; ++k) {
+    const int i = warp * (CE_PACK_ROWS / WARPS) + k;
+    const int64_t row = row0 + i;
+    if (row >= a.n) break;
+    const int32_t word = words[i];
+    int64_t to = row;
+    if (a.to.compact) {
+      int ahead = 0;
+      for (int j = 0; j < i; ++j) ahead += words[j] >= 0;
+      to = word >= 0 ? before + ahead : -1;
+      if (lane == 0) a.to.slot[row] = static_cast<int32_t>(to);
+      if (to < 0) continue;
+    }
+    if (lane == 0) {
+      a.to.word[to] = word;
+      if (a.to.dloss != nullptr) {
+        const float d = word >= 0 ? a.dloss[row] : 0.0f;
+        a.to.dloss[to] = d;
+        a.to.lse[to] = word >= 0 ? a.lse[row] : 0.0f;
+        most = fmaxf(most, fabsf(d));
+      }
+    }
+    const T* from = static_cast<const T*>(a.hidden) + row * a.stride;
+    T* dst = static_cast<T*>(a.to.rows) + to * a.pitch;
+    if (a.vectors) {
+      for (int j = lane * VEC; j < a.pitch; j += 32 * VEC)
+        *reinterpret_cast<uint4*>(dst + j) = word >= 0 ? *reinterpret_cast<const uint4*>(from + j) : uint4{0, 0, 0, 0};
+    } else {
+      for (int j = lane; j < a.pitch; j += 32) dst[j] = word >= 0 && j < a.D ? from[j] : from_float<T>(0.0f);
+    }
+  }
+  if (a.to.largest != nullptr) {
+    if (lane == 0) peak[warp] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < WARPS; ++w) most = fmaxf(most, peak[w]);
+      a.to.largest[blockIdx.x] = most;
+    }
+  }
+  if (a.to.compact && blockIdx.x == gridDim.x - 1) {
+    if (threadIdx.x == 0) *a.to.live = live;
+    int64_t end = (static_cast<int64_t>(live) + 63) / 64 * 64;
+    if (end == 0) end = 64;
+    if (end > a.n) end = a.n;
+    for (int64_t r = live + warp; r < end; r += WARPS) {
+      T* dst = static_cast<T*>(a.to.rows) + r * a.pitch;
+      for (int j = lane; j < a.pitch; j += 32) dst[j] = from_float<T>(0.0f);
+    }
+  }
 }
 
 // ---- products on the CUDA cores ------------------------------------------------------------------------------------
@@ -133,8 +239,8 @@ struct StatsArgs {
   int64_t row_blocks, col_tiles, slices;
   const int32_t* word;
   float* target_logit;
-  float* top;    // [slices][n]
-  float* total;  // [slices][n]
+  float* top;    // [n][slices]
+  float* total;  // [n][slices]
 };
 
 
@@ -188,28 +294,60 @@ __global__ void __launch_bounds__(CE_THREADS, 2) ce_stats_kernel(const Operand<t
     for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(FULL_MASK, s, o);
     const int64_t row = m0 + tile_at(ty, i);
     if (tx == 0 && row < a.n) {
-      a.top[slice * a.n + row] = top[i];
-      a.total[slice * a.n + row] = s;
+      a.top[row * a.slices + slice] = top[i];
+      a.total[row * a.slices + slice] = s;
     }
   }
 }
 
-__global__ void __launch_bounds__(CE_THREADS) ce_join_kernel(const float* __restrict__ top, const float* __restrict__ total,
-                                                             const int64_t parts, const int64_t n, const int32_t* __restrict__ word,
-                                                             const float* __restrict__ target_logit, float* __restrict__ loss,
-                                                             float* __restrict__ lse) {
+struct JoinArgs {
+  const float *top, *total;
+  int64_t parts, n, V, ignore_index;
+  const void* target;
+  int32_t ids64;
+  const int32_t *word, *slot;
+  const float* target_logit;
+  float *loss, *lse;
+  int32_t* status;
+};
+
+// A warp joins one row's parts, in an order that depends on their number alone
+__global__ void __launch_bounds__(CE_THREADS) ce_join_kernel(const __grid_constant__ JoinArgs a) {
   pdl_enter();
-  const int64_t row = blockIdx.x * static_cast<int64_t>(CE_THREADS) + threadIdx.x;
-  if (row >= n) return;
+  const int64_t row = blockIdx.x * static_cast<int64_t>(CE_THREADS / 32) + (threadIdx.x >> 5);
+  if (row >= a.n) return;
+  const int lane = threadIdx.x & 31;
+  int64_t c = row;  // its packed row
+  bool live;
+  if (a.slot != nullptr) {
+    c = a.slot[row];
+    live = c >= 0;
+  } else if (a.word != nullptr) {
+    live = a.word[row] >= 0;
+  } else {
+    bool wrong;
+    live = target_word(a.target, a.ids64, row, a.V, a.ignore_index, &wrong) >= 0;
+    if (wrong && lane == 0) raise_status(a.status, DGS_ERR_RANGE);
+  }
+  if (!live) {
+    if (lane == 0) a.loss[row] = a.lse[row] = 0.0f;
+    return;
+  }
+  const float *top = a.top + c * a.parts, *total = a.total + c * a.parts;
   float m = -INFINITY;
-  for (int64_t p = 0; p < parts; ++p) m = fmaxf(m, top[p * n + row]);
+  for (int64_t p = lane; p < a.parts; p += 32) m = fmaxf(m, top[p]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
   const float base = m == -INFINITY ? 0.0f : m;
   float s = 0.0f;
-  for (int64_t p = 0; p < parts; ++p) s += total[p * n + row] * expf(top[p * n + row] - base);
-  const float l = logf(s);
-  const bool live = word[row] >= 0;
-  lse[row] = live ? base + l : 0.0f;
-  loss[row] = live ? (base - target_logit[row]) + l : 0.0f;  // logits of one size meet first: exact, or nearly
+  for (int64_t p = lane; p < a.parts; p += 32) s += total[p] * expf(top[p] - base);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL_MASK, s, o);
+  if (lane == 0) {
+    const float l = logf(s);
+    a.lse[row] = base + l;
+    a.loss[row] = (base - a.target_logit[c]) + l;  // logits of one size meet first: exact, or nearly
+  }
 }
 
 struct GradArgs {
@@ -276,15 +414,36 @@ __global__ void __launch_bounds__(CE_THREADS, 2) ce_product_kernel(const Operand
 
 template <typename T>
 __global__ void __launch_bounds__(CE_THREADS) ce_sum_kernel(const float* __restrict__ parts, const int64_t splits, const int64_t split_elems,
-                                                            const int64_t n, const int D, const int pitch, T* __restrict__ out) {
+                                                            const int64_t n, const int D, const int pitch,
+                                                            const int32_t* __restrict__ slot, const bool fours, T* __restrict__ out) {
   pdl_enter();
-  const int64_t count = n * D;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(CE_THREADS) + threadIdx.x; i < count; i += gridDim.x * static_cast<int64_t>(CE_THREADS)) {
-    const int64_t row = i / D;
-    const float* p = parts + row * pitch + (i - row * D);
-    float s = 0.0f;
-    for (int64_t k = 0; k < splits; ++k) s += p[k * split_elems];
-    out[i] = from_float<T>(s);
+  const int lane = threadIdx.x & 31;
+  for (int64_t row = blockIdx.x * static_cast<int64_t>(CE_THREADS / 32) + (threadIdx.x >> 5); row < n;
+       row += gridDim.x * static_cast<int64_t>(CE_THREADS / 32)) {
+    const int64_t c = slot != nullptr ? slot[row] : row;
+    const float* p = parts + c * pitch;
+    T* to = out + row * D;
+    if (fours) {
+      for (int j = lane * 4; j < D; j += 128) {
+        float v[4] = {};
+        if (c >= 0) {
+          for (int64_t k = 0; k < splits; ++k) {
+            float t[4];
+            load_vec<float, 4>(p + k * split_elems + j, t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += t[i];
+          }
+        }
+        store_vec<T, 4>(to + j, v);
+      }
+    } else {
+      for (int j = lane; j < D; j += 32) {
+        float v = 0.0f;
+        if (c >= 0)
+          for (int64_t k = 0; k < splits; ++k) v += p[k * split_elems + j];
+        to[j] = from_float<T>(v);
+      }
+    }
   }
 }
 
@@ -294,7 +453,7 @@ struct Plan {
   int64_t row_blocks, col_tiles, slices;
   int64_t piece;                       // classes of a piece
   int64_t splits;                      // of a piece's classes in dh's product
-  size_t packed, word, target_logit, top, total, g, dh;
+  size_t packed, word, target_logit, top, total, dloss, lse, g, dh;
   size_t forward_bytes, backward_bytes;
 };
 
@@ -320,25 +479,12 @@ Plan make_plan(int64_t n, int64_t D, int64_t V) {
   p.total = l.take(p.slices * n * 4);
   p.forward_bytes = l.bytes;
   l = common;
+  p.dloss = l.take(n * 4);
+  p.lse = l.take(n * 4);
   p.g = l.take(n * p.piece * 4);
   p.dh = l.take(p.splits * n * D * 4);
   p.backward_bytes = l.bytes;
   return p;
-}
-
-template <typename T>
-int pack(const CeProblem& q, void* packed, int64_t pitch, int32_t* word, float* target_logit, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(tiles(q.n, CE_THREADS / 32)));
-  const T* h = static_cast<const T*>(q.hidden);
-  T* to = static_cast<T*>(packed);
-  const int D = static_cast<int>(q.D), pt = static_cast<int>(pitch);
-  if (q.ids64)
-    DGS_CUDA_TRY(launch_training(ce_pack_kernel<T, int64_t>, grid, CE_THREADS, 0, s, h, q.hidden_stride, static_cast<const int64_t*>(q.target),
-                                 q.n, D, pt, q.V, q.ignore_index, to, word, target_logit, q.status));
-  else
-    DGS_CUDA_TRY(launch_training(ce_pack_kernel<T, int32_t>, grid, CE_THREADS, 0, s, h, q.hidden_stride, static_cast<const int32_t*>(q.target),
-                                 q.n, D, pt, q.V, q.ignore_index, to, word, target_logit, q.status));
-  return DGS_OK;
 }
 
 int forward32(const CeProblem& q, float* loss, float* lse, cudaStream_t s) {
@@ -346,25 +492,35 @@ int forward32(const CeProblem& q, float* loss, float* lse, cudaStream_t s) {
   const float* packed = reinterpret_cast<const float*>(q.ws + p.packed);
   int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
   float* tl = reinterpret_cast<float*>(q.ws + p.target_logit);
-  if (int rc = ce_pack(q, q.ws + p.packed, p.pitch, word, tl, s)) return rc;
+  CePacked to{};
+  to.rows = q.ws + p.packed;
+  to.pitch = p.pitch;
+  to.word = word;
+  if (int rc = ce_pack(q, to, nullptr, nullptr, s)) return rc;
   float *top = reinterpret_cast<float*>(q.ws + p.top), *total = reinterpret_cast<float*>(q.ws + p.total);
   const StatsArgs a{q.n, q.V, static_cast<int>(q.D), p.row_blocks, p.col_tiles, p.slices, word, tl, top, total};
   DGS_CUDA_TRY(launch_training(ce_stats_kernel, dim3(static_cast<unsigned>(p.row_blocks * p.slices)), CE_THREADS, 0, s,
                                Operand<true>{packed, p.pitch, q.n}, Operand<true>{static_cast<const float*>(q.weight), q.weight_stride, q.V}, a));
-  return ce_join(q, top, total, p.slices, word, tl, loss, lse, s);
+  return ce_join(q, top, total, p.slices, word, nullptr, tl, loss, lse, s);
 }
 
 int backward32(const CeProblem& q, const float* dloss, const float* lse, float* dhidden, float* dweight, cudaStream_t s) {
   const Plan p = make_plan(q.n, q.D, q.V);
   int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
   const float* packed = reinterpret_cast<const float*>(q.ws + p.packed);
-  if (int rc = ce_pack(q, q.ws + p.packed, p.pitch, word, nullptr, s)) return rc;
+  CePacked to{};
+  to.rows = q.ws + p.packed;
+  to.pitch = p.pitch;
+  to.word = word;
+  to.dloss = reinterpret_cast<float*>(q.ws + p.dloss);
+  to.lse = reinterpret_cast<float*>(q.ws + p.lse);
+  if (int rc = ce_pack(q, to, dloss, lse, s)) return rc;
   float *g = reinterpret_cast<float*>(q.ws + p.g), *dh = reinterpret_cast<float*>(q.ws + p.dh);
   const unsigned dtiles = static_cast<unsigned>(tiles(q.D, CE_COLS));
   for (int64_t v0 = 0; v0 < q.V; v0 += p.piece) {
     const int64_t width = q.V - v0 < p.piece ? q.V - v0 : p.piece;
     const float* wp = static_cast<const float*>(q.weight) + v0 * q.weight_stride;
-    const GradArgs a{q.n, q.V, v0, p.piece, p.row_blocks, static_cast<int>(q.D), word, dloss, lse, g};
+    const GradArgs a{q.n, q.V, v0, p.piece, p.row_blocks, static_cast<int>(q.D), word, to.dloss, to.lse, g};
     DGS_CUDA_TRY(launch_training(ce_grad_kernel, dim3(static_cast<unsigned>(p.row_blocks * tiles(width, CE_COLS))), CE_THREADS, 0, s,
                                  Operand<true>{packed, p.pitch, q.n}, Operand<true>{wp, q.weight_stride, width}, a));
     if (dhidden != nullptr)
@@ -374,7 +530,7 @@ int backward32(const CeProblem& q, const float* dloss, const float* lse, float* 
       DGS_CUDA_TRY(launch_training(ce_product_kernel<false>, dim3(static_cast<unsigned>(tiles(width, CE_ROWS)), dtiles), CE_THREADS, 0, s,
                                    Operand<false>{g, p.piece, width}, Operand<false>{packed, p.pitch, q.D}, q.n, dweight + v0 * q.D, false));
   }
-  if (dhidden != nullptr) return ce_sum(dh, p.splits, q.n, q.D, q.n, q.D, dhidden, DGS_F32, s);
+  if (dhidden != nullptr) return ce_sum(dh, p.splits, q.n, q.D, q.n, q.D, nullptr, dhidden, DGS_F32, s);
   return DGS_OK;
 }
 
@@ -392,29 +548,42 @@ int check(const char* who, const CeProblem& q) {
 
 }  // namespace
 
-int ce_pack(const CeProblem& q, void* packed, int64_t pitch, int32_t* word, float* target_logit, cudaStream_t s) {
+int ce_pack(const CeProblem& q, const CePacked& p, const float* dloss, const float* lse, cudaStream_t s) {
+  const int64_t per16 = 16 / dtype_bytes(q.dtype);
+  const bool vectors = q.D == p.pitch && p.pitch % per16 == 0 && q.hidden_stride % per16 == 0 && aligned_to(q.hidden, 16);
+  const PackArgs a{q.hidden, q.hidden_stride, q.target, q.ids64,  vectors, q.n, q.V, q.ignore_index, static_cast<int32_t>(q.D),
+                   static_cast<int32_t>(p.pitch), p, dloss, lse, q.status};
+  if (p.compact)
+    DGS_CUDA_TRY(launch_training(ce_count_kernel, dim3(static_cast<unsigned>(tiles(q.n, CE_COUNT_ROWS))), CE_THREADS, 0, s, a));
+  const dim3 grid(static_cast<unsigned>(ce_pack_ctas(q.n)));
   // (16-bit elements are moved as they are, whichever of the two types they have)
-  return q.dtype == DGS_F32 ? pack<float>(q, packed, pitch, word, target_logit, s) : pack<__half>(q, packed, pitch, word, target_logit, s);
-}
-
-int ce_join(const CeProblem& q, const float* top, const float* total, int64_t parts, const int32_t* word, const float* target_logit,
-            float* loss, float* lse, cudaStream_t s) {
-  DGS_CUDA_TRY(launch_training(ce_join_kernel, dim3(static_cast<unsigned>(tiles(q.n, CE_THREADS))), CE_THREADS, 0, s, top, total, parts, q.n,
-                               word, target_logit, loss, lse));
+  if (q.dtype == DGS_F32) DGS_CUDA_TRY(launch_training(ce_pack_kernel<float>, grid, CE_THREADS, 0, s, a));
+  else DGS_CUDA_TRY(launch_training(ce_pack_kernel<__half>, grid, CE_THREADS, 0, s, a));
   return DGS_OK;
 }
 
-int ce_sum(const float* parts, int64_t splits, int64_t n, int64_t D, int64_t rows, int64_t pitch, void* out, int32_t dtype, cudaStream_t s) {
-  const int64_t need = tiles(n * D, CE_THREADS), most = static_cast<int64_t>(sm_count()) * 16;
+int ce_join(const CeProblem& q, const float* top, const float* total, int64_t parts, const int32_t* word, const int32_t* slot,
+            const float* target_logit, float* loss, float* lse, cudaStream_t s) {
+  const JoinArgs a{top, total, parts, q.n, q.V, q.ignore_index, q.target, q.ids64, word, slot, target_logit, loss, lse, q.status};
+  DGS_CUDA_TRY(launch_training(ce_join_kernel, dim3(static_cast<unsigned>(tiles(q.n, CE_THREADS / 32))), CE_THREADS, 0, s, a));
+  return DGS_OK;
+}
+
+int ce_sum(const float* parts, int64_t splits, int64_t n, int64_t D, int64_t rows, int64_t pitch, const int32_t* slot, void* out,
+           int32_t dtype, cudaStream_t s) {
+  const int64_t need = tiles(n, CE_THREADS / 32), most = static_cast<int64_t>(sm_count()) * 16;
   const dim3 grid(static_cast<unsigned>(need < most ? need : most));
   const int d = static_cast<int>(D), pt = static_cast<int>(pitch);
+  const bool fours = D % 4 == 0 && pitch % 4 == 0 && aligned_to(out, 16);
   if (dtype == DGS_F32)
-    DGS_CUDA_TRY(launch_training(ce_sum_kernel<float>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, static_cast<float*>(out)));
+    DGS_CUDA_TRY(launch_training(ce_sum_kernel<float>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, slot, fours,
+                                 static_cast<float*>(out)));
   else if (dtype == DGS_BF16)
-    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__nv_bfloat16>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt,
+    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__nv_bfloat16>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, slot, fours,
                                  static_cast<__nv_bfloat16*>(out)));
   else
-    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__half>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, static_cast<__half*>(out)));
+    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__half>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, slot, fours,
+                                 static_cast<__half*>(out)));
   return DGS_OK;
 }
 

@@ -45,19 +45,47 @@ inline int64_t slices_for(int64_t rows, int64_t cols, int64_t slots) {
   return best;
 }
 
-// cross_entropy.cu: rows with a valid target, packed `pitch` elements apart (zero where there is none), the targets as 32-bit
-// words (-1: none); target_logit (may be null) is cleared.
-int ce_pack(const CeProblem& q, void* packed, int64_t pitch, int32_t* word, float* target_logit, cudaStream_t s);
-// loss and lse from `parts` (maximum, sum) pairs a row: top, total [parts][n]
-int ce_join(const CeProblem& q, const float* top, const float* total, int64_t parts, const int32_t* word, const float* target_logit,
-            float* loss, float* lse, cudaStream_t s);
-// out[n][D] of `dtype` = the sum of parts[splits][rows][pitch], rows >= n
-int ce_sum(const float* parts, int64_t splits, int64_t n, int64_t D, int64_t rows, int64_t pitch, void* out, int32_t dtype, cudaStream_t s);
+// The rows that count, as cross_entropy.cu packs them.  Packed row c holds what the products read: the hidden row, its target
+// as a 32-bit word (-1: none), and for the backward pass dloss and lse.  Either row c is row c of the call (rows without a valid
+// target: zeros, word -1), or (compact) the rows with a valid target alone, in their order; then slot[i] is row i's place among
+// them (-1: none), *live their number, and the packed rows from there to the next multiple of 64 (one at least) are zeros.
+struct CePacked {
+  void* rows;
+  int64_t pitch;
+  int32_t* word;
+  float *dloss, *lse;      // null in the forward pass
+  float* largest;          // [ce_pack_ctas(n)] largest |dloss| among a CTA's rows; may be null
+  bool compact;
+  int32_t *slot, *live;
+  int32_t* counts;         // [tiles(n, CE_COUNT_ROWS)], scratch
+};
+constexpr int CE_PACK_ROWS = 16, CE_COUNT_ROWS = 1024;
+inline int64_t ce_pack_ctas(int64_t n) { return tiles(n, CE_PACK_ROWS); }
+
+// cross_entropy.cu
+int ce_pack(const CeProblem& q, const CePacked& p, const float* dloss, const float* lse, cudaStream_t s);
+// loss and lse from `parts` (maximum, sum) pairs of each packed row, [row][parts].  word: that of packed rows; null: rows are those
+// of the call, and the targets are looked at here.
+int ce_join(const CeProblem& q, const float* top, const float* total, int64_t parts, const int32_t* word, const int32_t* slot,
+            const float* target_logit, float* loss, float* lse, cudaStream_t s);
+// out[n][D] = the sums of parts[splits][rows][pitch]; slot as above or null
+int ce_sum(const float* parts, int64_t splits, int64_t n, int64_t D, int64_t rows, int64_t pitch, const int32_t* slot, void* out,
+           int32_t dtype, cudaStream_t s);
 
 // cross_entropy_mma.cu
 size_t ce_mma_forward_bytes(int64_t n, int64_t D, int64_t V);
 size_t ce_mma_backward_bytes(int64_t n, int64_t D, int64_t V);
 int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s);
 int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, void* dhidden, void* dweight, cudaStream_t s);
+
+#ifdef __CUDACC__
+// a row's target as a word, -1 where it is ignored or no class
+__device__ __forceinline__ int32_t target_word(const void* target, bool ids64, int64_t row, int64_t V, int64_t ignore_index, bool* wrong) {
+  const int64_t t = ids64 ? static_cast<const int64_t*>(target)[row] : static_cast<int64_t>(static_cast<const int32_t*>(target)[row]);
+  const bool in = t >= 0 && t < V;
+  *wrong = !in && t != ignore_index;
+  return in && t != ignore_index ? static_cast<int32_t>(t) : -1;
+}
+#endif
 
 }  // namespace dgs

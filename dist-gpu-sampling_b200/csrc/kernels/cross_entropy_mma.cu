@@ -79,7 +79,7 @@ enum OutKind { OUT_F32_STORE, OUT_F32_ADD, OUT_TYPED, OUT_TYPED_ODD };
 
 // One of the two products of a PRODUCT launch
 struct Part {
-  int32_t a_mn;     // A is held with m contiguous
+  int32_t a_mn;     // A is held with m contiguous; its k are rows of the call (dW), else its m are (dh)
   int32_t items, n_tiles, splits;
   int32_t k_blocks;
   int32_t n_total;  // columns of the result
@@ -93,16 +93,21 @@ struct alignas(64) MmaArgs {
   CUtensorMap a[2], b[2], out[2];
   Part part[2];
   int32_t items, parts;
-  int32_t row_blocks, col_tiles, slices, k_blocks;
+  int32_t col_tiles, slices, k_blocks;
   int64_t n, V;  // GRAD: V is the width of the piece
   int32_t v0;    // GRAD: first class of the piece
-  const int32_t* word;
+  const int32_t* live;  // the number of packed rows, <= n; null: n
+  const int32_t* word;  // of packed rows; null: the rows are those of the call, and so are the targets (STATS)
+  const void* target;
+  int64_t ignore_index;
+  int32_t ids64;
+  int32_t largest_count;
   float* target_logit;
   float* top;
   float* total;
   const float* dloss;
   const float* lse;
-  const float* scale;  // 16-bit floats: the factor of G and its inverse; null: 1
+  const float* largest;  // float16: the largest |dloss| of each CTA that packed rows; null: G is not scaled
   int32_t* status;
 };
 
@@ -114,25 +119,54 @@ struct Tile {
   int32_t split;
 };
 
+// What depends on the number of packed rows, which a launch learns from memory
+struct Extent {
+  int32_t rows, row_blocks, items, first_items;  // first_items: of part 0 (PRODUCT)
+  int32_t row_k_blocks;
+};
 template <int MODE>
-__device__ __forceinline__ Tile tile_of(const MmaArgs& a, int item, int t) {
+__device__ __forceinline__ Extent extent_of(const MmaArgs& a) {
+  Extent e;
+  e.rows = a.live != nullptr ? *a.live : static_cast<int32_t>(a.n);
+  e.row_blocks = e.rows > 0 ? (e.rows + M_TILE - 1) / M_TILE : 1;  // (no row at all: one block of zeros)
+  e.row_k_blocks = e.rows > 0 ? (e.rows + K_TILE - 1) / K_TILE : 1;
+  e.first_items = 0;
+  if constexpr (MODE == STATS) {
+    e.items = e.row_blocks * a.slices;
+  } else if constexpr (MODE == GRAD) {
+    e.items = e.row_blocks * a.col_tiles;
+  } else {
+    e.items = 0;
+    for (int i = 0; i < a.parts; ++i) {
+      const int m_tiles = a.part[i].a_mn ? (a.part[i].m_total + M_TILE - 1) / M_TILE : e.row_blocks;
+      const int items = m_tiles * a.part[i].n_tiles * a.part[i].splits;
+      if (i == 0) e.first_items = items;
+      e.items += items;
+    }
+  }
+  return e;
+}
+
+template <int MODE>
+__device__ __forceinline__ Tile tile_of(const MmaArgs& a, const Extent& ext, int item, int t) {
   Tile x;
   x.which = 0;
   x.split = 0;
   x.n = N_TILE;
   if constexpr (MODE == PRODUCT) {
-    x.which = item >= a.part[0].items;
+    x.which = item >= ext.first_items;
     const Part& p = a.part[x.which];
-    const int i = item - (x.which ? a.part[0].items : 0);
+    const int i = item - (x.which ? ext.first_items : 0);
+    const int k_blocks = p.a_mn ? ext.row_k_blocks : p.k_blocks;
     const int nt = i % p.n_tiles, rest = i / p.n_tiles;
     x.split = rest % p.splits;
     x.m0 = rest / p.splits * M_TILE;
     x.n0 = nt * N_TILE;
     if (p.n_total - x.n0 <= N_TILE / 2) x.n = N_TILE / 2;
-    x.k0 = static_cast<int32_t>(static_cast<int64_t>(p.k_blocks) * x.split / p.splits);
-    x.k1 = static_cast<int32_t>(static_cast<int64_t>(p.k_blocks) * (x.split + 1) / p.splits);
+    x.k0 = static_cast<int32_t>(static_cast<int64_t>(k_blocks) * x.split / p.splits);
+    x.k1 = static_cast<int32_t>(static_cast<int64_t>(k_blocks) * (x.split + 1) / p.splits);
   } else {
-    x.m0 = item % a.row_blocks * M_TILE;
+    x.m0 = item % ext.row_blocks * M_TILE;
     x.n0 = t * N_TILE;
     x.k0 = 0;
     x.k1 = a.k_blocks;
@@ -141,13 +175,13 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, int item, int t) {
 }
 // the column tiles [t0, t1) of an item
 template <int MODE>
-__device__ __forceinline__ void range_of(const MmaArgs& a, int item, int* t0, int* t1) {
+__device__ __forceinline__ void range_of(const MmaArgs& a, const Extent& ext, int item, int* t0, int* t1) {
   if constexpr (MODE == STATS) {
-    const int slice = item / a.row_blocks;
+    const int slice = item / ext.row_blocks;
     *t0 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * slice / a.slices);
     *t1 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * (slice + 1) / a.slices);
   } else if constexpr (MODE == GRAD) {
-    *t0 = item / a.row_blocks;
+    *t0 = item / ext.row_blocks;
     *t1 = *t0 + 1;
   } else {
     *t0 = 0;
@@ -220,6 +254,18 @@ __device__ __forceinline__ void st_shared(uint32_t addr, uint32_t x, uint32_t y,
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// float16: G is scaled by a power of two that brings its largest possible value, max |dloss|, to just below 2^15, so that
+// probabilities down to 2^-29 of it stay normal numbers; the products' results are scaled back.
+__device__ __forceinline__ float grad_factor(const float* largest, int count, int lane, bool inverse) {
+  float m = 0.0f;
+  for (int i = lane; i < count; i += 32) m = fmaxf(m, largest[i]);
+  m = __uint_as_float(__reduce_max_sync(FULL_MASK, __float_as_uint(m)));
+  int e = 0;
+  if (m > 0.0f && m < INFINITY) frexpf(m, &e);  // m = f 2^e, f in [1/2, 1)
+  e = e < -100 ? -100 : e > 100 ? 100 : e;
+  return ldexpf(1.0f, inverse ? e - 15 : 15 - e);
+}
+
 template <int MODE, bool BF16>
 __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_mma_kernel(const __grid_constant__ MmaArgs a) {
   constexpr int STAGES = stages<MODE>();
@@ -253,6 +299,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_word) : "memory");
   pdl_enter();
+  const Extent ext = extent_of<MODE>(a);
 
   bool ok = true;  // this thread's waits have all ended well
   if (warp == 0 && lane == 0) {
@@ -260,11 +307,11 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
     fence_async_global();  // operands that ordinary stores of an earlier launch wrote
     int st = 0;
     uint32_t phase = 0;
-    for (int item = pair; ok && item < a.items; item += pairs) {
+    for (int item = pair; ok && item < ext.items; item += pairs) {
       int t0, t1;
-      range_of<MODE>(a, item, &t0, &t1);
+      range_of<MODE>(a, ext, item, &t0, &t1);
       for (int t = t0; ok && t < t1; ++t) {
-        const Tile x = tile_of<MODE>(a, item, t);
+        const Tile x = tile_of<MODE>(a, ext, item, t);
         const CUtensorMap *ma = &a.a[x.which], *mb = &a.b[x.which];
         const bool a_mn = MODE == PRODUCT && a.part[x.which].a_mn;
         const uint32_t bytes = 2 * A_BYTES + x.n * (K_TILE * 2);  // of both CTAs
@@ -298,11 +345,11 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
     // ---- products
     int st = 0, buf = 0;
     uint32_t phase = 0, acc_phase = 0;
-    for (int item = pair; ok && item < a.items; item += pairs) {
+    for (int item = pair; ok && item < ext.items; item += pairs) {
       int t0, t1;
-      range_of<MODE>(a, item, &t0, &t1);
+      range_of<MODE>(a, ext, item, &t0, &t1);
       for (int t = t0; ok && t < t1; ++t) {
-        const Tile x = tile_of<MODE>(a, item, t);
+        const Tile x = tile_of<MODE>(a, ext, item, t);
         const bool a_mn = MODE == PRODUCT && a.part[x.which].a_mn;
         constexpr bool b_mn = MODE == PRODUCT;
         const uint32_t idesc = mma_desc(BF16, a_mn, b_mn, M_TILE, x.n);
@@ -335,18 +382,20 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
     const uint32_t free_bar = in_cta(acc_empty, 0);
     int buf = 0;
     uint32_t acc_phase = 0;
-    const float factor = MODE != STATS && a.scale != nullptr ? a.scale[MODE == PRODUCT] : 1.0f;
-    for (int item = pair; ok && item < a.items; item += pairs) {
+    float factor = 1.0f;
+    if (MODE != STATS && a.largest != nullptr) factor = grad_factor(a.largest, a.largest_count, lane, MODE == PRODUCT);
+    for (int item = pair; ok && item < ext.items; item += pairs) {
       int t0, t1;
-      range_of<MODE>(a, item, &t0, &t1);
+      range_of<MODE>(a, ext, item, &t0, &t1);
       RowSum sum;
       for (int t = t0; t < t1; ++t) {
-        const Tile x = tile_of<MODE>(a, item, t);
+        const Tile x = tile_of<MODE>(a, ext, item, t);
         const int32_t row = x.m0 + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
         int32_t word = -1;
         float grad = 0.0f, lse = 0.0f;
-        if (MODE != PRODUCT && row < a.n) {
-          word = a.word[row];
+        if (MODE != PRODUCT && row < ext.rows) {
+          bool wrong;
+          word = MODE == GRAD || a.word != nullptr ? a.word[row] : target_word(a.target, a.ids64, row, a.V, a.ignore_index, &wrong);
           if (MODE == GRAD && word >= 0) {
             grad = a.dloss[row] * factor;
             lse = a.lse[row];
@@ -460,11 +509,11 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
         if (buf == 0) acc_phase ^= 1;
       }
       if (MODE == STATS && ok) {
-        const int32_t row = item % a.row_blocks * M_TILE + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
-        const int64_t part = item / a.row_blocks * COL_GROUPS + group;
-        if (row < a.n) {
-          a.top[part * a.n + row] = sum.top;
-          a.total[part * a.n + row] = sum.total;
+        const int32_t row = item % ext.row_blocks * M_TILE + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
+        const int64_t at = static_cast<int64_t>(row) * (a.slices * COL_GROUPS) + item / ext.row_blocks * COL_GROUPS + group;
+        if (row < ext.rows) {
+          a.top[at] = sum.top;
+          a.total[at] = sum.total;
         }
       }
     }
@@ -482,39 +531,19 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
   if (warp == 2) tmem_free(tmem, TMEM_COLS);
 }
 
-// float16: G is scaled by a power of two that brings its largest possible value, max |dloss|, to just below 2^15, so that
-// probabilities down to 2^-29 of it stay normal numbers.  scale = {factor, its inverse}.
-__global__ void __launch_bounds__(1024) ce_scale_kernel(const float* __restrict__ dloss, const int32_t* __restrict__ word,
-                                                        const int64_t n, float* __restrict__ scale) {
-  __shared__ float top[32];
-  pdl_enter();
-  float m = 0.0f;
-  for (int64_t i = threadIdx.x; i < n; i += 1024)
-    if (word[i] >= 0) m = fmaxf(m, fabsf(dloss[i]));
-  m = __uint_as_float(__reduce_max_sync(FULL_MASK, __float_as_uint(m)));
-  if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    m = __uint_as_float(__reduce_max_sync(FULL_MASK, __float_as_uint(top[threadIdx.x])));
-    if (threadIdx.x == 0) {
-      int e = 0;
-      if (m > 0.0f && m < INFINITY) frexpf(m, &e);  // m = f 2^e, f in [1/2, 1)
-      e = e < -100 ? -100 : e > 100 ? 100 : e;
-      scale[0] = ldexpf(1.0f, 15 - e);
-      scale[1] = ldexpf(1.0f, e - 15);
-    }
-  }
-}
-
 // The weight's rows, `pitch` elements apart (rows of an odd length cannot be fetched by TMA where they lie)
 __global__ void __launch_bounds__(256) ce_pack_weight_kernel(const uint16_t* __restrict__ weight, const int64_t stride, const int64_t V,
                                                              const int D, const int pitch, uint16_t* __restrict__ packed) {
   pdl_enter();
-  const int64_t count = V * pitch;
-  for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < count; i += gridDim.x * int64_t(256)) {
-    const int64_t row = i / pitch;
-    const int j = static_cast<int>(i - row * pitch);
-    packed[i] = j < D ? weight[row * stride + j] : uint16_t(0);
+  const int lane = threadIdx.x & 31;
+  for (int64_t row = blockIdx.x * int64_t(8) + (threadIdx.x >> 5); row < V; row += gridDim.x * int64_t(8)) {
+    const uint16_t* from = weight + row * stride;
+    uint32_t* to = reinterpret_cast<uint32_t*>(packed + row * pitch);
+#pragma unroll 4
+    for (int j = lane * 2; j < pitch; j += 64) {
+      const uint32_t lo = j < D ? from[j] : 0u, hi = j + 1 < D ? from[j + 1] : 0u;
+      to[j >> 1] = lo | (hi << 16);
+    }
   }
 }
 
@@ -522,10 +551,16 @@ __global__ void __launch_bounds__(256) ce_pack_weight_kernel(const uint16_t* __r
 struct MmaPlan {
   int64_t pitch, row_blocks, col_tiles, slices, pairs;
   int64_t piece, splits, dpitch;
-  bool one_piece;
-  size_t packed, word, weight, target_logit, top, total, scale, g, dh;
+  bool one_piece, compact;
+  size_t packed, word, slot, live, counts, weight, target_logit, top, total, dloss, lse, largest, g, dh;
   size_t forward_bytes, backward_bytes;
 };
+
+// Whether the rows without a valid target are left out of the products.  That takes a launch more, and dh leaves by way of its
+// 32-bit form to be spread over the call's rows: COMPACT_COST.  Below, the products themselves take some 40 us.
+bool worth_compacting(int64_t n, int64_t D, int64_t V) {
+  return static_cast<double>(n) * static_cast<double>(D) * static_cast<double>(V) >= 2e10 && n <= (int64_t(1) << 22);
+}
 
 MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   MmaPlan p{};
@@ -546,9 +581,15 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   if (most < 16) most = 16;
   p.splits = tiles(dh_k, most);
   if (p.splits > 32) p.splits = 32;
+  p.compact = worth_compacting(n, D, V);
   Layout l;
   p.packed = l.take(n * p.pitch * 2);
   p.word = l.take(n * 4);
+  if (p.compact) {
+    p.slot = l.take(n * 4);
+    p.live = l.take(4);
+    p.counts = l.take(tiles(n, CE_COUNT_ROWS) * 4);
+  }
   if (D % 8 != 0) p.weight = l.take(V * p.pitch * 2);
   const Layout common = l;
   p.target_logit = l.take(n * 4);
@@ -556,9 +597,11 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.total = l.take(COL_GROUPS * p.slices * n * 4);
   p.forward_bytes = l.bytes;
   l = common;
-  p.scale = l.take(8);
+  p.dloss = l.take(n * 4);
+  p.lse = l.take(n * 4);
+  p.largest = l.take(ce_pack_ctas(n) * 4);
   p.g = l.take(n * p.piece * 2);
-  if (!(p.one_piece && p.splits == 1)) p.dh = l.take(p.splits * p.row_blocks * M_TILE * p.dpitch * 4);
+  if (!(p.one_piece && p.splits == 1 && !p.compact)) p.dh = l.take(p.splits * p.row_blocks * M_TILE * p.dpitch * 4);
   p.backward_bytes = l.bytes;
   return p;
 }
@@ -595,7 +638,7 @@ int fetchable_weight(const CeProblem& q, const MmaPlan& p, Weight* w, cudaStream
   DGS_REQUIRE(q.D % 8 != 0, DGS_ERR_INVALID, "linear_cross_entropy: rows of %lld 16-bit elements must begin at 16-byte boundaries",
               static_cast<long long>(q.D));
   uint16_t* packed = reinterpret_cast<uint16_t*>(q.ws + p.weight);
-  const int64_t need = tiles(q.V * p.pitch, 256 * 4), most = static_cast<int64_t>(sm_count()) * 8;
+  const int64_t need = tiles(q.V, 8), most = static_cast<int64_t>(sm_count()) * 8;
   DGS_CUDA_TRY(launch_training(ce_pack_weight_kernel, dim3(static_cast<unsigned>(need < most ? need : most)), 256, 0, s, w->p,
                                q.weight_stride, q.V, static_cast<int>(q.D), static_cast<int>(p.pitch), packed));
   *w = Weight{packed, p.pitch};
@@ -607,49 +650,68 @@ int fetchable_weight(const CeProblem& q, const MmaPlan& p, Weight* w, cudaStream
 size_t ce_mma_forward_bytes(int64_t n, int64_t D, int64_t V) { return make_plan(n, D, V).forward_bytes; }
 size_t ce_mma_backward_bytes(int64_t n, int64_t D, int64_t V) { return make_plan(n, D, V).backward_bytes; }
 
+static CePacked packed_rows(const CeProblem& q, const MmaPlan& p) {
+  CePacked r{};
+  r.rows = q.ws + p.packed;
+  r.pitch = p.pitch;
+  r.word = reinterpret_cast<int32_t*>(q.ws + p.word);
+  r.compact = p.compact;
+  if (p.compact) {
+    r.slot = reinterpret_cast<int32_t*>(q.ws + p.slot);
+    r.live = reinterpret_cast<int32_t*>(q.ws + p.live);
+    r.counts = reinterpret_cast<int32_t*>(q.ws + p.counts);
+  }
+  return r;
+}
+
 int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) {
   const MmaPlan p = make_plan(q.n, q.D, q.V);
-  void* packed = q.ws + p.packed;
-  int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
-  float* tl = reinterpret_cast<float*>(q.ws + p.target_logit);
-  if (int rc = ce_pack(q, packed, p.pitch, word, tl, s)) return rc;
+  CePacked r = packed_rows(q, p);
+  // A row's statistics depend on that row alone: rows that TMA can fetch need no packing (what an ignored row holds ends there)
+  const bool where_they_lie = !p.compact && aligned_to(q.hidden, 16) && (q.n == 1 ? q.D : q.hidden_stride) % 8 == 0;
+  if (!where_they_lie) {
+    if (int rc = ce_pack(q, r, nullptr, nullptr, s)) return rc;
+  }
   Weight w;
   if (int rc = fetchable_weight(q, p, &w, s)) return rc;
   MmaArgs a{};
-  if (int rc = make_map(&a.a[0], packed, q.dtype, q.D, q.n, p.pitch, K_TILE, M_CTA)) return rc;
+  if (int rc = make_map(&a.a[0], where_they_lie ? q.hidden : r.rows, q.dtype, q.D, q.n,
+                        where_they_lie ? (q.n == 1 ? q.D : q.hidden_stride) : p.pitch, K_TILE, M_CTA))
+    return rc;
   if (int rc = make_map(&a.b[0], w.p, q.dtype, q.D, q.V, w.stride, K_TILE, N_TILE / 2)) return rc;
   a.items = static_cast<int32_t>(p.row_blocks * p.slices);
-  a.row_blocks = static_cast<int32_t>(p.row_blocks);
   a.col_tiles = static_cast<int32_t>(p.col_tiles);
   a.slices = static_cast<int32_t>(p.slices);
   a.k_blocks = static_cast<int32_t>(tiles(q.D, K_TILE));
   a.n = q.n;
   a.V = q.V;
-  a.word = word;
-  a.target_logit = tl;
+  a.live = r.live;
+  a.word = where_they_lie ? nullptr : r.word;
+  a.target = q.target;
+  a.ids64 = q.ids64;
+  a.ignore_index = q.ignore_index;
+  a.target_logit = reinterpret_cast<float*>(q.ws + p.target_logit);
   a.top = reinterpret_cast<float*>(q.ws + p.top);
   a.total = reinterpret_cast<float*>(q.ws + p.total);
   a.status = q.status;
   if (int rc = launch<STATS>(a, p.pairs, q.dtype, s)) return rc;
-  return ce_join(q, a.top, a.total, COL_GROUPS * p.slices, word, tl, loss, lse, s);
+  return ce_join(q, a.top, a.total, COL_GROUPS * p.slices, a.word, r.slot, a.target_logit, loss, lse, s);
 }
 
 int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, void* dhidden, void* dweight, cudaStream_t s) {
   const MmaPlan p = make_plan(q.n, q.D, q.V);
-  void* packed = q.ws + p.packed;
-  int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
-  if (int rc = ce_pack(q, packed, p.pitch, word, nullptr, s)) return rc;
-  float* scale = nullptr;
-  if (q.dtype == DGS_F16) {
-    scale = reinterpret_cast<float*>(q.ws + p.scale);
-    DGS_CUDA_TRY(launch_training(ce_scale_kernel, dim3(1), 1024, 0, s, dloss, word, q.n, scale));
-  }
+  CePacked r = packed_rows(q, p);
+  r.dloss = reinterpret_cast<float*>(q.ws + p.dloss);
+  r.lse = reinterpret_cast<float*>(q.ws + p.lse);
+  if (q.dtype == DGS_F16) r.largest = reinterpret_cast<float*>(q.ws + p.largest);
+  if (int rc = ce_pack(q, r, dloss, lse, s)) return rc;
+  const void* packed = r.rows;
   Weight w;
   if (int rc = fetchable_weight(q, p, &w, s)) return rc;
   uint16_t* g = reinterpret_cast<uint16_t*>(q.ws + p.g);
   float* dh = reinterpret_cast<float*>(q.ws + p.dh);
   // results whose rows begin at 16-byte boundaries leave by TMA
-  const bool dh_direct = p.one_piece && p.splits == 1, even = q.D % 8 == 0;
+  const bool dh_direct = p.one_piece && p.splits == 1 && !p.compact, even = q.D % 8 == 0;
   const int32_t d_tiles = static_cast<int32_t>(tiles(q.D, N_TILE));
   for (int64_t v0 = 0; v0 < q.V; v0 += p.piece) {
     const int64_t width = q.V - v0 < p.piece ? q.V - v0 : p.piece;
@@ -658,17 +720,18 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     if (int rc = make_map(&a.a[0], packed, q.dtype, q.D, q.n, p.pitch, K_TILE, M_CTA)) return rc;
     if (int rc = make_map(&a.b[0], wp, q.dtype, q.D, width, w.stride, K_TILE, N_TILE / 2)) return rc;
     if (int rc = make_map(&a.out[0], g, q.dtype, width, q.n, p.piece, 64, 32)) return rc;
-    a.row_blocks = static_cast<int32_t>(p.row_blocks);
     a.col_tiles = static_cast<int32_t>(tiles(width, N_TILE));
-    a.items = a.row_blocks * a.col_tiles;
+    a.items = static_cast<int32_t>(p.row_blocks) * a.col_tiles;
     a.k_blocks = static_cast<int32_t>(tiles(q.D, K_TILE));
     a.n = q.n;
     a.V = width;
     a.v0 = static_cast<int32_t>(v0);
-    a.word = word;
-    a.dloss = dloss;
-    a.lse = lse;
-    a.scale = scale;
+    a.live = r.live;
+    a.word = r.word;
+    a.dloss = r.dloss;
+    a.lse = r.lse;
+    a.largest = r.largest;
+    a.largest_count = static_cast<int32_t>(ce_pack_ctas(q.n));
     a.status = q.status;
     if (int rc = launch<GRAD>(a, p.pairs, q.dtype, s)) return rc;
 
@@ -717,11 +780,14 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     }
     m.parts = parts;
     m.items = m.part[0].items + m.part[1].items;
-    m.scale = scale;
+    m.n = q.n;
+    m.live = r.live;
+    m.largest = r.largest;
+    m.largest_count = a.largest_count;
     m.status = q.status;
     if (int rc = launch<PRODUCT>(m, p.pairs, q.dtype, s)) return rc;
   }
-  if (dhidden != nullptr && !dh_direct) return ce_sum(dh, p.splits, q.n, q.D, p.row_blocks * M_TILE, p.dpitch, dhidden, q.dtype, s);
+  if (dhidden != nullptr && !dh_direct) return ce_sum(dh, p.splits, q.n, q.D, p.row_blocks * M_TILE, p.dpitch, r.slot, dhidden, q.dtype, s);
   return DGS_OK;
 }
 
