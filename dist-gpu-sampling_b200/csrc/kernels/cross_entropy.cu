@@ -147,7 +147,24 @@ __global__ void __launch_bounds__(CE_THREADS) ce_pack_kernel(const __grid_consta
     }
   }
   if (a.to.compact && blockIdx.x == gridDim.x - 1) {
-    if (threadIdx.x == 0) *a.to.live = live;
+    if (warp == 0) {  // slices_for, a lane for every 32nd number of slices: fewest tiles in the busiest slot, then fewest slices
+      const int blocks = live > 0 ? (live + a.to.block_rows - 1) / a.to.block_rows : 1;
+      unsigned long long best = ~0ull;
+      for (int k = 1 + lane; k <= a.to.col_tiles && k <= a.to.slots; k += 32) {
+        const unsigned long long rounds = (static_cast<unsigned long long>(blocks) * k + a.to.slots - 1) / a.to.slots;
+        const unsigned long long cost = (rounds * ((a.to.col_tiles + k - 1) / k)) << 10 | k;
+        best = cost < best ? cost : best;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(FULL_MASK, best, o);
+        best = other < best ? other : best;
+      }
+      if (lane == 0) {
+        a.to.live[0] = live;
+        a.to.live[1] = static_cast<int32_t>(best & 1023);
+      }
+    }
     int64_t end = (static_cast<int64_t>(live) + 63) / 64 * 64;
     if (end == 0) end = 64;
     if (end > a.n) end = a.n;
@@ -302,10 +319,10 @@ __global__ void __launch_bounds__(CE_THREADS, 2) ce_stats_kernel(const Operand<t
 
 struct JoinArgs {
   const float *top, *total;
-  int64_t parts, n, V, ignore_index;
+  int64_t groups, slices, n, V, ignore_index;
   const void* target;
   int32_t ids64;
-  const int32_t *word, *slot;
+  const int32_t *live, *word, *slot;
   const float* target_logit;
   float *loss, *lse;
   int32_t* status;
@@ -333,14 +350,15 @@ __global__ void __launch_bounds__(CE_THREADS) ce_join_kernel(const __grid_consta
     if (lane == 0) a.loss[row] = a.lse[row] = 0.0f;
     return;
   }
-  const float *top = a.top + c * a.parts, *total = a.total + c * a.parts;
+  const int64_t parts = a.groups * (a.live != nullptr ? a.live[1] : a.slices);
+  const float *top = a.top + c * parts, *total = a.total + c * parts;
   float m = -INFINITY;
-  for (int64_t p = lane; p < a.parts; p += 32) m = fmaxf(m, top[p]);
+  for (int64_t p = lane; p < parts; p += 32) m = fmaxf(m, top[p]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
   const float base = m == -INFINITY ? 0.0f : m;
   float s = 0.0f;
-  for (int64_t p = lane; p < a.parts; p += 32) s += total[p] * expf(top[p] - base);
+  for (int64_t p = lane; p < parts; p += 32) s += total[p] * expf(top[p] - base);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL_MASK, s, o);
   if (lane == 0) {
@@ -501,7 +519,7 @@ int forward32(const CeProblem& q, float* loss, float* lse, cudaStream_t s) {
   const StatsArgs a{q.n, q.V, static_cast<int>(q.D), p.row_blocks, p.col_tiles, p.slices, word, tl, top, total};
   DGS_CUDA_TRY(launch_training(ce_stats_kernel, dim3(static_cast<unsigned>(p.row_blocks * p.slices)), CE_THREADS, 0, s,
                                Operand<true>{packed, p.pitch, q.n}, Operand<true>{static_cast<const float*>(q.weight), q.weight_stride, q.V}, a));
-  return ce_join(q, top, total, p.slices, word, nullptr, tl, loss, lse, s);
+  return ce_join(q, top, total, 1, p.slices, nullptr, word, nullptr, tl, loss, lse, s);
 }
 
 int backward32(const CeProblem& q, const float* dloss, const float* lse, float* dhidden, float* dweight, cudaStream_t s) {
@@ -562,9 +580,9 @@ int ce_pack(const CeProblem& q, const CePacked& p, const float* dloss, const flo
   return DGS_OK;
 }
 
-int ce_join(const CeProblem& q, const float* top, const float* total, int64_t parts, const int32_t* word, const int32_t* slot,
-            const float* target_logit, float* loss, float* lse, cudaStream_t s) {
-  const JoinArgs a{top, total, parts, q.n, q.V, q.ignore_index, q.target, q.ids64, word, slot, target_logit, loss, lse, q.status};
+int ce_join(const CeProblem& q, const float* top, const float* total, int64_t groups, int64_t slices, const int32_t* live,
+            const int32_t* word, const int32_t* slot, const float* target_logit, float* loss, float* lse, cudaStream_t s) {
+  const JoinArgs a{top, total, groups, slices, q.n, q.V, q.ignore_index, q.target, q.ids64, live, word, slot, target_logit, loss, lse, q.status};
   DGS_CUDA_TRY(launch_training(ce_join_kernel, dim3(static_cast<unsigned>(tiles(q.n, CE_THREADS / 32))), CE_THREADS, 0, s, a));
   return DGS_OK;
 }

@@ -48,7 +48,8 @@ inline int64_t slices_for(int64_t rows, int64_t cols, int64_t slots) {
 // The rows that count, as cross_entropy.cu packs them.  Packed row c holds what the products read: the hidden row, its target
 // as a 32-bit word (-1: none), and for the backward pass dloss and lse.  Either row c is row c of the call (rows without a valid
 // target: zeros, word -1), or (compact) the rows with a valid target alone, in their order; then slot[i] is row i's place among
-// them (-1: none), *live their number, and the packed rows from there to the next multiple of 64 (one at least) are zeros.
+// them (-1: none), live[0] their number, live[1] the slices for that many rows in blocks of block_rows, and the packed rows from
+// there to the next multiple of 64 (one at least) are zeros.
 struct CePacked {
   void* rows;
   int64_t pitch;
@@ -57,6 +58,7 @@ struct CePacked {
   float* largest;          // [ce_pack_ctas(n)] largest |dloss| among a CTA's rows; may be null
   bool compact;
   int32_t *slot, *live;
+  int32_t block_rows, col_tiles, slots;  // what slices_for takes
   int32_t* counts;         // [tiles(n, CE_COUNT_ROWS)], scratch
 };
 constexpr int CE_PACK_ROWS = 16, CE_COUNT_ROWS = 1024;
@@ -64,10 +66,10 @@ inline int64_t ce_pack_ctas(int64_t n) { return tiles(n, CE_PACK_ROWS); }
 
 // cross_entropy.cu
 int ce_pack(const CeProblem& q, const CePacked& p, const float* dloss, const float* lse, cudaStream_t s);
-// loss and lse from `parts` (maximum, sum) pairs of each packed row, [row][parts].  word: that of packed rows; null: rows are those
-// of the call, and the targets are looked at here.
-int ce_join(const CeProblem& q, const float* top, const float* total, int64_t parts, const int32_t* word, const int32_t* slot,
-            const float* target_logit, float* loss, float* lse, cudaStream_t s);
+// loss and lse from (maximum, sum) pairs of each packed row, [row][slices][groups].  live, slot: those of compact rows, or null.
+// word: that of packed rows; null: rows are those of the call, and the targets are looked at here.
+int ce_join(const CeProblem& q, const float* top, const float* total, int64_t groups, int64_t slices, const int32_t* live,
+            const int32_t* word, const int32_t* slot, const float* target_logit, float* loss, float* lse, cudaStream_t s);
 // out[n][D] = the sums of parts[splits][rows][pitch]; slot as above or null
 int ce_sum(const float* parts, int64_t splits, int64_t n, int64_t D, int64_t rows, int64_t pitch, const int32_t* slot, void* out,
            int32_t dtype, cudaStream_t s);

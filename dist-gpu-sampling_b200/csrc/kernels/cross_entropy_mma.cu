@@ -63,7 +63,10 @@ constexpr uint32_t BOX_BYTES = 64 * K_TILE * 2;  // 64 of m (or n) by 64 of k, M
 constexpr uint32_t STAGING_BYTES = 4096;         // 32 rows of 128 bytes: one store of a warp
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int64_t PIECE_BYTES = int64_t(96) << 20;  // of G
+// Of G.  Two products read it, so it passes through HBM about three times unless L2 holds it (96 MB and less), which at D >= 200
+// is hidden behind the products; larger pieces waste less on rounds that are not full (8 192 rows of 1 024, 65 537 classes:
+// 48 MB 4.07 ms, 96 MB 3.64, 384 MB 3.53, 768 MB 3.57).
+constexpr int64_t PIECE_BYTES = int64_t(256) << 20;
 
 enum Mode { STATS, GRAD, PRODUCT };
 template <int MODE>
@@ -80,7 +83,7 @@ enum OutKind { OUT_F32_STORE, OUT_F32_ADD, OUT_TYPED, OUT_TYPED_ODD };
 // One of the two products of a PRODUCT launch
 struct Part {
   int32_t a_mn;     // A is held with m contiguous; its k are rows of the call (dW), else its m are (dh)
-  int32_t items, n_tiles, splits;
+  int32_t n_tiles, n_step, splits;  // tiles of n_step columns: N_TILE, or half of it
   int32_t k_blocks;
   int32_t n_total;  // columns of the result
   int32_t m_total;
@@ -122,7 +125,7 @@ struct Tile {
 // What depends on the number of packed rows, which a launch learns from memory
 struct Extent {
   int32_t rows, row_blocks, items, first_items;  // first_items: of part 0 (PRODUCT)
-  int32_t row_k_blocks;
+  int32_t row_k_blocks, slices;
 };
 template <int MODE>
 __device__ __forceinline__ Extent extent_of(const MmaArgs& a) {
@@ -131,8 +134,9 @@ __device__ __forceinline__ Extent extent_of(const MmaArgs& a) {
   e.row_blocks = e.rows > 0 ? (e.rows + M_TILE - 1) / M_TILE : 1;  // (no row at all: one block of zeros)
   e.row_k_blocks = e.rows > 0 ? (e.rows + K_TILE - 1) / K_TILE : 1;
   e.first_items = 0;
+  e.slices = a.live != nullptr ? a.live[1] : a.slices;
   if constexpr (MODE == STATS) {
-    e.items = e.row_blocks * a.slices;
+    e.items = e.row_blocks * e.slices;
   } else if constexpr (MODE == GRAD) {
     e.items = e.row_blocks * a.col_tiles;
   } else {
@@ -161,8 +165,8 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const Extent& ext, int
     const int nt = i % p.n_tiles, rest = i / p.n_tiles;
     x.split = rest % p.splits;
     x.m0 = rest / p.splits * M_TILE;
-    x.n0 = nt * N_TILE;
-    if (p.n_total - x.n0 <= N_TILE / 2) x.n = N_TILE / 2;
+    x.n0 = nt * p.n_step;
+    if (p.n_step < N_TILE || p.n_total - x.n0 <= N_TILE / 2) x.n = N_TILE / 2;
     x.k0 = static_cast<int32_t>(static_cast<int64_t>(k_blocks) * x.split / p.splits);
     x.k1 = static_cast<int32_t>(static_cast<int64_t>(k_blocks) * (x.split + 1) / p.splits);
   } else {
@@ -178,8 +182,8 @@ template <int MODE>
 __device__ __forceinline__ void range_of(const MmaArgs& a, const Extent& ext, int item, int* t0, int* t1) {
   if constexpr (MODE == STATS) {
     const int slice = item / ext.row_blocks;
-    *t0 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * slice / a.slices);
-    *t1 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * (slice + 1) / a.slices);
+    *t0 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * slice / ext.slices);
+    *t1 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * (slice + 1) / ext.slices);
   } else if constexpr (MODE == GRAD) {
     *t0 = item / ext.row_blocks;
     *t1 = *t0 + 1;
@@ -195,9 +199,28 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// A logit (or lse) so large that its product with log2(e) may leave the range of 32-bit floats: the type's lowest value as a
-// mask, infinities
+// A logit (or lse) whose product with log2(e) may leave the range of 32-bit floats (the type's lowest value as a mask), or that is
+// no finite number
 __device__ __forceinline__ bool far(float x) { return !(fabsf(x) < 1e38f); }
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// e^(v - base) for 32 values that are no NaN, in pairs: packed additions and multiplications halve what stands beside the 16 ex2 a
+// clock and SM (1 024 rows of 128 against 2.4 M classes: 845 -> 723 us.  A share of the exponentials as polynomials on the
+// multiply-add units does not help: every sixth pair 733, every fourth 797).
+__device__ __forceinline__ void exp_pairs(const uint32_t (&v)[32], float base, uint64_t (&e)[16]) {
+  const float minus = -base * LOG2E;
+  const uint64_t scale2 = two(LOG2E, LOG2E), minus2 = two(minus, minus);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float lo, hi;
+    split2(fma2(two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, minus2), &lo, &hi);
+    e[i] = two(ex2(lo), ex2(hi));
+  }
+}
 
 // Running maximum of one row and the sum of e^(s - top)
 struct RowSum {
@@ -210,24 +233,29 @@ struct RowSum {
     }
     float m[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = fmaxf(at(v, i), at(v, i + 4));
+    for (int i = 0; i < 4; ++i) m[i] = max_or_nan(at(v, i), at(v, i + 4));
 #pragma unroll
-    for (int i = 8; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], at(v, i));
-    const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 8; i < 32; ++i) m[i & 3] = max_or_nan(m[i & 3], at(v, i));
+    const float now = max_or_nan(max_or_nan(max_or_nan(m[0], m[1]), max_or_nan(m[2], m[3])), top);
+    float s;
     if (!far(now)) {
-      const float base = now * LOG2E;
-      total *= ex2((top - now) * LOG2E);  // (0 while top is minus infinity; a NaN stays one)
+      total *= ex2((top - now) * LOG2E);  // (0 while top is minus infinity)
+      uint64_t e[16];
+      exp_pairs(v, now, e);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) s[i & 3] += ex2(fmaf(at(v, i), LOG2E, -base));
+      for (int i = 4; i < 16; ++i) e[i & 3] = add2(e[i & 3], e[i]);
+      float lo, hi;
+      split2(add2(add2(e[0], e[1]), add2(e[2], e[3])), &lo, &hi);
+      s = lo + hi;
     } else {
       const float base = now == -INFINITY ? 0.0f : now;  // nothing but minus infinity so far
       total *= ex2((top - base) * LOG2E);
+      s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) s[i & 3] += ex2((at(v, i) - base) * LOG2E);
+      for (int i = 0; i < 32; ++i) s += ex2((at(v, i) - base) * LOG2E);
     }
     top = now;
-    total += (s[0] + s[1]) + (s[2] + s[3]);
+    total += s;
   }
   static __device__ __forceinline__ float at(const uint32_t (&v)[32], int i) { return __uint_as_float(v[i]); }
 };
@@ -424,10 +452,17 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
               if (at < 32u && word >= 0) a.target_logit[row] = pick(now, static_cast<int>(at));
               if (left > 0) sum.add(now, left);
             } else if constexpr (MODE == GRAD) {
-              if (!far(lse)) {
-                const float base = lse * LOG2E;
+              if (!far(lse)) {  // (then no logit is a NaN)
+                uint64_t e[16];
+                exp_pairs(now, lse, e);
+                const uint64_t grad2 = two(grad, grad);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) now[i] = __float_as_uint(grad * ex2(fmaf(__uint_as_float(now[i]), LOG2E, -base)));
+                for (int i = 0; i < 16; ++i) {
+                  float lo, hi;
+                  split2(mul2(e[i], grad2), &lo, &hi);
+                  now[2 * i] = __float_as_uint(lo);
+                  now[2 * i + 1] = __float_as_uint(hi);
+                }
               } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) now[i] = __float_as_uint(grad * ex2((__uint_as_float(now[i]) - lse) * LOG2E));
@@ -510,7 +545,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
       }
       if (MODE == STATS && ok) {
         const int32_t row = item % ext.row_blocks * M_TILE + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
-        const int64_t at = static_cast<int64_t>(row) * (a.slices * COL_GROUPS) + item / ext.row_blocks * COL_GROUPS + group;
+        const int64_t at = static_cast<int64_t>(row) * (ext.slices * COL_GROUPS) + item / ext.row_blocks * COL_GROUPS + group;
         if (row < ext.rows) {
           a.top[at] = sum.top;
           a.total[at] = sum.total;
@@ -551,10 +586,38 @@ __global__ void __launch_bounds__(256) ce_pack_weight_kernel(const uint16_t* __r
 struct MmaPlan {
   int64_t pitch, row_blocks, col_tiles, slices, pairs;
   int64_t piece, splits, dpitch;
-  bool one_piece, compact;
+  bool one_piece, compact, dh_first;
   size_t packed, word, slot, live, counts, weight, target_logit, top, total, dloss, lse, largest, g, dh;
   size_t forward_bytes, backward_bytes;
 };
+
+// How often dh's tiles are cut along the classes, and whether they come before dW's: the launch deals its items to the pairs in
+// turn, and the cut is the one whose busiest pair has the least to do, in blocks of K_TILE plus what an item costs besides.
+int64_t splits_for(int64_t row_blocks, int64_t d_tiles, int64_t dh_k, int64_t dw_tiles, int64_t dw_k, int64_t pairs, bool* dh_first) {
+  constexpr int64_t kItem = 6, kMostSplits = 16;
+  int64_t best = 1, least = INT64_MAX;
+  *dh_first = true;
+  for (int64_t s = 1; s <= kMostSplits && s * 4 <= dh_k + 3; ++s) {
+    const int64_t count[2] = {row_blocks * d_tiles * s, dw_tiles * d_tiles}, cost[2] = {tiles(dh_k, s) + kItem, dw_k + kItem};
+    for (int first = 0; first < 2; ++first) {
+      const int64_t n0 = count[first], n1 = count[1 - first], c0 = cost[first], c1 = cost[1 - first];
+      // pair q gets every pairs-th item from q on; those of the second kind begin where the first kind ended
+      const int64_t r0 = n0 % pairs;
+      int64_t most = 0;
+      for (int64_t q = 0; q < pairs; ++q) {
+        const int64_t turn = (q - r0 + pairs) % pairs;
+        const int64_t mine = (n0 / pairs + (q < r0)) * c0 + (n1 / pairs + (turn < n1 % pairs)) * c1;
+        if (mine > most) most = mine;
+      }
+      if (most < least) {
+        least = most;
+        best = s;
+        *dh_first = first == 0;
+      }
+    }
+  }
+  return best;
+}
 
 // Whether the rows without a valid target are left out of the products.  That takes a launch more, and dh leaves by way of its
 // 32-bit form to be spread over the call's rows: COMPACT_COST.  Below, the products themselves take some 40 us.
@@ -569,32 +632,35 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.row_blocks = tiles(n, M_TILE);
   p.col_tiles = tiles(V, N_TILE);
   p.slices = slices_for(p.row_blocks, p.col_tiles, p.pairs);
-  p.piece = PIECE_BYTES / 2 / (n > 0 ? n : 1) / N_TILE * N_TILE;
-  if (p.piece < N_TILE) p.piece = N_TILE;
-  if (p.piece > p.col_tiles * N_TILE) p.piece = p.col_tiles * N_TILE;
+  // as many column tiles as PIECE_BYTES allow, rounded down to full rounds of the GRAD launch
+  int64_t piece_tiles = PIECE_BYTES / 2 / (n > 0 ? n : 1) / N_TILE;
+  if (piece_tiles < 1) piece_tiles = 1;
+  if (piece_tiles >= p.col_tiles) {
+    piece_tiles = p.col_tiles;
+  } else if (p.row_blocks * piece_tiles >= p.pairs) {
+    const int64_t rounds = p.row_blocks * piece_tiles / p.pairs, full = rounds * p.pairs / p.row_blocks;
+    if (full > 0) piece_tiles = full;
+  }
+  p.piece = piece_tiles * N_TILE;
   p.one_piece = p.piece >= V;
   p.dpitch = up(D, 4);
-  // dh's tiles are cut along the classes until none is longer than half of what each pair has to do
-  const int64_t d_tiles = tiles(D, N_TILE), dh_tiles = p.row_blocks * d_tiles, dh_k = tiles(p.piece, K_TILE);
-  const int64_t dw_k = tiles(n, K_TILE), all = dh_tiles * dh_k + tiles(p.piece, M_TILE) * d_tiles * dw_k;
-  int64_t most = all / p.pairs / 2;
-  if (most < 16) most = 16;
-  p.splits = tiles(dh_k, most);
-  if (p.splits > 32) p.splits = 32;
+  p.splits = splits_for(p.row_blocks, tiles(D, N_TILE), tiles(p.piece, K_TILE), piece_tiles, tiles(n, K_TILE), p.pairs, &p.dh_first);
   p.compact = worth_compacting(n, D, V);
   Layout l;
   p.packed = l.take(n * p.pitch * 2);
   p.word = l.take(n * 4);
   if (p.compact) {
     p.slot = l.take(n * 4);
-    p.live = l.take(4);
+    p.live = l.take(8);
     p.counts = l.take(tiles(n, CE_COUNT_ROWS) * 4);
   }
   if (D % 8 != 0) p.weight = l.take(V * p.pitch * 2);
   const Layout common = l;
   p.target_logit = l.take(n * 4);
-  p.top = l.take(COL_GROUPS * p.slices * n * 4);
-  p.total = l.take(COL_GROUPS * p.slices * n * 4);
+  // (compact: the number of slices follows the number of rows, which is not known here)
+  const int64_t most_slices = !p.compact ? p.slices : p.col_tiles < p.pairs ? p.col_tiles : p.pairs;
+  p.top = l.take(COL_GROUPS * most_slices * n * 4);
+  p.total = l.take(COL_GROUPS * most_slices * n * 4);
   p.forward_bytes = l.bytes;
   l = common;
   p.dloss = l.take(n * 4);
@@ -660,6 +726,9 @@ static CePacked packed_rows(const CeProblem& q, const MmaPlan& p) {
     r.slot = reinterpret_cast<int32_t*>(q.ws + p.slot);
     r.live = reinterpret_cast<int32_t*>(q.ws + p.live);
     r.counts = reinterpret_cast<int32_t*>(q.ws + p.counts);
+    r.block_rows = M_TILE;
+    r.col_tiles = static_cast<int32_t>(p.col_tiles);
+    r.slots = static_cast<int32_t>(p.pairs);
   }
   return r;
 }
@@ -695,7 +764,7 @@ int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) 
   a.total = reinterpret_cast<float*>(q.ws + p.total);
   a.status = q.status;
   if (int rc = launch<STATS>(a, p.pairs, q.dtype, s)) return rc;
-  return ce_join(q, a.top, a.total, COL_GROUPS * p.slices, a.word, r.slot, a.target_logit, loss, lse, s);
+  return ce_join(q, a.top, a.total, COL_GROUPS, p.slices, r.live, a.word, r.slot, a.target_logit, loss, lse, s);
 }
 
 int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, void* dhidden, void* dweight, cudaStream_t s) {
@@ -712,7 +781,6 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
   float* dh = reinterpret_cast<float*>(q.ws + p.dh);
   // results whose rows begin at 16-byte boundaries leave by TMA
   const bool dh_direct = p.one_piece && p.splits == 1 && !p.compact, even = q.D % 8 == 0;
-  const int32_t d_tiles = static_cast<int32_t>(tiles(q.D, N_TILE));
   for (int64_t v0 = 0; v0 < q.V; v0 += p.piece) {
     const int64_t width = q.V - v0 < p.piece ? q.V - v0 : p.piece;
     const uint16_t* wp = w.p + v0 * w.stride;
@@ -736,50 +804,54 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     if (int rc = launch<GRAD>(a, p.pairs, q.dtype, s)) return rc;
 
     MmaArgs m{};
-    int parts = 0;
+    // half as wide tiles where that gives more pairs something to do (1 024 rows of 256 against 172 classes: 5 tiles of 256)
+    const int64_t wide = tiles(q.D, N_TILE) * (p.row_blocks * p.splits + tiles(width, M_TILE));
+    const int32_t n_step = 2 * wide <= p.pairs ? N_TILE / 2 : N_TILE, d_tiles = static_cast<int32_t>(tiles(q.D, n_step));
+    const int both = dhidden != nullptr && dweight != nullptr, at_dh = both && !p.dh_first, at_dw = both && p.dh_first;
+    int64_t dh_items = 0, dw_items = 0;
     if (dhidden != nullptr) {
-      Part& t = m.part[parts];
+      Part& t = m.part[at_dh];
       t.a_mn = 0;
       t.n_tiles = d_tiles;
+      t.n_step = n_step;
       t.k_blocks = static_cast<int32_t>(tiles(width, K_TILE));
       // (the first piece has work for every split; a narrow last one adds to as many as it has)
       t.splits = static_cast<int32_t>(p.splits < t.k_blocks ? p.splits : t.k_blocks);
-      t.items = static_cast<int32_t>(p.row_blocks * d_tiles * t.splits);
+      dh_items = p.row_blocks * d_tiles * t.splits;
       t.n_total = static_cast<int32_t>(q.D);
       t.m_total = static_cast<int32_t>(q.n);
       t.split_rows = p.row_blocks * M_TILE;
       t.out_kind = !dh_direct ? (v0 > 0 ? OUT_F32_ADD : OUT_F32_STORE) : even && aligned_to(dhidden, 16) ? OUT_TYPED : OUT_TYPED_ODD;
       t.odd = dhidden;
-      if (int rc = make_map(&m.a[parts], g, q.dtype, width, q.n, p.piece, K_TILE, M_CTA)) return rc;
-      if (int rc = make_map(&m.b[parts], wp, q.dtype, q.D, width, w.stride, 64, K_TILE)) return rc;
+      if (int rc = make_map(&m.a[at_dh], g, q.dtype, width, q.n, p.piece, K_TILE, M_CTA)) return rc;
+      if (int rc = make_map(&m.b[at_dh], wp, q.dtype, q.D, width, w.stride, 64, K_TILE)) return rc;
       if (t.out_kind == OUT_TYPED) {
-        if (int rc = make_map(&m.out[parts], dhidden, q.dtype, q.D, q.n, q.D, 64, 32)) return rc;
+        if (int rc = make_map(&m.out[at_dh], dhidden, q.dtype, q.D, q.n, q.D, 64, 32)) return rc;
       } else if (t.out_kind != OUT_TYPED_ODD) {
-        if (int rc = make_map(&m.out[parts], dh, DGS_F32, q.D, p.splits * t.split_rows, p.dpitch, 32, 32)) return rc;
+        if (int rc = make_map(&m.out[at_dh], dh, DGS_F32, q.D, p.splits * t.split_rows, p.dpitch, 32, 32)) return rc;
       }
-      ++parts;
     }
     if (dweight != nullptr) {
-      Part& t = m.part[parts];
+      Part& t = m.part[at_dw];
       t.a_mn = 1;
       t.n_tiles = d_tiles;
+      t.n_step = n_step;
       t.splits = 1;
       t.k_blocks = static_cast<int32_t>(tiles(q.n, K_TILE));
-      t.items = static_cast<int32_t>(tiles(width, M_TILE)) * d_tiles;
+      dw_items = tiles(width, M_TILE) * d_tiles;
       t.n_total = static_cast<int32_t>(q.D);
       t.m_total = static_cast<int32_t>(width);
       uint16_t* to = static_cast<uint16_t*>(dweight) + v0 * q.D;
       t.out_kind = even && aligned_to(dweight, 16) ? OUT_TYPED : OUT_TYPED_ODD;
       t.odd = to;
-      if (int rc = make_map(&m.a[parts], g, q.dtype, width, q.n, p.piece, 64, K_TILE)) return rc;
-      if (int rc = make_map(&m.b[parts], packed, q.dtype, q.D, q.n, p.pitch, 64, K_TILE)) return rc;
+      if (int rc = make_map(&m.a[at_dw], g, q.dtype, width, q.n, p.piece, 64, K_TILE)) return rc;
+      if (int rc = make_map(&m.b[at_dw], packed, q.dtype, q.D, q.n, p.pitch, 64, K_TILE)) return rc;
       if (t.out_kind == OUT_TYPED) {
-        if (int rc = make_map(&m.out[parts], to, q.dtype, q.D, width, q.D, 64, 32)) return rc;
+        if (int rc = make_map(&m.out[at_dw], to, q.dtype, q.D, width, q.D, 64, 32)) return rc;
       }
-      ++parts;
     }
-    m.parts = parts;
-    m.items = m.part[0].items + m.part[1].items;
+    m.parts = 1 + both;
+    m.items = static_cast<int32_t>(dh_items + dw_items);
     m.n = q.n;
     m.live = r.live;
     m.largest = r.largest;
