@@ -132,10 +132,28 @@ __global__ void __launch_bounds__(CE_THREADS) ce_pack_kernel(const __grid_consta
     const T* from = static_cast<const T*>(a.hidden) + row * a.stride;
     T* dst = static_cast<T*>(a.to.rows) + to * a.pitch;
     if (a.vectors) {
-      for (int j = lane * VEC; j < a.pitch; j += 32 * VEC)
-        *reinterpret_cast<uint4*>(dst + j) = word >= 0 ? *reinterpret_cast<const uint4*>(from + j) : uint4{0, 0, 0, 0};
+      for (int j0 = lane * VEC; j0 < a.pitch; j0 += 4 * 32 * VEC) {
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int j = j0 + u * 32 * VEC;
+          v[u] = word >= 0 && j < a.pitch ? *reinterpret_cast<const uint4*>(from + j) : uint4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int j = j0 + u * 32 * VEC;
+          if (j < a.pitch) *reinterpret_cast<uint4*>(dst + j) = v[u];
+        }
+      }
     } else {
-      for (int j = lane; j < a.pitch; j += 32) dst[j] = word >= 0 && j < a.D ? from[j] : from_float<T>(0.0f);
+      for (int j0 = lane; j0 < a.pitch; j0 += 8 * 32) {
+        T v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = word >= 0 && j0 + u * 32 < a.D ? from[j0 + u * 32] : from_float<T>(0.0f);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (j0 + u * 32 < a.pitch) dst[j0 + u * 32] = v[u];
+      }
     }
   }
   if (a.to.largest != nullptr) {
@@ -352,13 +370,27 @@ __global__ void __launch_bounds__(CE_THREADS) ce_join_kernel(const __grid_consta
   }
   const int64_t parts = a.groups * (a.live != nullptr ? a.live[1] : a.slices);
   const float *top = a.top + c * parts, *total = a.total + c * parts;
-  float m = -INFINITY;
-  for (int64_t p = lane; p < parts; p += 32) m = fmaxf(m, top[p]);
+  float m = -INFINITY, s = 0.0f;
+  for (int64_t p0 = lane; p0 < parts; p0 += 128) {
+    float t[4], e[4];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
-  const float base = m == -INFINITY ? 0.0f : m;
-  float s = 0.0f;
-  for (int64_t p = lane; p < parts; p += 32) s += total[p] * expf(top[p] - base);
+    for (int k = 0; k < 4; ++k) {
+      const bool in = p0 + 32 * k < parts;
+      t[k] = in ? top[p0 + 32 * k] : -INFINITY;
+      e[k] = in ? total[p0 + 32 * k] : 0.0f;
+    }
+    const float now = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), m);
+    const float base = now == -INFINITY ? 0.0f : now;
+    s *= expf(m - base);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s += e[k] * expf(t[k] - base);
+    m = now;
+  }
+  float all = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(FULL_MASK, all, o));
+  const float base = all == -INFINITY ? 0.0f : all;
+  s *= expf(m - base);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL_MASK, s, o);
   if (lane == 0) {
@@ -433,7 +465,8 @@ __global__ void __launch_bounds__(CE_THREADS, 2) ce_product_kernel(const Operand
 template <typename T>
 __global__ void __launch_bounds__(CE_THREADS) ce_sum_kernel(const float* __restrict__ parts, const int64_t splits, const int64_t split_elems,
                                                             const int64_t n, const int D, const int pitch,
-                                                            const int32_t* __restrict__ slot, const bool fours, T* __restrict__ out) {
+                                                            const int32_t* __restrict__ slot, const bool vectors, const bool fours,
+                                                            T* __restrict__ out) {
   pdl_enter();
   const int lane = threadIdx.x & 31;
   for (int64_t row = blockIdx.x * static_cast<int64_t>(CE_THREADS / 32) + (threadIdx.x >> 5); row < n;
@@ -441,25 +474,28 @@ __global__ void __launch_bounds__(CE_THREADS) ce_sum_kernel(const float* __restr
     const int64_t c = slot != nullptr ? slot[row] : row;
     const float* p = parts + c * pitch;
     T* to = out + row * D;
-    if (fours) {
-      for (int j = lane * 4; j < D; j += 128) {
-        float v[4] = {};
-        if (c >= 0) {
-          for (int64_t k = 0; k < splits; ++k) {
-            float t[4];
+    for (int j = lane * 4; j < D; j += 128) {
+      float v[4] = {};
+      if (c >= 0) {
+#pragma unroll 4
+        for (int64_t k = 0; k < splits; ++k) {
+          float t[4];
+          if (vectors) {
             load_vec<float, 4>(p + k * split_elems + j, t);
+          } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += t[i];
+            for (int i = 0; i < 4; ++i) t[i] = j + i < D ? p[k * split_elems + j + i] : 0.0f;
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] += t[i];
         }
-        store_vec<T, 4>(to + j, v);
       }
-    } else {
-      for (int j = lane; j < D; j += 32) {
-        float v = 0.0f;
-        if (c >= 0)
-          for (int64_t k = 0; k < splits; ++k) v += p[k * split_elems + j];
-        to[j] = from_float<T>(v);
+      if (fours) {
+        store_vec<T, 4>(to + j, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j + i < D) to[j + i] = from_float<T>(v[i]);
       }
     }
   }
@@ -592,15 +628,15 @@ int ce_sum(const float* parts, int64_t splits, int64_t n, int64_t D, int64_t row
   const int64_t need = tiles(n, CE_THREADS / 32), most = static_cast<int64_t>(sm_count()) * 16;
   const dim3 grid(static_cast<unsigned>(need < most ? need : most));
   const int d = static_cast<int>(D), pt = static_cast<int>(pitch);
-  const bool fours = D % 4 == 0 && pitch % 4 == 0 && aligned_to(out, 16);
+  const bool vectors = pitch % 4 == 0, fours = vectors && D % 4 == 0 && aligned_to(out, 16);
   if (dtype == DGS_F32)
-    DGS_CUDA_TRY(launch_training(ce_sum_kernel<float>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, slot, fours,
+    DGS_CUDA_TRY(launch_training(ce_sum_kernel<float>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, slot, vectors, fours,
                                  static_cast<float*>(out)));
   else if (dtype == DGS_BF16)
-    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__nv_bfloat16>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, slot, fours,
+    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__nv_bfloat16>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, slot, vectors, fours,
                                  static_cast<__nv_bfloat16*>(out)));
   else
-    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__half>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, slot, fours,
+    DGS_CUDA_TRY(launch_training(ce_sum_kernel<__half>, grid, CE_THREADS, 0, s, parts, splits, rows * pitch, n, d, pt, slot, vectors, fours,
                                  static_cast<__half*>(out)));
   return DGS_OK;
 }

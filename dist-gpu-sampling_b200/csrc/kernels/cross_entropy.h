@@ -34,9 +34,18 @@ struct Layout {
 // Slices of `cols` column tiles for `rows` row blocks on `slots` CTAs that run at once: the cut with the fewest tiles in
 // the busiest slot.
 inline int64_t slices_for(int64_t rows, int64_t cols, int64_t slots) {
-  int64_t best = 1, least = tiles(rows, slots) * cols;
-  for (int64_t s = 2; s <= cols && s <= slots; ++s) {
-    const int64_t cost = tiles(rows * s, slots) * tiles(cols, s);
+  // (in 32 bits and with one division a candidate: this is worked out on every call)
+  if (rows >= (int64_t(1) << 20)) return 1;
+  const uint32_t r = static_cast<uint32_t>(rows), c = static_cast<uint32_t>(cols), most = static_cast<uint32_t>(cols < slots ? cols : slots);
+  uint32_t best = 1, rounds = 0, room = 0;  // rounds = tiles(r * s, slots), room = rounds * slots - r * s
+  uint64_t least = UINT64_MAX;
+  for (uint32_t s = 1; s <= most; ++s) {
+    while (room < r) {
+      room += static_cast<uint32_t>(slots);
+      ++rounds;
+    }
+    room -= r;
+    const uint64_t cost = static_cast<uint64_t>(rounds) * ((c + s - 1) / s);
     if (cost < least) {
       least = cost;
       best = s;

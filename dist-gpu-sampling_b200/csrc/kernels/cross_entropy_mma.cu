@@ -571,13 +571,27 @@ __global__ void __launch_bounds__(256) ce_pack_weight_kernel(const uint16_t* __r
                                                              const int D, const int pitch, uint16_t* __restrict__ packed) {
   pdl_enter();
   const int lane = threadIdx.x & 31;
-  for (int64_t row = blockIdx.x * int64_t(8) + (threadIdx.x >> 5); row < V; row += gridDim.x * int64_t(8)) {
-    const uint16_t* from = weight + row * stride;
-    uint32_t* to = reinterpret_cast<uint32_t*>(packed + row * pitch);
-#pragma unroll 4
-    for (int j = lane * 2; j < pitch; j += 64) {
-      const uint32_t lo = j < D ? from[j] : 0u, hi = j + 1 < D ? from[j + 1] : 0u;
-      to[j >> 1] = lo | (hi << 16);
+  constexpr int U = 4;  // words of a row under way a lane, for two rows
+  for (int64_t row0 = (blockIdx.x * int64_t(8) + (threadIdx.x >> 5)) * 2; row0 < V; row0 += gridDim.x * int64_t(16)) {
+    for (int j0 = lane * 2; j0 < pitch; j0 += 64 * U) {
+      uint16_t v[2][U][2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int j = j0 + u * 64 + h;
+            v[r][u][h] = row0 + r < V && j < D ? weight[(row0 + r) * stride + j] : uint16_t(0);
+          }
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int j = j0 + u * 64;
+          if (row0 + r < V && j < pitch)
+            *reinterpret_cast<uint32_t*>(packed + (row0 + r) * pitch + j) = v[r][u][0] | (static_cast<uint32_t>(v[r][u][1]) << 16);
+        }
     }
   }
 }
@@ -601,14 +615,11 @@ int64_t splits_for(int64_t row_blocks, int64_t d_tiles, int64_t dh_k, int64_t dw
     const int64_t count[2] = {row_blocks * d_tiles * s, dw_tiles * d_tiles}, cost[2] = {tiles(dh_k, s) + kItem, dw_k + kItem};
     for (int first = 0; first < 2; ++first) {
       const int64_t n0 = count[first], n1 = count[1 - first], c0 = cost[first], c1 = cost[1 - first];
-      // pair q gets every pairs-th item from q on; those of the second kind begin where the first kind ended
-      const int64_t r0 = n0 % pairs;
-      int64_t most = 0;
-      for (int64_t q = 0; q < pairs; ++q) {
-        const int64_t turn = (q - r0 + pairs) % pairs;
-        const int64_t mine = (n0 / pairs + (q < r0)) * c0 + (n1 / pairs + (turn < n1 % pairs)) * c1;
-        if (mine > most) most = mine;
-      }
+      // the first r0 pairs have one item of the first kind more than the others; those of the second kind begin where these ended,
+      // and r1 pairs, the next ones round the circle, have one more of them
+      const int64_t r0 = n0 % pairs, r1 = n1 % pairs;
+      const int64_t more = r0 + r1 > pairs ? c0 + c1 : r0 > 0 && (r1 == 0 || c0 > c1) ? c0 : r1 > 0 ? c1 : 0;
+      const int64_t most = n0 / pairs * c0 + n1 / pairs * c1 + more;
       if (most < least) {
         least = most;
         best = s;
@@ -704,7 +715,7 @@ int fetchable_weight(const CeProblem& q, const MmaPlan& p, Weight* w, cudaStream
   DGS_REQUIRE(q.D % 8 != 0, DGS_ERR_INVALID, "linear_cross_entropy: rows of %lld 16-bit elements must begin at 16-byte boundaries",
               static_cast<long long>(q.D));
   uint16_t* packed = reinterpret_cast<uint16_t*>(q.ws + p.weight);
-  const int64_t need = tiles(q.V, 8), most = static_cast<int64_t>(sm_count()) * 8;
+  const int64_t need = tiles(q.V, 16), most = static_cast<int64_t>(sm_count()) * 8;
   DGS_CUDA_TRY(launch_training(ce_pack_weight_kernel, dim3(static_cast<unsigned>(need < most ? need : most)), 256, 0, s, w->p,
                                q.weight_stride, q.V, static_cast<int>(q.D), static_cast<int>(p.pitch), packed));
   *w = Weight{packed, p.pitch};
