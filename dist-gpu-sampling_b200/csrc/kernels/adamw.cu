@@ -14,7 +14,7 @@
 //
 // The arithmetic is 32-bit, operation by operation as written above: no contraction to fused multiply-add, IEEE division
 // and square root.  A moment that falls between two codes is then rounded the same way wherever the formula is evaluated
-// in 32 bits; the kernel waits for HBM, so the longer instructions are hidden.
+// in 32 bits.
 #include <cmath>
 #include <type_traits>
 
@@ -58,24 +58,61 @@ struct Moments8 {
   float* v_scale;
 };
 
-__device__ __forceinline__ float update(float p, float g, float& m, float& v, const Scalars& k) {
+// the new parameter; `root` receives that of the second moment
+__device__ __forceinline__ float update(float p, float g, float& m, float& v, float& root, const Scalars& k) {
   m = __fadd_rn(__fmul_rn(m, k.b1), __fmul_rn(g, k.c1));
   v = __fadd_rn(__fmul_rn(v, k.b2), __fmul_rn(__fmul_rn(g, g), k.c2));
-  const float under = __fadd_rn(__fmul_rn(__fsqrt_rn(v), k.root2), k.eps);
+  root = __fsqrt_rn(v);
+  const float under = __fadd_rn(__fmul_rn(root, k.root2), k.eps);
   return __fsub_rn(__fmul_rn(p, k.keep), __fmul_rn(__fdiv_rn(m, under), k.step));
 }
 
 // the largest of the warp's non-negative values; a NaN counts as larger than any (its bits are)
 __device__ __forceinline__ float warp_max_bits(uint32_t bits) { return __uint_as_float(__reduce_max_sync(FULL_MASK, bits)); }
 
-__device__ __forceinline__ float first_moment(int c, float scale) {
-  const float u = __fmul_rn(static_cast<float>(c), 1.0f / 127.0f);
+// Codes and values.  A byte becomes a float by standing in the low bits of 2^23 (8388608), and a float its nearest whole number
+// there by adding 1.5 * 2^23 (12582912): the units that convert take 16 values a clock and SM, which square roots and divisions
+// need here.
+constexpr float kByte = 8388608.0f, kRound = 12582912.0f;
+template <bool SIGNED>
+__device__ __forceinline__ float code_value(uint32_t word, int byte) {  // byte 0..3 of a word of codes (known when compiled)
+  const uint32_t bits = __byte_perm(SIGNED ? word ^ 0x80808080u : word, 0x4B000000u, 0x7440u + byte);
+  return __fsub_rn(__uint_as_float(bits), SIGNED ? kByte + 128.0f : kByte);
+}
+__device__ __forceinline__ float first_moment(float c, float scale) {
+  const float u = __fmul_rn(c, 1.0f / 127.0f);
   return __fmul_rn(__fmul_rn(u, fabsf(u)), scale);
 }
-__device__ __forceinline__ float second_moment(int c, float scale) {
-  const float u = __fmul_rn(static_cast<float>(c), 1.0f / 255.0f);
+__device__ __forceinline__ float second_moment(float c, float scale) {
+  const float u = __fmul_rn(c, 1.0f / 255.0f);
   const float r = __fmul_rn(__fmul_rn(u, u), scale);
   return __fmul_rn(r, r);
+}
+
+__device__ __forceinline__ float sqrt_near(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// The code of x is rint(steps * sqrt(x / scale)), 0 <= x <= scale, each operation rounded to nearest.
+__device__ __forceinline__ float exact_code(float x, float scale, float steps) {
+  // (a scale of zero, or one that is no number, leaves the code zero)
+  return scale > 0.0f ? rintf(__fmul_rn(__fsqrt_rn(__fdiv_rn(x, scale)), steps)) : 0.0f;
+}
+// The same without the IEEE division and root: the value before rint is within steps * 4.3e-7 of the one above (six roundings of
+// 2^-24, two of them halved by the root, and sqrt.approx with 2^-23), so it gives the same code unless it stands that near to a
+// half.  `doubt` collects how near to a half the values come; `inverse` = 1 / scale.
+__device__ __forceinline__ float quick_code(float x, float inverse, float steps, float& doubt) {
+  const float value = __fmul_rn(sqrt_near(__fmul_rn(x, inverse)), steps);
+  const float whole = __fsub_rn(__fadd_rn(value, kRound), kRound);
+  doubt = fmaxf(doubt, fabsf(__fsub_rn(value, whole)) + steps * 4.3e-7f);
+  return whole;
+}
+// the low bytes of four whole numbers
+__device__ __forceinline__ uint32_t bytes_of(float a, float b, float c, float d) {
+  const uint32_t ab = __byte_perm(__float_as_uint(a + kRound), __float_as_uint(b + kRound), 0x0040);
+  const uint32_t cd = __byte_perm(__float_as_uint(c + kRound), __float_as_uint(d + kRound), 0x0040);
+  return __byte_perm(ab, cd, 0x5410);
 }
 
 template <int N, typename Moments>
@@ -93,11 +130,11 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
     }
     const Entry& e = list.e[lo];
     const int64_t i = (chunk - e.first_chunk) * AW_CHUNK + static_cast<int64_t>(threadIdx.x) * AW_VALUES;
-    const int64_t left = e.n - i;  // elements of the tensor from this thread's first on
     // whole warps leave together: a warp that has any element takes part with all its lanes (the scales of a block)
     if (e.n - (i - static_cast<int64_t>(threadIdx.x & 31) * AW_VALUES) <= 0) continue;
-    float p[AW_VALUES], g[AW_VALUES], m[AW_VALUES], v[AW_VALUES];
-    const bool full = e.whole && left >= AW_VALUES;
+    const int left = e.n - i >= AW_VALUES ? AW_VALUES : e.n > i ? static_cast<int>(e.n - i) : 0;  // this thread's elements
+    float p[AW_VALUES], g[AW_VALUES], m[AW_VALUES], v[AW_VALUES], root[AW_VALUES];
+    const bool full = e.whole && left == AW_VALUES;
     if (full) {
       load_vec_as_float<AW_VALUES>(e.param, e.param_dtype, i, p);
       load_vec_as_float<AW_VALUES>(e.grad, e.grad_dtype, i, g);
@@ -110,23 +147,20 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
     }
     const int64_t at = e.at + i;
     if constexpr (kEight) {
-      Vec<int8_t, AW_VALUES> mc;
-      Vec<uint8_t, AW_VALUES> vc;
       // a slot is whole blocks, so all eight codes are there; those beyond the tensor's end count as zero
-      mc = *reinterpret_cast<const Vec<int8_t, AW_VALUES>*>(mo.m + at);
-      vc = *reinterpret_cast<const Vec<uint8_t, AW_VALUES>*>(mo.v + at);
+      const uint2 mc = *reinterpret_cast<const uint2*>(mo.m + at), vc = *reinterpret_cast<const uint2*>(mo.v + at);
       const float ma = mo.m_scale[at / AW_BLOCK], va = mo.v_scale[at / AW_BLOCK];
 #pragma unroll
       for (int j = 0; j < AW_VALUES; ++j) {
-        m[j] = j < left ? first_moment(mc.v[j], ma) : 0.0f;
-        v[j] = j < left ? second_moment(vc.v[j], va) : 0.0f;
+        m[j] = first_moment(code_value<true>(j < 4 ? mc.x : mc.y, j & 3), ma);
+        v[j] = second_moment(code_value<false>(j < 4 ? vc.x : vc.y, j & 3), va);
       }
     } else {
       load_vec<float, AW_VALUES>(mo.m + at, m);
       load_vec<float, AW_VALUES>(mo.v + at, v);
     }
 #pragma unroll
-    for (int j = 0; j < AW_VALUES; ++j) p[j] = update(p[j], g[j], m[j], v[j], k);
+    for (int j = 0; j < AW_VALUES; ++j) p[j] = update(p[j], g[j], m[j], v[j], root[j], k);
     if (full) {
       store_vec_from_float<AW_VALUES>(e.param, e.param_dtype, i, p);
       if (e.copy != nullptr) store_vec_from_float<AW_VALUES>(e.copy, e.copy_dtype, i, p);
@@ -140,30 +174,40 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
       }
     }
     if constexpr (kEight) {
+      if (left < AW_VALUES) {
+#pragma unroll
+        for (int j = 0; j < AW_VALUES; ++j)
+          if (j >= left) m[j] = root[j] = 0.0f;
+      }
       uint32_t mb = 0, vb = 0;
 #pragma unroll
       for (int j = 0; j < AW_VALUES; ++j) {
-        if (j >= left) m[j] = v[j] = 0.0f;
-        v[j] = __fsqrt_rn(v[j]);
         mb = max(mb, __float_as_uint(fabsf(m[j])));
-        vb = max(vb, __float_as_uint(fabsf(v[j])));
+        vb = max(vb, __float_as_uint(root[j]));
       }
       const float ma = warp_max_bits(mb), va = warp_max_bits(vb);
-      Vec<int8_t, AW_VALUES> mc;
-      Vec<uint8_t, AW_VALUES> vc;
+      const bool plain = ma >= 1e-30f && ma <= 1e30f && va >= 1e-30f && va <= 1e30f;  // scales that have an inverse
+      const float mi = __fdiv_rn(1.0f, ma), vi = __fdiv_rn(1.0f, va);
+      float mc[AW_VALUES], vc[AW_VALUES], doubt = 0.0f;
 #pragma unroll
       for (int j = 0; j < AW_VALUES; ++j) {
-        // a scale of zero, or one that is no number, leaves the code zero
-        const float tm = ma > 0.0f ? __fsqrt_rn(__fdiv_rn(fabsf(m[j]), ma)) : 0.0f;
-        const float tv = va > 0.0f ? __fsqrt_rn(__fdiv_rn(v[j], va)) : 0.0f;
-        const int cm = __float2int_rn(__fmul_rn(tm, 127.0f));
-        int cv = __float2int_rn(__fmul_rn(tv, 255.0f));
-        if (v[j] > 0.0f && cv < 1) cv = 1;
-        mc.v[j] = static_cast<int8_t>(m[j] < 0.0f ? -cm : cm);
-        vc.v[j] = static_cast<uint8_t>(cv);
+        mc[j] = quick_code(fabsf(m[j]), mi, 127.0f, doubt);
+        vc[j] = quick_code(root[j], vi, 255.0f, doubt);
       }
-      *reinterpret_cast<Vec<int8_t, AW_VALUES>*>(mo.m + at) = mc;
-      *reinterpret_cast<Vec<uint8_t, AW_VALUES>*>(mo.v + at) = vc;
+      if (!plain || doubt >= 0.5f) {  // 7 % of the warps
+#pragma unroll
+        for (int j = 0; j < AW_VALUES; ++j) {
+          mc[j] = exact_code(fabsf(m[j]), ma, 127.0f);
+          vc[j] = exact_code(root[j], va, 255.0f);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < AW_VALUES; ++j) {
+        mc[j] = copysignf(mc[j], m[j]);
+        if (root[j] > 0.0f) vc[j] = fmaxf(vc[j], 1.0f);
+      }
+      *reinterpret_cast<uint2*>(mo.m + at) = uint2{bytes_of(mc[0], mc[1], mc[2], mc[3]), bytes_of(mc[4], mc[5], mc[6], mc[7])};
+      *reinterpret_cast<uint2*>(mo.v + at) = uint2{bytes_of(vc[0], vc[1], vc[2], vc[3]), bytes_of(vc[4], vc[5], vc[6], vc[7])};
       if ((threadIdx.x & 31) == 0) {
         mo.m_scale[at / AW_BLOCK] = ma;
         mo.v_scale[at / AW_BLOCK] = va;
@@ -185,19 +229,31 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
   }
 }
 
-template <typename Code>
-__global__ void __launch_bounds__(AW_THREADS) adamw_values_kernel(const Code* __restrict__ codes, const float* __restrict__ scales,
-                                                                  const int64_t n, float* __restrict__ out) {
+// Four codes a lane at a time, so that a warp's stores lie side by side, and four such groups under way.
+template <bool SECOND>
+__global__ void __launch_bounds__(AW_THREADS) adamw_values_kernel(const uint32_t* __restrict__ codes, const float* __restrict__ scales,
+                                                                  const int64_t words, float4* __restrict__ out) {
+  constexpr int U = 4;
   pdl_enter();
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * AW_THREADS + threadIdx.x) * AW_VALUES; i < n;
-       i += static_cast<int64_t>(gridDim.x) * AW_CHUNK) {
-    const Vec<Code, AW_VALUES> c = *reinterpret_cast<const Vec<Code, AW_VALUES>*>(codes + i);
-    const float scale = scales[i / AW_BLOCK];
-    float v[AW_VALUES];
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * (AW_THREADS * U) + threadIdx.x; i0 < words;
+       i0 += static_cast<int64_t>(gridDim.x) * (AW_THREADS * U)) {
+    uint32_t c[U];
+    float scale[U];
 #pragma unroll
-    for (int j = 0; j < AW_VALUES; ++j)
-      v[j] = std::is_signed<Code>::value ? first_moment(c.v[j], scale) : second_moment(c.v[j], scale);
-    store_vec<float, AW_VALUES>(out + i, v);
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + u * AW_THREADS;
+      c[u] = i < words ? codes[i] : 0u;
+      scale[u] = i < words ? scales[i / (AW_BLOCK / 4)] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + u * AW_THREADS;
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = SECOND ? second_moment(code_value<false>(c[u], j), scale[u]) : first_moment(code_value<true>(c[u], j), scale[u]);
+      if (i < words) out[i] = float4{v[0], v[1], v[2], v[3]};
+    }
   }
 }
 
@@ -297,12 +353,10 @@ extern "C" int dgs_adamw_state_values(const void* codes, int32_t second, const f
   if (n == 0) return DGS_OK;
   DGS_REQUIRE(codes != nullptr && scales != nullptr && out != nullptr && aligned_to(codes, 8) && aligned_to(out, 16), DGS_ERR_INVALID,
               "adamw_state_values: null or unaligned argument");
-  const int64_t need = (n + AW_CHUNK - 1) / AW_CHUNK, most = static_cast<int64_t>(sm_count()) * 8;
+  const int64_t words = n / 4, need = (words + AW_THREADS * 4 - 1) / (AW_THREADS * 4), most = static_cast<int64_t>(sm_count()) * 8;
   const dim3 grid(static_cast<unsigned>(need < most ? need : most));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (second != 0)
-    DGS_CUDA_TRY(launch_training(adamw_values_kernel<uint8_t>, grid, AW_THREADS, 0, s, static_cast<const uint8_t*>(codes), scales, n, out));
-  else
-    DGS_CUDA_TRY(launch_training(adamw_values_kernel<int8_t>, grid, AW_THREADS, 0, s, static_cast<const int8_t*>(codes), scales, n, out));
+  DGS_CUDA_TRY(launch_training(second != 0 ? adamw_values_kernel<true> : adamw_values_kernel<false>, grid, AW_THREADS, 0, s,
+                               static_cast<const uint32_t*>(codes), scales, words, reinterpret_cast<float4*>(out)));
   return DGS_OK;
 }
