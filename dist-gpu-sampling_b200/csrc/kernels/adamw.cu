@@ -79,14 +79,19 @@ __device__ __forceinline__ float code_value(uint32_t word, int byte) {  // byte 
   const uint32_t bits = __byte_perm(SIGNED ? word ^ 0x80808080u : word, 0x4B000000u, 0x7440u + byte);
   return __fsub_rn(__uint_as_float(bits), SIGNED ? kByte + 128.0f : kByte);
 }
-__device__ __forceinline__ float first_moment(float c, float scale) {
-  const float u = __fmul_rn(c, 1.0f / 127.0f);
-  return __fmul_rn(__fmul_rn(u, fabsf(u)), scale);
+// Two at a time where nothing but multiplications follow one another (a packed addition behind a packed multiplication may become
+// one operation with one rounding).
+__device__ __forceinline__ uint64_t both(float v) { return two(v, v); }
+__device__ __forceinline__ uint64_t abs2(uint64_t v) { return v & 0x7fffffff7fffffffull; }
+// of bytes `byte` and byte + 1
+__device__ __forceinline__ void first_moments(uint32_t word, int byte, float scale, float* m0, float* m1) {
+  const uint64_t u = mul2(two(code_value<true>(word, byte), code_value<true>(word, byte + 1)), both(1.0f / 127.0f));
+  split2(mul2(mul2(u, abs2(u)), both(scale)), m0, m1);
 }
-__device__ __forceinline__ float second_moment(float c, float scale) {
-  const float u = __fmul_rn(c, 1.0f / 255.0f);
-  const float r = __fmul_rn(__fmul_rn(u, u), scale);
-  return __fmul_rn(r, r);
+__device__ __forceinline__ void second_moments(uint32_t word, int byte, float scale, float* v0, float* v1) {
+  const uint64_t u = mul2(two(code_value<false>(word, byte), code_value<false>(word, byte + 1)), both(1.0f / 255.0f));
+  const uint64_t r = mul2(mul2(u, u), both(scale));
+  split2(mul2(r, r), v0, v1);
 }
 
 __device__ __forceinline__ float sqrt_near(float x) {
@@ -99,14 +104,17 @@ __device__ __forceinline__ float exact_code(float x, float scale, float steps) {
   // (a scale of zero, or one that is no number, leaves the code zero)
   return scale > 0.0f ? rintf(__fmul_rn(__fsqrt_rn(__fdiv_rn(x, scale)), steps)) : 0.0f;
 }
-// The same without the IEEE division and root: the value before rint is within steps * 4.3e-7 of the one above (six roundings of
-// 2^-24, two of them halved by the root, and sqrt.approx with 2^-23), so it gives the same code unless it stands that near to a
-// half.  `doubt` collects how near to a half the values come; `inverse` = 1 / scale.
-__device__ __forceinline__ float quick_code(float x, float inverse, float steps, float& doubt) {
-  const float value = __fmul_rn(sqrt_near(__fmul_rn(x, inverse)), steps);
-  const float whole = __fsub_rn(__fadd_rn(value, kRound), kRound);
-  doubt = fmaxf(doubt, fabsf(__fsub_rn(value, whole)) + steps * 4.3e-7f);
-  return whole;
+// The same for two without the IEEE division and root: the values before rint are within steps * 4.3e-7 of those above (six
+// roundings of 2^-24, two of them halved by the root, and sqrt.approx with 2^-23), so the codes are the same unless one stands that
+// near to a half.  `far` collects how far the values are from their codes; `inverse` = 1 / scale.
+__device__ __forceinline__ void quick_codes(uint64_t x, float inverse, float steps, float& far, float* c0, float* c1) {
+  float a, b;
+  split2(mul2(x, both(inverse)), &a, &b);
+  const uint64_t value = mul2(two(sqrt_near(a), sqrt_near(b)), both(steps));
+  const uint64_t whole = add2(add2(value, both(kRound)), both(-kRound));
+  split2(fma2(whole, both(-1.0f), value), &a, &b);
+  far = fmaxf(far, fmaxf(fabsf(a), fabsf(b)));
+  split2(whole, c0, c1);
 }
 // the low bytes of four whole numbers
 __device__ __forceinline__ uint32_t bytes_of(float a, float b, float c, float d) {
@@ -151,9 +159,9 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
       const uint2 mc = *reinterpret_cast<const uint2*>(mo.m + at), vc = *reinterpret_cast<const uint2*>(mo.v + at);
       const float ma = mo.m_scale[at / AW_BLOCK], va = mo.v_scale[at / AW_BLOCK];
 #pragma unroll
-      for (int j = 0; j < AW_VALUES; ++j) {
-        m[j] = first_moment(code_value<true>(j < 4 ? mc.x : mc.y, j & 3), ma);
-        v[j] = second_moment(code_value<false>(j < 4 ? vc.x : vc.y, j & 3), va);
+      for (int j = 0; j < AW_VALUES; j += 2) {
+        first_moments(j < 4 ? mc.x : mc.y, j & 3, ma, &m[j], &m[j + 1]);
+        second_moments(j < 4 ? vc.x : vc.y, j & 3, va, &v[j], &v[j + 1]);
       }
     } else {
       load_vec<float, AW_VALUES>(mo.m + at, m);
@@ -188,13 +196,13 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
       const float ma = warp_max_bits(mb), va = warp_max_bits(vb);
       const bool plain = ma >= 1e-30f && ma <= 1e30f && va >= 1e-30f && va <= 1e30f;  // scales that have an inverse
       const float mi = __fdiv_rn(1.0f, ma), vi = __fdiv_rn(1.0f, va);
-      float mc[AW_VALUES], vc[AW_VALUES], doubt = 0.0f;
+      float mc[AW_VALUES], vc[AW_VALUES], far_m = 0.0f, far_v = 0.0f;
 #pragma unroll
-      for (int j = 0; j < AW_VALUES; ++j) {
-        mc[j] = quick_code(fabsf(m[j]), mi, 127.0f, doubt);
-        vc[j] = quick_code(root[j], vi, 255.0f, doubt);
+      for (int j = 0; j < AW_VALUES; j += 2) {
+        quick_codes(abs2(two(m[j], m[j + 1])), mi, 127.0f, far_m, &mc[j], &mc[j + 1]);
+        quick_codes(two(root[j], root[j + 1]), vi, 255.0f, far_v, &vc[j], &vc[j + 1]);
       }
-      if (!plain || doubt >= 0.5f) {  // 7 % of the warps
+      if (!plain || far_m >= 0.5f - 127.0f * 4.3e-7f || far_v >= 0.5f - 255.0f * 4.3e-7f) {  // some lane of one warp in fourteen
 #pragma unroll
         for (int j = 0; j < AW_VALUES; ++j) {
           mc[j] = exact_code(fabsf(m[j]), ma, 127.0f);
@@ -250,8 +258,10 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_values_kernel(const uint32_t
       const int64_t i = i0 + u * AW_THREADS;
       float v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        v[j] = SECOND ? second_moment(code_value<false>(c[u], j), scale[u]) : first_moment(code_value<true>(c[u], j), scale[u]);
+      for (int j = 0; j < 4; j += 2) {
+        if (SECOND) second_moments(c[u], j, scale[u], &v[j], &v[j + 1]);
+        else first_moments(c[u], j, scale[u], &v[j], &v[j + 1]);
+      }
       if (i < words) out[i] = float4{v[0], v[1], v[2], v[3]};
     }
   }

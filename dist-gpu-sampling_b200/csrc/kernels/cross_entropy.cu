@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(CE_THREADS) ce_pack_kernel(const __grid_consta
     if (warp == 0) {  // slices_for, a lane for every 32nd number of slices: fewest tiles in the busiest slot, then fewest slices
       const int blocks = live > 0 ? (live + a.to.block_rows - 1) / a.to.block_rows : 1;
       unsigned long long best = ~0ull;
-      for (int k = 1 + lane; k <= a.to.col_tiles && k <= a.to.slots; k += 32) {
+      for (int k = 1 + lane; k <= a.to.col_tiles && k <= a.to.slots && (k == 1 || int64_t(blocks) * k <= kMostRounds * a.to.slots); k += 32) {
         const unsigned long long rounds = (static_cast<unsigned long long>(blocks) * k + a.to.slots - 1) / a.to.slots;
         const unsigned long long cost = (rounds * ((a.to.col_tiles + k - 1) / k)) << 10 | k;
         best = cost < best ? cost : best;

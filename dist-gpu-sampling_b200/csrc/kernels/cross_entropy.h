@@ -32,14 +32,16 @@ struct Layout {
 };
 
 // Slices of `cols` column tiles for `rows` row blocks on `slots` CTAs that run at once: the cut with the fewest tiles in
-// the busiest slot.
+// the busiest slot.  More than one slice only while that gives a slot no more than kMostRounds of them, which also bounds what
+// the slices' results take.
+constexpr int64_t kMostRounds = 8;
 inline int64_t slices_for(int64_t rows, int64_t cols, int64_t slots) {
   // (in 32 bits and with one division a candidate: this is worked out on every call)
-  if (rows >= (int64_t(1) << 20)) return 1;
+  if (rows > kMostRounds * slots) return 1;
   const uint32_t r = static_cast<uint32_t>(rows), c = static_cast<uint32_t>(cols), most = static_cast<uint32_t>(cols < slots ? cols : slots);
   uint32_t best = 1, rounds = 0, room = 0;  // rounds = tiles(r * s, slots), room = rounds * slots - r * s
   uint64_t least = UINT64_MAX;
-  for (uint32_t s = 1; s <= most; ++s) {
+  for (uint32_t s = 1; s <= most && (s == 1 || r * s <= kMostRounds * slots); ++s) {
     while (room < r) {
       room += static_cast<uint32_t>(slots);
       ++rounds;

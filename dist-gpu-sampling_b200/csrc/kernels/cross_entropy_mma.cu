@@ -611,7 +611,7 @@ int64_t splits_for(int64_t row_blocks, int64_t d_tiles, int64_t dh_k, int64_t dw
   constexpr int64_t kItem = 6, kMostSplits = 16;
   int64_t best = 1, least = INT64_MAX;
   *dh_first = true;
-  for (int64_t s = 1; s <= kMostSplits && s * 4 <= dh_k + 3; ++s) {
+  for (int64_t s = 1; s <= kMostSplits && (s == 1 || (s * 4 <= dh_k && row_blocks * d_tiles * s <= 32 * pairs)); ++s) {
     const int64_t count[2] = {row_blocks * d_tiles * s, dw_tiles * d_tiles}, cost[2] = {tiles(dh_k, s) + kItem, dw_k + kItem};
     for (int first = 0; first < 2; ++first) {
       const int64_t n0 = count[first], n1 = count[1 - first], c0 = cost[first], c1 = cost[1 - first];
@@ -668,10 +668,11 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   if (D % 8 != 0) p.weight = l.take(V * p.pitch * 2);
   const Layout common = l;
   p.target_logit = l.take(n * 4);
-  // (compact: the number of slices follows the number of rows, which is not known here)
-  const int64_t most_slices = !p.compact ? p.slices : p.col_tiles < p.pairs ? p.col_tiles : p.pairs;
-  p.top = l.take(COL_GROUPS * most_slices * n * 4);
-  p.total = l.take(COL_GROUPS * most_slices * n * 4);
+  // (compact: the number of slices follows the number of rows, which is not known here; but blocks * slices <= kMostRounds * pairs
+  // unless there is one slice)
+  const int64_t most = p.compact ? n + kMostRounds * p.pairs * M_TILE : n * p.slices;
+  p.top = l.take(COL_GROUPS * most * 4);
+  p.total = l.take(COL_GROUPS * most * 4);
   p.forward_bytes = l.bytes;
   l = common;
   p.dloss = l.take(n * 4);

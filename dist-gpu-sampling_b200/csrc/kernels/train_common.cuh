@@ -101,6 +101,29 @@ __device__ __forceinline__ void store_vec_from_float(void* p, int32_t dtype, int
   else store_vec<__half, VEC>(static_cast<__half*>(p) + i, in);
 }
 
+// ---- two 32-bit floats in one instruction ---------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split2(uint64_t v, float* lo, float* hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // launch_chained (common.cuh) with a two-dimensional grid and dynamic shared memory
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_training(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t s,
