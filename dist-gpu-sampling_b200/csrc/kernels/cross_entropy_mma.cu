@@ -68,14 +68,28 @@ constexpr float LOG2E = 1.4426950408889634f;
 // 48 MB 4.07 ms, 96 MB 3.64, 384 MB 3.53, 768 MB 3.57).
 constexpr int64_t PIECE_BYTES = int64_t(256) << 20;
 
-enum Mode { STATS, GRAD, PRODUCT };
+// G in 16 bits is as far from its value as results of that type are from theirs, and the errors of many rows and results average:
+// gradients come out up to sqrt(2) times as far off as their own rounding.  They do not average where there are few: a row's results
+// all carry the rounding of its largest entry, the target's.  There G takes two planes, its rounded value and what that leaves,
+// and both products run over the two; with no more than FEW_ROWS rows reading and writing W and dW still takes longer.
+constexpr int64_t FEW_ROWS = 128, FEW_RESULTS = 1024;
+
+// NARROW is STATS for no more than NARROW_COLS classes.  A tensor core cuts what it adds to an accumulator of 32 bits instead of
+// rounding it, which shows in the loss of few classes (1e-6 of it at 4 classes and rows of 1 000, where it hardly shows at 1 000
+// classes).  There the products stop every NARROW_K blocks of k and the parts are added in registers.
+enum Mode { STATS, GRAD, PRODUCT, NARROW };
+constexpr int NARROW_COLS = N_TILE / 2, NARROW_K = 4;
+template <int MODE>
+constexpr bool is_stats() {
+  return MODE == STATS || MODE == NARROW;
+}
 template <int MODE>
 constexpr int stages() {
-  return MODE == STATS ? 6 : 5;
+  return is_stats<MODE>() ? 6 : 5;
 }
 template <int MODE>
 constexpr uint32_t smem_bytes() {  // alignment, stages, a staging buffer for each warp, barriers
-  return 1024 + stages<MODE>() * STAGE_BYTES + (MODE == STATS ? 0 : EPILOGUE_WARPS * STAGING_BYTES) + 256;
+  return 1024 + stages<MODE>() * STAGE_BYTES + (is_stats<MODE>() ? 0 : EPILOGUE_WARPS * STAGING_BYTES) + 256;
 }
 
 enum OutKind { OUT_F32_STORE, OUT_F32_ADD, OUT_TYPED, OUT_TYPED_ODD };
@@ -88,6 +102,8 @@ struct Part {
   int32_t n_total;  // columns of the result
   int32_t m_total;
   int32_t out_kind;
+  int32_t planes;      // of G: blocks of k alternate between them
+  int32_t plane_rows;  // rows of G between them
   int64_t split_rows;  // rows between the splits' partial results
   void* odd;           // OUT_TYPED_ODD: the result itself, rows of n_total elements
 };
@@ -110,7 +126,9 @@ struct alignas(64) MmaArgs {
   float* total;
   const float* dloss;
   const float* lse;
-  const float* largest;  // float16: the largest |dloss| of each CTA that packed rows; null: G is not scaled
+  uint16_t* low;         // GRAD: the second plane of G, rows low_pitch elements apart; null: there is one plane
+  int64_t low_pitch;
+  const float* largest;  // the largest |dloss| of each CTA that packed rows
   int32_t* status;
 };
 
@@ -137,6 +155,8 @@ __device__ __forceinline__ Extent extent_of(const MmaArgs& a) {
   e.slices = a.live != nullptr ? a.live[1] : a.slices;
   if constexpr (MODE == STATS) {
     e.items = e.row_blocks * e.slices;
+  } else if constexpr (MODE == NARROW) {
+    e.items = e.row_blocks;
   } else if constexpr (MODE == GRAD) {
     e.items = e.row_blocks * a.col_tiles;
   } else {
@@ -161,7 +181,7 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const Extent& ext, int
     x.which = item >= ext.first_items;
     const Part& p = a.part[x.which];
     const int i = item - (x.which ? ext.first_items : 0);
-    const int k_blocks = p.a_mn ? ext.row_k_blocks : p.k_blocks;
+    const int k_blocks = p.planes * (p.a_mn ? ext.row_k_blocks : p.k_blocks);
     const int nt = i % p.n_tiles, rest = i / p.n_tiles;
     x.split = rest % p.splits;
     x.m0 = rest / p.splits * M_TILE;
@@ -169,6 +189,12 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const Extent& ext, int
     if (p.n_step < N_TILE || p.n_total - x.n0 <= N_TILE / 2) x.n = N_TILE / 2;
     x.k0 = static_cast<int32_t>(static_cast<int64_t>(k_blocks) * x.split / p.splits);
     x.k1 = static_cast<int32_t>(static_cast<int64_t>(k_blocks) * (x.split + 1) / p.splits);
+  } else if constexpr (MODE == NARROW) {
+    x.n = NARROW_COLS;
+    x.m0 = item * M_TILE;
+    x.n0 = 0;
+    x.k0 = t * NARROW_K;
+    x.k1 = a.k_blocks < x.k0 + NARROW_K ? a.k_blocks : x.k0 + NARROW_K;
   } else {
     x.m0 = item % ext.row_blocks * M_TILE;
     x.n0 = t * N_TILE;
@@ -177,13 +203,16 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const Extent& ext, int
   }
   return x;
 }
-// the column tiles [t0, t1) of an item
+// the column tiles (NARROW: runs along k) [t0, t1) of an item
 template <int MODE>
 __device__ __forceinline__ void range_of(const MmaArgs& a, const Extent& ext, int item, int* t0, int* t1) {
   if constexpr (MODE == STATS) {
     const int slice = item / ext.row_blocks;
     *t0 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * slice / ext.slices);
     *t1 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * (slice + 1) / ext.slices);
+  } else if constexpr (MODE == NARROW) {
+    *t0 = 0;
+    *t1 = (a.k_blocks + NARROW_K - 1) / NARROW_K;
   } else if constexpr (MODE == GRAD) {
     *t0 = item / ext.row_blocks;
     *t1 = *t0 + 1;
@@ -278,20 +307,31 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&t);
   }
 }
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t v, float* lo, float* hi) {
+  if constexpr (BF16) {
+    *lo = __uint_as_float(v << 16);
+    *hi = __uint_as_float(v & 0xffff0000u);
+  } else {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    *lo = t.x;
+    *hi = t.y;
+  }
+}
 __device__ __forceinline__ void st_shared(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// float16: G is scaled by a power of two that brings its largest possible value, max |dloss|, to just below 2^15, so that
-// probabilities down to 2^-29 of it stay normal numbers; the products' results are scaled back.
+// G is scaled so that its largest possible value, max |dloss|, becomes 2^15, and the products' results are scaled back.  float16:
+// probabilities down to 2^-29 of it stay normal numbers.  Both types: the entries that weigh most, those of targets with a small
+// probability, stand just below a power of two, where rounding to the type is off least (half as far as just above one: 275 rows
+// with weights between half and three halves of 1 / 275 gave gradients 1.57 times as far off as their own rounding without it).
 __device__ __forceinline__ float grad_factor(const float* largest, int count, int lane, bool inverse) {
   float m = 0.0f;
   for (int i = lane; i < count; i += 32) m = fmaxf(m, largest[i]);
   m = __uint_as_float(__reduce_max_sync(FULL_MASK, __float_as_uint(m)));
-  int e = 0;
-  if (m > 0.0f && m < INFINITY) frexpf(m, &e);  // m = f 2^e, f in [1/2, 1)
-  e = e < -100 ? -100 : e > 100 ? 100 : e;
-  return ldexpf(1.0f, inverse ? e - 15 : 15 - e);
+  m = m > 0.0f ? fminf(fmaxf(m, 1e-30f), 1e30f) : 1.0f;
+  return inverse ? m * (1.0f / 32768.0f) : 32768.0f / m;
 }
 
 template <int MODE, bool BF16>
@@ -300,7 +340,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
   extern __shared__ unsigned char smem_raw[];
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = smem + STAGES * STAGE_BYTES;
-  const uint32_t words = staging + (MODE == STATS ? 0 : EPILOGUE_WARPS * STAGING_BYTES);
+  const uint32_t words = staging + (is_stats<MODE>() ? 0 : EPILOGUE_WARPS * STAGING_BYTES);
   const uint32_t full = words, empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16, tmem_word = acc_empty + 16;
   volatile int32_t* dead = reinterpret_cast<volatile int32_t*>(smem_raw + (tmem_word + 8 - smem_addr(smem_raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -348,12 +388,14 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
           if (!(ok = !*dead && bar_wait(empty + 8 * st, phase ^ 1))) break;
           const uint32_t to = smem + st * STAGE_BYTES, bar = in_cta(full + 8 * st, 0);
           if (rank == 0) bar_expect(full + 8 * st, bytes);
-          const int32_t k = kb * K_TILE;
+          // two planes: their blocks take turns, so that the other operand's block comes out of L2 the second time
+          const bool two_planes = MODE == PRODUCT && a.part[x.which].planes == 2;
+          const int32_t k = (two_planes ? kb >> 1 : kb) * K_TILE, plane = two_planes && (kb & 1) ? a.part[x.which].plane_rows : 0;
           if (a_mn) {
-            load_box(to, ma, m, k, bar);
-            load_box(to + BOX_BYTES, ma, m + 64, k, bar);
+            load_box(to, ma, m, k + plane, bar);
+            load_box(to + BOX_BYTES, ma, m + 64, k + plane, bar);
           } else {
-            load_box(to, ma, k, m, bar);
+            load_box(to, ma, k, m + plane, bar);
           }
           if (MODE == PRODUCT) {
             load_box(to + A_BYTES, mb, n, k, bar);
@@ -404,18 +446,20 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
     }
   } else if (warp >= FIRST_EPILOGUE_WARP) {
     // ---- finished accumulators: a warp reads the 32 lanes (rows) that its number allows, and a quarter of the columns
-    const int quarter = warp & 3, group = (warp - FIRST_EPILOGUE_WARP) >> 2, c0 = group * GROUP_COLS;
+    constexpr int COLS = MODE == NARROW ? NARROW_COLS / COL_GROUPS : GROUP_COLS;
+    const int quarter = warp & 3, group = (warp - FIRST_EPILOGUE_WARP) >> 2, c0 = group * COLS;
     const uint32_t from0 = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
     const uint32_t stage_at = staging + (warp - FIRST_EPILOGUE_WARP) * STAGING_BYTES;
     const uint32_t free_bar = in_cta(acc_empty, 0);
     int buf = 0;
     uint32_t acc_phase = 0;
     float factor = 1.0f;
-    if (MODE != STATS && a.largest != nullptr) factor = grad_factor(a.largest, a.largest_count, lane, MODE == PRODUCT);
+    if (!is_stats<MODE>()) factor = grad_factor(a.largest, a.largest_count, lane, MODE == PRODUCT);
     for (int item = pair; ok && item < ext.items; item += pairs) {
       int t0, t1;
       range_of<MODE>(a, ext, item, &t0, &t1);
       RowSum sum;
+      uint32_t logits[MODE == NARROW ? 32 : 1];
       for (int t = t0; t < t1; ++t) {
         const Tile x = tile_of<MODE>(a, ext, item, t);
         const int32_t row = x.m0 + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
@@ -433,9 +477,9 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
         ok = __all_sync(FULL_MASK, ok);
         if (!ok) break;
         fence_after();
-        const int chunks = c0 < x.n ? GROUP_COLS / 32 : 0;  // a narrow tile has nothing for half of the warps
+        const int chunks = c0 < x.n ? COLS / 32 : 0;  // a narrow tile has nothing for half of the warps
 #pragma unroll
-        for (int c = 0; c < GROUP_COLS / 32; ++c) {
+        for (int c = 0; c < COLS / 32; ++c) {
           if (c < chunks) {
             uint32_t now[32];
             tmem_load32(from0 + buf * N_TILE + c * 32, now);
@@ -446,7 +490,16 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
               if (lane == 0) bar_arrive_in(free_bar + 8 * buf);
             }
             const int32_t col = x.n0 + c0 + c * 32;  // first of the 32
-            if constexpr (MODE == STATS) {
+            if constexpr (MODE == NARROW) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                logits[i] = t == t0 ? now[i] : __float_as_uint(__uint_as_float(logits[i]) + __uint_as_float(now[i]));
+              if (t + 1 == t1) {
+                const uint32_t at = static_cast<uint32_t>(word - col);
+                if (at < 32u && word >= 0) a.target_logit[row] = pick(logits, static_cast<int>(at));
+                if (col < a.V) sum.add(logits, static_cast<int32_t>(a.V) - col);
+              }
+            } else if constexpr (MODE == STATS) {
               const int32_t left = static_cast<int32_t>(a.V) - col;
               const uint32_t at = static_cast<uint32_t>(word - col);
               if (at < 32u && word >= 0) a.target_logit[row] = pick(now, static_cast<int>(at));
@@ -478,7 +531,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
                 for (int i = 0; i < 32; ++i) now[i] = 0;
               }
             }
-            if constexpr (MODE != STATS) {
+            if constexpr (!is_stats<MODE>()) {
               const int kind = MODE == GRAD ? static_cast<int>(OUT_TYPED) : a.part[x.which].out_kind;
               const bool typed = kind == OUT_TYPED || kind == OUT_TYPED_ODD;
               if (MODE == PRODUCT) {
@@ -499,6 +552,15 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
                   for (int i = 0; i < 4; ++i)
                     p[i] = pack2<BF16>(__uint_as_float(now[j * 8 + i * 2]), __uint_as_float(now[j * 8 + i * 2 + 1]));
                   st_shared(at_row + (((c & 1) * 4 + j) ^ (lane & 7)) * 16, p[0], p[1], p[2], p[3]);
+                  if (MODE == GRAD && a.low != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                      float hi0, hi1;
+                      unpack2<BF16>(p[i], &hi0, &hi1);
+                      p[i] = pack2<BF16>(__uint_as_float(now[j * 8 + i * 2]) - hi0, __uint_as_float(now[j * 8 + i * 2 + 1]) - hi1);
+                    }
+                    *reinterpret_cast<uint4*>(a.low + row * a.low_pitch + col + j * 8) = uint4{p[0], p[1], p[2], p[3]};
+                  }
                 }
               } else {
 #pragma unroll
@@ -543,7 +605,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
         buf ^= 1;
         if (buf == 0) acc_phase ^= 1;
       }
-      if (MODE == STATS && ok) {
+      if (is_stats<MODE>() && ok) {
         const int32_t row = item % ext.row_blocks * M_TILE + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
         const int64_t at = static_cast<int64_t>(row) * (ext.slices * COL_GROUPS) + item / ext.row_blocks * COL_GROUPS + group;
         if (row < ext.rows) {
@@ -552,7 +614,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
         }
       }
     }
-    if (MODE != STATS && lane == 0) store_wait_all();
+    if (!is_stats<MODE>() && lane == 0) store_wait_all();
   }
   if (!ok) {
     *dead = 1;
@@ -600,6 +662,7 @@ __global__ void __launch_bounds__(256) ce_pack_weight_kernel(const uint16_t* __r
 struct MmaPlan {
   int64_t pitch, row_blocks, col_tiles, slices, pairs;
   int64_t piece, splits, dpitch;
+  int64_t planes, g_rows;  // of G; rows of a plane
   bool one_piece, compact, dh_first;
   size_t packed, word, slot, live, counts, weight, target_logit, top, total, dloss, lse, largest, g, dh;
   size_t forward_bytes, backward_bytes;
@@ -644,7 +707,9 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.col_tiles = tiles(V, N_TILE);
   p.slices = slices_for(p.row_blocks, p.col_tiles, p.pairs);
   // as many column tiles as PIECE_BYTES allow, rounded down to full rounds of the GRAD launch
-  int64_t piece_tiles = PIECE_BYTES / 2 / (n > 0 ? n : 1) / N_TILE;
+  p.planes = n <= FEW_ROWS || (n < V ? n : V) * D <= FEW_RESULTS ? 2 : 1;
+  p.g_rows = p.planes == 2 ? p.row_blocks * M_TILE : n;
+  int64_t piece_tiles = PIECE_BYTES / 2 / (p.planes * p.g_rows) / N_TILE;
   if (piece_tiles < 1) piece_tiles = 1;
   if (piece_tiles >= p.col_tiles) {
     piece_tiles = p.col_tiles;
@@ -655,7 +720,8 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.piece = piece_tiles * N_TILE;
   p.one_piece = p.piece >= V;
   p.dpitch = up(D, 4);
-  p.splits = splits_for(p.row_blocks, tiles(D, N_TILE), tiles(p.piece, K_TILE), piece_tiles, tiles(n, K_TILE), p.pairs, &p.dh_first);
+  p.splits = splits_for(p.row_blocks, tiles(D, N_TILE), p.planes * tiles(p.piece, K_TILE), piece_tiles, p.planes * tiles(n, K_TILE),
+                        p.pairs, &p.dh_first);
   p.compact = worth_compacting(n, D, V);
   Layout l;
   p.packed = l.take(n * p.pitch * 2);
@@ -678,7 +744,7 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.dloss = l.take(n * 4);
   p.lse = l.take(n * 4);
   p.largest = l.take(ce_pack_ctas(n) * 4);
-  p.g = l.take(n * p.piece * 2);
+  p.g = l.take(p.planes * p.g_rows * p.piece * 2);
   if (!(p.one_piece && p.splits == 1 && !p.compact)) p.dh = l.take(p.splits * p.row_blocks * M_TILE * p.dpitch * 4);
   p.backward_bytes = l.bytes;
   return p;
@@ -759,7 +825,8 @@ int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) 
   if (int rc = make_map(&a.a[0], where_they_lie ? q.hidden : r.rows, q.dtype, q.D, q.n,
                         where_they_lie ? (q.n == 1 ? q.D : q.hidden_stride) : p.pitch, K_TILE, M_CTA))
     return rc;
-  if (int rc = make_map(&a.b[0], w.p, q.dtype, q.D, q.V, w.stride, K_TILE, N_TILE / 2)) return rc;
+  const bool narrow = q.V <= NARROW_COLS;
+  if (int rc = make_map(&a.b[0], w.p, q.dtype, q.D, q.V, w.stride, K_TILE, narrow ? NARROW_COLS / 2 : N_TILE / 2)) return rc;
   a.items = static_cast<int32_t>(p.row_blocks * p.slices);
   a.col_tiles = static_cast<int32_t>(p.col_tiles);
   a.slices = static_cast<int32_t>(p.slices);
@@ -775,7 +842,7 @@ int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) 
   a.top = reinterpret_cast<float*>(q.ws + p.top);
   a.total = reinterpret_cast<float*>(q.ws + p.total);
   a.status = q.status;
-  if (int rc = launch<STATS>(a, p.pairs, q.dtype, s)) return rc;
+  if (int rc = narrow ? launch<NARROW>(a, p.pairs, q.dtype, s) : launch<STATS>(a, p.pairs, q.dtype, s)) return rc;
   return ce_join(q, a.top, a.total, COL_GROUPS, p.slices, r.live, a.word, r.slot, a.target_logit, loss, lse, s);
 }
 
@@ -784,7 +851,7 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
   CePacked r = packed_rows(q, p);
   r.dloss = reinterpret_cast<float*>(q.ws + p.dloss);
   r.lse = reinterpret_cast<float*>(q.ws + p.lse);
-  if (q.dtype == DGS_F16) r.largest = reinterpret_cast<float*>(q.ws + p.largest);
+  r.largest = reinterpret_cast<float*>(q.ws + p.largest);
   if (int rc = ce_pack(q, r, dloss, lse, s)) return rc;
   const void* packed = r.rows;
   Weight w;
@@ -799,7 +866,9 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     MmaArgs a{};
     if (int rc = make_map(&a.a[0], packed, q.dtype, q.D, q.n, p.pitch, K_TILE, M_CTA)) return rc;
     if (int rc = make_map(&a.b[0], wp, q.dtype, q.D, width, w.stride, K_TILE, N_TILE / 2)) return rc;
-    if (int rc = make_map(&a.out[0], g, q.dtype, width, q.n, p.piece, 64, 32)) return rc;
+    if (int rc = make_map(&a.out[0], g, q.dtype, width, p.g_rows, p.piece, 64, 32)) return rc;
+    a.low = p.planes == 2 ? g + p.g_rows * p.piece : nullptr;
+    a.low_pitch = p.piece;
     a.col_tiles = static_cast<int32_t>(tiles(width, N_TILE));
     a.items = static_cast<int32_t>(p.row_blocks) * a.col_tiles;
     a.k_blocks = static_cast<int32_t>(tiles(q.D, K_TILE));
@@ -824,18 +893,21 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     if (dhidden != nullptr) {
       Part& t = m.part[at_dh];
       t.a_mn = 0;
+      t.planes = static_cast<int32_t>(p.planes);
+      t.plane_rows = static_cast<int32_t>(p.g_rows);
       t.n_tiles = d_tiles;
       t.n_step = n_step;
       t.k_blocks = static_cast<int32_t>(tiles(width, K_TILE));
       // (the first piece has work for every split; a narrow last one adds to as many as it has)
-      t.splits = static_cast<int32_t>(p.splits < t.k_blocks ? p.splits : t.k_blocks);
+      const int64_t k_all = p.planes * t.k_blocks;
+      t.splits = static_cast<int32_t>(p.splits < k_all ? p.splits : k_all);
       dh_items = p.row_blocks * d_tiles * t.splits;
       t.n_total = static_cast<int32_t>(q.D);
       t.m_total = static_cast<int32_t>(q.n);
       t.split_rows = p.row_blocks * M_TILE;
       t.out_kind = !dh_direct ? (v0 > 0 ? OUT_F32_ADD : OUT_F32_STORE) : even && aligned_to(dhidden, 16) ? OUT_TYPED : OUT_TYPED_ODD;
       t.odd = dhidden;
-      if (int rc = make_map(&m.a[at_dh], g, q.dtype, width, q.n, p.piece, K_TILE, M_CTA)) return rc;
+      if (int rc = make_map(&m.a[at_dh], g, q.dtype, width, p.planes * p.g_rows, p.piece, K_TILE, M_CTA)) return rc;
       if (int rc = make_map(&m.b[at_dh], wp, q.dtype, q.D, width, w.stride, 64, K_TILE)) return rc;
       if (t.out_kind == OUT_TYPED) {
         if (int rc = make_map(&m.out[at_dh], dhidden, q.dtype, q.D, q.n, q.D, 64, 32)) return rc;
@@ -846,6 +918,8 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     if (dweight != nullptr) {
       Part& t = m.part[at_dw];
       t.a_mn = 1;
+      t.planes = static_cast<int32_t>(p.planes);
+      t.plane_rows = static_cast<int32_t>(p.g_rows);
       t.n_tiles = d_tiles;
       t.n_step = n_step;
       t.splits = 1;
@@ -856,7 +930,7 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
       uint16_t* to = static_cast<uint16_t*>(dweight) + v0 * q.D;
       t.out_kind = even && aligned_to(dweight, 16) ? OUT_TYPED : OUT_TYPED_ODD;
       t.odd = to;
-      if (int rc = make_map(&m.a[at_dw], g, q.dtype, width, q.n, p.piece, 64, K_TILE)) return rc;
+      if (int rc = make_map(&m.a[at_dw], g, q.dtype, width, p.planes * p.g_rows, p.piece, 64, K_TILE)) return rc;
       if (int rc = make_map(&m.b[at_dw], packed, q.dtype, q.D, q.n, p.pitch, 64, K_TILE)) return rc;
       if (t.out_kind == OUT_TYPED) {
         if (int rc = make_map(&m.out[at_dw], to, q.dtype, q.D, width, q.D, 64, 32)) return rc;
