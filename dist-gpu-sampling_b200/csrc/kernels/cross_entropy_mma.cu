@@ -69,10 +69,13 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int64_t PIECE_BYTES = int64_t(256) << 20;
 
 // G in 16 bits is as far from its value as results of that type are from theirs, and the errors of many rows and results average:
-// gradients come out up to sqrt(2) times as far off as their own rounding.  They do not average where there are few: a row's results
-// all carry the rounding of its largest entry, the target's.  There G takes two planes, its rounded value and what that leaves,
-// and both products run over the two; with no more than FEW_ROWS rows reading and writing W and dW still takes longer.
-constexpr int64_t FEW_ROWS = 128, FEW_RESULTS = 1024;
+// gradients come out up to sqrt(2) times as far off as their own rounding.  They do not average where there are few: a row's
+// results all carry the rounding of its largest entry, the target's.  There G takes two planes, its rounded value and what that
+// leaves, and both products run over the two.  Forward and backward at rows of 512 and 50 000 classes: 8 rows 84 -> 98 us, 64 rows
+// 86 -> 102, 256 rows 93 -> 168; so the fewer the rows, the more classes may there be.
+inline bool two_planes(int64_t n, int64_t D, int64_t V) {
+  return n <= 16 || (n <= 256 && n * n * V <= (int64_t(1) << 28)) || (n < V ? n : V) * D <= 1024;
+}
 
 // NARROW is STATS for no more than NARROW_COLS classes.  A tensor core cuts what it adds to an accumulator of 32 bits instead of
 // rounding it, which shows in the loss of few classes (1e-6 of it at 4 classes and rows of 1 000, where it hardly shows at 1 000
@@ -103,7 +106,8 @@ struct Part {
   int32_t m_total;
   int32_t out_kind;
   int32_t planes;      // of G: blocks of k alternate between them
-  int32_t plane_rows;  // rows of G between them
+  int32_t plane_rows;  // rows of G between them (a box that runs over the end of one meets rows of the other: its rows of h are
+                       // zeros there, or its results are not stored)
   int64_t split_rows;  // rows between the splits' partial results
   void* odd;           // OUT_TYPED_ODD: the result itself, rows of n_total elements
 };
@@ -389,8 +393,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
           const uint32_t to = smem + st * STAGE_BYTES, bar = in_cta(full + 8 * st, 0);
           if (rank == 0) bar_expect(full + 8 * st, bytes);
           // two planes: their blocks take turns, so that the other operand's block comes out of L2 the second time
-          const bool two_planes = MODE == PRODUCT && a.part[x.which].planes == 2;
-          const int32_t k = (two_planes ? kb >> 1 : kb) * K_TILE, plane = two_planes && (kb & 1) ? a.part[x.which].plane_rows : 0;
+          const bool alternate = MODE == PRODUCT && a.part[x.which].planes == 2;
+          const int32_t k = (alternate ? kb >> 1 : kb) * K_TILE, plane = alternate && (kb & 1) ? a.part[x.which].plane_rows : 0;
           if (a_mn) {
             load_box(to, ma, m, k + plane, bar);
             load_box(to + BOX_BYTES, ma, m + 64, k + plane, bar);
@@ -559,7 +563,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
                       unpack2<BF16>(p[i], &hi0, &hi1);
                       p[i] = pack2<BF16>(__uint_as_float(now[j * 8 + i * 2]) - hi0, __uint_as_float(now[j * 8 + i * 2 + 1]) - hi1);
                     }
-                    *reinterpret_cast<uint4*>(a.low + row * a.low_pitch + col + j * 8) = uint4{p[0], p[1], p[2], p[3]};
+                    if (row < a.n) *reinterpret_cast<uint4*>(a.low + row * a.low_pitch + col + j * 8) = uint4{p[0], p[1], p[2], p[3]};
                   }
                 }
               } else {
@@ -662,7 +666,7 @@ __global__ void __launch_bounds__(256) ce_pack_weight_kernel(const uint16_t* __r
 struct MmaPlan {
   int64_t pitch, row_blocks, col_tiles, slices, pairs;
   int64_t piece, splits, dpitch;
-  int64_t planes, g_rows;  // of G; rows of a plane
+  int64_t planes;  // of G
   bool one_piece, compact, dh_first;
   size_t packed, word, slot, live, counts, weight, target_logit, top, total, dloss, lse, largest, g, dh;
   size_t forward_bytes, backward_bytes;
@@ -671,10 +675,11 @@ struct MmaPlan {
 // How often dh's tiles are cut along the classes, and whether they come before dW's: the launch deals its items to the pairs in
 // turn, and the cut is the one whose busiest pair has the least to do, in blocks of K_TILE plus what an item costs besides.
 int64_t splits_for(int64_t row_blocks, int64_t d_tiles, int64_t dh_k, int64_t dw_tiles, int64_t dw_k, int64_t pairs, bool* dh_first) {
-  constexpr int64_t kItem = 6, kMostSplits = 16;
+  constexpr int64_t kItem = 6, kMostSplits = 64;
   int64_t best = 1, least = INT64_MAX;
   *dh_first = true;
-  for (int64_t s = 1; s <= kMostSplits && (s == 1 || (s * 4 <= dh_k && row_blocks * d_tiles * s <= 32 * pairs)); ++s) {
+  // (1 to 8, then steps of an eighth to a quarter: this is worked out on every call)
+  for (int64_t s = 1; s <= kMostSplits && (s == 1 || (s * 4 <= dh_k && row_blocks * d_tiles * s <= 32 * pairs)); s += s < 8 ? 1 : s < 16 ? 2 : s < 32 ? 4 : 8) {
     const int64_t count[2] = {row_blocks * d_tiles * s, dw_tiles * d_tiles}, cost[2] = {tiles(dh_k, s) + kItem, dw_k + kItem};
     for (int first = 0; first < 2; ++first) {
       const int64_t n0 = count[first], n1 = count[1 - first], c0 = cost[first], c1 = cost[1 - first];
@@ -707,9 +712,8 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.col_tiles = tiles(V, N_TILE);
   p.slices = slices_for(p.row_blocks, p.col_tiles, p.pairs);
   // as many column tiles as PIECE_BYTES allow, rounded down to full rounds of the GRAD launch
-  p.planes = n <= FEW_ROWS || (n < V ? n : V) * D <= FEW_RESULTS ? 2 : 1;
-  p.g_rows = p.planes == 2 ? p.row_blocks * M_TILE : n;
-  int64_t piece_tiles = PIECE_BYTES / 2 / (p.planes * p.g_rows) / N_TILE;
+  p.planes = two_planes(n, D, V) ? 2 : 1;
+  int64_t piece_tiles = PIECE_BYTES / 2 / (p.planes * n) / N_TILE;
   if (piece_tiles < 1) piece_tiles = 1;
   if (piece_tiles >= p.col_tiles) {
     piece_tiles = p.col_tiles;
@@ -744,7 +748,7 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.dloss = l.take(n * 4);
   p.lse = l.take(n * 4);
   p.largest = l.take(ce_pack_ctas(n) * 4);
-  p.g = l.take(p.planes * p.g_rows * p.piece * 2);
+  p.g = l.take(p.planes * n * p.piece * 2);
   if (!(p.one_piece && p.splits == 1 && !p.compact)) p.dh = l.take(p.splits * p.row_blocks * M_TILE * p.dpitch * 4);
   p.backward_bytes = l.bytes;
   return p;
@@ -866,8 +870,8 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     MmaArgs a{};
     if (int rc = make_map(&a.a[0], packed, q.dtype, q.D, q.n, p.pitch, K_TILE, M_CTA)) return rc;
     if (int rc = make_map(&a.b[0], wp, q.dtype, q.D, width, w.stride, K_TILE, N_TILE / 2)) return rc;
-    if (int rc = make_map(&a.out[0], g, q.dtype, width, p.g_rows, p.piece, 64, 32)) return rc;
-    a.low = p.planes == 2 ? g + p.g_rows * p.piece : nullptr;
+    if (int rc = make_map(&a.out[0], g, q.dtype, width, q.n, p.piece, 64, 32)) return rc;
+    a.low = p.planes == 2 ? g + q.n * p.piece : nullptr;
     a.low_pitch = p.piece;
     a.col_tiles = static_cast<int32_t>(tiles(width, N_TILE));
     a.items = static_cast<int32_t>(p.row_blocks) * a.col_tiles;
@@ -894,7 +898,7 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
       Part& t = m.part[at_dh];
       t.a_mn = 0;
       t.planes = static_cast<int32_t>(p.planes);
-      t.plane_rows = static_cast<int32_t>(p.g_rows);
+      t.plane_rows = static_cast<int32_t>(q.n);
       t.n_tiles = d_tiles;
       t.n_step = n_step;
       t.k_blocks = static_cast<int32_t>(tiles(width, K_TILE));
@@ -907,7 +911,7 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
       t.split_rows = p.row_blocks * M_TILE;
       t.out_kind = !dh_direct ? (v0 > 0 ? OUT_F32_ADD : OUT_F32_STORE) : even && aligned_to(dhidden, 16) ? OUT_TYPED : OUT_TYPED_ODD;
       t.odd = dhidden;
-      if (int rc = make_map(&m.a[at_dh], g, q.dtype, width, p.planes * p.g_rows, p.piece, K_TILE, M_CTA)) return rc;
+      if (int rc = make_map(&m.a[at_dh], g, q.dtype, width, p.planes * q.n, p.piece, K_TILE, M_CTA)) return rc;
       if (int rc = make_map(&m.b[at_dh], wp, q.dtype, q.D, width, w.stride, 64, K_TILE)) return rc;
       if (t.out_kind == OUT_TYPED) {
         if (int rc = make_map(&m.out[at_dh], dhidden, q.dtype, q.D, q.n, q.D, 64, 32)) return rc;
@@ -919,7 +923,7 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
       Part& t = m.part[at_dw];
       t.a_mn = 1;
       t.planes = static_cast<int32_t>(p.planes);
-      t.plane_rows = static_cast<int32_t>(p.g_rows);
+      t.plane_rows = static_cast<int32_t>(q.n);
       t.n_tiles = d_tiles;
       t.n_step = n_step;
       t.splits = 1;
@@ -930,7 +934,7 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
       uint16_t* to = static_cast<uint16_t*>(dweight) + v0 * q.D;
       t.out_kind = even && aligned_to(dweight, 16) ? OUT_TYPED : OUT_TYPED_ODD;
       t.odd = to;
-      if (int rc = make_map(&m.a[at_dw], g, q.dtype, width, p.planes * p.g_rows, p.piece, 64, K_TILE)) return rc;
+      if (int rc = make_map(&m.a[at_dw], g, q.dtype, width, p.planes * q.n, p.piece, 64, K_TILE)) return rc;
       if (int rc = make_map(&m.b[at_dw], packed, q.dtype, q.D, q.n, p.pitch, 64, K_TILE)) return rc;
       if (t.out_kind == OUT_TYPED) {
         if (int rc = make_map(&m.out[at_dw], to, q.dtype, q.D, width, q.D, 64, 32)) return rc;
