@@ -459,24 +459,33 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
     uint32_t acc_phase = 0;
     float factor = 1.0f;
     if (!is_stats<MODE>()) factor = grad_factor(a.largest, a.largest_count, lane, MODE == PRODUCT);
+    // what a row brings along; GRAD's next row is asked for a tile ahead
+    const int32_t my_row = static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
+    int32_t next_word = -1;
+    float next_grad = 0.0f, next_lse = 0.0f;
+    auto ask = [&](int item) {
+      const int32_t row = tile_of<MODE>(a, ext, item, 0).m0 + my_row;
+      next_word = -1;
+      if (item >= ext.items || row >= ext.rows) return;
+      bool wrong;
+      next_word = MODE == GRAD || a.word != nullptr ? a.word[row] : target_word(a.target, a.ids64, row, a.V, a.ignore_index, &wrong);
+      if (MODE == GRAD) {
+        next_grad = a.dloss[row];
+        next_lse = a.lse[row];
+      }
+    };
+    if (MODE != PRODUCT) ask(pair);
     for (int item = pair; ok && item < ext.items; item += pairs) {
       int t0, t1;
       range_of<MODE>(a, ext, item, &t0, &t1);
       RowSum sum;
       uint32_t logits[MODE == NARROW ? 32 : 1];
+      const int32_t word = next_word;
+      const float grad = next_grad * factor, lse = next_lse;
+      if (MODE != PRODUCT) ask(item + pairs);
       for (int t = t0; t < t1; ++t) {
         const Tile x = tile_of<MODE>(a, ext, item, t);
-        const int32_t row = x.m0 + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
-        int32_t word = -1;
-        float grad = 0.0f, lse = 0.0f;
-        if (MODE != PRODUCT && row < ext.rows) {
-          bool wrong;
-          word = MODE == GRAD || a.word != nullptr ? a.word[row] : target_word(a.target, a.ids64, row, a.V, a.ignore_index, &wrong);
-          if (MODE == GRAD && word >= 0) {
-            grad = a.dloss[row] * factor;
-            lse = a.lse[row];
-          }
-        }
+        const int32_t row = x.m0 + my_row;
         ok = !*dead && bar_wait(acc_full + 8 * buf, acc_phase);
         ok = __all_sync(FULL_MASK, ok);
         if (!ok) break;
