@@ -183,10 +183,12 @@ __global__ void __launch_bounds__(CE_THREADS) ce_pack_kernel(const __grid_consta
         a.to.live[1] = static_cast<int32_t>(best & 1023);
       }
     }
-    int64_t end = (static_cast<int64_t>(live) + 63) / 64 * 64;
-    if (end == 0) end = 64;
+  }
+  if (a.to.compact) {  // zeros to the end of the last block, for the products' sake and because what lay there may be no numbers
+    int64_t end = (static_cast<int64_t>(live) + a.to.block_rows - 1) / a.to.block_rows * a.to.block_rows;
+    if (end == 0) end = a.to.block_rows;
     if (end > a.n) end = a.n;
-    for (int64_t r = live + warp; r < end; r += WARPS) {
+    for (int64_t r = live + static_cast<int64_t>(blockIdx.x) * WARPS + warp; r < end; r += static_cast<int64_t>(gridDim.x) * WARPS) {
       T* dst = static_cast<T*>(a.to.rows) + r * a.pitch;
       for (int j = lane; j < a.pitch; j += 32) dst[j] = from_float<T>(0.0f);
     }

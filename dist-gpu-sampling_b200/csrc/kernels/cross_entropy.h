@@ -60,7 +60,7 @@ inline int64_t slices_for(int64_t rows, int64_t cols, int64_t slots) {
 // as a 32-bit word (-1: none), and for the backward pass dloss and lse.  Either row c is row c of the call (rows without a valid
 // target: zeros, word -1), or (compact) the rows with a valid target alone, in their order; then slot[i] is row i's place among
 // them (-1: none), live[0] their number, live[1] the slices for that many rows in blocks of block_rows, and the packed rows from
-// there to the next multiple of 64 (one at least) are zeros.
+// there to the end of the block (the first one, where there is no row) are zeros.
 struct CePacked {
   void* rows;
   int64_t pitch;
