@@ -490,7 +490,9 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
         ok = __all_sync(FULL_MASK, ok);
         if (!ok) break;
         fence_after();
-        const int chunks = c0 < x.n ? COLS / 32 : 0;  // a narrow tile has nothing for half of the warps
+        // a narrow tile has nothing for half of the warps, a block that is not full nothing for those behind its last row
+        const int32_t last_row = is_stats<MODE>() ? ext.rows : MODE == GRAD ? static_cast<int32_t>(a.n) : a.part[x.which].m_total;
+        const int chunks = c0 < x.n && row - lane < last_row ? COLS / 32 : 0;
 #pragma unroll
         for (int c = 0; c < COLS / 32; ++c) {
           if (c < chunks) {
@@ -641,32 +643,66 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
   if (warp == 2) tmem_free(tmem, TMEM_COLS);
 }
 
-// The weight's rows, `pitch` elements apart (rows of an odd length cannot be fetched by TMA where they lie)
+// The weight's rows, `pitch` elements apart (rows of an odd length cannot be fetched by TMA where they lie).  A lane makes eight
+// elements out of the two aligned 16-byte words that hold them; words that reach over the matrix's first or last byte are read
+// element by element.
+__device__ __forceinline__ uint4 eight_elements(const uint16_t* from, int count, uintptr_t first, uintptr_t end) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(from), word = at & ~uintptr_t(15);
+  const uint32_t skip = static_cast<uint32_t>(at - word) >> 1;  // elements in front of the first
+  if (word >= first && word + (skip ? 32 : 16) <= end) {
+    const uint4 a = *reinterpret_cast<const uint4*>(word);
+    uint32_t v[8] = {a.x, a.y, a.z, a.w, 0, 0, 0, 0};
+    if (skip) {
+      const uint4 b = *reinterpret_cast<const uint4*>(word + 16);
+      v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+    // whole words first, then the odd element
+    if (skip & 4) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) v[i] = i + 2 < 8 ? v[i + 2] : 0;
+    }
+    if (skip & 2) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) v[i] = v[i + 1];
+    }
+    if (skip & 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __funnelshift_r(v[i], v[i + 1], 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = 2 * i + 1 < count ? v[i] : 2 * i < count ? v[i] & 0xffffu : 0u;
+    return uint4{v[0], v[1], v[2], v[3]};
+  }
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = 2 * i < count ? from[2 * i] : 0u, hi = 2 * i + 1 < count ? from[2 * i + 1] : 0u;
+    v[i] = lo | (hi << 16);
+  }
+  return uint4{v[0], v[1], v[2], v[3]};
+}
+
 __global__ void __launch_bounds__(256) ce_pack_weight_kernel(const uint16_t* __restrict__ weight, const int64_t stride, const int64_t V,
                                                              const int D, const int pitch, uint16_t* __restrict__ packed) {
   pdl_enter();
-  const int lane = threadIdx.x & 31;
-  constexpr int U = 4;  // words of a row under way a lane, for two rows
-  for (int64_t row0 = (blockIdx.x * int64_t(8) + (threadIdx.x >> 5)) * 2; row0 < V; row0 += gridDim.x * int64_t(16)) {
-    for (int j0 = lane * 2; j0 < pitch; j0 += 64 * U) {
-      uint16_t v[2][U][2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int j = j0 + u * 64 + h;
-            v[r][u][h] = row0 + r < V && j < D ? weight[(row0 + r) * stride + j] : uint16_t(0);
-          }
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int j = j0 + u * 64;
-          if (row0 + r < V && j < pitch)
-            *reinterpret_cast<uint32_t*>(packed + (row0 + r) * pitch + j) = v[r][u][0] | (static_cast<uint32_t>(v[r][u][1]) << 16);
-        }
+  const uintptr_t first = reinterpret_cast<uintptr_t>(weight), end = reinterpret_cast<uintptr_t>(weight + (V - 1) * stride + D);
+  const int chunks = pitch / 8;
+  const int64_t all = V * chunks, step = static_cast<int64_t>(gridDim.x) * 256;
+  // (row and chunk are carried along: a division of 64 bits for every eight elements would cost more than moving them)
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / chunks;
+  int chunk = static_cast<int>(i - row * chunks);
+  const int64_t step_rows = step / chunks;
+  const int step_chunks = static_cast<int>(step - step_rows * chunks);
+#pragma unroll 4
+  for (; i < all; i += step) {
+    const int left = D - chunk * 8;
+    *reinterpret_cast<uint4*>(packed + row * pitch + chunk * 8) =
+        eight_elements(weight + row * stride + chunk * 8, left < 8 ? left : 8, first, end);
+    row += step_rows;
+    chunk += step_chunks;
+    if (chunk >= chunks) {
+      chunk -= chunks;
+      ++row;
     }
   }
 }
@@ -797,7 +833,7 @@ int fetchable_weight(const CeProblem& q, const MmaPlan& p, Weight* w, cudaStream
   DGS_REQUIRE(q.D % 8 != 0, DGS_ERR_INVALID, "linear_cross_entropy: rows of %lld 16-bit elements must begin at 16-byte boundaries",
               static_cast<long long>(q.D));
   uint16_t* packed = reinterpret_cast<uint16_t*>(q.ws + p.weight);
-  const int64_t need = tiles(q.V, 16), most = static_cast<int64_t>(sm_count()) * 8;
+  const int64_t need = tiles(q.V * (p.pitch / 8), 256), most = static_cast<int64_t>(sm_count()) * 8;
   DGS_CUDA_TRY(launch_training(ce_pack_weight_kernel, dim3(static_cast<unsigned>(need < most ? need : most)), 256, 0, s, w->p,
                                q.weight_stride, q.V, static_cast<int>(q.D), static_cast<int>(p.pitch), packed));
   *w = Weight{packed, p.pitch};
