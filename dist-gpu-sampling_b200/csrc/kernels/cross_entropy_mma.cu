@@ -80,11 +80,21 @@ inline bool two_planes(int64_t n, int64_t D, int64_t V) {
 // NARROW is STATS for no more than NARROW_COLS classes.  A tensor core cuts what it adds to an accumulator of 32 bits instead of
 // rounding it, which shows in the loss of few classes (1e-6 of it at 4 classes and rows of 1 000, where it hardly shows at 1 000
 // classes).  There the products stop every NARROW_K blocks of k and the parts are added in registers.
-enum Mode { STATS, GRAD, PRODUCT, NARROW };
+//
+// FEW_STATS and FEW_GRAD are STATS and GRAD for no more than FEW_ROWS rows, with the operands changed over: classes are the
+// accumulator's rows and the rows its 32 columns.  A lane works on its own class for eight rows; the other way round the few
+// lanes that have a row would pass over all classes (FEW_GAIN).  What is left is the reading of W.
+enum Mode { STATS, GRAD, PRODUCT, NARROW, FEW_STATS, FEW_GRAD };
 constexpr int NARROW_COLS = N_TILE / 2, NARROW_K = 4;
+constexpr int FEW_ROWS = 32, FEW_EACH = 8;  // rows; those that a warp works on
+constexpr int FEW_PARTS = 8;                // statistics of a row and slice: four warps in each CTA of the pair
+template <int MODE>
+constexpr bool is_few() {
+  return MODE == FEW_STATS || MODE == FEW_GRAD;
+}
 template <int MODE>
 constexpr bool is_stats() {
-  return MODE == STATS || MODE == NARROW;
+  return MODE == STATS || MODE == NARROW || MODE == FEW_STATS;
 }
 template <int MODE>
 constexpr int stages() {
@@ -92,7 +102,7 @@ constexpr int stages() {
 }
 template <int MODE>
 constexpr uint32_t smem_bytes() {  // alignment, stages, a staging buffer for each warp, barriers
-  return 1024 + stages<MODE>() * STAGE_BYTES + (is_stats<MODE>() ? 0 : EPILOGUE_WARPS * STAGING_BYTES) + 256;
+  return 1024 + stages<MODE>() * STAGE_BYTES + (is_stats<MODE>() || is_few<MODE>() ? 0 : EPILOGUE_WARPS * STAGING_BYTES) + 256;
 }
 
 enum OutKind { OUT_F32_STORE, OUT_F32_ADD, OUT_TYPED, OUT_TYPED_ODD };
@@ -130,7 +140,8 @@ struct alignas(64) MmaArgs {
   float* total;
   const float* dloss;
   const float* lse;
-  uint16_t* low;         // GRAD: the second plane of G, rows low_pitch elements apart; null: there is one plane
+  uint16_t* g;           // FEW_GRAD: G, rows low_pitch elements apart
+  uint16_t* low;         // (FEW_)GRAD: the second plane of G, rows low_pitch elements apart; null: there is one plane
   int64_t low_pitch;
   const float* largest;  // the largest |dloss| of each CTA that packed rows
   int32_t* status;
@@ -161,6 +172,10 @@ __device__ __forceinline__ Extent extent_of(const MmaArgs& a) {
     e.items = e.row_blocks * e.slices;
   } else if constexpr (MODE == NARROW) {
     e.items = e.row_blocks;
+  } else if constexpr (MODE == FEW_STATS) {
+    e.items = a.slices;
+  } else if constexpr (MODE == FEW_GRAD) {
+    e.items = a.col_tiles;
   } else if constexpr (MODE == GRAD) {
     e.items = e.row_blocks * a.col_tiles;
   } else {
@@ -193,6 +208,12 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const Extent& ext, int
     if (p.n_step < N_TILE || p.n_total - x.n0 <= N_TILE / 2) x.n = N_TILE / 2;
     x.k0 = static_cast<int32_t>(static_cast<int64_t>(k_blocks) * x.split / p.splits);
     x.k1 = static_cast<int32_t>(static_cast<int64_t>(k_blocks) * (x.split + 1) / p.splits);
+  } else if constexpr (is_few<MODE>()) {
+    x.n = FEW_ROWS;
+    x.m0 = t * M_TILE;  // classes
+    x.n0 = 0;
+    x.k0 = 0;
+    x.k1 = a.k_blocks;
   } else if constexpr (MODE == NARROW) {
     x.n = NARROW_COLS;
     x.m0 = item * M_TILE;
@@ -210,7 +231,13 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const Extent& ext, int
 // the column tiles (NARROW: runs along k) [t0, t1) of an item
 template <int MODE>
 __device__ __forceinline__ void range_of(const MmaArgs& a, const Extent& ext, int item, int* t0, int* t1) {
-  if constexpr (MODE == STATS) {
+  if constexpr (MODE == FEW_STATS) {
+    *t0 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * item / a.slices);
+    *t1 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * (item + 1) / a.slices);
+  } else if constexpr (MODE == FEW_GRAD) {
+    *t0 = item;
+    *t1 = item + 1;
+  } else if constexpr (MODE == STATS) {
     const int slice = item / ext.row_blocks;
     *t0 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * slice / ext.slices);
     *t1 = static_cast<int>(static_cast<int64_t>(a.col_tiles) * (slice + 1) / ext.slices);
@@ -344,7 +371,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
   extern __shared__ unsigned char smem_raw[];
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging = smem + STAGES * STAGE_BYTES;
-  const uint32_t words = staging + (is_stats<MODE>() ? 0 : EPILOGUE_WARPS * STAGING_BYTES);
+  const uint32_t words = staging + (is_stats<MODE>() || is_few<MODE>() ? 0 : EPILOGUE_WARPS * STAGING_BYTES);
   const uint32_t full = words, empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16, tmem_word = acc_empty + 16;
   volatile int32_t* dead = reinterpret_cast<volatile int32_t*>(smem_raw + (tmem_word + 8 - smem_addr(smem_raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -448,7 +475,99 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
         if (buf == 0) acc_phase ^= 1;
       }
     }
-  } else if (warp >= FIRST_EPILOGUE_WARP) {
+  } else if (is_few<MODE>() && warp >= FIRST_EPILOGUE_WARP) {
+    // ---- finished accumulators, classes by rows: a lane has one class of the tile, the warp eight rows
+    const int quarter = warp & 3, group = (warp - FIRST_EPILOGUE_WARP) >> 2, r0 = group * FEW_EACH;
+    const uint32_t from0 = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + r0;
+    const uint32_t free_bar = in_cta(acc_empty, 0);
+    int buf = 0;
+    uint32_t acc_phase = 0;
+    const float factor = MODE == FEW_GRAD ? grad_factor(a.largest, a.largest_count, lane, false) : 1.0f;
+    int32_t word[FEW_EACH];
+    float grad[FEW_EACH], lse[FEW_EACH];
+#pragma unroll
+    for (int r = 0; r < FEW_EACH; ++r) {
+      word[r] = -1;
+      grad[r] = lse[r] = 0.0f;
+      if (r0 + r < ext.rows) {
+        bool wrong;
+        word[r] = MODE == FEW_GRAD || a.word != nullptr ? a.word[r0 + r] : target_word(a.target, a.ids64, r0 + r, a.V, a.ignore_index, &wrong);
+        if (MODE == FEW_GRAD) {
+          grad[r] = a.dloss[r0 + r] * factor;
+          lse[r] = a.lse[r0 + r];
+        }
+      }
+    }
+    for (int item = pair; ok && item < ext.items; item += pairs) {
+      int t0, t1;
+      range_of<MODE>(a, ext, item, &t0, &t1);
+      float top[FEW_EACH], total[FEW_EACH];  // of this lane's classes
+#pragma unroll
+      for (int r = 0; r < FEW_EACH; ++r) top[r] = -INFINITY, total[r] = 0.0f;
+      for (int t = t0; t < t1; ++t) {
+        ok = !*dead && bar_wait(acc_full + 8 * buf, acc_phase);
+        ok = __all_sync(FULL_MASK, ok);
+        if (!ok) break;
+        fence_after();
+        uint32_t bits[FEW_EACH];
+        tmem_read8(from0 + buf * N_TILE, bits);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive_in(free_bar + 8 * buf);
+        buf ^= 1;
+        if (buf == 0) acc_phase ^= 1;
+        const int32_t c = t * M_TILE + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;  // FEW_GRAD: of the piece
+        if (c >= a.V) continue;
+#pragma unroll
+        for (int r = 0; r < FEW_EACH; ++r) {
+          if (r0 + r >= a.n) break;  // (the same for all lanes)
+          const float v = __uint_as_float(bits[r]);
+          if constexpr (MODE == FEW_STATS) {
+            if (c == word[r]) a.target_logit[r0 + r] = v;
+            const float d = v - top[r], e = ex2(-fabsf(d) * LOG2E);
+            if (v > top[r]) {
+              total[r] = total[r] * e + 1.0f;  // (0 * 0 + 1 for the first)
+              top[r] = v;
+            } else if (v != -INFINITY) {
+              total[r] += e;  // (a NaN goes this way and stays)
+            }
+          } else {
+            float g = 0.0f;
+            if (word[r] >= 0) {
+              g = ex2((v - lse[r]) * LOG2E);
+              if (c + a.v0 == word[r]) g -= 1.0f;
+              g *= grad[r];
+            }
+            const uint32_t hi = pack2<BF16>(g, 0.0f);
+            const int64_t at = static_cast<int64_t>(r0 + r) * a.low_pitch + c;
+            a.g[at] = static_cast<uint16_t>(hi);
+            if (a.low != nullptr) {
+              float back, none;
+              unpack2<BF16>(hi, &back, &none);
+              a.low[at] = static_cast<uint16_t>(pack2<BF16>(g - back, 0.0f));
+            }
+          }
+        }
+      }
+      if (MODE == FEW_STATS && ok) {
+        // one pair for the warp's lanes, in an order that is always the same
+#pragma unroll
+        for (int r = 0; r < FEW_EACH; ++r) {
+          float m = top[r];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
+          float s = m == -INFINITY ? total[r] : total[r] * ex2((top[r] - m) * LOG2E);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL_MASK, s, o);
+          if (lane == 0 && r0 + r < ext.rows) {
+            const int64_t at = (static_cast<int64_t>(r0 + r) * a.slices + item) * FEW_PARTS + static_cast<int64_t>(rank) * 4 + quarter;
+            a.top[at] = m;
+            a.total[at] = s;
+          }
+        }
+      }
+    }
+  } else if (!is_few<MODE>() && warp >= FIRST_EPILOGUE_WARP) {
     // ---- finished accumulators: a warp reads the 32 lanes (rows) that its number allows, and a quarter of the columns
     constexpr int COLS = MODE == NARROW ? NARROW_COLS / COL_GROUPS : GROUP_COLS;
     const int quarter = warp & 3, group = (warp - FIRST_EPILOGUE_WARP) >> 2, c0 = group * COLS;
@@ -712,7 +831,7 @@ struct MmaPlan {
   int64_t pitch, row_blocks, col_tiles, slices, pairs;
   int64_t piece, splits, dpitch;
   int64_t planes;  // of G
-  bool one_piece, compact, dh_first;
+  bool one_piece, compact, dh_first, few;
   size_t packed, word, slot, live, counts, weight, target_logit, top, total, dloss, lse, largest, g, dh;
   size_t forward_bytes, backward_bytes;
 };
@@ -757,7 +876,8 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.pitch = up(D, 8);
   p.row_blocks = tiles(n, M_TILE);
   p.col_tiles = tiles(V, N_TILE);
-  p.slices = slices_for(p.row_blocks, p.col_tiles, p.pairs);
+  p.few = n <= FEW_ROWS && V > NARROW_COLS;
+  p.slices = !p.few ? slices_for(p.row_blocks, p.col_tiles, p.pairs) : p.col_tiles < p.pairs ? p.col_tiles : p.pairs;
   // as many column tiles as PIECE_BYTES allow, rounded down to full rounds of the GRAD launch
   p.planes = two_planes(n, D, V) ? 2 : 1;
   int64_t piece_tiles = PIECE_BYTES / 2 / (p.planes * n) / N_TILE;
@@ -787,9 +907,9 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.target_logit = l.take(n * 4);
   // (compact: the number of slices follows the number of rows, which is not known here; but blocks * slices <= kMostRounds * pairs
   // unless there is one slice)
-  const int64_t most = p.compact ? n + kMostRounds * p.pairs * M_TILE : n * p.slices;
-  p.top = l.take(COL_GROUPS * most * 4);
-  p.total = l.take(COL_GROUPS * most * 4);
+  const int64_t most = p.few ? n * p.slices * FEW_PARTS : (p.compact ? n + kMostRounds * p.pairs * M_TILE : n * p.slices) * COL_GROUPS;
+  p.top = l.take(most * 4);
+  p.total = l.take(most * 4);
   p.forward_bytes = l.bytes;
   l = common;
   p.dloss = l.take(n * 4);
@@ -873,11 +993,12 @@ int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) 
   Weight w;
   if (int rc = fetchable_weight(q, p, &w, s)) return rc;
   MmaArgs a{};
-  if (int rc = make_map(&a.a[0], where_they_lie ? q.hidden : r.rows, q.dtype, q.D, q.n,
-                        where_they_lie ? (q.n == 1 ? q.D : q.hidden_stride) : p.pitch, K_TILE, M_CTA))
+  const bool narrow = !p.few && q.V <= NARROW_COLS;
+  const void* rows = where_they_lie ? q.hidden : r.rows;
+  const int64_t pitch = !where_they_lie ? p.pitch : q.n == 1 ? q.D : q.hidden_stride;
+  if (int rc = make_map(p.few ? &a.b[0] : &a.a[0], rows, q.dtype, q.D, q.n, pitch, K_TILE, p.few ? FEW_ROWS / 2 : M_CTA)) return rc;
+  if (int rc = make_map(p.few ? &a.a[0] : &a.b[0], w.p, q.dtype, q.D, q.V, w.stride, K_TILE, p.few ? M_CTA : narrow ? NARROW_COLS / 2 : N_TILE / 2))
     return rc;
-  const bool narrow = q.V <= NARROW_COLS;
-  if (int rc = make_map(&a.b[0], w.p, q.dtype, q.D, q.V, w.stride, K_TILE, narrow ? NARROW_COLS / 2 : N_TILE / 2)) return rc;
   a.items = static_cast<int32_t>(p.row_blocks * p.slices);
   a.col_tiles = static_cast<int32_t>(p.col_tiles);
   a.slices = static_cast<int32_t>(p.slices);
@@ -893,8 +1014,11 @@ int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) 
   a.top = reinterpret_cast<float*>(q.ws + p.top);
   a.total = reinterpret_cast<float*>(q.ws + p.total);
   a.status = q.status;
-  if (int rc = narrow ? launch<NARROW>(a, p.pairs, q.dtype, s) : launch<STATS>(a, p.pairs, q.dtype, s)) return rc;
-  return ce_join(q, a.top, a.total, COL_GROUPS, p.slices, r.live, a.word, r.slot, a.target_logit, loss, lse, s);
+  if (int rc = p.few    ? launch<FEW_STATS>(a, p.pairs, q.dtype, s)
+               : narrow ? launch<NARROW>(a, p.pairs, q.dtype, s)
+                        : launch<STATS>(a, p.pairs, q.dtype, s))
+    return rc;
+  return ce_join(q, a.top, a.total, p.few ? FEW_PARTS : COL_GROUPS, p.slices, p.few ? nullptr : r.live, a.word, r.slot, a.target_logit, loss, lse, s);
 }
 
 int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, void* dhidden, void* dweight, cudaStream_t s) {
@@ -915,11 +1039,12 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     const int64_t width = q.V - v0 < p.piece ? q.V - v0 : p.piece;
     const uint16_t* wp = w.p + v0 * w.stride;
     MmaArgs a{};
-    if (int rc = make_map(&a.a[0], packed, q.dtype, q.D, q.n, p.pitch, K_TILE, M_CTA)) return rc;
-    if (int rc = make_map(&a.b[0], wp, q.dtype, q.D, width, w.stride, K_TILE, N_TILE / 2)) return rc;
+    if (int rc = make_map(p.few ? &a.b[0] : &a.a[0], packed, q.dtype, q.D, q.n, p.pitch, K_TILE, p.few ? FEW_ROWS / 2 : M_CTA)) return rc;
+    if (int rc = make_map(p.few ? &a.a[0] : &a.b[0], wp, q.dtype, q.D, width, w.stride, K_TILE, p.few ? M_CTA : N_TILE / 2)) return rc;
     if (int rc = make_map(&a.out[0], g, q.dtype, width, q.n, p.piece, 64, 32)) return rc;
     a.low = p.planes == 2 ? g + q.n * p.piece : nullptr;
     a.low_pitch = p.piece;
+    a.g = g;
     a.col_tiles = static_cast<int32_t>(tiles(width, N_TILE));
     a.items = static_cast<int32_t>(p.row_blocks) * a.col_tiles;
     a.k_blocks = static_cast<int32_t>(tiles(q.D, K_TILE));
@@ -933,7 +1058,7 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     a.largest = r.largest;
     a.largest_count = static_cast<int32_t>(ce_pack_ctas(q.n));
     a.status = q.status;
-    if (int rc = launch<GRAD>(a, p.pairs, q.dtype, s)) return rc;
+    if (int rc = p.few ? launch<FEW_GRAD>(a, p.pairs, q.dtype, s) : launch<GRAD>(a, p.pairs, q.dtype, s)) return rc;
 
     MmaArgs m{};
     // half as wide tiles where that gives more pairs something to do (1 024 rows of 256 against 172 classes: 5 tiles of 256)
