@@ -373,19 +373,21 @@ __global__ void __launch_bounds__(CE_THREADS) ce_join_kernel(const __grid_consta
   const int64_t parts = a.groups * (a.live != nullptr ? a.live[1] : a.slices);
   const float *top = a.top + c * parts, *total = a.total + c * parts;
   float m = -INFINITY, s = 0.0f;
-  for (int64_t p0 = lane; p0 < parts; p0 += 128) {
-    float t[4], e[4];
+  constexpr int U = 8;  // parts under way a lane
+  for (int64_t p0 = lane; p0 < parts; p0 += 32 * U) {
+    float t[U], e[U], now = m;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < U; ++k) {
       const bool in = p0 + 32 * k < parts;
       t[k] = in ? top[p0 + 32 * k] : -INFINITY;
       e[k] = in ? total[p0 + 32 * k] : 0.0f;
     }
-    const float now = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), m);
+#pragma unroll
+    for (int k = 0; k < U; ++k) now = fmaxf(now, t[k]);
     const float base = now == -INFINITY ? 0.0f : now;
     s *= expf(m - base);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s += e[k] * expf(t[k] - base);
+    for (int k = 0; k < U; ++k) s += e[k] * expf(t[k] - base);
     m = now;
   }
   float all = m;
@@ -470,35 +472,37 @@ __global__ void __launch_bounds__(CE_THREADS) ce_sum_kernel(const float* __restr
                                                             const int32_t* __restrict__ slot, const bool vectors, const bool fours,
                                                             T* __restrict__ out) {
   pdl_enter();
-  const int lane = threadIdx.x & 31;
-  for (int64_t row = blockIdx.x * static_cast<int64_t>(CE_THREADS / 32) + (threadIdx.x >> 5); row < n;
-       row += gridDim.x * static_cast<int64_t>(CE_THREADS / 32)) {
+  const int lane = threadIdx.x & 31, chunks = (D + 127) / 128;
+  // a warp takes 128 columns of a row
+  for (int64_t w = blockIdx.x * static_cast<int64_t>(CE_THREADS / 32) + (threadIdx.x >> 5); w < n * chunks;
+       w += gridDim.x * static_cast<int64_t>(CE_THREADS / 32)) {
+    const int64_t row = w / chunks;
+    const int j = static_cast<int>(w - row * chunks) * 128 + lane * 4;
+    if (j >= D) continue;
     const int64_t c = slot != nullptr ? slot[row] : row;
-    const float* p = parts + c * pitch;
-    T* to = out + row * D;
-    for (int j = lane * 4; j < D; j += 128) {
-      float v[4] = {};
-      if (c >= 0) {
-#pragma unroll 4
-        for (int64_t k = 0; k < splits; ++k) {
-          float t[4];
-          if (vectors) {
-            load_vec<float, 4>(p + k * split_elems + j, t);
-          } else {
+    const float* p = parts + c * pitch + j;
+    T* to = out + row * D + j;
+    float v[4] = {};
+    if (c >= 0) {
+#pragma unroll 8
+      for (int64_t k = 0; k < splits; ++k) {
+        float t[4];
+        if (vectors) {
+          load_vec<float, 4>(p + k * split_elems, t);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = j + i < D ? p[k * split_elems + j + i] : 0.0f;
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] += t[i];
+          for (int i = 0; i < 4; ++i) t[i] = j + i < D ? p[k * split_elems + i] : 0.0f;
         }
-      }
-      if (fours) {
-        store_vec<T, 4>(to + j, v);
-      } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (j + i < D) to[j + i] = from_float<T>(v[i]);
+        for (int i = 0; i < 4; ++i) v[i] += t[i];
       }
+    }
+    if (fours) {
+      store_vec<T, 4>(to, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i < D) to[i] = from_float<T>(v[i]);
     }
   }
 }
@@ -627,7 +631,7 @@ int ce_join(const CeProblem& q, const float* top, const float* total, int64_t gr
 
 int ce_sum(const float* parts, int64_t splits, int64_t n, int64_t D, int64_t rows, int64_t pitch, const int32_t* slot, void* out,
            int32_t dtype, cudaStream_t s) {
-  const int64_t need = tiles(n, CE_THREADS / 32), most = static_cast<int64_t>(sm_count()) * 16;
+  const int64_t need = tiles(n * tiles(D, 128), CE_THREADS / 32), most = static_cast<int64_t>(sm_count()) * 16;
   const dim3 grid(static_cast<unsigned>(need < most ? need : most));
   const int d = static_cast<int>(D), pt = static_cast<int>(pitch);
   const bool vectors = pitch % 4 == 0, fours = vectors && D % 4 == 0 && aligned_to(out, 16);

@@ -83,7 +83,8 @@ inline bool two_planes(int64_t n, int64_t D, int64_t V) {
 //
 // FEW_STATS and FEW_GRAD are STATS and GRAD for no more than FEW_ROWS rows, with the operands changed over: classes are the
 // accumulator's rows and the rows its 32 columns.  A lane works on its own class for eight rows; the other way round the few
-// lanes that have a row would pass over all classes (FEW_GAIN).  What is left is the reading of W.
+// lanes that have a row would pass over all classes (8 rows of 203 against 800 000 classes, forward: 249 us, so 188).  What is left
+// is the reading of W.
 enum Mode { STATS, GRAD, PRODUCT, NARROW, FEW_STATS, FEW_GRAD };
 constexpr int NARROW_COLS = N_TILE / 2, NARROW_K = 4;
 constexpr int FEW_ROWS = 32, FEW_EACH = 8;  // rows; those that a warp works on
