@@ -6,7 +6,8 @@ The product is two shared libraries built in-tree by `build.py`:
   lib/libdgs.so        torch.classes.dgs_classes.ChunkTensor + torch.ops.dgs_ops.*
 
 This module only loads them and mirrors the small Python glue of the reference
-(communicator bootstrap, ChunkTensor creation, the sample_blocks loop).  There
+(communicator bootstrap, ChunkTensor creation, the sample_blocks loop); training.py
+holds the operators of a training step on what the samplers deliver.  There
 is no CPU fallback: if the libraries are missing, loading raises.
 
 (The directory name contains a hyphen; import it with

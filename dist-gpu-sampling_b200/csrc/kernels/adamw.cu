@@ -3,10 +3,12 @@
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
 //   p = (1 - lr wd) p - (m / (sqrt(v) / sqrt(1 - b2^t) + eps)) (lr / (1 - b1^t)),  copy = p in the copy's type
 //
-// Every element is read and written once: bound by HBM.  The moments lie in flat buffers in which every tensor has a slot
-// of whole 256-element blocks, so a warp's 256 elements are one block of the 8-bit form and the list needs three pointers
-// a tensor.  The list travels in the kernel's parameters (nothing is copied to the device and nothing is kept), a CTA finds
-// its tensor by bisecting the list's chunk numbers.
+// Every element is read and written once: bound by HBM with moments in 32 bits (313 M parameters, gradients and copies in 16 bits:
+// 1.44 ms, 6.1 TB/s), by issue slots in 8 bits (60 M parameters: 244 us, 3.9 TB/s, some hundred instructions an element).
+//
+// The moments lie in flat buffers in which every tensor has a slot of whole 256-element blocks, so a warp's 256 elements are one
+// block of the 8-bit form and the list needs three pointers a tensor.  The list travels in the kernel's parameters (nothing is
+// copied to the device and nothing is kept), a CTA finds its tensor by bisecting the list's chunk numbers.
 //
 // 8 bits, per block: m = a sgn(c) (c / 127)^2 with a = max |m|, and sqrt(v) = a (c / 255)^2 with a = max sqrt(v).  The
 // squares give small values finer steps; the second moment is held as its root because that is what divides, and a root

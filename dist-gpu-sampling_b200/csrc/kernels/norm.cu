@@ -3,7 +3,8 @@
 //   mean_i = avg_j x_ij,  rstd_i = 1 / sqrt(avg_j (x_ij - mean_i)^2 + eps),  h_ij = (x_ij - mean_i) rstd_i,  y = h w + b
 //   g = dy w,  dx_ij = rstd_i (g_ij - avg_j g_ij - h_ij avg_j (g_ij h_ij)),  dw_j = sum_i dy_ij h_ij,  db_j = sum_i dy_ij
 //
-// Both directions read every element once and are bound by HBM.  A row stays in the registers of the threads that share
+// Both directions read every element once and are bound by HBM: 430 000 x 100 float32 57 us forward and 80 us backward (6.0 and
+// 6.4 TB/s), 16 384 x 4 096 bfloat16 46 and 78 us (5.8 and 5.2 TB/s; two sums over the CTA stand between a row's loads and stores).  A row stays in the registers of the threads that share
 // it between its passes (mean, centred squares, result), so the variance is that of the centred values and does not
 // cancel.  All sums are in 32 bits.
 //   - TPR threads share a row, NV vectors of VEC elements each: 4 to 32 threads of a warp (shuffles alone), or a CTA of 256
