@@ -107,9 +107,22 @@ template <int MODE>
 constexpr int stages() {
   return is_stats<MODE>() ? 6 : 5;
 }
+// Where a row block meets all classes in one go, its CTAs join the four column groups' statistics themselves, by way of shared
+// memory; JOINS of them, so that a warp that is ahead does not write over what another still reads (the accumulators let none be
+// more than two tiles ahead).
+constexpr int JOINS = 4;
+struct JoinRows {
+  float2 sum[COL_GROUPS][M_CTA];  // (maximum, sum)
+  float target[M_CTA];
+};
+template <int MODE>
+constexpr bool may_join() {
+  return MODE == STATS || MODE == NARROW;
+}
 template <int MODE>
 constexpr uint32_t smem_bytes() {  // alignment, stages, a staging buffer for each warp, barriers
-  return 1024 + stages<MODE>() * STAGE_BYTES + (is_stats<MODE>() || is_few<MODE>() ? 0 : EPILOGUE_WARPS * STAGING_BYTES) + 256;
+  return 1024 + stages<MODE>() * STAGE_BYTES + (is_stats<MODE>() || is_few<MODE>() ? 0 : EPILOGUE_WARPS * STAGING_BYTES) + 256 +
+         (may_join<MODE>() ? JOINS * static_cast<uint32_t>(sizeof(JoinRows)) : 0);
 }
 
 enum OutKind { OUT_F32_STORE, OUT_F32_ADD, OUT_TYPED, OUT_TYPED_ODD };
@@ -145,6 +158,7 @@ struct alignas(64) MmaArgs {
   float* target_logit;
   float* top;
   float* total;
+  float *loss_out, *lse_out;  // STATS, NARROW: the rows' results, where there is one slice and rows are those of the call; else null
   const float* dloss;
   const float* lse;
   uint16_t* g;           // FEW_GRAD: G, rows low_pitch elements apart
@@ -381,6 +395,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
   const uint32_t words = staging + (is_stats<MODE>() || is_few<MODE>() ? 0 : EPILOGUE_WARPS * STAGING_BYTES);
   const uint32_t full = words, empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16, tmem_word = acc_empty + 16;
   volatile int32_t* dead = reinterpret_cast<volatile int32_t*>(smem_raw + (tmem_word + 8 - smem_addr(smem_raw)));
+  const uint32_t joined = tmem_word + 16;  // a barrier for each of JOINS
+  JoinRows* join_rows = reinterpret_cast<JoinRows*>(smem_raw + (words + 256 - smem_addr(smem_raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -394,6 +410,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
       bar_init(acc_full + 8 * i, 1);
       bar_init(acc_empty + 8 * i, 2 * EPILOGUE_WARPS);
     }
+    for (int i = 0; i < JOINS; ++i) bar_init(joined + 8 * i, EPILOGUE_WARPS);
     *dead = 0;
     bar_init_fence();
   }
@@ -601,7 +618,10 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
       }
     };
     if (MODE != PRODUCT) ask(pair);
-    for (int item = pair; ok && item < ext.items; item += pairs) {
+    int round = 0;  // items so far
+    for (int item = pair; ok && item < ext.items; item += pairs, ++round) {
+      JoinRows* join = may_join<MODE>() && a.loss_out != nullptr ? join_rows + round % JOINS : nullptr;
+      const int in_cta_row = quarter * 32 + lane;
       int t0, t1;
       range_of<MODE>(a, ext, item, &t0, &t1);
       RowSum sum;
@@ -637,13 +657,13 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
                 logits[i] = t == t0 ? now[i] : __float_as_uint(__uint_as_float(logits[i]) + __uint_as_float(now[i]));
               if (t + 1 == t1) {
                 const uint32_t at = static_cast<uint32_t>(word - col);
-                if (at < 32u && word >= 0) a.target_logit[row] = pick(logits, static_cast<int>(at));
+                if (at < 32u && word >= 0) *(join ? &join->target[in_cta_row] : &a.target_logit[row]) = pick(logits, static_cast<int>(at));
                 if (col < a.V) sum.add(logits, static_cast<int32_t>(a.V) - col);
               }
             } else if constexpr (MODE == STATS) {
               const int32_t left = static_cast<int32_t>(a.V) - col;
               const uint32_t at = static_cast<uint32_t>(word - col);
-              if (at < 32u && word >= 0) a.target_logit[row] = pick(now, static_cast<int>(at));
+              if (at < 32u && word >= 0) *(join ? &join->target[in_cta_row] : &a.target_logit[row]) = pick(now, static_cast<int>(at));
               if (left > 0) sum.add(now, left);
             } else if constexpr (MODE == GRAD) {
               if (!far(lse)) {  // (then no logit is a NaN)
@@ -746,7 +766,31 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
         buf ^= 1;
         if (buf == 0) acc_phase ^= 1;
       }
-      if (is_stats<MODE>() && ok) {
+      if (may_join<MODE>() && ok && join != nullptr) {
+        join->sum[group][in_cta_row] = float2{sum.top, sum.total};
+        __syncwarp();
+        if (lane == 0) bar_arrive(joined + 8 * (round % JOINS));
+        if (group == 0) {
+          ok = !*dead && bar_wait(joined + 8 * (round % JOINS), (round / JOINS) & 1);
+          ok = __all_sync(FULL_MASK, ok);
+          if (!ok) break;
+          const int32_t row = item * M_TILE + my_row;
+          float m = -INFINITY, s = 0.0f;
+#pragma unroll
+          for (int g = 0; g < COL_GROUPS; ++g) m = fmaxf(m, join->sum[g][in_cta_row].x);
+          const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int g = 0; g < COL_GROUPS; ++g) s += join->sum[g][in_cta_row].y * expf(join->sum[g][in_cta_row].x - base);
+          if (row < ext.rows) {
+            bool wrong = false;
+            if (a.word == nullptr) target_word(a.target, a.ids64, row, a.V, a.ignore_index, &wrong);
+            if (wrong) raise_status(a.status, DGS_ERR_RANGE);
+            const float l = logf(s);
+            a.lse_out[row] = word >= 0 ? base + l : 0.0f;
+            a.loss_out[row] = word >= 0 ? (base - join->target[in_cta_row]) + l : 0.0f;
+          }
+        }
+      } else if (is_stats<MODE>() && ok) {
         const int32_t row = item % ext.row_blocks * M_TILE + static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
         const int64_t at = static_cast<int64_t>(row) * (ext.slices * COL_GROUPS) + item / ext.row_blocks * COL_GROUPS + group;
         if (row < ext.rows) {
@@ -1021,10 +1065,16 @@ int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) 
   a.top = reinterpret_cast<float*>(q.ws + p.top);
   a.total = reinterpret_cast<float*>(q.ws + p.total);
   a.status = q.status;
+  const bool join_there = p.slices == 1 && !p.compact && !p.few;
+  if (join_there) {
+    a.loss_out = loss;
+    a.lse_out = lse;
+  }
   if (int rc = p.few    ? launch<FEW_STATS>(a, p.pairs, q.dtype, s)
                : narrow ? launch<NARROW>(a, p.pairs, q.dtype, s)
                         : launch<STATS>(a, p.pairs, q.dtype, s))
     return rc;
+  if (join_there) return DGS_OK;
   return ce_join(q, a.top, a.total, p.few ? FEW_PARTS : COL_GROUPS, p.slices, p.few ? nullptr : r.live, a.word, r.slot, a.target_logit, loss, lse, s);
 }
 

@@ -39,6 +39,9 @@ __device__ __forceinline__ void bar_init_fence() { asm volatile("fence.mbarrier_
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void bar_arrive_in(uint32_t cluster_bar) {
   // (what it orders are accesses to TMEM, by the tcgen05 fences around it: a release at the cluster's scope would wait for
   // this thread's ordinary stores as well)
