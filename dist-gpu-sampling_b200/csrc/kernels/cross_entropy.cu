@@ -5,15 +5,16 @@
 //
 // Forward: a block of rows meets the vocabulary tile by tile; each row carries a running maximum and a running sum of
 // exponentials, so a tile of logits lives in registers only.  The vocabulary is cut into slices where there are fewer row
-// blocks than SMs; a last launch joins the slices' (maximum, sum) pairs in their order.
+// blocks than SMs; a last launch joins the slices' (maximum, sum) pairs in their order (16-bit operands whose row blocks meet
+// all classes at once join theirs on the spot).
 // Backward: the vocabulary is taken in pieces.  Per piece the logits are computed again, leave as G into a buffer of 96 MB
 // (256 MB in 16 bits), and two products read it: dh grows in 32 bits over the pieces, dW's rows of the piece are
 // complete.  That is 8 n V D operations for a training step instead of 6 with the logits kept (n V values, 2.1 GB at
 // 8 192 rows and 65 537 classes).
 //
 // This file: the entry points, the launches around the products, and the products of 32-bit operands on the CUDA cores (fused
-// multiply-adds in 32 bits, which the tensor cores do not have): bound by their rate, 34 TFLOP/s at 4 096 rows of 256 against
-// 30 000 classes.  16-bit operands: cross_entropy_mma.cu.
+// multiply-adds in 32 bits, which the tensor cores do not have): bound by their rate, 33 TFLOP/s forward and 26 backward at
+// 4 096 rows of 256 against 30 000 classes (a library product of those sizes: 56).  16-bit operands: cross_entropy_mma.cu.
 //
 // A first launch copies the hidden rows into packed rows and the targets into 32-bit words: rows without a valid target
 // become zero there, so that what stands in an ignored row (an infinity, say) reaches neither dh nor dW, and alignment

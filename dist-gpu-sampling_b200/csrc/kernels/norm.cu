@@ -4,14 +4,14 @@
 //   g = dy w,  dx_ij = rstd_i (g_ij - avg_j g_ij - h_ij avg_j (g_ij h_ij)),  dw_j = sum_i dy_ij h_ij,  db_j = sum_i dy_ij
 //
 // Both directions read every element once and are bound by HBM: 430 000 x 100 float32 57 us forward and 80 us backward (6.0 and
-// 6.4 TB/s), 16 384 x 4 096 bfloat16 46 and 78 us (5.8 and 5.2 TB/s; two sums over the CTA stand between a row's loads and stores).  A row stays in the registers of the threads that share
-// it between its passes (mean, centred squares, result), so the variance is that of the centred values and does not
-// cancel.  All sums are in 32 bits.
+// 6.4 TB/s), 16 384 x 4 096 bfloat16 46 and 78 us (5.8 and 5.2 TB/s; two sums over the CTA stand between a row's loads and
+// stores).  A row stays in the registers of the threads that share it between its passes (mean, centred squares, result), so
+// the variance is that of the centred values and does not cancel.  All sums are in 32 bits.
 //   - TPR threads share a row, NV vectors of VEC elements each: 4 to 32 threads of a warp (shuffles alone), or a CTA of 256
 //     or 512 for rows beyond a warp's registers; rows that no variant holds go through kernels that read them again.
 //   - Backward: a thread keeps the same columns for all rows of its CTA, so the column sums grow in its registers; each
-//     CTA writes one partial row and a second launch adds the partial rows in their order.  No atomics: the same inputs
-//     give the same bits.
+//     CTA writes one partial row and a second launch adds the partial rows in their order; rows that one cluster takes at
+//     once are added out of its CTAs' shared memory instead.  No atomics: the same inputs give the same bits.
 #include "train_common.cuh"
 
 namespace dgs {
@@ -327,8 +327,22 @@ struct NormBackArgs {
   int64_t n;
   int D;
   void* dx;        // may be null
-  float* partial;  // [CTAs][2][D], or null when the parameters' gradients are not wanted
+  float* partial;  // [CTAs][2][D], or null when the parameters' gradients are not wanted or are made here
+  // few CTAs: one cluster, whose CTAs add their column sums out of one another's shared memory
+  void *dweight, *dbias;
+  int32_t ctas;
 };
+
+__device__ __forceinline__ float shared_of(uint32_t addr, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
 
 template <typename T, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(threads_of<TPR>(), VEC * NV <= 16 ? 512 / threads_of<TPR>() : 1) norm_backward_kernel(const __grid_constant__ NormBackArgs a) {
@@ -441,8 +455,13 @@ __global__ void __launch_bounds__(threads_of<TPR>(), VEC * NV <= 16 ? 512 / thre
       }
     }
   }
-  if (a.partial == nullptr) return;
-  float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.D;
+  const bool together = a.dweight != nullptr;
+  if (a.partial == nullptr && !together) return;
+  if (together) {  // the ring becomes this CTA's column sums
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+  }
+  float* out = together ? reinterpret_cast<float*>(ring) : a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.D;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = t + k * TPR;
@@ -466,6 +485,17 @@ __global__ void __launch_bounds__(threads_of<TPR>(), VEC * NV <= 16 ? 512 / thre
         for (int i = 0; i < VEC; ++i) out[half * a.D + c * VEC + i] = mine[i];
       }
     }
+  }
+  if (together) {
+    cluster_barrier();
+    const uint32_t sums = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+    for (int j = blockIdx.x * threads_of<TPR>() + threadIdx.x; j < 2 * a.D; j += a.ctas * threads_of<TPR>()) {
+      float v = 0.0f;
+      for (int c = 0; c < a.ctas; ++c) v += shared_of(sums + j * 4, c);
+      if (j < a.D) store_from_float(a.dweight, a.param_dtype, j, v);
+      else store_from_float(a.dbias, a.param_dtype, j - a.D, v);
+    }
+    cluster_barrier();  // nobody leaves while its sums are read
   }
 }
 
@@ -591,6 +621,12 @@ inline int64_t ctas_for(int64_t n, int rows, int per_sm) {
 
 constexpr int LN_CTAS_PER_SM = 4;  // backward, at most: each CTA writes a partial row of its own
 
+// Backward, rows that a cluster of eight CTAs takes at once: one launch and no partial sums in memory, 11.4 -> 9.1 us a call and
+// in a graph 4.7 -> 4.4 (64 rows of 256 floats), 7.2 -> 6.9 (64 of 1 024 bf16). Rows for four such rounds are slower there
+// (473 rows of 236 bf16 6.1 -> 9.1 us, 512 of 256 floats 4.9 -> 6.3): they keep the grid and the second launch.
+constexpr int LN_CLUSTER = 8;
+constexpr int64_t LN_CLUSTER_COLUMNS = 4096;  // whose sums, 32 KB, need no leave beside the static arrays
+
 // CTAs of a kernel that an SM holds at once, asked for once per kernel and device, and its leave to use `smem` bytes
 constexpr int LN_MAX_DEVICES = 64;
 template <typename K>
@@ -600,7 +636,9 @@ int resident(K kernel, int threads, size_t smem, std::atomic<int> (&known)[LN_MA
   DGS_REQUIRE(dev >= 0 && dev < LN_MAX_DEVICES, DGS_ERR_UNSUPPORTED, "layer_norm: device ordinal %d", dev);
   *held = known[dev].load(std::memory_order_acquire);
   if (*held == 0) {
-    if (smem > 0) DGS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    // (what every kernel may have holds for the rest, and for the column sums of a cluster)
+    if (smem > LN_CLUSTER_COLUMNS * 2 * sizeof(float))
+      DGS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     DGS_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(held, kernel, threads, smem));
     if (*held < 1) *held = 1;
     known[dev].store(*held, std::memory_order_release);
@@ -691,9 +729,10 @@ int forward(const NormArgs& a, cudaStream_t s) {
 template <typename T>
 struct Backward {
   static constexpr bool kBackward = true;
-  const NormBackArgs& a;
+  NormBackArgs a;
   cudaStream_t s;
   int64_t* partials;
+  void *dweight, *dbias;
   template <int VEC, int TPR, int NV>
   int run() const {
     static std::atomic<int> known[LN_MAX_DEVICES] = {};
@@ -701,6 +740,20 @@ struct Backward {
     constexpr size_t smem = ring_bytes<T, VEC, TPR, NV, R, 2>();
     constexpr int threads = threads_of<TPR>();
     auto kernel = norm_backward_kernel<T, VEC, TPR, NV>;
+    constexpr int64_t rows = threads / TPR * R;
+    if (dweight != nullptr && a.n <= rows * LN_CLUSTER && a.D <= LN_CLUSTER_COLUMNS) {
+      NormBackArgs b = a;
+      b.partial = nullptr;
+      b.dweight = dweight;
+      b.dbias = dbias;
+      b.ctas = static_cast<int32_t>((a.n + rows - 1) / rows);
+      const size_t sums = 2 * static_cast<size_t>(a.D) * sizeof(float), bytes = smem > sums ? smem : sums;
+      int held = 0;
+      if (int rc = resident(kernel, threads, smem, known, &held)) return rc;
+      *partials = 0;
+      DGS_CUDA_TRY(launch_clusters(kernel, dim3(static_cast<unsigned>(b.ctas)), threads, bytes, s, static_cast<unsigned>(b.ctas), b));
+      return DGS_OK;
+    }
     int held = 0;
     if (int rc = resident(kernel, threads, smem, known, &held)) return rc;
     *partials = ctas_for(a.n, threads / TPR * R, held < LN_CTAS_PER_SM ? held : LN_CTAS_PER_SM);
@@ -720,11 +773,11 @@ struct Backward {
 };
 
 template <typename T>
-int backward(const NormBackArgs& a, int64_t* partials, cudaStream_t s) {
+int backward(const NormBackArgs& a, int64_t* partials, void* dweight, void* dbias, cudaStream_t s) {
   constexpr int VEC = full_vec<T>();
   const bool whole = a.D % VEC == 0 && a.x_stride % VEC == 0 && a.dy_stride % VEC == 0 && aligned_to(a.x, 16) &&
                      aligned_to(a.dy, 16) && aligned_to(a.dx, 16) && aligned_to(a.weight, 16);
-  const Backward<T> f{a, s, partials};
+  const Backward<T> f{a, s, partials, dweight, dbias};
   if (whole) return with_shape<VEC>(shape_for(a.D / VEC, VEC, most_vectors<VEC, true>()), f);
   return with_shape<1>(shape_for(a.D, 1, most_vectors<1, true>()), f);
 }
@@ -790,13 +843,24 @@ extern "C" int dgs_layer_norm_backward(const void* dy, int64_t dy_stride, const 
   const size_t need = dgs_layer_norm_backward_workspace_bytes(n, D);
   DGS_REQUIRE(dweight == nullptr || (workspace != nullptr && workspace_bytes >= need && aligned_to(workspace, 16)), DGS_ERR_INVALID,
               "layer_norm_backward: workspace of %zu bytes, 16-byte aligned, is needed", need);
-  const NormBackArgs a{dy,   dy_stride, x, x_stride,            weight, param_dtype,
-                       mean, rstd,      n, static_cast<int>(D), dx,     dweight != nullptr ? static_cast<float*>(workspace) : nullptr};
+  NormBackArgs a{};
+  a.dy = dy;
+  a.dy_stride = dy_stride;
+  a.x = x;
+  a.x_stride = x_stride;
+  a.weight = weight;
+  a.param_dtype = param_dtype;
+  a.mean = mean;
+  a.rstd = rstd;
+  a.n = n;
+  a.D = static_cast<int>(D);
+  a.dx = dx;
+  a.partial = dweight != nullptr ? static_cast<float*>(workspace) : nullptr;
   int64_t partials = 0;
-  const int rc = dtype == DGS_F32    ? backward<float>(a, &partials, s)
-                 : dtype == DGS_BF16 ? backward<__nv_bfloat16>(a, &partials, s)
-                                     : backward<__half>(a, &partials, s);
-  if (rc != DGS_OK || dweight == nullptr) return rc;
+  const int rc = dtype == DGS_F32    ? backward<float>(a, &partials, dweight, dbias, s)
+                 : dtype == DGS_BF16 ? backward<__nv_bfloat16>(a, &partials, dweight, dbias, s)
+                                     : backward<__half>(a, &partials, dweight, dbias, s);
+  if (rc != DGS_OK || dweight == nullptr || partials == 0) return rc;  // (no partial sums: the gradients are there)
   DGS_CUDA_TRY(launch_training(norm_join_kernel, dim3(static_cast<unsigned>((2 * D + 31) / 32)), LN_JOIN_THREADS, 0, s, a.partial,
                                static_cast<int>(partials), a.D, dweight, dbias, param_dtype));
   return DGS_OK;

@@ -124,21 +124,31 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// launch_chained (common.cuh) with a two-dimensional grid and dynamic shared memory
-template <typename... KArgs, typename... Args>
-inline cudaError_t launch_training(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t s,
-                                   Args&&... args) {
+// launch_chained (common.cuh) with a grid of up to three dimensions, dynamic shared memory and clusters of that many CTAs (0, 1: none)
+template <typename... KArgs>
+inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t s, unsigned cluster,
+                                   KArgs... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(block, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = chained_launches_enabled(SITE_TRAINING) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  cfg.numAttrs = 0;
+  if (chained_launches_enabled(SITE_TRAINING)) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs++].val.clusterDim = {cluster, 1, 1};
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_training(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t s, Args&&... args) {
+  return launch_clusters(kernel, grid, block, smem, s, 0u, static_cast<KArgs>(args)...);
 }
 
 #endif  // __CUDACC__

@@ -133,6 +133,14 @@ def test_wanted_gradients(ops):
     assert none.numel() == 0 and torch.equal(dw, dw2) and torch.equal(db, db2)
 
 
+@pytest.mark.parametrize("D", [20, 100, 256, 1024, 4096])
+@pytest.mark.parametrize("rows", [8, 16, 32, 64, 128, 256, 512, 1024])
+def test_about_one_cluster_of_rows(ops, rows, D):
+    for n in (rows - 1, rows, rows + 1):
+        check(*make(n, D, torch.bfloat16, torch.float32), ops)
+        check(*make(n, D, torch.float32, torch.float32, pad=1), ops)
+
+
 @pytest.mark.parametrize("n,D", [(5000, 100), (3001, 1024), (700, 4096)])
 def test_same_bits_again(ops, n, D):
     x, dy, w, b = make(n, D, torch.bfloat16, torch.float32)
