@@ -5,7 +5,8 @@
 //   STATS    logits of a row block against a slice of the vocabulary; running maximum and sum of every row in registers
 //            (NARROW, FEW_STATS: the same for few classes, few rows)
 //   GRAD     logits of a piece again, left as G in 16 bits (FEW_GRAD: for few rows)
-//   PRODUCT  dh += G W and dW = G^T h of a piece, the tiles of both in one launch
+//   PRODUCT  dh += G W and dW = G^T h of a piece, the tiles of both in one launch (dW of one or two narrow rows: a kernel of its own
+//            on the CUDA cores)
 // A pair's tile is 256 x 256: each CTA of the pair holds 128 rows of it in its TMEM, fetches its 128 rows of A and its half
 // of B, so an operand element crosses from L2 once per pair.  Roles: warp 0 fetches (TMA, five or six stages of 64 along k),
 // warp 1 of the pair's first CTA issues the products, sixteen more work on finished accumulators (eight: 1.8 times as long at
@@ -877,12 +878,110 @@ __global__ void __launch_bounds__(256) ce_pack_weight_kernel(const uint16_t* __r
   }
 }
 
+// dW for one or two rows of few columns and many classes: no product to speak of but the writing of dW, which tiles of the tensor
+// core pass through their accumulators, 256 x 256 values for 64 of k of which one or two count.  A thread keeps the rows' values of
+// VEC columns and takes CLASSES classes at a time: a load of G a row and plane, sums in 32 bits, stores side by side.  Forward and
+// backward, one row against 831 627 classes: 80 columns 311 -> 272 us (30 of it this kernel, 4.5 TB/s; the product for dh that is
+// left takes 150), 75 columns 485 -> 397, 256 columns 417 -> 397; two rows: 75 columns 493 -> 421, 256 columns 417 -> 420.  With
+// eight rows it loses (80 columns 333 -> 363), and below some 50 000 classes the launch costs more than it saves (2 000 classes
+// 28 -> 30); against 140 000 one row of 80 goes from 78 to 73.
+constexpr int FEW_WEIGHT = 2, FEW_WEIGHT_THREADS = 256;
+constexpr int64_t FEW_WEIGHT_CLASSES = int64_t(1) << 17;
+struct FewWeightArgs {
+  const uint16_t* rows;  // packed
+  int64_t pitch;
+  const uint16_t* g;
+  int64_t g_pitch;
+  int32_t n, D, across;  // across: threads that share a class
+  int64_t width;                 // classes of the piece
+  uint16_t* out;
+  const float* largest;
+  int32_t largest_count;
+};
+
+template <bool BF16, int VEC, int ROWS>
+__global__ void __launch_bounds__(FEW_WEIGHT_THREADS, 2) ce_few_weight_kernel(const __grid_constant__ FewWeightArgs a) {
+  constexpr int CLASSES = VEC == 1 ? 8 : 4;
+  pdl_enter();
+  const float factor = grad_factor(a.largest, a.largest_count, threadIdx.x & 31, true);
+  const int group = threadIdx.x / a.across, groups = FEW_WEIGHT_THREADS / a.across;
+  const int col = threadIdx.x % a.across * VEC;
+  if (group >= groups) return;
+  float h[ROWS][VEC];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float unused;
+      h[i][e] = 0.0f;
+      if (i < a.n) unpack2<BF16>(a.rows[i * a.pitch + col + e], &h[i][e], &unused);
+    }
+  for (int64_t v = (static_cast<int64_t>(blockIdx.x) * groups + group) * CLASSES; v < a.width;
+       v += static_cast<int64_t>(gridDim.x) * groups * CLASSES) {
+    uint32_t both[ROWS][2][CLASSES / 2];  // of two planes, all under way at once
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {  // (G's rows have room for whole tiles: nothing is read behind them)
+        const uint16_t* from = a.g + (static_cast<int64_t>(q) * a.n + i) * a.g_pitch + v;
+        if constexpr (CLASSES == 8) {
+          const uint4 x = i < a.n ? *reinterpret_cast<const uint4*>(from) : uint4{0, 0, 0, 0};
+          both[i][q][0] = x.x, both[i][q][1] = x.y, both[i][q][2] = x.z, both[i][q][3] = x.w;
+        } else {
+          const uint2 x = i < a.n ? *reinterpret_cast<const uint2*>(from) : uint2{0, 0};
+          both[i][q][0] = x.x, both[i][q][1] = x.y;
+        }
+      }
+    }
+    float acc[CLASSES][VEC] = {};
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+#pragma unroll
+      for (int k = 0; k < CLASSES; k += 2) {
+        float high[2], low[2];
+        unpack2<BF16>(both[i][0][k / 2], &high[0], &high[1]);
+        unpack2<BF16>(both[i][1][k / 2], &low[0], &low[1]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          acc[k][e] = fmaf(high[0] + low[0], h[i][e], acc[k][e]);
+          acc[k + 1][e] = fmaf(high[1] + low[1], h[i][e], acc[k + 1][e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < CLASSES; ++k) {
+      if (v + k < a.width) {
+        uint16_t* to = a.out + (v + k) * a.D + col;
+        if constexpr (VEC == 1) {
+          *to = static_cast<uint16_t>(pack2<BF16>(acc[k][0] * factor, 0.0f));
+        } else {
+          *reinterpret_cast<uint2*>(to) =
+              uint2{pack2<BF16>(acc[k][0] * factor, acc[k][1] * factor), pack2<BF16>(acc[k][2] * factor, acc[k][3] * factor)};
+        }
+      }
+    }
+  }
+}
+
+template <bool BF16>
+int few_weight(FewWeightArgs a, cudaStream_t s) {
+  const bool fours = a.D % 4 == 0 && aligned_to(a.out, 8);
+  const int classes = fours ? 4 : 8;
+  a.across = a.D / (fours ? 4 : 1);  // (D <= N_TILE)
+  const int64_t need = tiles(a.width, FEW_WEIGHT_THREADS / a.across * classes), most = static_cast<int64_t>(sm_count()) * 16;
+  const dim3 grid(static_cast<unsigned>(need < most ? need : most));
+  auto kernel = a.n == 1 ? fours ? ce_few_weight_kernel<BF16, 4, 1> : ce_few_weight_kernel<BF16, 1, 1>
+                         : fours ? ce_few_weight_kernel<BF16, 4, 2> : ce_few_weight_kernel<BF16, 1, 2>;
+  DGS_CUDA_TRY(launch_training(kernel, grid, FEW_WEIGHT_THREADS, 0, s, a));
+  return DGS_OK;
+}
+
 // ---- host side -----------------------------------------------------------------------------------------------------
 struct MmaPlan {
   int64_t pitch, row_blocks, col_tiles, slices, pairs;
   int64_t piece, splits, dpitch;
   int64_t planes;  // of G
-  bool one_piece, compact, dh_first, few;
+  bool one_piece, compact, dh_first, few, few_weight;
   size_t packed, word, slot, live, counts, weight, target_logit, top, total, dloss, lse, largest, g, dh;
   size_t forward_bytes, backward_bytes;
 };
@@ -942,9 +1041,10 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   p.piece = piece_tiles * N_TILE;
   p.one_piece = p.piece >= V;
   p.dpitch = up(D, 4);
-  p.splits = splits_for(p.row_blocks, tiles(D, N_TILE), p.planes * tiles(p.piece, K_TILE), piece_tiles, p.planes * tiles(n, K_TILE),
-                        p.pairs, &p.dh_first);
   p.compact = worth_compacting(n, D, V);
+  p.few_weight = n <= FEW_WEIGHT && n * D <= N_TILE && V >= FEW_WEIGHT_CLASSES && p.planes == 2 && !p.compact;
+  p.splits = splits_for(p.row_blocks, tiles(D, N_TILE), p.planes * tiles(p.piece, K_TILE), p.few_weight ? 0 : piece_tiles, p.planes * tiles(n, K_TILE),
+                        p.pairs, &p.dh_first);
   Layout l;
   p.packed = l.take(n * p.pitch * 2);
   p.word = l.take(n * 4);
@@ -1121,7 +1221,8 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     // half as wide tiles where that gives more pairs something to do (1 024 rows of 256 against 172 classes: 5 tiles of 256)
     const int64_t wide = tiles(q.D, N_TILE) * (p.row_blocks * p.splits + tiles(width, M_TILE));
     const int32_t n_step = 2 * wide <= p.pairs ? N_TILE / 2 : N_TILE, d_tiles = static_cast<int32_t>(tiles(q.D, n_step));
-    const int both = dhidden != nullptr && dweight != nullptr, at_dh = both && !p.dh_first, at_dw = both && p.dh_first;
+    const bool dw_there = dweight != nullptr && !p.few_weight;
+    const int both = dhidden != nullptr && dw_there, at_dh = both && !p.dh_first, at_dw = both && p.dh_first;
     int64_t dh_items = 0, dw_items = 0;
     if (dhidden != nullptr) {
       Part& t = m.part[at_dh];
@@ -1148,7 +1249,7 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
         if (int rc = make_map(&m.out[at_dh], dh, DGS_F32, q.D, p.splits * t.split_rows, p.dpitch, 32, 32)) return rc;
       }
     }
-    if (dweight != nullptr) {
+    if (dw_there) {
       Part& t = m.part[at_dw];
       t.a_mn = 1;
       t.planes = static_cast<int32_t>(p.planes);
@@ -1176,7 +1277,13 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     m.largest = r.largest;
     m.largest_count = a.largest_count;
     m.status = q.status;
-    if (int rc = launch<PRODUCT>(m, p.pairs, q.dtype, s)) return rc;
+    if (m.items > 0)
+      if (int rc = launch<PRODUCT>(m, p.pairs, q.dtype, s)) return rc;
+    if (dweight != nullptr && p.few_weight) {
+      const FewWeightArgs f{static_cast<const uint16_t*>(packed), p.pitch, g, p.piece, static_cast<int32_t>(q.n),
+                            static_cast<int32_t>(q.D), 0, width, static_cast<uint16_t*>(dweight) + v0 * q.D, r.largest, a.largest_count};
+      if (int rc = q.dtype == DGS_BF16 ? few_weight<true>(f, s) : few_weight<false>(f, s)) return rc;
+    }
   }
   if (dhidden != nullptr && !dh_direct) return ce_sum(dh, p.splits, q.n, q.D, p.row_blocks * M_TILE, p.dpitch, r.slot, dhidden, q.dtype, s);
   return DGS_OK;

@@ -65,6 +65,17 @@ def test_sizes(ops, n, D, V, dtype):
     check(ops, *make(n, D, V, dtype))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 9])
+@pytest.mark.parametrize("D", [1, 4, 75, 256, 260, 1030, 1100])
+def test_few_rows(ops, dtype, n, D):
+    for V, ignored in ((129, 0.0), (1003, 0.4), (20_011, 0.0), (140_011, 0.4)):
+        h, w, t, dl = make(n, D, V, dtype, ignored, seed=n)
+        _, lse, dh, dw = check(ops, h, w, t, dl)
+        alone = [ops._CAPI_linear_cross_entropy_backward(dl, h, w, t, lse, -100, a, not a)[0 if a else 1] for a in (True, False)]
+        assert torch.equal(alone[0], dh) and torch.equal(alone[1], dw)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("ignored", [0.3, 0.97, 1.0])
 def test_ignored_rows(ops, dtype, ignored):
