@@ -88,14 +88,16 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
 
 
 class AdamW:
-    """AdamW over a list of tensors, one launch a step, moments in 32 or in 8 bits.
+    """AdamW over a list of tensors, one launch a step (for lists of up to 512), moments in 32 or in 8 bits.
 
         optimizer = AdamW([p for p in model.parameters()], lr=1e-3)
         optimizer = AdamW(masters, copies=model_params, bits=8)      # 32-bit parameters, 16-bit model
 
     params are written in place (contiguous; float32, bfloat16 or float16).  copies, if given, receive every new parameter in
     their own type, and gradients are taken from them: 16-bit model parameters with 32-bit masters.  A tensor without a
-    gradient stays as it is.  The moments lie in two flat buffers, a slot of whole 256-element blocks for each tensor."""
+    gradient stays as it is, and the step does not count for it: the bias corrections go by the steps that a tensor's own
+    moments have seen (`tensor_steps`; a launch for each of the counts that a step meets).  The moments lie in two flat
+    buffers, a slot of whole 256-element blocks for each tensor."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, copies=None):
         import torch
@@ -108,6 +110,7 @@ class AdamW:
         if self.copies and len(self.copies) != len(self.params):
             raise ValueError("AdamW: %d parameters and %d copies" % (len(self.params), len(self.copies)))
         self.lr, self.betas, self.eps, self.weight_decay, self.bits, self.steps = lr, tuple(betas), eps, weight_decay, bits, 0
+        self.tensor_steps = [0] * len(self.params)
         self._ops = _ops()
         blocks = sum(-(-p.numel() // 256) for p in self.params)
         dev = self.params[0].device
@@ -129,15 +132,25 @@ class AdamW:
         """One step with `grads` (None in the place of a gradient that is absent), or with the tensors' own .grad."""
         if grads is None:
             grads = [p.grad for p in self.copies or self.params]
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError("AdamW: %d parameters and %d gradients" % (len(self.params), len(grads)))
+        counts = [n if g is None else n + 1 for n, g in zip(self.tensor_steps, grads)]
+        due = {n for n, g in zip(counts, grads) if g is not None}
+        for n in sorted(due):
+            now = grads if len(due) == 1 else [g if c == n else None for c, g in zip(counts, grads)]
+            self._step(now, n)
+            self.tensor_steps = [t if g is None else n for t, g in zip(self.tensor_steps, now)]
+        self.steps += 1
+
+    def _step(self, grads, step):
         st, (b1, b2) = self.state, self.betas
-        step = self.steps + 1
         if self.bits == 32:
             self._ops._CAPI_adamw_step(self.params, grads, self.copies, st["exp_avg"], st["exp_avg_sq"], self.lr, b1, b2, self.eps,
                                        self.weight_decay, step)
         else:
             self._ops._CAPI_adamw_step_8bit(self.params, grads, self.copies, st["exp_avg"], st["exp_avg_scale"], st["exp_avg_sq"],
                                             st["exp_avg_sq_scale"], self.lr, b1, b2, self.eps, self.weight_decay, step)
-        self.steps = step
 
     def moments(self):
         """(first, second) moments as two flat float32 tensors, laid out like the state."""
@@ -148,7 +161,7 @@ class AdamW:
                 self._ops._CAPI_adamw_state_values(st["exp_avg_sq"], st["exp_avg_sq_scale"]))
 
     def state_dict(self):
-        return {"steps": self.steps, "bits": self.bits, "sizes": [p.numel() for p in self.params],
+        return {"steps": self.steps, "tensor_steps": list(self.tensor_steps), "bits": self.bits, "sizes": [p.numel() for p in self.params],
                 "state": {k: v.clone() for k, v in self.state.items()}}
 
     def load_state_dict(self, saved):
@@ -157,3 +170,5 @@ class AdamW:
         for k, v in self.state.items():
             v.copy_(saved["state"][k])
         self.steps = saved["steps"]
+        # (a state without counts of its own is of the time when one stood for all tensors)
+        self.tensor_steps = list(saved.get("tensor_steps", [self.steps] * len(self.params)))
