@@ -194,10 +194,10 @@ inline std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyBackwardCUDA(t
 }
 
 namespace {
-// The list of one step.  `keep` holds gradients that had to be made contiguous.
+// The list of one step.  `keep` holds gradients that had to be made contiguous, `written` what the step writes.
 struct AdamWList {
   std::vector<dgs_adamw_tensor> tensors;
-  std::vector<torch::Tensor> keep;
+  std::vector<torch::Tensor> keep, written;
   int64_t slots = 0;  // elements of all slots
 };
 inline AdamWList adamw_list(const char* op, const std::vector<torch::Tensor>& params,
@@ -237,10 +237,12 @@ inline AdamWList adamw_list(const char* op, const std::vector<torch::Tensor>& pa
     }
     t.param = p.data_ptr();
     list.tensors.push_back(t);
+    list.written.push_back(p);
+    if (!copies.empty()) list.written.push_back(copies[i]);
   }
   return list;
 }
-// the tensors were written behind torch's back: what autograd saved of them is out of date
+// The tensors were written behind torch's back: what autograd saved of them is out of date.  (Of those without a gradient it is not.)
 inline void mark_written(const std::vector<torch::Tensor>& ts) {
   for (const torch::Tensor& t : ts)
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -264,8 +266,7 @@ inline void AdamWStepCUDA(std::vector<torch::Tensor> params, c10::List<c10::opti
   check_moment(exp_avg_sq, torch::kFloat, list.slots, exp_avg.device(), op, "exp_avg_sq");
   DGS_CHECK_RC(dgs_adamw_step(list.tensors.data(), static_cast<int32_t>(list.tensors.size()), exp_avg.data_ptr<float>(),
                               exp_avg_sq.data_ptr<float>(), lr, beta1, beta2, eps, weight_decay, step, current_stream()));
-  mark_written(params);
-  mark_written(copies);
+  mark_written(list.written);
 }
 
 inline void AdamWStep8bitCUDA(std::vector<torch::Tensor> params, c10::List<c10::optional<torch::Tensor>> grads,
@@ -285,8 +286,7 @@ inline void AdamWStep8bitCUDA(std::vector<torch::Tensor> params, c10::List<c10::
   DGS_CHECK_RC(dgs_adamw_step_8bit(list.tensors.data(), static_cast<int32_t>(list.tensors.size()), exp_avg.data_ptr<int8_t>(),
                                    exp_avg_scale.data_ptr<float>(), exp_avg_sq.data_ptr<uint8_t>(), exp_avg_sq_scale.data_ptr<float>(),
                                    lr, beta1, beta2, eps, weight_decay, step, current_stream()));
-  mark_written(params);
-  mark_written(copies);
+  mark_written(list.written);
 }
 
 inline torch::Tensor AdamWStateValuesCUDA(torch::Tensor codes, torch::Tensor scales) {
