@@ -2,6 +2,10 @@
 // vocabulary, AdamW.  Additions (no counterparts in the reference's src/pybind.cc); thin layers over the C ABI like the
 // operators of ops.cc.
 #pragma once
+#include <algorithm>
+#include <initializer_list>
+#include <utility>
+
 #include "chunk_tensor.h"
 
 namespace dgs {
@@ -197,7 +201,8 @@ namespace {
 // The list of one step.  `keep` holds gradients that had to be made contiguous, `written` what the step writes.
 struct AdamWList {
   std::vector<dgs_adamw_tensor> tensors;
-  std::vector<torch::Tensor> keep, written;
+  std::vector<torch::Tensor> keep;
+  std::vector<const torch::Tensor*> written;
   int64_t slots = 0;  // elements of all slots
 };
 inline AdamWList adamw_list(const char* op, const std::vector<torch::Tensor>& params,
@@ -207,6 +212,7 @@ inline AdamWList adamw_list(const char* op, const std::vector<torch::Tensor>& pa
   TORCH_CHECK(copies.empty() || copies.size() == params.size(), op, ": ", params.size(), " parameters and ", copies.size(), " copies");
   AdamWList list;
   list.tensors.reserve(params.size());
+  list.written.reserve(2 * params.size());
   for (size_t i = 0; i < params.size(); ++i) {
     const torch::Tensor& p = params[i];
     check_on(p, dev, op, "every parameter");
@@ -237,15 +243,42 @@ inline AdamWList adamw_list(const char* op, const std::vector<torch::Tensor>& pa
     }
     t.param = p.data_ptr();
     list.tensors.push_back(t);
-    list.written.push_back(p);
-    if (!copies.empty()) list.written.push_back(copies[i]);
+    list.written.push_back(&p);
+    if (!copies.empty()) list.written.push_back(&copies[i]);
   }
   return list;
 }
 // The tensors were written behind torch's back: what autograd saved of them is out of date.  (Of those without a gradient it is not.)
-inline void mark_written(const std::vector<torch::Tensor>& ts) {
-  for (const torch::Tensor& t : ts)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+inline void mark_written(const std::vector<const torch::Tensor*>& ts) {
+  for (const torch::Tensor* t : ts)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+// No element may have two writers: they would race.  (A copy that is its own parameter has one, which writes the same value twice.)
+class Written {
+ public:
+  explicit Written(size_t most) { spans_.reserve(most); }
+  void add(const void* p, int64_t bytes) {
+    if (bytes > 0) spans_.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes);
+  }
+  void check(const char* op) {
+    std::sort(spans_.begin(), spans_.end());
+    for (size_t i = 1; i < spans_.size(); ++i)
+      TORCH_CHECK(spans_[i - 1].second <= spans_[i].first, op, ": parameters, copies and moments are written in place and must not overlap");
+  }
+
+ private:
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans_;
+};
+// moments: with the number of elements of each that the slots take
+inline void check_written(const char* op, const AdamWList& list, std::initializer_list<std::pair<const torch::Tensor*, int64_t>> moments) {
+  Written w(2 * list.tensors.size() + moments.size());
+  for (const dgs_adamw_tensor& t : list.tensors) {
+    const auto bytes = [&](int32_t dtype) { return t.n * (dtype == DGS_F32 ? 4 : 2); };
+    w.add(t.param, bytes(t.param_dtype));
+    if (t.copy != nullptr && !(t.copy == t.param && t.copy_dtype == t.param_dtype)) w.add(t.copy, bytes(t.copy_dtype));
+  }
+  for (const auto& [m, elems] : moments) w.add(m->data_ptr(), elems * m->element_size());
+  w.check(op);
 }
 inline void check_moment(const torch::Tensor& t, torch::ScalarType type, int64_t elems, const torch::Device& dev, const char* op,
                          const char* what) {
@@ -264,6 +297,7 @@ inline void AdamWStepCUDA(std::vector<torch::Tensor> params, c10::List<c10::opti
   const AdamWList list = adamw_list(op, params, grads, copies, exp_avg.device());
   check_moment(exp_avg, torch::kFloat, list.slots, exp_avg.device(), op, "exp_avg");
   check_moment(exp_avg_sq, torch::kFloat, list.slots, exp_avg.device(), op, "exp_avg_sq");
+  check_written(op, list, {{&exp_avg, list.slots}, {&exp_avg_sq, list.slots}});
   DGS_CHECK_RC(dgs_adamw_step(list.tensors.data(), static_cast<int32_t>(list.tensors.size()), exp_avg.data_ptr<float>(),
                               exp_avg_sq.data_ptr<float>(), lr, beta1, beta2, eps, weight_decay, step, current_stream()));
   mark_written(list.written);
@@ -283,6 +317,7 @@ inline void AdamWStep8bitCUDA(std::vector<torch::Tensor> params, c10::List<c10::
   check_moment(exp_avg_sq, torch::kByte, list.slots, dev, op, "exp_avg_sq");
   check_moment(exp_avg_scale, torch::kFloat, blocks, dev, op, "exp_avg_scale");
   check_moment(exp_avg_sq_scale, torch::kFloat, blocks, dev, op, "exp_avg_sq_scale");
+  check_written(op, list, {{&exp_avg, list.slots}, {&exp_avg_scale, blocks}, {&exp_avg_sq, list.slots}, {&exp_avg_sq_scale, blocks}});
   DGS_CHECK_RC(dgs_adamw_step_8bit(list.tensors.data(), static_cast<int32_t>(list.tensors.size()), exp_avg.data_ptr<int8_t>(),
                                    exp_avg_scale.data_ptr<float>(), exp_avg_sq.data_ptr<uint8_t>(), exp_avg_sq_scale.data_ptr<float>(),
                                    lr, beta1, beta2, eps, weight_decay, step, current_stream()));
