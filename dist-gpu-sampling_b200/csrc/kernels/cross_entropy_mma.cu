@@ -18,8 +18,7 @@
 // SM that it gives (a fifth of the time is spent waiting for them); at rows of 128 the exponentials, 16 a clock and SM (1 024 rows
 // against 2.4 M classes: 0.81 ms, the unit is busy for 83 % of it) and in the backward pass G's way through HBM; with few rows the
 // reading of W (8 rows of 1 024 against 150 000 classes: 60 us, 5.1 TB/s).
-// exp(s - m) = 2^(s log2(e) - m log2(e)): one fused multiply-add and one ex2 an element.  The rounding of m log2(e) changes a
-// row's lse by less than the rounding of the lse itself.
+// exp(s - m) = 2^((s - m) log2(e)): half a packed addition, half a packed multiplication and one ex2 an element.
 //
 // Every wait is bounded.  One that runs out marks the CTA's words as dead, all roles leave, the status word gets
 // DGS_ERR_CUDA, and the pair frees its TMEM as usual.
@@ -281,25 +280,22 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// A logit (or lse) whose product with log2(e) may leave the range of 32-bit floats (the type's lowest value as a mask), or that is
-// no finite number
-__device__ __forceinline__ bool far(float x) { return !(fabsf(x) < 1e38f); }
 __device__ __forceinline__ float max_or_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
-// e^(v - base) for 32 values that are no NaN, in pairs: packed additions and multiplications halve what stands beside the 16 ex2 a
-// clock and SM (1 024 rows of 128 against 2.4 M classes: 845 -> 723 us.  A share of the exponentials as polynomials on the
-// multiply-add units does not help: every sixth pair 733, every fourth 797).
+// e^(v - base) for 32 values, in pairs: packed additions and multiplications halve what stands beside the 16 ex2 a clock and SM.
+// (A share of the exponentials as polynomials on the multiply-add units does not help.)  The difference comes first and is exact, or
+// nearly, where it counts: the largest logit of a row gives exactly one, so its loss is never negative.  v log2(e) - rn(base log2(e))
+// in one operation would be off by 2^-24 |base| in each exponent, and so would be the loss.
 __device__ __forceinline__ void exp_pairs(const uint32_t (&v)[32], float base, uint64_t (&e)[16]) {
-  const float minus = -base * LOG2E;
-  const uint64_t scale2 = two(LOG2E, LOG2E), minus2 = two(minus, minus);
+  const uint64_t scale2 = two(LOG2E, LOG2E), minus2 = two(-base, -base);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float lo, hi;
-    split2(fma2(two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, minus2), &lo, &hi);
+    split2(mul2(add2(two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), minus2), scale2), &lo, &hi);
     e[i] = two(ex2(lo), ex2(hi));
   }
 }
@@ -319,25 +315,16 @@ struct RowSum {
 #pragma unroll
     for (int i = 8; i < 32; ++i) m[i & 3] = max_or_nan(m[i & 3], at(v, i));
     const float now = max_or_nan(max_or_nan(max_or_nan(m[0], m[1]), max_or_nan(m[2], m[3])), top);
-    float s;
-    if (!far(now)) {
-      total *= ex2((top - now) * LOG2E);  // (0 while top is minus infinity)
-      uint64_t e[16];
-      exp_pairs(v, now, e);
+    // nothing but minus infinity so far: the exponential must not see their difference
+    const float base = now == -INFINITY ? 0.0f : now;
+    uint64_t e[16];
+    exp_pairs(v, base, e);
 #pragma unroll
-      for (int i = 4; i < 16; ++i) e[i & 3] = add2(e[i & 3], e[i]);
-      float lo, hi;
-      split2(add2(add2(e[0], e[1]), add2(e[2], e[3])), &lo, &hi);
-      s = lo + hi;
-    } else {
-      const float base = now == -INFINITY ? 0.0f : now;  // nothing but minus infinity so far
-      total *= ex2((top - base) * LOG2E);
-      s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) s += ex2((at(v, i) - base) * LOG2E);
-    }
+    for (int i = 4; i < 16; ++i) e[i & 3] = add2(e[i & 3], e[i]);
+    float lo, hi;
+    split2(add2(add2(e[0], e[1]), add2(e[2], e[3])), &lo, &hi);
+    total = total * ex2((top - base) * LOG2E) + (lo + hi);  // (0 while top is minus infinity)
     top = now;
-    total += s;
   }
   static __device__ __forceinline__ float at(const uint32_t (&v)[32], int i) { return __uint_as_float(v[i]); }
 };
@@ -667,20 +654,15 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
               if (at < 32u && word >= 0) *(join ? &join->target[in_cta_row] : &a.target_logit[row]) = pick(now, static_cast<int>(at));
               if (left > 0) sum.add(now, left);
             } else if constexpr (MODE == GRAD) {
-              if (!far(lse)) {  // (then no logit is a NaN)
-                uint64_t e[16];
-                exp_pairs(now, lse, e);
-                const uint64_t grad2 = two(grad, grad);
+              uint64_t e[16];
+              exp_pairs(now, lse, e);
+              const uint64_t grad2 = two(grad, grad);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  float lo, hi;
-                  split2(mul2(e[i], grad2), &lo, &hi);
-                  now[2 * i] = __float_as_uint(lo);
-                  now[2 * i + 1] = __float_as_uint(hi);
-                }
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) now[i] = __float_as_uint(grad * ex2((__uint_as_float(now[i]) - lse) * LOG2E));
+              for (int i = 0; i < 16; ++i) {
+                float lo, hi;
+                split2(mul2(e[i], grad2), &lo, &hi);
+                now[2 * i] = __float_as_uint(lo);
+                now[2 * i + 1] = __float_as_uint(hi);
               }
               const uint32_t at = static_cast<uint32_t>(word - a.v0 - col);
               if (at < 32u && word >= 0) {
