@@ -151,6 +151,8 @@ ABI_SIGNATURES = {
     "dgs_linear_cross_entropy_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
     "dgs_linear_cross_entropy_backward": (ctypes.c_int, [_VP, _VP, _I64, _VP, _I64, _I32, _VP, _I32, _VP, _I64, _I64, _I64, _I64,
                                                          _VP, _VP, _VP, _SZ, _VP, _VP]),
+    "dgs_linear_cross_entropy_backward_from_loss": (ctypes.c_int, [_VP, _VP, _I64, _VP, _I64, _I32, _VP, _I32, _VP, _VP, _I64, _I64,
+                                                                   _I64, _I64, _VP, _VP, _VP, _SZ, _VP, _VP]),
     "dgs_adamw_slot_elems": (_I64, [_I64]),
     "dgs_adamw_step": (ctypes.c_int, [_AP, _I32, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _VP]),
     "dgs_adamw_step_8bit": (ctypes.c_int, [_AP, _I32, _VP, _VP, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _VP]),

@@ -168,11 +168,11 @@ inline std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyCUDA(torch::Te
   return std::make_tuple(loss, lse);
 }
 
-// (dhidden, dweight); what is not wanted comes back with no elements
-inline std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyBackwardCUDA(torch::Tensor grad_loss, torch::Tensor hidden,
-                                                                               torch::Tensor weight, torch::Tensor target,
-                                                                               torch::Tensor lse, int64_t ignore_index,
-                                                                               bool want_hidden, bool want_weight) {
+// (dhidden, dweight); what is not wanted comes back with no elements.  loss: may be undefined
+inline std::tuple<torch::Tensor, torch::Tensor> cross_entropy_backward(torch::Tensor grad_loss, const torch::Tensor& hidden,
+                                                                       const torch::Tensor& weight, const torch::Tensor& target,
+                                                                       torch::Tensor lse, torch::Tensor loss, int64_t ignore_index,
+                                                                       bool want_hidden, bool want_weight) {
   const char* op = "_CAPI_linear_cross_entropy_backward";
   CrossEntropyInputs in = cross_entropy_inputs(op, hidden, weight, target);
   check_on(grad_loss, hidden.device(), op, "grad_loss");
@@ -180,6 +180,12 @@ inline std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyBackwardCUDA(t
   TORCH_CHECK(grad_loss.scalar_type() == torch::kFloat && lse.scalar_type() == torch::kFloat && grad_loss.dim() == 1 && lse.dim() == 1 &&
                   grad_loss.size(0) == in.n && lse.size(0) == in.n,
               op, ": grad_loss and lse must be float32 with one value for each row of hidden");
+  if (loss.defined()) {
+    check_on(loss, hidden.device(), op, "loss");
+    TORCH_CHECK(loss.scalar_type() == torch::kFloat && loss.dim() == 1 && loss.size(0) == in.n, op,
+                ": loss must be float32 with one value for each row of hidden");
+    loss = loss.contiguous();
+  }
   c10::cuda::CUDAGuard guard(hidden.device());
   lay_out(in, hidden, weight, target);
   grad_loss = grad_loss.contiguous();
@@ -189,12 +195,26 @@ inline std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyBackwardCUDA(t
   const size_t wb = want_hidden || want_weight ? dgs_linear_cross_entropy_backward_workspace_bytes(in.n, in.D, in.V, in.dtype) : 0;
   torch::Tensor ws = byte_scratch(wb, hidden.device());
   const Lease w(op, hidden.device().index(), current_stream());
-  DGS_CHECK_RC(dgs_linear_cross_entropy_backward(
+  DGS_CHECK_RC(dgs_linear_cross_entropy_backward_from_loss(
       grad_loss.data_ptr<float>(), in.hidden.t.data_ptr(), in.hidden.stride, in.weight.t.data_ptr(), in.weight.stride, in.dtype,
-      in.target.data_ptr(), in.ids64, lse.data_ptr<float>(), in.n, in.D, in.V, ignore_index, want_hidden ? dh.data_ptr() : nullptr,
-      want_weight ? dw.data_ptr() : nullptr, ws.data_ptr(), wb, w.status(), current_stream()));
+      in.target.data_ptr(), in.ids64, lse.data_ptr<float>(), loss.defined() ? loss.data_ptr<float>() : nullptr, in.n, in.D, in.V, ignore_index,
+      want_hidden ? dh.data_ptr() : nullptr, want_weight ? dw.data_ptr() : nullptr, ws.data_ptr(), wb, w.status(), current_stream()));
   w.finish();
   return std::make_tuple(dh, dw);
+}
+inline std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyBackwardCUDA(torch::Tensor grad_loss, torch::Tensor hidden,
+                                                                               torch::Tensor weight, torch::Tensor target,
+                                                                               torch::Tensor lse, int64_t ignore_index,
+                                                                               bool want_hidden, bool want_weight) {
+  return cross_entropy_backward(grad_loss, hidden, weight, target, lse, {}, ignore_index, want_hidden, want_weight);
+}
+// ... with the loss that the forward call gave beside lse
+inline std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyBackwardFromLossCUDA(torch::Tensor grad_loss, torch::Tensor hidden,
+                                                                                       torch::Tensor weight, torch::Tensor target,
+                                                                                       torch::Tensor lse, torch::Tensor loss,
+                                                                                       int64_t ignore_index, bool want_hidden,
+                                                                                       bool want_weight) {
+  return cross_entropy_backward(grad_loss, hidden, weight, target, lse, loss, ignore_index, want_hidden, want_weight);
 }
 
 namespace {

@@ -3,6 +3,10 @@
 //   s_iv = h_i . W_v,  lse_i = log sum_v exp(s_iv),  loss_i = lse_i - s_i,t(i)
 //   G_iv = dloss_i (exp(s_iv - lse_i) - [v = t(i)]),  dh = G W,  dW = G^T h
 //
+// At the target exp(s - lse) - 1 = expm1(-loss).  lse is a sum in 32 bits, off by 2^-25 of itself: of a row that is nearly right,
+// with a loss of 1e-4 at logits of 100, the difference to one would be off by some percent, the loss is not.  Where it is given to
+// the backward pass that entry comes from it.
+//
 // Forward: a block of rows meets the vocabulary tile by tile; each row carries a running maximum and a running sum of
 // exponentials, so a tile of logits lives in registers only.  The vocabulary is cut into slices where there are fewer row
 // blocks than SMs; a last launch joins the slices' (maximum, sum) pairs in their order (16-bit operands whose row blocks meet
@@ -39,7 +43,7 @@ struct PackArgs {
   int64_t n, V, ignore_index;
   int32_t D, pitch;
   CePacked to;
-  const float *dloss, *lse;
+  const float *dloss, *lse, *loss;
   int32_t* status;
 };
 
@@ -128,6 +132,7 @@ __global__ void __launch_bounds__(CE_THREADS) ce_pack_kernel(const __grid_consta
         const float d = word >= 0 ? a.dloss[row] : 0.0f;
         a.to.dloss[to] = d;
         a.to.lse[to] = word >= 0 ? a.lse[row] : 0.0f;
+        if (a.to.hit != nullptr) a.to.hit[to] = word >= 0 ? expm1f(-a.loss[row]) : 0.0f;
         most = fmaxf(most, fabsf(d));
       }
     }
@@ -414,6 +419,7 @@ struct GradArgs {
   const int32_t* word;
   const float* dloss;
   const float* lse;
+  const float* hit;
   float* g;  // [n][pitch]
 };
 
@@ -430,12 +436,13 @@ __global__ void __launch_bounds__(CE_THREADS, 2) ce_grad_kernel(const Operand<tr
     const int64_t row = m0 + tile_at(ty, i);
     if (row >= a.n) continue;
     const int32_t word = a.word[row];
-    const float scale = word >= 0 ? a.dloss[row] : 0.0f, lse = a.lse[row];
+    const float scale = word >= 0 ? a.dloss[row] : 0.0f, lse = a.lse[row], hit = a.hit != nullptr ? a.hit[row] : 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int64_t c = n0 + tile_at(tx, j);
       if (a.v0 + c >= a.V || c >= a.pitch) continue;
-      const float p = expf(acc[i][j] - lse) - (a.v0 + c == word ? 1.0f : 0.0f);
+      float p = expf(acc[i][j] - lse);
+      if (a.v0 + c == word) p = a.hit != nullptr ? hit : p - 1.0f;
       a.g[row * a.pitch + c] = word >= 0 ? scale * p : 0.0f;
     }
   }
@@ -515,7 +522,7 @@ struct Plan {
   int64_t row_blocks, col_tiles, slices;
   int64_t piece;                       // classes of a piece
   int64_t splits;                      // of a piece's classes in dh's product
-  size_t packed, word, target_logit, top, total, dloss, lse, g, dh;
+  size_t packed, word, target_logit, top, total, dloss, lse, hit, g, dh;
   size_t forward_bytes, backward_bytes;
 };
 
@@ -543,6 +550,7 @@ Plan make_plan(int64_t n, int64_t D, int64_t V) {
   l = common;
   p.dloss = l.take(n * 4);
   p.lse = l.take(n * 4);
+  p.hit = l.take(n * 4);
   p.g = l.take(n * p.piece * 4);
   p.dh = l.take(p.splits * n * D * 4);
   p.backward_bytes = l.bytes;
@@ -558,7 +566,7 @@ int forward32(const CeProblem& q, float* loss, float* lse, cudaStream_t s) {
   to.rows = q.ws + p.packed;
   to.pitch = p.pitch;
   to.word = word;
-  if (int rc = ce_pack(q, to, nullptr, nullptr, s)) return rc;
+  if (int rc = ce_pack(q, to, nullptr, nullptr, nullptr, s)) return rc;
   float *top = reinterpret_cast<float*>(q.ws + p.top), *total = reinterpret_cast<float*>(q.ws + p.total);
   const StatsArgs a{q.n, q.V, static_cast<int>(q.D), p.row_blocks, p.col_tiles, p.slices, word, tl, top, total};
   DGS_CUDA_TRY(launch_training(ce_stats_kernel, dim3(static_cast<unsigned>(p.row_blocks * p.slices)), CE_THREADS, 0, s,
@@ -566,7 +574,7 @@ int forward32(const CeProblem& q, float* loss, float* lse, cudaStream_t s) {
   return ce_join(q, top, total, 1, p.slices, nullptr, word, nullptr, tl, loss, lse, s);
 }
 
-int backward32(const CeProblem& q, const float* dloss, const float* lse, float* dhidden, float* dweight, cudaStream_t s) {
+int backward32(const CeProblem& q, const float* dloss, const float* lse, const float* loss, float* dhidden, float* dweight, cudaStream_t s) {
   const Plan p = make_plan(q.n, q.D, q.V);
   int32_t* word = reinterpret_cast<int32_t*>(q.ws + p.word);
   const float* packed = reinterpret_cast<const float*>(q.ws + p.packed);
@@ -576,13 +584,14 @@ int backward32(const CeProblem& q, const float* dloss, const float* lse, float* 
   to.word = word;
   to.dloss = reinterpret_cast<float*>(q.ws + p.dloss);
   to.lse = reinterpret_cast<float*>(q.ws + p.lse);
-  if (int rc = ce_pack(q, to, dloss, lse, s)) return rc;
+  to.hit = loss != nullptr ? reinterpret_cast<float*>(q.ws + p.hit) : nullptr;
+  if (int rc = ce_pack(q, to, dloss, lse, loss, s)) return rc;
   float *g = reinterpret_cast<float*>(q.ws + p.g), *dh = reinterpret_cast<float*>(q.ws + p.dh);
   const unsigned dtiles = static_cast<unsigned>(tiles(q.D, CE_COLS));
   for (int64_t v0 = 0; v0 < q.V; v0 += p.piece) {
     const int64_t width = q.V - v0 < p.piece ? q.V - v0 : p.piece;
     const float* wp = static_cast<const float*>(q.weight) + v0 * q.weight_stride;
-    const GradArgs a{q.n, q.V, v0, p.piece, p.row_blocks, static_cast<int>(q.D), word, to.dloss, to.lse, g};
+    const GradArgs a{q.n, q.V, v0, p.piece, p.row_blocks, static_cast<int>(q.D), word, to.dloss, to.lse, to.hit, g};
     DGS_CUDA_TRY(launch_training(ce_grad_kernel, dim3(static_cast<unsigned>(p.row_blocks * tiles(width, CE_COLS))), CE_THREADS, 0, s,
                                  Operand<true>{packed, p.pitch, q.n}, Operand<true>{wp, q.weight_stride, width}, a));
     if (dhidden != nullptr)
@@ -610,11 +619,11 @@ int check(const char* who, const CeProblem& q) {
 
 }  // namespace
 
-int ce_pack(const CeProblem& q, const CePacked& p, const float* dloss, const float* lse, cudaStream_t s) {
+int ce_pack(const CeProblem& q, const CePacked& p, const float* dloss, const float* lse, const float* loss, cudaStream_t s) {
   const int64_t per16 = 16 / dtype_bytes(q.dtype);
   const bool vectors = q.D == p.pitch && p.pitch % per16 == 0 && q.hidden_stride % per16 == 0 && aligned_to(q.hidden, 16);
   const PackArgs a{q.hidden, q.hidden_stride, q.target, q.ids64,  vectors, q.n, q.V, q.ignore_index, static_cast<int32_t>(q.D),
-                   static_cast<int32_t>(p.pitch), p, dloss, lse, q.status};
+                   static_cast<int32_t>(p.pitch), p, dloss, lse, loss, q.status};
   if (p.compact)
     DGS_CUDA_TRY(launch_training(ce_count_kernel, dim3(static_cast<unsigned>(tiles(q.n, CE_COUNT_ROWS))), CE_THREADS, 0, s, a));
   const dim3 grid(static_cast<unsigned>(ce_pack_ctas(q.n)));
@@ -679,11 +688,11 @@ extern "C" size_t dgs_linear_cross_entropy_backward_workspace_bytes(int64_t n, i
   return dtype == DGS_F32 ? make_plan(n, D, V).backward_bytes : ce_mma_backward_bytes(n, D, V);
 }
 
-extern "C" int dgs_linear_cross_entropy_backward(const float* dloss, const void* hidden, int64_t hidden_stride, const void* weight,
-                                                 int64_t weight_stride, int32_t dtype, const void* target, int32_t ids64,
-                                                 const float* lse, int64_t n, int64_t D, int64_t V, int64_t ignore_index, void* dhidden,
-                                                 void* dweight, void* workspace, size_t workspace_bytes, int32_t* status,
-                                                 dgs_stream_t stream) {
+extern "C" int dgs_linear_cross_entropy_backward_from_loss(const float* dloss, const void* hidden, int64_t hidden_stride, const void* weight,
+                                                           int64_t weight_stride, int32_t dtype, const void* target, int32_t ids64,
+                                                           const float* lse, const float* loss, int64_t n, int64_t D, int64_t V,
+                                                           int64_t ignore_index, void* dhidden, void* dweight, void* workspace,
+                                                           size_t workspace_bytes, int32_t* status, dgs_stream_t stream) {
   const CeProblem q{hidden, hidden_stride, weight, weight_stride, dtype, target, ids64 != 0, n, D, V, ignore_index, static_cast<char*>(workspace), status};
   if (int rc = check("linear_cross_entropy_backward", q)) return rc;
   if (dhidden == nullptr && dweight == nullptr) return DGS_OK;
@@ -697,6 +706,15 @@ extern "C" int dgs_linear_cross_entropy_backward(const float* dloss, const void*
   const size_t need = dgs_linear_cross_entropy_backward_workspace_bytes(n, D, V, dtype);
   DGS_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned_to(workspace, 256), DGS_ERR_INVALID,
               "linear_cross_entropy_backward: workspace of %zu bytes, 256-byte aligned, is needed", need);
-  return dtype == DGS_F32 ? backward32(q, dloss, lse, static_cast<float*>(dhidden), static_cast<float*>(dweight), s)
-                          : ce_mma_backward(q, dloss, lse, dhidden, dweight, s);
+  return dtype == DGS_F32 ? backward32(q, dloss, lse, loss, static_cast<float*>(dhidden), static_cast<float*>(dweight), s)
+                          : ce_mma_backward(q, dloss, lse, loss, dhidden, dweight, s);
+}
+
+extern "C" int dgs_linear_cross_entropy_backward(const float* dloss, const void* hidden, int64_t hidden_stride, const void* weight,
+                                                 int64_t weight_stride, int32_t dtype, const void* target, int32_t ids64,
+                                                 const float* lse, int64_t n, int64_t D, int64_t V, int64_t ignore_index, void* dhidden,
+                                                 void* dweight, void* workspace, size_t workspace_bytes, int32_t* status,
+                                                 dgs_stream_t stream) {
+  return dgs_linear_cross_entropy_backward_from_loss(dloss, hidden, hidden_stride, weight, weight_stride, dtype, target, ids64, lse, nullptr, n, D,
+                                                     V, ignore_index, dhidden, dweight, workspace, workspace_bytes, status, stream);
 }

@@ -57,7 +57,7 @@ inline int64_t slices_for(int64_t rows, int64_t cols, int64_t slots) {
 }
 
 // The rows that count, as cross_entropy.cu packs them.  Packed row c holds what the products read: the hidden row, its target
-// as a 32-bit word (-1: none), and for the backward pass dloss and lse.  Either row c is row c of the call (rows without a valid
+// as a 32-bit word (-1: none), and for the backward pass dloss, lse and, where the loss is given, the target's entry p - 1.  Either row c is row c of the call (rows without a valid
 // target: zeros, word -1), or (compact) the rows with a valid target alone, in their order; then slot[i] is row i's place among
 // them (-1: none), live[0] their number, live[1] the slices for that many rows in blocks of block_rows, and the packed rows from
 // there to the end of the block (the first one, where there is no row) are zeros.
@@ -66,6 +66,7 @@ struct CePacked {
   int64_t pitch;
   int32_t* word;
   float *dloss, *lse;      // null in the forward pass
+  float* hit;              // p - 1 at the target; null where the loss is not given
   float* largest;          // [ce_pack_ctas(n)] largest |dloss| among a CTA's rows; may be null
   bool compact;
   int32_t *slot, *live;
@@ -76,7 +77,7 @@ constexpr int CE_PACK_ROWS = 16, CE_COUNT_ROWS = 1024;
 inline int64_t ce_pack_ctas(int64_t n) { return tiles(n, CE_PACK_ROWS); }
 
 // cross_entropy.cu
-int ce_pack(const CeProblem& q, const CePacked& p, const float* dloss, const float* lse, cudaStream_t s);
+int ce_pack(const CeProblem& q, const CePacked& p, const float* dloss, const float* lse, const float* loss, cudaStream_t s);
 // loss and lse from (maximum, sum) pairs of each packed row, [row][slices][groups].  live, slot: those of compact rows, or null.
 // word: that of packed rows; null: rows are those of the call, and the targets are looked at here.
 int ce_join(const CeProblem& q, const float* top, const float* total, int64_t groups, int64_t slices, const int32_t* live,
@@ -89,7 +90,7 @@ int ce_sum(const float* parts, int64_t splits, int64_t n, int64_t D, int64_t row
 size_t ce_mma_forward_bytes(int64_t n, int64_t D, int64_t V);
 size_t ce_mma_backward_bytes(int64_t n, int64_t D, int64_t V);
 int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s);
-int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, void* dhidden, void* dweight, cudaStream_t s);
+int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, const float* loss, void* dhidden, void* dweight, cudaStream_t s);
 
 #ifdef __CUDACC__
 // a row's target as a word, -1 where it is ignored or no class

@@ -161,6 +161,7 @@ struct alignas(64) MmaArgs {
   float *loss_out, *lse_out;  // STATS, NARROW: the rows' results, where there is one slice and rows are those of the call; else null
   const float* dloss;
   const float* lse;
+  const float* hit;      // the targets' entries p - 1; null: from lse
   uint16_t* g;           // FEW_GRAD: G, rows low_pitch elements apart
   uint16_t* low;         // (FEW_)GRAD: the second plane of G, rows low_pitch elements apart; null: there is one plane
   int64_t low_pitch;
@@ -496,17 +497,18 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
     uint32_t acc_phase = 0;
     const float factor = MODE == FEW_GRAD ? grad_factor(a.largest, a.largest_count, lane, false) : 1.0f;
     int32_t word[FEW_EACH];
-    float grad[FEW_EACH], lse[FEW_EACH];
+    float grad[FEW_EACH], lse[FEW_EACH], hit[FEW_EACH];
 #pragma unroll
     for (int r = 0; r < FEW_EACH; ++r) {
       word[r] = -1;
-      grad[r] = lse[r] = 0.0f;
+      grad[r] = lse[r] = hit[r] = 0.0f;
       if (r0 + r < ext.rows) {
         bool wrong;
         word[r] = MODE == FEW_GRAD || a.word != nullptr ? a.word[r0 + r] : target_word(a.target, a.ids64, r0 + r, a.V, a.ignore_index, &wrong);
         if (MODE == FEW_GRAD) {
           grad[r] = a.dloss[r0 + r] * factor;
           lse[r] = a.lse[r0 + r];
+          if (a.hit != nullptr) hit[r] = a.hit[r0 + r];
         }
       }
     }
@@ -547,7 +549,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
             float g = 0.0f;
             if (word[r] >= 0) {
               g = ex2((v - lse[r]) * LOG2E);
-              if (c + a.v0 == word[r]) g -= 1.0f;
+              if (c + a.v0 == word[r]) g = a.hit != nullptr ? hit[r] : g - 1.0f;
               g *= grad[r];
             }
             const uint32_t hi = pack2<BF16>(g, 0.0f);
@@ -593,7 +595,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
     // what a row brings along; GRAD's next row is asked for a tile ahead
     const int32_t my_row = static_cast<int32_t>(rank) * M_CTA + quarter * 32 + lane;
     int32_t next_word = -1;
-    float next_grad = 0.0f, next_lse = 0.0f;
+    float next_grad = 0.0f, next_lse = 0.0f, next_hit = 0.0f;
     auto ask = [&](int item) {
       const int32_t row = tile_of<MODE>(a, ext, item, 0).m0 + my_row;
       next_word = -1;
@@ -603,6 +605,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
       if (MODE == GRAD) {
         next_grad = a.dloss[row];
         next_lse = a.lse[row];
+        if (a.hit != nullptr) next_hit = a.hit[row];
       }
     };
     if (MODE != PRODUCT) ask(pair);
@@ -615,7 +618,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
       RowSum sum;
       uint32_t logits[MODE == NARROW ? 32 : 1];
       const int32_t word = next_word;
-      const float grad = next_grad * factor, lse = next_lse;
+      const float grad = next_grad * factor, lse = next_lse, hit = next_hit;
       if (MODE != PRODUCT) ask(item + pairs);
       for (int t = t0; t < t1; ++t) {
         const Tile x = tile_of<MODE>(a, ext, item, t);
@@ -668,7 +671,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) __cluster_dims__(2, 1, 1) ce_m
               if (at < 32u && word >= 0) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                  if (i == static_cast<int>(at)) now[i] = __float_as_uint(__uint_as_float(now[i]) - grad);
+                  if (i == static_cast<int>(at)) now[i] = __float_as_uint(a.hit != nullptr ? grad * hit : __uint_as_float(now[i]) - grad);
               }
               if (word < 0) {
 #pragma unroll
@@ -964,7 +967,7 @@ struct MmaPlan {
   int64_t piece, splits, dpitch;
   int64_t planes;  // of G
   bool one_piece, compact, dh_first, few, few_weight;
-  size_t packed, word, slot, live, counts, weight, target_logit, top, total, dloss, lse, largest, g, dh;
+  size_t packed, word, slot, live, counts, weight, target_logit, top, total, dloss, lse, hit, largest, g, dh;
   size_t forward_bytes, backward_bytes;
 };
 
@@ -1047,6 +1050,7 @@ MmaPlan make_plan(int64_t n, int64_t D, int64_t V) {
   l = common;
   p.dloss = l.take(n * 4);
   p.lse = l.take(n * 4);
+  p.hit = l.take(n * 4);
   p.largest = l.take(ce_pack_ctas(n) * 4);
   p.g = l.take(p.planes * n * p.piece * 2);
   if (!(p.one_piece && p.splits == 1 && !p.compact)) p.dh = l.take(p.splits * p.row_blocks * M_TILE * p.dpitch * 4);
@@ -1121,7 +1125,7 @@ int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) 
   // A row's statistics depend on that row alone: rows that TMA can fetch need no packing (what an ignored row holds ends there)
   const bool where_they_lie = !p.compact && aligned_to(q.hidden, 16) && (q.n == 1 ? q.D : q.hidden_stride) % 8 == 0;
   if (!where_they_lie) {
-    if (int rc = ce_pack(q, r, nullptr, nullptr, s)) return rc;
+    if (int rc = ce_pack(q, r, nullptr, nullptr, nullptr, s)) return rc;
   }
   Weight w;
   if (int rc = fetchable_weight(q, p, &w, s)) return rc;
@@ -1160,13 +1164,14 @@ int ce_mma_forward(const CeProblem& q, float* loss, float* lse, cudaStream_t s) 
   return ce_join(q, a.top, a.total, p.few ? FEW_PARTS : COL_GROUPS, p.slices, p.few ? nullptr : r.live, a.word, r.slot, a.target_logit, loss, lse, s);
 }
 
-int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, void* dhidden, void* dweight, cudaStream_t s) {
+int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, const float* loss, void* dhidden, void* dweight, cudaStream_t s) {
   const MmaPlan p = make_plan(q.n, q.D, q.V);
   CePacked r = packed_rows(q, p);
   r.dloss = reinterpret_cast<float*>(q.ws + p.dloss);
   r.lse = reinterpret_cast<float*>(q.ws + p.lse);
   r.largest = reinterpret_cast<float*>(q.ws + p.largest);
-  if (int rc = ce_pack(q, r, dloss, lse, s)) return rc;
+  r.hit = loss != nullptr ? reinterpret_cast<float*>(q.ws + p.hit) : nullptr;
+  if (int rc = ce_pack(q, r, dloss, lse, loss, s)) return rc;
   const void* packed = r.rows;
   Weight w;
   if (int rc = fetchable_weight(q, p, &w, s)) return rc;
@@ -1194,6 +1199,7 @@ int ce_mma_backward(const CeProblem& q, const float* dloss, const float* lse, vo
     a.word = r.word;
     a.dloss = r.dloss;
     a.lse = r.lse;
+    a.hit = r.hit;
     a.largest = r.largest;
     a.largest_count = static_cast<int32_t>(ce_pack_ctas(q.n));
     a.status = q.status;

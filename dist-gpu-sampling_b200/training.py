@@ -44,19 +44,20 @@ def _define():
 
     class LinearCrossEntropy(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, hidden, weight, target, ignore_index):
+        def forward(ctx, hidden, weight, target, ignore_index, shown):
             loss, lse = ops._CAPI_linear_cross_entropy(hidden, weight, target, ignore_index)
-            ctx.save_for_backward(hidden, weight, target, lse)
+            # (a caller who sees the rows' losses may change them in place)
+            ctx.save_for_backward(hidden, weight, target, lse, loss.clone() if shown else loss)
             ctx.ignore_index = ignore_index
             return loss
 
         @staticmethod
         @torch.autograd.function.once_differentiable
         def backward(ctx, grad):
-            hidden, weight, target, lse = ctx.saved_tensors
+            hidden, weight, target, lse, loss = ctx.saved_tensors
             want_h, want_w = ctx.needs_input_grad[:2]
-            dh, dw = ops._CAPI_linear_cross_entropy_backward(grad, hidden, weight, target, lse, ctx.ignore_index, want_h, want_w)
-            return dh if want_h else None, dw if want_w else None, None, None
+            dh, dw = ops._CAPI_linear_cross_entropy_backward.from_loss(grad, hidden, weight, target, lse, loss, ctx.ignore_index, want_h, want_w)
+            return dh if want_h else None, dw if want_w else None, None, None, None
 
     _functions.update(norm=LayerNorm, loss=LinearCrossEntropy)
 
@@ -79,7 +80,7 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
         raise ValueError("linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
     if not _functions:
         _define()
-    loss = _functions["loss"].apply(hidden, weight, target, int(ignore_index))
+    loss = _functions["loss"].apply(hidden, weight, target, int(ignore_index), reduction == "none")
     if reduction == "none":
         return loss
     if reduction == "sum":

@@ -431,6 +431,16 @@ DGS_API int dgs_linear_cross_entropy_backward(const float* dloss, const void* hi
                                               const float* lse, int64_t n, int64_t D, int64_t V, int64_t ignore_index,
                                               void* dhidden, void* dweight, void* workspace, size_t workspace_bytes,
                                               int32_t* status, dgs_stream_t stream);
+/* The same with the forward call's loss as well (NULL: without), from which the
+ * targets' entries come: exp(s - lse) - 1 = expm1(-loss).  Out of lse alone they are
+ * within 2^-24 |lse| dloss, which is percents of them where the loss is 1e-4 at
+ * logits of 100. */
+DGS_API int dgs_linear_cross_entropy_backward_from_loss(const float* dloss, const void* hidden, int64_t hidden_stride,
+                                                        const void* weight, int64_t weight_stride, int32_t dtype,
+                                                        const void* target, int32_t ids64, const float* lse, const float* loss,
+                                                        int64_t n, int64_t D, int64_t V, int64_t ignore_index, void* dhidden,
+                                                        void* dweight, void* workspace, size_t workspace_bytes, int32_t* status,
+                                                        dgs_stream_t stream);
 
 /* One AdamW step (decoupled weight decay, bias correction) over `count` tensors:
  *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,
