@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(CE_THREADS) ce_pack_kernel(const __grid_consta
         a.to.dloss[to] = d;
         a.to.lse[to] = word >= 0 ? a.lse[row] : 0.0f;
         if (a.to.hit != nullptr) a.to.hit[to] = word >= 0 ? expm1f(-a.loss[row]) : 0.0f;
-        most = fmaxf(most, fabsf(d));
+        if (fabsf(d) < INFINITY) most = fmaxf(most, fabsf(d));  // (an infinite one would leave nothing of the others)
       }
     }
     const T* from = static_cast<const T*>(a.hidden) + row * a.stride;

@@ -67,7 +67,7 @@ struct CePacked {
   int32_t* word;
   float *dloss, *lse;      // null in the forward pass
   float* hit;              // p - 1 at the target; null where the loss is not given
-  float* largest;          // [ce_pack_ctas(n)] largest |dloss| among a CTA's rows; may be null
+  float* largest;          // [ce_pack_ctas(n)] largest finite |dloss| among a CTA's rows; may be null
   bool compact;
   int32_t *slot, *live;
   int32_t block_rows, col_tiles, slots;  // what slices_for takes
