@@ -156,6 +156,7 @@ ABI_SIGNATURES = {
     "dgs_adamw_slot_elems": (_I64, [_I64]),
     "dgs_adamw_step": (ctypes.c_int, [_AP, _I32, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _VP]),
     "dgs_adamw_step_8bit": (ctypes.c_int, [_AP, _I32, _VP, _VP, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _VP]),
+    "dgs_adamw_step_8bit_unbiased": (ctypes.c_int, [_AP, _I32, _VP, _VP, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _U64, _VP]),
     "dgs_adamw_state_values": (ctypes.c_int, [_VP, _I32, _VP, _I64, _VP, _VP]),
 }
 

@@ -576,5 +576,6 @@ TORCH_LIBRARY(dgs_ops, m) {
       .def("_CAPI_linear_cross_entropy_backward.from_loss", &LinearCrossEntropyBackwardFromLossCUDA)
       .def("_CAPI_adamw_step", &AdamWStepCUDA)
       .def("_CAPI_adamw_step_8bit", &AdamWStep8bitCUDA)
+      .def("_CAPI_adamw_step_8bit.unbiased", &AdamWStep8bitUnbiasedCUDA)
       .def("_CAPI_adamw_state_values", &AdamWStateValuesCUDA);
 }

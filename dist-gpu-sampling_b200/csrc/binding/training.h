@@ -323,11 +323,12 @@ inline void AdamWStepCUDA(std::vector<torch::Tensor> params, c10::List<c10::opti
   mark_written(list.written);
 }
 
-inline void AdamWStep8bitCUDA(std::vector<torch::Tensor> params, c10::List<c10::optional<torch::Tensor>> grads,
-                              std::vector<torch::Tensor> copies, torch::Tensor exp_avg, torch::Tensor exp_avg_scale,
-                              torch::Tensor exp_avg_sq, torch::Tensor exp_avg_sq_scale, double lr, double beta1, double beta2, double eps,
-                              double weight_decay, int64_t step) {
-  const char* op = "_CAPI_adamw_step_8bit";
+namespace {
+// seed: of codes rounded at random; null: the nearest codes
+inline void adamw_step_8bit(const char* op, const std::vector<torch::Tensor>& params, const c10::List<c10::optional<torch::Tensor>>& grads,
+                            const std::vector<torch::Tensor>& copies, const torch::Tensor& exp_avg, const torch::Tensor& exp_avg_scale,
+                            const torch::Tensor& exp_avg_sq, const torch::Tensor& exp_avg_sq_scale, double lr, double beta1, double beta2,
+                            double eps, double weight_decay, int64_t step, const int64_t* seed) {
   CHECK_CUDA(exp_avg);
   c10::cuda::CUDAGuard guard(exp_avg.device());
   const torch::Device dev = exp_avg.device();
@@ -338,10 +339,33 @@ inline void AdamWStep8bitCUDA(std::vector<torch::Tensor> params, c10::List<c10::
   check_moment(exp_avg_scale, torch::kFloat, blocks, dev, op, "exp_avg_scale");
   check_moment(exp_avg_sq_scale, torch::kFloat, blocks, dev, op, "exp_avg_sq_scale");
   check_written(op, list, {{&exp_avg, list.slots}, {&exp_avg_scale, blocks}, {&exp_avg_sq, list.slots}, {&exp_avg_sq_scale, blocks}});
-  DGS_CHECK_RC(dgs_adamw_step_8bit(list.tensors.data(), static_cast<int32_t>(list.tensors.size()), exp_avg.data_ptr<int8_t>(),
-                                   exp_avg_scale.data_ptr<float>(), exp_avg_sq.data_ptr<uint8_t>(), exp_avg_sq_scale.data_ptr<float>(),
-                                   lr, beta1, beta2, eps, weight_decay, step, current_stream()));
+  const dgs_adamw_tensor* ts = list.tensors.data();
+  const int32_t count = static_cast<int32_t>(list.tensors.size());
+  int8_t* m = exp_avg.data_ptr<int8_t>();
+  uint8_t* v = exp_avg_sq.data_ptr<uint8_t>();
+  float *ms = exp_avg_scale.data_ptr<float>(), *vs = exp_avg_sq_scale.data_ptr<float>();
+  if (seed == nullptr)
+    DGS_CHECK_RC(dgs_adamw_step_8bit(ts, count, m, ms, v, vs, lr, beta1, beta2, eps, weight_decay, step, current_stream()));
+  else
+    DGS_CHECK_RC(dgs_adamw_step_8bit_unbiased(ts, count, m, ms, v, vs, lr, beta1, beta2, eps, weight_decay, step,
+                                              static_cast<uint64_t>(*seed), current_stream()));
   mark_written(list.written);
+}
+}  // namespace
+
+inline void AdamWStep8bitCUDA(std::vector<torch::Tensor> params, c10::List<c10::optional<torch::Tensor>> grads,
+                              std::vector<torch::Tensor> copies, torch::Tensor exp_avg, torch::Tensor exp_avg_scale,
+                              torch::Tensor exp_avg_sq, torch::Tensor exp_avg_sq_scale, double lr, double beta1, double beta2, double eps,
+                              double weight_decay, int64_t step) {
+  adamw_step_8bit("_CAPI_adamw_step_8bit", params, grads, copies, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, lr, beta1, beta2,
+                  eps, weight_decay, step, nullptr);
+}
+inline void AdamWStep8bitUnbiasedCUDA(std::vector<torch::Tensor> params, c10::List<c10::optional<torch::Tensor>> grads,
+                                      std::vector<torch::Tensor> copies, torch::Tensor exp_avg, torch::Tensor exp_avg_scale,
+                                      torch::Tensor exp_avg_sq, torch::Tensor exp_avg_sq_scale, double lr, double beta1, double beta2,
+                                      double eps, double weight_decay, int64_t step, int64_t seed) {
+  adamw_step_8bit("_CAPI_adamw_step_8bit.unbiased", params, grads, copies, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, lr, beta1,
+                  beta2, eps, weight_decay, step, &seed);
 }
 
 inline torch::Tensor AdamWStateValuesCUDA(torch::Tensor codes, torch::Tensor scales) {

@@ -4,7 +4,8 @@
 //   p = (1 - lr wd) p - (m / (sqrt(v) / sqrt(1 - b2^t) + eps)) (lr / (1 - b1^t)),  copy = p in the copy's type
 //
 // Every element is read and written once: bound by HBM with moments in 32 bits (313 M parameters, gradients and copies in 16 bits:
-// 1.44 ms, 6.1 TB/s), by issue slots in 8 bits (60 M parameters: 244 us, 3.9 TB/s, some hundred instructions an element).
+// 1.44 ms, 6.1 TB/s), by issue slots in 8 bits (60 M parameters: nearest codes 252 us,
+// 3.8 TB/s, some hundred instructions an element; unbiased ones 358).
 //
 // The moments lie in flat buffers in which every tensor has a slot of whole 256-element blocks, so a warp's 256 elements are one
 // block of the 8-bit form and the list needs three pointers a tensor.  The list travels in the kernel's parameters (nothing is
@@ -14,12 +15,21 @@
 // squares give small values finer steps; the second moment is held as its root because that is what divides, and a root
 // that is not zero never gets the code zero, which would make its element's step arbitrarily large.
 //
+// A code is the nearest one, or (unbiased) the one below or above with the probabilities that leave the moment its mean.  The nearest
+// code is the better one for a single step, and over many it holds a moment fast: with b2 = 0.999 a moment changes by at most
+// 0.1 % a step downwards, and half a code is 2 / c of it, 0.8 % at c = 255, so beside a moment that grows or stays the
+// others of its block hardly fall, and grow only by large gradients.  256 elements, the gradients of half of them cut tenfold at
+// step 2000: their stored roots are 2.6 times the exact ones at step 4000 and 9.6 times at 8000, and the parameters have moved
+// 31 % wrong; unbiased, 0.99 times (a single one up to 1.3) and 6 %.  The random words are Philox's of (seed, step, element),
+// so the same call gives the same bits, whatever the launch.
+//
 // The arithmetic is 32-bit, operation by operation as written above: no contraction to fused multiply-add, IEEE division
 // and square root.  A moment that falls between two codes is then rounded the same way wherever the formula is evaluated
 // in 32 bits.
 #include <cmath>
 #include <type_traits>
 
+#include "philox.cuh"
 #include "train_common.cuh"
 
 namespace dgs {
@@ -58,6 +68,9 @@ struct Moments8 {
   float* m_scale;
   uint8_t* v;
   float* v_scale;
+};
+struct Moments8Unbiased : Moments8 {
+  uint64_t key;  // of the step's random words
 };
 
 // the new parameter; `root` receives that of the second moment
@@ -118,6 +131,21 @@ __device__ __forceinline__ void quick_codes(uint64_t x, float inverse, float ste
   far = fmaxf(far, fmaxf(fabsf(a), fabsf(b)));
   split2(whole, c0, c1);
 }
+// The code below a value, or the one above with the probability that leaves the value its mean.  A whole number may count as the one
+// above its predecessor with probability one.  The largest value's code is the last one.  Of an element's 32 random bits 11 are
+// the first moment's and 21 the second's, whose small changes go by small probabilities (0.001 c / 4 with b2 = 0.999).
+__device__ __forceinline__ float whole_below(float x) { return __fsub_rn(__fadd_rn(__fsub_rn(x, 0.5f), kRound), kRound); }
+// (`bits` of 23, as a number between 0 and 1)
+__device__ __forceinline__ float unit(uint32_t bits, float half) { return __uint_as_float(0x3f800000u | bits) - (1.0f - half); }
+__device__ __forceinline__ float unbiased_first(float part, uint32_t random) {  // part of the scale = (c / 127)^2
+  const float q = part * 16129.0f, c = whole_below(sqrt_near(q)), u = unit((random & 2047u) << 12, 0x1p-12f);
+  return fminf(u * (2.0f * c + 1.0f) < q - c * c ? c + 1.0f : c, 127.0f);
+}
+__device__ __forceinline__ float unbiased_second(float part, uint32_t random) {  // part of the scale = (c / 255)^2, of its square ^4
+  const float s = part * 65025.0f, c = whole_below(sqrt_near(s)), cc = c * c, above = cc + (2.0f * c + 1.0f);
+  const float u = unit((random >> 11) << 2, 0x1p-22f);
+  return fminf(u * ((above - cc) * (above + cc)) < (s - cc) * (s + cc) ? c + 1.0f : c, 255.0f);
+}
 // the low bytes of four whole numbers
 __device__ __forceinline__ uint32_t bytes_of(float a, float b, float c, float d) {
   const uint32_t ab = __byte_perm(__float_as_uint(a + kRound), __float_as_uint(b + kRound), 0x0040);
@@ -129,7 +157,7 @@ template <int N, typename Moments>
 __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant__ List<N> list, const int count,
                                                            const int64_t chunks, const Moments mo,
                                                            const __grid_constant__ Scalars k) {
-  constexpr bool kEight = std::is_same<Moments, Moments8>::value;
+  constexpr bool kEight = std::is_base_of<Moments8, Moments>::value, kUnbiased = std::is_same<Moments, Moments8Unbiased>::value;
   pdl_enter();
   for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     int lo = 0, hi = count - 1;
@@ -198,17 +226,34 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
       const float ma = warp_max_bits(mb), va = warp_max_bits(vb);
       const bool plain = ma >= 1e-30f && ma <= 1e30f && va >= 1e-30f && va <= 1e30f;  // scales that have an inverse
       const float mi = __fdiv_rn(1.0f, ma), vi = __fdiv_rn(1.0f, va);
-      float mc[AW_VALUES], vc[AW_VALUES], far_m = 0.0f, far_v = 0.0f;
+      float mc[AW_VALUES], vc[AW_VALUES];
+      if constexpr (kUnbiased) {
 #pragma unroll
-      for (int j = 0; j < AW_VALUES; j += 2) {
-        quick_codes(abs2(two(m[j], m[j + 1])), mi, 127.0f, far_m, &mc[j], &mc[j + 1]);
-        quick_codes(two(root[j], root[j + 1]), vi, 255.0f, far_v, &vc[j], &vc[j + 1]);
-      }
-      if (!plain || far_m >= 0.5f - 127.0f * 4.3e-7f || far_v >= 0.5f - 255.0f * 4.3e-7f) {  // some lane of one warp in fourteen
+        for (int j = 0; j < AW_VALUES; j += 4) {
+          const uint64_t four_of = static_cast<uint64_t>(at + j) >> 2;
+          const Philox4 r = philox4x32_10(mo.key, static_cast<uint32_t>(four_of), static_cast<uint32_t>(four_of >> 32), 0u, 0u);
+          const uint32_t random[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int j = 0; j < AW_VALUES; ++j) {
-          mc[j] = exact_code(fabsf(m[j]), ma, 127.0f);
-          vc[j] = exact_code(root[j], va, 255.0f);
+          for (int i = 0; i < 4; ++i) {
+            const float mp = plain ? fabsf(m[j + i]) * mi : ma > 0.0f ? __fdiv_rn(fabsf(m[j + i]), ma) : 0.0f;
+            const float vp = plain ? root[j + i] * vi : va > 0.0f ? __fdiv_rn(root[j + i], va) : 0.0f;
+            mc[j + i] = unbiased_first(mp, random[i]);
+            vc[j + i] = unbiased_second(vp, random[i]);
+          }
+        }
+      } else {
+        float far_m = 0.0f, far_v = 0.0f;
+#pragma unroll
+        for (int j = 0; j < AW_VALUES; j += 2) {
+          quick_codes(abs2(two(m[j], m[j + 1])), mi, 127.0f, far_m, &mc[j], &mc[j + 1]);
+          quick_codes(two(root[j], root[j + 1]), vi, 255.0f, far_v, &vc[j], &vc[j + 1]);
+        }
+        if (!plain || far_m >= 0.5f - 127.0f * 4.3e-7f || far_v >= 0.5f - 255.0f * 4.3e-7f) {  // some lane of one warp in fourteen
+#pragma unroll
+          for (int j = 0; j < AW_VALUES; ++j) {
+            mc[j] = exact_code(fabsf(m[j]), ma, 127.0f);
+            vc[j] = exact_code(root[j], va, 255.0f);
+          }
         }
       }
 #pragma unroll
@@ -347,16 +392,30 @@ extern "C" int dgs_adamw_step(const dgs_adamw_tensor* tensors, int32_t count, fl
   return step_all("adamw_step", tensors, count, Moments32{exp_avg, exp_avg_sq}, k, static_cast<cudaStream_t>(stream));
 }
 
+static int step_8bit(const char* who, const dgs_adamw_tensor* tensors, int32_t count, const Moments8& mo, const uint64_t* seed, double lr,
+                     double beta1, double beta2, double eps, double weight_decay, int64_t step, dgs_stream_t stream) {
+  Scalars k;
+  if (int rc = make_scalars(who, lr, beta1, beta2, eps, weight_decay, step, &k)) return rc;
+  DGS_REQUIRE(count <= 0 || (mo.m != nullptr && mo.v != nullptr && mo.m_scale != nullptr && mo.v_scale != nullptr && aligned_to(mo.m, 8) &&
+                             aligned_to(mo.v, 8)),
+              DGS_ERR_INVALID, "%s: moments that are null or not 8-byte aligned", who);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (seed == nullptr) return step_all(who, tensors, count, mo, k, s);
+  return step_all(who, tensors, count, Moments8Unbiased{mo, fold_rng_key(*seed, static_cast<uint64_t>(step))}, k, s);
+}
+
 extern "C" int dgs_adamw_step_8bit(const dgs_adamw_tensor* tensors, int32_t count, int8_t* exp_avg, float* exp_avg_scale,
                                    uint8_t* exp_avg_sq, float* exp_avg_sq_scale, double lr, double beta1, double beta2,
                                    double eps, double weight_decay, int64_t step, dgs_stream_t stream) {
-  Scalars k;
-  if (int rc = make_scalars("adamw_step_8bit", lr, beta1, beta2, eps, weight_decay, step, &k)) return rc;
-  DGS_REQUIRE(count <= 0 || (exp_avg != nullptr && exp_avg_sq != nullptr && exp_avg_scale != nullptr &&
-                             exp_avg_sq_scale != nullptr && aligned_to(exp_avg, 8) && aligned_to(exp_avg_sq, 8)),
-              DGS_ERR_INVALID, "adamw_step_8bit: moments that are null or not 8-byte aligned");
-  return step_all("adamw_step_8bit", tensors, count, Moments8{exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale}, k,
-                  static_cast<cudaStream_t>(stream));
+  return step_8bit("adamw_step_8bit", tensors, count, Moments8{exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale}, nullptr, lr, beta1,
+                   beta2, eps, weight_decay, step, stream);
+}
+
+extern "C" int dgs_adamw_step_8bit_unbiased(const dgs_adamw_tensor* tensors, int32_t count, int8_t* exp_avg, float* exp_avg_scale,
+                                            uint8_t* exp_avg_sq, float* exp_avg_sq_scale, double lr, double beta1, double beta2,
+                                            double eps, double weight_decay, int64_t step, uint64_t seed, dgs_stream_t stream) {
+  return step_8bit("adamw_step_8bit_unbiased", tensors, count, Moments8{exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale}, &seed, lr,
+                   beta1, beta2, eps, weight_decay, step, stream);
 }
 
 extern "C" int dgs_adamw_state_values(const void* codes, int32_t second, const float* scales, int64_t n, float* out,

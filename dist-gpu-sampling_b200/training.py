@@ -98,9 +98,14 @@ class AdamW:
     their own type, and gradients are taken from them: 16-bit model parameters with 32-bit masters.  A tensor without a
     gradient stays as it is, and the step does not count for it: the bias corrections go by the steps that a tensor's own
     moments have seen (`tensor_steps`; a launch for each of the counts that a step meets).  The moments lie in two flat
-    buffers, a slot of whole 256-element blocks for each tensor."""
+    buffers, a slot of whole 256-element blocks for each tensor.
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, copies=None):
+    bits=8: a moment's code is rounded down or up at random so that the moment keeps its mean over the steps.  The root of a second
+    moment whose code is c (255 for its block's largest, 255 sqrt(root / largest) for the others) then stands within some
+    sqrt(1 / (2 c)) of its value: 5 % beside the largest, 15 % at a hundredth of it.  seed: of that rounding; with the same seed the
+    same steps give the same bits."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=32, copies=None, seed=0):
         import torch
         if bits not in (32, 8):
             raise ValueError("AdamW: bits must be 32 or 8, got %r" % (bits,))
@@ -111,7 +116,7 @@ class AdamW:
         if self.copies and len(self.copies) != len(self.params):
             raise ValueError("AdamW: %d parameters and %d copies" % (len(self.params), len(self.copies)))
         self.lr, self.betas, self.eps, self.weight_decay, self.bits, self.steps = lr, tuple(betas), eps, weight_decay, bits, 0
-        self.tensor_steps = [0] * len(self.params)
+        self.tensor_steps, self.seed = [0] * len(self.params), int(seed)
         self._ops = _ops()
         blocks = sum(-(-p.numel() // 256) for p in self.params)
         dev = self.params[0].device
@@ -150,8 +155,8 @@ class AdamW:
             self._ops._CAPI_adamw_step(self.params, grads, self.copies, st["exp_avg"], st["exp_avg_sq"], self.lr, b1, b2, self.eps,
                                        self.weight_decay, step)
         else:
-            self._ops._CAPI_adamw_step_8bit(self.params, grads, self.copies, st["exp_avg"], st["exp_avg_scale"], st["exp_avg_sq"],
-                                            st["exp_avg_sq_scale"], self.lr, b1, b2, self.eps, self.weight_decay, step)
+            self._ops._CAPI_adamw_step_8bit.unbiased(self.params, grads, self.copies, st["exp_avg"], st["exp_avg_scale"], st["exp_avg_sq"],
+                                                     st["exp_avg_sq_scale"], self.lr, b1, b2, self.eps, self.weight_decay, step, self.seed)
 
     def moments(self):
         """(first, second) moments as two flat float32 tensors, laid out like the state."""

@@ -470,6 +470,13 @@ DGS_API int dgs_adamw_step(const dgs_adamw_tensor* tensors, int32_t count, float
 DGS_API int dgs_adamw_step_8bit(const dgs_adamw_tensor* tensors, int32_t count, int8_t* exp_avg, float* exp_avg_scale,
                                 uint8_t* exp_avg_sq, float* exp_avg_sq_scale, double lr, double beta1, double beta2, double eps,
                                 double weight_decay, int64_t step, dgs_stream_t stream);
+/* The same with each code rounded down or up at random, so that the moment keeps
+ * its mean: what many steps in a row need, whose small changes the nearest code
+ * would drop.  The random words are a function of (seed, step, place in the
+ * buffers): the same call gives the same bits. */
+DGS_API int dgs_adamw_step_8bit_unbiased(const dgs_adamw_tensor* tensors, int32_t count, int8_t* exp_avg, float* exp_avg_scale,
+                                         uint8_t* exp_avg_sq, float* exp_avg_sq_scale, double lr, double beta1, double beta2,
+                                         double eps, double weight_decay, int64_t step, uint64_t seed, dgs_stream_t stream);
 /* The moments that n codes (whole blocks) stand for; second != 0: codes of v. */
 DGS_API int dgs_adamw_state_values(const void* codes, int32_t second, const float* scales, int64_t n, float* out,
                                    dgs_stream_t stream);
