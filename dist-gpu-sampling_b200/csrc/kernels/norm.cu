@@ -586,6 +586,7 @@ constexpr int most_vectors() {
 struct Shape {
   int tpr, nv;
 };
+// (with_shape has a kernel for each shape that is returned here, and for no other)
 inline Shape shape_for(int64_t nvec, int vec, int most_nv) {
   const int nv16 = 16 / vec;
   if (vec > 1) {
@@ -600,9 +601,11 @@ inline Shape shape_for(int64_t nvec, int vec, int most_nv) {
     for (int nv = 2; nv <= 32; nv *= 2)
       if (nvec <= 32 * nv) return {32, nv};
   }
-  for (int nv = 1; nv <= 2; nv *= 2)
-    if (nvec <= 256 * nv) return {256, nv};
-  for (int nv = 1; nv <= most_nv; nv *= 2)
+  if (vec > 1) {
+    for (int nv = vec == 8 ? 1 : 2; nv <= 2; nv *= 2)
+      if (nvec <= 256 * nv) return {256, nv};
+  }
+  for (int nv = vec > 1 ? 2 : 4; nv <= most_nv; nv *= 2)
     if (nvec <= static_cast<int64_t>(512) * nv) return {512, nv};
   return {0, 0};
 }
@@ -674,10 +677,14 @@ int with_shape(const Shape& s, const F& f) {
           default: return f.template run<1, 32, 32>();
         }
       }
-    case 256: return s.nv == 1 ? f.template run<VEC, 256, 1>() : f.template run<VEC, 256, 2>();
+    case 256:
+      if constexpr (VEC == 8)
+        if (s.nv == 1) return f.template run<VEC, 256, 1>();
+      if constexpr (VEC > 1)
+        if (s.nv == 2) return f.template run<VEC, 256, 2>();
+      break;
     case 512:
-      if (s.nv == 1) return f.template run<VEC, 512, 1>();
-      if constexpr (MOST >= 2)
+      if constexpr (VEC > 1)
         if (s.nv == 2) return f.template run<VEC, 512, 2>();
       if constexpr (MOST >= 4)
         if (s.nv == 4) return f.template run<VEC, 512, 4>();
