@@ -136,6 +136,9 @@ class AdamW:
 
     def step(self, grads=None):
         """One step with `grads` (None in the place of a gradient that is absent), or with the tensors' own .grad."""
+        import torch
+        if self.params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a step that a CUDA graph recorded would repeat its count for ever; call step() outside of it")
         if grads is None:
             grads = [p.grad for p in self.copies or self.params]
         grads = list(grads)
