@@ -287,8 +287,6 @@ struct StatsArgs {
   float* total;  // [n][slices]
 };
 
-
-
 __global__ void __launch_bounds__(CE_THREADS, 2) ce_stats_kernel(const Operand<true> h, const Operand<true> w,
                                                                  const __grid_constant__ StatsArgs a) {
   __shared__ __align__(16) Stage sm;

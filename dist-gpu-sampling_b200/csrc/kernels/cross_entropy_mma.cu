@@ -16,8 +16,8 @@
 // What bounds it: at long rows the products (8 192 x 1 024 against 65 537 classes: forward 0.74 ms, 1.48 PFLOP/s; with the backward
 // pass 3.6 ms, 1.22 PFLOP/s over the four products, under the power cap), whose operands come out of L2 at the 47 bytes a clock and
 // SM that it gives (a fifth of the time is spent waiting for them); at rows of 128 the exponentials, 16 a clock and SM (1 024 rows
-// against 2.4 M classes: 0.81 ms, the unit is busy for 83 % of it) and in the backward pass G's way through HBM; with few rows the
-// reading of W (8 rows of 1 024 against 150 000 classes: 60 us, 5.1 TB/s).
+// against 2.4 M classes: 0.83 ms, the unit is busy for 79 % of it, at the 1.68 GHz that power leaves) and in the backward pass G's
+// way through HBM; with few rows the reading of W (8 rows of 1 024 against 150 000 classes: 60 us, 5.1 TB/s).
 // exp(s - m) = 2^((s - m) log2(e)): half a packed addition, half a packed multiplication and one ex2 an element.
 //
 // Every wait is bounded.  One that runs out marks the CTA's words as dead, all roles leave, the status word gets

@@ -7,8 +7,8 @@
         loss.backward()
         optimizer.step()
 
-Thin autograd and optimizer layers over torch.ops.dgs_ops._CAPI_layer_norm*, _CAPI_linear_cross_entropy* and
-_CAPI_adamw_step*, which may be called directly as well.  No counterparts in the reference, whose trainers take these from
+Autograd functions and an optimizer over torch.ops.dgs_ops._CAPI_layer_norm*, _CAPI_linear_cross_entropy* and
+_CAPI_adamw_step*, which may be called directly as well (without autograd).  No counterparts in the reference, whose trainers take these from
 torch (oppo_bench/single_node/chunktensor.py:120-172).  torch is imported with the first call, as in the rest of the package.
 """
 import importlib
@@ -64,7 +64,7 @@ def _define():
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over x's last dimension, with gradients for x, weight and bias.
-    x: float32, bfloat16 or float16; weight and bias of one type, x's or another of the three."""
+    x: float32, bfloat16 or float16; weight and bias of one type, x's or another of the three (a bias needs a weight)."""
     if not _functions:
         _define()
     return _functions["norm"].apply(x, weight, bias, float(eps))
@@ -73,7 +73,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="mean"):
     """Softmax cross entropy of the logits hidden @ weight.T against `target`, with gradients for hidden and weight.
 
-    hidden [n, D] and weight [V, D] share one type; target holds n ids (int64 or int32).  Rows whose target is ignore_index
+    hidden [n, D] and weight [V, D] share one type (16 bits run on the tensor cores; float32 runs on the CUDA cores, at about half the
+    speed of torch with the logits held); target holds n ids (int64 or int32).  Rows whose target is ignore_index
     count as nothing: loss 0, no gradient, whatever their hidden values are.  reduction: "mean" over the other rows (no such
     row: nan, as torch's cross_entropy has it), "sum", or "none" for one float32 loss per row."""
     if reduction not in ("mean", "sum", "none"):
