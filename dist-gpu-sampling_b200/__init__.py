@@ -84,12 +84,20 @@ class AdamWTensor(ctypes.Structure):
                 ("copy_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class Attention(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v")] + \
+               [(n, ctypes.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
+               [("q_offsets", ctypes.c_void_p), ("k_offsets", ctypes.c_void_p), ("n_q", ctypes.c_int64), ("n_k", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("seqs", "heads", "kv_heads", "d", "dtype", "ids64", "causal")] + [("scale", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/dgs_b200.h declares
 _I32, _I64, _U64, _VP, _SZ = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_size_t
 _DP, _SP = ctypes.POINTER(ChunkDesc), ctypes.POINTER(Segments)
 _I64P = ctypes.POINTER(ctypes.c_int64)
 _HP = ctypes.POINTER(Hop)
 _AP, _F32, _F64 = ctypes.POINTER(AdamWTensor), ctypes.c_float, ctypes.c_double
+_TP = ctypes.POINTER(Attention)
 ABI_SIGNATURES = {
     "dgs_last_error": (ctypes.c_char_p, []),
     "dgs_device_check": (ctypes.c_int, []),
@@ -158,6 +166,9 @@ ABI_SIGNATURES = {
     "dgs_adamw_step_8bit": (ctypes.c_int, [_AP, _I32, _VP, _VP, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _VP]),
     "dgs_adamw_step_8bit_unbiased": (ctypes.c_int, [_AP, _I32, _VP, _VP, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _U64, _VP]),
     "dgs_adamw_state_values": (ctypes.c_int, [_VP, _I32, _VP, _I64, _VP, _VP]),
+    "dgs_attention_workspace_bytes": (_SZ, [_TP, _I32]),
+    "dgs_attention_forward": (ctypes.c_int, [_TP, _VP, _VP, _VP, _SZ, _VP, _VP]),
+    "dgs_attention_backward": (ctypes.c_int, [_TP, _VP, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP]),
 }
 
 
@@ -361,4 +372,4 @@ def block_csc(coo_row, coo_col, n_dst, rows_sorted=True):
 from .placement import (CACHE_PRIORITY, get_available_memory, permute_edge_tensor, plan_capacities,  # noqa: E402,F401
                         reduce_min_over_ranks, renumber_by_degree)
 # the training step behind the samplers
-from .training import AdamW, layer_norm, linear_cross_entropy  # noqa: E402,F401
+from .training import AdamW, attention, layer_norm, linear_cross_entropy  # noqa: E402,F401

@@ -7,6 +7,7 @@ Plain nvcc / g++ command lines, no build system.  nvcc cross-compiles for
 sm_100a without a GPU; the built files stay in the tree (git-ignored) so that
 they travel with a snapshot of the repository.
 """
+import concurrent.futures
 import hashlib
 import os
 import shutil
@@ -29,6 +30,7 @@ ABI_SOURCES = [
     "kernels/cross_entropy.cu",
     "kernels/cross_entropy_mma.cu",
     "kernels/adamw.cu",
+    "kernels/attention.cu",
     "host/error.cc",
     "host/comm.cc",
     "host/store.cc",
@@ -44,6 +46,7 @@ HEADERS = [
     "kernels/train_common.cuh",
     "kernels/tensor_core.cuh",
     "kernels/cross_entropy.h",
+    "kernels/attention.h",
     "host/comm.h",
     "../../include/dgs_b200.h",
 ]
@@ -92,7 +95,7 @@ def build_abi(force=False, verbose=False, ptxas_info=False):
     os.makedirs(OBJ, exist_ok=True)
     headers = [os.path.join(CSRC, h) for h in HEADERS]
     flags = list(NVCC_FLAGS) + (["-Xptxas", "-v"] if ptxas_info else [])
-    objs, relink, log = [], force or not os.path.exists(abi_path()), ""
+    objs, relink, log, stale = [], force or not os.path.exists(abi_path()), "", []
     for rel in ABI_SOURCES:
         src = os.path.join(CSRC, rel)
         obj = os.path.join(OBJ, rel.replace("/", "_") + ".o")
@@ -100,12 +103,14 @@ def build_abi(force=False, verbose=False, ptxas_info=False):
         dig = _digest([src] + headers, " ".join(flags))
         old = open(stamp).read() if os.path.exists(stamp) else ""
         if force or ptxas_info or old != dig or not os.path.exists(obj):
-            cmd = [_nvcc()] + flags + ["-x", "cu", "-c", src, "-o", obj]
-            log += _run(cmd, verbose)
-            with open(stamp, "w") as f:
-                f.write(dig)
+            stale.append(([_nvcc()] + flags + ["-x", "cu", "-c", src, "-o", obj], stamp, dig))
             relink = True
         objs.append(obj)
+    with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count()) as pool:
+        for (_, stamp, dig), out in zip(stale, pool.map(lambda job: _run(job[0], verbose), stale)):
+            log += out
+            with open(stamp, "w") as f:
+                f.write(dig)
     if relink:
         cmd = [_nvcc(), "-shared", "-cudart", "shared", "-o", abi_path()] + objs + [
             "-ldl", "-Xlinker", "-rpath", "-Xlinker", "/usr/local/cuda/lib64"]
@@ -120,7 +125,8 @@ def build_binding(force=False, verbose=False):
 
     src = os.path.join(CSRC, "binding", "ops.cc")
     hdrs = [os.path.join(ROOT, "include", "dgs_b200.h")] + \
-        [os.path.join(CSRC, "binding", h) for h in ("chunk_tensor.h", "host_words.h", "pipeline.h", "training.h")]
+        [os.path.join(CSRC, "binding", h) for h in ("chunk_tensor.h", "host_words.h", "pipeline.h", "training.h",
+                                                        "training_block.h")]
     out = binding_path()
     stamp = out + ".sha"
     dig = _digest([src] + hdrs, torch.__version__)

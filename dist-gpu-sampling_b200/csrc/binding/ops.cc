@@ -4,7 +4,8 @@
 // of include/dgs_b200.h.  Only this directory (binding/) sees torch types; every
 // kernel launch goes through an extern "C" entry point.  chunk_tensor.h holds the
 // ChunkTensor class, host_words.h the pinned size / status words leased per call,
-// pipeline.h the BlockPipeline class (several mini-batches in flight), training.h the operators of a training step.
+// pipeline.h the BlockPipeline class (several mini-batches in flight), training.h and training_block.h the operators of a training
+// step.
 //
 // Conventions kept from the reference: one process per GPU, tensors returned
 // on the current CUDA device, ChunkTensor construction/destruction collective
@@ -31,6 +32,7 @@
 #include "host_words.h"
 #include "pipeline.h"
 #include "training.h"
+#include "training_block.h"
 
 namespace dgs {
 namespace {
@@ -577,5 +579,8 @@ TORCH_LIBRARY(dgs_ops, m) {
       .def("_CAPI_adamw_step", &AdamWStepCUDA)
       .def("_CAPI_adamw_step_8bit", &AdamWStep8bitCUDA)
       .def("_CAPI_adamw_step_8bit.unbiased", &AdamWStep8bitUnbiasedCUDA)
-      .def("_CAPI_adamw_state_values", &AdamWStateValuesCUDA);
+      .def("_CAPI_adamw_state_values", &AdamWStateValuesCUDA)
+      // ... and of the blocks of a model in front of it, see training_block.h
+      .def("_CAPI_attention", &AttentionCUDA)
+      .def("_CAPI_attention_backward", &AttentionBackwardCUDA);
 }

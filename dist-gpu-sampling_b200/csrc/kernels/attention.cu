@@ -1,0 +1,776 @@
+// Softmax attention of packed sequences: queries rows [q_offsets[s], q_offsets[s + 1]), keys and values rows of k_offsets; query head
+// a reads key head a / (heads / kv_heads); with `causal` query i of Lq sees the keys j <= i + Lk - Lq.
+//
+//   x_ij = scale q_i.k_j,  lse_i = log sum_j exp x_ij,  p_ij = exp(x_ij - lse_i),  o_i = sum_j p_ij v_j    (no key: o = 0, lse = -inf)
+//   dv_j = sum_i p_ij do_i,  e_ij = do_i.v_j,  delta_i = sum_j p_ij e_ij,  ds_ij = p_ij (e_ij - delta_i),
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i   (over all queries and heads that read j)
+//
+// This file: the plan of a call, and the rows of sequences with few queries (a seed over its sampled neighbours, a read-out over
+// a graph) and of 32-bit operands, on the CUDA cores; sequences of at least ATTN_TILE_QUERIES queries in 16 bits are tiles on the
+// tensor cores (attention_mma.cu).  Nothing is added by atomics: the same inputs give the same bits.
+#include "attention.h"
+
+namespace dgs {
+namespace {
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_ONE_CTA = 2048;  // sequences up to which one CTA makes the plan and clears its counts itself
+constexpr int ROW_WARPS = 8;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// ---- plan -----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int64_t offset_at(const void* p, int32_t wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+// A warp for each sequence: its place, whose its rows are, the parts of rows with many keys, the tiles of long ones.
+__global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_constant__ AttnArgs a, int32_t backward, int32_t clear) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31;
+  if (clear) {
+    if (threadIdx.x < ATTN_COUNTS) a.counts[threadIdx.x] = 0;
+    if (threadIdx.x < 2 && a.norms != nullptr) a.norms[threadIdx.x] = 0.0f;
+    __syncthreads();
+  }
+  const int warps = gridDim.x * (PLAN_THREADS / 32);
+  for (int s = blockIdx.x * (PLAN_THREADS / 32) + (threadIdx.x >> 5); s < a.seqs; s += warps) {
+    const int64_t q0 = offset_at(a.q_offsets, a.offsets64, s), q1 = offset_at(a.q_offsets, a.offsets64, s + 1);
+    const int64_t k0 = offset_at(a.k_offsets, a.offsets64, s), k1 = offset_at(a.k_offsets, a.offsets64, s + 1);
+    AttnSeq e{0, 0, 0, 0};
+    if (q0 >= 0 && q0 <= q1 && q1 <= a.n_q && k0 >= 0 && k0 <= k1 && k1 <= a.n_k)
+      e = {static_cast<int32_t>(q0), static_cast<int32_t>(q1 - q0), static_cast<int32_t>(k0), static_cast<int32_t>(k1 - k0)};
+    else if (lane == 0)
+      raise_status(a.status, DGS_ERR_RANGE);
+    if (lane == 0) a.seq[s] = e;
+    for (int i = lane; i < e.q_len; i += 32) a.q_seq[e.q0 + i] = s;
+    if (backward)
+      for (int i = lane; i < e.k_len; i += 32) a.k_seq[e.k0 + i] = s;
+    if (attn_in_tiles(a, e)) continue;
+    if (attn_is_split(e) && e.q_len > 0) {
+      const int parts = (e.k_len + ATTN_SPLIT_KEYS - 1) / ATTN_SPLIT_KEYS, all = parts * e.q_len;
+      int first = 0;
+      if (lane == 0) first = atomicAdd(&a.counts[ATTN_N_SPLITS], all);
+      first = __shfl_sync(FULL_MASK, first, 0);
+      for (int i = lane; i < all; i += 32) {
+        const int row = i / parts, part = i - row * parts;
+        if (first + i >= a.split_bound) break;  // (cannot be: the bound is of the sizes; offsets that overlap may get here)
+        a.splits[first + i] = make_int4(e.q0 + row, part * ATTN_SPLIT_KEYS, first + row * parts, parts);
+        for (int c = 0; c < a.kv_heads; ++c) a.arrived[static_cast<int64_t>(first + i) * a.kv_heads + c] = 0;
+      }
+    }
+  }
+}
+
+// ---- rows: a group of G lanes holds a row of DP elements, VEC of them a lane; a warp holds 32 / G keys at once ------------
+template <typename T>
+constexpr int vec_of() {
+  return 16 / static_cast<int>(sizeof(T));
+}
+constexpr int UNROLL = 4;
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_row(const T* p, bool there, float (&v)[VEC]) {
+  if (there) {
+    load_vec<T, VEC>(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
+  }
+}
+template <int VEC>
+__device__ __forceinline__ float dot(const float (&a)[VEC], const float (&b)[VEC]) {
+  float s = a[0] * b[0];
+#pragma unroll
+  for (int e = 1; e < VEC; ++e) s = fmaf(a[e], b[e], s);
+  return s;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
+  return v;
+}
+
+// The keys j0 + first, .. of one row, every `step` batches: running maximum (of log2 values), sum and weighted values of R heads, each
+// group of lanes with its own.
+template <typename T, int DP, int R>
+__device__ __forceinline__ void forward_keys(const T* k, int64_t k_row, const T* v, int64_t v_row, int j0, int j1, int step, bool in_d,
+                                             const float (&q)[R][vec_of<T>()], float (&m)[R], float (&l)[R], float (&acc)[R][vec_of<T>()]) {
+  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G;
+  const int sub = (threadIdx.x & 31) / G;
+  for (int j = j0; j < j1; j += step) {
+    Vec<T, VEC> kr[UNROLL], vr[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int at = j + u * KEYS + sub;
+      const bool there = at < j1 && in_d;
+      kr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(k + at * k_row) : Vec<T, VEC>{};
+      vr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(v + at * v_row) : Vec<T, VEC>{};
+    }
+    float x[R][UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      float kf[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) kf[e] = to_float<T>(kr[u].v[e]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r][u] = group_sum<G>(dot<VEC>(q[r], kf));
+    }
+    float scale[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = m[r];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        if (j + u * KEYS + sub >= j1) x[r][u] = -INFINITY;
+        top = fmaxf(top, x[r][u]);
+      }
+      const float ref = top == -INFINITY ? 0.0f : top;
+      scale[r] = exp2f(m[r] - ref);
+      m[r] = top;
+      l[r] *= scale[r];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        x[r][u] = exp2f(x[r][u] - ref);
+        l[r] += x[r][u];
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[r][e] *= scale[r];
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float f = to_float<T>(vr[u].v[e]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][e] = fmaf(x[r][u], f, acc[r][e]);
+      }
+  }
+}
+
+// (m, l, acc) of two sets of keys joined
+template <int VEC>
+__device__ __forceinline__ void join(float& m, float& l, float (&acc)[VEC], float m2, float l2, const float (&acc2)[VEC]) {
+  const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
+  const float s1 = exp2f(m - ref), s2 = exp2f(m2 - ref);
+  l = l * s1 + l2 * s2;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[e] = acc[e] * s1 + acc2[e] * s2;
+  m = top;
+}
+
+// the lanes that hold the same elements of other keys
+template <int G, int VEC>
+__device__ __forceinline__ void join_groups(float& m, float& l, float (&acc)[VEC]) {
+#pragma unroll
+  for (int o = G; o < 32; o <<= 1) {
+    float other[VEC];
+    const float m2 = __shfl_xor_sync(FULL_MASK, m, o), l2 = __shfl_xor_sync(FULL_MASK, l, o);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) other[e] = __shfl_xor_sync(FULL_MASK, acc[e], o);
+    join<VEC>(m, l, acc, m2, l2, other);
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void finish_row(const AttnArgs& a, int row, int head, int vec, bool writes, float m, float l, const float (&acc)[VEC]) {
+  if (!writes) return;
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (nan stays nan)
+  float o[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) o[e] = acc[e] * inv;
+  store_vec<T, VEC>(static_cast<T*>(a.out) + (static_cast<int64_t>(row) * a.heads + head) * a.d + vec * VEC, o);
+  if (vec == 0) a.lse[static_cast<int64_t>(head) * a.n_q + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// The sequence of a row, or none (a row outside of all of them)
+__device__ __forceinline__ AttnSeq sequence_of(const AttnArgs& a, const int32_t* map, int row, bool key, bool* found) {
+  const int s = map[row];
+  AttnSeq e{0, 0, 0, 0};
+  *found = false;
+  if (s >= 0 && s < a.seqs) {
+    e = a.seq[s];
+    const int at = row - (key ? e.k0 : e.q0);
+    *found = at >= 0 && at < (key ? e.k_len : e.q_len);
+  }
+  return e;
+}
+
+// keys that a query sees
+__device__ __forceinline__ int keys_seen(const AttnArgs& a, const AttnSeq& e, int row) {
+  if (!a.causal) return e.k_len;
+  const int n = row - e.q0 + 1 + e.k_len - e.q_len;
+  return n < 0 ? 0 : n < e.k_len ? n : e.k_len;
+}
+
+template <typename T, int DP, int R>
+__device__ __forceinline__ void load_heads(const AttnView& x, int row, int head0, int heads, int vec, bool in_d, float by,
+                                           float (&q)[R][vec_of<T>()]) {
+  constexpr int VEC = vec_of<T>();
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    load_row<T, VEC>(static_cast<const T*>(x.p) + row * x.row + (head0 + r) * x.head + vec * VEC, in_d && r < heads, q[r]);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) q[r][e] *= by;
+  }
+}
+
+// A warp for each query row and key head, for the heads of its group R at a time; the first `split_ctas` CTAs take the parts of
+// rows with many keys, the last part of a row to be there joins them in their order.
+// Bound by HBM where every query has keys of its own.
+template <typename T, int DP, int R>
+__global__ __launch_bounds__(ROW_WARPS * 32) void attn_rows_kernel(const __grid_constant__ AttnArgs a, int32_t split_ctas) {
+  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G;
+  __shared__ float shared[ROW_WARPS][DP + 2];
+  __shared__ bool last;
+  pdl_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vec = lane % G, group = a.heads / a.kv_heads;
+  const bool in_d = vec * VEC < a.d;
+  if (static_cast<int>(blockIdx.x) < split_ctas) {
+    const int floats = a.d + 2, n = min(a.counts[ATTN_N_SPLITS], a.split_bound);
+    for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * a.kv_heads; t += split_ctas) {
+      const int item = static_cast<int>(t / a.kv_heads), c = static_cast<int>(t - static_cast<int64_t>(item) * a.kv_heads);
+      const int4 it = a.splits[item];
+      bool found;
+      const AttnSeq e = sequence_of(a, a.q_seq, it.x, false, &found);
+      const int seen = found ? keys_seen(a, e, it.x) : 0, j0 = it.y, j1 = min(seen, j0 + ATTN_SPLIT_KEYS);
+      const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + vec * VEC;
+      const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + vec * VEC;
+      for (int h0 = 0; h0 < group; h0 += R) {
+        const int heads = min(R, group - h0);
+        float q[R][VEC], m[R], l[R], acc[R][VEC];
+        load_heads<T, DP, R>(a.q, it.x, c * group + h0, heads, vec, in_d, a.scale * LOG2E, q);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          m[r] = -INFINITY;
+          l[r] = 0.0f;
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) acc[r][x] = 0.0f;
+        }
+        forward_keys<T, DP, R>(k, a.k.row, v, a.v.row, j0 + warp * KEYS * UNROLL, j1, ROW_WARPS * KEYS * UNROLL, in_d, q, m, l, acc);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          join_groups<G, VEC>(m[r], l[r], acc[r]);
+          if (r >= heads) continue;  // (the same for all threads)
+          __syncthreads();           // `shared` may be written again
+          if (lane < G) {
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) shared[warp][vec * VEC + x] = acc[r][x];
+            if (lane == 0) {
+              shared[warp][DP] = m[r];
+              shared[warp][DP + 1] = l[r];
+            }
+          }
+          __syncthreads();
+          // the warps' parts, an element a thread
+          float top = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < ROW_WARPS; ++w) top = fmaxf(top, shared[w][DP]);
+          const float ref = top == -INFINITY ? 0.0f : top;
+          float* part = a.parts + (static_cast<int64_t>(item) * a.heads + c * group + h0 + r) * floats;
+          for (int x = threadIdx.x; x <= a.d; x += ROW_WARPS * 32) {
+            const int at = x < a.d ? x : DP + 1;
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < ROW_WARPS; ++w) sum += shared[w][at] * exp2f(shared[w][DP] - ref);
+            part[x < a.d ? x : a.d + 1] = sum;
+            if (x == 0) part[a.d] = top;
+          }
+        }
+      }
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0)
+        last = atomicAdd(&a.arrived[static_cast<int64_t>(it.z) * a.kv_heads + c], 1u) + 1 == static_cast<uint32_t>(it.w);
+      __syncthreads();
+      if (last && found) {
+        __threadfence();
+        for (int h = warp; h < group; h += ROW_WARPS) {
+          const int head = c * group + h;
+          const float* part = a.parts + (static_cast<int64_t>(it.z) * a.heads + head) * floats;
+          const int64_t apart = static_cast<int64_t>(a.heads) * floats;
+          float top = -INFINITY;
+          for (int p = lane; p < it.w; p += 32) top = fmaxf(top, __ldcg(part + p * apart + a.d));
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+          const float ref = top == -INFINITY ? 0.0f : top;
+          float l = 0.0f, acc[DP / 32];
+#pragma unroll
+          for (int x = 0; x < DP / 32; ++x) acc[x] = 0.0f;
+#pragma unroll 4
+          for (int p = 0; p < it.w; ++p) {
+            const float by = exp2f(__ldcg(part + p * apart + a.d) - ref);
+            l += __ldcg(part + p * apart + a.d + 1) * by;
+#pragma unroll
+            for (int x = 0; x < DP / 32; ++x)
+              if (x * 32 + lane < a.d) acc[x] += __ldcg(part + p * apart + x * 32 + lane) * by;
+          }
+#pragma unroll
+          for (int x = 0; x < DP / 32; ++x) {
+            const float one[1] = {acc[x]};
+            const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+            if (x * 32 + lane < a.d)
+              static_cast<T*>(a.out)[(static_cast<int64_t>(it.x) * a.heads + head) * a.d + x * 32 + lane] = from_float<T>(one[0] * inv);
+          }
+          if (lane == 0) a.lse[static_cast<int64_t>(head) * a.n_q + it.x] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
+        }
+      }
+      __syncthreads();  // `last` may be written again
+    }
+    return;
+  }
+  const int64_t t = static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp;
+  if (t >= static_cast<int64_t>(a.n_q) * a.kv_heads) return;
+  const int row = static_cast<int>(t / a.kv_heads), c = static_cast<int>(t - static_cast<int64_t>(row) * a.kv_heads);
+  bool found;
+  const AttnSeq e = sequence_of(a, a.q_seq, row, false, &found);
+  if (found && (attn_in_tiles(a, e) || attn_is_split(e))) return;
+  const int seen = found ? keys_seen(a, e, row) : 0;
+  const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + vec * VEC;
+  const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + vec * VEC;
+  for (int h0 = 0; h0 < group; h0 += R) {
+    const int heads = min(R, group - h0);
+    float q[R][VEC], m[R], l[R], acc[R][VEC];
+    load_heads<T, DP, R>(a.q, row, c * group + h0, heads, vec, in_d && seen > 0, a.scale * LOG2E, q);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < VEC; ++x) acc[r][x] = 0.0f;
+    }
+    forward_keys<T, DP, R>(k, a.k.row, v, a.v.row, 0, seen, KEYS * UNROLL, in_d, q, m, l, acc);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      join_groups<G, VEC>(m[r], l[r], acc[r]);
+      finish_row<T, VEC>(a, row, c * group + h0 + r, vec, lane < G && in_d && r < heads, m[r], l[r], acc[r]);
+    }
+  }
+}
+
+// ---- backward --------------------------------------------------------------------------------------------------------
+// Over some keys of one row, for R heads: sum p e k, sum p k (so that dq = scale (the first - delta times the second) takes one pass) and
+// sum p e = delta.  `ref`: log2-sum-exp of the row.
+template <typename T, int DP, int R>
+__device__ __forceinline__ void backward_keys(const T* k, int64_t k_row, const T* v, int64_t v_row, int j0, int j1, int step, bool in_d,
+                                              const float (&q)[R][vec_of<T>()], const float (&g)[R][vec_of<T>()], const float (&ref)[R],
+                                              float (&pek)[R][vec_of<T>()], float (&pk)[R][vec_of<T>()], float (&delta)[R]) {
+  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G, U = 2;
+  const int sub = (threadIdx.x & 31) / G;
+  for (int j = j0; j < j1; j += step) {
+    Vec<T, VEC> kr[U], vr[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = j + u * KEYS + sub;
+      const bool there = at < j1 && in_d;
+      kr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(k + at * k_row) : Vec<T, VEC>{};
+      vr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(v + at * v_row) : Vec<T, VEC>{};
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float kf[VEC], vf[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        kf[e] = to_float<T>(kr[u].v[e]);
+        vf[e] = to_float<T>(vr[u].v[e]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float x = group_sum<G>(dot<VEC>(q[r], kf)), e = group_sum<G>(dot<VEC>(g[r], vf));
+        const float p = j + u * KEYS + sub < j1 ? exp2f(x - ref[r]) : 0.0f;
+        delta[r] = fmaf(p, e, delta[r]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          pek[r][i] = fmaf(p * e, kf[i], pek[r][i]);
+          pk[r][i] = fmaf(p, kf[i], pk[r][i]);
+        }
+      }
+    }
+  }
+}
+template <int G, int VEC>
+__device__ __forceinline__ void add_groups(float (&v)[VEC]) {
+#pragma unroll
+  for (int o = G; o < 32; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] += __shfl_xor_sync(FULL_MASK, v[e], o);
+}
+template <int G>
+__device__ __forceinline__ float add_groups(float v) {
+#pragma unroll
+  for (int o = G; o < 32; o <<= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
+  return v;
+}
+
+// dq and delta, in the shape of attn_rows_kernel
+template <typename T, int DP, int R>
+__global__ __launch_bounds__(ROW_WARPS * 32) void attn_rows_dq_kernel(const __grid_constant__ AttnArgs a, int32_t split_ctas) {
+  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G, U = 2;
+  __shared__ float shared[ROW_WARPS][2 * DP + 1];
+  __shared__ bool last;
+  pdl_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vec = lane % G, group = a.heads / a.kv_heads;
+  const bool in_d = vec * VEC < a.d;
+  const bool splits = static_cast<int>(blockIdx.x) < split_ctas;
+  const int n_splits = splits ? min(a.counts[ATTN_N_SPLITS], a.split_bound) : 0;
+  const int64_t tasks = splits ? static_cast<int64_t>(n_splits) * a.kv_heads : static_cast<int64_t>(a.n_q) * a.kv_heads;
+  const int64_t step = splits ? split_ctas : tasks;  // (a row's warp has one task)
+  for (int64_t t = splits ? blockIdx.x : static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp; t < tasks; t += step) {
+    const int item = static_cast<int>(t / a.kv_heads), c = static_cast<int>(t - static_cast<int64_t>(item) * a.kv_heads);
+    const int4 it = splits ? a.splits[item] : make_int4(item, 0, 0, 0);
+    const int row = it.x;
+    bool found;
+    const AttnSeq e = sequence_of(a, a.q_seq, row, false, &found);
+    if (!splits && found && (attn_in_tiles(a, e) || attn_is_split(e))) return;
+    const int seen = found ? keys_seen(a, e, row) : 0;
+    const int j0 = it.y, j1 = splits ? min(seen, j0 + ATTN_SPLIT_KEYS) : seen;
+    const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + vec * VEC;
+    const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + vec * VEC;
+    const int floats = 2 * a.d + 1;
+    for (int h0 = 0; h0 < group; h0 += R) {
+      const int heads = min(R, group - h0), head = c * group + h0;
+      float q[R][VEC], g[R][VEC], ref[R], pek[R][VEC], pk[R][VEC], delta[R];
+      load_heads<T, DP, R>(a.q, row, head, heads, vec, in_d && seen > 0, a.scale * LOG2E, q);
+      load_heads<T, DP, R>(a.dout, row, head, heads, vec, in_d && seen > 0, 1.0f, g);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        ref[r] = seen > 0 && r < heads ? a.lse[static_cast<int64_t>(head + r) * a.n_q + row] * LOG2E : 0.0f;
+        if (ref[r] == -INFINITY) ref[r] = INFINITY;  // (a row that had no finite score has no weights)
+        delta[r] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) pek[r][x] = pk[r][x] = 0.0f;
+      }
+      backward_keys<T, DP, R>(k, a.k.row, v, a.v.row, splits ? j0 + warp * KEYS * U : 0, j1, (splits ? ROW_WARPS : 1) * KEYS * U, in_d, q, g,
+                              ref, pek, pk, delta);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        add_groups<G, VEC>(pek[r]);
+        add_groups<G, VEC>(pk[r]);
+        delta[r] = add_groups<G>(delta[r]);
+        if (r >= heads) continue;  // (the same for all threads of a warp, and of a CTA where parts are added)
+        if (!splits) {
+          if (lane < G && in_d) {
+            float dq[VEC];
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) dq[x] = a.scale * fmaf(-delta[r], pk[r][x], pek[r][x]);
+            if (a.dq != nullptr)
+              store_vec<T, VEC>(static_cast<T*>(a.dq) + (static_cast<int64_t>(row) * a.heads + head + r) * a.d + vec * VEC, dq);
+            if (vec == 0) a.delta[static_cast<int64_t>(head + r) * a.n_q + row] = delta[r];
+          }
+          continue;
+        }
+        __syncthreads();  // `shared` may be written again
+        if (lane < G) {
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) {
+            shared[warp][vec * VEC + x] = pek[r][x];
+            shared[warp][DP + vec * VEC + x] = pk[r][x];
+          }
+          if (lane == 0) shared[warp][2 * DP] = delta[r];
+        }
+        __syncthreads();
+        float* part = a.parts + (static_cast<int64_t>(item) * a.heads + head + r) * floats;
+        for (int x = threadIdx.x; x < floats; x += ROW_WARPS * 32) {
+          const int at = x < a.d ? x : x < 2 * a.d ? DP + x - a.d : 2 * DP;
+          float sum = 0.0f;
+#pragma unroll
+          for (int w = 0; w < ROW_WARPS; ++w) sum += shared[w][at];
+          part[x] = sum;
+        }
+      }
+    }
+    if (!splits) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0)
+      last = atomicAdd(&a.arrived[static_cast<int64_t>(it.z) * a.kv_heads + c], 1u) + 1 == static_cast<uint32_t>(it.w);
+    __syncthreads();
+    if (last && found) {
+      __threadfence();
+      for (int h = warp; h < group; h += ROW_WARPS) {
+        const int head = c * group + h;
+        const float* part = a.parts + (static_cast<int64_t>(it.z) * a.heads + head) * floats;
+        const int64_t apart = static_cast<int64_t>(a.heads) * floats;
+        float delta = 0.0f, pek[DP / 32], pk[DP / 32];
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x) pek[x] = pk[x] = 0.0f;
+#pragma unroll 4
+        for (int p = 0; p < it.w; ++p) {
+          delta += __ldcg(part + p * apart + 2 * a.d);
+#pragma unroll
+          for (int x = 0; x < DP / 32; ++x)
+            if (x * 32 + lane < a.d) {
+              pek[x] += __ldcg(part + p * apart + x * 32 + lane);
+              pk[x] += __ldcg(part + p * apart + a.d + x * 32 + lane);
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x)
+          if (x * 32 + lane < a.d && a.dq != nullptr)
+            static_cast<T*>(a.dq)[(static_cast<int64_t>(row) * a.heads + head) * a.d + x * 32 + lane] =
+                from_float<T>(a.scale * fmaf(-delta, pk[x], pek[x]));
+        if (lane == 0) a.delta[static_cast<int64_t>(head) * a.n_q + row] = delta;
+      }
+    }
+    __syncthreads();  // `last` may be written again
+  }
+}
+
+// dk and dv: a group of lanes for each key row and key head, over the queries that see it and the heads of its group
+template <typename T, int DP>
+__global__ __launch_bounds__(ROW_WARPS * 32) void attn_rows_dkv_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G;
+  pdl_enter();
+  const int lane = threadIdx.x & 31, vec = lane % G, group = a.heads / a.kv_heads;
+  const bool in_d = vec * VEC < a.d;
+  const int64_t t = (static_cast<int64_t>(blockIdx.x) * ROW_WARPS + (threadIdx.x >> 5)) * KEYS + lane / G;
+  const bool here = t < static_cast<int64_t>(a.n_k) * a.kv_heads;
+  const int row = here ? static_cast<int>(t / a.kv_heads) : 0, c = here ? static_cast<int>(t - static_cast<int64_t>(row) * a.kv_heads) : 0;
+  bool found = false;
+  AttnSeq e{0, 0, 0, 0};
+  if (here) e = sequence_of(a, a.k_seq, row, true, &found);
+  const bool mine = here && !(found && attn_in_tiles(a, e));
+  int first = 0;  // query that sees this key first
+  if (a.causal) first = max(0, row - e.k0 - (e.k_len - e.q_len));
+  const int queries = mine && found ? max(0, e.q_len - first) : 0;
+  const int most = __reduce_max_sync(FULL_MASK, queries);
+  float k[VEC], v[VEC], dk[VEC], dv[VEC];
+  load_row<T, VEC>(static_cast<const T*>(a.k.p) + row * a.k.row + c * a.k.head + vec * VEC, in_d && queries > 0, k);
+  load_row<T, VEC>(static_cast<const T*>(a.v.p) + row * a.v.row + c * a.v.head + vec * VEC, in_d && queries > 0, v);
+#pragma unroll
+  for (int x = 0; x < VEC; ++x) dk[x] = dv[x] = 0.0f;
+  for (int i = 0; i < most; ++i) {
+    const bool on = i < queries;
+    const int at = e.q0 + first + (on ? i : 0);
+    for (int h = 0; h < group; ++h) {
+      const int head = c * group + h;
+      float q[VEC], g[VEC];
+      load_row<T, VEC>(static_cast<const T*>(a.q.p) + at * a.q.row + head * a.q.head + vec * VEC, in_d && on, q);
+      load_row<T, VEC>(static_cast<const T*>(a.dout.p) + at * a.dout.row + head * a.dout.head + vec * VEC, in_d && on, g);
+      float ref = on ? a.lse[static_cast<int64_t>(head) * a.n_q + at] : INFINITY;
+      const float delta = on ? a.delta[static_cast<int64_t>(head) * a.n_q + at] : 0.0f;
+      if (ref == -INFINITY) ref = INFINITY;
+      const float x = group_sum<G>(dot<VEC>(q, k)) * a.scale, e2 = group_sum<G>(dot<VEC>(g, v));
+      const float p = on ? exp2f((x - ref) * LOG2E) : 0.0f, ds = p * (e2 - delta);
+#pragma unroll
+      for (int n = 0; n < VEC; ++n) {
+        dv[n] = fmaf(p, g[n], dv[n]);
+        dk[n] = fmaf(ds, q[n], dk[n]);
+      }
+    }
+  }
+  if (!mine || !in_d) return;
+#pragma unroll
+  for (int n = 0; n < VEC; ++n) dk[n] *= a.scale;
+  const int64_t to = (static_cast<int64_t>(row) * a.kv_heads + c) * a.d + vec * VEC;
+  store_vec<T, VEC>(static_cast<T*>(a.dk) + to, dk);
+  store_vec<T, VEC>(static_cast<T*>(a.dv) + to, dv);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+struct Layout {
+  int64_t bytes = 0;
+  int64_t take(int64_t n) {
+    const int64_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  }
+};
+
+// Parts that rows with many keys can have, whatever the offsets: parts <= k_len / ATTN_SPLIT_KEYS + 1 for each of a sequence's queries
+int64_t split_bound(int64_t n_q, int64_t n_k, int64_t seqs) {
+  if (n_k <= ATTN_SPLIT_FROM) return 0;
+  const int64_t queries = n_q < ATTN_SPLIT_QUERIES ? n_q : ATTN_SPLIT_QUERIES;
+  const int64_t longest = n_k / (ATTN_SPLIT_FROM + 1), some = ATTN_SPLIT_QUERIES * (longest < seqs ? longest : seqs);
+  return queries * (n_k / ATTN_SPLIT_KEYS) + (n_q < some ? n_q : some);
+}
+
+// Workspace of a call; `base` == nullptr: its size alone
+int64_t lay_out(const dgs_attention& p, bool backward, char* base, AttnArgs* a) {
+  Layout l;
+  a->split_bound = static_cast<int32_t>(split_bound(p.n_q, p.n_k, p.seqs));
+  const int64_t floats = backward ? 2 * p.d + 1 : p.d + 2;
+  auto at = [&](int64_t bytes) { return base + l.take(bytes); };
+  a->counts = reinterpret_cast<int32_t*>(at(ATTN_COUNTS * 4));
+  a->norms = reinterpret_cast<float*>(at(8));
+  a->seq = reinterpret_cast<AttnSeq*>(at(p.seqs * static_cast<int64_t>(sizeof(AttnSeq))));
+  a->q_seq = reinterpret_cast<int32_t*>(at(p.n_q * 4));
+  a->k_seq = reinterpret_cast<int32_t*>(at(backward ? p.n_k * 4 : 0));
+  a->splits = reinterpret_cast<int4*>(at(int64_t(16) * a->split_bound));
+  a->arrived = reinterpret_cast<uint32_t*>(at(int64_t(4) * a->split_bound * p.kv_heads));
+  a->parts = reinterpret_cast<float*>(at(int64_t(4) * a->split_bound * p.heads * floats));
+  a->delta = reinterpret_cast<float*>(at(backward ? int64_t(4) * p.heads * p.n_q : 0));
+  return l.bytes;
+}
+
+int check(const char* who, const dgs_attention* p) {
+  DGS_REQUIRE(p != nullptr, DGS_ERR_INVALID, "%s: null argument", who);
+  const int esz = dtype_bytes(p->dtype);
+  DGS_REQUIRE(esz != 0, DGS_ERR_UNSUPPORTED, "%s: element type %d", who, p->dtype);
+  DGS_REQUIRE(p->n_q >= 0 && p->n_k >= 0 && p->seqs >= 0 && p->n_q < (int64_t(1) << 30) && p->n_k < (int64_t(1) << 30), DGS_ERR_INVALID,
+              "%s: %lld query rows, %lld key rows, %d sequences", who, static_cast<long long>(p->n_q), static_cast<long long>(p->n_k), p->seqs);
+  DGS_REQUIRE(p->heads >= 1 && p->kv_heads >= 1 && p->heads % p->kv_heads == 0 && p->heads <= 65535, DGS_ERR_INVALID,
+              "%s: %d query heads over %d key heads", who, p->heads, p->kv_heads);
+  const int vec = 16 / esz;
+  DGS_REQUIRE(p->d >= vec && p->d <= ATTN_MAX_D && p->d % vec == 0, DGS_ERR_UNSUPPORTED,
+              "%s: heads of %d elements (multiples of %d up to %d)", who, p->d, vec, ATTN_MAX_D);
+  DGS_REQUIRE(p->q_row % vec == 0 && p->q_head % vec == 0 && p->k_row % vec == 0 && p->k_head % vec == 0 && p->v_row % vec == 0 &&
+                  p->v_head % vec == 0 && aligned_to(p->q, 16) && aligned_to(p->k, 16) && aligned_to(p->v, 16),
+              DGS_ERR_INVALID, "%s: heads must begin at 16-byte boundaries", who);
+  DGS_REQUIRE(p->q_row >= 0 && p->q_head >= 0 && p->k_row >= 0 && p->k_head >= 0 && p->v_row >= 0 && p->v_head >= 0, DGS_ERR_INVALID,
+              "%s: strides must not be negative", who);
+  DGS_REQUIRE(p->scale - p->scale == 0.0f, DGS_ERR_INVALID, "%s: scale must be a finite number", who);
+  DGS_REQUIRE((p->n_q == 0 || p->q != nullptr) && (p->n_k == 0 || (p->k != nullptr && p->v != nullptr)) &&
+                  p->q_offsets != nullptr && p->k_offsets != nullptr,
+              DGS_ERR_INVALID, "%s: null argument", who);
+  DGS_REQUIRE(split_bound(p->n_q, p->n_k, p->seqs) < (int64_t(1) << 27), DGS_ERR_INVALID, "%s: too many rows", who);
+  return DGS_OK;
+}
+
+AttnArgs arguments(const dgs_attention& p) {
+  AttnArgs a{};
+  a.q = {p.q, p.q_row, p.q_head};
+  a.k = {p.k, p.k_row, p.k_head};
+  a.v = {p.v, p.v_row, p.v_head};
+  a.q_offsets = p.q_offsets;
+  a.k_offsets = p.k_offsets;
+  a.offsets64 = p.ids64;
+  a.seqs = p.seqs;
+  a.n_q = static_cast<int32_t>(p.n_q);
+  a.n_k = static_cast<int32_t>(p.n_k);
+  a.heads = p.heads;
+  a.kv_heads = p.kv_heads;
+  a.d = p.d;
+  a.causal = p.causal != 0;
+  a.tiles = 0;
+  a.scale = p.scale;
+  return a;
+}
+
+int launch_plan(const AttnArgs& a, bool backward, cudaStream_t s) {
+  const bool one = a.seqs <= PLAN_ONE_CTA;
+  if (!one) {
+    DGS_CUDA_TRY(cudaMemsetAsync(a.counts, 0, ATTN_COUNTS * 4, s));
+    DGS_CUDA_TRY(cudaMemsetAsync(a.norms, 0, 8, s));
+  }
+  const int64_t ctas = one ? 1 : (static_cast<int64_t>(a.seqs) + PLAN_THREADS / 32 - 1) / (PLAN_THREADS / 32);
+  const int64_t most = 2 * static_cast<int64_t>(sm_count());
+  DGS_CUDA_TRY(launch_training(attn_plan_kernel, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), PLAN_THREADS, 0, s, a,
+                               static_cast<int32_t>(backward), static_cast<int32_t>(one)));
+  return DGS_OK;
+}
+
+// f.run<T, DP, R>() with the elements of a head filled up to DP, R heads of a group at once (MOST of them at most)
+template <typename T, int DP, int MOST, typename F>
+int with_heads(const AttnArgs& a, const F& f) {
+  const int group = a.heads / a.kv_heads;
+  if (group == 1) return f.template run<T, DP, 1>();
+  if (group == 2 || MOST == 2) return f.template run<T, DP, 2>();
+  return f.template run<T, DP, MOST>();
+}
+template <typename T, int MOST, typename F>
+int with_width(const AttnArgs& a, const F& f) {
+  return a.d <= 32 ? with_heads<T, 32, MOST>(a, f) : a.d <= 64 ? with_heads<T, 64, MOST>(a, f) : with_heads<T, 128, MOST>(a, f);
+}
+template <int MOST, typename F>
+int with_type(int32_t dtype, const AttnArgs& a, const F& f) {
+  return dtype == DGS_F32    ? with_width<float, MOST>(a, f)
+         : dtype == DGS_BF16 ? with_width<__nv_bfloat16, MOST>(a, f)
+                             : with_width<__half, MOST>(a, f);
+}
+
+int split_ctas(const AttnArgs& a) {
+  const int64_t tasks = static_cast<int64_t>(a.split_bound) * a.kv_heads, most = static_cast<int64_t>(sm_count()) * 4;
+  return static_cast<int>(tasks < most ? tasks : most);
+}
+unsigned row_ctas(const AttnArgs& a) { return static_cast<unsigned>((static_cast<int64_t>(a.n_q) * a.kv_heads + ROW_WARPS - 1) / ROW_WARPS); }
+
+struct RowsForward {
+  const AttnArgs& a;
+  cudaStream_t s;
+  template <typename T, int DP, int R>
+  int run() const {
+    const int splits = split_ctas(a);
+    DGS_CUDA_TRY(launch_training(attn_rows_kernel<T, DP, R>, dim3(splits + row_ctas(a)), ROW_WARPS * 32, 0, s, a, splits));
+    return DGS_OK;
+  }
+};
+struct RowsBackward {
+  const AttnArgs& a;
+  cudaStream_t s;
+  template <typename T, int DP, int R>
+  int run() const {
+    const int splits = split_ctas(a);
+    DGS_CUDA_TRY(launch_training(attn_rows_dq_kernel<T, DP, R>, dim3(splits + row_ctas(a)), ROW_WARPS * 32, 0, s, a, splits));
+    if (a.dk == nullptr || a.n_k == 0) return DGS_OK;
+    constexpr int rows = ROW_WARPS * 32 / (DP / vec_of<T>());
+    DGS_CUDA_TRY(launch_training(attn_rows_dkv_kernel<T, DP>,
+                                 dim3(static_cast<unsigned>((static_cast<int64_t>(a.n_k) * a.kv_heads + rows - 1) / rows)), ROW_WARPS * 32, 0,
+                                 s, a));
+    return DGS_OK;
+  }
+};
+
+}  // namespace
+}  // namespace dgs
+
+using namespace dgs;
+
+extern "C" size_t dgs_attention_workspace_bytes(const dgs_attention* p, int32_t backward) {
+  if (p == nullptr || p->n_q < 0 || p->n_k < 0 || p->seqs < 0 || p->heads < 1 || p->kv_heads < 1 || p->d < 1) return 0;
+  AttnArgs a{};
+  return static_cast<size_t>(lay_out(*p, backward != 0, nullptr, &a));
+}
+
+extern "C" int dgs_attention_forward(const dgs_attention* p, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                     int32_t* status, dgs_stream_t stream) {
+  if (int rc = check("attention", p)) return rc;
+  if (p->n_q == 0) return DGS_OK;
+  DGS_REQUIRE(out != nullptr && lse != nullptr && aligned_to(out, 16), DGS_ERR_INVALID, "attention: out (16-byte aligned) and lse are needed");
+  const size_t need = dgs_attention_workspace_bytes(p, 0);
+  DGS_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned_to(workspace, 256), DGS_ERR_INVALID,
+              "attention: workspace of %zu bytes, 256-byte aligned, is needed", need);
+  AttnArgs a = arguments(*p);
+  lay_out(*p, false, static_cast<char*>(workspace), &a);
+  a.out = out;
+  a.lse = lse;
+  a.status = status;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (int rc = launch_plan(a, false, s)) return rc;
+  return with_type<4>(p->dtype, a, RowsForward{a, s});
+}
+
+extern "C" int dgs_attention_backward(const dgs_attention* p, const void* dout, int64_t dout_row, int64_t dout_head, const void* out,
+                                      const float* lse, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                      int32_t* status, dgs_stream_t stream) {
+  if (int rc = check("attention_backward", p)) return rc;
+  DGS_REQUIRE((dk == nullptr) == (dv == nullptr), DGS_ERR_INVALID, "attention_backward: the gradients of keys and values come together");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const size_t esz = dtype_bytes(p->dtype), kv = static_cast<size_t>(p->n_k) * p->kv_heads * p->d * esz;
+  if (p->n_q == 0) {
+    if (dk != nullptr && kv != 0) {
+      DGS_CUDA_TRY(cudaMemsetAsync(dk, 0, kv, s));
+      DGS_CUDA_TRY(cudaMemsetAsync(dv, 0, kv, s));
+    }
+    return DGS_OK;
+  }
+  if (dq == nullptr && dk == nullptr) return DGS_OK;
+  const int64_t vec = 16 / static_cast<int64_t>(esz);
+  DGS_REQUIRE(dout != nullptr && out != nullptr && lse != nullptr && aligned_to(dout, 16) && aligned_to(out, 16) && aligned_to(dq, 16) &&
+                  aligned_to(dk, 16) && aligned_to(dv, 16) && dout_row % vec == 0 && dout_head % vec == 0 && dout_row >= 0 && dout_head >= 0,
+              DGS_ERR_INVALID, "attention_backward: dout, out, lse and gradients must be there, heads must begin at 16-byte boundaries");
+  const size_t need = dgs_attention_workspace_bytes(p, 1);
+  DGS_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned_to(workspace, 256), DGS_ERR_INVALID,
+              "attention_backward: workspace of %zu bytes, 256-byte aligned, is needed", need);
+  AttnArgs a = arguments(*p);
+  lay_out(*p, true, static_cast<char*>(workspace), &a);
+  a.dout = {dout, dout_row, dout_head};
+  a.out = const_cast<void*>(out);
+  a.lse = const_cast<float*>(lse);
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.status = status;
+  if (int rc = launch_plan(a, true, s)) return rc;
+  return with_type<2>(p->dtype, a, RowsBackward{a, s});
+}

@@ -1,0 +1,53 @@
+// What the kernels of packed attention share (attention.cu: the plan, rows on the CUDA cores, entry points; attention_mma.cu: tiles
+// on the tensor cores).  Not part of the C ABI.
+#pragma once
+#include "train_common.cuh"
+
+namespace dgs {
+
+// Rows of one sequence; a sequence whose offsets are not in order has none.
+struct AttnSeq {
+  int32_t q0, q_len, k0, k_len;
+};
+
+struct AttnView {
+  const void* p;
+  int64_t row, head;  // strides in elements
+};
+
+struct AttnArgs {
+  AttnView q, k, v, dout;
+  const void *q_offsets, *k_offsets;
+  int32_t offsets64;
+  int32_t seqs, n_q, n_k, heads, kv_heads, d, causal, tiles;  // tiles: long sequences go to the tensor cores
+  float scale;
+  // results: contiguous rows of `heads` (`kv_heads`) times d elements; lse and delta [heads, n_q]
+  void* out;
+  float* lse;
+  void *dq, *dk, *dv;
+  // workspace
+  AttnSeq* seq;                 // [seqs]
+  int32_t *q_seq, *k_seq;       // the sequence of a row; only entries whose sequence holds the row mean anything
+  int32_t* counts;              // ATTN_COUNTS words
+  int4* splits;                 // {row, first key, index of the row's first part, parts}
+  uint32_t* arrived;            // parts that are there, one word for each part (the first of a row's is used) and key head
+  float* parts;                 // [part][heads][part_floats]
+  int4 *q_tiles, *k_tiles;      // {sequence, first row, ..} of the tiles, heaviest first
+  float* delta;
+  float* norms;                 // [2] the largest row norms of dout and v (as they are ordered, through unsigned words)
+  int32_t* status;
+  int32_t split_bound, q_tile_bound, k_tile_bound;
+};
+
+enum { ATTN_N_SPLITS = 0, ATTN_N_Q_TILES = 1, ATTN_N_K_TILES = 2, ATTN_COUNTS = 8 };
+
+constexpr int ATTN_MAX_D = 128;
+constexpr int ATTN_SPLIT_FROM = 256;   // keys from which a CTA takes a row instead of a warp, ...
+constexpr int ATTN_SPLIT_KEYS = 1024;  // ... so many at a time
+constexpr int ATTN_SPLIT_QUERIES = 16; // (with more queries there are warps enough)
+constexpr int ATTN_TILE_QUERIES = 48;  // queries from which a sequence goes to the tensor cores
+
+__host__ __device__ inline bool attn_in_tiles(const AttnArgs& a, const AttnSeq& s) { return a.tiles && s.q_len >= ATTN_TILE_QUERIES && s.k_len > 0; }
+__host__ __device__ inline bool attn_is_split(const AttnSeq& s) { return s.k_len > ATTN_SPLIT_FROM && s.q_len <= ATTN_SPLIT_QUERIES; }
+
+}  // namespace dgs

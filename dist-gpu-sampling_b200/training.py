@@ -59,7 +59,25 @@ def _define():
             dh, dw = ops._CAPI_linear_cross_entropy_backward.from_loss(grad, hidden, weight, target, lse, loss, ctx.ignore_index, want_h, want_w)
             return dh if want_h else None, dw if want_w else None, None, None, None
 
-    _functions.update(norm=LayerNorm, loss=LinearCrossEntropy)
+    class Attention(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, v, q_offsets, k_offsets, causal, scale):
+            out, lse = ops._CAPI_attention(q, k, v, q_offsets, k_offsets, causal, scale)
+            ctx.save_for_backward(q, k, v, out, lse, q_offsets, k_offsets)
+            ctx.causal, ctx.scale = causal, scale
+            ctx.mark_non_differentiable(lse)
+            return out, lse
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad, _):
+            q, k, v, out, lse, q_offsets, k_offsets = ctx.saved_tensors
+            want_q, want_k, want_v = ctx.needs_input_grad[:3]
+            dq, dk, dv = ops._CAPI_attention_backward(grad, q, k, v, out, lse, q_offsets, k_offsets, ctx.causal, ctx.scale, want_q,
+                                                      want_k or want_v)
+            return dq if want_q else None, dk if want_k else None, dv if want_v else None, None, None, None, None
+
+    _functions.update(norm=LayerNorm, loss=LinearCrossEntropy, attention=Attention)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -87,6 +105,28 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     if reduction == "sum":
         return loss.sum()
     return loss.sum() / (target != ignore_index).sum()
+
+
+def attention(q, k, v, q_offsets, k_offsets=None, causal=False, scale=None, return_lse=False):
+    """Softmax attention of packed sequences of different lengths, with gradients for q, k and v.
+
+    q [n_q, heads, d], k and v [n_k, key heads, d] share one type (float32, bfloat16 or float16; heads a multiple of key heads, d up
+    to 128) and may be parts of a wider tensor.  Sequence s is the query rows q_offsets[s] to q_offsets[s + 1] and the key rows of
+    k_offsets (default: the same) likewise.  Every node of a block over its sampled neighbours, `indptr, indices = block_csc(row, col, n_dst)`:
+
+        attention(q, k[indices], v[indices], torch.arange(n_dst + 1, device="cuda"), indptr)
+
+    causal: query i of Lq sees the keys j <= i + Lk - Lq (the last query sees all of them).  scale: 1 / sqrt(d) by default.  A query that
+    sees no key gives zeros, and so do rows outside of all sequences.  return_lse: also the logarithm of the sum of exponentials
+    [heads, n_q] (float32, without a gradient; -inf where no key is seen).  Sequences of 48 queries and more run on the tensor cores in
+    16 bits; float32 runs on the CUDA cores.  Gradients are added in a fixed order."""
+    if k_offsets is None:
+        k_offsets = q_offsets
+    if not _functions:
+        _define()
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    out, lse = _functions["attention"].apply(q, k, v, q_offsets, k_offsets, bool(causal), scale)
+    return (out, lse) if return_lse else out
 
 
 class AdamW:

@@ -481,6 +481,39 @@ DGS_API int dgs_adamw_step_8bit_unbiased(const dgs_adamw_tensor* tensors, int32_
 DGS_API int dgs_adamw_state_values(const void* codes, int32_t second, const float* scales, int64_t n, float* out,
                                    dgs_stream_t stream);
 
+/* Softmax attention of packed sequences: sequence s holds the query rows
+ * [q_offsets[s], q_offsets[s + 1]) and the key and value rows of k_offsets (for a
+ * sampled block the queries are its seeds and k_offsets is its indptr).  Query head a
+ * reads key head a / (heads / kv_heads).  With x_ij = scale q_i . k_j, for the keys
+ * that query i sees (all of its sequence; causal: j <= i + Lk - Lq):
+ *   lse_i = log sum_j exp x_ij,  out_i = sum_j exp(x_ij - lse_i) v_j
+ * A query that sees no key has out 0 and lse -inf; so have rows outside of all
+ * sequences, whatever they hold, and their gradients are 0.  q [n_q, heads, d], k and v
+ * [n_k, kv_heads, d] of one type have strides in elements; heads of d elements must
+ * begin at 16-byte boundaries, d a multiple of 16 bytes and at most 128.
+ * out is contiguous, lse [heads, n_q].  Offsets (int64 when ids64, else int32; seqs + 1
+ * of each) that are not in order or beyond the rows raise DGS_ERR_RANGE in *status
+ * (which may be NULL); their sequences have no rows then.  workspace: 256-byte
+ * aligned. */
+typedef struct dgs_attention {
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const void *q_offsets, *k_offsets;
+  int64_t n_q, n_k;
+  int32_t seqs, heads, kv_heads, d;
+  int32_t dtype, ids64, causal;
+  float scale;
+} dgs_attention;
+DGS_API size_t dgs_attention_workspace_bytes(const dgs_attention* problem, int32_t backward);
+DGS_API int dgs_attention_forward(const dgs_attention* problem, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                  int32_t* status, dgs_stream_t stream);
+/* Gradients for dout [n_q, heads, d] (strides dout_row, dout_head), contiguous: dq
+ * (may be NULL), dk and dv (both or neither).  out and lse as the forward call gave
+ * them.  Added in a fixed order: the same inputs give the same bits. */
+DGS_API int dgs_attention_backward(const dgs_attention* problem, const void* dout, int64_t dout_row, int64_t dout_head,
+                                   const void* out, const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                                   size_t workspace_bytes, int32_t* status, dgs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
