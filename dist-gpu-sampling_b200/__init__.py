@@ -91,13 +91,21 @@ class Attention(ctypes.Structure):
                [(n, ctypes.c_int32) for n in ("seqs", "heads", "kv_heads", "d", "dtype", "ids64", "causal")] + [("scale", ctypes.c_float)]
 
 
+class ResidualNorm(ctypes.Structure):
+    _fields_ = [("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64), ("gate", ctypes.c_void_p), ("gate_stride", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("post_weight", "post_bias", "weight", "bias")] + \
+               [("n", ctypes.c_int64), ("D", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "param_dtype", "gate_kind", "post", "pre")] + \
+               [(n, ctypes.c_float) for n in ("x_scale", "y_scale", "eps")]
+
+
 # name -> (restype, argtypes); every symbol include/dgs_b200.h declares
 _I32, _I64, _U64, _VP, _SZ = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_size_t
 _DP, _SP = ctypes.POINTER(ChunkDesc), ctypes.POINTER(Segments)
 _I64P = ctypes.POINTER(ctypes.c_int64)
 _HP = ctypes.POINTER(Hop)
 _AP, _F32, _F64 = ctypes.POINTER(AdamWTensor), ctypes.c_float, ctypes.c_double
-_TP = ctypes.POINTER(Attention)
+_TP, _NP = ctypes.POINTER(Attention), ctypes.POINTER(ResidualNorm)
 ABI_SIGNATURES = {
     "dgs_last_error": (ctypes.c_char_p, []),
     "dgs_device_check": (ctypes.c_int, []),
@@ -169,6 +177,13 @@ ABI_SIGNATURES = {
     "dgs_attention_workspace_bytes": (_SZ, [_TP, _I32]),
     "dgs_attention_forward": (ctypes.c_int, [_TP, _VP, _VP, _VP, _SZ, _VP, _VP]),
     "dgs_attention_backward": (ctypes.c_int, [_TP, _VP, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP]),
+    "dgs_residual_norm_forward": (ctypes.c_int, [_NP, _VP, _I64] + [_VP] * 7),
+    "dgs_residual_norm_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "dgs_residual_norm_backward": (ctypes.c_int, [_NP, _VP, _VP, _I64, _VP, _I64] + [_VP] * 12 + [_SZ, _VP]),
+    "dgs_keep_8bit": (ctypes.c_int, [_VP, _I64, _I32, _I64, _I64, _VP, _VP, _VP]),
+    "dgs_kept_8bit_values": (ctypes.c_int, [_VP, _I64, _VP, _I64, _I64, _I32, _VP, _VP]),
+    "dgs_kept_8bit_weight_grad_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
+    "dgs_kept_8bit_weight_grad": (ctypes.c_int, [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _I64, _I64, _VP, _VP, _VP, _SZ, _VP]),
 }
 
 
@@ -372,4 +387,5 @@ def block_csc(coo_row, coo_col, n_dst, rows_sorted=True):
 from .placement import (CACHE_PRIORITY, get_available_memory, permute_edge_tensor, plan_capacities,  # noqa: E402,F401
                         reduce_min_over_ranks, renumber_by_degree)
 # the training step behind the samplers
-from .training import AdamW, attention, layer_norm, linear_cross_entropy  # noqa: E402,F401
+from .training import (AdamW, attention, keep_8bit, kept_8bit_values, layer_norm, linear_8bit, linear_cross_entropy,  # noqa: E402,F401
+                       residual_norm)

@@ -31,6 +31,8 @@ ABI_SOURCES = [
     "kernels/cross_entropy_mma.cu",
     "kernels/adamw.cu",
     "kernels/attention.cu",
+    "kernels/residual_norm.cu",
+    "kernels/kept.cu",
     "host/error.cc",
     "host/comm.cc",
     "host/store.cc",
@@ -47,6 +49,7 @@ HEADERS = [
     "kernels/tensor_core.cuh",
     "kernels/cross_entropy.h",
     "kernels/attention.h",
+    "kernels/kept.h",
     "host/comm.h",
     "../../include/dgs_b200.h",
 ]

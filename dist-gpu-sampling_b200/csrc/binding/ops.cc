@@ -582,5 +582,10 @@ TORCH_LIBRARY(dgs_ops, m) {
       .def("_CAPI_adamw_state_values", &AdamWStateValuesCUDA)
       // ... and of the blocks of a model in front of it, see training_block.h
       .def("_CAPI_attention", &AttentionCUDA)
-      .def("_CAPI_attention_backward", &AttentionBackwardCUDA);
+      .def("_CAPI_attention_backward", &AttentionBackwardCUDA)
+      .def("_CAPI_residual_norm", &ResidualNormCUDA)
+      .def("_CAPI_residual_norm_backward", &ResidualNormBackwardCUDA)
+      .def("_CAPI_keep_8bit", &Keep8bitCUDA)
+      .def("_CAPI_kept_8bit_values", &Kept8bitValuesCUDA)
+      .def("_CAPI_kept_8bit_weight_grad", &Kept8bitWeightGradCUDA);
 }

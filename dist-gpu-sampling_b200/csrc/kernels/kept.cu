@@ -1,0 +1,345 @@
+// Rows kept for the backward pass in 8 bits, and the gradient of a linear layer's weight from them.
+//
+//   a = max |x| over 128 columns of a row,  c = rint(x (127 / a)),  x ~ c (a / 127)
+//   dW[o, d] = sum_n g[n, o] v[n, d],  db[o] = sum_n g[n, o]
+//
+// Codes: bound by HBM, one byte written for every element read.
+#include "kept.h"
+
+namespace dgs {
+namespace {
+
+constexpr int KEEP_THREADS = 256;
+constexpr int KEEP_UNROLL = 4;
+
+// ---- codes and values -------------------------------------------------------------------------------------------------
+struct KeepArgs {
+  const void* x;
+  int64_t x_stride;
+  int8_t* codes;
+  const int8_t* codes_in;
+  int64_t codes_stride;
+  float* scales;
+  const float* scales_in;
+  void* out;
+  int64_t n, tasks;  // tasks: groups of all rows
+  int32_t D, groups;
+};
+
+__device__ __forceinline__ void row_and_group(const KeepArgs& a, int64_t task, int64_t* row, int* group) {
+  if (a.groups == 1) {
+    *row = task;
+    *group = 0;
+  } else if (a.tasks <= 0xffffffffll) {
+    *row = static_cast<uint32_t>(task) / static_cast<uint32_t>(a.groups);
+    *group = static_cast<int>(static_cast<uint32_t>(task) - static_cast<uint32_t>(*row) * a.groups);
+  } else {
+    *row = task / a.groups;
+    *group = static_cast<int>(task - *row * a.groups);
+  }
+}
+
+// LANES lanes hold a group, VEC adjacent elements each (VEC == 1: KEPT_GROUP / 32 elements 32 apart).  A value that is not finite makes the
+// scale one that is not: magnitudes are compared as words, where nan is above infinity.
+template <typename T, int VEC>
+__global__ __launch_bounds__(KEEP_THREADS) void keep_kernel(const __grid_constant__ KeepArgs a) {
+  constexpr int LANES = VEC == 1 ? 32 : KEPT_GROUP / VEC, E = VEC == 1 ? KEPT_GROUP / 32 : VEC, APART = VEC == 1 ? 32 : 1;
+  constexpr int PER_CTA = KEEP_THREADS / LANES;
+  pdl_enter();
+  const int lane = threadIdx.x % LANES, first = VEC == 1 ? lane : lane * VEC;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * PER_CTA;
+  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * PER_CTA + threadIdx.x / LANES; t0 - threadIdx.x / LANES < a.tasks; t0 += step * KEEP_UNROLL) {
+    float x[KEEP_UNROLL][E];
+    int64_t row[KEEP_UNROLL];
+    int group[KEEP_UNROLL];
+#pragma unroll
+    for (int u = 0; u < KEEP_UNROLL; ++u) {
+      const int64_t t = t0 + u * step;
+      row_and_group(a, t < a.tasks ? t : 0, &row[u], &group[u]);
+      const int c = group[u] * KEPT_GROUP + first;
+      const T* p = static_cast<const T*>(a.x) + row[u] * a.x_stride + c;
+      if constexpr (VEC == 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = t < a.tasks && c + e * APART < a.D ? to_float<T>(p[e * APART]) : 0.0f;
+      } else if (t < a.tasks && c < a.D) {
+        load_vec<T, VEC>(p, x[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < KEEP_UNROLL; ++u) {
+      const int64_t t = t0 + u * step;
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[u][e]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(FULL_MASK, top, o));
+      if (t >= a.tasks) continue;
+      const float big = __uint_as_float(top), by = big > 0.0f ? 127.0f / big : 0.0f;
+      int8_t c[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) c[e] = static_cast<int8_t>(max(-127, min(127, __float2int_rn(x[u][e] * by))));
+      const int at = group[u] * KEPT_GROUP + first;
+      int8_t* to = a.codes + row[u] * a.D + at;
+      if constexpr (VEC == 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (at + e * APART < a.D) to[e * APART] = c[e];
+      } else if (at < a.D) {
+        Vec<int8_t, VEC> v;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v.v[e] = c[e];
+        *reinterpret_cast<Vec<int8_t, VEC>*>(to) = v;
+      }
+      if (lane == 0) a.scales[row[u] * a.groups + group[u]] = big / 127.0f;
+    }
+  }
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(KEEP_THREADS) void kept_values_kernel(const __grid_constant__ KeepArgs a) {
+  constexpr int LANES = VEC == 1 ? 32 : KEPT_GROUP / VEC, E = VEC == 1 ? KEPT_GROUP / 32 : VEC, APART = VEC == 1 ? 32 : 1;
+  constexpr int PER_CTA = KEEP_THREADS / LANES;
+  pdl_enter();
+  const int lane = threadIdx.x % LANES, first = VEC == 1 ? lane : lane * VEC;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * PER_CTA;
+  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * PER_CTA + threadIdx.x / LANES; t0 < a.tasks; t0 += step * KEEP_UNROLL) {
+    Vec<int8_t, E> c[KEEP_UNROLL];
+    float scale[KEEP_UNROLL];
+    int64_t row[KEEP_UNROLL];
+    int at[KEEP_UNROLL];
+#pragma unroll
+    for (int u = 0; u < KEEP_UNROLL; ++u) {
+      const int64_t t = t0 + u * step;
+      int group;
+      row_and_group(a, t < a.tasks ? t : 0, &row[u], &group);
+      at[u] = t < a.tasks ? group * KEPT_GROUP + first : a.D;
+      const int8_t* p = a.codes_in + row[u] * a.codes_stride + at[u];
+      if constexpr (VEC == 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) c[u].v[e] = at[u] + e * APART < a.D ? p[e * APART] : 0;
+      } else {
+        c[u] = at[u] < a.D ? *reinterpret_cast<const Vec<int8_t, E>*>(p) : Vec<int8_t, E>{};
+      }
+      scale[u] = at[u] < a.D ? a.scales_in[row[u] * a.groups + group] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < KEEP_UNROLL; ++u) {
+      T* to = static_cast<T*>(a.out) + row[u] * a.D + at[u];
+      float v[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = static_cast<float>(c[u].v[e]) * scale[u];
+      if constexpr (VEC == 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (at[u] + e * APART < a.D) to[e * APART] = from_float<T>(v[e]);
+      } else if (at[u] < a.D) {
+        store_vec<T, VEC>(to, v);
+      }
+    }
+  }
+}
+
+unsigned keep_ctas(int64_t tasks, int lanes) {
+  const int64_t per = static_cast<int64_t>(KEEP_THREADS / lanes) * KEEP_UNROLL, need = (tasks + per - 1) / per;
+  const int64_t most = static_cast<int64_t>(sm_count()) * 8;
+  return static_cast<unsigned>(need < most ? need : most);
+}
+
+template <typename T>
+int keep(const KeepArgs& a, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (a.D % VEC == 0 && (a.x_stride % VEC == 0 || a.n <= 1) && aligned_to(a.x, 16) && aligned_to(a.codes, VEC))
+    DGS_CUDA_TRY(launch_training(keep_kernel<T, VEC>, dim3(keep_ctas(a.tasks, KEPT_GROUP / VEC)), KEEP_THREADS, 0, s, a));
+  else
+    DGS_CUDA_TRY(launch_training(keep_kernel<T, 1>, dim3(keep_ctas(a.tasks, 32)), KEEP_THREADS, 0, s, a));
+  return DGS_OK;
+}
+template <typename T>
+int values(const KeepArgs& a, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (a.D % VEC == 0 && (a.codes_stride % VEC == 0 || a.n <= 1) && aligned_to(a.out, 16) && aligned_to(a.codes_in, VEC))
+    DGS_CUDA_TRY(launch_training(kept_values_kernel<T, VEC>, dim3(keep_ctas(a.tasks, KEPT_GROUP / VEC)), KEEP_THREADS, 0, s, a));
+  else
+    DGS_CUDA_TRY(launch_training(kept_values_kernel<T, 1>, dim3(keep_ctas(a.tasks, 32)), KEEP_THREADS, 0, s, a));
+  return DGS_OK;
+}
+
+// ---- the weight's gradient on the CUDA cores ------------------------------------------------------------------------------
+// A tile of 64 x 64 results a CTA over a share of the rows, 4 x 4 a thread; the shares are added in their order afterwards.
+constexpr int WG_TILE = 64, WG_ROWS = 16, WG_THREADS = 256;
+
+template <typename T>
+__global__ __launch_bounds__(WG_THREADS) void kept_grad_kernel(const __grid_constant__ KeptGradArgs a) {
+  __shared__ __align__(16) float g[WG_ROWS][WG_TILE + 4], v[WG_ROWS][WG_TILE + 4];
+  pdl_enter();
+  const int o0 = blockIdx.y * WG_TILE, d0 = blockIdx.x * WG_TILE, split = blockIdx.z;
+  const int64_t r0 = a.n * split / a.splits, r1 = a.n * (split + 1) / a.splits;
+  const int to = threadIdx.x / 16 * 4, td = threadIdx.x % 16 * 4;
+  float acc[4][4] = {}, db = 0.0f;
+  for (int64_t r = r0; r < r1; r += WG_ROWS) {
+    for (int i = threadIdx.x; i < WG_ROWS * WG_TILE; i += WG_THREADS) {
+      const int row = i / WG_TILE, c = i % WG_TILE;
+      const bool in = r + row < r1;
+      g[row][c] = in && o0 + c < a.O ? to_float<T>(static_cast<const T*>(a.grad)[(r + row) * a.grad_stride + o0 + c]) : 0.0f;
+      v[row][c] = in && d0 + c < a.D ? to_float<T>(from_float<T>(static_cast<float>(a.codes[(r + row) * a.codes_stride + d0 + c]) *
+                                                                 a.scales[(r + row) * a.groups + (d0 + c) / KEPT_GROUP]))
+                                     : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < WG_ROWS; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(&g[k][to]), y = *reinterpret_cast<const float4*>(&v[k][td]);
+      const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[i], ys[j], acc[i][j]);
+    }
+    if (threadIdx.x < WG_TILE)
+#pragma unroll
+      for (int k = 0; k < WG_ROWS; ++k) db += g[k][threadIdx.x];
+    __syncthreads();
+  }
+  float* part = a.parts + static_cast<int64_t>(split) * a.O * a.D;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (o0 + to + i < a.O && d0 + td + j < a.D) part[static_cast<int64_t>(o0 + to + i) * a.D + d0 + td + j] = acc[i][j];
+  if (d0 == 0 && threadIdx.x < WG_TILE && o0 + threadIdx.x < a.O) a.bias_parts[static_cast<int64_t>(split) * a.O + o0 + threadIdx.x] = db;
+}
+
+// shares added in their order
+template <typename T>
+__global__ __launch_bounds__(KEEP_THREADS) void kept_join_kernel(const __grid_constant__ KeptGradArgs a) {
+  pdl_enter();
+  const int64_t all = static_cast<int64_t>(a.O) * a.D, step = static_cast<int64_t>(gridDim.x) * KEEP_THREADS;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * KEEP_THREADS + threadIdx.x; i < all; i += step) {
+    float s = 0.0f;
+#pragma unroll 8
+    for (int p = 0; p < a.splits; ++p) s += a.parts[p * all + i];
+    static_cast<T*>(a.dweight)[i] = from_float<T>(s);
+  }
+  if (a.dbias != nullptr)
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * KEEP_THREADS + threadIdx.x; i < a.O; i += step) {
+      float s = 0.0f;
+#pragma unroll 8
+      for (int p = 0; p < a.splits; ++p) s += a.bias_parts[static_cast<int64_t>(p) * a.O + i];
+      static_cast<T*>(a.dbias)[i] = from_float<T>(s);
+    }
+}
+
+// Shares of the rows: enough CTAs for four on each SM, shares of 256 rows at least
+int64_t shares(int64_t n, int64_t O, int64_t D) {
+  const int64_t tiles = ((O + WG_TILE - 1) / WG_TILE) * ((D + WG_TILE - 1) / WG_TILE);
+  int64_t want = (static_cast<int64_t>(sm_count()) * 4 + tiles - 1) / tiles;
+  const int64_t most = (n + 255) / 256;
+  if (want > most) want = most;
+  return want < 1 ? 1 : want;
+}
+
+template <typename T>
+int weight_grad(const KeptGradArgs& a, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((a.D + WG_TILE - 1) / WG_TILE), static_cast<unsigned>((a.O + WG_TILE - 1) / WG_TILE),
+                  static_cast<unsigned>(a.splits));
+  DGS_CUDA_TRY(launch_training(kept_grad_kernel<T>, grid, WG_THREADS, 0, s, a));
+  const int64_t need = (static_cast<int64_t>(a.O) * a.D + KEEP_THREADS - 1) / KEEP_THREADS, most = static_cast<int64_t>(sm_count()) * 8;
+  DGS_CUDA_TRY(launch_training(kept_join_kernel<T>, dim3(static_cast<unsigned>(need < most ? need : most)), KEEP_THREADS, 0, s, a));
+  return DGS_OK;
+}
+
+constexpr int64_t KEPT_MAX_SIDE = int64_t(1) << 22;  // elements of a row
+
+int check(const char* who, int64_t n, int64_t D, int32_t dtype) {
+  DGS_REQUIRE(dtype_bytes(dtype) != 0, DGS_ERR_UNSUPPORTED, "%s: element type %d", who, dtype);
+  DGS_REQUIRE(n >= 0 && D >= 1 && D <= KEPT_MAX_SIDE && n <= (int64_t(1) << 40), DGS_ERR_INVALID, "%s: %lld rows of %lld elements", who,
+              static_cast<long long>(n), static_cast<long long>(D));
+  return DGS_OK;
+}
+
+}  // namespace
+}  // namespace dgs
+
+using namespace dgs;
+
+extern "C" int dgs_keep_8bit(const void* x, int64_t x_stride, int32_t dtype, int64_t n, int64_t D, int8_t* codes, float* scales,
+                             dgs_stream_t stream) {
+  if (int rc = check("keep_8bit", n, D, dtype)) return rc;
+  DGS_REQUIRE(x_stride >= D || n <= 1, DGS_ERR_INVALID, "keep_8bit: rows that overlap");
+  if (n == 0) return DGS_OK;
+  DGS_REQUIRE(x != nullptr && codes != nullptr && scales != nullptr, DGS_ERR_INVALID, "keep_8bit: null argument");
+  KeepArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.codes = codes;
+  a.scales = scales;
+  a.n = n;
+  a.D = static_cast<int32_t>(D);
+  a.groups = static_cast<int32_t>((D + KEPT_GROUP - 1) / KEPT_GROUP);
+  a.tasks = n * a.groups;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == DGS_F32 ? keep<float>(a, s) : dtype == DGS_BF16 ? keep<__nv_bfloat16>(a, s) : keep<__half>(a, s);
+}
+
+extern "C" int dgs_kept_8bit_values(const int8_t* codes, int64_t codes_stride, const float* scales, int64_t n, int64_t D, int32_t dtype,
+                                    void* out, dgs_stream_t stream) {
+  if (int rc = check("kept_8bit_values", n, D, dtype)) return rc;
+  DGS_REQUIRE(codes_stride >= D || n <= 1, DGS_ERR_INVALID, "kept_8bit_values: rows that overlap");
+  if (n == 0) return DGS_OK;
+  DGS_REQUIRE(codes != nullptr && scales != nullptr && out != nullptr, DGS_ERR_INVALID, "kept_8bit_values: null argument");
+  KeepArgs a{};
+  a.codes_in = codes;
+  a.codes_stride = codes_stride;
+  a.scales_in = scales;
+  a.out = out;
+  a.n = n;
+  a.D = static_cast<int32_t>(D);
+  a.groups = static_cast<int32_t>((D + KEPT_GROUP - 1) / KEPT_GROUP);
+  a.tasks = n * a.groups;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == DGS_F32 ? values<float>(a, s) : dtype == DGS_BF16 ? values<__nv_bfloat16>(a, s) : values<__half>(a, s);
+}
+
+extern "C" size_t dgs_kept_8bit_weight_grad_workspace_bytes(int64_t n, int64_t O, int64_t D, int32_t dtype) {
+  if (n <= 0 || O <= 0 || D <= 0 || dtype_bytes(dtype) == 0) return 0;
+  const size_t splits = static_cast<size_t>(shares(n, O, D));
+  return splits * (static_cast<size_t>(O) * D + O) * sizeof(float);
+}
+
+extern "C" int dgs_kept_8bit_weight_grad(const void* grad, int64_t grad_stride, int32_t dtype, const int8_t* codes, int64_t codes_stride,
+                                         const float* scales, int64_t n, int64_t O, int64_t D, void* dweight, void* dbias,
+                                         void* workspace, size_t workspace_bytes, dgs_stream_t stream) {
+  if (int rc = check("kept_8bit_weight_grad", n, D, dtype)) return rc;
+  DGS_REQUIRE(O >= 1 && O <= KEPT_MAX_SIDE, DGS_ERR_INVALID, "kept_8bit_weight_grad: %lld rows of the weight", static_cast<long long>(O));
+  DGS_REQUIRE((grad_stride >= O && codes_stride >= D) || n <= 1, DGS_ERR_INVALID, "kept_8bit_weight_grad: rows that overlap");
+  DGS_REQUIRE(dweight != nullptr, DGS_ERR_INVALID, "kept_8bit_weight_grad: null argument");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n == 0) {
+    DGS_CUDA_TRY(cudaMemsetAsync(dweight, 0, static_cast<size_t>(O) * D * dtype_bytes(dtype), s));
+    if (dbias != nullptr) DGS_CUDA_TRY(cudaMemsetAsync(dbias, 0, static_cast<size_t>(O) * dtype_bytes(dtype), s));
+    return DGS_OK;
+  }
+  const size_t need = dgs_kept_8bit_weight_grad_workspace_bytes(n, O, D, dtype);
+  DGS_REQUIRE(grad != nullptr && codes != nullptr && scales != nullptr, DGS_ERR_INVALID, "kept_8bit_weight_grad: null argument");
+  DGS_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned_to(workspace, 256), DGS_ERR_INVALID,
+              "kept_8bit_weight_grad: workspace of %zu bytes, 256-byte aligned, is needed", need);
+  KeptGradArgs a{};
+  a.grad = grad;
+  a.grad_stride = grad_stride;
+  a.codes = codes;
+  a.codes_stride = codes_stride;
+  a.scales = scales;
+  a.n = n;
+  a.O = static_cast<int32_t>(O);
+  a.D = static_cast<int32_t>(D);
+  a.groups = static_cast<int32_t>((D + KEPT_GROUP - 1) / KEPT_GROUP);
+  a.splits = static_cast<int32_t>(shares(n, O, D));
+  a.parts = static_cast<float*>(workspace);
+  a.bias_parts = a.parts + static_cast<int64_t>(a.splits) * O * D;
+  a.dweight = dweight;
+  a.dbias = dbias;
+  return dtype == DGS_F32 ? weight_grad<float>(a, s) : dtype == DGS_BF16 ? weight_grad<__nv_bfloat16>(a, s) : weight_grad<__half>(a, s);
+}

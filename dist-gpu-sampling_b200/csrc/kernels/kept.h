@@ -1,0 +1,21 @@
+// What the kernels of rows kept in 8 bits share (kept.cu: codes, values, entry points).  Not part of the C ABI.
+#pragma once
+#include "train_common.cuh"
+
+namespace dgs {
+
+constexpr int KEPT_GROUP = 128;  // elements of a row that share a scale
+
+struct KeptGradArgs {
+  const void* grad;
+  int64_t grad_stride;
+  const int8_t* codes;
+  int64_t codes_stride;
+  const float* scales;
+  int64_t n;
+  int32_t O, D, groups, splits;
+  float *parts, *bias_parts;  // [splits][O][D], [splits][O]
+  void *dweight, *dbias;
+};
+
+}  // namespace dgs

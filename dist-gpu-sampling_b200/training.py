@@ -77,7 +77,48 @@ def _define():
                                                       want_k or want_v)
             return dq if want_q else None, dk if want_k else None, dv if want_v else None, None, None, None, None
 
-    _functions.update(norm=LayerNorm, loss=LinearCrossEntropy, attention=Attention)
+    class ResidualNorm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, y, gate, post, post_weight, post_bias, pre, weight, bias, x_scale, y_scale, eps):
+            total, out, *stats = ops._CAPI_residual_norm(x, y, gate, post, post_weight, post_bias, pre, weight, bias, x_scale, y_scale, eps)
+            ctx.save_for_backward(total, y, gate, post_weight, post_bias, weight, *stats)
+            ctx.forms, ctx.scales = (post, pre), (x_scale, y_scale)
+            ctx.set_materialize_grads(False)
+            return (total, out) if pre != "none" else (total, None)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, dsum, dout):
+            total, y, gate, post_weight, post_bias, weight, *stats = ctx.saved_tensors
+            if dsum is None and dout is None:
+                return (None,) * 12
+            dx, dy, dgate, dpw, dpb, dw, db = ops._CAPI_residual_norm_backward(
+                dsum, dout, total, y, gate, ctx.forms[0], post_weight, post_bias, ctx.forms[1], weight, *stats, *ctx.scales)
+            grads = (dx, dy, dgate, None, dpw, dpb, None, dw, db, None, None, None)
+            return tuple(g if want else None for g, want in zip(grads, ctx.needs_input_grad))
+
+    class Linear8bit(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight, bias):
+            rows = x.reshape(-1, x.shape[-1])
+            ctx.shape = x.shape
+            ctx.save_for_backward(weight, *ops._CAPI_keep_8bit(rows) if ctx.needs_input_grad[1] else ())
+            return torch.nn.functional.linear(x, weight, bias)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad):
+            weight, *kept = ctx.saved_tensors
+            want_x, want_w, want_b = ctx.needs_input_grad
+            rows = grad.reshape(-1, grad.shape[-1])
+            dw = db = None
+            if want_w:
+                dw, db = ops._CAPI_kept_8bit_weight_grad(rows, *kept, want_b)
+            elif want_b:
+                db = rows.sum(0, dtype=torch.float32).to(grad.dtype)
+            return (rows @ weight).view(ctx.shape) if want_x else None, dw, db if want_b else None
+
+    _functions.update(norm=LayerNorm, loss=LinearCrossEntropy, attention=Attention, residual=ResidualNorm, linear=Linear8bit)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -127,6 +168,48 @@ def attention(q, k, v, q_offsets, k_offsets=None, causal=False, scale=None, retu
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     out, lse = _functions["attention"].apply(q, k, v, q_offsets, k_offsets, bool(causal), scale)
     return (out, lse) if return_lse else out
+
+
+def residual_norm(x, y, gate=None, post=None, post_weight=None, post_bias=None, norm="rms", weight=None, bias=None, x_scale=1.0,
+                  y_scale=1.0, eps=1e-6):
+    """The end of a block and the norm in front of the next one, with gradients for all tensors:
+
+        sum = x_scale * x + y_scale * gate * post(y),   out = norm(sum)        -> (sum, out)
+
+    x (the residual rows) and y (the block's output) have one shape and type.  post and norm: "rms", "layer" or None, over the last
+    dimension (up to 8192 elements), each with a weight and a bias where they are given; norm=None gives None for out.  gate: a value for
+    each column [D], for each row [..., 1] or for each element.  The norm is of the sum as it is stored, in x's type."""
+    if not _functions:
+        _define()
+    for name in (post, norm):
+        if name not in (None, "rms", "layer"):
+            raise ValueError("residual_norm: a norm must be 'rms', 'layer' or None, got %r" % (name,))
+    return _functions["residual"].apply(x, y, gate, post or "none", post_weight, post_bias, norm or "none", weight, bias, float(x_scale),
+                                        float(y_scale), float(eps))
+
+
+def keep_8bit(x):
+    """Rows [n, D] in 8 bits: (codes [n, D] int8, scales [n, ceil(D / 128)] float32).  A code is the nearest of 255 even steps between minus
+    and plus the largest magnitude a among its row's 128 columns: within a / 254 of the value."""
+    return _ops()._CAPI_keep_8bit(x)
+
+
+def kept_8bit_values(codes, scales, dtype=None):
+    """The rows that keep_8bit's codes and scales stand for (dtype: float32 by default)."""
+    import torch
+    return _ops()._CAPI_kept_8bit_values(codes, scales, dtype or torch.float32)
+
+
+def linear_8bit(x, weight, bias=None):
+    """x @ weight.T + bias whose input is kept for the backward pass in 8 bits (keep_8bit) instead of its own type: half the memory of
+    16-bit activations, a quarter of 32-bit ones.  The result and the gradient of x are those of torch's linear; the weight's gradient is
+    taken from the kept rows, in one pass over their codes.  x [..., D], weight [O, D] and bias [O] of one type (16 bits run on the tensor
+    cores)."""
+    if not _functions:
+        _define()
+    if x.dtype != weight.dtype or (bias is not None and bias.dtype != weight.dtype):
+        raise ValueError("linear_8bit: x, weight and bias must share one type")
+    return _functions["linear"].apply(x, weight, bias)
 
 
 class AdamW:

@@ -514,6 +514,61 @@ DGS_API int dgs_attention_backward(const dgs_attention* problem, const void* dou
                                    const void* out, const float* lse, void* dq, void* dk, void* dv, void* workspace,
                                    size_t workspace_bytes, int32_t* status, dgs_stream_t stream);
 
+/* The end of a block and the norm in front of the next one, row by row:
+ *   z = post(y),  sum = x_scale x + y_scale gate z  (stored in x's type),  out = pre(sum)
+ * A norm is (v - mean) / sqrt(avg (v - mean)^2 + eps) * weight + bias (DGS_NORM_LAYER),
+ * the same with mean 0 (DGS_NORM_RMS), or nothing; weight == NULL: 1, bias == NULL: 0
+ * (a bias needs a weight).  The gate is a value for each row [n], for each column [D]
+ * or for each element [n, D] (rows gate_stride apart), or absent.  Rows of up to 8192
+ * elements; weights, biases and a column gate are of type param_dtype, the rest of
+ * type dtype.  Statistics are in 32 bits. */
+enum { DGS_NORM_NONE = 0, DGS_NORM_RMS = 1, DGS_NORM_LAYER = 2 };
+enum { DGS_GATE_NONE = 0, DGS_GATE_ROW = 1, DGS_GATE_COLUMN = 2, DGS_GATE_ELEMENT = 3 };
+typedef struct dgs_residual_norm {
+  const void* y;
+  int64_t y_stride;
+  const void* gate;
+  int64_t gate_stride;
+  const void *post_weight, *post_bias, *weight, *bias;
+  int64_t n, D;
+  int32_t dtype, param_dtype, gate_kind, post, pre;
+  float x_scale, y_scale, eps;
+} dgs_residual_norm;
+/* sum and out (without a pre norm: not written) are contiguous; post_rstd[n], rstd[n]
+ * and, for layer norms, post_mean[n], mean[n] are what the backward pass takes. */
+DGS_API int dgs_residual_norm_forward(const dgs_residual_norm* problem, const void* x, int64_t x_stride, void* sum, void* out,
+                                      float* post_mean, float* post_rstd, float* mean, float* rstd, dgs_stream_t stream);
+/* Gradients for those of sum and out (either may be NULL: zero); contiguous results,
+ * NULL where they are not wanted.  dgate has the gate's shape; the gradients of
+ * weights, biases and of a column gate are summed in a fixed order and take the
+ * workspace, 16-byte aligned. */
+DGS_API size_t dgs_residual_norm_backward_workspace_bytes(int64_t n, int64_t D);
+DGS_API int dgs_residual_norm_backward(const dgs_residual_norm* problem, const void* sum, const void* dsum, int64_t dsum_stride,
+                                       const void* dout, int64_t dout_stride, const float* post_mean, const float* post_rstd,
+                                       const float* mean, const float* rstd, void* dx, void* dy, void* dgate, void* dpost_weight,
+                                       void* dpost_bias, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                                       dgs_stream_t stream);
+
+/* Rows kept for the backward pass in 8 bits: for each row and each 128 of its columns
+ * a = max |x|, codes c = rint(x * (127 / a)) and the scale a / 127, in 32-bit IEEE
+ * arithmetic; c * scale stands for x, within a / 254 (a float32 a within 2^-23 of the
+ * largest number may come back as infinity).  A group that does not hold finite
+ * numbers throughout keeps none.  codes [n, D] contiguous, scales [n, ceil(D / 128)]. */
+DGS_API int dgs_keep_8bit(const void* x, int64_t x_stride, int32_t dtype, int64_t n, int64_t D, int8_t* codes, float* scales,
+                          dgs_stream_t stream);
+/* The rows that codes (codes_stride apart) and scales stand for, rounded to dtype. */
+DGS_API int dgs_kept_8bit_values(const int8_t* codes, int64_t codes_stride, const float* scales, int64_t n, int64_t D, int32_t dtype,
+                                 void* out, dgs_stream_t stream);
+/* The weight's gradient of a linear layer whose input rows were kept so:
+ *   dweight[O, D] = grad[n, O]^T values[n, D],  dbias[O] = column sums of grad (may be NULL)
+ * in grad's type.  For 16-bit types the values are rounded to that type as they are
+ * read (the products are then exact, sums are in 32 bits).  Rows are added in a fixed
+ * order.  workspace: 256-byte aligned. */
+DGS_API size_t dgs_kept_8bit_weight_grad_workspace_bytes(int64_t n, int64_t O, int64_t D, int32_t dtype);
+DGS_API int dgs_kept_8bit_weight_grad(const void* grad, int64_t grad_stride, int32_t dtype, const int8_t* codes, int64_t codes_stride,
+                                      const float* scales, int64_t n, int64_t O, int64_t D, void* dweight, void* dbias,
+                                      void* workspace, size_t workspace_bytes, dgs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
