@@ -31,6 +31,7 @@ ABI_SOURCES = [
     "kernels/cross_entropy_mma.cu",
     "kernels/adamw.cu",
     "kernels/attention.cu",
+    "kernels/attention_mma.cu",
     "kernels/residual_norm.cu",
     "kernels/kept.cu",
     "host/error.cc",

@@ -23,17 +23,52 @@ __device__ __forceinline__ int64_t offset_at(const void* p, int32_t wide, int64_
   return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
 }
 
+// Tiles in order of their work: a bucket for each quarter of a power of two of steps, the heaviest first
+constexpr int PLAN_BUCKETS = 128;
+__device__ __forceinline__ int bucket_of(int steps) {
+  const int top = 31 - __clz(steps | 1), quarter = top >= 2 ? (steps >> (top - 2)) & 3 : 0;
+  return PLAN_BUCKETS - 1 - (top * 4 + quarter);
+}
+__device__ __forceinline__ int tiles_of(int rows, int tile) { return (rows + tile - 1) / tile; }
+
+// the n-th tile of queries (`rows` each), or of keys
+__device__ __forceinline__ AttnTile query_tile(const AttnArgs& a, const AttnSeq& e, int n) {
+  AttnTile t{};
+  const int at = n * a.q_tile_rows;
+  t.row = e.q0 + at;
+  t.rows = min(a.q_tile_rows, e.q_len - at);
+  t.other = e.k0;
+  t.others = e.k_len;
+  t.seen = a.causal ? at + 1 + e.k_len - e.q_len : e.k_len;
+  const int last = a.causal ? min(e.k_len, t.seen + t.rows - 1) : e.k_len;
+  t.steps = last > 0 ? tiles_of(last, ATTN_TILE) : 0;
+  return t;
+}
+__device__ __forceinline__ AttnTile key_tile(const AttnArgs& a, const AttnSeq& e, int n) {
+  AttnTile t{};
+  const int at = n * ATTN_TILE, first = a.causal ? min(e.q_len, max(0, at - (e.k_len - e.q_len))) : 0;
+  t.row = e.k0 + at;
+  t.rows = min(ATTN_TILE, e.k_len - at);
+  t.other = e.q0 + first;
+  t.others = e.q_len - first;
+  t.seen = a.causal ? at - (e.k_len - e.q_len) - first : INT32_MIN / 2;
+  t.steps = tiles_of(t.others, ATTN_TILE);
+  return t;
+}
+
 // A warp for each sequence: its place, whose its rows are, the parts of rows with many keys, the tiles of long ones.
-__global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_constant__ AttnArgs a, int32_t backward, int32_t clear) {
+__global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_constant__ AttnArgs a, int32_t backward, int32_t alone) {
+  __shared__ int bucket[2][PLAN_BUCKETS];
   pdl_enter();
-  const int lane = threadIdx.x & 31;
-  if (clear) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (alone) {
     if (threadIdx.x < ATTN_COUNTS) a.counts[threadIdx.x] = 0;
-    if (threadIdx.x < 2 && a.norms != nullptr) a.norms[threadIdx.x] = 0.0f;
+    if (threadIdx.x < 2) a.norms[threadIdx.x] = 0.0f;
+    if (threadIdx.x < 2 * PLAN_BUCKETS) bucket[threadIdx.x / PLAN_BUCKETS][threadIdx.x % PLAN_BUCKETS] = 0;
     __syncthreads();
   }
   const int warps = gridDim.x * (PLAN_THREADS / 32);
-  for (int s = blockIdx.x * (PLAN_THREADS / 32) + (threadIdx.x >> 5); s < a.seqs; s += warps) {
+  for (int s = blockIdx.x * (PLAN_THREADS / 32) + warp; s < a.seqs; s += warps) {
     const int64_t q0 = offset_at(a.q_offsets, a.offsets64, s), q1 = offset_at(a.q_offsets, a.offsets64, s + 1);
     const int64_t k0 = offset_at(a.k_offsets, a.offsets64, s), k1 = offset_at(a.k_offsets, a.offsets64, s + 1);
     AttnSeq e{0, 0, 0, 0};
@@ -45,7 +80,22 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
     for (int i = lane; i < e.q_len; i += 32) a.q_seq[e.q0 + i] = s;
     if (backward)
       for (int i = lane; i < e.k_len; i += 32) a.k_seq[e.k0 + i] = s;
-    if (attn_in_tiles(a, e)) continue;
+    if (attn_in_tiles(a, e)) {
+      const int nq = tiles_of(e.q_len, a.q_tile_rows), nk = backward ? tiles_of(e.k_len, ATTN_TILE) : 0;
+      if (alone) {  // counted first, placed below
+        for (int i = lane; i < nq; i += 32) atomicAdd(&bucket[0][bucket_of(query_tile(a, e, i).steps)], 1);
+        for (int i = lane; i < nk; i += 32) atomicAdd(&bucket[1][bucket_of(key_tile(a, e, i).steps)], 1);
+        continue;
+      }
+      int at[2] = {0, 0};
+      if (lane < 2) at[0] = atomicAdd(&a.counts[lane ? ATTN_N_K_TILES : ATTN_N_Q_TILES], lane ? nk : nq);
+      at[1] = __shfl_sync(FULL_MASK, at[0], 1);
+      at[0] = __shfl_sync(FULL_MASK, at[0], 0);
+      // (the bounds are of the sizes; offsets that overlap may get beyond them)
+      for (int i = lane; i < nq && at[0] + i < a.q_tile_bound; i += 32) a.q_tiles[at[0] + i] = query_tile(a, e, i);
+      for (int i = lane; i < nk && at[1] + i < a.k_tile_bound; i += 32) a.k_tiles[at[1] + i] = key_tile(a, e, i);
+      continue;
+    }
     if (attn_is_split(e) && e.q_len > 0) {
       const int parts = (e.k_len + ATTN_SPLIT_KEYS - 1) / ATTN_SPLIT_KEYS, all = parts * e.q_len;
       int first = 0;
@@ -53,10 +103,43 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
       first = __shfl_sync(FULL_MASK, first, 0);
       for (int i = lane; i < all; i += 32) {
         const int row = i / parts, part = i - row * parts;
-        if (first + i >= a.split_bound) break;  // (cannot be: the bound is of the sizes; offsets that overlap may get here)
+        if (first + i >= a.split_bound) break;
         a.splits[first + i] = make_int4(e.q0 + row, part * ATTN_SPLIT_KEYS, first + row * parts, parts);
         for (int c = 0; c < a.kv_heads; ++c) a.arrived[static_cast<int64_t>(first + i) * a.kv_heads + c] = 0;
       }
+    }
+  }
+  if (!alone || !a.tiles) return;
+  __syncthreads();
+  if (warp < 2) {  // where each bucket begins
+    int carry = 0;
+    for (int b = lane; b < PLAN_BUCKETS; b += 32) {
+      const int n = bucket[warp][b];
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(FULL_MASK, sum, o);
+        if (lane >= o) sum += up;
+      }
+      bucket[warp][b] = carry + sum - n;
+      carry += __shfl_sync(FULL_MASK, sum, 31);
+    }
+    if (lane == 0) a.counts[warp ? ATTN_N_K_TILES : ATTN_N_Q_TILES] = carry;
+  }
+  __syncthreads();
+  for (int s = warp; s < a.seqs; s += PLAN_THREADS / 32) {
+    const AttnSeq e = a.seq[s];
+    if (!attn_in_tiles(a, e)) continue;
+    for (int i = lane; i < tiles_of(e.q_len, a.q_tile_rows); i += 32) {
+      const AttnTile t = query_tile(a, e, i);
+      const int at = atomicAdd(&bucket[0][bucket_of(t.steps)], 1);
+      if (at < a.q_tile_bound) a.q_tiles[at] = t;
+    }
+    if (!backward) continue;
+    for (int i = lane; i < tiles_of(e.k_len, ATTN_TILE); i += 32) {
+      const AttnTile t = key_tile(a, e, i);
+      const int at = atomicAdd(&bucket[1][bucket_of(t.steps)], 1);
+      if (at < a.k_tile_bound) a.k_tiles[at] = t;
     }
   }
 }
@@ -600,6 +683,16 @@ int64_t lay_out(const dgs_attention& p, bool backward, char* base, AttnArgs* a) 
   a->arrived = reinterpret_cast<uint32_t*>(at(int64_t(4) * a->split_bound * p.kv_heads));
   a->parts = reinterpret_cast<float*>(at(int64_t(4) * a->split_bound * p.heads * floats));
   a->delta = reinterpret_cast<float*>(at(backward ? int64_t(4) * p.heads * p.n_q : 0));
+  // (a scale that is not positive, which no model has, stays on the CUDA cores: the tiles take the largest score for the largest weight)
+  a->tiles = !backward && p.dtype != DGS_F32 && p.n_q >= ATTN_TILE_QUERIES && p.n_k > 0 && p.seqs > 0 && p.scale > 1e-30f;
+  a->q_tile_rows = backward ? ATTN_TILE : 2 * ATTN_TILE;
+  // tiles, whatever the offsets: rows / tile + 1 for each of the sequences that can be that long
+  const int64_t longest = p.n_q / ATTN_TILE_QUERIES, some = a->tiles ? (longest < p.seqs ? longest : p.seqs) : 0;
+  a->q_tile_bound = static_cast<int32_t>(a->tiles ? p.n_q / a->q_tile_rows + some : 0);
+  a->k_tile_bound = static_cast<int32_t>(a->tiles && backward ? p.n_k / ATTN_TILE + some : 0);
+  a->q_tiles = reinterpret_cast<AttnTile*>(at(a->q_tile_bound * static_cast<int64_t>(sizeof(AttnTile))));
+  a->k_tiles = reinterpret_cast<AttnTile*>(at(a->k_tile_bound * static_cast<int64_t>(sizeof(AttnTile))));
+  a->lse2 = reinterpret_cast<float*>(at(a->tiles && backward ? int64_t(4) * p.heads * p.n_q : 0));
   return l.bytes;
 }
 
@@ -642,7 +735,6 @@ AttnArgs arguments(const dgs_attention& p) {
   a.kv_heads = p.kv_heads;
   a.d = p.d;
   a.causal = p.causal != 0;
-  a.tiles = 0;
   a.scale = p.scale;
   return a;
 }
@@ -737,6 +829,8 @@ extern "C" int dgs_attention_forward(const dgs_attention* p, void* out, float* l
   a.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int rc = launch_plan(a, false, s)) return rc;
+  if (a.tiles)
+    if (int rc = attn_tiles_forward(a, p->dtype, s)) return rc;
   return with_type<4>(p->dtype, a, RowsForward{a, s});
 }
 
@@ -772,5 +866,7 @@ extern "C" int dgs_attention_backward(const dgs_attention* p, const void* dout, 
   a.dv = dv;
   a.status = status;
   if (int rc = launch_plan(a, true, s)) return rc;
+  if (a.tiles)
+    if (int rc = attn_tiles_backward(a, p->dtype, s)) return rc;
   return with_type<2>(p->dtype, a, RowsBackward{a, s});
 }

@@ -10,6 +10,16 @@ struct AttnSeq {
   int32_t q0, q_len, k0, k_len;
 };
 
+// A tile of query rows (all heads take it), or of key rows with the query rows that see them.
+struct __align__(16) AttnTile {
+  int32_t row, rows;           // the tile's rows
+  int32_t other, others;       // first row and number of the rows on the other side: the keys; the queries that see one of the keys
+  int32_t seen;                // causal: keys of `others` that the tile's first query sees (may be negative); key tiles: the tile's first key as the
+                               // first of `others` counts the keys that it sees (key j of the tile is seen by query i if j + seen <= i)
+  int32_t steps;               // tiles on the other side
+  int32_t pad[2];
+};
+
 struct AttnView {
   const void* p;
   int64_t row, head;  // strides in elements
@@ -32,11 +42,11 @@ struct AttnArgs {
   int4* splits;                 // {row, first key, index of the row's first part, parts}
   uint32_t* arrived;            // parts that are there, one word for each part (the first of a row's is used) and key head
   float* parts;                 // [part][heads][part_floats]
-  int4 *q_tiles, *k_tiles;      // {sequence, first row, ..} of the tiles, heaviest first
-  float* delta;
+  AttnTile *q_tiles, *k_tiles;  // heaviest first where one CTA makes the plan
+  float *delta, *lse2;  // [heads, n_q]; lse in powers of two, as the tiles' backward pass takes it
   float* norms;                 // [2] the largest row norms of dout and v (as they are ordered, through unsigned words)
   int32_t* status;
-  int32_t split_bound, q_tile_bound, k_tile_bound;
+  int32_t split_bound, q_tile_bound, k_tile_bound, q_tile_rows;
 };
 
 enum { ATTN_N_SPLITS = 0, ATTN_N_Q_TILES = 1, ATTN_N_K_TILES = 2, ATTN_COUNTS = 8 };
@@ -47,7 +57,13 @@ constexpr int ATTN_SPLIT_KEYS = 1024;  // ... so many at a time
 constexpr int ATTN_SPLIT_QUERIES = 16; // (with more queries there are warps enough)
 constexpr int ATTN_TILE_QUERIES = 48;  // queries from which a sequence goes to the tensor cores
 
+constexpr int ATTN_TILE = 128;         // rows of a tile of keys, and of queries in the backward pass (twice as many in the forward one)
+
 __host__ __device__ inline bool attn_in_tiles(const AttnArgs& a, const AttnSeq& s) { return a.tiles && s.q_len >= ATTN_TILE_QUERIES && s.k_len > 0; }
 __host__ __device__ inline bool attn_is_split(const AttnSeq& s) { return s.k_len > ATTN_SPLIT_FROM && s.q_len <= ATTN_SPLIT_QUERIES; }
+
+// attention_mma.cu: the sequences that attn_in_tiles names, after the plan
+int attn_tiles_forward(const AttnArgs& a, int32_t dtype, cudaStream_t s);
+int attn_tiles_backward(const AttnArgs& a, int32_t dtype, cudaStream_t s);
 
 }  // namespace dgs
