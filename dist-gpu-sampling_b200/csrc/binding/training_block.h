@@ -35,7 +35,7 @@ struct Heads {
 };
 inline Heads as_heads(const torch::Tensor& t, int64_t width) {
   const int64_t vec = 16 / t.element_size();
-  const auto whole = [&](int64_t dim) { return t.size(dim) <= 1 || (t.stride(dim) >= 0 && t.stride(dim) % vec == 0); };
+  const auto whole = [&](int64_t dim) { return t.size(dim) <= 1 || (t.stride(dim) > 0 && t.stride(dim) % vec == 0); };
   if (t.size(2) == width && (t.stride(2) == 1 || width == 1) && whole(0) && whole(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
     return {t, t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
   torch::Tensor c = device_empty({t.size(0), t.size(1), width}, t.scalar_type(), t.device());

@@ -684,7 +684,7 @@ int64_t lay_out(const dgs_attention& p, bool backward, char* base, AttnArgs* a) 
   a->parts = reinterpret_cast<float*>(at(int64_t(4) * a->split_bound * p.heads * floats));
   a->delta = reinterpret_cast<float*>(at(backward ? int64_t(4) * p.heads * p.n_q : 0));
   // (a scale that is not positive, which no model has, stays on the CUDA cores: the tiles take the largest score for the largest weight)
-  a->tiles = !backward && p.dtype != DGS_F32 && p.n_q >= ATTN_TILE_QUERIES && p.n_k > 0 && p.seqs > 0 && p.scale > 1e-30f;
+  a->tiles = p.dtype != DGS_F32 && p.n_q >= ATTN_TILE_QUERIES && p.n_k > 0 && p.seqs > 0 && p.scale > 1e-30f;
   a->q_tile_rows = backward ? ATTN_TILE : 2 * ATTN_TILE;
   // tiles, whatever the offsets: rows / tile + 1 for each of the sequences that can be that long
   const int64_t longest = p.n_q / ATTN_TILE_QUERIES, some = a->tiles ? (longest < p.seqs ? longest : p.seqs) : 0;
@@ -710,8 +710,10 @@ int check(const char* who, const dgs_attention* p) {
   DGS_REQUIRE(p->q_row % vec == 0 && p->q_head % vec == 0 && p->k_row % vec == 0 && p->k_head % vec == 0 && p->v_row % vec == 0 &&
                   p->v_head % vec == 0 && aligned_to(p->q, 16) && aligned_to(p->k, 16) && aligned_to(p->v, 16),
               DGS_ERR_INVALID, "%s: heads must begin at 16-byte boundaries", who);
-  DGS_REQUIRE(p->q_row >= 0 && p->q_head >= 0 && p->k_row >= 0 && p->k_head >= 0 && p->v_row >= 0 && p->v_head >= 0, DGS_ERR_INVALID,
-              "%s: strides must not be negative", who);
+  const auto apart = [](int64_t stride, int64_t n) { return stride > 0 || n <= 1; };
+  DGS_REQUIRE(apart(p->q_row, p->n_q) && apart(p->q_head, p->heads) && apart(p->k_row, p->n_k) && apart(p->k_head, p->kv_heads) &&
+                  apart(p->v_row, p->n_k) && apart(p->v_head, p->kv_heads),
+              DGS_ERR_INVALID, "%s: strides must be positive", who);
   DGS_REQUIRE(p->scale - p->scale == 0.0f, DGS_ERR_INVALID, "%s: scale must be a finite number", who);
   DGS_REQUIRE((p->n_q == 0 || p->q != nullptr) && (p->n_k == 0 || (p->k != nullptr && p->v != nullptr)) &&
                   p->q_offsets != nullptr && p->k_offsets != nullptr,
@@ -851,7 +853,8 @@ extern "C" int dgs_attention_backward(const dgs_attention* p, const void* dout, 
   if (dq == nullptr && dk == nullptr) return DGS_OK;
   const int64_t vec = 16 / static_cast<int64_t>(esz);
   DGS_REQUIRE(dout != nullptr && out != nullptr && lse != nullptr && aligned_to(dout, 16) && aligned_to(out, 16) && aligned_to(dq, 16) &&
-                  aligned_to(dk, 16) && aligned_to(dv, 16) && dout_row % vec == 0 && dout_head % vec == 0 && dout_row >= 0 && dout_head >= 0,
+                  aligned_to(dk, 16) && aligned_to(dv, 16) && dout_row % vec == 0 && dout_head % vec == 0 && (dout_row > 0 || p->n_q == 1) &&
+                  (dout_head > 0 || p->heads == 1),
               DGS_ERR_INVALID, "attention_backward: dout, out, lse and gradients must be there, heads must begin at 16-byte boundaries");
   const size_t need = dgs_attention_workspace_bytes(p, 1);
   DGS_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned_to(workspace, 256), DGS_ERR_INVALID,

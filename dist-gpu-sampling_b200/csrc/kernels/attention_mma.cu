@@ -6,8 +6,16 @@
 //   O += P V            P out of TMEM, V as it lies (its rows are the sum's index), O stays in TMEM for all keys
 // While one tile's exponentials run, the tensor cores work on the other's products.  `ref` follows the running maximum of a row only
 // when that has grown by more than 2^8 (the sums are in 32 bits and divided in the end), so O is hardly ever rescaled.
-// Rows travel by cp.async: rows behind a sequence's end, and elements behind a head's, are zeros and never those of a neighbour.
+// Backward: the gradients of keys and values by tiles of 128 keys, those of the queries by tiles of 128 queries, so every sum is
+// made by one CTA in a fixed order, for the price of the scores and of dO V^T computed twice (7 products a pair of tiles, not 5).
+//   keys     S^T = K Q^T, P^T = exp2(S^T c - lse), dV += P^T dO;  E^T = V dO^T, dS^T = P^T (E^T - delta), dK += dS^T Q
+//   queries  S = Q K^T, E = dO V^T, dQ += dS K
+// with P^T, dS^T and dS out of TMEM; S^T's products run while dS^T is made and the other way round.
+// Whole tiles travel by TMA.  Where a product's sum runs over a tile's rows, rows behind a sequence's end have to be zeros, not the next
+// sequence's: such last tiles come row by row through cp.async.
 // Every wait is bounded; a wait that runs out raises DGS_ERR_CUDA in the status word and all roles leave.
+#include <type_traits>
+
 #include "attention.h"
 #include "tensor_core.cuh"
 
@@ -54,16 +62,21 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+struct TileArgs {
+  AttnArgs a;
+  CUtensorMap q, k, v, dout;
+};
+
 // ---- rows into shared memory ------------------------------------------------------------------------------------------
-// 128 rows of a head (`there` of them exist), panels of 64 elements, 128-byte swizzle, asked for with cp.async by the loading threads
+// 128 rows of a head (`there` of them exist, the others become zeros), panels of 64 elements, 128-byte swizzle, by the loading threads
 template <int DP>
 __device__ __forceinline__ void ask_tile(uint32_t dst, const char* p, int64_t row_bytes, int there, int d, int t) {
-  constexpr int CHUNKS = DP / 8, ROWS = LOAD_THREADS / CHUNKS;  // 16-byte pieces of a row; rows a pass (a multiple of 8, or half of it)
+  constexpr int CHUNKS = DP / 8, ROWS = LOAD_THREADS / CHUNKS;  // 16-byte pieces of a row; rows a pass
   const int c = t % CHUNKS, r0 = t / CHUNKS;
   const bool in_d = c * 8 < d;
   const char* src = p + r0 * row_bytes + c * 16;
   const uint32_t base = dst + (c / 8) * PANEL + r0 * 128;
-#pragma unroll
+#pragma unroll 4
   for (int i = 0; i < ATTN_TILE / ROWS; ++i) {
     const int r = r0 + i * ROWS;
     const bool in = in_d && r < there;
@@ -72,31 +85,58 @@ __device__ __forceinline__ void ask_tile(uint32_t dst, const char* p, int64_t ro
     src += ROWS * row_bytes;
   }
 }
-__device__ __forceinline__ void ask_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void ask_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
-// A ring of stages that the loading threads fill in order; a stage is handed over once the two asked for after it are under way.
-template <int STAGES>
-struct Ring {
-  uint32_t full, empty;
-  int at = 0, handed = 0;  // stages asked for, handed over
-  __device__ __forceinline__ int slot() const { return at % STAGES; }
-  __device__ __forceinline__ bool wait_empty(const volatile int* dead) const {
-    return !*dead && bar_wait(empty + 8 * (at % STAGES), ((at / STAGES) & 1) ^ 1);
+// What the loading threads do, each of them: a ring of stages filled in order.
+template <int DP, int STAGES>
+struct Loader {
+  uint32_t tiles, full, empty;  // shared memory of the stages, their barriers
+  int t;
+  const volatile int* dead;
+  int at = 0;        // stages filled
+  int waiting = 0;   // the newest of them that came by cp.async and are not handed over
+
+  __device__ __forceinline__ void panels(uint32_t dst, const CUtensorMap* map, int32_t head, int32_t row, uint32_t bar) const {
+#pragma unroll
+    for (int p = 0; p < DP / 64; ++p) load_box_one(dst + p * PANEL, map, p * 64, head, row, bar);
   }
-  template <int LEFT>
-  __device__ __forceinline__ void hand_over() {  // all but the newest LEFT
-    ask_wait<LEFT>();
-    fence_async_smem();
-    for (; handed < at - LEFT; ++handed) bar_arrive(full + 8 * (handed % STAGES));
+  // a whole tile by TMA; `bar` counts every loading thread
+  __device__ __forceinline__ void box(uint32_t dst, const CUtensorMap* map, int32_t head, int32_t row, uint32_t bar) const {
+    if (t == 0) {
+      bar_expect(bar, tile_bytes<DP>());
+      panels(dst, map, head, row, bar);
+    } else {
+      bar_arrive(bar);
+    }
   }
-  __device__ __forceinline__ void asked() {
-    ask_commit();
+  // two tiles side by side behind one barrier (or the first alone)
+  __device__ __forceinline__ void boxes(uint32_t dst, const CUtensorMap* map, int32_t head, int32_t row, const CUtensorMap* map2, int32_t head2,
+                                        int32_t row2, bool both, uint32_t bar) const {
+    if (t == 0) {
+      bar_expect(bar, (both ? 2 : 1) * tile_bytes<DP>());
+      panels(dst, map, head, row, bar);
+      if (both) panels(dst + tile_bytes<DP>(), map2, head2, row2, bar);
+    } else {
+      bar_arrive(bar);
+    }
+  }
+  __device__ __forceinline__ bool free_stage() const { return !*dead && bar_wait(empty + 8 * (at % STAGES), ((at / STAGES) & 1) ^ 1); }
+  // the next stage: rows row.. of a head, `there` of them; zeros: whether those behind them must be zeros
+  __device__ __forceinline__ void fill(const CUtensorMap* map, const AttnView& view, int32_t head, int32_t row, int there, bool zeros, int d) {
+    const uint32_t dst = tiles + (at % STAGES) * tile_bytes<DP>();
+    if (there >= ATTN_TILE || !zeros) {
+      box(dst, map, head, row, full + 8 * (at % STAGES));
+    } else {
+      ask_tile<DP>(dst, static_cast<const char*>(view.p) + (row * view.row + head * view.head) * 2, view.row * 2, there, d, t);
+      ++waiting;
+    }
     ++at;
-    hand_over<2>();
+  }
+  // (called with those that wait being the newest stages)
+  __device__ __forceinline__ void hand_over() {
+    if (waiting == 0) return;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    fence_async_smem();
+    for (; waiting > 0; --waiting) bar_arrive(full + 8 * ((at - waiting) % STAGES));
   }
 };
 
@@ -156,9 +196,10 @@ __device__ __forceinline__ float scores(uint32_t tmem, int seen, uint32_t (&v)[4
 }
 
 template <int DP, bool BF16>
-__global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __grid_constant__ AttnArgs a) {
+__global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __grid_constant__ TileArgs args) {
   using Shape = ForwardShape<DP>;
   constexpr int STAGES = Shape::STAGES;
+  const AttnArgs& a = args.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t smem = smem_addr(smem_raw), bars = smem + Shape::BARS;
   const uint32_t q_full = bars, q_empty = bars + 8, s_full = bars + 16, p_full = bars + 32, o_full = bars + 48, full = bars + 64,
@@ -187,8 +228,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_word) : "memory");
   pdl_enter();
-  const int n_items = min(a.counts[ATTN_N_Q_TILES], a.q_tile_bound);
-  const int64_t items = static_cast<int64_t>(n_items) * a.heads;
+  const int64_t items = static_cast<int64_t>(min(a.counts[ATTN_N_Q_TILES], a.q_tile_bound)) * a.heads;
   const int group = a.heads / a.kv_heads;
   bool ok = true;
 
@@ -196,41 +236,26 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
     // ---- rows
     fewer_registers<FEW_REGISTERS>();
     if (warp <= SOFTMAX_WARPS + LOAD_WARPS) {  // (the last warp fills the warpgroup)
-    const int t = threadIdx.x - (SOFTMAX_WARPS + 1) * 32;
-    Ring<STAGES> ring{full, empty};
-    int n = 0;  // items with keys so far
-    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const int index = static_cast<int>(item / a.heads), head = static_cast<int>(item - static_cast<int64_t>(index) * a.heads);
-      const AttnTile x = tile_at(a.q_tiles + index);
-      if (x.steps == 0) continue;
-      const char* q = static_cast<const char*>(a.q.p) + (x.row * a.q.row + head * a.q.head) * 2;
-      const char* k = static_cast<const char*>(a.k.p) + (x.other * a.k.row + (head / group) * a.k.head) * 2;
-      const char* v = static_cast<const char*>(a.v.p) + (x.other * a.v.row + (head / group) * a.v.head) * 2;
-      if (!(ok = !*dead && bar_wait(q_empty, (n & 1) ^ 1))) break;
-      ask_tile<DP>(smem, q, a.q.row * 2, x.rows, a.d, t);
-      if (x.rows > ATTN_TILE) ask_tile<DP>(smem + tile_bytes<DP>(), q + ATTN_TILE * a.q.row * 2, a.q.row * 2, x.rows - ATTN_TILE, a.d, t);
-      ask_commit();
-      // K0, V0, K1, V1, ..
-      for (int j = 0; ok && j < 2 * x.steps; ++j) {
-        if (!(ok = ring.wait_empty(dead))) break;
-        const int at = (j >> 1) * ATTN_TILE;
-        const bool key = (j & 1) == 0;
-        const AttnView& view = key ? a.k : a.v;
-        ask_tile<DP>(smem + Shape::RING + ring.slot() * tile_bytes<DP>(), (key ? k : v) + at * view.row * 2, view.row * 2, x.others - at, a.d, t);
-        if (j == 0) {
-          ask_commit();
-          ++ring.at;
-          ask_wait<1>();
-          fence_async_smem();
-          bar_arrive(q_full);
-        } else {
-          ring.asked();
+      fence_async_global();  // rows that ordinary stores of an earlier launch wrote
+      Loader<DP, STAGES> load{smem + Shape::RING, full, empty, static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32, dead};
+      int n = 0;  // items with keys so far
+      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const int index = static_cast<int>(item / a.heads), head = static_cast<int>(item - static_cast<int64_t>(index) * a.heads);
+        const AttnTile x = tile_at(a.q_tiles + index);
+        if (x.steps == 0) continue;
+        if (!(ok = !*dead && bar_wait(q_empty, (n & 1) ^ 1))) break;
+        load.boxes(smem, &args.q, head, x.row, &args.q, head, x.row + ATTN_TILE, x.rows > ATTN_TILE, q_full);
+        // K0, V0, K1, V1, ..  (only V's rows are summed over)
+        for (int j = 0; ok && j < x.steps; ++j) {
+          const int at = j * ATTN_TILE;
+          if (!(ok = load.free_stage())) break;
+          load.fill(&args.k, a.k, head / group, x.other + at, x.others - at, false, a.d);
+          if (!(ok = load.free_stage())) break;
+          load.fill(&args.v, a.v, head / group, x.other + at, x.others - at, true, a.d);
         }
+        load.hand_over();
+        ++n;
       }
-      ring.template hand_over<0>();
-      ++n;
-    }
-    ask_wait<0>();
     }
   } else if (warp == SOFTMAX_WARPS) {
     // ---- products
@@ -394,8 +419,538 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
   }
 }
 
+// ---- backward -----------------------------------------------------------------------------------------------------------
+// fp16 keeps few powers of two: weights are lifted by 2^12 and dS scaled so that its bound becomes 2^15 at the most.  |e| is at most B,
+// the largest |do_i| times the largest |v_j|, and |p (e - delta)| = p (1 - p) |e - the others' mean| at most B / 2.
+template <bool BF16>
+constexpr float lift() {
+  return BF16 ? 0.0f : 12.0f;
+}
+template <bool BF16>
+__device__ __forceinline__ float slope_scale(const AttnArgs& a) {
+  if constexpr (BF16) return 1.0f;
+  const float b = a.norms[0] * a.norms[1];
+  if (!(b > 0.0f) || b - b != 0.0f) return 1.0f / 4096.0f;
+  int e;
+  frexpf(b, &e);
+  return ldexpf(1.0f, max(-100, min(100, 4 - e)));
+}
+
+constexpr int DELTA_THREADS = 256;
+
+// Rows of the tiles' sequences: delta = do.o, lse in powers of two (less the lift), the largest norm of do.  16 lanes a row and head.
+template <typename T>
+__global__ __launch_bounds__(DELTA_THREADS) void attn_delta_kernel(const __grid_constant__ AttnArgs a, float down, int32_t norm) {
+  pdl_enter();
+  const int lane = threadIdx.x % 16, head = blockIdx.y;
+  const int row = blockIdx.x * (DELTA_THREADS / 16) + threadIdx.x / 16;
+  bool mine = false;
+  if (row < a.n_q) {
+    const int s = a.q_seq[row];
+    if (s >= 0 && s < a.seqs) {
+      const AttnSeq e = a.seq[s];
+      mine = row >= e.q0 && row - e.q0 < e.q_len && attn_in_tiles(a, e);
+    }
+  }
+  float sum = 0.0f, square = 0.0f;
+  if (mine && lane * 8 < a.d) {
+    float x[8], y[8];
+    load_vec<T, 8>(static_cast<const T*>(a.dout.p) + row * a.dout.row + head * a.dout.head + lane * 8, x);
+    load_vec<T, 8>(static_cast<const T*>(a.out) + (static_cast<int64_t>(row) * a.heads + head) * a.d + lane * 8, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sum = fmaf(x[i], y[i], sum);
+      square = fmaf(x[i], x[i], square);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(FULL_MASK, sum, o);
+    square += __shfl_xor_sync(FULL_MASK, square, o);
+  }
+  if (mine && lane == 0) {
+    const int64_t at = static_cast<int64_t>(head) * a.n_q + row;
+    const float lse = a.lse[at];
+    a.delta[at] = sum;
+    a.lse2[at] = lse == -INFINITY ? INFINITY : lse * LOG2E - down;  // (a row that sees no key has no weights)
+  }
+  if (norm) {
+    const unsigned top = __reduce_max_sync(FULL_MASK, mine ? __float_as_uint(sqrtf(square)) : 0u);
+    if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(reinterpret_cast<unsigned*>(a.norms), top);
+  }
+}
+
+// the largest norm of v over all rows of the tiles' sequences
+template <typename T>
+__global__ __launch_bounds__(DELTA_THREADS) void attn_norm_kernel(const __grid_constant__ AttnArgs a) {
+  pdl_enter();
+  const int lane = threadIdx.x % 16, head = blockIdx.y;
+  const int row = blockIdx.x * (DELTA_THREADS / 16) + threadIdx.x / 16;
+  bool mine = false;
+  if (row < a.n_k) {
+    const int s = a.k_seq[row];
+    if (s >= 0 && s < a.seqs) {
+      const AttnSeq e = a.seq[s];
+      mine = row >= e.k0 && row - e.k0 < e.k_len && attn_in_tiles(a, e);
+    }
+  }
+  float square = 0.0f;
+  if (mine && lane * 8 < a.d) {
+    float x[8];
+    load_vec<T, 8>(static_cast<const T*>(a.v.p) + row * a.v.row + head * a.v.head + lane * 8, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) square = fmaf(x[i], x[i], square);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) square += __shfl_xor_sync(FULL_MASK, square, o);
+  const unsigned top = __reduce_max_sync(FULL_MASK, mine ? __float_as_uint(sqrtf(square)) : 0u);
+  if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(reinterpret_cast<unsigned*>(a.norms) + 1, top);
+}
+
+template <int DP>
+struct BackwardShape {
+  static constexpr int STAGES = DP == 128 ? 5 : 8;
+  static constexpr uint32_t RING = 2 * tile_bytes<DP>(), STATS = RING + STAGES * tile_bytes<DP>(), BARS = STATS + 2 * 2 * ATTN_TILE * 4,
+                            SMEM = BARS + 256;
+};
+
+// a row of DP values out of TMEM, times `by`, into contiguous rows of d elements
+template <int FROM, int TO, bool BF16>
+__device__ __forceinline__ void store_row(uint32_t tmem, bool there, float by, char* to, int d) {
+#pragma unroll
+  for (int q = FROM / 32; q < TO / 32; ++q) {
+    uint32_t r[32];
+    tmem_load32(tmem + q * 32, r);
+    tmem_wait(r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = pack2<BF16>(__uint_as_float(r[i * 8 + e * 2]) * by, __uint_as_float(r[i * 8 + e * 2 + 1]) * by);
+      if (there && q * 32 + i * 8 < d) *reinterpret_cast<uint4*>(to + (q * 32 + i * 8) * 2) = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+  }
+}
+template <int FROM, int TO>
+__device__ __forceinline__ void store_zeros(bool there, char* to, int d) {
+#pragma unroll
+  for (int i = FROM / 8; i < TO / 8; ++i)
+    if (there && i * 8 < d) *reinterpret_cast<uint4*>(to + i * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// dK and dV of 128 keys of one key head, over the queries of all heads of its group
+template <int DP, bool BF16>
+__global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_constant__ TileArgs args) {
+  using Shape = BackwardShape<DP>;
+  constexpr int STAGES = Shape::STAGES;
+  const AttnArgs& a = args.a;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t smem = smem_addr(smem_raw), bars = smem + Shape::BARS;
+  const uint32_t kv_full = bars, kv_empty = bars + 8, s_full = bars + 16, e_full = bars + 24, p_full = bars + 32, ds_full = bars + 40,
+                 done = bars + 48, stats_full = bars + 56, stats_empty = bars + 72, full = bars + 88, empty = full + 8 * STAGES,
+                 tmem_word = empty + 8 * STAGES;
+  volatile int* dead = reinterpret_cast<volatile int*>(smem_raw + (tmem_word + 4 - smem));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    bar_init(kv_full, LOAD_THREADS);
+    bar_init(kv_empty, 1);
+    bar_init(s_full, 1);
+    bar_init(e_full, 1);
+    bar_init(p_full, SOFTMAX_WARPS * 32);
+    bar_init(ds_full, SOFTMAX_WARPS * 32);
+    bar_init(done, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(stats_full + 8 * i, LOAD_THREADS);
+      bar_init(stats_empty + 8 * i, SOFTMAX_WARPS * 32);
+    }
+    for (int i = 0; i < STAGES; ++i) {
+      bar_init(full + 8 * i, LOAD_THREADS);
+      bar_init(empty + 8 * i, 1);
+    }
+    *dead = 0;
+    bar_init_fence();
+  }
+  if (warp == 0) tmem_alloc_one(tmem_word, TMEM_COLS);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_word) : "memory");
+  pdl_enter();
+  const int64_t items = static_cast<int64_t>(min(a.counts[ATTN_N_K_TILES], a.k_tile_bound)) * a.kv_heads;
+  const int group = a.heads / a.kv_heads;
+  bool ok = true;
+
+  if (warp > SOFTMAX_WARPS) {
+    // ---- rows
+    fewer_registers<FEW_REGISTERS>();
+    if (warp <= SOFTMAX_WARPS + LOAD_WARPS) {
+      fence_async_global();
+      const int t = static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32;
+      Loader<DP, STAGES> load{smem + Shape::RING, full, empty, t, dead};
+      int n = 0, step = 0;
+      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const int index = static_cast<int>(item / a.kv_heads), kv = static_cast<int>(item - static_cast<int64_t>(index) * a.kv_heads);
+        const AttnTile x = tile_at(a.k_tiles + index);
+        if (x.steps == 0) continue;
+        if (!(ok = !*dead && bar_wait(kv_empty, (n & 1) ^ 1))) break;
+        load.boxes(smem, &args.k, kv, x.row, &args.v, kv, x.row, true, kv_full);
+        for (int u = 0; ok && u < x.steps * group; ++u, ++step) {
+          const int head = kv * group + u / x.steps, at = u % x.steps * ATTN_TILE, row = x.other + at, left = x.others - at;
+          if (!(ok = load.free_stage())) break;
+          load.fill(&args.q, a.q, head, row, left, true, a.d);
+          const int slot = step & 1;
+          if (!(ok = !*dead && bar_wait(stats_empty + 8 * slot, ((step >> 1) & 1) ^ 1))) break;
+          const uint32_t to = smem + Shape::STATS + slot * 2 * ATTN_TILE * 4;
+          const int64_t from = static_cast<int64_t>(head) * a.n_q + row;
+#pragma unroll
+          for (int i = 0; i < ATTN_TILE / LOAD_THREADS; ++i) {
+            const int c = t + i * LOAD_THREADS;
+            const int64_t src = from + (c < left ? c : 0);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + c * 4), "l"(a.lse2 + src), "r"(c < left ? 4 : 0) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + (ATTN_TILE + c) * 4), "l"(a.delta + src),
+                         "r"(c < left ? 4 : 0)
+                         : "memory");
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(stats_full + 8 * slot) : "memory");
+          if (!(ok = load.free_stage())) break;
+          load.fill(&args.dout, a.dout, head, row, left, true, a.d);
+          load.hand_over();
+        }
+        ++n;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+  } else if (warp == SOFTMAX_WARPS) {
+    // ---- products
+    fewer_registers<FEW_REGISTERS>();
+    if (lane == 0) {
+      const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
+      const uint32_t s = tmem, e = tmem + 128, dv = tmem + 256, dk = tmem + 256 + DP;
+      const uint32_t k = smem, v = smem + tile_bytes<DP>();
+      int st = 0, n = 0, at = 0;
+      const auto stage = [&](int i) { return smem + Shape::RING + (i % STAGES) * tile_bytes<DP>(); };
+      const auto ready = [&](int i) { return !*dead && bar_wait(full + 8 * (i % STAGES), (i / STAGES) & 1); };
+      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const AttnTile x = tile_at(a.k_tiles + item / a.kv_heads);
+        if (x.steps == 0) continue;
+        if (!(ok = !*dead && bar_wait(kv_full, n & 1) && ready(st))) break;
+        fence_after();
+        product_rows<DP>(s, k, stage(st), by_rows);
+        mma_commit_one(s_full);
+        if (!(ok = ready(st + 1))) break;
+        product_rows<DP>(e, v, stage(st + 1), by_rows);
+        mma_commit_one(e_full);
+        const int steps = x.steps * group;
+        for (int u = 0; ok && u < steps; ++u, st += 2, ++at) {
+          const bool more = u + 1 < steps;
+          if (!(ok = !*dead && bar_wait(p_full, at & 1))) break;
+          fence_after();
+          product_columns<DP>(dv, s, 64, stage(st + 1), by_columns, u > 0);
+          if (more) {
+            if (!(ok = ready(st + 2))) break;
+            product_rows<DP>(s, k, stage(st + 2), by_rows);
+            mma_commit_one(s_full);
+          }
+          mma_commit_one(empty + 8 * ((st + 1) % STAGES));
+          if (!(ok = !*dead && bar_wait(ds_full, at & 1))) break;
+          fence_after();
+          product_columns<DP>(dk, e, 64, stage(st), by_columns, u > 0);
+          mma_commit_one(empty + 8 * (st % STAGES));
+          if (more) {
+            if (!(ok = ready(st + 3))) break;
+            product_rows<DP>(e, v, stage(st + 3), by_rows);
+            mma_commit_one(e_full);
+          }
+        }
+        if (!ok) break;
+        mma_commit_one(done);
+        mma_commit_one(kv_empty);
+        ++n;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- weights and slopes: a key a thread, half of the queries a warpgroup
+    more_registers<MANY_REGISTERS>();
+    const int half = warp / 4, mine = warp % 4 * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+    const uint32_t s = tmem + half * 64 + lanes, e = tmem + 128 + half * 64 + lanes;
+    const float c = a.scale * LOG2E, by = slope_scale<BF16>(a);
+    int at = 0, items_done = 0;
+    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      const int index = static_cast<int>(item / a.kv_heads), kv = static_cast<int>(item - static_cast<int64_t>(index) * a.kv_heads);
+      const AttnTile x = tile_at(a.k_tiles + index);
+      const bool there = mine < x.rows;
+      char* to = static_cast<char*>(half ? a.dk : a.dv) + (static_cast<int64_t>(x.row + mine) * a.kv_heads + kv) * a.d * 2;
+      if (x.steps == 0) {
+        store_zeros<0, DP>(there, to, a.d);
+        continue;
+      }
+      for (int u = 0; u < x.steps * group; ++u, ++at) {
+        const int slot = at & 1, q0 = u % x.steps * ATTN_TILE + half * 64;
+        const float4* stats = reinterpret_cast<const float4*>(smem_raw + Shape::STATS + slot * 2 * ATTN_TILE * 4 + half * 64 * 4);
+        if (!(ok = !*dead && bar_wait(stats_full + 8 * slot, (at >> 1) & 1) && bar_wait(s_full, at & 1))) break;
+        fence_after();
+        uint32_t r[2][32];
+        float p[64];
+        tmem_load32(s, r[0]);
+        tmem_load32(s + 32, r[1]);
+        tmem_wait(r[0]);
+        tmem_wait(r[1]);
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+          const float4 lse = stats[i / 4];
+          p[i] = ex2(fmaf(__uint_as_float(r[i / 32][i % 32]), c, -lse.x));
+          p[i + 1] = ex2(fmaf(__uint_as_float(r[i / 32][i % 32 + 1]), c, -lse.y));
+          p[i + 2] = ex2(fmaf(__uint_as_float(r[i / 32][i % 32 + 2]), c, -lse.z));
+          p[i + 3] = ex2(fmaf(__uint_as_float(r[i / 32][i % 32 + 3]), c, -lse.w));
+        }
+        if (x.seen + ATTN_TILE - 1 > q0) {  // (some key of the tile is behind some query)
+#pragma unroll
+          for (int i = 0; i < 64; ++i) p[i] = mine + x.seen <= q0 + i ? p[i] : 0.0f;
+        }
+        uint32_t y[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) y[i] = pack2<BF16>(p[2 * i], p[2 * i + 1]);
+        tmem_store32(s, y);
+        tmem_store_wait();
+        fence_before();
+        bar_arrive(p_full);
+        if (!(ok = !*dead && bar_wait(e_full, at & 1))) break;
+        fence_after();
+        tmem_load32(e, r[0]);
+        tmem_load32(e + 32, r[1]);
+        tmem_wait(r[0]);
+        tmem_wait(r[1]);
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+          const float4 delta = stats[ATTN_TILE / 4 + i / 4];
+          const float d0 = p[i] * by * (__uint_as_float(r[i / 32][i % 32]) - delta.x);
+          const float d1 = p[i + 1] * by * (__uint_as_float(r[i / 32][i % 32 + 1]) - delta.y);
+          const float d2 = p[i + 2] * by * (__uint_as_float(r[i / 32][i % 32 + 2]) - delta.z);
+          const float d3 = p[i + 3] * by * (__uint_as_float(r[i / 32][i % 32 + 3]) - delta.w);
+          y[i / 2] = pack2<BF16>(d0, d1);
+          y[i / 2 + 1] = pack2<BF16>(d2, d3);
+        }
+        tmem_store32(e, y);
+        tmem_store_wait();
+        fence_before();
+        bar_arrive(stats_empty + 8 * slot);
+        bar_arrive(ds_full);
+      }
+      if (!ok) break;
+      if (!(ok = !*dead && bar_wait(done, items_done++ & 1))) break;
+      fence_after();
+      const float last = half ? a.scale / (by * exp2f(lift<BF16>())) : exp2f(-lift<BF16>());
+      store_row<0, DP, BF16>(tmem + 256 + half * DP + lanes, there, last, to, a.d);
+      fence_before();
+    }
+  }
+  if (!ok) {
+    *dead = 1;
+    raise_status(a.status, DGS_ERR_CUDA);
+  }
+  __syncthreads();
+  if (*dead)
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  if (warp == 0) {
+    fence_after();
+    tmem_free_one(tmem, TMEM_COLS);
+  }
+}
+
+// dQ of 128 queries of one head
+template <int DP, bool BF16>
+__global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_constant__ TileArgs args) {
+  using Shape = BackwardShape<DP>;
+  constexpr int STAGES = Shape::STAGES;
+  const AttnArgs& a = args.a;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t smem = smem_addr(smem_raw), bars = smem + Shape::BARS;
+  const uint32_t q_full = bars, q_empty = bars + 8, s_full = bars + 16, e_full = bars + 32, e_read = bars + 40, ds_full = bars + 48,
+                 done = bars + 64, full = bars + 72, empty = full + 8 * STAGES, tmem_word = empty + 8 * STAGES;
+  volatile int* dead = reinterpret_cast<volatile int*>(smem_raw + (tmem_word + 4 - smem));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    bar_init(q_full, LOAD_THREADS);
+    bar_init(q_empty, 1);
+    bar_init(s_full, 1);
+    bar_init(s_full + 8, 1);
+    bar_init(e_full, 1);
+    bar_init(e_read, SOFTMAX_WARPS * 32);
+    // (two: the slopes of a step may be there before the products' thread has looked for those of the step before)
+    bar_init(ds_full, SOFTMAX_WARPS * 32);
+    bar_init(ds_full + 8, SOFTMAX_WARPS * 32);
+    bar_init(done, 1);
+    for (int i = 0; i < STAGES; ++i) {
+      bar_init(full + 8 * i, LOAD_THREADS);
+      bar_init(empty + 8 * i, 1);
+    }
+    *dead = 0;
+    bar_init_fence();
+  }
+  if (warp == 0) tmem_alloc_one(tmem_word, TMEM_COLS);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_word) : "memory");
+  pdl_enter();
+  const int64_t items = static_cast<int64_t>(min(a.counts[ATTN_N_Q_TILES], a.q_tile_bound)) * a.heads;
+  const int group = a.heads / a.kv_heads;
+  bool ok = true;
+
+  if (warp > SOFTMAX_WARPS) {
+    // ---- rows
+    fewer_registers<FEW_REGISTERS>();
+    if (warp <= SOFTMAX_WARPS + LOAD_WARPS) {
+      fence_async_global();
+      Loader<DP, STAGES> load{smem + Shape::RING, full, empty, static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32, dead};
+      int n = 0;
+      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const int index = static_cast<int>(item / a.heads), head = static_cast<int>(item - static_cast<int64_t>(index) * a.heads);
+        const AttnTile x = tile_at(a.q_tiles + index);
+        if (x.steps == 0) continue;
+        if (!(ok = !*dead && bar_wait(q_empty, (n & 1) ^ 1))) break;
+        load.boxes(smem, &args.q, head, x.row, &args.dout, head, x.row, true, q_full);
+        // K0, V0, K1, V1, ..  (K's rows are summed over)
+        for (int j = 0; ok && j < x.steps; ++j) {
+          const int at = j * ATTN_TILE;
+          if (!(ok = load.free_stage())) break;
+          load.fill(&args.k, a.k, head / group, x.other + at, x.others - at, true, a.d);
+          load.hand_over();
+          if (!(ok = load.free_stage())) break;
+          load.fill(&args.v, a.v, head / group, x.other + at, x.others - at, false, a.d);
+        }
+        ++n;
+      }
+    }
+  } else if (warp == SOFTMAX_WARPS) {
+    // ---- products
+    fewer_registers<FEW_REGISTERS>();
+    if (lane == 0) {
+      const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
+      const uint32_t s[2] = {tmem, tmem + 128}, e = tmem + 256, dq = tmem + 384;
+      const uint32_t q = smem, g = smem + tile_bytes<DP>();
+      int st = 0, n = 0, at = 0;
+      const auto stage = [&](int i) { return smem + Shape::RING + (i % STAGES) * tile_bytes<DP>(); };
+      const auto ready = [&](int i) { return !*dead && bar_wait(full + 8 * (i % STAGES), (i / STAGES) & 1); };
+      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const AttnTile x = tile_at(a.q_tiles + item / a.heads);
+        if (x.steps == 0) continue;
+        if (!(ok = !*dead && bar_wait(q_full, n & 1) && ready(st))) break;
+        fence_after();
+        product_rows<DP>(s[at & 1], q, stage(st), by_rows);
+        mma_commit_one(s_full + 8 * (at & 1));
+        if (!(ok = ready(st + 1))) break;
+        product_rows<DP>(e, g, stage(st + 1), by_rows);
+        mma_commit_one(e_full);
+        mma_commit_one(empty + 8 * ((st + 1) % STAGES));
+        for (int j = 0; ok && j < x.steps; ++j, st += 2, ++at) {
+          if (j + 1 < x.steps) {
+            if (!(ok = ready(st + 2))) break;
+            product_rows<DP>(s[(at + 1) & 1], q, stage(st + 2), by_rows);
+            mma_commit_one(s_full + 8 * ((at + 1) & 1));
+            if (!(ok = ready(st + 3) && !*dead && bar_wait(e_read, at & 1))) break;
+            fence_after();
+            product_rows<DP>(e, g, stage(st + 3), by_rows);
+            mma_commit_one(e_full);
+            mma_commit_one(empty + 8 * ((st + 3) % STAGES));
+          }
+          if (!(ok = !*dead && bar_wait(ds_full + 8 * (at & 1), (at >> 1) & 1))) break;
+          fence_after();
+          product_columns<DP>(dq, s[at & 1], 64, stage(st), by_columns, j > 0);
+          mma_commit_one(empty + 8 * (st % STAGES));
+        }
+        if (!ok) break;
+        mma_commit_one(done);
+        mma_commit_one(q_empty);
+        ++n;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- slopes: a query a thread, half of the keys a warpgroup
+    more_registers<MANY_REGISTERS>();
+    const int half = warp / 4, mine = warp % 4 * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+    const uint32_t e = tmem + 256 + half * 64 + lanes;
+    const float c = a.scale * LOG2E, by = slope_scale<BF16>(a);
+    int at = 0, items_done = 0;
+    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      const int index = static_cast<int>(item / a.heads), head = static_cast<int>(item - static_cast<int64_t>(index) * a.heads);
+      const AttnTile x = tile_at(a.q_tiles + index);
+      const bool there = mine < x.rows;
+      char* to = static_cast<char*>(a.dq) + (static_cast<int64_t>(x.row + mine) * a.heads + head) * a.d * 2;
+      if (x.steps == 0) {
+        if (half) store_zeros<DP / 2, DP>(there, to, a.d);
+        else store_zeros<0, DP / 2>(there, to, a.d);
+        continue;
+      }
+      const int64_t stat = static_cast<int64_t>(head) * a.n_q + x.row + mine;
+      const float lse = there ? a.lse2[stat] : INFINITY, delta = there ? a.delta[stat] : 0.0f;
+      const int seen = a.causal ? min(x.others, x.seen + mine) : x.others, first = a.causal ? min(x.seen, x.others) : x.others;
+      for (int j = 0; j < x.steps; ++j, ++at) {
+        const uint32_t s = tmem + (at & 1) * 128 + half * 64 + lanes;
+        if (!(ok = !*dead && bar_wait(s_full + 8 * (at & 1), (at >> 1) & 1))) break;
+        fence_after();
+        uint32_t r[2][32];
+        float p[64];
+        tmem_load32(s, r[0]);
+        tmem_load32(s + 32, r[1]);
+        tmem_wait(r[0]);
+        tmem_wait(r[1]);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) p[i] = ex2(fmaf(__uint_as_float(r[i / 32][i % 32]), c, -lse));
+        if (!(ok = !*dead && bar_wait(e_full, at & 1))) break;
+        fence_after();
+        tmem_load32(e, r[0]);
+        tmem_load32(e + 32, r[1]);
+        tmem_wait(r[0]);
+        tmem_wait(r[1]);
+        fence_before();
+        bar_arrive(e_read);
+        const int left = seen - j * ATTN_TILE - half * 64;
+        uint32_t y[32];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) p[i] = p[i] * by * (__uint_as_float(r[i / 32][i % 32]) - delta);
+        if (first < (j + 1) * ATTN_TILE) {  // (what lies behind the keys that are seen may be anything)
+#pragma unroll
+          for (int i = 0; i < 64; ++i) p[i] = i < left ? p[i] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) y[i] = pack2<BF16>(p[2 * i], p[2 * i + 1]);
+        tmem_store32(s, y);
+        tmem_store_wait();
+        fence_before();
+        bar_arrive(ds_full + 8 * (at & 1));
+      }
+      if (!ok) break;
+      if (!(ok = !*dead && bar_wait(done, items_done++ & 1))) break;
+      fence_after();
+      const float last = a.scale / (by * exp2f(lift<BF16>()));
+      if (half) store_row<DP / 2, DP, BF16>(tmem + 384 + lanes, there, last, to, a.d);
+      else store_row<0, DP / 2, BF16>(tmem + 384 + lanes, there, last, to, a.d);
+      fence_before();
+    }
+  }
+  if (!ok) {
+    *dead = 1;
+    raise_status(a.status, DGS_ERR_CUDA);
+  }
+  __syncthreads();
+  if (*dead)
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  if (warp == 0) {
+    fence_after();
+    tmem_free_one(tmem, TMEM_COLS);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
 template <typename Kernel>
-int launch_tiles(Kernel kernel, const AttnArgs& a, int64_t items, uint32_t smem, std::atomic<bool>* known, cudaStream_t s) {
+int launch_tiles(Kernel kernel, const TileArgs& args, int64_t items, uint32_t smem, std::atomic<bool>* known, cudaStream_t s) {
   int dev = 0;
   DGS_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= MAX_DEVICES || !known[dev].load(std::memory_order_relaxed)) {
@@ -403,24 +958,59 @@ int launch_tiles(Kernel kernel, const AttnArgs& a, int64_t items, uint32_t smem,
     if (dev < MAX_DEVICES) known[dev].store(true, std::memory_order_relaxed);
   }
   const int64_t most = sm_count();
-  DGS_CUDA_TRY(launch_training(kernel, dim3(static_cast<unsigned>(items < most ? items : most)), TILE_THREADS, smem, s, a));
+  DGS_CUDA_TRY(launch_training(kernel, dim3(static_cast<unsigned>(items < most ? items : most)), TILE_THREADS, smem, s, args));
   return DGS_OK;
 }
 
+int heads_map(CUtensorMap* map, const AttnView& v, int32_t dtype, int d, int heads, int64_t rows) {
+  return make_heads_map(map, v.p, dtype, d, heads, v.head, rows, v.row, 64, ATTN_TILE);
+}
+
 template <int DP, bool BF16>
-int forward(const AttnArgs& a, cudaStream_t s) {
+int forward(const TileArgs& t, cudaStream_t s) {
   static_assert(ForwardShape<DP>::SMEM <= MAX_SMEM, "shared memory");
   static std::atomic<bool> known[MAX_DEVICES] = {};
-  return launch_tiles(attn_forward_kernel<DP, BF16>, a, static_cast<int64_t>(a.q_tile_bound) * a.heads, ForwardShape<DP>::SMEM, known, s);
+  return launch_tiles(attn_forward_kernel<DP, BF16>, t, static_cast<int64_t>(t.a.q_tile_bound) * t.a.heads, ForwardShape<DP>::SMEM, known, s);
+}
+
+template <int DP, bool BF16>
+int backward(const TileArgs& t, cudaStream_t s) {
+  static_assert(BackwardShape<DP>::SMEM <= MAX_SMEM, "shared memory");
+  static std::atomic<bool> known[2][MAX_DEVICES] = {};
+  const AttnArgs& a = t.a;
+  using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+  const auto ctas = [](int rows) { return static_cast<unsigned>((rows + DELTA_THREADS / 16 - 1) / (DELTA_THREADS / 16)); };
+  DGS_CUDA_TRY(launch_training(attn_delta_kernel<T>, dim3(ctas(a.n_q), a.heads), DELTA_THREADS, 0, s, a, lift<BF16>(), static_cast<int32_t>(!BF16)));
+  if (!BF16) DGS_CUDA_TRY(launch_training(attn_norm_kernel<T>, dim3(ctas(a.n_k), a.kv_heads), DELTA_THREADS, 0, s, a));
+  if (a.dk != nullptr)
+    if (int rc = launch_tiles(attn_dkv_kernel<DP, BF16>, t, static_cast<int64_t>(a.k_tile_bound) * a.kv_heads, BackwardShape<DP>::SMEM, known[0], s))
+      return rc;
+  if (a.dq != nullptr)
+    return launch_tiles(attn_dq_kernel<DP, BF16>, t, static_cast<int64_t>(a.q_tile_bound) * a.heads, BackwardShape<DP>::SMEM, known[1], s);
+  return DGS_OK;
 }
 
 }  // namespace
 
 int attn_tiles_forward(const AttnArgs& a, int32_t dtype, cudaStream_t s) {
-  if (a.d <= 64) return dtype == DGS_BF16 ? forward<64, true>(a, s) : forward<64, false>(a, s);
-  return dtype == DGS_BF16 ? forward<128, true>(a, s) : forward<128, false>(a, s);
+  TileArgs t{};
+  t.a = a;
+  if (int rc = heads_map(&t.q, a.q, dtype, a.d, a.heads, a.n_q)) return rc;
+  if (int rc = heads_map(&t.k, a.k, dtype, a.d, a.kv_heads, a.n_k)) return rc;
+  if (int rc = heads_map(&t.v, a.v, dtype, a.d, a.kv_heads, a.n_k)) return rc;
+  if (a.d <= 64) return dtype == DGS_BF16 ? forward<64, true>(t, s) : forward<64, false>(t, s);
+  return dtype == DGS_BF16 ? forward<128, true>(t, s) : forward<128, false>(t, s);
 }
 
-int attn_tiles_backward(const AttnArgs&, int32_t, cudaStream_t) { return DGS_OK; }
+int attn_tiles_backward(const AttnArgs& a, int32_t dtype, cudaStream_t s) {
+  TileArgs t{};
+  t.a = a;
+  if (int rc = heads_map(&t.q, a.q, dtype, a.d, a.heads, a.n_q)) return rc;
+  if (int rc = heads_map(&t.k, a.k, dtype, a.d, a.kv_heads, a.n_k)) return rc;
+  if (int rc = heads_map(&t.v, a.v, dtype, a.d, a.kv_heads, a.n_k)) return rc;
+  if (int rc = heads_map(&t.dout, a.dout, dtype, a.d, a.heads, a.n_q)) return rc;
+  if (a.d <= 64) return dtype == DGS_BF16 ? backward<64, true>(t, s) : backward<64, false>(t, s);
+  return dtype == DGS_BF16 ? backward<128, true>(t, s) : backward<128, false>(t, s);
+}
 
 }  // namespace dgs

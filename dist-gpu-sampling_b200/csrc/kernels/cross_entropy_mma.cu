@@ -28,8 +28,9 @@
 namespace dgs {
 namespace tc {
 
-int make_map(CUtensorMap* map, const void* base, int32_t dtype, int64_t cols, int64_t rows, int64_t pitch, uint32_t box_cols,
-             uint32_t box_rows) {
+namespace {
+int encode(CUtensorMap* map, const void* base, int32_t dtype, uint32_t rank, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                               CUtensorMapFloatOOBfill);
@@ -41,18 +42,37 @@ int make_map(CUtensorMap* map, const void* base, int32_t dtype, int64_t cols, in
     DGS_REQUIRE(found == cudaDriverEntryPointSuccess && fn != nullptr, DGS_ERR_CUDA, "the driver has no tensor maps");
     known.store(fn, std::memory_order_release);
   }
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * dtype_bytes(dtype)};
-  const cuuint32_t box[2] = {box_cols, box_rows}, step[2] = {1, 1};
+  const cuuint32_t step[3] = {1, 1, 1};
   const CUtensorMapDataType type = dtype == DGS_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : dtype == DGS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const CUresult rc = reinterpret_cast<Encode>(fn)(map, type, 2, const_cast<void*>(base), dims, strides, box, step,
+  const CUresult rc = reinterpret_cast<Encode>(fn)(map, type, rank, const_cast<void*>(base), dims, strides, box, step,
                                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  DGS_REQUIRE(rc == CUDA_SUCCESS, DGS_ERR_CUDA, "tensor map of %lld x %lld elements, %lld apart: error %d", static_cast<long long>(rows),
-              static_cast<long long>(cols), static_cast<long long>(pitch), static_cast<int>(rc));
+  DGS_REQUIRE(rc == CUDA_SUCCESS, DGS_ERR_CUDA, "tensor map of %lld x %lld elements, %lld bytes apart: error %d",
+              static_cast<long long>(dims[1]), static_cast<long long>(dims[0]), static_cast<long long>(strides[0]), static_cast<int>(rc));
   return DGS_OK;
+}
+}  // namespace
+
+int make_map(CUtensorMap* map, const void* base, int32_t dtype, int64_t cols, int64_t rows, int64_t pitch, uint32_t box_cols,
+             uint32_t box_rows) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * dtype_bytes(dtype)};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  return encode(map, base, dtype, 2, dims, strides, box);
+}
+
+int make_heads_map(CUtensorMap* map, const void* base, int32_t dtype, int64_t d, int64_t heads, int64_t head_pitch, int64_t rows,
+                   int64_t row_pitch, uint32_t box_cols, uint32_t box_rows) {
+  // (a stride along which nothing lies is any that the encoding takes)
+  if (heads <= 1 && head_pitch <= 0) head_pitch = d;
+  if (rows <= 1 && row_pitch <= 0) row_pitch = d;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_pitch) * dtype_bytes(dtype),
+                                 static_cast<cuuint64_t>(row_pitch) * dtype_bytes(dtype)};
+  const cuuint32_t box[3] = {box_cols, 1, box_rows};
+  return encode(map, base, dtype, 3, dims, strides, box);
 }
 
 }  // namespace tc

@@ -82,6 +82,13 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       "l"(map), "r"(x), "r"(y), "r"(cluster_bar)
       : "memory");
 }
+// One box of a map of three dimensions, for a CTA on its own
+__device__ __forceinline__ void load_box_one(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void store_box(const CUtensorMap* map, int32_t x, int32_t y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
                "r"(src)
@@ -213,6 +220,9 @@ __device__ __forceinline__ uint32_t mma_desc(bool bf16, bool a_mn, bool b_mn, ui
 // box_cols elements are 128 bytes.
 int make_map(CUtensorMap* map, const void* base, int32_t dtype, int64_t cols, int64_t rows, int64_t pitch, uint32_t box_cols,
              uint32_t box_rows);
+// rows of `heads` heads of d elements each (pitches in elements), moved in boxes of box_cols elements of one head in box_rows rows
+int make_heads_map(CUtensorMap* map, const void* base, int32_t dtype, int64_t d, int64_t heads, int64_t head_pitch, int64_t rows,
+                   int64_t row_pitch, uint32_t box_cols, uint32_t box_rows);
 
 }  // namespace tc
 }  // namespace dgs

@@ -8,7 +8,12 @@ of a row, with 16 U for exp2 and its argument's own rounding, |x| U).
   ds    = p (e - delta); delta may come from the rounded out:  E = sum |do| (r |o| + (r + 2 s + n U) sum p |v|); rounded itself:
         dev = (r + 2 s + n U) p (|e| + |delta|) + p (E + n U sum|do||v|max)
   dq    r |dq| + scale sum_j dev |k|,  dk  r |dk| + scale sum_i dev |q|
-(float32 operands and delta taken in 32 bits are held to the same, with r = U.)  2^-24 of fp16's smallest steps is added."""
+(float32 operands and delta taken in 32 bits are held to the same, with r = U.)
+Below the normal numbers roundings are absolute.  exp2 flushes weights under F = 2^-126 to 0, so every p may be off by F.  In fp16
+half a step is 2^-25 at the most: the forward pass holds weights lifted by 2^4 or more (the row's largest is at least that), which leaves
+2^-29 of p; the backward pass lifts them by 2^12, which leaves 2^-37, and scales ds so that its bound 2 B 2^12 s / 4 is between 2^14 and 2^15,
+B the largest |do| times the largest |v| (norms of rows) of all sequences: 2^-25 of that is at most B 2^-40.  One smallest step for the
+results' own rounding."""
 import math
 
 import pytest
@@ -49,6 +54,11 @@ def definition(q, k, v, do, q_lens, k_lens, causal, scale):
     tol = {n: torch.zeros_like(t) for n, t in res.items()}
     res["lse"] = torch.full((h, nq), -math.inf, device="cuda", dtype=torch.float64)
     tol["lse"] = torch.zeros_like(res["lse"])
+    half = dt == torch.float16
+    nq, nk = sum(q_lens), sum(k_lens)
+    F = 2.0 ** -126
+    floor_out, floor_p = F + 2.0 ** -29 * half, F + 2.0 ** -37 * half
+    floor_ds = 2.0 ** -40 * half * do[:nq].norm(dim=2).amax() * v[:nk].norm(dim=2).amax() if nq and nk else 0.0
     a = c = 0
     for lq, lk in zip(q_lens, k_lens):
         A, C = slice(a, a + lq), slice(c, c + lk)
@@ -76,14 +86,14 @@ def definition(q, k, v, do, q_lens, k_lens, causal, scale):
             off = off + U * torch.where(live, lse.abs(), 0.0)[:, None]
             step = r + 2 * off
             res["out"][A, x], res["lse"][x, A] = o, lse
-            tol["out"][A, x] = r * o.abs() + (step + lk * U) * (p @ V.abs())
+            tol["out"][A, x] = r * o.abs() + ((step + lk * U) * p + floor_out) @ V.abs()
             tol["lse"][x, A] = off[:, 0] * 2 + U * torch.where(live, lse.abs(), 0.0)
             res["dq"][A, x] = ds @ K * scale
             res["dk"][C, x // g] += ds.t() @ Q * scale
             res["dv"][C, x // g] += p.t() @ D
-            tol["dv"][C, x // g] += ((step + (lq + 8) * U) * p).t() @ D.abs()
+            tol["dv"][C, x // g] += ((step + (lq + 8) * U) * p + floor_p).t() @ D.abs()
             E = (D.abs() * (r * o.abs() + (step + (lk + d) * U) * (p @ V.abs()))).sum(1, keepdim=True)
-            dev = (step + (lk + lq + 8) * U) * p * (e.abs() + delta.abs()) + p * (E + (d + 4) * U * (D.abs() @ V.abs().t()))
+            dev = ((step + (lk + lq + 8) * U) * p + floor_p) * (e.abs() + delta.abs()) + floor_ds + p * (E + (d + 4) * U * (D.abs() @ V.abs().t()))
             tol["dq"][A, x] = abs(scale) * (dev @ K.abs())
             tol["dk"][C, x // g] += abs(scale) * (dev.t() @ Q.abs())
     for n in ("dq", "dk", "dv"):
@@ -365,6 +375,21 @@ def test_recorded_and_replayed(ops):
         torch.cuda.synchronize()
         for g, res in graphs:
             assert all(torch.equal(a, b) for a, b in zip(res, want))
+
+
+def test_many_calls_in_flight(ops):
+    """Calls queued one behind the other, each with several tiles for every SM: no wait of theirs may run out."""
+    lens = [2048] * 4
+    q, k, v, do = make(lens, lens, 8, 4, 128, torch.bfloat16)
+    o = offsets(lens)
+    out, lse = ops._CAPI_attention(q, k, v, o, o, True, 0.1)
+    base = ops._CAPI_attention_backward(do, q, k, v, out, lse, o, o, True, 0.1, True, True)
+    for _ in range(100):
+        last = ops._CAPI_attention_backward(do, q, k, v, out, lse, o, o, True, 0.1, True, True)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(base, last))
+    again = ops._CAPI_attention(q, k, v, o, o, True, 0.1)  # (an error of an earlier call would be raised here)
+    assert torch.equal(again[0], out)
 
 
 def test_on_another_stream(ops):
