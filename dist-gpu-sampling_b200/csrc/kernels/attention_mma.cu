@@ -27,7 +27,7 @@ constexpr int SOFTMAX_WARPS = 8, LOAD_WARPS = 2;
 constexpr int LOAD_THREADS = LOAD_WARPS * 32;
 constexpr int TILE_THREADS = 384;  // three warpgroups: two of a row (or half of one) a thread, one of the products' and the loading warps
 // Registers: 3 x 128 x 168 at the launch; the first two take what the third leaves
-constexpr int MANY_REGISTERS = 208, FEW_REGISTERS = 80;
+constexpr int MANY_REGISTERS = 200, FEW_REGISTERS = 104;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int MAX_SMEM = 232448;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -141,6 +141,25 @@ struct Loader {
 };
 
 // ---- products ---------------------------------------------------------------------------------------------------------
+// The products' thread: a stage of the ring, ahead of which it may look.
+template <int DP, int STAGES>
+struct Stage {
+  uint32_t tiles, full, empty;
+  const volatile int* dead;
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ int slot_of(int ahead) const { return slot + ahead < STAGES ? slot + ahead : slot + ahead - STAGES; }
+  __device__ __forceinline__ uint32_t tile(int ahead) const { return tiles + slot_of(ahead) * tile_bytes<DP>(); }
+  __device__ __forceinline__ bool ready(int ahead) const {
+    return !*dead && bar_wait(full + 8 * slot_of(ahead), slot + ahead < STAGES ? phase : phase ^ 1);
+  }
+  __device__ __forceinline__ void release(int ahead) const { mma_commit_one(empty + 8 * slot_of(ahead)); }
+  __device__ __forceinline__ void advance(int by) {
+    slot += by;
+    if (slot >= STAGES) slot -= STAGES, phase ^= 1;
+  }
+};
+
 // D[128, 128] = A[128, DP] B[128, DP]^T, both K-major tiles in shared memory
 template <int DP>
 __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
@@ -177,22 +196,56 @@ struct ForwardShape {
   static constexpr uint32_t RING = 2 * tile_bytes<DP>(), BARS = RING + STAGES * tile_bytes<DP>(), SMEM = BARS + 256;
 };
 
-// 128 scores of a row in powers of two: the largest, with those that the row does not see at minus infinity
+// One tile's 128 scores of a row: read for the largest, read again for the weights, 32 columns at a time with the next 32 on their way
+// (held in registers between the two they spill).  `seen`: columns that the row sees (MASK: fewer than 128 may be).
 template <bool MASK>
-__device__ __forceinline__ float scores(uint32_t tmem, int seen, uint32_t (&v)[4][32]) {
+__device__ __forceinline__ float largest(uint32_t s, int seen) {
+  uint32_t v[2][32];
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  tmem_load32(s, v[0]);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_load32(tmem + c * 32, v[c]);
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_wait(v[c]);
-  float top = -INFINITY;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
+  for (int q = 0; q < 4; ++q) {
+    tmem_wait(v[q & 1]);
+    if (q < 3) tmem_load32(s + (q + 1) * 32, v[(q + 1) & 1]);
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      if (MASK && c * 32 + i >= seen) v[c][i] = __float_as_uint(-INFINITY);
-      top = fmaxf(top, __uint_as_float(v[c][i]));
+      float x = __uint_as_float(v[q & 1][i]);
+      if (MASK) x = q * 32 + i < seen ? x : -INFINITY;
+      top[i & 3] = fmaxf(top[i & 3], x);
     }
-  return top;
+  }
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+// weights exp2(score c - base) into the scores' place, 16 bits each; returns their sum
+template <bool MASK, bool BF16>
+__device__ __forceinline__ float weigh(uint32_t s, int seen, float c, float base) {
+  const uint64_t c2 = two(c, c), base2 = two(-base, -base);
+  uint64_t sum[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
+  uint32_t v[2][32];
+  tmem_load32(s, v[0]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    tmem_wait(v[q & 1]);
+    if (q < 3) tmem_load32(s + (q + 1) * 32, v[(q + 1) & 1]);
+    uint32_t p[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float lo, hi;
+      split2(fma2(two(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])), c2, base2), &lo, &hi);
+      lo = ex2(lo);
+      hi = ex2(hi);
+      if (MASK) {
+        lo = q * 32 + 2 * i < seen ? lo : 0.0f;
+        hi = q * 32 + 2 * i + 1 < seen ? hi : 0.0f;
+      }
+      sum[i & 1] = add2(sum[i & 1], two(lo, hi));
+      p[i] = pack2<BF16>(lo, hi);
+    }
+    tmem_store16(s + q * 16, p);
+  }
+  float lo, hi;
+  split2(add2(sum[0], sum[1]), &lo, &hi);
+  return lo + hi;
 }
 
 template <int DP, bool BF16>
@@ -262,39 +315,47 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
     fewer_registers<FEW_REGISTERS>();
     if (lane == 0) {
       const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
-      const uint32_t s[2] = {tmem, tmem + 128}, o[2] = {tmem + 256, tmem + 256 + DP};
-      int st = 0, p_at[2] = {0, 0}, n = 0;
-      const auto stage = [&](int i) { return smem + Shape::RING + (i % STAGES) * tile_bytes<DP>(); };
-      const auto ready = [&](int i) { return !*dead && bar_wait(full + 8 * (i % STAGES), (i / STAGES) & 1); };
+      Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
+      uint32_t p_phase[2] = {0, 0};
+      int n = 0;
+      // O += P V of the tile of queries w, then S of the next keys
+      const auto step = [&](auto which, bool first, bool more) {
+        constexpr uint32_t w = decltype(which)::value;
+        const uint32_t s = tmem + w * 128;
+        if (*dead || !bar_wait(p_full + 8 * w, p_phase[w])) return false;
+        p_phase[w] ^= 1;
+        fence_after();
+        product_columns<DP>(tmem + 256 + w * DP, s, 32, st.tile(1), by_columns, !first);
+        if (more) {
+          product_rows<DP>(s, smem + w * tile_bytes<DP>(), st.tile(2), by_rows);
+          mma_commit_one(s_full + 8 * w);
+        } else {
+          mma_commit_one(o_full + 8 * w);
+        }
+        return true;
+      };
+      using One = std::integral_constant<uint32_t, 0>;
+      using Two = std::integral_constant<uint32_t, 1>;
       for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
         const AttnTile x = tile_at(a.q_tiles + item / a.heads);
         if (x.steps == 0) continue;
-        const int two = x.rows > ATTN_TILE ? 2 : 1;
-        if (!(ok = !*dead && bar_wait(q_full, n & 1) && ready(st))) break;
+        const bool two = x.rows > ATTN_TILE;
+        if (!(ok = !*dead && bar_wait(q_full, n & 1) && st.ready(0))) break;
         fence_after();
-        for (int w = 0; w < two; ++w) {
-          product_rows<DP>(s[w], smem + w * tile_bytes<DP>(), stage(st), by_rows);
-          mma_commit_one(s_full + 8 * w);
+        product_rows<DP>(tmem, smem, st.tile(0), by_rows);
+        mma_commit_one(s_full);
+        if (two) {
+          product_rows<DP>(tmem + 128, smem + tile_bytes<DP>(), st.tile(0), by_rows);
+          mma_commit_one(s_full + 8);
         }
-        mma_commit_one(empty + 8 * (st % STAGES));
+        st.release(0);
         for (int j = 0; ok && j < x.steps; ++j) {
           const bool more = j + 1 < x.steps;
-          if (!(ok = ready(st + 1) && (!more || ready(st + 2)))) break;
-          for (int w = 0; w < two; ++w) {
-            if (!(ok = !*dead && bar_wait(p_full + 8 * w, p_at[w]++ & 1))) break;
-            fence_after();
-            product_columns<DP>(o[w], s[w], 32, stage(st + 1), by_columns, j > 0);
-            if (more) {
-              product_rows<DP>(s[w], smem + w * tile_bytes<DP>(), stage(st + 2), by_rows);
-              mma_commit_one(s_full + 8 * w);
-            } else {
-              mma_commit_one(o_full + 8 * w);
-            }
-          }
-          if (!ok) break;
-          mma_commit_one(empty + 8 * ((st + 1) % STAGES));
-          if (more) mma_commit_one(empty + 8 * ((st + 2) % STAGES));
-          st += 2;
+          if (!(ok = st.ready(1) && (!more || st.ready(2)))) break;
+          if (!(ok = step(One{}, j == 0, more) && (!two || step(Two{}, j == 0, more)))) break;
+          st.release(1);
+          if (more) st.release(2);
+          st.advance(2);
         }
         if (!ok) break;
         mma_commit_one(q_empty);
@@ -324,15 +385,9 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
         for (int j = 0; j < x.steps; ++j) {
           if (!(ok = !*dead && bar_wait(s_full + 8 * w, at++ & 1))) break;
           fence_after();
-          uint32_t v[4][32];
           const int left = seen - j * ATTN_TILE;
-          float top;
-          if (first >= (j + 1) * ATTN_TILE && x.others >= (j + 1) * ATTN_TILE) {
-            top = scores<false>(s, ATTN_TILE, v);
-          } else {
-            top = scores<true>(s, left, v);
-          }
-          top *= c;
+          const bool whole = first >= (j + 1) * ATTN_TILE && x.others >= (j + 1) * ATTN_TILE;
+          const float top = c * (whole ? largest<false>(s, ATTN_TILE) : largest<true>(s, left));
           if (__any_sync(FULL_MASK, top > ref + LAZY)) {
             const float next = fmaxf(top, ref), by = next == -INFINITY ? 1.0f : ex2(ref - next);
             ref = next;
@@ -350,27 +405,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
             }
           }
           const float base = ref == -INFINITY ? 0.0f : ref - LIFT;
-          const uint64_t c2 = two(c, c), base2 = two(-base, -base);
-          uint64_t sum = two(0.0f, 0.0f), sum_b = sum;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t p[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int q = h * 2 + i / 16, at2 = (i % 16) * 2;
-              float lo, hi;
-              split2(fma2(two(__uint_as_float(v[q][at2]), __uint_as_float(v[q][at2 + 1])), c2, base2), &lo, &hi);
-              lo = ex2(lo);
-              hi = ex2(hi);
-              if (i & 1) sum_b = add2(sum_b, two(lo, hi));
-              else sum = add2(sum, two(lo, hi));
-              p[i] = pack2<BF16>(lo, hi);
-            }
-            tmem_store32(s + h * 32, p);
-          }
-          float lo, hi;
-          split2(add2(sum, sum_b), &lo, &hi);
-          l += lo + hi;
+          l += whole ? weigh<false, BF16>(s, ATTN_TILE, c, base) : weigh<true, BF16>(s, left, c, base);
           tmem_store_wait();
           fence_before();
           bar_arrive(p_full + 8 * w);
@@ -628,40 +663,39 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
       const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
       const uint32_t s = tmem, e = tmem + 128, dv = tmem + 256, dk = tmem + 256 + DP;
       const uint32_t k = smem, v = smem + tile_bytes<DP>();
-      int st = 0, n = 0, at = 0;
-      const auto stage = [&](int i) { return smem + Shape::RING + (i % STAGES) * tile_bytes<DP>(); };
-      const auto ready = [&](int i) { return !*dead && bar_wait(full + 8 * (i % STAGES), (i / STAGES) & 1); };
+      Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
+      int n = 0;
+      uint32_t at = 0;
       for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
         const AttnTile x = tile_at(a.k_tiles + item / a.kv_heads);
         if (x.steps == 0) continue;
-        if (!(ok = !*dead && bar_wait(kv_full, n & 1) && ready(st))) break;
+        if (!(ok = !*dead && bar_wait(kv_full, n & 1) && st.ready(0))) break;
         fence_after();
-        product_rows<DP>(s, k, stage(st), by_rows);
+        product_rows<DP>(s, k, st.tile(0), by_rows);
         mma_commit_one(s_full);
-        if (!(ok = ready(st + 1))) break;
-        product_rows<DP>(e, v, stage(st + 1), by_rows);
+        if (!(ok = st.ready(1))) break;
+        product_rows<DP>(e, v, st.tile(1), by_rows);
         mma_commit_one(e_full);
         const int steps = x.steps * group;
-        for (int u = 0; ok && u < steps; ++u, st += 2, ++at) {
+        for (int u = 0; ok && u < steps; ++u, at ^= 1) {
           const bool more = u + 1 < steps;
-          if (!(ok = !*dead && bar_wait(p_full, at & 1))) break;
+          if (!(ok = (!more || st.ready(2)) && !*dead && bar_wait(p_full, at))) break;
           fence_after();
-          product_columns<DP>(dv, s, 64, stage(st + 1), by_columns, u > 0);
+          product_columns<DP>(dv, s, 64, st.tile(1), by_columns, u > 0);
           if (more) {
-            if (!(ok = ready(st + 2))) break;
-            product_rows<DP>(s, k, stage(st + 2), by_rows);
+            product_rows<DP>(s, k, st.tile(2), by_rows);
             mma_commit_one(s_full);
           }
-          mma_commit_one(empty + 8 * ((st + 1) % STAGES));
-          if (!(ok = !*dead && bar_wait(ds_full, at & 1))) break;
+          st.release(1);
+          if (!(ok = (!more || st.ready(3)) && !*dead && bar_wait(ds_full, at))) break;
           fence_after();
-          product_columns<DP>(dk, e, 64, stage(st), by_columns, u > 0);
-          mma_commit_one(empty + 8 * (st % STAGES));
+          product_columns<DP>(dk, e, 64, st.tile(0), by_columns, u > 0);
           if (more) {
-            if (!(ok = ready(st + 3))) break;
-            product_rows<DP>(e, v, stage(st + 3), by_rows);
+            product_rows<DP>(e, v, st.tile(3), by_rows);
             mma_commit_one(e_full);
           }
+          st.release(0);
+          st.advance(2);
         }
         if (!ok) break;
         mma_commit_one(done);
@@ -831,37 +865,37 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
     fewer_registers<FEW_REGISTERS>();
     if (lane == 0) {
       const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
-      const uint32_t s[2] = {tmem, tmem + 128}, e = tmem + 256, dq = tmem + 384;
-      const uint32_t q = smem, g = smem + tile_bytes<DP>();
-      int st = 0, n = 0, at = 0;
-      const auto stage = [&](int i) { return smem + Shape::RING + (i % STAGES) * tile_bytes<DP>(); };
-      const auto ready = [&](int i) { return !*dead && bar_wait(full + 8 * (i % STAGES), (i / STAGES) & 1); };
+      const uint32_t e = tmem + 256, dq = tmem + 384, q = smem, g = smem + tile_bytes<DP>();
+      Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
+      int n = 0;
+      uint32_t at = 0;
       for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
         const AttnTile x = tile_at(a.q_tiles + item / a.heads);
         if (x.steps == 0) continue;
-        if (!(ok = !*dead && bar_wait(q_full, n & 1) && ready(st))) break;
+        if (!(ok = !*dead && bar_wait(q_full, n & 1) && st.ready(0))) break;
         fence_after();
-        product_rows<DP>(s[at & 1], q, stage(st), by_rows);
+        product_rows<DP>(tmem + (at & 1) * 128, q, st.tile(0), by_rows);
         mma_commit_one(s_full + 8 * (at & 1));
-        if (!(ok = ready(st + 1))) break;
-        product_rows<DP>(e, g, stage(st + 1), by_rows);
+        if (!(ok = st.ready(1))) break;
+        product_rows<DP>(e, g, st.tile(1), by_rows);
         mma_commit_one(e_full);
-        mma_commit_one(empty + 8 * ((st + 1) % STAGES));
-        for (int j = 0; ok && j < x.steps; ++j, st += 2, ++at) {
+        st.release(1);
+        for (int j = 0; ok && j < x.steps; ++j, ++at) {
           if (j + 1 < x.steps) {
-            if (!(ok = ready(st + 2))) break;
-            product_rows<DP>(s[(at + 1) & 1], q, stage(st + 2), by_rows);
+            if (!(ok = st.ready(2))) break;
+            product_rows<DP>(tmem + ((at + 1) & 1) * 128, q, st.tile(2), by_rows);
             mma_commit_one(s_full + 8 * ((at + 1) & 1));
-            if (!(ok = ready(st + 3) && !*dead && bar_wait(e_read, at & 1))) break;
+            if (!(ok = st.ready(3) && !*dead && bar_wait(e_read, at & 1))) break;
             fence_after();
-            product_rows<DP>(e, g, stage(st + 3), by_rows);
+            product_rows<DP>(e, g, st.tile(3), by_rows);
             mma_commit_one(e_full);
-            mma_commit_one(empty + 8 * ((st + 3) % STAGES));
+            st.release(3);
           }
           if (!(ok = !*dead && bar_wait(ds_full + 8 * (at & 1), (at >> 1) & 1))) break;
           fence_after();
-          product_columns<DP>(dq, s[at & 1], 64, stage(st), by_columns, j > 0);
-          mma_commit_one(empty + 8 * (st % STAGES));
+          product_columns<DP>(dq, tmem + (at & 1) * 128, 64, st.tile(0), by_columns, j > 0);
+          st.release(0);
+          st.advance(2);
         }
         if (!ok) break;
         mma_commit_one(done);
