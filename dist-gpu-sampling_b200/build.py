@@ -34,6 +34,7 @@ ABI_SOURCES = [
     "kernels/attention_mma.cu",
     "kernels/residual_norm.cu",
     "kernels/kept.cu",
+    "kernels/kept_mma.cu",
     "host/error.cc",
     "host/comm.cc",
     "host/store.cc",

@@ -167,11 +167,10 @@ int values(const KeepArgs& a, cudaStream_t s) {
   return DGS_OK;
 }
 
-// ---- the weight's gradient on the CUDA cores ------------------------------------------------------------------------------
+// ---- the weight's gradient of 32-bit operands, on the CUDA cores ------------------------------------------------------------------------------
 // A tile of 64 x 64 results a CTA over a share of the rows, 4 x 4 a thread; the shares are added in their order afterwards.
 constexpr int WG_TILE = 64, WG_ROWS = 16, WG_THREADS = 256;
 
-template <typename T>
 __global__ __launch_bounds__(WG_THREADS) void kept_grad_kernel(const __grid_constant__ KeptGradArgs a) {
   __shared__ __align__(16) float g[WG_ROWS][WG_TILE + 4], v[WG_ROWS][WG_TILE + 4];
   pdl_enter();
@@ -183,9 +182,8 @@ __global__ __launch_bounds__(WG_THREADS) void kept_grad_kernel(const __grid_cons
     for (int i = threadIdx.x; i < WG_ROWS * WG_TILE; i += WG_THREADS) {
       const int row = i / WG_TILE, c = i % WG_TILE;
       const bool in = r + row < r1;
-      g[row][c] = in && o0 + c < a.O ? to_float<T>(static_cast<const T*>(a.grad)[(r + row) * a.grad_stride + o0 + c]) : 0.0f;
-      v[row][c] = in && d0 + c < a.D ? to_float<T>(from_float<T>(static_cast<float>(a.codes[(r + row) * a.codes_stride + d0 + c]) *
-                                                                 a.scales[(r + row) * a.groups + (d0 + c) / KEPT_GROUP]))
+      g[row][c] = in && o0 + c < a.O ? static_cast<const float*>(a.grad)[(r + row) * a.grad_stride + o0 + c] : 0.0f;
+      v[row][c] = in && d0 + c < a.D ? static_cast<float>(a.codes[(r + row) * a.codes_stride + d0 + c]) * a.scales[(r + row) * a.groups + (d0 + c) / KEPT_GROUP]
                                      : 0.0f;
     }
     __syncthreads();
@@ -233,7 +231,8 @@ __global__ __launch_bounds__(KEEP_THREADS) void kept_join_kernel(const __grid_co
 }
 
 // Shares of the rows: enough CTAs for four on each SM, shares of 256 rows at least
-int64_t shares(int64_t n, int64_t O, int64_t D) {
+int64_t shares(int64_t n, int64_t O, int64_t D, int32_t dtype) {
+  if (dtype != DGS_F32) return kept_mma_shares(n, O, D);
   const int64_t tiles = ((O + WG_TILE - 1) / WG_TILE) * ((D + WG_TILE - 1) / WG_TILE);
   int64_t want = (static_cast<int64_t>(sm_count()) * 4 + tiles - 1) / tiles;
   const int64_t most = (n + 255) / 256;
@@ -242,13 +241,21 @@ int64_t shares(int64_t n, int64_t O, int64_t D) {
 }
 
 template <typename T>
-int weight_grad(const KeptGradArgs& a, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((a.D + WG_TILE - 1) / WG_TILE), static_cast<unsigned>((a.O + WG_TILE - 1) / WG_TILE),
-                  static_cast<unsigned>(a.splits));
-  DGS_CUDA_TRY(launch_training(kept_grad_kernel<T>, grid, WG_THREADS, 0, s, a));
+int join(const KeptGradArgs& a, cudaStream_t s) {
   const int64_t need = (static_cast<int64_t>(a.O) * a.D + KEEP_THREADS - 1) / KEEP_THREADS, most = static_cast<int64_t>(sm_count()) * 8;
   DGS_CUDA_TRY(launch_training(kept_join_kernel<T>, dim3(static_cast<unsigned>(need < most ? need : most)), KEEP_THREADS, 0, s, a));
   return DGS_OK;
+}
+
+int weight_grad(const KeptGradArgs& a, int32_t dtype, cudaStream_t s) {
+  if (dtype != DGS_F32) {
+    if (int rc = kept_mma_weight_grad(a, dtype, s)) return rc;
+    return a.splits == 1 ? DGS_OK : dtype == DGS_BF16 ? join<__nv_bfloat16>(a, s) : join<__half>(a, s);
+  }
+  const dim3 grid(static_cast<unsigned>((a.D + WG_TILE - 1) / WG_TILE), static_cast<unsigned>((a.O + WG_TILE - 1) / WG_TILE),
+                  static_cast<unsigned>(a.splits));
+  DGS_CUDA_TRY(launch_training(kept_grad_kernel, grid, WG_THREADS, 0, s, a));
+  return join<float>(a, s);
 }
 
 constexpr int64_t KEPT_MAX_SIDE = int64_t(1) << 22;  // elements of a row
@@ -305,7 +312,7 @@ extern "C" int dgs_kept_8bit_values(const int8_t* codes, int64_t codes_stride, c
 
 extern "C" size_t dgs_kept_8bit_weight_grad_workspace_bytes(int64_t n, int64_t O, int64_t D, int32_t dtype) {
   if (n <= 0 || O <= 0 || D <= 0 || dtype_bytes(dtype) == 0) return 0;
-  const size_t splits = static_cast<size_t>(shares(n, O, D));
+  const size_t splits = static_cast<size_t>(shares(n, O, D, dtype));
   return splits * (static_cast<size_t>(O) * D + O) * sizeof(float);
 }
 
@@ -336,10 +343,10 @@ extern "C" int dgs_kept_8bit_weight_grad(const void* grad, int64_t grad_stride, 
   a.O = static_cast<int32_t>(O);
   a.D = static_cast<int32_t>(D);
   a.groups = static_cast<int32_t>((D + KEPT_GROUP - 1) / KEPT_GROUP);
-  a.splits = static_cast<int32_t>(shares(n, O, D));
+  a.splits = static_cast<int32_t>(shares(n, O, D, dtype));
   a.parts = static_cast<float*>(workspace);
   a.bias_parts = a.parts + static_cast<int64_t>(a.splits) * O * D;
   a.dweight = dweight;
   a.dbias = dbias;
-  return dtype == DGS_F32 ? weight_grad<float>(a, s) : dtype == DGS_BF16 ? weight_grad<__nv_bfloat16>(a, s) : weight_grad<__half>(a, s);
+  return weight_grad(a, dtype, s);
 }

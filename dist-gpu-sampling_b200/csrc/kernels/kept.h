@@ -1,4 +1,4 @@
-// What the kernels of rows kept in 8 bits share (kept.cu: codes, values, entry points).  Not part of the C ABI.
+// What the kernels of rows kept in 8 bits share (kept.cu: codes, values, entry points; kept_mma.cu: the weight's gradient on the tensor cores).  Not part of the C ABI.
 #pragma once
 #include "train_common.cuh"
 
@@ -17,5 +17,9 @@ struct KeptGradArgs {
   float *parts, *bias_parts;  // [splits][O][D], [splits][O]
   void *dweight, *dbias;
 };
+
+// kept_mma.cu: 16-bit gradients on the tensor cores; one share writes the results, several leave parts to be added
+int64_t kept_mma_shares(int64_t n, int64_t O, int64_t D);
+int kept_mma_weight_grad(const KeptGradArgs& a, int32_t dtype, cudaStream_t s);
 
 }  // namespace dgs

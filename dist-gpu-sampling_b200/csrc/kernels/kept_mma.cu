@@ -1,0 +1,334 @@
+// The gradient of a linear layer's weight from rows kept in 8 bits, 16-bit gradients, on the tensor cores:
+//   dW[o, d] = sum_n g[n, o] v[n, d],  v = code * scale rounded to g's type (so that products are exact; sums are in 32 bits)
+//
+// A CTA takes 256 x 256 results over a share of the rows, 64 at a time: eight warps fetch rows of g and codes, turn the codes into
+// values and leave both in shared memory as they lie (the sum's index outermost: MN-major tiles), one thread issues the products
+// (cta_group::1, two accumulators of 128 x 256 in TMEM).  The rows' next 64 are fetched into registers while these are stored.
+// With few results the rows are cut into shares that fill the SMs; shares are added in their order by a second launch.
+// Bound by HBM where a result tile takes all columns (430 000 rows of 256 against 47: 358 bytes a row), by the tensor cores beyond.
+#include "kept.h"
+#include "tensor_core.cuh"
+
+namespace dgs {
+namespace {
+using namespace tc;
+
+constexpr int TILE = 256, ROWS = 64, FETCH_THREADS = 256, THREADS = FETCH_THREADS + 32, STAGES = 3;
+constexpr uint32_t PANEL = ROWS * 128;                 // 64 columns of 64 rows
+constexpr uint32_t OPERAND = TILE / 64 * PANEL, STAGE = 2 * OPERAND;
+constexpr uint32_t BARS = STAGES * STAGE, SMEM = BARS + 128;
+constexpr int G_CHUNKS = TILE / 8, G_TASKS = ROWS * G_CHUNKS / FETCH_THREADS;   // 16-byte pieces of g's rows, a thread's
+constexpr int C_CHUNKS = TILE / 16, C_TASKS = ROWS * C_CHUNKS / FETCH_THREADS;  // 16 codes
+constexpr int MAX_DEVICES = 64;
+
+// 16 bytes of a row from byte `at` on; what lies at or behind byte `end` comes as anything, but is not read where a whole word does.
+// ALIGNED: rows begin at 16-byte boundaries, else they are put together out of the aligned words that hold them.
+template <bool ALIGNED>
+struct Piece {
+  uint32_t w[ALIGNED ? 4 : 5];
+  __device__ __forceinline__ void fetch(const char* row, int64_t at, int64_t end) {
+    if constexpr (ALIGNED) {
+      const uint4 v = at < end ? __ldg(reinterpret_cast<const uint4*>(row + at)) : make_uint4(0, 0, 0, 0);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+      const char* p = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row + at) & ~uintptr_t(3));
+      const char* stop = at < end ? row + end : p;
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = p + 4 * i < stop ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
+    }
+  }
+  __device__ __forceinline__ void line_up(const char* row, int64_t at) {
+    if constexpr (!ALIGNED) {
+      const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + at) & 3) * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], shift);
+    }
+  }
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// four codes to four values, 16 bits each: a byte with its sign turned, in the last place of 2^23, is a number that 2^23 + 128 takes to the code
+template <bool BF16>
+__device__ __forceinline__ void values_of(uint32_t codes, float scale, uint32_t* lo, uint32_t* hi) {
+  const uint32_t u = codes ^ 0x80808080u;
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | i)) - 8388736.0f) * scale;
+  *lo = pack2<BF16>(v[0], v[1]);
+  *hi = pack2<BF16>(v[2], v[3]);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t w, float* lo, float* hi) {
+  if constexpr (BF16) {
+    *lo = __uint_as_float(w << 16);
+    *hi = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    *lo = f.x;
+    *hi = f.y;
+  }
+}
+
+template <bool BF16, bool G_ALIGNED, bool C_ALIGNED>
+__global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_constant__ KeptGradArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t smem = smem_addr(smem_raw), full = smem + BARS, empty = full + 8 * STAGES, done = empty + 8 * STAGES, summed = done + 8,
+                 tmem_word = summed + 8;
+  volatile int* dead = reinterpret_cast<volatile int*>(smem_raw + (tmem_word + 4 - smem));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      bar_init(full + 8 * i, FETCH_THREADS);
+      bar_init(empty + 8 * i, 1);
+    }
+    bar_init(done, 1);
+    bar_init(summed, FETCH_THREADS);
+    *dead = 0;
+    bar_init_fence();
+  }
+  if (warp == 0) tmem_alloc_one(tmem_word, 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_word) : "memory");
+  pdl_enter();
+  const int d0 = blockIdx.x * TILE, o0 = blockIdx.y * TILE, split = blockIdx.z;
+  const int64_t r0 = a.n * split / a.splits, r1 = a.n * (split + 1) / a.splits;
+  const int blocks = static_cast<int>((r1 - r0 + ROWS - 1) / ROWS);
+  const int cols = min(TILE, a.D - d0), outs = min(TILE, a.O - o0);
+  bool ok = true;
+
+  if (warp < FETCH_THREADS / 32) {
+    const char* g = static_cast<const char*>(a.grad) + static_cast<int64_t>(o0) * 2;
+    const char* c = reinterpret_cast<const char*>(a.codes) + d0;
+    const int g_chunk = threadIdx.x % G_CHUNKS, g_row = threadIdx.x / G_CHUNKS;  // (the same piece of every row of this thread)
+    const int c_chunk = threadIdx.x % C_CHUNKS, c_row = threadIdx.x / C_CHUNKS;
+    constexpr int G_STEP = FETCH_THREADS / G_CHUNKS, C_STEP = FETCH_THREADS / C_CHUNKS;
+    const int64_t g_pitch = a.grad_stride * 2, g_end = static_cast<int64_t>(outs) * 2, group = (d0 + c_chunk * 16) / KEPT_GROUP;
+    const bool g_in = g_chunk * 8 < outs, c_in = c_chunk * 16 < cols;
+    const bool sums = a.dbias != nullptr && blockIdx.x == 0;
+    float db[8] = {};
+    Piece<G_ALIGNED> gp[G_TASKS];
+    Piece<C_ALIGNED> cp[C_TASKS];
+    float scale[C_TASKS];
+    const auto fetch = [&](int64_t r) {
+#pragma unroll
+      for (int i = 0; i < G_TASKS; ++i) {
+        const int64_t row = r + g_row + i * G_STEP;
+        gp[i].fetch(g + row * g_pitch, g_chunk * 16, row < r1 && g_in ? g_end : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < C_TASKS; ++i) {
+        const int64_t row = r + c_row + i * C_STEP;
+        cp[i].fetch(c + row * a.codes_stride, c_chunk * 16, row < r1 && c_in ? cols : 0);
+        scale[i] = row < r1 && c_in ? __ldg(a.scales + row * a.groups + group) : 0.0f;
+      }
+    };
+    if (blocks > 0) fetch(r0);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int b = 0; b < blocks; ++b) {
+      const int64_t r = r0 + static_cast<int64_t>(b) * ROWS;
+      if (!(ok = !*dead && bar_wait(empty + 8 * slot, phase ^ 1))) break;
+      const uint32_t to_g = smem + slot * STAGE + (g_chunk / 8) * PANEL, to_c = smem + slot * STAGE + OPERAND + (c_chunk / 4) * PANEL;
+      if (g_in) {
+#pragma unroll
+        for (int i = 0; i < G_TASKS; ++i) {
+          const int row = g_row + i * G_STEP;
+          gp[i].line_up(g + (r + row) * g_pitch, g_chunk * 16);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to_g + row * 128 + (((g_chunk & 7) ^ (row & 7)) << 4)), "r"(gp[i].w[0]),
+                       "r"(gp[i].w[1]), "r"(gp[i].w[2]), "r"(gp[i].w[3])
+                       : "memory");
+          if (sums) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float lo, hi;
+              unpack2<BF16>(gp[i].w[e], &lo, &hi);
+              db[2 * e] += lo;
+              db[2 * e + 1] += hi;
+            }
+          }
+        }
+      }
+      if (c_in) {
+#pragma unroll
+        for (int i = 0; i < C_TASKS; ++i) {
+          const int row = c_row + i * C_STEP;
+          cp[i].line_up(c + (r + row) * a.codes_stride, c_chunk * 16);
+          uint32_t v[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) values_of<BF16>(cp[i].w[e], scale[i], &v[2 * e], &v[2 * e + 1]);
+          // neighbouring panels begin at the same banks: every second one stores its halves the other way round
+          const int turn = (c_chunk >> 2) & 1;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int half = h ^ turn;
+            const uint32_t to = to_c + row * 128 + ((((c_chunk & 3) * 2 + half) ^ (row & 7)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(half ? v[4] : v[0]), "r"(half ? v[5] : v[1]),
+                         "r"(half ? v[6] : v[2]), "r"(half ? v[7] : v[3])
+                         : "memory");
+          }
+        }
+      }
+      fence_async_smem();
+      bar_arrive(full + 8 * slot);
+      if (b + 1 < blocks) fetch(r + ROWS);
+      if (++slot == STAGES) slot = 0, phase ^= 1;
+    }
+    if (ok && blocks > 0) ok = !*dead && bar_wait(done, 0);
+    if (ok) {
+      // ---- results: a row of the weight a thread
+      fence_after();
+      const int o = warp / 4 * 128 + warp % 4 * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+      if (warp / 4 * 128 < outs) {
+#pragma unroll 1
+        for (int q = 0; q * 32 < cols; ++q) {
+          uint32_t v[32];
+          if (blocks > 0) {
+            tmem_load32(tmem + warp / 4 * 256 + q * 32 + lanes, v);
+            tmem_wait(v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0;
+          }
+          if (o >= outs) continue;
+          const int64_t at = static_cast<int64_t>(o0 + o) * a.D + d0 + q * 32;
+          const int left = cols - q * 32;
+          if (a.splits == 1) {
+            uint16_t* to = static_cast<uint16_t*>(a.dweight) + at;
+            if (left >= 32 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = pack2<BF16>(__uint_as_float(v[i * 8 + e * 2]), __uint_as_float(v[i * 8 + e * 2 + 1]));
+                reinterpret_cast<uint4*>(to)[i] = make_uint4(y[0], y[1], y[2], y[3]);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i < left) to[i] = static_cast<uint16_t>(pack2<BF16>(__uint_as_float(v[i]), 0.0f));
+            }
+          } else {
+            float* to = a.parts + static_cast<int64_t>(split) * a.O * a.D + at;
+            if (left >= 32 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i < left) to[i] = __uint_as_float(v[i]);
+            }
+          }
+        }
+      }
+      if (sums) {
+        // the threads that took the same columns, in their order (the tiles' memory is free)
+        float* part = reinterpret_cast<float*>(smem_raw);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[g_row * TILE + g_chunk * 8 + e] = db[e];
+        bar_arrive(summed);
+        ok = !*dead && bar_wait(summed, 0);
+        float s = 0.0f;
+#pragma unroll
+        for (int q = 0; q < G_STEP; ++q) s += part[q * TILE + threadIdx.x];
+        if (ok && static_cast<int>(threadIdx.x) < outs) {
+          if (a.splits > 1) a.bias_parts[static_cast<int64_t>(split) * a.O + o0 + threadIdx.x] = s;
+          else static_cast<uint16_t*>(a.dbias)[o0 + threadIdx.x] = static_cast<uint16_t>(pack2<BF16>(s, 0.0f));
+        }
+      }
+      fence_before();
+    }
+  } else if (lane == 0) {
+    // ---- products
+    const uint32_t n = static_cast<uint32_t>((cols + 15) / 16 * 16), idesc = mma_desc(BF16, true, true, 128, n);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int b = 0; b < blocks; ++b) {
+      if (!(ok = !*dead && bar_wait(full + 8 * slot, phase))) break;
+      fence_after();
+      const uint64_t da = smem_desc(smem + slot * STAGE, PANEL, 1024), dv = smem_desc(smem + slot * STAGE + OPERAND, PANEL, 1024);
+#pragma unroll
+      for (int k = 0; k < ROWS / 16; ++k) {
+        mma_one(tmem, da + k * (2048 >> 4), dv + k * (2048 >> 4), idesc, b > 0 || k > 0);
+        if (outs > 128) mma_one(tmem + 256, da + (2 * PANEL >> 4) + k * (2048 >> 4), dv + k * (2048 >> 4), idesc, b > 0 || k > 0);
+      }
+      mma_commit_one(empty + 8 * slot);
+      if (++slot == STAGES) slot = 0, phase ^= 1;
+    }
+    if (ok) mma_commit_one(done);
+  }
+  __syncwarp();
+  if (!ok) *dead = 1;
+  __syncthreads();
+  if (*dead) {
+    // (no status word here: an error leaves the results not a number)
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    if (threadIdx.x == 0) {
+      if (a.splits > 1) a.parts[static_cast<int64_t>(split) * a.O * a.D + static_cast<int64_t>(o0) * a.D + d0] = __uint_as_float(0x7fffffffu);
+      else static_cast<uint16_t*>(a.dweight)[static_cast<int64_t>(o0) * a.D + d0] = 0x7fffu;
+    }
+  }
+  if (warp == 0) {
+    fence_after();
+    tmem_free_one(tmem, 512);
+  }
+}
+
+template <bool BF16, bool G_ALIGNED, bool C_ALIGNED>
+int launch(const KeptGradArgs& a, cudaStream_t s) {
+  static_assert(SMEM <= 232448, "shared memory");
+  static std::atomic<bool> known[MAX_DEVICES] = {};
+  auto kernel = kept_mma_kernel<BF16, G_ALIGNED, C_ALIGNED>;
+  int dev = 0;
+  DGS_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= MAX_DEVICES || !known[dev].load(std::memory_order_relaxed)) {
+    DGS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM)));
+    if (dev < MAX_DEVICES) known[dev].store(true, std::memory_order_relaxed);
+  }
+  const dim3 grid(static_cast<unsigned>((a.D + TILE - 1) / TILE), static_cast<unsigned>((a.O + TILE - 1) / TILE), static_cast<unsigned>(a.splits));
+  DGS_CUDA_TRY(launch_training(kernel, grid, THREADS, SMEM, s, a));
+  return DGS_OK;
+}
+template <bool BF16>
+int launch_aligned(const KeptGradArgs& a, cudaStream_t s) {
+  const bool g = a.grad_stride % 8 == 0 && a.O % 8 == 0 && aligned_to(a.grad, 16);
+  const bool c = a.codes_stride % 16 == 0 && a.D % 16 == 0 && aligned_to(a.codes, 16);
+  return g ? (c ? launch<BF16, true, true>(a, s) : launch<BF16, true, false>(a, s))
+           : (c ? launch<BF16, false, true>(a, s) : launch<BF16, false, false>(a, s));
+}
+
+}  // namespace
+
+// Shares of the rows: what a share takes (rows at a tile's 16 cycles each, in as many rounds of CTAs as there are) against writing and
+// adding one more (8 bytes a result): both in units of a row of a tile, some 9.4 ns; 4 TB/s.
+int64_t kept_mma_shares(int64_t n, int64_t O, int64_t D) {
+  const int64_t tiles = ((O + TILE - 1) / TILE) * ((D + TILE - 1) / TILE), sms = sm_count();
+  int64_t most = (n + 8 * ROWS - 1) / (8 * ROWS), best = 1;
+  if (most > sms) most = sms;
+  double least = 0.0;
+  for (int64_t s = 1; s <= most; ++s) {
+    const double rounds = static_cast<double>((tiles * s + sms - 1) / sms);
+    const double cost = rounds * static_cast<double>(n) / static_cast<double>(s) + (s > 1 ? static_cast<double>(s) * O * D * 8.0 / 4e12 / 9.4e-9 : 0.0);
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+int kept_mma_weight_grad(const KeptGradArgs& a, int32_t dtype, cudaStream_t s) {
+  return dtype == DGS_BF16 ? launch_aligned<true>(a, s) : launch_aligned<false>(a, s);
+}
+
+}  // namespace dgs
