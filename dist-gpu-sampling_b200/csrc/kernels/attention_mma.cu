@@ -40,15 +40,6 @@ constexpr uint32_t tile_bytes() {
 }
 constexpr uint32_t PANEL = ATTN_TILE * 128;  // 128 rows of 64 elements
 
-template <int N>
-__device__ __forceinline__ void more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

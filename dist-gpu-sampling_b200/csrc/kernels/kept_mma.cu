@@ -13,11 +13,13 @@ namespace dgs {
 namespace {
 using namespace tc;
 
-constexpr int TILE = 256, ROWS = 64, FETCH_THREADS = 256, THREADS = FETCH_THREADS + 32, STAGES = 3;
+constexpr int TILE = 256, ROWS = 64, FETCH_THREADS = 256, THREADS = FETCH_THREADS + 128, STAGES = 3;
+// Registers: 3 x 128 x 168 at the launch; the two warpgroups that fetch take what the products' one leaves
+constexpr int MANY_REGISTERS = 216, FEW_REGISTERS = 72;
 constexpr uint32_t PANEL = ROWS * 128;                 // 64 columns of 64 rows
 constexpr uint32_t OPERAND = TILE / 64 * PANEL, STAGE = 2 * OPERAND;
 constexpr uint32_t BARS = STAGES * STAGE, SMEM = BARS + 128;
-constexpr int G_CHUNKS = TILE / 8, G_TASKS = ROWS * G_CHUNKS / FETCH_THREADS;   // 16-byte pieces of g's rows, a thread's
+constexpr int NARROW = 64;  // results a row of the weight: up to here two of a row's pieces a thread instead of eight, and a block more on its way
 constexpr int C_CHUNKS = TILE / 16, C_TASKS = ROWS * C_CHUNKS / FETCH_THREADS;  // 16 codes
 constexpr int MAX_DEVICES = 64;
 
@@ -57,9 +59,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 template <bool BF16>
 __device__ __forceinline__ void values_of(uint32_t codes, float scale, uint32_t* lo, uint32_t* hi) {
   const uint32_t u = codes ^ 0x80808080u;
+  const uint64_t less = two(-8388736.0f, -8388736.0f), by = two(scale, scale);
+  const auto number = [&](int i) { return __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | i)); };
   float v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | i)) - 8388736.0f) * scale;
+  split2(mul2(add2(two(number(0), number(1)), less), by), &v[0], &v[1]);
+  split2(mul2(add2(two(number(2), number(3)), less), by), &v[2], &v[3]);
   *lo = pack2<BF16>(v[0], v[1]);
   *hi = pack2<BF16>(v[2], v[3]);
 }
@@ -76,9 +80,19 @@ __device__ __forceinline__ void unpack2(uint32_t w, float* lo, float* hi) {
   }
 }
 
-template <bool BF16, bool G_ALIGNED, bool C_ALIGNED>
+// A thread's share of 64 rows on their way: the same pieces of some rows of g, 16 codes and their scale of others
+template <bool G_ALIGNED, bool C_ALIGNED, int G_TASKS>
+struct Block {
+  Piece<G_ALIGNED> g[G_TASKS];
+  Piece<C_ALIGNED> c[C_TASKS];
+  float scale[C_TASKS];
+};
+
+template <bool BF16, bool G_ALIGNED, bool C_ALIGNED, bool FEW>
 __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_constant__ KeptGradArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
+  constexpr int G_CHUNKS = (FEW ? NARROW : TILE) / 8, G_TASKS = ROWS * G_CHUNKS / FETCH_THREADS;  // 16-byte pieces of g's rows
+  constexpr int DEPTH = FEW ? 3 : 2;                                                              // blocks of rows on their way
   const uint32_t smem = smem_addr(smem_raw), full = smem + BARS, empty = full + 8 * STAGES, done = empty + 8 * STAGES, summed = done + 8,
                  tmem_word = summed + 8;
   volatile int* dead = reinterpret_cast<volatile int*>(smem_raw + (tmem_word + 4 - smem));
@@ -107,6 +121,7 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
   bool ok = true;
 
   if (warp < FETCH_THREADS / 32) {
+    more_registers<MANY_REGISTERS>();
     const char* g = static_cast<const char*>(a.grad) + static_cast<int64_t>(o0) * 2;
     const char* c = reinterpret_cast<const char*>(a.codes) + d0;
     const int g_chunk = threadIdx.x % G_CHUNKS, g_row = threadIdx.x / G_CHUNKS;  // (the same piece of every row of this thread)
@@ -116,42 +131,37 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
     const bool g_in = g_chunk * 8 < outs, c_in = c_chunk * 16 < cols;
     const bool sums = a.dbias != nullptr && blockIdx.x == 0;
     float db[8] = {};
-    Piece<G_ALIGNED> gp[G_TASKS];
-    Piece<C_ALIGNED> cp[C_TASKS];
-    float scale[C_TASKS];
-    const auto fetch = [&](int64_t r) {
+    Block<G_ALIGNED, C_ALIGNED, G_TASKS> on_way[DEPTH];
+    const auto fetch = [&](Block<G_ALIGNED, C_ALIGNED, G_TASKS>& x, int64_t r) {
 #pragma unroll
       for (int i = 0; i < G_TASKS; ++i) {
         const int64_t row = r + g_row + i * G_STEP;
-        gp[i].fetch(g + row * g_pitch, g_chunk * 16, row < r1 && g_in ? g_end : 0);
+        x.g[i].fetch(g + row * g_pitch, g_chunk * 16, row < r1 && g_in ? g_end : 0);
       }
 #pragma unroll
       for (int i = 0; i < C_TASKS; ++i) {
         const int64_t row = r + c_row + i * C_STEP;
-        cp[i].fetch(c + row * a.codes_stride, c_chunk * 16, row < r1 && c_in ? cols : 0);
-        scale[i] = row < r1 && c_in ? __ldg(a.scales + row * a.groups + group) : 0.0f;
+        x.c[i].fetch(c + row * a.codes_stride, c_chunk * 16, row < r1 && c_in ? cols : 0);
+        x.scale[i] = row < r1 && c_in ? __ldg(a.scales + row * a.groups + group) : 0.0f;
       }
     };
-    if (blocks > 0) fetch(r0);
     int slot = 0;
     uint32_t phase = 0;
-    for (int b = 0; b < blocks; ++b) {
-      const int64_t r = r0 + static_cast<int64_t>(b) * ROWS;
-      if (!(ok = !*dead && bar_wait(empty + 8 * slot, phase ^ 1))) break;
+    const auto store = [&](Block<G_ALIGNED, C_ALIGNED, G_TASKS>& x, int64_t r) {
       const uint32_t to_g = smem + slot * STAGE + (g_chunk / 8) * PANEL, to_c = smem + slot * STAGE + OPERAND + (c_chunk / 4) * PANEL;
       if (g_in) {
 #pragma unroll
         for (int i = 0; i < G_TASKS; ++i) {
           const int row = g_row + i * G_STEP;
-          gp[i].line_up(g + (r + row) * g_pitch, g_chunk * 16);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to_g + row * 128 + (((g_chunk & 7) ^ (row & 7)) << 4)), "r"(gp[i].w[0]),
-                       "r"(gp[i].w[1]), "r"(gp[i].w[2]), "r"(gp[i].w[3])
+          x.g[i].line_up(g + (r + row) * g_pitch, g_chunk * 16);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to_g + row * 128 + (((g_chunk & 7) ^ (row & 7)) << 4)), "r"(x.g[i].w[0]),
+                       "r"(x.g[i].w[1]), "r"(x.g[i].w[2]), "r"(x.g[i].w[3])
                        : "memory");
           if (sums) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float lo, hi;
-              unpack2<BF16>(gp[i].w[e], &lo, &hi);
+              unpack2<BF16>(x.g[i].w[e], &lo, &hi);
               db[2 * e] += lo;
               db[2 * e + 1] += hi;
             }
@@ -162,10 +172,10 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < C_TASKS; ++i) {
           const int row = c_row + i * C_STEP;
-          cp[i].line_up(c + (r + row) * a.codes_stride, c_chunk * 16);
+          x.c[i].line_up(c + (r + row) * a.codes_stride, c_chunk * 16);
           uint32_t v[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) values_of<BF16>(cp[i].w[e], scale[i], &v[2 * e], &v[2 * e + 1]);
+          for (int e = 0; e < 4; ++e) values_of<BF16>(x.c[i].w[e], x.scale[i], &v[2 * e], &v[2 * e + 1]);
           // neighbouring panels begin at the same banks: every second one stores its halves the other way round
           const int turn = (c_chunk >> 2) & 1;
 #pragma unroll
@@ -178,10 +188,21 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
           }
         }
       }
-      fence_async_smem();
-      bar_arrive(full + 8 * slot);
-      if (b + 1 < blocks) fetch(r + ROWS);
-      if (++slot == STAGES) slot = 0, phase ^= 1;
+    };
+#pragma unroll
+    for (int w = 0; w < DEPTH; ++w) fetch(on_way[w], r0 + w * ROWS);  // (rows behind the share are not read)
+    for (int b0 = 0; ok && b0 < blocks; b0 += DEPTH) {
+#pragma unroll
+      for (int w = 0; w < DEPTH; ++w) {
+        if (!ok || b0 + w >= blocks) continue;
+        const int64_t r = r0 + static_cast<int64_t>(b0 + w) * ROWS;
+        if (!(ok = !*dead && bar_wait(empty + 8 * slot, phase ^ 1))) continue;
+        store(on_way[w], r);
+        fence_async_smem();
+        bar_arrive(full + 8 * slot);
+        fetch(on_way[w], r + DEPTH * ROWS);
+        if (++slot == STAGES) slot = 0, phase ^= 1;
+      }
     }
     if (ok && blocks > 0) ok = !*dead && bar_wait(done, 0);
     if (ok) {
@@ -235,37 +256,40 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
         // the threads that took the same columns, in their order (the tiles' memory is free)
         float* part = reinterpret_cast<float*>(smem_raw);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) part[g_row * TILE + g_chunk * 8 + e] = db[e];
+        for (int e = 0; e < 8; ++e) part[g_row * G_CHUNKS * 8 + g_chunk * 8 + e] = db[e];
         bar_arrive(summed);
         ok = !*dead && bar_wait(summed, 0);
-        float s = 0.0f;
-#pragma unroll
-        for (int q = 0; q < G_STEP; ++q) s += part[q * TILE + threadIdx.x];
         if (ok && static_cast<int>(threadIdx.x) < outs) {
+          float s = 0.0f;
+#pragma unroll 8
+          for (int q = 0; q < G_STEP; ++q) s += part[q * G_CHUNKS * 8 + threadIdx.x];
           if (a.splits > 1) a.bias_parts[static_cast<int64_t>(split) * a.O + o0 + threadIdx.x] = s;
           else static_cast<uint16_t*>(a.dbias)[o0 + threadIdx.x] = static_cast<uint16_t>(pack2<BF16>(s, 0.0f));
         }
       }
       fence_before();
     }
-  } else if (lane == 0) {
-    // ---- products
-    const uint32_t n = static_cast<uint32_t>((cols + 15) / 16 * 16), idesc = mma_desc(BF16, true, true, 128, n);
-    int slot = 0;
-    uint32_t phase = 0;
-    for (int b = 0; b < blocks; ++b) {
-      if (!(ok = !*dead && bar_wait(full + 8 * slot, phase))) break;
-      fence_after();
-      const uint64_t da = smem_desc(smem + slot * STAGE, PANEL, 1024), dv = smem_desc(smem + slot * STAGE + OPERAND, PANEL, 1024);
+  } else {
+    fewer_registers<FEW_REGISTERS>();
+    if (warp == FETCH_THREADS / 32 && lane == 0) {
+      // ---- products
+      const uint32_t n = static_cast<uint32_t>((cols + 15) / 16 * 16), idesc = mma_desc(BF16, true, true, 128, n);
+      int slot = 0;
+      uint32_t phase = 0;
+      for (int b = 0; b < blocks; ++b) {
+        if (!(ok = !*dead && bar_wait(full + 8 * slot, phase))) break;
+        fence_after();
+        const uint64_t da = smem_desc(smem + slot * STAGE, PANEL, 1024), dv = smem_desc(smem + slot * STAGE + OPERAND, PANEL, 1024);
 #pragma unroll
-      for (int k = 0; k < ROWS / 16; ++k) {
-        mma_one(tmem, da + k * (2048 >> 4), dv + k * (2048 >> 4), idesc, b > 0 || k > 0);
-        if (outs > 128) mma_one(tmem + 256, da + (2 * PANEL >> 4) + k * (2048 >> 4), dv + k * (2048 >> 4), idesc, b > 0 || k > 0);
+        for (int k = 0; k < ROWS / 16; ++k) {
+          mma_one(tmem, da + k * (2048 >> 4), dv + k * (2048 >> 4), idesc, b > 0 || k > 0);
+          if (outs > 128) mma_one(tmem + 256, da + (2 * PANEL >> 4) + k * (2048 >> 4), dv + k * (2048 >> 4), idesc, b > 0 || k > 0);
+        }
+        mma_commit_one(empty + 8 * slot);
+        if (++slot == STAGES) slot = 0, phase ^= 1;
       }
-      mma_commit_one(empty + 8 * slot);
-      if (++slot == STAGES) slot = 0, phase ^= 1;
+      if (ok) mma_commit_one(done);
     }
-    if (ok) mma_commit_one(done);
   }
   __syncwarp();
   if (!ok) *dead = 1;
@@ -284,11 +308,11 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
   }
 }
 
-template <bool BF16, bool G_ALIGNED, bool C_ALIGNED>
+template <bool BF16, bool G_ALIGNED, bool C_ALIGNED, bool FEW>
 int launch(const KeptGradArgs& a, cudaStream_t s) {
   static_assert(SMEM <= 232448, "shared memory");
   static std::atomic<bool> known[MAX_DEVICES] = {};
-  auto kernel = kept_mma_kernel<BF16, G_ALIGNED, C_ALIGNED>;
+  auto kernel = kept_mma_kernel<BF16, G_ALIGNED, C_ALIGNED, FEW>;
   int dev = 0;
   DGS_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= MAX_DEVICES || !known[dev].load(std::memory_order_relaxed)) {
@@ -303,8 +327,11 @@ template <bool BF16>
 int launch_aligned(const KeptGradArgs& a, cudaStream_t s) {
   const bool g = a.grad_stride % 8 == 0 && a.O % 8 == 0 && aligned_to(a.grad, 16);
   const bool c = a.codes_stride % 16 == 0 && a.D % 16 == 0 && aligned_to(a.codes, 16);
-  return g ? (c ? launch<BF16, true, true>(a, s) : launch<BF16, true, false>(a, s))
-           : (c ? launch<BF16, false, true>(a, s) : launch<BF16, false, false>(a, s));
+  if (a.O <= NARROW)
+    return g ? (c ? launch<BF16, true, true, true>(a, s) : launch<BF16, true, false, true>(a, s))
+             : (c ? launch<BF16, false, true, true>(a, s) : launch<BF16, false, false, true>(a, s));
+  return g ? (c ? launch<BF16, true, true, false>(a, s) : launch<BF16, true, false, false>(a, s))
+           : (c ? launch<BF16, false, true, false>(a, s) : launch<BF16, false, false, false>(a, s));
 }
 
 }  // namespace

@@ -31,6 +31,16 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
   return r;
 }
 
+// ---- registers of a warpgroup: what the block was launched with, shared out anew -----------------------------------------
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // ---- mbarriers ----------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
