@@ -39,65 +39,105 @@ __device__ __forceinline__ void row_and_group(const KeepArgs& a, int64_t task, i
   }
 }
 
-// LANES lanes hold a group, VEC adjacent elements each (VEC == 1: KEPT_GROUP / 32 elements 32 apart).  A value that is not finite makes the
-// scale one that is not: magnitudes are compared as words, where nan is above infinity.
+// Magnitudes are compared as words, where nan is above infinity: a value that is not finite makes the scale one that is not.
+template <typename T>
+__device__ __forceinline__ uint32_t largest_word(uint32_t top, uint32_t w);  // w: one value of 32 bits or two of 16
+template <>
+__device__ __forceinline__ uint32_t largest_word<float>(uint32_t top, uint32_t w) {
+  return max(top, w & 0x7fffffffu);
+}
+template <>
+__device__ __forceinline__ uint32_t largest_word<__nv_bfloat16>(uint32_t top, uint32_t w) {
+  return __vmaxu2(top, w & 0x7fff7fffu);
+}
+template <>
+__device__ __forceinline__ uint32_t largest_word<__half>(uint32_t top, uint32_t w) {
+  return __vmaxu2(top, w & 0x7fff7fffu);
+}
+template <typename T>
+__device__ __forceinline__ float largest_value(uint32_t top) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(top);
+  const uint16_t one = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+  return to_float<T>(*reinterpret_cast<const T*>(&one));
+}
+
+constexpr float ROUND = 12582912.0f;  // 1.5 * 2^23: a number of up to 2^22 added to it is rounded to a whole one, in the last bits of the sum
+// the code of x: the product rounded to 32 bits, then to the nearest whole number (ties to the even one)
+__device__ __forceinline__ uint32_t code_of(float x, float by) { return __float_as_uint(__fadd_rn(__fmul_rn(x, by), ROUND)); }
+
+// Codes of VEC adjacent values a lane (VEC == 1: four that are 32 apart), a group of 128 in LANES lanes.
 template <typename T, int VEC>
 __global__ __launch_bounds__(KEEP_THREADS) void keep_kernel(const __grid_constant__ KeepArgs a) {
   constexpr int LANES = VEC == 1 ? 32 : KEPT_GROUP / VEC, E = VEC == 1 ? KEPT_GROUP / 32 : VEC, APART = VEC == 1 ? 32 : 1;
-  constexpr int PER_CTA = KEEP_THREADS / LANES;
+  constexpr int PER_CTA = KEEP_THREADS / LANES, WORDS = E * static_cast<int>(sizeof(T)) / 4;
   pdl_enter();
   const int lane = threadIdx.x % LANES, first = VEC == 1 ? lane : lane * VEC;
   const int64_t step = static_cast<int64_t>(gridDim.x) * PER_CTA;
   for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * PER_CTA + threadIdx.x / LANES; t0 - threadIdx.x / LANES < a.tasks; t0 += step * KEEP_UNROLL) {
-    float x[KEEP_UNROLL][E];
+    union Held {
+      T v[E];
+      uint32_t w[WORDS];
+      __device__ Held() {}
+    } x[KEEP_UNROLL];
     int64_t row[KEEP_UNROLL];
-    int group[KEEP_UNROLL];
+    int at[KEEP_UNROLL], group[KEEP_UNROLL];
 #pragma unroll
     for (int u = 0; u < KEEP_UNROLL; ++u) {
       const int64_t t = t0 + u * step;
       row_and_group(a, t < a.tasks ? t : 0, &row[u], &group[u]);
-      const int c = group[u] * KEPT_GROUP + first;
-      const T* p = static_cast<const T*>(a.x) + row[u] * a.x_stride + c;
+      at[u] = t < a.tasks ? group[u] * KEPT_GROUP + first : a.D;
+      const T* p = static_cast<const T*>(a.x) + row[u] * a.x_stride + at[u];
       if constexpr (VEC == 1) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[u][e] = t < a.tasks && c + e * APART < a.D ? to_float<T>(p[e * APART]) : 0.0f;
-      } else if (t < a.tasks && c < a.D) {
-        load_vec<T, VEC>(p, x[u]);
+        for (int e = 0; e < E; ++e) x[u].v[e] = at[u] + e * APART < a.D ? p[e * APART] : from_float<T>(0.0f);
       } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[u][e] = 0.0f;
+        const Vec<T, VEC> none{};
+        *reinterpret_cast<Vec<T, VEC>*>(x[u].v) = at[u] < a.D ? *reinterpret_cast<const Vec<T, VEC>*>(p) : none;
       }
     }
 #pragma unroll
     for (int u = 0; u < KEEP_UNROLL; ++u) {
-      const int64_t t = t0 + u * step;
       uint32_t top = 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[u][e]) & 0x7fffffffu);
+      for (int i = 0; i < WORDS; ++i) top = largest_word<T>(top, x[u].w[i]);
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(FULL_MASK, top, o));
-      if (t >= a.tasks) continue;
-      const float big = __uint_as_float(top), by = big > 0.0f ? 127.0f / big : 0.0f;
-      int8_t c[E];
+      for (int o = LANES / 2; o > 0; o >>= 1) top = largest_word<T>(top, __shfl_xor_sync(FULL_MASK, top, o));
+      const float big = largest_value<T>(top);
+      float by = big > 0.0f ? 127.0f / big : 0.0f;
+      if (!(big - big == 0.0f)) by = 0.0f;  // (nothing of such a group is kept)
+      uint32_t c[E];
+      if (by - by == 0.0f) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) c[e] = static_cast<int8_t>(max(-127, min(127, __float2int_rn(x[u][e] * by))));
-      const int at = group[u] * KEPT_GROUP + first;
-      int8_t* to = a.codes + row[u] * a.D + at;
+        for (int e = 0; e < E; ++e) c[e] = code_of(to_float<T>(x[u].v[e]), by);
+        if (!(big - big == 0.0f)) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) c[e] = 0;
+        }
+      } else {  // 127 / a is no finite number
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float v = to_float<T>(x[u].v[e]);
+          c[e] = v > 0.0f ? 127u : v < 0.0f ? static_cast<uint32_t>(-127) : 0u;
+        }
+      }
+      int8_t* to = a.codes + row[u] * a.D + at[u];
       if constexpr (VEC == 1) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (at + e * APART < a.D) to[e * APART] = c[e];
-      } else if (at < a.D) {
-        Vec<int8_t, VEC> v;
+          if (at[u] + e * APART < a.D) to[e * APART] = static_cast<int8_t>(c[e]);
+      } else if (at[u] < a.D) {
+        uint32_t w[VEC / 4];
 #pragma unroll
-        for (int e = 0; e < E; ++e) v.v[e] = c[e];
-        *reinterpret_cast<Vec<int8_t, VEC>*>(to) = v;
+        for (int i = 0; i < VEC / 4; ++i)
+          w[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
+        *reinterpret_cast<Vec<uint32_t, VEC / 4>*>(to) = *reinterpret_cast<Vec<uint32_t, VEC / 4>*>(w);
       }
-      if (lane == 0) a.scales[row[u] * a.groups + group[u]] = big / 127.0f;
+      if (lane == 0 && at[u] < a.D) a.scales[row[u] * a.groups + group[u]] = big / 127.0f;
     }
   }
 }
 
+// E codes a lane, adjacent (VEC > 1) or 32 apart
 template <typename T, int VEC>
 __global__ __launch_bounds__(KEEP_THREADS) void kept_values_kernel(const __grid_constant__ KeepArgs a) {
   constexpr int LANES = VEC == 1 ? 32 : KEPT_GROUP / VEC, E = VEC == 1 ? KEPT_GROUP / 32 : VEC, APART = VEC == 1 ? 32 : 1;
@@ -106,7 +146,11 @@ __global__ __launch_bounds__(KEEP_THREADS) void kept_values_kernel(const __grid_
   const int lane = threadIdx.x % LANES, first = VEC == 1 ? lane : lane * VEC;
   const int64_t step = static_cast<int64_t>(gridDim.x) * PER_CTA;
   for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * PER_CTA + threadIdx.x / LANES; t0 < a.tasks; t0 += step * KEEP_UNROLL) {
-    Vec<int8_t, E> c[KEEP_UNROLL];
+    union Held {
+      int8_t v[E];
+      uint32_t w[E / 4];
+      __device__ Held() {}
+    } c[KEEP_UNROLL];
     float scale[KEEP_UNROLL];
     int64_t row[KEEP_UNROLL];
     int at[KEEP_UNROLL];
@@ -120,23 +164,36 @@ __global__ __launch_bounds__(KEEP_THREADS) void kept_values_kernel(const __grid_
       if constexpr (VEC == 1) {
 #pragma unroll
         for (int e = 0; e < E; ++e) c[u].v[e] = at[u] + e * APART < a.D ? p[e * APART] : 0;
-      } else {
-        c[u] = at[u] < a.D ? *reinterpret_cast<const Vec<int8_t, E>*>(p) : Vec<int8_t, E>{};
+      } else if (at[u] < a.D) {
+        *reinterpret_cast<Vec<uint32_t, E / 4>*>(c[u].w) = *reinterpret_cast<const Vec<uint32_t, E / 4>*>(p);
       }
-      scale[u] = at[u] < a.D ? a.scales_in[row[u] * a.groups + group] : 0.0f;
+      scale[u] = at[u] < a.D ? __ldg(a.scales_in + row[u] * a.groups + group) : 0.0f;
     }
 #pragma unroll
     for (int u = 0; u < KEEP_UNROLL; ++u) {
+      if (at[u] >= a.D) continue;
       T* to = static_cast<T*>(a.out) + row[u] * a.D + at[u];
       float v[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = static_cast<float>(c[u].v[e]) * scale[u];
+      for (int i = 0; i < E / 4; ++i) {
+        // a byte with its sign turned in the last place of 2^23
+        const uint32_t w = c[u].w[i] ^ 0x80808080u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * i + e] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | e)) - 8388736.0f) * scale[u];
+      }
       if constexpr (VEC == 1) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (at[u] + e * APART < a.D) to[e * APART] = from_float<T>(v[e]);
-      } else if (at[u] < a.D) {
-        store_vec<T, VEC>(to, v);
+      } else {
+        constexpr int PIECE = VEC * sizeof(T) > 16 ? 16 / static_cast<int>(sizeof(T)) : VEC;
+#pragma unroll
+        for (int i = 0; i < VEC / PIECE; ++i) {
+          float part[PIECE];
+#pragma unroll
+          for (int e = 0; e < PIECE; ++e) part[e] = v[i * PIECE + e];
+          store_vec<T, PIECE>(to + i * PIECE, part);
+        }
       }
     }
   }
@@ -148,23 +205,34 @@ unsigned keep_ctas(int64_t tasks, int lanes) {
   return static_cast<unsigned>(need < most ? need : most);
 }
 
+// whether rows of both sides can be moved VEC elements at a time
+template <typename T, int VEC>
+bool by_vectors(const KeepArgs& a, const void* x, int64_t x_stride, const void* codes, int64_t codes_stride) {
+  constexpr size_t bytes = VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16;
+  return a.D % VEC == 0 && (x_stride % VEC == 0 || a.n <= 1) && (codes_stride % VEC == 0 || a.n <= 1) && aligned_to(x, bytes) && aligned_to(codes, VEC);
+}
+template <typename T, int VEC>
+int keep_by(const KeepArgs& a, cudaStream_t s) {
+  DGS_CUDA_TRY(launch_training(keep_kernel<T, VEC>, dim3(keep_ctas(a.tasks, VEC == 1 ? 32 : KEPT_GROUP / VEC)), KEEP_THREADS, 0, s, a));
+  return DGS_OK;
+}
 template <typename T>
 int keep(const KeepArgs& a, cudaStream_t s) {
   constexpr int VEC = 16 / sizeof(T);
-  if (a.D % VEC == 0 && (a.x_stride % VEC == 0 || a.n <= 1) && aligned_to(a.x, 16) && aligned_to(a.codes, VEC))
-    DGS_CUDA_TRY(launch_training(keep_kernel<T, VEC>, dim3(keep_ctas(a.tasks, KEPT_GROUP / VEC)), KEEP_THREADS, 0, s, a));
-  else
-    DGS_CUDA_TRY(launch_training(keep_kernel<T, 1>, dim3(keep_ctas(a.tasks, 32)), KEEP_THREADS, 0, s, a));
+  if (by_vectors<T, VEC>(a, a.x, a.x_stride, a.codes, a.D)) return keep_by<T, VEC>(a, s);
+  if (VEC > 4 && by_vectors<T, 4>(a, a.x, a.x_stride, a.codes, a.D)) return keep_by<T, 4>(a, s);
+  return keep_by<T, 1>(a, s);
+}
+template <typename T, int VEC>
+int values_by(const KeepArgs& a, cudaStream_t s) {
+  DGS_CUDA_TRY(launch_training(kept_values_kernel<T, VEC>, dim3(keep_ctas(a.tasks, VEC == 1 ? 32 : KEPT_GROUP / VEC)), KEEP_THREADS, 0, s, a));
   return DGS_OK;
 }
 template <typename T>
 int values(const KeepArgs& a, cudaStream_t s) {
-  constexpr int VEC = 16 / sizeof(T);
-  if (a.D % VEC == 0 && (a.codes_stride % VEC == 0 || a.n <= 1) && aligned_to(a.out, 16) && aligned_to(a.codes_in, VEC))
-    DGS_CUDA_TRY(launch_training(kept_values_kernel<T, VEC>, dim3(keep_ctas(a.tasks, KEPT_GROUP / VEC)), KEEP_THREADS, 0, s, a));
-  else
-    DGS_CUDA_TRY(launch_training(kept_values_kernel<T, 1>, dim3(keep_ctas(a.tasks, 32)), KEEP_THREADS, 0, s, a));
-  return DGS_OK;
+  if (by_vectors<T, 16>(a, a.out, a.D, a.codes_in, a.codes_stride)) return values_by<T, 16>(a, s);
+  if (by_vectors<T, 4>(a, a.out, a.D, a.codes_in, a.codes_stride)) return values_by<T, 4>(a, s);
+  return values_by<T, 1>(a, s);
 }
 
 // ---- the weight's gradient of 32-bit operands, on the CUDA cores ------------------------------------------------------------------------------
@@ -210,24 +278,40 @@ __global__ __launch_bounds__(WG_THREADS) void kept_grad_kernel(const __grid_cons
   if (d0 == 0 && threadIdx.x < WG_TILE && o0 + threadIdx.x < a.O) a.bias_parts[static_cast<int64_t>(split) * a.O + o0 + threadIdx.x] = db;
 }
 
-// shares added in their order
-template <typename T>
+// Shares added in a fixed order: WAYS warps take every WAYS-th share of the same 32 results (or 128: VEC of them a lane), then one adds theirs
+template <typename T, int WAYS, int VEC>
 __global__ __launch_bounds__(KEEP_THREADS) void kept_join_kernel(const __grid_constant__ KeptGradArgs a) {
+  __shared__ float part[KEEP_THREADS / 32][32][VEC];
   pdl_enter();
-  const int64_t all = static_cast<int64_t>(a.O) * a.D, step = static_cast<int64_t>(gridDim.x) * KEEP_THREADS;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * KEEP_THREADS + threadIdx.x; i < all; i += step) {
-    float s = 0.0f;
-#pragma unroll 8
-    for (int p = 0; p < a.splits; ++p) s += a.parts[p * all + i];
-    static_cast<T*>(a.dweight)[i] = from_float<T>(s);
-  }
-  if (a.dbias != nullptr)
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * KEEP_THREADS + threadIdx.x; i < a.O; i += step) {
-      float s = 0.0f;
-#pragma unroll 8
-      for (int p = 0; p < a.splits; ++p) s += a.bias_parts[static_cast<int64_t>(p) * a.O + i];
-      static_cast<T*>(a.dbias)[i] = from_float<T>(s);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, way = warp % WAYS;
+  constexpr int ALONG = KEEP_THREADS / 32 / WAYS;  // sets of results a CTA
+  const int64_t all = static_cast<int64_t>(a.O) * a.D, both = all + (a.dbias != nullptr ? a.O : 0);
+  const int64_t i = ((static_cast<int64_t>(blockIdx.x) * ALONG + warp / WAYS) * 32 + lane) * VEC;
+  float s[VEC] = {};
+  // (with VEC > 1 all and O are multiples of it)
+  const float* from = i < all ? a.parts + i : a.bias_parts + (i - all);
+  const int64_t apart = i < all ? all : a.O;
+  if (i < both) {
+#pragma unroll 4
+    for (int p = way; p < a.splits; p += WAYS) {
+      float x[VEC];
+      load_vec<float, VEC>(from + p * apart, x);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[e] += x[e];
     }
+  }
+  if constexpr (WAYS > 1) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) part[warp][lane][e] = s[e];
+    __syncthreads();
+    if (way != 0) return;
+#pragma unroll
+    for (int w = 1; w < WAYS; ++w)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[e] += part[warp + w][lane][e];
+  }
+  if (i < all) store_vec<T, VEC>(static_cast<T*>(a.dweight) + i, s);
+  else if (i < both) store_vec<T, VEC>(static_cast<T*>(a.dbias) + (i - all), s);
 }
 
 // Shares of the rows: enough CTAs for four on each SM, shares of 256 rows at least
@@ -240,11 +324,17 @@ int64_t shares(int64_t n, int64_t O, int64_t D, int32_t dtype) {
   return want < 1 ? 1 : want;
 }
 
+template <typename T, int WAYS, int VEC>
+int join_by(const KeptGradArgs& a, cudaStream_t s) {
+  const int64_t both = static_cast<int64_t>(a.O) * a.D + (a.dbias != nullptr ? a.O : 0), per = KEEP_THREADS / WAYS * VEC;
+  DGS_CUDA_TRY(launch_training(kept_join_kernel<T, WAYS, VEC>, dim3(static_cast<unsigned>((both + per - 1) / per)), KEEP_THREADS, 0, s, a));
+  return DGS_OK;
+}
 template <typename T>
 int join(const KeptGradArgs& a, cudaStream_t s) {
-  const int64_t need = (static_cast<int64_t>(a.O) * a.D + KEEP_THREADS - 1) / KEEP_THREADS, most = static_cast<int64_t>(sm_count()) * 8;
-  DGS_CUDA_TRY(launch_training(kept_join_kernel<T>, dim3(static_cast<unsigned>(need < most ? need : most)), KEEP_THREADS, 0, s, a));
-  return DGS_OK;
+  const bool wide = (static_cast<int64_t>(a.O) * a.D) % 4 == 0 && (a.dbias == nullptr || a.O % 4 == 0) && aligned_to(a.dweight, 16) && aligned_to(a.dbias, 16);
+  if (a.splits > 8) return wide ? join_by<T, 8, 4>(a, s) : join_by<T, 8, 1>(a, s);
+  return wide ? join_by<T, 1, 4>(a, s) : join_by<T, 1, 1>(a, s);
 }
 
 int weight_grad(const KeptGradArgs& a, int32_t dtype, cudaStream_t s) {

@@ -1,9 +1,9 @@
 // The gradient of a linear layer's weight from rows kept in 8 bits, 16-bit gradients, on the tensor cores:
 //   dW[o, d] = sum_n g[n, o] v[n, d],  v = code * scale rounded to g's type (so that products are exact; sums are in 32 bits)
 //
-// A CTA takes 256 x 256 results over a share of the rows, 64 at a time: eight warps fetch rows of g and codes, turn the codes into
-// values and leave both in shared memory as they lie (the sum's index outermost: MN-major tiles), one thread issues the products
-// (cta_group::1, two accumulators of 128 x 256 in TMEM).  The rows' next 64 are fetched into registers while these are stored.
+// A CTA takes 256 x 256 results over a share of the rows, 64 at a time: sixteen warps fetch rows of g and codes, turn the codes into
+// values and leave both in shared memory as they lie (the sum's index outermost: MN-major tiles), a thread of a seventeenth issues the
+// products (cta_group::1, two accumulators of 128 x 256 in TMEM).  The next blocks are on their way in registers.
 // With few results the rows are cut into shares that fill the SMs; shares are added in their order by a second launch.
 // Bound by HBM where a result tile takes all columns (430 000 rows of 256 against 47: 358 bytes a row), by the tensor cores beyond.
 #include "kept.h"
@@ -13,14 +13,14 @@ namespace dgs {
 namespace {
 using namespace tc;
 
-constexpr int TILE = 256, ROWS = 64, FETCH_THREADS = 256, THREADS = FETCH_THREADS + 128, STAGES = 3;
-// Registers: 3 x 128 x 168 at the launch; the two warpgroups that fetch take what the products' one leaves
-constexpr int MANY_REGISTERS = 216, FEW_REGISTERS = 72;
+constexpr int TILE = 256, ROWS = 64, FETCH_WARPS = 16, FETCHERS = FETCH_WARPS * 32, THREADS = FETCHERS + 128, STAGES = 3;
+// Registers: 5 x 128 x 96 at the launch; the four warpgroups that fetch take what the products' one leaves
+constexpr int MANY_REGISTERS = 104, FEW_REGISTERS = 64;
 constexpr uint32_t PANEL = ROWS * 128;                 // 64 columns of 64 rows
 constexpr uint32_t OPERAND = TILE / 64 * PANEL, STAGE = 2 * OPERAND;
 constexpr uint32_t BARS = STAGES * STAGE, SMEM = BARS + 128;
-constexpr int NARROW = 64;  // results a row of the weight: up to here two of a row's pieces a thread instead of eight, and a block more on its way
-constexpr int C_CHUNKS = TILE / 16, C_TASKS = ROWS * C_CHUNKS / FETCH_THREADS;  // 16 codes
+constexpr int NARROW = 64;  // results a row of the weight: up to here one piece of a row a thread instead of four, and more blocks on their way
+constexpr int C_CHUNKS = TILE / 16, C_TASKS = ROWS * C_CHUNKS / FETCHERS;  // 16 codes
 constexpr int MAX_DEVICES = 64;
 
 // 16 bytes of a row from byte `at` on; what lies at or behind byte `end` comes as anything, but is not read where a whole word does.
@@ -91,19 +91,19 @@ struct Block {
 template <bool BF16, bool G_ALIGNED, bool C_ALIGNED, bool FEW>
 __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_constant__ KeptGradArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  constexpr int G_CHUNKS = (FEW ? NARROW : TILE) / 8, G_TASKS = ROWS * G_CHUNKS / FETCH_THREADS;  // 16-byte pieces of g's rows
-  constexpr int DEPTH = FEW ? 3 : 2;                                                              // blocks of rows on their way
+  constexpr int G_CHUNKS = (FEW ? NARROW : TILE) / 8, G_TASKS = ROWS * G_CHUNKS / FETCHERS;  // 16-byte pieces of g's rows
+  constexpr int DEPTH = FEW ? 4 : 2;                                                        // blocks of rows on their way
   const uint32_t smem = smem_addr(smem_raw), full = smem + BARS, empty = full + 8 * STAGES, done = empty + 8 * STAGES, summed = done + 8,
                  tmem_word = summed + 8;
   volatile int* dead = reinterpret_cast<volatile int*>(smem_raw + (tmem_word + 4 - smem));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      bar_init(full + 8 * i, FETCH_THREADS);
+      bar_init(full + 8 * i, FETCHERS);
       bar_init(empty + 8 * i, 1);
     }
     bar_init(done, 1);
-    bar_init(summed, FETCH_THREADS);
+    bar_init(summed, FETCHERS);
     *dead = 0;
     bar_init_fence();
   }
@@ -120,13 +120,14 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
   const int cols = min(TILE, a.D - d0), outs = min(TILE, a.O - o0);
   bool ok = true;
 
-  if (warp < FETCH_THREADS / 32) {
+  if (warp < FETCH_WARPS) {
     more_registers<MANY_REGISTERS>();
     const char* g = static_cast<const char*>(a.grad) + static_cast<int64_t>(o0) * 2;
     const char* c = reinterpret_cast<const char*>(a.codes) + d0;
     const int g_chunk = threadIdx.x % G_CHUNKS, g_row = threadIdx.x / G_CHUNKS;  // (the same piece of every row of this thread)
-    const int c_chunk = threadIdx.x % C_CHUNKS, c_row = threadIdx.x / C_CHUNKS;
-    constexpr int G_STEP = FETCH_THREADS / G_CHUNKS, C_STEP = FETCH_THREADS / C_CHUNKS;
+    // eight neighbouring lanes: four pieces of one panel's rows, in two rows, so that their 16 bytes lie in different banks
+    const int c_chunk = (lane & 3) | (lane >> 3 << 2), c_row = warp * 2 + (lane >> 2 & 1);
+    constexpr int G_STEP = FETCHERS / G_CHUNKS, C_STEP = FETCHERS / C_CHUNKS;
     const int64_t g_pitch = a.grad_stride * 2, g_end = static_cast<int64_t>(outs) * 2, group = (d0 + c_chunk * 16) / KEPT_GROUP;
     const bool g_in = g_chunk * 8 < outs, c_in = c_chunk * 16 < cols;
     const bool sums = a.dbias != nullptr && blockIdx.x == 0;
@@ -176,14 +177,11 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
           uint32_t v[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) values_of<BF16>(x.c[i].w[e], x.scale[i], &v[2 * e], &v[2 * e + 1]);
-          // neighbouring panels begin at the same banks: every second one stores its halves the other way round
-          const int turn = (c_chunk >> 2) & 1;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int half = h ^ turn;
-            const uint32_t to = to_c + row * 128 + ((((c_chunk & 3) * 2 + half) ^ (row & 7)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(half ? v[4] : v[0]), "r"(half ? v[5] : v[1]),
-                         "r"(half ? v[6] : v[2]), "r"(half ? v[7] : v[3])
+            const uint32_t to = to_c + row * 128 + ((((c_chunk & 3) * 2 + h) ^ (row & 7)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[4 * h]), "r"(v[4 * h + 1]), "r"(v[4 * h + 2]),
+                         "r"(v[4 * h + 3])
                          : "memory");
           }
         }
@@ -208,14 +206,14 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
     if (ok) {
       // ---- results: a row of the weight a thread
       fence_after();
-      const int o = warp / 4 * 128 + warp % 4 * 32 + lane;
+      const int which = warp / 8, o = which * 128 + warp % 4 * 32 + lane;  // an accumulator, every second 32 of its columns
       const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-      if (warp / 4 * 128 < outs) {
+      if (which * 128 < outs) {
 #pragma unroll 1
-        for (int q = 0; q * 32 < cols; ++q) {
+        for (int q = warp / 4 % 2; q * 32 < cols; q += 2) {
           uint32_t v[32];
           if (blocks > 0) {
-            tmem_load32(tmem + warp / 4 * 256 + q * 32 + lanes, v);
+            tmem_load32(tmem + which * 256 + q * 32 + lanes, v);
             tmem_wait(v);
           } else {
 #pragma unroll
@@ -271,7 +269,7 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
     }
   } else {
     fewer_registers<FEW_REGISTERS>();
-    if (warp == FETCH_THREADS / 32 && lane == 0) {
+    if (warp == FETCH_WARPS && lane == 0) {
       // ---- products
       const uint32_t n = static_cast<uint32_t>((cols + 15) / 16 * 16), idesc = mma_desc(BF16, true, true, 128, n);
       int slot = 0;
