@@ -352,7 +352,7 @@ constexpr int64_t KEPT_MAX_SIDE = int64_t(1) << 22;  // elements of a row
 
 int check(const char* who, int64_t n, int64_t D, int32_t dtype) {
   DGS_REQUIRE(dtype_bytes(dtype) != 0, DGS_ERR_UNSUPPORTED, "%s: element type %d", who, dtype);
-  DGS_REQUIRE(n >= 0 && D >= 1 && D <= KEPT_MAX_SIDE && n <= (int64_t(1) << 40), DGS_ERR_INVALID, "%s: %lld rows of %lld elements", who,
+  DGS_REQUIRE(n >= 0 && D >= 1 && D <= KEPT_MAX_SIDE && n < (int64_t(1) << 31), DGS_ERR_INVALID, "%s: %lld rows of %lld elements", who,
               static_cast<long long>(n), static_cast<long long>(D));
   return DGS_OK;
 }

@@ -23,25 +23,26 @@ constexpr int NARROW = 64;  // results a row of the weight: up to here one piece
 constexpr int C_CHUNKS = TILE / 16, C_TASKS = ROWS * C_CHUNKS / FETCHERS;  // 16 codes
 constexpr int MAX_DEVICES = 64;
 
-// 16 bytes of a row from byte `at` on; what lies at or behind byte `end` comes as anything, but is not read where a whole word does.
-// ALIGNED: rows begin at 16-byte boundaries, else they are put together out of the aligned words that hold them.
+// 16 bytes from `p` on, of which `left` belong to the row (none: zeros).  ALIGNED: at 16-byte boundaries, whole; else put together out of
+// the aligned words that hold them (what lies behind the row comes as anything, a word that holds none of it is not read).
 template <bool ALIGNED>
 struct Piece {
   uint32_t w[ALIGNED ? 4 : 5];
-  __device__ __forceinline__ void fetch(const char* row, int64_t at, int64_t end) {
+  __device__ __forceinline__ void fetch(const char* p, int left) {
     if constexpr (ALIGNED) {
-      const uint4 v = at < end ? __ldg(reinterpret_cast<const uint4*>(row + at)) : make_uint4(0, 0, 0, 0);
+      const uint4 v = left > 0 ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
       w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     } else {
-      const char* p = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row + at) & ~uintptr_t(3));
-      const char* stop = at < end ? row + end : p;
+      const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3);
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p - off);
+      const int stop = left > 0 ? left + off : 0;
 #pragma unroll
-      for (int i = 0; i < 5; ++i) w[i] = p + 4 * i < stop ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
+      for (int i = 0; i < 5; ++i) w[i] = 4 * i < stop ? __ldg(q + i) : 0u;
     }
   }
-  __device__ __forceinline__ void line_up(const char* row, int64_t at) {
+  __device__ __forceinline__ void line_up(const char* p) {
     if constexpr (!ALIGNED) {
-      const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + at) & 3) * 8;
+      const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 3) * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], shift);
     }
@@ -122,41 +123,48 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
 
   if (warp < FETCH_WARPS) {
     more_registers<MANY_REGISTERS>();
-    const char* g = static_cast<const char*>(a.grad) + static_cast<int64_t>(o0) * 2;
-    const char* c = reinterpret_cast<const char*>(a.codes) + d0;
     const int g_chunk = threadIdx.x % G_CHUNKS, g_row = threadIdx.x / G_CHUNKS;  // (the same piece of every row of this thread)
     // eight neighbouring lanes: four pieces of one panel's rows, in two rows, so that their 16 bytes lie in different banks
     const int c_chunk = (lane & 3) | (lane >> 3 << 2), c_row = warp * 2 + (lane >> 2 & 1);
-    constexpr int G_STEP = FETCHERS / G_CHUNKS, C_STEP = FETCHERS / C_CHUNKS;
-    const int64_t g_pitch = a.grad_stride * 2, g_end = static_cast<int64_t>(outs) * 2, group = (d0 + c_chunk * 16) / KEPT_GROUP;
-    const bool g_in = g_chunk * 8 < outs, c_in = c_chunk * 16 < cols;
+    constexpr int G_STEP = FETCHERS / G_CHUNKS, C_STEP = FETCHERS / C_CHUNKS;  // (both multiples of 8: the swizzle is a thread's own)
+    const int64_t g_pitch = a.grad_stride * 2, c_pitch = a.codes_stride;
+    const int g_left = outs * 2 - g_chunk * 16, c_left = cols - c_chunk * 16;
+    const bool g_in = g_left > 0, c_in = c_left > 0;
     const bool sums = a.dbias != nullptr && blockIdx.x == 0;
+    // where this thread's first row of the next block to be fetched is; rows of the share from there on
+    const char* g = static_cast<const char*>(a.grad) + static_cast<int64_t>(o0) * 2 + (r0 + g_row) * g_pitch + g_chunk * 16;
+    const char* c = reinterpret_cast<const char*>(a.codes) + d0 + (r0 + c_row) * c_pitch + c_chunk * 16;
+    const float* scales = a.scales + (r0 + c_row) * a.groups + (d0 + c_chunk * 16) / KEPT_GROUP;
+    int rows = static_cast<int>(r1 - r0);
     float db[8] = {};
     Block<G_ALIGNED, C_ALIGNED, G_TASKS> on_way[DEPTH];
-    const auto fetch = [&](Block<G_ALIGNED, C_ALIGNED, G_TASKS>& x, int64_t r) {
+    const auto fetch = [&](Block<G_ALIGNED, C_ALIGNED, G_TASKS>& x) {
 #pragma unroll
-      for (int i = 0; i < G_TASKS; ++i) {
-        const int64_t row = r + g_row + i * G_STEP;
-        x.g[i].fetch(g + row * g_pitch, g_chunk * 16, row < r1 && g_in ? g_end : 0);
-      }
+      for (int i = 0; i < G_TASKS; ++i) x.g[i].fetch(g + i * (G_STEP * g_pitch), g_row + i * G_STEP < rows ? g_left : 0);
 #pragma unroll
       for (int i = 0; i < C_TASKS; ++i) {
-        const int64_t row = r + c_row + i * C_STEP;
-        x.c[i].fetch(c + row * a.codes_stride, c_chunk * 16, row < r1 && c_in ? cols : 0);
-        x.scale[i] = row < r1 && c_in ? __ldg(a.scales + row * a.groups + group) : 0.0f;
+        const bool in = c_row + i * C_STEP < rows;
+        x.c[i].fetch(c + i * (C_STEP * c_pitch), in ? c_left : 0);
+        x.scale[i] = in && c_in ? __ldg(scales + i * (C_STEP * a.groups)) : 0.0f;
       }
+      g += ROWS * g_pitch;
+      c += ROWS * c_pitch;
+      scales += static_cast<int64_t>(ROWS) * a.groups;
+      rows -= ROWS;
     };
     int slot = 0;
     uint32_t phase = 0;
-    const auto store = [&](Block<G_ALIGNED, C_ALIGNED, G_TASKS>& x, int64_t r) {
-      const uint32_t to_g = smem + slot * STAGE + (g_chunk / 8) * PANEL, to_c = smem + slot * STAGE + OPERAND + (c_chunk / 4) * PANEL;
+    const uint32_t g_to = smem + (g_chunk / 8) * PANEL + g_row * 128 + (((g_chunk & 7) ^ (g_row & 7)) << 4);
+    const uint32_t c_to = smem + OPERAND + (c_chunk / 4) * PANEL + c_row * 128, c_low = ((c_chunk & 3) * 2 ^ (c_row & 7)) << 4;
+    const auto store = [&](Block<G_ALIGNED, C_ALIGNED, G_TASKS>& x) {
+      const uint32_t at = slot * STAGE;
       if (g_in) {
 #pragma unroll
         for (int i = 0; i < G_TASKS; ++i) {
-          const int row = g_row + i * G_STEP;
-          x.g[i].line_up(g + (r + row) * g_pitch, g_chunk * 16);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to_g + row * 128 + (((g_chunk & 7) ^ (row & 7)) << 4)), "r"(x.g[i].w[0]),
-                       "r"(x.g[i].w[1]), "r"(x.g[i].w[2]), "r"(x.g[i].w[3])
+          // (DEPTH blocks of 64 rows on: the same place within a word as then)
+          x.g[i].line_up(g + i * (G_STEP * g_pitch));
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(g_to + at + i * (G_STEP * 128)), "r"(x.g[i].w[0]), "r"(x.g[i].w[1]),
+                       "r"(x.g[i].w[2]), "r"(x.g[i].w[3])
                        : "memory");
           if (sums) {
 #pragma unroll
@@ -172,33 +180,29 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
       if (c_in) {
 #pragma unroll
         for (int i = 0; i < C_TASKS; ++i) {
-          const int row = c_row + i * C_STEP;
-          x.c[i].line_up(c + (r + row) * a.codes_stride, c_chunk * 16);
+          x.c[i].line_up(c + i * (C_STEP * c_pitch));
           uint32_t v[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) values_of<BF16>(x.c[i].w[e], x.scale[i], &v[2 * e], &v[2 * e + 1]);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t to = to_c + row * 128 + ((((c_chunk & 3) * 2 + h) ^ (row & 7)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[4 * h]), "r"(v[4 * h + 1]), "r"(v[4 * h + 2]),
-                         "r"(v[4 * h + 3])
+          for (int h = 0; h < 2; ++h)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(c_to + at + i * (C_STEP * 128) + (c_low ^ (h << 4))), "r"(v[4 * h]),
+                         "r"(v[4 * h + 1]), "r"(v[4 * h + 2]), "r"(v[4 * h + 3])
                          : "memory");
-          }
         }
       }
     };
 #pragma unroll
-    for (int w = 0; w < DEPTH; ++w) fetch(on_way[w], r0 + w * ROWS);  // (rows behind the share are not read)
+    for (int w = 0; w < DEPTH; ++w) fetch(on_way[w]);  // (rows behind the share are not read)
     for (int b0 = 0; ok && b0 < blocks; b0 += DEPTH) {
 #pragma unroll
       for (int w = 0; w < DEPTH; ++w) {
         if (!ok || b0 + w >= blocks) continue;
-        const int64_t r = r0 + static_cast<int64_t>(b0 + w) * ROWS;
         if (!(ok = !*dead && bar_wait(empty + 8 * slot, phase ^ 1))) continue;
-        store(on_way[w], r);
+        store(on_way[w]);
         fence_async_smem();
         bar_arrive(full + 8 * slot);
-        fetch(on_way[w], r + DEPTH * ROWS);
+        fetch(on_way[w]);
         if (++slot == STAGES) slot = 0, phase ^= 1;
       }
     }
