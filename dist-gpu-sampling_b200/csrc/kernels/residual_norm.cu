@@ -7,10 +7,14 @@
 //   norm'(d) = rstd (d w - avg(d w) - h avg(d w h)), h the normed values (the plain average is left out in the root-mean-square form)
 //   dw = sum over rows of d h, db = sum of d, the gate's gradient summed over what it was spread over
 //
-// Bound by HBM: every row is read and written once in each direction.  TPR threads share a row, eight elements each, which stay in
+// Bound by HBM: every row is read and written once in each direction.  TPR threads share a row, E elements each, which stay in
 // registers from the first sum to the result; sums are in 32 bits and of centred values.  A thread keeps its columns for all rows of
 // its CTA, so column sums grow in registers; each CTA leaves one partial row and a second launch adds the partial rows in their
-// order (no atomics: the same inputs give the same bits).
+// order (no atomics: the same inputs give the same bits).  A gate of the columns is the same factor in every row, so its gradient and
+// those of the post norm's parameters come out of two sums: with S2 = sum g ys y^, S3 = sum g ys
+//   dpost_weight = gate S2,  dpost_bias = gate S3,  dgate = post_weight S2 + post_bias S3
+// At 12 bytes an element the issue slots allow some 60 instructions: weights lie in shared memory in 32 bits (a quarter of a load each, no
+// conversion), arithmetic is two elements an instruction, and with 16 elements a thread a row's sums over the CTA cost a twentieth.
 #include <initializer_list>
 
 #include "train_common.cuh"
@@ -18,13 +22,14 @@
 namespace dgs {
 namespace {
 
-constexpr int RN_ELEMS = 8;  // of a row, a thread
 constexpr int RN_MAX_D = 8192;
-constexpr int RN_SUMS = 5;   // column sums: dweight, dbias, dpost_weight, dpost_bias, dgate
+constexpr int RN_SUMS = 4;     // column sums: dout h, dout, S2, S3
+constexpr int RN_GRADS = 5;    // dweight, dbias, dpost_weight, dpost_bias, dgate
+constexpr int RN_PARAMS = 5;   // post_weight, post_bias, the columns' gate, weight, bias
 constexpr int RN_MAX_CTAS_PER_SM = 4;
 constexpr int RN_MAX_STAGES = 4;
 constexpr int RN_JOIN_THREADS = 1024;
-constexpr int RN_MAX_SMEM = 200 * 1024;
+constexpr int RN_MAX_SMEM = 220 * 1024;
 constexpr int RN_MAX_DEVICES = 64;
 
 struct Source {
@@ -34,7 +39,8 @@ struct Source {
 
 struct NormArgs {
   Source in[5];  // forward: x, y, gate of each element; backward: s, y, dout, ds, gate of each element
-  const void *row_gate, *column_gate, *post_weight, *post_bias, *weight, *bias;
+  const void* param[RN_PARAMS];
+  const void* row_gate;
   int64_t n;
   int32_t D, param_dtype, post, pre;  // DGS_NORM_*
   float xs, ys, eps;
@@ -44,45 +50,62 @@ struct NormArgs {
   // backward
   void *dx, *dy, *dgate;  // dgate: of each element, or of each row
   float* partial;         // [CTAs][RN_SUMS][D]
-  int32_t stages, stage_bytes;
+  int32_t stages, stage_bytes, ring_at, param_at[RN_PARAMS];  // shared memory: the weights that are there, in 32 bits, then the ring
 };
+enum { POST_WEIGHT, POST_BIAS, GATE, WEIGHT, BIAS };
 
 template <int TPR>
 constexpr int threads_of() {
   return TPR > 32 ? TPR : 256;
 }
 
-// COUNT sums over the threads of a row, returned to all of them.  Every thread of the CTA calls it; `red` alternates between two.
+// COUNT (up to 3) sums over the threads of a row, returned to all of them.  Every thread of the CTA calls it; `red` is not written again
+// before every thread has passed another such sum, or a barrier.
 template <int TPR, int COUNT>
-__device__ __forceinline__ void row_sums(float (&v)[COUNT], float (*red)[4]) {
+__device__ __forceinline__ void row_sums(float (&v)[COUNT], float4* red) {
 #pragma unroll
   for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
 #pragma unroll
     for (int q = 0; q < COUNT; ++q) v[q] += __shfl_xor_sync(FULL_MASK, v[q], o);
   if constexpr (TPR > 32) {
+    constexpr int WARPS = TPR / 32;
+    float* mine = reinterpret_cast<float*>(red + (threadIdx.x >> 5));
     if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-      for (int q = 0; q < COUNT; ++q) red[threadIdx.x >> 5][q] = v[q];
+      for (int q = 0; q < COUNT; ++q) mine[q] = v[q];
     }
     __syncthreads();
+    const float* other = reinterpret_cast<const float*>(red + (threadIdx.x & (WARPS - 1)));
 #pragma unroll
-    for (int q = 0; q < COUNT; ++q) v[q] = 0.0f;
+    for (int q = 0; q < COUNT; ++q) v[q] = other[q];
 #pragma unroll
-    for (int w = 0; w < TPR / 32; ++w)
+    for (int o = WARPS / 2; o > 0; o >>= 1)
 #pragma unroll
-      for (int q = 0; q < COUNT; ++q) v[q] += red[w][q];
+      for (int q = 0; q < COUNT; ++q) v[q] += __shfl_xor_sync(FULL_MASK, v[q], o);
   }
 }
 
-// The rows of up to COUNT arrays.  16-byte vectors travel by cp.async through a ring in shared memory, so the next rows are on
-// their way while one is summed; a thread fetches what it will read itself, so its own wait is all the synchronisation.  Narrower
-// vectors (rows off the 16-byte grid) are loaded where they are used.
-template <typename T, int VEC, int TPR, int COUNT>
+// two elements an instruction
+__device__ __forceinline__ void add_to(float* v, float lo, float hi) {
+  split2(add2(two(v[0], v[1]), two(lo, hi)), &v[0], &v[1]);
+}
+__device__ __forceinline__ void mul_to(float* v, float lo, float hi) {
+  split2(mul2(two(v[0], v[1]), two(lo, hi)), &v[0], &v[1]);
+}
+// v += a b
+__device__ __forceinline__ void fma_to(float* v, const float* a, const float* b) {
+  split2(fma2(two(a[0], a[1]), two(b[0], b[1]), two(v[0], v[1])), &v[0], &v[1]);
+}
+
+// Rows of up to COUNT arrays.  Vectors of 4, 8 or 16 bytes travel by cp.async through a ring in shared memory, so the next rows are on
+// their way while one is summed; a thread fetches what it will read itself, so its own wait is all the synchronisation.  Single
+// elements of two bytes are loaded where they are used.
+template <typename T, int VEC, int TPR, int E, int COUNT>
 struct Feed {
-  static constexpr int NV = RN_ELEMS / VEC, THREADS = threads_of<TPR>();
-  static constexpr bool kRing = sizeof(T) * VEC == 16;
+  static constexpr int NV = E / VEC, THREADS = threads_of<TPR>(), BYTES = VEC * static_cast<int>(sizeof(T));
+  static constexpr bool kRing = BYTES >= 4;
   const NormArgs& a;
-  uint32_t ring;
+  const unsigned char* ring;
   int t, stage;
   int64_t step, ahead;
 
@@ -91,36 +114,39 @@ struct Feed {
   __device__ __forceinline__ void issue(int64_t row, int st) {
     if constexpr (kRing) {
       if (row < a.n) {
-        uint32_t at = ring + st * a.stage_bytes + threadIdx.x * 16;
+        uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + st * a.stage_bytes + threadIdx.x * BYTES;
 #pragma unroll
         for (int q = 0; q < COUNT; ++q) {
           if (a.in[q].p == nullptr) continue;
           const T* p = static_cast<const T*>(a.in[q].p) + row * a.in[q].stride;
 #pragma unroll
           for (int k = 0; k < NV; ++k) {
-            if (in(k)) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(p + column(k)) : "memory");
-            at += THREADS * 16;
+            if (in(k)) {
+              if constexpr (BYTES == 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(p + column(k)) : "memory");
+              else
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(p + column(k)), "n"(BYTES) : "memory");
+            }
+            at += THREADS * BYTES;
           }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
   }
-  __device__ __forceinline__ void begin(int64_t row, int64_t apart, unsigned char* smem) {
+  __device__ __forceinline__ void begin(int64_t row, int64_t apart, const unsigned char* smem) {
     t = threadIdx.x % TPR;
     stage = 0;
     step = apart;
-    if constexpr (kRing) {
-      ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    ring = smem;
+    if constexpr (kRing)
       for (int s = 0; s < a.stages - 1; ++s) issue(row + s * step, s);
-    }
     ahead = (a.stages - 1) * step;
   }
   // the rows `row` of this stage: asks for those `stages - 1` steps on, waits for these
   __device__ __forceinline__ void next(int64_t row) {
     if constexpr (kRing) {
-      const int last = stage == 0 ? a.stages - 1 : stage - 1;
-      issue(row + ahead, last);
+      issue(row + ahead, stage == 0 ? a.stages - 1 : stage - 1);
       if (a.stages == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
       else if (a.stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
       else if (a.stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
@@ -131,12 +157,12 @@ struct Feed {
     if constexpr (kRing) stage = stage + 1 == a.stages ? 0 : stage + 1;
   }
   // array q's elements of the row (zeros outside); `slot`: how many arrays are there before it
-  __device__ __forceinline__ void get(int q, int slot, int64_t row, bool there, float (&v)[RN_ELEMS], const unsigned char* smem) const {
+  __device__ __forceinline__ void get(int q, int slot, int64_t row, bool there, float (&v)[E]) const {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float x[VEC];
       if (there && in(k)) {
-        const T* p = kRing ? reinterpret_cast<const T*>(smem + stage * a.stage_bytes + (slot * NV + k) * THREADS * 16 + threadIdx.x * 16)
+        const T* p = kRing ? reinterpret_cast<const T*>(ring + stage * a.stage_bytes + ((slot * NV + k) * THREADS + threadIdx.x) * BYTES)
                            : static_cast<const T*>(a.in[q].p) + row * a.in[q].stride + column(k);
         load_vec<T, VEC>(p, x);
       } else {
@@ -147,7 +173,7 @@ struct Feed {
       for (int e = 0; e < VEC; ++e) v[k * VEC + e] = x[e];
     }
   }
-  __device__ __forceinline__ void put(void* base, int64_t row, bool there, const float (&v)[RN_ELEMS]) const {
+  __device__ __forceinline__ void put(void* base, int64_t row, bool there, const float (&v)[E]) const {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if (!(there && in(k))) continue;
@@ -157,119 +183,152 @@ struct Feed {
       store_vec<T, VEC>(static_cast<T*>(base) + row * a.D + column(k), x);
     }
   }
-  __device__ __forceinline__ void param(const void* p, float absent, float (&v)[RN_ELEMS]) const {
+  __device__ __forceinline__ void zero_outside(float (&v)[E]) const {
+    if (TPR * E == a.D) return;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (!in(k)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[k * VEC + e] = 0.0f;
+      }
+  }
+  // Weights: all TPR * E columns (beyond D: zeros), the fours of a vector of eight apart, so that neighbouring threads' 16 bytes lie
+  // side by side.
+  static __device__ __forceinline__ int place(int c) {
+    if constexpr (VEC == 8) return (c % 8 / 4) * (TPR * E / 2) + c / 8 * 4 + c % 4;
+    return c;
+  }
+  __device__ __forceinline__ void lay_out(unsigned char* smem) const {
+#pragma unroll 1
+    for (int q = 0; q < RN_PARAMS; ++q) {
+      if (a.param[q] == nullptr || a.param_at[q] < 0) continue;
+      float* to = reinterpret_cast<float*>(smem + a.param_at[q]);
+      for (int c = threadIdx.x; c < TPR * E; c += THREADS) to[place(c)] = c < a.D ? load_as_float(a.param[q], a.param_dtype, c) : 0.0f;
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ void param(int q, const unsigned char* smem, float (&v)[E]) const {
+    if (a.param_at[q] < 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = in(i / VEC) ? load_as_float(a.param[q], a.param_dtype, column(i / VEC) + i % VEC) : 0.0f;
+      return;
+    }
+    const float* p = reinterpret_cast<const float*>(smem + a.param_at[q]);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      float x[VEC];
-      if (p != nullptr && in(k)) {
-        if constexpr (VEC == 1) x[0] = load_as_float(p, a.param_dtype, column(k));
-        else load_vec_as_float<VEC>(p, a.param_dtype, column(k), x);
+      const int c = column(k);
+      if constexpr (VEC >= 4) {
+#pragma unroll
+        for (int f = 0; f < VEC / 4; ++f) {
+          const float4 x = *reinterpret_cast<const float4*>(p + place(c + f * 4));
+          v[k * VEC + f * 4] = x.x, v[k * VEC + f * 4 + 1] = x.y, v[k * VEC + f * 4 + 2] = x.z, v[k * VEC + f * 4 + 3] = x.w;
+        }
       } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[e] = absent;
+        v[k] = p[c];
       }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[k * VEC + e] = x[e];
     }
   }
 };
 
-// normed values of v in place; every thread of the CTA calls it
-template <int TPR, int VEC, typename FeedT>
-__device__ __forceinline__ void normalise(const FeedT& f, bool layer, int D, float eps, float (&v)[RN_ELEMS], float* mean, float* rstd,
-                                          float (*red)[32][4]) {
+// normed values of v in place (zeros outside of the row); every thread of the CTA calls it
+template <int TPR, int E, typename FeedT>
+__device__ __forceinline__ void normalise(const FeedT& f, bool layer, int D, float eps, float (&v)[E], float* mean, float* rstd, float4 (*red)[32]) {
   const float inv = 1.0f / static_cast<float>(D);
   *mean = 0.0f;
   if (layer) {
-    float s[1] = {0.0f};
+    float s[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < RN_ELEMS; ++i) s[0] += v[i];
-    row_sums<TPR, 1>(s, red[0]);
-    *mean = s[0] * inv;
+    for (int i = 0; i < E; i += 2) add_to(s, v[i], v[i + 1]);
+    float t[1] = {s[0] + s[1]};
+    row_sums<TPR, 1>(t, red[0]);
+    *mean = t[0] * inv;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) add_to(v + i, -*mean, -*mean);
+    f.zero_outside(v);
   }
-  float s[1] = {0.0f};
+  float s[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < RN_ELEMS; ++i) {
-    if (f.in(i / VEC)) {
-      v[i] -= *mean;
-      s[0] = fmaf(v[i], v[i], s[0]);
-    }
-  }
-  row_sums<TPR, 1>(s, red[1]);
-  *rstd = 1.0f / sqrtf(fmaf(s[0], inv, eps));
+  for (int i = 0; i < E; i += 2) fma_to(s, v + i, v + i);
+  float t[1] = {s[0] + s[1]};
+  row_sums<TPR, 1>(t, red[1]);
+  *rstd = 1.0f / sqrtf(fmaf(t[0], inv, eps));
 #pragma unroll
-  for (int i = 0; i < RN_ELEMS; ++i) v[i] *= *rstd;
+  for (int i = 0; i < E; i += 2) mul_to(v + i, *rstd, *rstd);
 }
 
-template <typename T, int VEC, int TPR>
+// v = v weight + bias, each where it is there
+template <int E, typename FeedT>
+__device__ __forceinline__ void weigh(const FeedT& f, int weight, int bias, const unsigned char* smem, float (&v)[E]) {
+  float p[E];
+  if (f.a.param[weight] != nullptr) {
+    f.param(weight, smem, p);
+#pragma unroll
+    for (int i = 0; i < E; i += 2) mul_to(v + i, p[i], p[i + 1]);
+  }
+  if (f.a.param[bias] != nullptr) {
+    f.param(bias, smem, p);
+#pragma unroll
+    for (int i = 0; i < E; i += 2) add_to(v + i, p[i], p[i + 1]);
+  }
+}
+
+template <typename T, int VEC, int TPR, int E>
 __global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_kernel(const __grid_constant__ NormArgs a) {
   constexpr int ROWS = threads_of<TPR>() / TPR;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float red[4][32][4];
+  __shared__ float4 red[4][32];
   pdl_enter();
   const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
-  Feed<T, VEC, TPR, 3> f{a};
+  Feed<T, VEC, TPR, E, 3> f{a};
   const int64_t mine = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / TPR;
-  f.begin(mine, step, smem);
+  f.begin(mine, step, smem + a.ring_at);
+  f.lay_out(smem);
   for (int64_t row = mine; row - threadIdx.x / TPR < a.n; row += step) {
     f.next(row);
     const bool there = row < a.n;
-    float y[RN_ELEMS], p[RN_ELEMS], m, r;
-    f.get(1, 1, row, there, y, smem);
+    float y[E], p[E], m, r;
+    f.get(1, 1, row, there, y);
     if (a.post != DGS_NORM_NONE) {
-      normalise<TPR, VEC>(f, a.post == DGS_NORM_LAYER, a.D, a.eps, y, &m, &r, red);
+      normalise<TPR, E>(f, a.post == DGS_NORM_LAYER, a.D, a.eps, y, &m, &r, red);
       if (there && f.t == 0) {
         if (a.post == DGS_NORM_LAYER) a.post_mean[row] = m;
         a.post_rstd[row] = r;
       }
-      f.param(a.post_weight, 1.0f, p);
-      if (a.post_bias != nullptr) {
-        float b[RN_ELEMS];
-        f.param(a.post_bias, 0.0f, b);
-#pragma unroll
-        for (int i = 0; i < RN_ELEMS; ++i) y[i] = fmaf(y[i], p[i], b[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < RN_ELEMS; ++i) y[i] *= p[i];
-      }
+      weigh(f, POST_WEIGHT, POST_BIAS, smem, y);
     }
     if (a.in[2].p != nullptr) {
-      f.get(2, 2, row, there, p, smem);
+      f.get(2, 2, row, there, p);
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) y[i] *= p[i];
-    } else if (a.column_gate != nullptr) {
-      f.param(a.column_gate, 1.0f, p);
+      for (int i = 0; i < E; i += 2) mul_to(y + i, p[i], p[i + 1]);
+    } else if (a.param[GATE] != nullptr) {
+      f.param(GATE, smem, p);
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) y[i] *= p[i];
+      for (int i = 0; i < E; i += 2) mul_to(y + i, p[i], p[i + 1]);
     } else if (a.row_gate != nullptr) {
       const float by = there ? to_float<T>(static_cast<const T*>(a.row_gate)[row]) : 0.0f;
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) y[i] *= by;
+      for (int i = 0; i < E; i += 2) mul_to(y + i, by, by);
     }
-    f.get(0, 0, row, there, p, smem);
+    f.get(0, 0, row, there, p);
 #pragma unroll
-    for (int i = 0; i < RN_ELEMS; ++i) {
+    for (int i = 0; i < E; i += 2) {
+      mul_to(p + i, a.xs, a.xs);
+      const float ys[2] = {a.ys, a.ys};
+      fma_to(p + i, ys, y + i);
       // (the next norm is of the row as it is stored, so that the backward pass finds the same)
-      y[i] = to_float<T>(from_float<T>(fmaf(a.ys, y[i], a.xs * p[i])));
+      y[i] = to_float<T>(from_float<T>(p[i]));
+      y[i + 1] = to_float<T>(from_float<T>(p[i + 1]));
     }
     f.done();
     f.put(a.sum, row, there, y);
     if (a.pre != DGS_NORM_NONE) {
-      normalise<TPR, VEC>(f, a.pre == DGS_NORM_LAYER, a.D, a.eps, y, &m, &r, red + 2);
+      f.zero_outside(y);
+      normalise<TPR, E>(f, a.pre == DGS_NORM_LAYER, a.D, a.eps, y, &m, &r, red + 2);
       if (there && f.t == 0) {
         if (a.pre == DGS_NORM_LAYER) a.mean[row] = m;
         a.rstd[row] = r;
       }
-      f.param(a.weight, 1.0f, p);
-      if (a.bias != nullptr) {
-        float b[RN_ELEMS];
-        f.param(a.bias, 0.0f, b);
-#pragma unroll
-        for (int i = 0; i < RN_ELEMS; ++i) y[i] = fmaf(y[i], p[i], b[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < RN_ELEMS; ++i) y[i] *= p[i];
-      }
+      weigh(f, WEIGHT, BIAS, smem, y);
       f.put(a.out, row, there, y);
     }
     if constexpr (TPR > 32) {
@@ -279,136 +338,160 @@ __global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_kernel(const 
   }
 }
 
-// norm' of d (the gradient of the normed and weighted values) in place, zeros outside of the row; h the normed values; `also` is summed
-// over the row too
-template <int TPR, int VEC, typename FeedT>
-__device__ __forceinline__ void norm_back(const FeedT& f, bool layer, int D, float rstd, const float (&w)[RN_ELEMS], const float (&h)[RN_ELEMS],
-                                          float (&d)[RN_ELEMS], float* also, float (*red)[4]) {
-  float s[3] = {0.0f, 0.0f, *also};
+// norm' of d (the gradient of the normed values) in place, zeros outside of the row; h the normed values; `also` is summed over the row too
+template <int TPR, int E, typename FeedT>
+__device__ __forceinline__ void norm_back(const FeedT& f, bool layer, int D, float rstd, const float (&h)[E], float (&d)[E], float* also,
+                                          float4* red) {
+  float p[2] = {0.0f, 0.0f}, q[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < RN_ELEMS; ++i) {
-    d[i] *= w[i];
-    s[0] += d[i];
-    s[1] = fmaf(d[i], h[i], s[1]);
+  for (int i = 0; i < E; i += 2) {
+    add_to(p, d[i], d[i + 1]);
+    fma_to(q, d + i, h + i);
   }
+  float s[3] = {p[0] + p[1], q[0] + q[1], *also};
   row_sums<TPR, 3>(s, red);
-  const float inv = 1.0f / static_cast<float>(D), avg = layer ? s[0] * inv : 0.0f, dot = s[1] * inv;
+  const float inv = 1.0f / static_cast<float>(D), avg = layer ? s[0] * inv * rstd : 0.0f, dot = s[1] * inv * rstd;
   *also = s[2];
+  const float minus[2] = {-dot, -dot}, by[2] = {rstd, rstd};
 #pragma unroll
-  for (int i = 0; i < RN_ELEMS; ++i) d[i] = f.in(i / VEC) ? rstd * (d[i] - avg - h[i] * dot) : 0.0f;
+  for (int i = 0; i < E; i += 2) {
+    // d rstd - avg - h dot
+    float x[2] = {-avg, -avg};
+    fma_to(x, h + i, minus);
+    fma_to(x, d + i, by);
+    d[i] = x[0];
+    d[i + 1] = x[1];
+  }
+  f.zero_outside(d);
 }
 
-template <typename T, int VEC, int TPR>
+template <typename T, int VEC, int TPR, int E>
 __global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
   constexpr int THREADS = threads_of<TPR>(), ROWS = THREADS / TPR;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float red[2][32][4];
+  __shared__ float4 red[2][32];
   pdl_enter();
   const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
-  Feed<T, VEC, TPR, 5> f{a};
+  Feed<T, VEC, TPR, E, 5> f{a};
   const int64_t mine = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / TPR;
-  f.begin(mine, step, smem);
+  f.begin(mine, step, smem + a.ring_at);
+  f.lay_out(smem);
   int slot[5], slots = 0;
 #pragma unroll
   for (int q = 0; q < 5; ++q) {
     slot[q] = slots;
     slots += a.in[q].p != nullptr;
   }
-  float sums[RN_SUMS][RN_ELEMS];
+  float sums[RN_SUMS][E];
 #pragma unroll
   for (int q = 0; q < RN_SUMS; ++q)
 #pragma unroll
-    for (int i = 0; i < RN_ELEMS; ++i) sums[q][i] = 0.0f;
+    for (int i = 0; i < E; ++i) sums[q][i] = 0.0f;
+  const bool pre = a.pre != DGS_NORM_NONE && a.in[2].p != nullptr, post = a.post != DGS_NORM_NONE, layer = a.pre == DGS_NORM_LAYER;
+  const bool columns = a.param[GATE] != nullptr;
   for (int64_t row = mine; row - threadIdx.x / TPR < a.n; row += step) {
     f.next(row);
     const bool there = row < a.n;
-    float g[RN_ELEMS], h[RN_ELEMS], w[RN_ELEMS], none = 0.0f;
-    if (a.pre != DGS_NORM_NONE && a.in[2].p != nullptr) {
-      const float m = there && a.pre == DGS_NORM_LAYER ? a.mean[row] : 0.0f, r = there ? a.rstd[row] : 0.0f;
-      f.get(0, slot[0], row, there, h, smem);
-      f.get(2, slot[2], row, there, g, smem);
+    float g[E], h[E], w[E], none = 0.0f;
+    if (pre) {
+      const float m = there && layer ? a.mean[row] : 0.0f, r = there ? a.rstd[row] : 0.0f;
+      f.get(0, slot[0], row, there, h);
+      f.get(2, slot[2], row, there, g);
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) {
-        h[i] = f.in(i / VEC) ? (h[i] - m) * r : 0.0f;
-        sums[0][i] = fmaf(g[i], h[i], sums[0][i]);
-        sums[1][i] += g[i];
+      for (int i = 0; i < E; i += 2) {
+        if (layer) add_to(h + i, -m, -m);
+        mul_to(h + i, r, r);
       }
-      f.param(a.weight, 1.0f, w);
-      norm_back<TPR, VEC>(f, a.pre == DGS_NORM_LAYER, a.D, r, w, h, g, &none, red[0]);
+      f.zero_outside(h);
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        fma_to(sums[0] + i, g + i, h + i);
+        add_to(sums[1] + i, g[i], g[i + 1]);
+      }
+      if (a.param[WEIGHT] != nullptr) {
+        f.param(WEIGHT, smem, w);
+#pragma unroll
+        for (int i = 0; i < E; i += 2) mul_to(g + i, w[i], w[i + 1]);
+      }
+      norm_back<TPR, E>(f, layer, a.D, r, h, g, &none, red[0]);
     } else {
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) g[i] = 0.0f;
+      for (int i = 0; i < E; ++i) g[i] = 0.0f;
     }
     if (a.in[3].p != nullptr) {
-      f.get(3, slot[3], row, there, w, smem);
+      f.get(3, slot[3], row, there, w);
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) g[i] += w[i];
+      for (int i = 0; i < E; i += 2) add_to(g + i, w[i], w[i + 1]);
     }
     if (a.dx != nullptr) {
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) w[i] = a.xs * g[i];
+      for (int i = 0; i < E; i += 2) {
+        w[i] = g[i], w[i + 1] = g[i + 1];
+        mul_to(w + i, a.xs, a.xs);
+      }
       f.put(a.dx, row, there, w);
     }
     float r = 0.0f;
-    f.get(1, slot[1], row, there, h, smem);
-    if (a.post != DGS_NORM_NONE) {
+    f.get(1, slot[1], row, there, h);
+    if (post) {
       const float m = there && a.post == DGS_NORM_LAYER ? a.post_mean[row] : 0.0f;
       r = there ? a.post_rstd[row] : 0.0f;
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) h[i] = f.in(i / VEC) ? (h[i] - m) * r : 0.0f;
+      for (int i = 0; i < E; i += 2) {
+        if (a.post == DGS_NORM_LAYER) add_to(h + i, -m, -m);
+        mul_to(h + i, r, r);
+      }
+      f.zero_outside(h);
     }
 #pragma unroll
-    for (int i = 0; i < RN_ELEMS; ++i) g[i] *= a.ys;
+    for (int i = 0; i < E; i += 2) mul_to(g + i, a.ys, a.ys);
     float of_row = 0.0f;
-    if (a.dgate != nullptr || a.column_gate != nullptr) {
-      // the gate's gradient: g times post(y)
-      float z[RN_ELEMS];
+    if (a.dgate != nullptr) {  // of each row or element: g times post(y)
+      float z[E];
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) z[i] = h[i];
-      if (a.post != DGS_NORM_NONE) {
-        f.param(a.post_weight, 1.0f, w);
+      for (int i = 0; i < E; ++i) z[i] = h[i];
+      if (post) weigh(f, POST_WEIGHT, POST_BIAS, smem, z);
 #pragma unroll
-        for (int i = 0; i < RN_ELEMS; ++i) z[i] *= w[i];
-        if (a.post_bias != nullptr) {
-          f.param(a.post_bias, 0.0f, w);
+      for (int i = 0; i < E; i += 2) mul_to(z + i, g[i], g[i + 1]);
+      if (a.row_gate != nullptr) {
+        f.zero_outside(z);
+        float s[2] = {0.0f, 0.0f};
 #pragma unroll
-          for (int i = 0; i < RN_ELEMS; ++i) z[i] += w[i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) z[i] *= g[i];
-      if (a.column_gate != nullptr) {
-#pragma unroll
-        for (int i = 0; i < RN_ELEMS; ++i) sums[4][i] += z[i];
-      } else if (a.row_gate != nullptr) {
-#pragma unroll
-        for (int i = 0; i < RN_ELEMS; ++i) of_row += z[i];
+        for (int i = 0; i < E; i += 2) add_to(s, z[i], z[i + 1]);
+        of_row = s[0] + s[1];
       } else {
         f.put(a.dgate, row, there, z);
       }
     }
     if (a.in[4].p != nullptr) {
-      f.get(4, slot[4], row, there, w, smem);
+      f.get(4, slot[4], row, there, w);
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) g[i] *= w[i];
-    } else if (a.column_gate != nullptr) {
-      f.param(a.column_gate, 1.0f, w);
-#pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) g[i] *= w[i];
+      for (int i = 0; i < E; i += 2) mul_to(g + i, w[i], w[i + 1]);
     } else if (a.row_gate != nullptr) {
       const float by = there ? to_float<T>(static_cast<const T*>(a.row_gate)[row]) : 0.0f;
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) g[i] *= by;
+      for (int i = 0; i < E; i += 2) mul_to(g + i, by, by);
     }
     f.done();
-    if (a.post != DGS_NORM_NONE) {
+    if (post || columns) {
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) {
-        sums[2][i] = fmaf(g[i], h[i], sums[2][i]);
-        sums[3][i] += g[i];
+      for (int i = 0; i < E; i += 2) {
+        fma_to(sums[2] + i, g + i, h + i);
+        add_to(sums[3] + i, g[i], g[i + 1]);
       }
-      f.param(a.post_weight, 1.0f, w);
-      norm_back<TPR, VEC>(f, a.post == DGS_NORM_LAYER, a.D, r, w, h, g, &of_row, red[1]);
+    }
+    if (columns) {
+      f.param(GATE, smem, w);
+#pragma unroll
+      for (int i = 0; i < E; i += 2) mul_to(g + i, w[i], w[i + 1]);
+    }
+    if (post) {
+      if (a.param[POST_WEIGHT] != nullptr) {
+        f.param(POST_WEIGHT, smem, w);
+#pragma unroll
+        for (int i = 0; i < E; i += 2) mul_to(g + i, w[i], w[i + 1]);
+      }
+      norm_back<TPR, E>(f, a.post == DGS_NORM_LAYER, a.D, r, h, g, &of_row, red[1]);
     } else if (a.row_gate != nullptr) {
       float s[1] = {of_row};
       row_sums<TPR, 1>(s, red[1]);
@@ -418,7 +501,7 @@ __global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_backward_kern
     if (a.row_gate != nullptr && a.dgate != nullptr && there && f.t == 0) static_cast<T*>(a.dgate)[row] = from_float<T>(of_row);
     if constexpr (TPR > 32) {
       // (a row with one sum alone: `red` must not be written before all have read it)
-      if (a.pre == DGS_NORM_NONE || a.in[2].p == nullptr || (a.post == DGS_NORM_NONE && a.row_gate == nullptr)) __syncthreads();
+      if (!pre || (!post && a.row_gate == nullptr)) __syncthreads();
     }
   }
   if (a.partial == nullptr) return;
@@ -427,18 +510,18 @@ __global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_backward_kern
 #pragma unroll
     for (int q = 0; q < RN_SUMS; ++q)
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i)
+      for (int i = 0; i < E; ++i)
         if (f.in(i / VEC)) to[q * a.D + f.column(i / VEC) + i % VEC] = sums[q][i];
   } else {
     // the CTA's groups, in their order
-    constexpr int WIDTH = TPR * RN_ELEMS;
+    constexpr int WIDTH = TPR * E;
     float* all = reinterpret_cast<float*>(smem);  // [ROWS][WIDTH]
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
     for (int q = 0; q < RN_SUMS; ++q) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < RN_ELEMS; ++i) all[(threadIdx.x / TPR) * WIDTH + f.column(i / VEC) + i % VEC] = sums[q][i];
+      for (int i = 0; i < E; ++i) all[(threadIdx.x / TPR) * WIDTH + f.column(i / VEC) + i % VEC] = sums[q][i];
       __syncthreads();
       for (int c = threadIdx.x; c < a.D; c += THREADS) {
         float s = 0.0f;
@@ -452,24 +535,39 @@ __global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_backward_kern
 struct JoinArgs {
   const float* partial;
   int32_t partials, D, param_dtype;
-  void* to[RN_SUMS];
+  const void *post_weight, *post_bias, *gate;
+  void* to[RN_GRADS];
 };
 // partial rows added in their order: 32 columns a CTA, a warp for every 32nd row
 __global__ __launch_bounds__(RN_JOIN_THREADS) void residual_norm_join_kernel(const __grid_constant__ JoinArgs a) {
-  __shared__ float part[32][33];
+  __shared__ float part[RN_SUMS][32][33];
   pdl_enter();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = blockIdx.y, c = blockIdx.x * 32 + lane;
-  if (a.to[q] == nullptr) return;
-  float s = 0.0f;
-  if (c < a.D)
-    for (int r = warp; r < a.partials; r += 32) s += a.partial[(static_cast<int64_t>(r) * RN_SUMS + q) * a.D + c];
-  part[warp][lane] = s;
-  __syncthreads();
-  s = part[lane][warp];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float s[RN_SUMS] = {};
+  if (c < a.D) {
+#pragma unroll 4
+    for (int r = warp; r < a.partials; r += 32)
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL_MASK, s, o);
+      for (int q = 0; q < RN_SUMS; ++q) s[q] += a.partial[(static_cast<int64_t>(r) * RN_SUMS + q) * a.D + c];
+  }
+#pragma unroll
+  for (int q = 0; q < RN_SUMS; ++q) part[q][warp][lane] = s[q];
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < RN_SUMS; ++q) {
+    s[q] = part[q][lane][warp];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s[q] += __shfl_xor_sync(FULL_MASK, s[q], o);
+  }
   const int column = blockIdx.x * 32 + warp;
-  if (lane == 0 && column < a.D) store_from_float(a.to[q], a.param_dtype, column, s);
+  if (lane != 0 || column >= a.D) return;
+  const float gate = a.gate != nullptr ? load_as_float(a.gate, a.param_dtype, column) : 1.0f;
+  const float w = a.post_weight != nullptr ? load_as_float(a.post_weight, a.param_dtype, column) : 1.0f;
+  const float b = a.post_bias != nullptr ? load_as_float(a.post_bias, a.param_dtype, column) : 0.0f;
+  const float grads[RN_GRADS] = {s[0], s[1], gate * s[2], gate * s[3], fmaf(w, s[2], b * s[3])};
+#pragma unroll
+  for (int q = 0; q < RN_GRADS; ++q)
+    if (a.to[q] != nullptr) store_from_float(a.to[q], a.param_dtype, column, grads[q]);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -478,19 +576,30 @@ int64_t partial_rows(int64_t n) {
   return n < most ? n : most;
 }
 
-template <typename T, int VEC, int TPR, bool BACK>
+template <typename T, int VEC, int TPR, int E, bool BACK>
 int launch_rows(NormArgs a, int arrays, int* ctas, cudaStream_t s) {
-  constexpr int THREADS = threads_of<TPR>(), ROWS = THREADS / TPR, NV = RN_ELEMS / VEC;
-  constexpr bool ring = sizeof(T) * VEC == 16;
+  constexpr int THREADS = threads_of<TPR>(), ROWS = THREADS / TPR, NV = E / VEC, BYTES = VEC * static_cast<int>(sizeof(T));
   void (*kernel)(NormArgs);
-  if constexpr (BACK) kernel = residual_norm_backward_kernel<T, VEC, TPR>;
-  else kernel = residual_norm_kernel<T, VEC, TPR>;
-  // two CTAs of up to 256 threads or one larger one fill the SM's registers; what they have under way, its shared memory
-  constexpr int room = THREADS <= 256 ? RN_MAX_SMEM / 2 : RN_MAX_SMEM;
-  a.stage_bytes = ring ? arrays * NV * THREADS * 16 : 0;
-  a.stages = !ring ? 1 : a.stage_bytes * RN_MAX_STAGES <= room ? RN_MAX_STAGES : room / a.stage_bytes;
-  size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes;
-  const size_t joined = BACK && ROWS > 1 ? static_cast<size_t>(THREADS) * RN_ELEMS * sizeof(float) : 0;
+  if constexpr (BACK) kernel = residual_norm_backward_kernel<T, VEC, TPR, E>;
+  else kernel = residual_norm_kernel<T, VEC, TPR, E>;
+  a.ring_at = 0;
+  for (int q = 0; q < RN_PARAMS; ++q) {
+    a.param_at[q] = a.ring_at;
+    if (a.param[q] != nullptr) a.ring_at += TPR * E * static_cast<int>(sizeof(float));
+  }
+  a.stage_bytes = BYTES >= 4 ? arrays * NV * THREADS * BYTES : 0;
+  if (a.ring_at + a.stage_bytes > RN_MAX_SMEM) {  // (the widest rows of 32 bits: weights out of global memory)
+    a.ring_at = 0;
+    for (int& at : a.param_at) at = -1;
+  }
+  // what a CTA has under way: half of an SM's shared memory where its registers hold two of them, else all
+  const int room = (THREADS <= 256 && !BACK ? RN_MAX_SMEM / 2 : RN_MAX_SMEM) - a.ring_at;
+  a.stages = a.stage_bytes == 0 ? 1 : a.stage_bytes * RN_MAX_STAGES <= room ? RN_MAX_STAGES : room / a.stage_bytes;
+  if (a.stages < 2 && a.stage_bytes > 0) a.stages = (RN_MAX_SMEM - a.ring_at) / a.stage_bytes;  // (one CTA an SM, then)
+  if (a.stages > RN_MAX_STAGES) a.stages = RN_MAX_STAGES;
+  DGS_REQUIRE(a.stages >= 1, DGS_ERR_UNSUPPORTED, "residual_norm: rows of %d elements", a.D);
+  size_t smem = static_cast<size_t>(a.ring_at) + static_cast<size_t>(a.stages) * a.stage_bytes;
+  const size_t joined = BACK && ROWS > 1 ? static_cast<size_t>(THREADS) * E * sizeof(float) : 0;
   if (smem < joined) smem = joined;
   // CTAs that an SM holds of it, known for the size that was asked for last (two host calls less)
   static std::atomic<int64_t> known[RN_MAX_DEVICES] = {};
@@ -514,23 +623,30 @@ int launch_rows(NormArgs a, int arrays, int* ctas, cudaStream_t s) {
 
 template <typename T, int VEC, bool BACK>
 int with_row(const NormArgs& a, int arrays, int* ctas, cudaStream_t s) {
-  // eight elements a thread; the next wider form holds the rest
-  const int threads = (a.D + RN_ELEMS - 1) / RN_ELEMS;
-  if (threads <= 4) return launch_rows<T, VEC, 4, BACK>(a, arrays, ctas, s);
-  if (threads <= 16) return launch_rows<T, VEC, 16, BACK>(a, arrays, ctas, s);
-  if (threads <= 32) return launch_rows<T, VEC, 32, BACK>(a, arrays, ctas, s);
-  if (threads <= 128) return launch_rows<T, VEC, 128, BACK>(a, arrays, ctas, s);
-  if (threads <= 512) return launch_rows<T, VEC, 512, BACK>(a, arrays, ctas, s);
-  return launch_rows<T, VEC, 1024, BACK>(a, arrays, ctas, s);
+  if constexpr (VEC == 1) {  // single elements: a warp a row as soon as it can, so that a load takes them side by side
+    if (a.D <= 32) return launch_rows<T, 1, 8, 4, BACK>(a, arrays, ctas, s);
+    if (a.D <= 128) return launch_rows<T, 1, 32, 4, BACK>(a, arrays, ctas, s);
+  } else {
+    if (a.D <= 64) return launch_rows<T, VEC, 4, 16, BACK>(a, arrays, ctas, s);
+    if (a.D <= 128) return launch_rows<T, VEC, 8, 16, BACK>(a, arrays, ctas, s);
+    if (a.D <= 256) return launch_rows<T, VEC, 16, 16, BACK>(a, arrays, ctas, s);
+  }
+  if (a.D <= 512) return launch_rows<T, VEC, 32, 16, BACK>(a, arrays, ctas, s);
+  if (a.D <= 2048) return launch_rows<T, VEC, 128, 16, BACK>(a, arrays, ctas, s);
+  if (a.D <= 4096) return launch_rows<T, VEC, 256, 16, BACK>(a, arrays, ctas, s);
+  return launch_rows<T, VEC, 512, 16, BACK>(a, arrays, ctas, s);
 }
 
+template <typename T, bool BACK>
+int with_type(const NormArgs& a, int vec, int arrays, int* ctas, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2)
+    if (vec == 8) return with_row<T, 8, BACK>(a, arrays, ctas, s);
+  return vec >= 4 ? with_row<T, 4, BACK>(a, arrays, ctas, s) : with_row<T, 1, BACK>(a, arrays, ctas, s);
+}
 template <bool BACK>
-int run_rows(const NormArgs& a, int32_t dtype, bool vectors, int arrays, int* ctas, cudaStream_t s) {
-  if (dtype == DGS_F32)
-    return vectors ? with_row<float, 4, BACK>(a, arrays, ctas, s) : with_row<float, 1, BACK>(a, arrays, ctas, s);
-  if (dtype == DGS_BF16)
-    return vectors ? with_row<__nv_bfloat16, 8, BACK>(a, arrays, ctas, s) : with_row<__nv_bfloat16, 1, BACK>(a, arrays, ctas, s);
-  return vectors ? with_row<__half, 8, BACK>(a, arrays, ctas, s) : with_row<__half, 1, BACK>(a, arrays, ctas, s);
+int run_rows(const NormArgs& a, int32_t dtype, int vec, int arrays, int* ctas, cudaStream_t s) {
+  if (dtype == DGS_F32) return with_type<float, BACK>(a, vec, arrays, ctas, s);
+  return dtype == DGS_BF16 ? with_type<__nv_bfloat16, BACK>(a, vec, arrays, ctas, s) : with_type<__half, BACK>(a, vec, arrays, ctas, s);
 }
 
 int check(const char* who, const dgs_residual_norm* p) {
@@ -560,11 +676,11 @@ int check(const char* who, const dgs_residual_norm* p) {
 NormArgs arguments(const dgs_residual_norm& p) {
   NormArgs a{};
   a.row_gate = p.gate_kind == DGS_GATE_ROW ? p.gate : nullptr;
-  a.column_gate = p.gate_kind == DGS_GATE_COLUMN ? p.gate : nullptr;
-  a.post_weight = p.post_weight;
-  a.post_bias = p.post_bias;
-  a.weight = p.weight;
-  a.bias = p.bias;
+  a.param[POST_WEIGHT] = p.post_weight;
+  a.param[POST_BIAS] = p.post_bias;
+  a.param[GATE] = p.gate_kind == DGS_GATE_COLUMN ? p.gate : nullptr;
+  a.param[WEIGHT] = p.weight;
+  a.param[BIAS] = p.bias;
   a.n = p.n;
   a.D = static_cast<int32_t>(p.D);
   a.param_dtype = p.param_dtype;
@@ -576,17 +692,18 @@ NormArgs arguments(const dgs_residual_norm& p) {
   return a;
 }
 
-// whether every row of every array can be moved in 16-byte vectors
-bool in_vectors(const dgs_residual_norm& p, const NormArgs& a, int count, std::initializer_list<const void*> results) {
-  const int64_t vec = 16 / dtype_bytes(p.dtype);
-  if (p.D % vec != 0) return false;
-  for (int q = 0; q < count; ++q)
-    if (a.in[q].p != nullptr && (!aligned_to(a.in[q].p, 16) || (a.in[q].stride % vec != 0 && p.n > 1))) return false;
-  for (const void* r : results)
-    if (!aligned_to(r, 16)) return false;
-  for (const void* w : {a.post_weight, a.post_bias, a.weight, a.bias, a.column_gate})
-    if (!aligned_to(w, 16)) return false;
-  return true;
+// the widest vectors in which every row of every array can be moved: 16 bytes, four elements, or one element
+int vectors(const dgs_residual_norm& p, const NormArgs& a, int count, std::initializer_list<const void*> results) {
+  const int esz = dtype_bytes(p.dtype);
+  for (int vec = 16 / esz; vec >= 4; vec /= 2) {
+    const size_t bytes = static_cast<size_t>(vec) * esz;
+    bool fits = p.D % vec == 0;
+    for (int q = 0; q < count; ++q)
+      fits &= a.in[q].p == nullptr || (aligned_to(a.in[q].p, bytes) && (a.in[q].stride % vec == 0 || p.n <= 1));
+    for (const void* r : results) fits &= aligned_to(r, bytes);
+    if (fits) return vec;
+  }
+  return 1;
 }
 
 }  // namespace
@@ -614,7 +731,7 @@ extern "C" int dgs_residual_norm_forward(const dgs_residual_norm* p, const void*
   a.mean = mean;
   a.rstd = rstd;
   int ctas = 0;
-  return run_rows<false>(a, p->dtype, in_vectors(*p, a, 3, {sum, out}), a.in[2].p != nullptr ? 3 : 2, &ctas, static_cast<cudaStream_t>(stream));
+  return run_rows<false>(a, p->dtype, vectors(*p, a, 3, {sum, out}), a.in[2].p != nullptr ? 3 : 2, &ctas, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t dgs_residual_norm_backward_workspace_bytes(int64_t n, int64_t D) {
@@ -635,7 +752,7 @@ extern "C" int dgs_residual_norm_backward(const dgs_residual_norm* p, const void
               DGS_ERR_INVALID, "residual_norm_backward: a gradient of what is absent");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool column = p->gate_kind == DGS_GATE_COLUMN;
-  void* to[RN_SUMS] = {dweight, dbias, dpost_weight, dpost_bias, column ? dgate : nullptr};
+  void* to[RN_GRADS] = {dweight, dbias, dpost_weight, dpost_bias, column ? dgate : nullptr};
   bool any = false;
   for (void* t : to) any |= t != nullptr;
   if (p->n == 0) {
@@ -667,10 +784,10 @@ extern "C" int dgs_residual_norm_backward(const dgs_residual_norm* p, const void
   a.partial = any ? static_cast<float*>(workspace) : nullptr;
   int arrays = 0, ctas = 0;
   for (const Source& in : a.in) arrays += in.p != nullptr;
-  if (int rc = run_rows<true>(a, p->dtype, in_vectors(*p, a, 5, {dx, dy, a.dgate}), arrays, &ctas, s)) return rc;
+  if (int rc = run_rows<true>(a, p->dtype, vectors(*p, a, 5, {dx, dy, a.dgate}), arrays, &ctas, s)) return rc;
   if (!any) return DGS_OK;
-  JoinArgs j{a.partial, ctas, a.D, p->param_dtype, {}};
-  for (int q = 0; q < RN_SUMS; ++q) j.to[q] = to[q];
-  DGS_CUDA_TRY(launch_training(residual_norm_join_kernel, dim3(static_cast<unsigned>((p->D + 31) / 32), RN_SUMS), RN_JOIN_THREADS, 0, s, j));
+  JoinArgs j{a.partial, ctas, a.D, p->param_dtype, p->post_weight, p->post_bias, a.param[GATE], {}};
+  for (int q = 0; q < RN_GRADS; ++q) j.to[q] = to[q];
+  DGS_CUDA_TRY(launch_training(residual_norm_join_kernel, dim3(static_cast<unsigned>((p->D + 31) / 32)), RN_JOIN_THREADS, 0, s, j));
   return DGS_OK;
 }
