@@ -54,13 +54,21 @@ struct NormArgs {
 };
 enum { POST_WEIGHT, POST_BIAS, GATE, WEIGHT, BIAS };
 
-template <int TPR>
+// Threads of a CTA: as many as registers allow (64 a thread forward, 128 backward), so that several rows are under way beside one another
+// over one copy of the weights; rows narrower than a warp need few of them and take smaller CTAs.
+template <int TPR, bool BACK>
 constexpr int threads_of() {
-  return TPR > 32 ? TPR : 256;
+  return BACK ? 512 : TPR > 32 ? 1024 : 256;
 }
 
-// COUNT (up to 3) sums over the threads of a row, returned to all of them.  Every thread of the CTA calls it; `red` is not written again
-// before every thread has passed another such sum, or a barrier.
+// all threads of a row that several warps share
+template <int TPR>
+__device__ __forceinline__ void row_barrier() {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / TPR), "n"(TPR) : "memory");
+}
+
+// COUNT (up to 3) sums over the threads of a row, returned to all of them, who all call it; `red` is not written again before every one of
+// them has passed another such sum, or a barrier.
 template <int TPR, int COUNT>
 __device__ __forceinline__ void row_sums(float (&v)[COUNT], float4* red) {
 #pragma unroll
@@ -74,8 +82,8 @@ __device__ __forceinline__ void row_sums(float (&v)[COUNT], float4* red) {
 #pragma unroll
       for (int q = 0; q < COUNT; ++q) mine[q] = v[q];
     }
-    __syncthreads();
-    const float* other = reinterpret_cast<const float*>(red + (threadIdx.x & (WARPS - 1)));
+    row_barrier<TPR>();
+    const float* other = reinterpret_cast<const float*>(red + (threadIdx.x >> 5 & ~(WARPS - 1)) + (threadIdx.x & (WARPS - 1)));
 #pragma unroll
     for (int q = 0; q < COUNT; ++q) v[q] = other[q];
 #pragma unroll
@@ -100,9 +108,9 @@ __device__ __forceinline__ void fma_to(float* v, const float* a, const float* b)
 // Rows of up to COUNT arrays.  Vectors of 4, 8 or 16 bytes travel by cp.async through a ring in shared memory, so the next rows are on
 // their way while one is summed; a thread fetches what it will read itself, so its own wait is all the synchronisation.  Single
 // elements of two bytes are loaded where they are used.
-template <typename T, int VEC, int TPR, int E, int COUNT>
+template <typename T, int VEC, int TPR, int E, int COUNT, bool BACK>
 struct Feed {
-  static constexpr int NV = E / VEC, THREADS = threads_of<TPR>(), BYTES = VEC * static_cast<int>(sizeof(T));
+  static constexpr int NV = E / VEC, THREADS = threads_of<TPR, BACK>(), BYTES = VEC * static_cast<int>(sizeof(T));
   static constexpr bool kRing = BYTES >= 4;
   const NormArgs& a;
   const unsigned char* ring;
@@ -273,13 +281,13 @@ __device__ __forceinline__ void weigh(const FeedT& f, int weight, int bias, cons
 }
 
 template <typename T, int VEC, int TPR, int E>
-__global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int ROWS = threads_of<TPR>() / TPR;
+__global__ __launch_bounds__(threads_of<TPR, false>()) void residual_norm_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int ROWS = threads_of<TPR, false>() / TPR;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float4 red[4][32];
   pdl_enter();
   const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
-  Feed<T, VEC, TPR, E, 3> f{a};
+  Feed<T, VEC, TPR, E, 3, false> f{a};
   const int64_t mine = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / TPR;
   f.begin(mine, step, smem + a.ring_at);
   f.lay_out(smem);
@@ -333,7 +341,7 @@ __global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_kernel(const 
     }
     if constexpr (TPR > 32) {
       // (a row with one sum alone: `red` must not be written before all have read it)
-      if ((a.post != DGS_NORM_NONE) + (a.post == DGS_NORM_LAYER) + (a.pre != DGS_NORM_NONE) + (a.pre == DGS_NORM_LAYER) == 1) __syncthreads();
+      if ((a.post != DGS_NORM_NONE) + (a.post == DGS_NORM_LAYER) + (a.pre != DGS_NORM_NONE) + (a.pre == DGS_NORM_LAYER) == 1) row_barrier<TPR>();
     }
   }
 }
@@ -366,13 +374,13 @@ __device__ __forceinline__ void norm_back(const FeedT& f, bool layer, int D, flo
 }
 
 template <typename T, int VEC, int TPR, int E>
-__global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int THREADS = threads_of<TPR>(), ROWS = THREADS / TPR;
+__global__ __launch_bounds__(threads_of<TPR, true>()) void residual_norm_backward_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int THREADS = threads_of<TPR, true>(), ROWS = THREADS / TPR;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float4 red[2][32];
   pdl_enter();
   const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
-  Feed<T, VEC, TPR, E, 5> f{a};
+  Feed<T, VEC, TPR, E, 5, true> f{a};
   const int64_t mine = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / TPR;
   f.begin(mine, step, smem + a.ring_at);
   f.lay_out(smem);
@@ -501,7 +509,7 @@ __global__ __launch_bounds__(threads_of<TPR>()) void residual_norm_backward_kern
     if (a.row_gate != nullptr && a.dgate != nullptr && there && f.t == 0) static_cast<T*>(a.dgate)[row] = from_float<T>(of_row);
     if constexpr (TPR > 32) {
       // (a row with one sum alone: `red` must not be written before all have read it)
-      if (!pre || (!post && a.row_gate == nullptr)) __syncthreads();
+      if (!pre || (!post && a.row_gate == nullptr)) row_barrier<TPR>();
     }
   }
   if (a.partial == nullptr) return;
@@ -578,7 +586,7 @@ int64_t partial_rows(int64_t n) {
 
 template <typename T, int VEC, int TPR, int E, bool BACK>
 int launch_rows(NormArgs a, int arrays, int* ctas, cudaStream_t s) {
-  constexpr int THREADS = threads_of<TPR>(), ROWS = THREADS / TPR, NV = E / VEC, BYTES = VEC * static_cast<int>(sizeof(T));
+  constexpr int THREADS = threads_of<TPR, BACK>(), ROWS = THREADS / TPR, NV = E / VEC, BYTES = VEC * static_cast<int>(sizeof(T));
   void (*kernel)(NormArgs);
   if constexpr (BACK) kernel = residual_norm_backward_kernel<T, VEC, TPR, E>;
   else kernel = residual_norm_kernel<T, VEC, TPR, E>;
@@ -592,8 +600,8 @@ int launch_rows(NormArgs a, int arrays, int* ctas, cudaStream_t s) {
     a.ring_at = 0;
     for (int& at : a.param_at) at = -1;
   }
-  // what a CTA has under way: half of an SM's shared memory where its registers hold two of them, else all
-  const int room = (THREADS <= 256 && !BACK ? RN_MAX_SMEM / 2 : RN_MAX_SMEM) - a.ring_at;
+  // what a CTA has under way: a quarter of an SM's shared memory where an SM holds four, else all
+  const int room = (THREADS <= 256 ? RN_MAX_SMEM / 4 : RN_MAX_SMEM) - a.ring_at;
   a.stages = a.stage_bytes == 0 ? 1 : a.stage_bytes * RN_MAX_STAGES <= room ? RN_MAX_STAGES : room / a.stage_bytes;
   if (a.stages < 2 && a.stage_bytes > 0) a.stages = (RN_MAX_SMEM - a.ring_at) / a.stage_bytes;  // (one CTA an SM, then)
   if (a.stages > RN_MAX_STAGES) a.stages = RN_MAX_STAGES;
@@ -781,6 +789,8 @@ extern "C" int dgs_residual_norm_backward(const dgs_residual_norm* p, const void
   a.dx = dx;
   a.dy = dy;
   a.dgate = column ? nullptr : dgate;
+  if (a.dgate == nullptr) a.param[POST_BIAS] = nullptr;  // (rows need it for their gate's gradient alone)
+  a.param[BIAS] = nullptr;
   a.partial = any ? static_cast<float*>(workspace) : nullptr;
   int arrays = 0, ctas = 0;
   for (const Source& in : a.in) arrays += in.p != nullptr;
