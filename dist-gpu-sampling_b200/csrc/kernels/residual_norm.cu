@@ -142,13 +142,18 @@ struct Feed {
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
   }
-  __device__ __forceinline__ void begin(int64_t row, int64_t apart, const unsigned char* smem) {
+  __device__ __forceinline__ void begin(int64_t row, int64_t apart, unsigned char* smem) {
     t = threadIdx.x % TPR;
     stage = 0;
     step = apart;
     ring = smem;
-    if constexpr (kRing)
+    if constexpr (kRing) {
+      // what lies behind a row's end is never fetched: zeros, once
+      if (TPR * E != a.D)
+        for (int at = threadIdx.x * 4; at < a.stages * a.stage_bytes; at += THREADS * 4) *reinterpret_cast<uint32_t*>(smem + at) = 0;
+      __syncthreads();
       for (int s = 0; s < a.stages - 1; ++s) issue(row + s * step, s);
+    }
     ahead = (a.stages - 1) * step;
   }
   // the rows `row` of this stage: asks for those `stages - 1` steps on, waits for these
@@ -164,18 +169,15 @@ struct Feed {
   __device__ __forceinline__ void done() {
     if constexpr (kRing) stage = stage + 1 == a.stages ? 0 : stage + 1;
   }
-  // array q's elements of the row (zeros outside); `slot`: how many arrays are there before it
+  // Array q's elements of the row, zeros behind its end; `slot`: how many arrays are there before it.  (A row that is not there: anything.)
   __device__ __forceinline__ void get(int q, int slot, int64_t row, bool there, float (&v)[E]) const {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float x[VEC];
-      if (there && in(k)) {
-        const T* p = kRing ? reinterpret_cast<const T*>(ring + stage * a.stage_bytes + ((slot * NV + k) * THREADS + threadIdx.x) * BYTES)
-                           : static_cast<const T*>(a.in[q].p) + row * a.in[q].stride + column(k);
-        load_vec<T, VEC>(p, x);
+      if constexpr (kRing) {
+        load_vec<T, VEC>(reinterpret_cast<const T*>(ring + stage * a.stage_bytes + ((slot * NV + k) * THREADS + threadIdx.x) * BYTES), x);
       } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[e] = 0.0f;
+        x[0] = there && in(k) ? to_float<T>((static_cast<const T*>(a.in[q].p) + row * a.in[q].stride)[column(k)]) : 0.0f;
       }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[k * VEC + e] = x[e];
@@ -396,13 +398,24 @@ __global__ __launch_bounds__(threads_of<TPR, true>()) void residual_norm_backwar
 #pragma unroll
     for (int i = 0; i < E; ++i) sums[q][i] = 0.0f;
   const bool pre = a.pre != DGS_NORM_NONE && a.in[2].p != nullptr, post = a.post != DGS_NORM_NONE, layer = a.pre == DGS_NORM_LAYER;
-  const bool columns = a.param[GATE] != nullptr;
+  const bool columns = a.param[GATE] != nullptr, post_layer = a.post == DGS_NORM_LAYER;
+  // a row's statistics, asked for a row ahead
+  float next[4] = {};
+  const auto ask = [&](int64_t row) {
+    if (row >= a.n) return;
+    if (pre) next[1] = a.rstd[row];
+    if (pre && layer) next[0] = a.mean[row];
+    if (post) next[3] = a.post_rstd[row];
+    if (post_layer) next[2] = a.post_mean[row];
+  };
+  ask(mine);
   for (int64_t row = mine; row - threadIdx.x / TPR < a.n; row += step) {
     f.next(row);
     const bool there = row < a.n;
     float g[E], h[E], w[E], none = 0.0f;
+    const float m = next[0], r = next[1], post_m = next[2], post_r = next[3];
+    ask(row + step);
     if (pre) {
-      const float m = there && layer ? a.mean[row] : 0.0f, r = there ? a.rstd[row] : 0.0f;
       f.get(0, slot[0], row, there, h);
       f.get(2, slot[2], row, there, g);
 #pragma unroll
@@ -411,10 +424,12 @@ __global__ __launch_bounds__(threads_of<TPR, true>()) void residual_norm_backwar
         mul_to(h + i, r, r);
       }
       f.zero_outside(h);
+      if (there) {
 #pragma unroll
-      for (int i = 0; i < E; i += 2) {
-        fma_to(sums[0] + i, g + i, h + i);
-        add_to(sums[1] + i, g[i], g[i + 1]);
+        for (int i = 0; i < E; i += 2) {
+          fma_to(sums[0] + i, g + i, h + i);
+          add_to(sums[1] + i, g[i], g[i + 1]);
+        }
       }
       if (a.param[WEIGHT] != nullptr) {
         f.param(WEIGHT, smem, w);
@@ -439,15 +454,12 @@ __global__ __launch_bounds__(threads_of<TPR, true>()) void residual_norm_backwar
       }
       f.put(a.dx, row, there, w);
     }
-    float r = 0.0f;
     f.get(1, slot[1], row, there, h);
     if (post) {
-      const float m = there && a.post == DGS_NORM_LAYER ? a.post_mean[row] : 0.0f;
-      r = there ? a.post_rstd[row] : 0.0f;
 #pragma unroll
       for (int i = 0; i < E; i += 2) {
-        if (a.post == DGS_NORM_LAYER) add_to(h + i, -m, -m);
-        mul_to(h + i, r, r);
+        if (post_layer) add_to(h + i, -post_m, -post_m);
+        mul_to(h + i, post_r, post_r);
       }
       f.zero_outside(h);
     }
@@ -481,7 +493,7 @@ __global__ __launch_bounds__(threads_of<TPR, true>()) void residual_norm_backwar
       for (int i = 0; i < E; i += 2) mul_to(g + i, by, by);
     }
     f.done();
-    if (post || columns) {
+    if (there && (post || columns)) {
 #pragma unroll
       for (int i = 0; i < E; i += 2) {
         fma_to(sums[2] + i, g + i, h + i);
@@ -499,7 +511,7 @@ __global__ __launch_bounds__(threads_of<TPR, true>()) void residual_norm_backwar
 #pragma unroll
         for (int i = 0; i < E; i += 2) mul_to(g + i, w[i], w[i + 1]);
       }
-      norm_back<TPR, E>(f, a.post == DGS_NORM_LAYER, a.D, r, h, g, &of_row, red[1]);
+      norm_back<TPR, E>(f, post_layer, a.D, post_r, h, g, &of_row, red[1]);
     } else if (a.row_gate != nullptr) {
       float s[1] = {of_row};
       row_sums<TPR, 1>(s, red[1]);
