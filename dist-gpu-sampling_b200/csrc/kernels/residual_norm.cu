@@ -240,6 +240,12 @@ struct Feed {
   }
 };
 
+// 1 / sqrt(v): the approximation and one step of Newton's method, r + r (1 - v r r) / 2, within two units in the last place
+__device__ __forceinline__ float inverse_root(float v) {
+  const float r = rsqrtf(v), e = fmaf(-v * r, r, 1.0f);
+  return v > 0.0f && v < INFINITY ? fmaf(0.5f * r, e, r) : r;
+}
+
 // normed values of v in place (zeros outside of the row); every thread of the CTA calls it
 template <int TPR, int E, typename FeedT>
 __device__ __forceinline__ void normalise(const FeedT& f, bool layer, int D, float eps, float (&v)[E], float* mean, float* rstd, float4 (*red)[32]) {
@@ -261,7 +267,7 @@ __device__ __forceinline__ void normalise(const FeedT& f, bool layer, int D, flo
   for (int i = 0; i < E; i += 2) fma_to(s, v + i, v + i);
   float t[1] = {s[0] + s[1]};
   row_sums<TPR, 1>(t, red[1]);
-  *rstd = 1.0f / sqrtf(fmaf(t[0], inv, eps));
+  *rstd = inverse_root(fmaf(t[0], inv, eps));
 #pragma unroll
   for (int i = 0; i < E; i += 2) mul_to(v + i, *rstd, *rstd);
 }
