@@ -67,48 +67,62 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
     if (threadIdx.x < 2 * PLAN_BUCKETS) bucket[threadIdx.x / PLAN_BUCKETS][threadIdx.x % PLAN_BUCKETS] = 0;
     __syncthreads();
   }
-  const int warps = gridDim.x * (PLAN_THREADS / 32);
-  for (int s = blockIdx.x * (PLAN_THREADS / 32) + warp; s < a.seqs; s += warps) {
-    const int64_t q0 = offset_at(a.q_offsets, a.offsets64, s), q1 = offset_at(a.q_offsets, a.offsets64, s + 1);
-    const int64_t k0 = offset_at(a.k_offsets, a.offsets64, s), k1 = offset_at(a.k_offsets, a.offsets64, s + 1);
-    AttnSeq e{0, 0, 0, 0};
-    if (q0 >= 0 && q0 <= q1 && q1 <= a.n_q && k0 >= 0 && k0 <= k1 && k1 <= a.n_k)
-      e = {static_cast<int32_t>(q0), static_cast<int32_t>(q1 - q0), static_cast<int32_t>(k0), static_cast<int32_t>(k1 - k0)};
-    else if (lane == 0)
-      raise_status(a.status, DGS_ERR_RANGE);
-    if (lane == 0) a.seq[s] = e;
-    for (int i = lane; i < e.q_len; i += 32) a.q_seq[e.q0 + i] = s;
-    if (backward)
-      for (int i = lane; i < e.k_len; i += 32) a.k_seq[e.k0 + i] = s;
-    if (attn_in_tiles(a, e)) {
-      const int nq = tiles_of(e.q_len, a.q_tile_rows), nk = backward ? tiles_of(e.k_len, ATTN_TILE) : 0;
-      if (alone) {  // counted first, placed below
-        for (int i = lane; i < nq; i += 32) atomicAdd(&bucket[0][bucket_of(query_tile(a, e, i).steps)], 1);
-        for (int i = lane; i < nk; i += 32) atomicAdd(&bucket[1][bucket_of(key_tile(a, e, i).steps)], 1);
-        continue;
-      }
-      int at[2] = {0, 0};
-      if (lane < 2) at[0] = atomicAdd(&a.counts[lane ? ATTN_N_K_TILES : ATTN_N_Q_TILES], lane ? nk : nq);
-      at[1] = __shfl_sync(FULL_MASK, at[0], 1);
-      at[0] = __shfl_sync(FULL_MASK, at[0], 0);
-      // (the bounds are of the sizes; offsets that overlap may get beyond them)
-      for (int i = lane; i < nq && at[0] + i < a.q_tile_bound; i += 32) a.q_tiles[at[0] + i] = query_tile(a, e, i);
-      for (int i = lane; i < nk && at[1] + i < a.k_tile_bound; i += 32) a.k_tiles[at[1] + i] = key_tile(a, e, i);
-      continue;
+  // each warp reads the offsets of up to 32 sequences at once and then takes them in turn
+  const int warps = gridDim.x * (PLAN_THREADS / 32), batch = min(32, (a.seqs + warps - 1) / warps);
+  int tiles = 0, single = 0, several = 0;  // sequences of each kind
+  for (int s0 = (blockIdx.x * (PLAN_THREADS / 32) + warp) * batch; s0 < a.seqs; s0 += warps * batch) {
+    const int mine = s0 + lane;
+    AttnSeq own{0, 0, 0, 0};
+    if (lane < batch && mine < a.seqs) {
+      const int64_t q0 = offset_at(a.q_offsets, a.offsets64, mine), q1 = offset_at(a.q_offsets, a.offsets64, mine + 1);
+      const int64_t k0 = offset_at(a.k_offsets, a.offsets64, mine), k1 = offset_at(a.k_offsets, a.offsets64, mine + 1);
+      if (q0 >= 0 && q0 <= q1 && q1 <= a.n_q && k0 >= 0 && k0 <= k1 && k1 <= a.n_k)
+        own = {static_cast<int32_t>(q0), static_cast<int32_t>(q1 - q0), static_cast<int32_t>(k0), static_cast<int32_t>(k1 - k0)};
+      else
+        raise_status(a.status, DGS_ERR_RANGE);
+      a.seq[mine] = own;
+      if (attn_in_tiles(a, own)) tiles = 1;
+      else if (attn_is_single(a, own)) single = 1;
+      else several = 1;
     }
-    if (attn_is_split(e) && e.q_len > 0) {
-      const int parts = (e.k_len + ATTN_SPLIT_KEYS - 1) / ATTN_SPLIT_KEYS, all = parts * e.q_len;
-      int first = 0;
-      if (lane == 0) first = atomicAdd(&a.counts[ATTN_N_SPLITS], all);
-      first = __shfl_sync(FULL_MASK, first, 0);
-      for (int i = lane; i < all; i += 32) {
-        const int row = i / parts, part = i - row * parts;
-        if (first + i >= a.split_bound) break;
-        a.splits[first + i] = make_int4(e.q0 + row, part * ATTN_SPLIT_KEYS, first + row * parts, parts);
-        for (int c = 0; c < a.kv_heads; ++c) a.arrived[static_cast<int64_t>(first + i) * a.kv_heads + c] = 0;
+    for (int n = 0; n < batch && s0 + n < a.seqs; ++n) {
+      const int s = s0 + n;
+      const AttnSeq e{__shfl_sync(FULL_MASK, own.q0, n), __shfl_sync(FULL_MASK, own.q_len, n), __shfl_sync(FULL_MASK, own.k0, n),
+                      __shfl_sync(FULL_MASK, own.k_len, n)};
+      for (int i = lane; i < e.q_len; i += 32) a.q_seq[e.q0 + i] = s;
+      if (backward)
+        for (int i = lane; i < e.k_len; i += 32) a.k_seq[e.k0 + i] = s;
+      if (attn_in_tiles(a, e)) {
+        const int nq = tiles_of(e.q_len, a.q_tile_rows), nk = backward ? tiles_of(e.k_len, ATTN_TILE) : 0;
+        if (alone) {  // counted first, placed below
+          for (int i = lane; i < nq; i += 32) atomicAdd(&bucket[0][bucket_of(query_tile(a, e, i).steps)], 1);
+          for (int i = lane; i < nk; i += 32) atomicAdd(&bucket[1][bucket_of(key_tile(a, e, i).steps)], 1);
+          continue;
+        }
+        int at[2] = {0, 0};
+        if (lane < 2) at[0] = atomicAdd(&a.counts[lane ? ATTN_N_K_TILES : ATTN_N_Q_TILES], lane ? nk : nq);
+        at[1] = __shfl_sync(FULL_MASK, at[0], 1);
+        at[0] = __shfl_sync(FULL_MASK, at[0], 0);
+        // (the bounds are of the sizes; offsets that overlap may get beyond them)
+        for (int i = lane; i < nq && at[0] + i < a.q_tile_bound; i += 32) a.q_tiles[at[0] + i] = query_tile(a, e, i);
+        for (int i = lane; i < nk && at[1] + i < a.k_tile_bound; i += 32) a.k_tiles[at[1] + i] = key_tile(a, e, i);
+      } else if (attn_is_split(e) && e.q_len > 0) {
+        const int parts = (e.k_len + ATTN_SPLIT_KEYS - 1) / ATTN_SPLIT_KEYS, all = parts * e.q_len;
+        int first = 0;
+        if (lane == 0) first = atomicAdd(&a.counts[ATTN_N_SPLITS], all);
+        first = __shfl_sync(FULL_MASK, first, 0);
+        for (int i = lane; i < all; i += 32) {
+          const int row = i / parts, part = i - row * parts;
+          if (first + i >= a.split_bound) break;
+          a.splits[first + i] = make_int4(e.q0 + row, part * ATTN_SPLIT_KEYS, first + row * parts, parts);
+          for (int c = 0; c < a.kv_heads; ++c) a.arrived[static_cast<int64_t>(first + i) * a.kv_heads + c] = 0;
+        }
       }
     }
   }
+  // which kinds there are: kernels for the others leave at once
+  const unsigned kinds = __reduce_or_sync(FULL_MASK, (tiles ? 1u << ATTN_HAS_TILES : 0u) | (single ? 1u << ATTN_HAS_SINGLE : 0u) | (several ? 1u << ATTN_HAS_SEVERAL : 0u));
+  if (lane == 0 && kinds != 0) atomicOr(&a.counts[ATTN_KINDS], static_cast<int>(kinds));
   if (!alone || !a.tiles) return;
   __syncthreads();
   if (warp < 2) {  // where each bucket begins
@@ -144,12 +158,32 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
   }
 }
 
-// ---- rows: a group of G lanes holds a row of DP elements, VEC of them a lane; a warp holds 32 / G keys at once ------------
+// ---- rows ------------------------------------------------------------------------------------------------------------
+// A row of DP elements lies in G lanes, VEC elements each.  A warp holds 32 / G of them side by side: `side` key heads of one key (which
+// lie side by side in memory too), and where there are fewer heads than that, several keys.
 template <typename T>
 constexpr int vec_of() {
   return 16 / static_cast<int>(sizeof(T));
 }
-constexpr int UNROLL = 4;
+template <typename T, int DP>
+constexpr int lanes_of() {
+  return DP / vec_of<T>();
+}
+
+template <typename T, int DP>
+struct Lanes {
+  static constexpr int G = lanes_of<T, DP>(), SLOTS = 32 / G;
+  int vec, head, key, keys;  // this lane's elements, its head of those side by side, its key; keys at once
+  bool in_d;
+  __device__ __forceinline__ Lanes(const AttnArgs& a) {
+    const int lane = threadIdx.x & 31, slot = lane / G;
+    vec = lane % G;
+    head = slot & (a.side - 1);
+    key = slot / a.side;
+    keys = SLOTS / a.side;
+    in_d = vec * vec_of<T>() < a.d;
+  }
+};
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_row(const T* p, bool there, float (&v)[VEC]) {
@@ -174,54 +208,51 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// The keys j0 + first, .. of one row, every `step` batches: running maximum (of log2 values), sum and weighted values of R heads, each
-// group of lanes with its own.
-template <typename T, int DP, int R>
-__device__ __forceinline__ void forward_keys(const T* k, int64_t k_row, const T* v, int64_t v_row, int j0, int j1, int step, bool in_d,
-                                             const float (&q)[R][vec_of<T>()], float (&m)[R], float (&l)[R], float (&acc)[R][vec_of<T>()]) {
-  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G;
-  const int sub = (threadIdx.x & 31) / G;
+// Keys j0, j0 + step, .. (U times as many as lie side by side at once) of one row: running maximum (of log2 values), sum and weighted values
+// of R heads.
+template <typename T, int DP, int R, int U>
+__device__ __forceinline__ void forward_keys(const T* k, int64_t k_row, const T* v, int64_t v_row, int j0, int j1, int step, const Lanes<T, DP>& w,
+                                             bool in, const float (&q)[R][vec_of<T>()], float (&m)[R], float (&l)[R], float (&acc)[R][vec_of<T>()]) {
+  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>();
   for (int j = j0; j < j1; j += step) {
-    Vec<T, VEC> kr[UNROLL], vr[UNROLL];
+    Vec<T, VEC> kr[U], vr[U];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int at = j + u * KEYS + sub;
-      const bool there = at < j1 && in_d;
+    for (int u = 0; u < U; ++u) {
+      const int at = j + u * w.keys + w.key;
+      const bool there = at < j1 && in;
       kr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(k + at * k_row) : Vec<T, VEC>{};
       vr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(v + at * v_row) : Vec<T, VEC>{};
     }
-    float x[R][UNROLL];
+    float x[R][U];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
+    for (int u = 0; u < U; ++u) {
       float kf[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) kf[e] = to_float<T>(kr[u].v[e]);
 #pragma unroll
       for (int r = 0; r < R; ++r) x[r][u] = group_sum<G>(dot<VEC>(q[r], kf));
     }
-    float scale[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float top = m[r];
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        if (j + u * KEYS + sub >= j1) x[r][u] = -INFINITY;
+      for (int u = 0; u < U; ++u) {
+        if (j + u * w.keys + w.key >= j1) x[r][u] = -INFINITY;
         top = fmaxf(top, x[r][u]);
       }
-      const float ref = top == -INFINITY ? 0.0f : top;
-      scale[r] = exp2f(m[r] - ref);
+      const float ref = top == -INFINITY ? 0.0f : top, scale = exp2f(m[r] - ref);
       m[r] = top;
-      l[r] *= scale[r];
+      l[r] *= scale;
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
+      for (int u = 0; u < U; ++u) {
         x[r][u] = exp2f(x[r][u] - ref);
         l[r] += x[r][u];
       }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[r][e] *= scale[r];
+      for (int e = 0; e < VEC; ++e) acc[r][e] *= scale;
     }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float f = to_float<T>(vr[u].v[e]);
@@ -231,39 +262,24 @@ __device__ __forceinline__ void forward_keys(const T* k, int64_t k_row, const T*
   }
 }
 
-// (m, l, acc) of two sets of keys joined
+// the lanes that hold the same elements of other keys joined: (m, l, acc) each
 template <int VEC>
-__device__ __forceinline__ void join(float& m, float& l, float (&acc)[VEC], float m2, float l2, const float (&acc2)[VEC]) {
-  const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
-  const float s1 = exp2f(m - ref), s2 = exp2f(m2 - ref);
-  l = l * s1 + l2 * s2;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) acc[e] = acc[e] * s1 + acc2[e] * s2;
-  m = top;
-}
-
-// the lanes that hold the same elements of other keys
-template <int G, int VEC>
-__device__ __forceinline__ void join_groups(float& m, float& l, float (&acc)[VEC]) {
-#pragma unroll
-  for (int o = G; o < 32; o <<= 1) {
-    float other[VEC];
+__device__ __forceinline__ void join_keys(int first, float& m, float& l, float (&acc)[VEC]) {
+  for (int o = first; o < 32; o <<= 1) {
     const float m2 = __shfl_xor_sync(FULL_MASK, m, o), l2 = __shfl_xor_sync(FULL_MASK, l, o);
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
+    const float s1 = exp2f(m - ref), s2 = exp2f(m2 - ref);
+    l = l * s1 + l2 * s2;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) other[e] = __shfl_xor_sync(FULL_MASK, acc[e], o);
-    join<VEC>(m, l, acc, m2, l2, other);
+    for (int e = 0; e < VEC; ++e) acc[e] = acc[e] * s1 + __shfl_xor_sync(FULL_MASK, acc[e], o) * s2;
+    m = top;
   }
 }
-
-template <typename T, int VEC>
-__device__ __forceinline__ void finish_row(const AttnArgs& a, int row, int head, int vec, bool writes, float m, float l, const float (&acc)[VEC]) {
-  if (!writes) return;
-  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (nan stays nan)
-  float o[VEC];
+template <int VEC>
+__device__ __forceinline__ void add_keys(int first, float (&v)[VEC]) {
+  for (int o = first; o < 32; o <<= 1)
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) o[e] = acc[e] * inv;
-  store_vec<T, VEC>(static_cast<T*>(a.out) + (static_cast<int64_t>(row) * a.heads + head) * a.d + vec * VEC, o);
-  if (vec == 0) a.lse[static_cast<int64_t>(head) * a.n_q + row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+    for (int e = 0; e < VEC; ++e) v[e] += __shfl_xor_sync(FULL_MASK, v[e], o);
 }
 
 // The sequence of a row, or none (a row outside of all of them)
@@ -286,43 +302,86 @@ __device__ __forceinline__ int keys_seen(const AttnArgs& a, const AttnSeq& e, in
   return n < 0 ? 0 : n < e.k_len ? n : e.k_len;
 }
 
-template <typename T, int DP, int R>
-__device__ __forceinline__ void load_heads(const AttnView& x, int row, int head0, int heads, int vec, bool in_d, float by,
-                                           float (&q)[R][vec_of<T>()]) {
+template <typename T, int R>
+__device__ __forceinline__ void load_heads(const AttnView& x, int row, int head0, int heads, int vec, bool in, float by, float (&q)[R][vec_of<T>()]) {
   constexpr int VEC = vec_of<T>();
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    load_row<T, VEC>(static_cast<const T*>(x.p) + row * x.row + (head0 + r) * x.head + vec * VEC, in_d && r < heads, q[r]);
+    load_row<T, VEC>(static_cast<const T*>(x.p) + row * x.row + (head0 + r) * x.head + vec * VEC, in && r < heads, q[r]);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) q[r][e] *= by;
   }
 }
 
-// A warp for each query row and key head, for the heads of its group R at a time; the first `split_ctas` CTAs take the parts of
-// rows with many keys, the last part of a row to be there joins them in their order.
-// Bound by HBM where every query has keys of its own.
+// Rows a.rows_at_once at a time: whose they are is looked up side by side, a lane a row; `f` gets those that `mine` names, one after another.
+template <typename Mine, typename F>
+__device__ __forceinline__ void each_row(const AttnArgs& a, int64_t task, int64_t tasks_step, int rows, int blocks, const int32_t* map, bool key,
+                                         const Mine& mine, const F& f) {
+  const int lane = threadIdx.x & 31;
+  const int64_t all = static_cast<int64_t>((rows + a.rows_at_once - 1) / a.rows_at_once) * blocks;
+  for (; task < all; task += tasks_step) {
+    const int batch = static_cast<int>(task / blocks), block = static_cast<int>(task - static_cast<int64_t>(batch) * blocks);
+    const int row = batch * a.rows_at_once + lane;
+    bool found = false, take = false;
+    AttnSeq e{0, 0, 0, 0};
+    if (lane < a.rows_at_once && row < rows) {
+      e = sequence_of(a, map, row, key, &found);
+      take = mine(e, found);
+    }
+    if (!found) e = AttnSeq{0, 0, 0, 0};
+    for (unsigned todo = __ballot_sync(FULL_MASK, take); todo != 0; todo &= todo - 1) {
+      const int n = __ffs(todo) - 1;
+      const AttnSeq x{__shfl_sync(FULL_MASK, e.q0, n), __shfl_sync(FULL_MASK, e.q_len, n), __shfl_sync(FULL_MASK, e.k0, n),
+                      __shfl_sync(FULL_MASK, e.k_len, n)};
+      f(batch * a.rows_at_once + n, block, x);
+    }
+  }
+}
+
+// What a CTA's warps found of a row's part, one head side by side after another: [warp][head][DP values, ..]
+template <typename T, int DP, int FLOATS>
+struct Shared {
+  float v[ROW_WARPS][Lanes<T, DP>::SLOTS][FLOATS];
+};
+
+// the last part of a row to be there: true for the CTA that takes all of them
+__device__ __forceinline__ bool last_part(const AttnArgs& a, const int4& it, int block, bool* flag) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0)
+    *flag = atomicAdd(&a.arrived[static_cast<int64_t>(it.z) * a.kv_heads + block], 1u) + 1 == static_cast<uint32_t>(it.w);
+  __syncthreads();
+  const bool last = *flag;
+  if (last) __threadfence();
+  return last;
+}
+
+// Forward.  Rows with up to ATTN_SPLIT_FROM keys: a warp each, for all the key heads side by side.  The first `split_ctas` CTAs take the
+// parts of rows with many keys; the last part of a row to be there joins them in their order.  Bound by HBM where every query has keys
+// of its own.
 template <typename T, int DP, int R>
-__global__ __launch_bounds__(ROW_WARPS * 32) void attn_rows_kernel(const __grid_constant__ AttnArgs a, int32_t split_ctas) {
-  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G;
-  __shared__ float shared[ROW_WARPS][DP + 2];
-  __shared__ bool last;
+__global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __grid_constant__ AttnArgs a, int32_t split_ctas) {
+  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = R == 4 ? 2 : 4, SPLIT_U = R == 1 ? 4 : 2;
+  __shared__ Shared<T, DP, DP + 2> shared;
+  __shared__ bool flag;
   pdl_enter();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vec = lane % G, group = a.heads / a.kv_heads;
-  const bool in_d = vec * VEC < a.d;
+  const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
+  const Lanes<T, DP> w(a);
   if (static_cast<int>(blockIdx.x) < split_ctas) {
     const int floats = a.d + 2, n = min(a.counts[ATTN_N_SPLITS], a.split_bound);
-    for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * a.kv_heads; t += split_ctas) {
-      const int item = static_cast<int>(t / a.kv_heads), c = static_cast<int>(t - static_cast<int64_t>(item) * a.kv_heads);
+    for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * blocks; t += split_ctas) {
+      const int item = static_cast<int>(t / blocks), block = static_cast<int>(t - static_cast<int64_t>(item) * blocks);
       const int4 it = a.splits[item];
       bool found;
       const AttnSeq e = sequence_of(a, a.q_seq, it.x, false, &found);
-      const int seen = found ? keys_seen(a, e, it.x) : 0, j0 = it.y, j1 = min(seen, j0 + ATTN_SPLIT_KEYS);
-      const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + vec * VEC;
-      const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + vec * VEC;
+      const int c = block * a.side + w.head, j0 = it.y, j1 = min(found ? keys_seen(a, e, it.x) : 0, j0 + ATTN_SPLIT_KEYS);
+      const bool in = w.in_d && c < a.kv_heads;
+      const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
+      const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
       for (int h0 = 0; h0 < group; h0 += R) {
         const int heads = min(R, group - h0);
         float q[R][VEC], m[R], l[R], acc[R][VEC];
-        load_heads<T, DP, R>(a.q, it.x, c * group + h0, heads, vec, in_d, a.scale * LOG2E, q);
+        load_heads<T, R>(a.q, it.x, c * group + h0, heads, w.vec, in, a.scale * LOG2E, q);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           m[r] = -INFINITY;
@@ -330,46 +389,39 @@ __global__ __launch_bounds__(ROW_WARPS * 32) void attn_rows_kernel(const __grid_
 #pragma unroll
           for (int x = 0; x < VEC; ++x) acc[r][x] = 0.0f;
         }
-        forward_keys<T, DP, R>(k, a.k.row, v, a.v.row, j0 + warp * KEYS * UNROLL, j1, ROW_WARPS * KEYS * UNROLL, in_d, q, m, l, acc);
+        forward_keys<T, DP, R, SPLIT_U>(k, a.k.row, v, a.v.row, j0 + warp * w.keys * SPLIT_U, j1, ROW_WARPS * w.keys * SPLIT_U, w, in, q, m, l, acc);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          join_groups<G, VEC>(m[r], l[r], acc[r]);
+          join_keys<VEC>(a.side * G, m[r], l[r], acc[r]);
           if (r >= heads) continue;  // (the same for all threads)
           __syncthreads();           // `shared` may be written again
-          if (lane < G) {
+          if (w.key == 0) {
+            float* to = shared.v[warp][w.head];
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) shared[warp][vec * VEC + x] = acc[r][x];
-            if (lane == 0) {
-              shared[warp][DP] = m[r];
-              shared[warp][DP + 1] = l[r];
-            }
+            for (int x = 0; x < VEC; ++x) to[w.vec * VEC + x] = acc[r][x];
+            if (w.vec == 0) to[DP] = m[r], to[DP + 1] = l[r];
           }
           __syncthreads();
           // the warps' parts, an element a thread
-          float top = -INFINITY;
+          for (int i = threadIdx.x; i < a.side * (a.d + 1); i += ROW_WARPS * 32) {
+            const int hs = i / (a.d + 1), x = i - hs * (a.d + 1), at = x < a.d ? x : DP + 1, kv = block * a.side + hs;
+            if (kv >= a.kv_heads) continue;
+            float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-          for (int w = 0; w < ROW_WARPS; ++w) top = fmaxf(top, shared[w][DP]);
-          const float ref = top == -INFINITY ? 0.0f : top;
-          float* part = a.parts + (static_cast<int64_t>(item) * a.heads + c * group + h0 + r) * floats;
-          for (int x = threadIdx.x; x <= a.d; x += ROW_WARPS * 32) {
-            const int at = x < a.d ? x : DP + 1;
-            float sum = 0.0f;
+            for (int y = 0; y < ROW_WARPS; ++y) top = fmaxf(top, shared.v[y][hs][DP]);
+            const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int w = 0; w < ROW_WARPS; ++w) sum += shared[w][at] * exp2f(shared[w][DP] - ref);
+            for (int y = 0; y < ROW_WARPS; ++y) sum += shared.v[y][hs][at] * exp2f(shared.v[y][hs][DP] - ref);
+            float* part = a.parts + (static_cast<int64_t>(item) * a.heads + kv * group + h0 + r) * floats;
             part[x < a.d ? x : a.d + 1] = sum;
             if (x == 0) part[a.d] = top;
           }
         }
       }
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0)
-        last = atomicAdd(&a.arrived[static_cast<int64_t>(it.z) * a.kv_heads + c], 1u) + 1 == static_cast<uint32_t>(it.w);
-      __syncthreads();
-      if (last && found) {
-        __threadfence();
-        for (int h = warp; h < group; h += ROW_WARPS) {
-          const int head = c * group + h;
+      if (last_part(a, it, block, &flag) && found) {
+        const int lane = threadIdx.x & 31, first = block * a.side * group, all = min(a.heads - first, a.side * group);
+        for (int h = warp; h < all; h += ROW_WARPS) {
+          const int head = first + h;
           const float* part = a.parts + (static_cast<int64_t>(it.z) * a.heads + head) * floats;
           const int64_t apart = static_cast<int64_t>(a.heads) * floats;
           float top = -INFINITY;
@@ -388,64 +440,152 @@ __global__ __launch_bounds__(ROW_WARPS * 32) void attn_rows_kernel(const __grid_
             for (int x = 0; x < DP / 32; ++x)
               if (x * 32 + lane < a.d) acc[x] += __ldcg(part + p * apart + x * 32 + lane) * by;
           }
+          const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (nan stays nan)
 #pragma unroll
-          for (int x = 0; x < DP / 32; ++x) {
-            const float one[1] = {acc[x]};
-            const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+          for (int x = 0; x < DP / 32; ++x)
             if (x * 32 + lane < a.d)
-              static_cast<T*>(a.out)[(static_cast<int64_t>(it.x) * a.heads + head) * a.d + x * 32 + lane] = from_float<T>(one[0] * inv);
-          }
+              static_cast<T*>(a.out)[(static_cast<int64_t>(it.x) * a.heads + head) * a.d + x * 32 + lane] = from_float<T>(acc[x] * inv);
           if (lane == 0) a.lse[static_cast<int64_t>(head) * a.n_q + it.x] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
         }
       }
-      __syncthreads();  // `last` may be written again
+      __syncthreads();  // `flag` may be written again
     }
     return;
   }
-  const int64_t t = static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp;
-  if (t >= static_cast<int64_t>(a.n_q) * a.kv_heads) return;
-  const int row = static_cast<int>(t / a.kv_heads), c = static_cast<int>(t - static_cast<int64_t>(row) * a.kv_heads);
-  bool found;
-  const AttnSeq e = sequence_of(a, a.q_seq, row, false, &found);
-  if (found && (attn_in_tiles(a, e) || attn_is_split(e))) return;
-  const int seen = found ? keys_seen(a, e, row) : 0;
-  const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + vec * VEC;
-  const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + vec * VEC;
-  for (int h0 = 0; h0 < group; h0 += R) {
-    const int heads = min(R, group - h0);
-    float q[R][VEC], m[R], l[R], acc[R][VEC];
-    load_heads<T, DP, R>(a.q, row, c * group + h0, heads, vec, in_d && seen > 0, a.scale * LOG2E, q);
+  const int64_t ctas = gridDim.x - split_ctas;
+  each_row(
+      a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
+      [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(e)); },
+      [&](int row, int block, const AttnSeq& e) {
+        const int seen = keys_seen(a, e, row), c = block * a.side + w.head;
+        const bool in = w.in_d && c < a.kv_heads;
+        const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
+        const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
+        for (int h0 = 0; h0 < group; h0 += R) {
+          const int heads = min(R, group - h0);
+          float q[R][VEC], m[R], l[R], acc[R][VEC];
+          load_heads<T, R>(a.q, row, c * group + h0, heads, w.vec, in && seen > 0, a.scale * LOG2E, q);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      m[r] = -INFINITY;
-      l[r] = 0.0f;
+          for (int r = 0; r < R; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
 #pragma unroll
-      for (int x = 0; x < VEC; ++x) acc[r][x] = 0.0f;
-    }
-    forward_keys<T, DP, R>(k, a.k.row, v, a.v.row, 0, seen, KEYS * UNROLL, in_d, q, m, l, acc);
+            for (int x = 0; x < VEC; ++x) acc[r][x] = 0.0f;
+          }
+          forward_keys<T, DP, R, U>(k, a.k.row, v, a.v.row, 0, seen, w.keys * U, w, in, q, m, l, acc);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      join_groups<G, VEC>(m[r], l[r], acc[r]);
-      finish_row<T, VEC>(a, row, c * group + h0 + r, vec, lane < G && in_d && r < heads, m[r], l[r], acc[r]);
-    }
-  }
+          for (int r = 0; r < R; ++r) {
+            join_keys<VEC>(a.side * G, m[r], l[r], acc[r]);
+            if (!(w.key == 0 && in && r < heads)) continue;
+            const int head = c * group + h0 + r;
+            const float inv = l[r] > 0.0f ? 1.0f / l[r] : (l[r] == 0.0f ? 0.0f : l[r]);
+            float o[VEC];
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) o[x] = acc[r][x] * inv;
+            store_vec<T, VEC>(static_cast<T*>(a.out) + (static_cast<int64_t>(row) * a.heads + head) * a.d + w.vec * VEC, o);
+            if (w.vec == 0) a.lse[static_cast<int64_t>(head) * a.n_q + row] = l[r] == 0.0f ? -INFINITY : (m[r] + log2f(l[r])) * LN2;
+          }
+        }
+      });
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------
-// Over some keys of one row, for R heads: sum p e k, sum p k (so that dq = scale (the first - delta times the second) takes one pass) and
-// sum p e = delta.  `ref`: log2-sum-exp of the row.
+// log2-sum-exp of a row; a row that had no finite score has no weights
+__device__ __forceinline__ float reference_of(const AttnArgs& a, int head, int row, bool there) {
+  const float lse = there ? a.lse[static_cast<int64_t>(head) * a.n_q + row] * LOG2E : 0.0f;
+  return lse == -INFINITY ? INFINITY : lse;
+}
+
+// Sequences of one query and few keys (a seed over its neighbours): nobody else reads these keys, so one pass over them gives all
+// three gradients.  A warp a query, delta = do.o from the stored result.  Bound by HBM: K and V read, dK and dV written.
 template <typename T, int DP, int R>
-__device__ __forceinline__ void backward_keys(const T* k, int64_t k_row, const T* v, int64_t v_row, int j0, int j1, int step, bool in_d,
-                                              const float (&q)[R][vec_of<T>()], const float (&g)[R][vec_of<T>()], const float (&ref)[R],
+__global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_single_backward_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = R == 1 ? 4 : 2;
+  pdl_enter();
+  if ((a.counts[ATTN_KINDS] >> ATTN_HAS_SINGLE & 1) == 0) return;
+  const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
+  const Lanes<T, DP> w(a);
+  each_row(
+      a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
+      [&](const AttnSeq& e, bool found) { return found && !attn_in_tiles(a, e) && attn_is_single(a, e); },
+      [&](int row, int block, const AttnSeq& e) {
+        const int seen = e.k_len, c = block * a.side + w.head;  // (the one query sees all keys, causal or not)
+        const bool in = w.in_d && c < a.kv_heads;
+        const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
+        const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
+        const int64_t to = (static_cast<int64_t>(e.k0) * a.kv_heads + c) * a.d + w.vec * VEC, to_row = static_cast<int64_t>(a.kv_heads) * a.d;
+        float q[R][VEC], g[R][VEC], dq[R][VEC], ref[R], delta[R];
+        load_heads<T, R>(a.q, row, c * group, group, w.vec, in && seen > 0, 1.0f, q);
+        load_heads<T, R>(a.dout, row, c * group, group, w.vec, in && seen > 0, 1.0f, g);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float o[VEC];
+          const bool there = in && seen > 0 && r < group;
+          load_row<T, VEC>(static_cast<const T*>(a.out) + (static_cast<int64_t>(row) * a.heads + c * group + r) * a.d + w.vec * VEC, there, o);
+          delta[r] = group_sum<G>(dot<VEC>(g[r], o));
+          ref[r] = reference_of(a, c * group + r, row, there);
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) dq[r][x] = 0.0f;
+        }
+        for (int j = 0; j < seen; j += w.keys * U) {
+          Vec<T, VEC> kr[U], vr[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int at = j + u * w.keys + w.key;
+            const bool there = at < seen && in;
+            kr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(k + at * a.k.row) : Vec<T, VEC>{};
+            vr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(v + at * a.v.row) : Vec<T, VEC>{};
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int at = j + u * w.keys + w.key;
+            float kf[VEC], vf[VEC], dk[VEC], dv[VEC];
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) {
+              kf[x] = to_float<T>(kr[u].v[x]);
+              vf[x] = to_float<T>(vr[u].v[x]);
+              dk[x] = dv[x] = 0.0f;
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              const float x = group_sum<G>(dot<VEC>(q[r], kf)) * (a.scale * LOG2E), y = group_sum<G>(dot<VEC>(g[r], vf));
+              const float p = at < seen && r < group ? exp2f(x - ref[r]) : 0.0f, ds = p * (y - delta[r]) * a.scale;
+#pragma unroll
+              for (int n = 0; n < VEC; ++n) {
+                dv[n] = fmaf(p, g[r][n], dv[n]);
+                dk[n] = fmaf(ds, q[r][n], dk[n]);
+                dq[r][n] = fmaf(ds, kf[n], dq[r][n]);
+              }
+            }
+            if (a.dk != nullptr && at < seen && in) {
+              store_vec<T, VEC>(static_cast<T*>(a.dk) + to + at * to_row, dk);
+              store_vec<T, VEC>(static_cast<T*>(a.dv) + to + at * to_row, dv);
+            }
+          }
+        }
+        if (a.dq == nullptr) return;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          add_keys<VEC>(a.side * G, dq[r]);
+          if (w.key == 0 && in && r < group)
+            store_vec<T, VEC>(static_cast<T*>(a.dq) + (static_cast<int64_t>(row) * a.heads + c * group + r) * a.d + w.vec * VEC, dq[r]);
+        }
+      });
+}
+
+// Over some keys of one row, for R heads: sum p e k, sum p k (so that dq = scale (the first - delta times the second) takes one pass) and
+// sum p e = delta.
+template <typename T, int DP, int R>
+__device__ __forceinline__ void backward_keys(const T* k, int64_t k_row, const T* v, int64_t v_row, int j0, int j1, int step, const Lanes<T, DP>& w,
+                                              bool in, const float (&q)[R][vec_of<T>()], const float (&g)[R][vec_of<T>()], const float (&ref)[R],
                                               float (&pek)[R][vec_of<T>()], float (&pk)[R][vec_of<T>()], float (&delta)[R]) {
-  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G, U = 2;
-  const int sub = (threadIdx.x & 31) / G;
+  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = 2;
   for (int j = j0; j < j1; j += step) {
     Vec<T, VEC> kr[U], vr[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int at = j + u * KEYS + sub;
-      const bool there = at < j1 && in_d;
+      const int at = j + u * w.keys + w.key;
+      const bool there = at < j1 && in;
       kr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(k + at * k_row) : Vec<T, VEC>{};
       vr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(v + at * v_row) : Vec<T, VEC>{};
     }
@@ -460,7 +600,7 @@ __device__ __forceinline__ void backward_keys(const T* k, int64_t k_row, const T
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float x = group_sum<G>(dot<VEC>(q[r], kf)), e = group_sum<G>(dot<VEC>(g[r], vf));
-        const float p = j + u * KEYS + sub < j1 ? exp2f(x - ref[r]) : 0.0f;
+        const float p = j + u * w.keys + w.key < j1 ? exp2f(x - ref[r]) : 0.0f;
         delta[r] = fmaf(p, e, delta[r]);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -471,183 +611,204 @@ __device__ __forceinline__ void backward_keys(const T* k, int64_t k_row, const T
     }
   }
 }
-template <int G, int VEC>
-__device__ __forceinline__ void add_groups(float (&v)[VEC]) {
-#pragma unroll
-  for (int o = G; o < 32; o <<= 1)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] += __shfl_xor_sync(FULL_MASK, v[e], o);
-}
-template <int G>
-__device__ __forceinline__ float add_groups(float v) {
-#pragma unroll
-  for (int o = G; o < 32; o <<= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
-  return v;
-}
 
-// dq and delta, in the shape of attn_rows_kernel
+// dq and delta of the rows of other sequences, in the shape of attn_rows_kernel
 template <typename T, int DP, int R>
-__global__ __launch_bounds__(ROW_WARPS * 32) void attn_rows_dq_kernel(const __grid_constant__ AttnArgs a, int32_t split_ctas) {
-  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G, U = 2;
-  __shared__ float shared[ROW_WARPS][2 * DP + 1];
-  __shared__ bool last;
+__global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const __grid_constant__ AttnArgs a, int32_t split_ctas) {
+  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = 2;
+  __shared__ Shared<T, DP, 2 * DP + 1> shared;
+  __shared__ bool flag;
   pdl_enter();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vec = lane % G, group = a.heads / a.kv_heads;
-  const bool in_d = vec * VEC < a.d;
-  const bool splits = static_cast<int>(blockIdx.x) < split_ctas;
-  const int n_splits = splits ? min(a.counts[ATTN_N_SPLITS], a.split_bound) : 0;
-  const int64_t tasks = splits ? static_cast<int64_t>(n_splits) * a.kv_heads : static_cast<int64_t>(a.n_q) * a.kv_heads;
-  const int64_t step = splits ? split_ctas : tasks;  // (a row's warp has one task)
-  for (int64_t t = splits ? blockIdx.x : static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp; t < tasks; t += step) {
-    const int item = static_cast<int>(t / a.kv_heads), c = static_cast<int>(t - static_cast<int64_t>(item) * a.kv_heads);
-    const int4 it = splits ? a.splits[item] : make_int4(item, 0, 0, 0);
-    const int row = it.x;
-    bool found;
-    const AttnSeq e = sequence_of(a, a.q_seq, row, false, &found);
-    if (!splits && found && (attn_in_tiles(a, e) || attn_is_split(e))) return;
-    const int seen = found ? keys_seen(a, e, row) : 0;
-    const int j0 = it.y, j1 = splits ? min(seen, j0 + ATTN_SPLIT_KEYS) : seen;
-    const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + vec * VEC;
-    const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + vec * VEC;
-    const int floats = 2 * a.d + 1;
-    for (int h0 = 0; h0 < group; h0 += R) {
-      const int heads = min(R, group - h0), head = c * group + h0;
-      float q[R][VEC], g[R][VEC], ref[R], pek[R][VEC], pk[R][VEC], delta[R];
-      load_heads<T, DP, R>(a.q, row, head, heads, vec, in_d && seen > 0, a.scale * LOG2E, q);
-      load_heads<T, DP, R>(a.dout, row, head, heads, vec, in_d && seen > 0, 1.0f, g);
+  const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
+  const Lanes<T, DP> w(a);
+  float q[R][VEC], g[R][VEC], ref[R], pek[R][VEC], pk[R][VEC], delta[R];
+  const auto begin = [&](int row, int head, int heads, bool in) {
+    load_heads<T, R>(a.q, row, head, heads, w.vec, in, a.scale * LOG2E, q);
+    load_heads<T, R>(a.dout, row, head, heads, w.vec, in, 1.0f, g);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        ref[r] = seen > 0 && r < heads ? a.lse[static_cast<int64_t>(head + r) * a.n_q + row] * LOG2E : 0.0f;
-        if (ref[r] == -INFINITY) ref[r] = INFINITY;  // (a row that had no finite score has no weights)
-        delta[r] = 0.0f;
+    for (int r = 0; r < R; ++r) {
+      ref[r] = reference_of(a, head + r, row, in && r < heads);
+      delta[r] = 0.0f;
 #pragma unroll
-        for (int x = 0; x < VEC; ++x) pek[r][x] = pk[r][x] = 0.0f;
+      for (int x = 0; x < VEC; ++x) pek[r][x] = pk[r][x] = 0.0f;
+    }
+  };
+  const auto add = [&](int r) {
+    add_keys<VEC>(a.side * G, pek[r]);
+    add_keys<VEC>(a.side * G, pk[r]);
+    float one[1] = {delta[r]};
+    add_keys<1>(a.side * G, one);
+    delta[r] = one[0];
+  };
+  if (static_cast<int>(blockIdx.x) < split_ctas) {
+    const int floats = 2 * a.d + 1, n = min(a.counts[ATTN_N_SPLITS], a.split_bound);
+    for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * blocks; t += split_ctas) {
+      const int item = static_cast<int>(t / blocks), block = static_cast<int>(t - static_cast<int64_t>(item) * blocks);
+      const int4 it = a.splits[item];
+      bool found;
+      const AttnSeq e = sequence_of(a, a.q_seq, it.x, false, &found);
+      const int c = block * a.side + w.head, j0 = it.y, j1 = min(found ? keys_seen(a, e, it.x) : 0, j0 + ATTN_SPLIT_KEYS);
+      const bool in = w.in_d && c < a.kv_heads;
+      const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
+      const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
+      for (int h0 = 0; h0 < group; h0 += R) {
+        const int heads = min(R, group - h0);
+        begin(it.x, c * group + h0, heads, in && j1 > 0);
+        backward_keys<T, DP, R>(k, a.k.row, v, a.v.row, j0 + warp * w.keys * U, j1, ROW_WARPS * w.keys * U, w, in, q, g, ref, pek, pk, delta);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          add(r);
+          if (r >= heads) continue;  // (the same for all threads)
+          __syncthreads();           // `shared` may be written again
+          if (w.key == 0) {
+            float* to = shared.v[warp][w.head];
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) {
+              to[w.vec * VEC + x] = pek[r][x];
+              to[DP + w.vec * VEC + x] = pk[r][x];
+            }
+            if (w.vec == 0) to[2 * DP] = delta[r];
+          }
+          __syncthreads();
+          for (int i = threadIdx.x; i < a.side * floats; i += ROW_WARPS * 32) {
+            const int hs = i / floats, x = i - hs * floats, at = x < a.d ? x : x < 2 * a.d ? DP + x - a.d : 2 * DP, kv = block * a.side + hs;
+            if (kv >= a.kv_heads) continue;
+            float sum = 0.0f;
+#pragma unroll
+            for (int y = 0; y < ROW_WARPS; ++y) sum += shared.v[y][hs][at];
+            a.parts[(static_cast<int64_t>(item) * a.heads + kv * group + h0 + r) * floats + x] = sum;
+          }
+        }
       }
-      backward_keys<T, DP, R>(k, a.k.row, v, a.v.row, splits ? j0 + warp * KEYS * U : 0, j1, (splits ? ROW_WARPS : 1) * KEYS * U, in_d, q, g,
-                              ref, pek, pk, delta);
+      if (last_part(a, it, block, &flag) && found) {
+        const int lane = threadIdx.x & 31, first = block * a.side * group, all = min(a.heads - first, a.side * group);
+        for (int h = warp; h < all; h += ROW_WARPS) {
+          const int head = first + h;
+          const float* part = a.parts + (static_cast<int64_t>(it.z) * a.heads + head) * floats;
+          const int64_t apart = static_cast<int64_t>(a.heads) * floats;
+          float sum = 0.0f, ek[DP / 32], pk1[DP / 32];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        add_groups<G, VEC>(pek[r]);
-        add_groups<G, VEC>(pk[r]);
-        delta[r] = add_groups<G>(delta[r]);
-        if (r >= heads) continue;  // (the same for all threads of a warp, and of a CTA where parts are added)
-        if (!splits) {
-          if (lane < G && in_d) {
+          for (int x = 0; x < DP / 32; ++x) ek[x] = pk1[x] = 0.0f;
+#pragma unroll 4
+          for (int p = 0; p < it.w; ++p) {
+            sum += __ldcg(part + p * apart + 2 * a.d);
+#pragma unroll
+            for (int x = 0; x < DP / 32; ++x)
+              if (x * 32 + lane < a.d) {
+                ek[x] += __ldcg(part + p * apart + x * 32 + lane);
+                pk1[x] += __ldcg(part + p * apart + a.d + x * 32 + lane);
+              }
+          }
+#pragma unroll
+          for (int x = 0; x < DP / 32; ++x)
+            if (x * 32 + lane < a.d && a.dq != nullptr)
+              static_cast<T*>(a.dq)[(static_cast<int64_t>(it.x) * a.heads + head) * a.d + x * 32 + lane] =
+                  from_float<T>(a.scale * fmaf(-sum, pk1[x], ek[x]));
+          if (lane == 0) a.delta[static_cast<int64_t>(head) * a.n_q + it.x] = sum;
+        }
+      }
+      __syncthreads();  // `flag` may be written again
+    }
+    return;
+  }
+  const int64_t ctas = gridDim.x - split_ctas;
+  each_row(
+      a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
+      [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(e) || attn_is_single(a, e)); },
+      [&](int row, int block, const AttnSeq& e) {
+        const int seen = keys_seen(a, e, row), c = block * a.side + w.head;
+        const bool in = w.in_d && c < a.kv_heads;
+        const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
+        const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
+        for (int h0 = 0; h0 < group; h0 += R) {
+          const int heads = min(R, group - h0), head = c * group + h0;
+          begin(row, head, heads, in && seen > 0);
+          backward_keys<T, DP, R>(k, a.k.row, v, a.v.row, 0, seen, w.keys * U, w, in, q, g, ref, pek, pk, delta);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            add(r);
+            if (!(w.key == 0 && in && r < heads)) continue;
             float dq[VEC];
 #pragma unroll
             for (int x = 0; x < VEC; ++x) dq[x] = a.scale * fmaf(-delta[r], pk[r][x], pek[r][x]);
             if (a.dq != nullptr)
-              store_vec<T, VEC>(static_cast<T*>(a.dq) + (static_cast<int64_t>(row) * a.heads + head + r) * a.d + vec * VEC, dq);
-            if (vec == 0) a.delta[static_cast<int64_t>(head + r) * a.n_q + row] = delta[r];
+              store_vec<T, VEC>(static_cast<T*>(a.dq) + (static_cast<int64_t>(row) * a.heads + head + r) * a.d + w.vec * VEC, dq);
+            if (w.vec == 0) a.delta[static_cast<int64_t>(head + r) * a.n_q + row] = delta[r];
           }
-          continue;
         }
-        __syncthreads();  // `shared` may be written again
-        if (lane < G) {
-#pragma unroll
-          for (int x = 0; x < VEC; ++x) {
-            shared[warp][vec * VEC + x] = pek[r][x];
-            shared[warp][DP + vec * VEC + x] = pk[r][x];
-          }
-          if (lane == 0) shared[warp][2 * DP] = delta[r];
-        }
-        __syncthreads();
-        float* part = a.parts + (static_cast<int64_t>(item) * a.heads + head + r) * floats;
-        for (int x = threadIdx.x; x < floats; x += ROW_WARPS * 32) {
-          const int at = x < a.d ? x : x < 2 * a.d ? DP + x - a.d : 2 * DP;
-          float sum = 0.0f;
-#pragma unroll
-          for (int w = 0; w < ROW_WARPS; ++w) sum += shared[w][at];
-          part[x] = sum;
-        }
-      }
-    }
-    if (!splits) return;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0)
-      last = atomicAdd(&a.arrived[static_cast<int64_t>(it.z) * a.kv_heads + c], 1u) + 1 == static_cast<uint32_t>(it.w);
-    __syncthreads();
-    if (last && found) {
-      __threadfence();
-      for (int h = warp; h < group; h += ROW_WARPS) {
-        const int head = c * group + h;
-        const float* part = a.parts + (static_cast<int64_t>(it.z) * a.heads + head) * floats;
-        const int64_t apart = static_cast<int64_t>(a.heads) * floats;
-        float delta = 0.0f, pek[DP / 32], pk[DP / 32];
-#pragma unroll
-        for (int x = 0; x < DP / 32; ++x) pek[x] = pk[x] = 0.0f;
-#pragma unroll 4
-        for (int p = 0; p < it.w; ++p) {
-          delta += __ldcg(part + p * apart + 2 * a.d);
-#pragma unroll
-          for (int x = 0; x < DP / 32; ++x)
-            if (x * 32 + lane < a.d) {
-              pek[x] += __ldcg(part + p * apart + x * 32 + lane);
-              pk[x] += __ldcg(part + p * apart + a.d + x * 32 + lane);
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < DP / 32; ++x)
-          if (x * 32 + lane < a.d && a.dq != nullptr)
-            static_cast<T*>(a.dq)[(static_cast<int64_t>(row) * a.heads + head) * a.d + x * 32 + lane] =
-                from_float<T>(a.scale * fmaf(-delta, pk[x], pek[x]));
-        if (lane == 0) a.delta[static_cast<int64_t>(head) * a.n_q + row] = delta;
-      }
-    }
-    __syncthreads();  // `last` may be written again
-  }
+      });
 }
 
-// dk and dv: a group of lanes for each key row and key head, over the queries that see it and the heads of its group
-template <typename T, int DP>
-__global__ __launch_bounds__(ROW_WARPS * 32) void attn_rows_dkv_kernel(const __grid_constant__ AttnArgs a) {
-  constexpr int VEC = vec_of<T>(), G = DP / VEC, KEYS = 32 / G;
+// dk and dv of the keys of other sequences: a slot of lanes for each key row and key head, over the queries that see it, the heads of its group R
+// at a time.  Keys that no sequence holds get zeros.
+template <typename T, int DP, int R>
+__global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dkv_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>();
   pdl_enter();
-  const int lane = threadIdx.x & 31, vec = lane % G, group = a.heads / a.kv_heads;
-  const bool in_d = vec * VEC < a.d;
-  const int64_t t = (static_cast<int64_t>(blockIdx.x) * ROW_WARPS + (threadIdx.x >> 5)) * KEYS + lane / G;
-  const bool here = t < static_cast<int64_t>(a.n_k) * a.kv_heads;
-  const int row = here ? static_cast<int>(t / a.kv_heads) : 0, c = here ? static_cast<int>(t - static_cast<int64_t>(row) * a.kv_heads) : 0;
-  bool found = false;
-  AttnSeq e{0, 0, 0, 0};
-  if (here) e = sequence_of(a, a.k_seq, row, true, &found);
-  const bool mine = here && !(found && attn_in_tiles(a, e));
-  int first = 0;  // query that sees this key first
-  if (a.causal) first = max(0, row - e.k0 - (e.k_len - e.q_len));
-  const int queries = mine && found ? max(0, e.q_len - first) : 0;
-  const int most = __reduce_max_sync(FULL_MASK, queries);
-  float k[VEC], v[VEC], dk[VEC], dv[VEC];
-  load_row<T, VEC>(static_cast<const T*>(a.k.p) + row * a.k.row + c * a.k.head + vec * VEC, in_d && queries > 0, k);
-  load_row<T, VEC>(static_cast<const T*>(a.v.p) + row * a.v.row + c * a.v.head + vec * VEC, in_d && queries > 0, v);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
+  const Lanes<T, DP> w(a);
+  const int64_t all = static_cast<int64_t>((a.n_k + a.rows_at_once - 1) / a.rows_at_once) * blocks;
+  for (int64_t task = static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp; task < all; task += static_cast<int64_t>(gridDim.x) * ROW_WARPS) {
+    const int batch = static_cast<int>(task / blocks), block = static_cast<int>(task - static_cast<int64_t>(batch) * blocks);
+    const int begin = batch * a.rows_at_once, mine = begin + lane;
+    bool found = false, take = false;
+    AttnSeq own{0, 0, 0, 0};
+    if (lane < a.rows_at_once && mine < a.n_k) {
+      own = sequence_of(a, a.k_seq, mine, true, &found);
+      take = !found || !(attn_in_tiles(a, own) || attn_is_single(a, own));
+      if (!found) own = AttnSeq{0, 0, 0, 0};
+    }
+    unsigned todo = __ballot_sync(FULL_MASK, take);
+    while (todo != 0) {
+      // as many of them as lie side by side
+      int n = -1;
+      for (int i = 0; i < w.keys && todo != 0; ++i, todo &= todo - 1)
+        if (i == w.key) n = __ffs(todo) - 1;
+      const int from = n < 0 ? 0 : n, row = begin + from, c = block * a.side + w.head;
+      const AttnSeq e{__shfl_sync(FULL_MASK, own.q0, from), __shfl_sync(FULL_MASK, own.q_len, from), __shfl_sync(FULL_MASK, own.k0, from),
+                      __shfl_sync(FULL_MASK, own.k_len, from)};
+      const bool here = n >= 0 && c < a.kv_heads, in = here && w.in_d;
+      const int first = a.causal ? max(0, row - e.k0 - (e.k_len - e.q_len)) : 0;  // query that sees this key first
+      const int queries = here ? max(0, e.q_len - first) : 0;
+      const int most = __reduce_max_sync(FULL_MASK, queries);
+      float k[VEC], v[VEC], dk[VEC], dv[VEC];
+      load_row<T, VEC>(static_cast<const T*>(a.k.p) + row * a.k.row + c * a.k.head + w.vec * VEC, in && queries > 0, k);
+      load_row<T, VEC>(static_cast<const T*>(a.v.p) + row * a.v.row + c * a.v.head + w.vec * VEC, in && queries > 0, v);
 #pragma unroll
-  for (int x = 0; x < VEC; ++x) dk[x] = dv[x] = 0.0f;
-  for (int i = 0; i < most; ++i) {
-    const bool on = i < queries;
-    const int at = e.q0 + first + (on ? i : 0);
-    for (int h = 0; h < group; ++h) {
-      const int head = c * group + h;
-      float q[VEC], g[VEC];
-      load_row<T, VEC>(static_cast<const T*>(a.q.p) + at * a.q.row + head * a.q.head + vec * VEC, in_d && on, q);
-      load_row<T, VEC>(static_cast<const T*>(a.dout.p) + at * a.dout.row + head * a.dout.head + vec * VEC, in_d && on, g);
-      float ref = on ? a.lse[static_cast<int64_t>(head) * a.n_q + at] : INFINITY;
-      const float delta = on ? a.delta[static_cast<int64_t>(head) * a.n_q + at] : 0.0f;
-      if (ref == -INFINITY) ref = INFINITY;
-      const float x = group_sum<G>(dot<VEC>(q, k)) * a.scale, e2 = group_sum<G>(dot<VEC>(g, v));
-      const float p = on ? exp2f((x - ref) * LOG2E) : 0.0f, ds = p * (e2 - delta);
+      for (int x = 0; x < VEC; ++x) dk[x] = dv[x] = 0.0f;
+      for (int i = 0; i < most; ++i) {
+        const bool on = i < queries;
+        const int at = e.q0 + first + (on ? i : 0);
+        for (int h0 = 0; h0 < group; h0 += R) {
+          const int heads = min(R, group - h0), head = c * group + h0;
+          float q[R][VEC], g[R][VEC], ref[R], delta[R];
+          load_heads<T, R>(a.q, at, head, heads, w.vec, in && on, 1.0f, q);
+          load_heads<T, R>(a.dout, at, head, heads, w.vec, in && on, 1.0f, g);
 #pragma unroll
-      for (int n = 0; n < VEC; ++n) {
-        dv[n] = fmaf(p, g[n], dv[n]);
-        dk[n] = fmaf(ds, q[n], dk[n]);
+          for (int r = 0; r < R; ++r) {
+            ref[r] = reference_of(a, head + r, at, here && on && r < heads);
+            delta[r] = here && on && r < heads ? a.delta[static_cast<int64_t>(head + r) * a.n_q + at] : 0.0f;
+          }
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float x = group_sum<G>(dot<VEC>(q[r], k)) * (a.scale * LOG2E), y = group_sum<G>(dot<VEC>(g[r], v));
+            const float p = on && r < heads ? exp2f(x - ref[r]) : 0.0f, ds = p * (y - delta[r]);
+#pragma unroll
+            for (int x2 = 0; x2 < VEC; ++x2) {
+              dv[x2] = fmaf(p, g[r][x2], dv[x2]);
+              dk[x2] = fmaf(ds, q[r][x2], dk[x2]);
+            }
+          }
+        }
       }
+      if (!in) continue;
+#pragma unroll
+      for (int x = 0; x < VEC; ++x) dk[x] *= a.scale;
+      const int64_t to = (static_cast<int64_t>(row) * a.kv_heads + c) * a.d + w.vec * VEC;
+      store_vec<T, VEC>(static_cast<T*>(a.dk) + to, dk);
+      store_vec<T, VEC>(static_cast<T*>(a.dv) + to, dv);
     }
   }
-  if (!mine || !in_d) return;
-#pragma unroll
-  for (int n = 0; n < VEC; ++n) dk[n] *= a.scale;
-  const int64_t to = (static_cast<int64_t>(row) * a.kv_heads + c) * a.d + vec * VEC;
-  store_vec<T, VEC>(static_cast<T*>(a.dk) + to, dk);
-  store_vec<T, VEC>(static_cast<T*>(a.dv) + to, dv);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -777,15 +938,41 @@ int split_ctas(const AttnArgs& a) {
   const int64_t tasks = static_cast<int64_t>(a.split_bound) * a.kv_heads, most = static_cast<int64_t>(sm_count()) * 4;
   return static_cast<int>(tasks < most ? tasks : most);
 }
-unsigned row_ctas(const AttnArgs& a) { return static_cast<unsigned>((static_cast<int64_t>(a.n_q) * a.kv_heads + ROW_WARPS - 1) / ROW_WARPS); }
+// CTAs for so many rows: enough to fill the SMs, which then take the rows in turn
+unsigned row_ctas(const AttnArgs& a, int64_t rows) {
+  const int64_t blocks = (a.kv_heads + a.side - 1) / a.side, tasks = (rows + a.rows_at_once - 1) / a.rows_at_once * blocks;
+  const int64_t need = (tasks + ROW_WARPS - 1) / ROW_WARPS, most = static_cast<int64_t>(sm_count()) * 16;
+  return static_cast<unsigned>(need < most ? need : most);
+}
+// how the lanes of a warp are shared out, and how many rows a warp looks up at once: more where there are rows enough for all warps
+template <typename T, int DP>
+AttnArgs with_lanes(AttnArgs a, int64_t rows) {
+  a.side = 1;
+  while (a.side < a.kv_heads && a.side < 32 / lanes_of<T, DP>()) a.side *= 2;
+  const int64_t warps = static_cast<int64_t>(sm_count()) * 32;
+  a.rows_at_once = 1;
+  while (a.rows_at_once < 8 && rows >= warps * 2 * a.rows_at_once) a.rows_at_once *= 2;
+  return a;
+}
 
 struct RowsForward {
   const AttnArgs& a;
   cudaStream_t s;
   template <typename T, int DP, int R>
   int run() const {
-    const int splits = split_ctas(a);
-    DGS_CUDA_TRY(launch_training(attn_rows_kernel<T, DP, R>, dim3(splits + row_ctas(a)), ROW_WARPS * 32, 0, s, a, splits));
+    const AttnArgs b = with_lanes<T, DP>(a, a.n_q);
+    const int splits = split_ctas(b);
+    DGS_CUDA_TRY(launch_training(attn_rows_kernel<T, DP, R>, dim3(splits + row_ctas(b, b.n_q)), ROW_WARPS * 32, 0, s, b, splits));
+    return DGS_OK;
+  }
+};
+struct RowsSingle {
+  const AttnArgs& a;
+  cudaStream_t s;
+  template <typename T, int DP, int R>
+  int run() const {
+    const AttnArgs b = with_lanes<T, DP>(a, a.n_q);
+    DGS_CUDA_TRY(launch_training(attn_single_backward_kernel<T, DP, R>, dim3(row_ctas(b, b.n_q)), ROW_WARPS * 32, 0, s, b));
     return DGS_OK;
   }
 };
@@ -794,13 +981,12 @@ struct RowsBackward {
   cudaStream_t s;
   template <typename T, int DP, int R>
   int run() const {
-    const int splits = split_ctas(a);
-    DGS_CUDA_TRY(launch_training(attn_rows_dq_kernel<T, DP, R>, dim3(splits + row_ctas(a)), ROW_WARPS * 32, 0, s, a, splits));
-    if (a.dk == nullptr || a.n_k == 0) return DGS_OK;
-    constexpr int rows = ROW_WARPS * 32 / (DP / vec_of<T>());
-    DGS_CUDA_TRY(launch_training(attn_rows_dkv_kernel<T, DP>,
-                                 dim3(static_cast<unsigned>((static_cast<int64_t>(a.n_k) * a.kv_heads + rows - 1) / rows)), ROW_WARPS * 32, 0,
-                                 s, a));
+    AttnArgs b = with_lanes<T, DP>(a, a.n_q);
+    const int splits = split_ctas(b);
+    DGS_CUDA_TRY(launch_training(attn_rows_dq_kernel<T, DP, R>, dim3(splits + row_ctas(b, b.n_q)), ROW_WARPS * 32, 0, s, b, splits));
+    if (b.dk == nullptr || b.n_k == 0) return DGS_OK;
+    b = with_lanes<T, DP>(a, a.n_k);
+    DGS_CUDA_TRY(launch_training(attn_rows_dkv_kernel<T, DP, R>, dim3(row_ctas(b, b.n_k)), ROW_WARPS * 32, 0, s, b));
     return DGS_OK;
   }
 };
@@ -871,5 +1057,7 @@ extern "C" int dgs_attention_backward(const dgs_attention* p, const void* dout, 
   if (int rc = launch_plan(a, true, s)) return rc;
   if (a.tiles)
     if (int rc = attn_tiles_backward(a, p->dtype, s)) return rc;
+  if (a.heads / a.kv_heads <= ATTN_SINGLE_GROUP)
+    if (int rc = with_type<4>(p->dtype, a, RowsSingle{a, s})) return rc;
   return with_type<2>(p->dtype, a, RowsBackward{a, s});
 }

@@ -47,9 +47,11 @@ struct AttnArgs {
   float* norms;                 // [2] the largest row norms of dout and v (as they are ordered, through unsigned words)
   int32_t* status;
   int32_t split_bound, q_tile_bound, k_tile_bound, q_tile_rows;
+  int32_t side, rows_at_once;  // rows on the CUDA cores: key heads side by side in a warp, rows that it looks up at once
 };
 
-enum { ATTN_N_SPLITS = 0, ATTN_N_Q_TILES = 1, ATTN_N_K_TILES = 2, ATTN_COUNTS = 8 };
+enum { ATTN_N_SPLITS = 0, ATTN_N_Q_TILES = 1, ATTN_N_K_TILES = 2, ATTN_KINDS = 3, ATTN_COUNTS = 8 };
+enum { ATTN_HAS_TILES = 0, ATTN_HAS_SINGLE = 1, ATTN_HAS_SEVERAL = 2 };  // bits of the word ATTN_KINDS
 
 constexpr int ATTN_MAX_D = 128;
 constexpr int ATTN_SPLIT_FROM = 256;   // keys from which a CTA takes a row instead of a warp, ...
@@ -60,6 +62,11 @@ constexpr int ATTN_TILE_QUERIES = 48;  // queries from which a sequence goes to 
 constexpr int ATTN_TILE = 128;         // rows of a tile of keys, and of queries in the backward pass (twice as many in the forward one)
 
 __host__ __device__ inline bool attn_in_tiles(const AttnArgs& a, const AttnSeq& s) { return a.tiles && s.q_len >= ATTN_TILE_QUERIES && s.k_len > 0; }
+// one query over a few keys: its backward pass is one kernel (whose registers hold so many heads of a group)
+constexpr int ATTN_SINGLE_GROUP = 4;
+__host__ __device__ inline bool attn_is_single(const AttnArgs& a, const AttnSeq& s) {
+  return s.q_len == 1 && s.k_len <= ATTN_SPLIT_FROM && a.heads <= ATTN_SINGLE_GROUP * a.kv_heads;
+}
 __host__ __device__ inline bool attn_is_split(const AttnSeq& s) { return s.k_len > ATTN_SPLIT_FROM && s.q_len <= ATTN_SPLIT_QUERIES; }
 
 // attention_mma.cu: the sequences that attn_in_tiles names, after the plan

@@ -464,73 +464,83 @@ __device__ __forceinline__ float slope_scale(const AttnArgs& a) {
 
 constexpr int DELTA_THREADS = 256;
 
+// the sequence of a row is one of the tiles'
+__device__ __forceinline__ bool in_a_tile(const AttnArgs& a, const int32_t* map, int row, bool key) {
+  const int s = map[row];
+  if (s < 0 || s >= a.seqs) return false;
+  const AttnSeq e = a.seq[s];
+  const int at = row - (key ? e.k0 : e.q0);
+  return at >= 0 && at < (key ? e.k_len : e.q_len) && attn_in_tiles(a, e);
+}
+// the largest of a CTA's values, into a word of which values are ordered as unsigned words
+__device__ __forceinline__ void largest_of_cta(float v, float* to) {
+  __shared__ unsigned top;
+  if (threadIdx.x == 0) top = 0;
+  __syncthreads();
+  const unsigned w = __reduce_max_sync(FULL_MASK, __float_as_uint(v));
+  if ((threadIdx.x & 31) == 0 && w != 0) atomicMax(&top, w);
+  __syncthreads();
+  if (threadIdx.x == 0 && top != 0) atomicMax(reinterpret_cast<unsigned*>(to), top);
+}
+
 // Rows of the tiles' sequences: delta = do.o, lse in powers of two (less the lift), the largest norm of do.  16 lanes a row and head.
 template <typename T>
 __global__ __launch_bounds__(DELTA_THREADS) void attn_delta_kernel(const __grid_constant__ AttnArgs a, float down, int32_t norm) {
   pdl_enter();
+  if ((a.counts[ATTN_KINDS] >> ATTN_HAS_TILES & 1) == 0) return;
   const int lane = threadIdx.x % 16, head = blockIdx.y;
-  const int row = blockIdx.x * (DELTA_THREADS / 16) + threadIdx.x / 16;
-  bool mine = false;
-  if (row < a.n_q) {
-    const int s = a.q_seq[row];
-    if (s >= 0 && s < a.seqs) {
-      const AttnSeq e = a.seq[s];
-      mine = row >= e.q0 && row - e.q0 < e.q_len && attn_in_tiles(a, e);
+  float top = 0.0f;
+  for (int row0 = blockIdx.x * (DELTA_THREADS / 16); row0 < a.n_q; row0 += gridDim.x * (DELTA_THREADS / 16)) {
+    const int row = row0 + threadIdx.x / 16;
+    const bool mine = row < a.n_q && in_a_tile(a, a.q_seq, row, false);
+    float sum = 0.0f, square = 0.0f;
+    if (mine && lane * 8 < a.d) {
+      float x[8], y[8];
+      load_vec<T, 8>(static_cast<const T*>(a.dout.p) + row * a.dout.row + head * a.dout.head + lane * 8, x);
+      load_vec<T, 8>(static_cast<const T*>(a.out) + (static_cast<int64_t>(row) * a.heads + head) * a.d + lane * 8, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sum = fmaf(x[i], y[i], sum);
+        square = fmaf(x[i], x[i], square);
+      }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(FULL_MASK, sum, o);
+      square += __shfl_xor_sync(FULL_MASK, square, o);
+    }
+    if (mine && lane == 0) {
+      const int64_t at = static_cast<int64_t>(head) * a.n_q + row;
+      const float lse = a.lse[at];
+      a.delta[at] = sum;
+      a.lse2[at] = lse == -INFINITY ? INFINITY : lse * LOG2E - down;  // (a row that sees no key has no weights)
+      top = fmaxf(top, sqrtf(square));
     }
   }
-  float sum = 0.0f, square = 0.0f;
-  if (mine && lane * 8 < a.d) {
-    float x[8], y[8];
-    load_vec<T, 8>(static_cast<const T*>(a.dout.p) + row * a.dout.row + head * a.dout.head + lane * 8, x);
-    load_vec<T, 8>(static_cast<const T*>(a.out) + (static_cast<int64_t>(row) * a.heads + head) * a.d + lane * 8, y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum = fmaf(x[i], y[i], sum);
-      square = fmaf(x[i], x[i], square);
-    }
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(FULL_MASK, sum, o);
-    square += __shfl_xor_sync(FULL_MASK, square, o);
-  }
-  if (mine && lane == 0) {
-    const int64_t at = static_cast<int64_t>(head) * a.n_q + row;
-    const float lse = a.lse[at];
-    a.delta[at] = sum;
-    a.lse2[at] = lse == -INFINITY ? INFINITY : lse * LOG2E - down;  // (a row that sees no key has no weights)
-  }
-  if (norm) {
-    const unsigned top = __reduce_max_sync(FULL_MASK, mine ? __float_as_uint(sqrtf(square)) : 0u);
-    if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(reinterpret_cast<unsigned*>(a.norms), top);
-  }
+  if (norm) largest_of_cta(top, a.norms);
 }
 
 // the largest norm of v over all rows of the tiles' sequences
 template <typename T>
 __global__ __launch_bounds__(DELTA_THREADS) void attn_norm_kernel(const __grid_constant__ AttnArgs a) {
   pdl_enter();
+  if ((a.counts[ATTN_KINDS] >> ATTN_HAS_TILES & 1) == 0) return;
   const int lane = threadIdx.x % 16, head = blockIdx.y;
-  const int row = blockIdx.x * (DELTA_THREADS / 16) + threadIdx.x / 16;
-  bool mine = false;
-  if (row < a.n_k) {
-    const int s = a.k_seq[row];
-    if (s >= 0 && s < a.seqs) {
-      const AttnSeq e = a.seq[s];
-      mine = row >= e.k0 && row - e.k0 < e.k_len && attn_in_tiles(a, e);
+  float top = 0.0f;
+  for (int row0 = blockIdx.x * (DELTA_THREADS / 16); row0 < a.n_k; row0 += gridDim.x * (DELTA_THREADS / 16)) {
+    const int row = row0 + threadIdx.x / 16;
+    float square = 0.0f;
+    if (row < a.n_k && lane * 8 < a.d && in_a_tile(a, a.k_seq, row, true)) {
+      float x[8];
+      load_vec<T, 8>(static_cast<const T*>(a.v.p) + row * a.v.row + head * a.v.head + lane * 8, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) square = fmaf(x[i], x[i], square);
     }
-  }
-  float square = 0.0f;
-  if (mine && lane * 8 < a.d) {
-    float x[8];
-    load_vec<T, 8>(static_cast<const T*>(a.v.p) + row * a.v.row + head * a.v.head + lane * 8, x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) square = fmaf(x[i], x[i], square);
+    for (int o = 8; o > 0; o >>= 1) square += __shfl_xor_sync(FULL_MASK, square, o);
+    top = fmaxf(top, sqrtf(square));
   }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) square += __shfl_xor_sync(FULL_MASK, square, o);
-  const unsigned top = __reduce_max_sync(FULL_MASK, mine ? __float_as_uint(sqrtf(square)) : 0u);
-  if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(reinterpret_cast<unsigned*>(a.norms) + 1, top);
+  largest_of_cta(top, a.norms + 1);
 }
 
 template <int DP>
@@ -1004,9 +1014,12 @@ int backward(const TileArgs& t, cudaStream_t s) {
   static std::atomic<bool> known[2][MAX_DEVICES] = {};
   const AttnArgs& a = t.a;
   using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
-  const auto ctas = [](int rows) { return static_cast<unsigned>((rows + DELTA_THREADS / 16 - 1) / (DELTA_THREADS / 16)); };
-  DGS_CUDA_TRY(launch_training(attn_delta_kernel<T>, dim3(ctas(a.n_q), a.heads), DELTA_THREADS, 0, s, a, lift<BF16>(), static_cast<int32_t>(!BF16)));
-  if (!BF16) DGS_CUDA_TRY(launch_training(attn_norm_kernel<T>, dim3(ctas(a.n_k), a.kv_heads), DELTA_THREADS, 0, s, a));
+  const auto ctas = [](int rows, int heads) {
+    const int need = (rows + DELTA_THREADS / 16 - 1) / (DELTA_THREADS / 16), most = (sm_count() * 8 + heads - 1) / heads;
+    return static_cast<unsigned>(need < most ? need : most);
+  };
+  DGS_CUDA_TRY(launch_training(attn_delta_kernel<T>, dim3(ctas(a.n_q, a.heads), a.heads), DELTA_THREADS, 0, s, a, lift<BF16>(), static_cast<int32_t>(!BF16)));
+  if (!BF16) DGS_CUDA_TRY(launch_training(attn_norm_kernel<T>, dim3(ctas(a.n_k, a.kv_heads), a.kv_heads), DELTA_THREADS, 0, s, a));
   if (a.dk != nullptr)
     if (int rc = launch_tiles(attn_dkv_kernel<DP, BF16>, t, static_cast<int64_t>(a.k_tile_bound) * a.kv_heads, BackwardShape<DP>::SMEM, known[0], s))
       return rc;
