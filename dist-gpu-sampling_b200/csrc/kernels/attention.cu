@@ -106,7 +106,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
         // (the bounds are of the sizes; offsets that overlap may get beyond them)
         for (int i = lane; i < nq && at[0] + i < a.q_tile_bound; i += 32) a.q_tiles[at[0] + i] = query_tile(a, e, i);
         for (int i = lane; i < nk && at[1] + i < a.k_tile_bound; i += 32) a.k_tiles[at[1] + i] = key_tile(a, e, i);
-      } else if (attn_is_split(e) && e.q_len > 0) {
+      } else if (attn_is_split(a, e) && e.q_len > 0) {
         const int parts = (e.k_len + ATTN_SPLIT_KEYS - 1) / ATTN_SPLIT_KEYS, all = parts * e.q_len;
         int first = 0;
         if (lane == 0) first = atomicAdd(&a.counts[ATTN_N_SPLITS], all);
@@ -455,7 +455,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
   const int64_t ctas = gridDim.x - split_ctas;
   each_row(
       a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
-      [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(e)); },
+      [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e)); },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = keys_seen(a, e, row), c = block * a.side + w.head;
         const bool in = w.in_d && c < a.kv_heads;
@@ -714,7 +714,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
   const int64_t ctas = gridDim.x - split_ctas;
   each_row(
       a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
-      [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(e) || attn_is_single(a, e)); },
+      [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e) || attn_is_single(a, e)); },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = keys_seen(a, e, row), c = block * a.side + w.head;
         const bool in = w.in_d && c < a.kv_heads;
@@ -845,10 +845,12 @@ int64_t lay_out(const dgs_attention& p, bool backward, char* base, AttnArgs* a) 
   a->parts = reinterpret_cast<float*>(at(int64_t(4) * a->split_bound * p.heads * floats));
   a->delta = reinterpret_cast<float*>(at(backward ? int64_t(4) * p.heads * p.n_q : 0));
   // (a scale that is not positive, which no model has, stays on the CUDA cores: the tiles take the largest score for the largest weight)
-  a->tiles = p.dtype != DGS_F32 && p.n_q >= ATTN_TILE_QUERIES && p.n_k > 0 && p.seqs > 0 && p.scale > 1e-30f;
-  a->q_tile_rows = backward ? ATTN_TILE : 2 * ATTN_TILE;
+  a->tiles = p.dtype != DGS_F32 && p.n_q >= ATTN_FEW_QUERIES && p.n_k > 0 && p.seqs > 0 && p.scale > 1e-30f;
+  // forward, a CTA's two tiles of queries: the same rows of two heads that share their keys, or neighbouring rows
+  a->head_pairs = p.heads / p.kv_heads % 2 == 0;
+  a->q_tile_rows = backward || a->head_pairs ? ATTN_TILE : 2 * ATTN_TILE;
   // tiles, whatever the offsets: rows / tile + 1 for each of the sequences that can be that long
-  const int64_t longest = p.n_q / ATTN_TILE_QUERIES, some = a->tiles ? (longest < p.seqs ? longest : p.seqs) : 0;
+  const int64_t longest = p.n_q / ATTN_FEW_QUERIES, some = a->tiles ? (longest < p.seqs ? longest : p.seqs) : 0;
   a->q_tile_bound = static_cast<int32_t>(a->tiles ? p.n_q / a->q_tile_rows + some : 0);
   a->k_tile_bound = static_cast<int32_t>(a->tiles && backward ? p.n_k / ATTN_TILE + some : 0);
   a->q_tiles = reinterpret_cast<AttnTile*>(at(a->q_tile_bound * static_cast<int64_t>(sizeof(AttnTile))));
@@ -948,7 +950,8 @@ unsigned row_ctas(const AttnArgs& a, int64_t rows) {
 template <typename T, int DP>
 AttnArgs with_lanes(AttnArgs a, int64_t rows) {
   a.side = 1;
-  while (a.side < a.kv_heads && a.side < 32 / lanes_of<T, DP>()) a.side *= 2;
+  if (a.n_k <= static_cast<int64_t>(ATTN_FEW_KEYS) * a.seqs)
+    while (a.side < a.kv_heads && a.side < 32 / lanes_of<T, DP>()) a.side *= 2;
   const int64_t warps = static_cast<int64_t>(sm_count()) * 32;
   a.rows_at_once = 1;
   while (a.rows_at_once < 8 && rows >= warps * 2 * a.rows_at_once) a.rows_at_once *= 2;

@@ -46,7 +46,7 @@ struct AttnArgs {
   float *delta, *lse2;  // [heads, n_q]; lse in powers of two, as the tiles' backward pass takes it
   float* norms;                 // [2] the largest row norms of dout and v (as they are ordered, through unsigned words)
   int32_t* status;
-  int32_t split_bound, q_tile_bound, k_tile_bound, q_tile_rows;
+  int32_t split_bound, q_tile_bound, k_tile_bound, q_tile_rows, head_pairs;
   int32_t side, rows_at_once;  // rows on the CUDA cores: key heads side by side in a warp, rows that it looks up at once
 };
 
@@ -57,17 +57,27 @@ constexpr int ATTN_MAX_D = 128;
 constexpr int ATTN_SPLIT_FROM = 256;   // keys from which a CTA takes a row instead of a warp, ...
 constexpr int ATTN_SPLIT_KEYS = 1024;  // ... so many at a time
 constexpr int ATTN_SPLIT_QUERIES = 16; // (with more queries there are warps enough)
-constexpr int ATTN_TILE_QUERIES = 48;  // queries from which a sequence goes to the tensor cores
+constexpr int ATTN_TILE = 128;         // rows of a tile of keys, and of queries
+constexpr int ATTN_TILE_QUERIES = 48;  // queries from which a sequence goes to the tensor cores whatever its keys, ...
+constexpr int ATTN_FEW_QUERIES = 8;    // ... or from which it does with so many pairs, unless there are keys enough to be split
+constexpr int ATTN_TILE_PAIRS = 2048, ATTN_MANY_KEYS = 4096;
+constexpr int ATTN_FEW_KEYS = 24;      // keys a sequence on average up to which a warp takes key heads side by side, beyond it takes keys
 
-constexpr int ATTN_TILE = 128;         // rows of a tile of keys, and of queries in the backward pass (twice as many in the forward one)
-
-__host__ __device__ inline bool attn_in_tiles(const AttnArgs& a, const AttnSeq& s) { return a.tiles && s.q_len >= ATTN_TILE_QUERIES && s.k_len > 0; }
+__host__ __device__ inline bool attn_many_keys(const AttnSeq& s) {
+  return s.k_len > ATTN_SPLIT_FROM && s.q_len <= ATTN_SPLIT_QUERIES && (s.q_len < ATTN_FEW_QUERIES || s.k_len > ATTN_MANY_KEYS);
+}
+__host__ __device__ inline bool attn_in_tiles(const AttnArgs& a, const AttnSeq& s) {
+  if (!a.tiles || s.k_len == 0 || s.q_len < ATTN_FEW_QUERIES) return false;
+  return s.q_len >= ATTN_TILE_QUERIES || (!attn_many_keys(s) && static_cast<int64_t>(s.q_len) * s.k_len >= ATTN_TILE_PAIRS);
+}
+__host__ __device__ inline bool attn_is_split(const AttnArgs& a, const AttnSeq& s) {
+  return s.k_len > ATTN_SPLIT_FROM && s.q_len <= ATTN_SPLIT_QUERIES && !attn_in_tiles(a, s);
+}
 // one query over a few keys: its backward pass is one kernel (whose registers hold so many heads of a group)
 constexpr int ATTN_SINGLE_GROUP = 4;
 __host__ __device__ inline bool attn_is_single(const AttnArgs& a, const AttnSeq& s) {
   return s.q_len == 1 && s.k_len <= ATTN_SPLIT_FROM && a.heads <= ATTN_SINGLE_GROUP * a.kv_heads;
 }
-__host__ __device__ inline bool attn_is_split(const AttnSeq& s) { return s.k_len > ATTN_SPLIT_FROM && s.q_len <= ATTN_SPLIT_QUERIES; }
 
 // attention_mma.cu: the sequences that attn_in_tiles names, after the plan
 int attn_tiles_forward(const AttnArgs& a, int32_t dtype, cudaStream_t s);

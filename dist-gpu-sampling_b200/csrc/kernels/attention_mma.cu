@@ -1,6 +1,7 @@
 // Attention of long sequences in 16 bits on the tensor cores (formulas: attention.cu).
 //
-// Forward: a CTA takes 256 queries of one head as two tiles of 128 and runs over the keys 128 at a time.
+// Forward: a CTA takes two tiles of 128 queries (the same rows of two heads that share their keys, or neighbouring rows of one head) and runs
+// over the keys 128 at a time.
 //   S = Q K^T           both operands out of shared memory, 128 columns of TMEM for each query tile
 //   P = exp2(S c - ref) a thread a row: TMEM -> registers -> TMEM, 16 bits, in S's place
 //   O += P V            P out of TMEM, V as it lies (its rows are the sum's index), O stays in TMEM for all keys
@@ -184,7 +185,8 @@ __device__ __forceinline__ AttnTile tile_at(const AttnTile* p) {
 template <int DP>
 struct ForwardShape {
   static constexpr int STAGES = DP == 128 ? 5 : 8;
-  static constexpr uint32_t RING = 2 * tile_bytes<DP>(), BARS = RING + STAGES * tile_bytes<DP>(), SMEM = BARS + 256;
+  static constexpr int QUERIES = DP == 128 ? 1 : 2;  // items whose queries fit: the next one's come while this one is worked on
+  static constexpr uint32_t QUERY_BYTES = 2 * tile_bytes<DP>(), RING = QUERIES * QUERY_BYTES, BARS = RING + STAGES * tile_bytes<DP>(), SMEM = BARS + 256;
 };
 
 // One tile's 128 scores of a row: read for the largest, read again for the weights, 32 columns at a time with the next 32 on their way
@@ -246,14 +248,15 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
   const AttnArgs& a = args.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t smem = smem_addr(smem_raw), bars = smem + Shape::BARS;
-  const uint32_t q_full = bars, q_empty = bars + 8, s_full = bars + 16, p_full = bars + 32, o_full = bars + 48, full = bars + 64,
+  constexpr int QUERIES = Shape::QUERIES;
+  const uint32_t q_full = bars, q_empty = bars + 16, s_full = bars + 32, p_full = bars + 48, o_full = bars + 64, full = bars + 80,
                  empty = full + 8 * STAGES, tmem_word = empty + 8 * STAGES;
   volatile int* dead = reinterpret_cast<volatile int*>(smem_raw + (tmem_word + 4 - smem));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    bar_init(q_full, LOAD_THREADS);
-    bar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      bar_init(q_full + 8 * i, LOAD_THREADS);
+      bar_init(q_empty + 8 * i, 1);
       bar_init(s_full + 8 * i, 1);
       bar_init(p_full + 8 * i, 128);
       bar_init(o_full + 8 * i, 1);
@@ -272,8 +275,8 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_word) : "memory");
   pdl_enter();
-  const int64_t items = static_cast<int64_t>(min(a.counts[ATTN_N_Q_TILES], a.q_tile_bound)) * a.heads;
-  const int group = a.heads / a.kv_heads;
+  const int group = a.heads / a.kv_heads, heads = a.head_pairs ? a.heads / 2 : a.heads;  // an item is a tile of queries and a head, or two of them
+  const int64_t items = static_cast<int64_t>(min(a.counts[ATTN_N_Q_TILES], a.q_tile_bound)) * heads;
   bool ok = true;
 
   if (warp > SOFTMAX_WARPS) {
@@ -284,11 +287,13 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
       Loader<DP, STAGES> load{smem + Shape::RING, full, empty, static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32, dead};
       int n = 0;  // items with keys so far
       for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-        const int index = static_cast<int>(item / a.heads), head = static_cast<int>(item - static_cast<int64_t>(index) * a.heads);
+        const int index = static_cast<int>(item / heads), head = static_cast<int>(item - static_cast<int64_t>(index) * heads) << a.head_pairs;
         const AttnTile x = tile_at(a.q_tiles + index);
         if (x.steps == 0) continue;
-        if (!(ok = !*dead && bar_wait(q_empty, (n & 1) ^ 1))) break;
-        load.boxes(smem, &args.q, head, x.row, &args.q, head, x.row + ATTN_TILE, x.rows > ATTN_TILE, q_full);
+        const int slot = n % QUERIES;
+        if (!(ok = !*dead && bar_wait(q_empty + 8 * slot, ((n / QUERIES) & 1) ^ 1))) break;
+        load.boxes(smem + slot * Shape::QUERY_BYTES, &args.q, head, x.row, &args.q, head + a.head_pairs, a.head_pairs ? x.row : x.row + ATTN_TILE,
+                   a.head_pairs || x.rows > ATTN_TILE, q_full + 8 * slot);
         // K0, V0, K1, V1, ..  (only V's rows are summed over)
         for (int j = 0; ok && j < x.steps; ++j) {
           const int at = j * ATTN_TILE;
@@ -310,7 +315,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
       uint32_t p_phase[2] = {0, 0};
       int n = 0;
       // O += P V of the tile of queries w, then S of the next keys
-      const auto step = [&](auto which, bool first, bool more) {
+      const auto step = [&](auto which, uint32_t q, bool first, bool more) {
         constexpr uint32_t w = decltype(which)::value;
         const uint32_t s = tmem + w * 128;
         if (*dead || !bar_wait(p_full + 8 * w, p_phase[w])) return false;
@@ -318,7 +323,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
         fence_after();
         product_columns<DP>(tmem + 256 + w * DP, s, 32, st.tile(1), by_columns, !first);
         if (more) {
-          product_rows<DP>(s, smem + w * tile_bytes<DP>(), st.tile(2), by_rows);
+          product_rows<DP>(s, q + w * tile_bytes<DP>(), st.tile(2), by_rows);
           mma_commit_one(s_full + 8 * w);
         } else {
           mma_commit_one(o_full + 8 * w);
@@ -328,28 +333,30 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
       using One = std::integral_constant<uint32_t, 0>;
       using Two = std::integral_constant<uint32_t, 1>;
       for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-        const AttnTile x = tile_at(a.q_tiles + item / a.heads);
+        const AttnTile x = tile_at(a.q_tiles + item / heads);
         if (x.steps == 0) continue;
-        const bool two = x.rows > ATTN_TILE;
-        if (!(ok = !*dead && bar_wait(q_full, n & 1) && st.ready(0))) break;
+        const bool two = a.head_pairs || x.rows > ATTN_TILE;
+        const int slot = n % QUERIES;
+        const uint32_t q = smem + slot * Shape::QUERY_BYTES;
+        if (!(ok = !*dead && bar_wait(q_full + 8 * slot, (n / QUERIES) & 1) && st.ready(0))) break;
         fence_after();
-        product_rows<DP>(tmem, smem, st.tile(0), by_rows);
+        product_rows<DP>(tmem, q, st.tile(0), by_rows);
         mma_commit_one(s_full);
         if (two) {
-          product_rows<DP>(tmem + 128, smem + tile_bytes<DP>(), st.tile(0), by_rows);
+          product_rows<DP>(tmem + 128, q + tile_bytes<DP>(), st.tile(0), by_rows);
           mma_commit_one(s_full + 8);
         }
         st.release(0);
         for (int j = 0; ok && j < x.steps; ++j) {
           const bool more = j + 1 < x.steps;
           if (!(ok = st.ready(1) && (!more || st.ready(2)))) break;
-          if (!(ok = step(One{}, j == 0, more) && (!two || step(Two{}, j == 0, more)))) break;
+          if (!(ok = step(One{}, q, j == 0, more) && (!two || step(Two{}, q, j == 0, more)))) break;
           st.release(1);
           if (more) st.release(2);
           st.advance(2);
         }
         if (!ok) break;
-        mma_commit_one(q_empty);
+        mma_commit_one(q_empty + 8 * slot);
         ++n;
       }
     }
@@ -360,18 +367,19 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
     const int w = warp / 4;
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const uint32_t s = tmem + w * 128 + lanes, o = tmem + 256 + w * DP + lanes;
-    const int mine = w * ATTN_TILE + warp % 4 * 32 + lane;
+    const int below = a.head_pairs ? 0 : w * ATTN_TILE, mine = below + warp % 4 * 32 + lane;  // rows of the item in front of this tile
     const float c = a.scale * LOG2E;
     // 2^4: weights of 16 bits that are far below a row's largest keep more of their digits
     constexpr float LIFT = BF16 ? 0.0f : 4.0f;
     int at = 0, o_at = 0;
     for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const int index = static_cast<int>(item / a.heads), head = static_cast<int>(item - static_cast<int64_t>(index) * a.heads);
+      const int index = static_cast<int>(item / heads);
+      const int head = (static_cast<int>(item - static_cast<int64_t>(index) * heads) << a.head_pairs) + (a.head_pairs ? w : 0);
       const AttnTile x = tile_at(a.q_tiles + index);
       const bool there = mine < x.rows;
       float l = 0.0f, ref = -INFINITY;
-      if (x.steps > 0 && w * ATTN_TILE < x.rows) {
-        const int first = a.causal ? x.seen + w * ATTN_TILE : x.others;  // keys that the first row of this tile sees
+      if (x.steps > 0 && below < x.rows) {
+        const int first = a.causal ? x.seen + below : x.others;  // keys that the first row of this tile sees
         const int seen = a.causal ? min(x.others, x.seen + mine) : x.others;
         for (int j = 0; j < x.steps; ++j) {
           if (!(ok = !*dead && bar_wait(s_full + 8 * w, at++ & 1))) break;
@@ -405,7 +413,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
         if (!(ok = !*dead && bar_wait(o_full + 8 * w, o_at++ & 1))) break;
         fence_after();
       }
-      if (w * ATTN_TILE >= x.rows) continue;
+      if (below >= x.rows) continue;
       const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (nan stays nan)
       char* to = static_cast<char*>(a.out) + ((static_cast<int64_t>(x.row + mine) * a.heads + head) * a.d) * 2;
 #pragma unroll
@@ -1005,7 +1013,7 @@ template <int DP, bool BF16>
 int forward(const TileArgs& t, cudaStream_t s) {
   static_assert(ForwardShape<DP>::SMEM <= MAX_SMEM, "shared memory");
   static std::atomic<bool> known[MAX_DEVICES] = {};
-  return launch_tiles(attn_forward_kernel<DP, BF16>, t, static_cast<int64_t>(t.a.q_tile_bound) * t.a.heads, ForwardShape<DP>::SMEM, known, s);
+  return launch_tiles(attn_forward_kernel<DP, BF16>, t, static_cast<int64_t>(t.a.q_tile_bound) * (t.a.head_pairs ? t.a.heads / 2 : t.a.heads), ForwardShape<DP>::SMEM, known, s);
 }
 
 template <int DP, bool BF16>
