@@ -173,14 +173,16 @@ constexpr int lanes_of() {
 template <typename T, int DP>
 struct Lanes {
   static constexpr int G = lanes_of<T, DP>(), SLOTS = 32 / G;
+  int side, blocks;          // key heads side by side, and how many times as many there are
   int vec, head, key, keys;  // this lane's elements, its head of those side by side, its key; keys at once
   bool in_d;
-  __device__ __forceinline__ Lanes(const AttnArgs& a) {
+  __device__ __forceinline__ Lanes(const AttnArgs& a, int heads_side_by_side) : side(heads_side_by_side) {
     const int lane = threadIdx.x & 31, slot = lane / G;
+    blocks = (a.kv_heads + side - 1) / side;
     vec = lane % G;
-    head = slot & (a.side - 1);
-    key = slot / a.side;
-    keys = SLOTS / a.side;
+    head = slot & (side - 1);
+    key = slot / side;
+    keys = SLOTS / side;
     in_d = vec * vec_of<T>() < a.d;
   }
 };
@@ -365,16 +367,18 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
   __shared__ Shared<T, DP, DP + 2> shared;
   __shared__ bool flag;
   pdl_enter();
-  const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
-  const Lanes<T, DP> w(a);
-  if (static_cast<int>(blockIdx.x) < split_ctas) {
+  const bool splits = static_cast<int>(blockIdx.x) < split_ctas;
+  const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
+  const Lanes<T, DP> w(a, splits ? a.split_side : a.side);
+  const int blocks = w.blocks;
+  if (splits) {
     const int floats = a.d + 2, n = min(a.counts[ATTN_N_SPLITS], a.split_bound);
     for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * blocks; t += split_ctas) {
       const int item = static_cast<int>(t / blocks), block = static_cast<int>(t - static_cast<int64_t>(item) * blocks);
       const int4 it = a.splits[item];
       bool found;
       const AttnSeq e = sequence_of(a, a.q_seq, it.x, false, &found);
-      const int c = block * a.side + w.head, j0 = it.y, j1 = min(found ? keys_seen(a, e, it.x) : 0, j0 + ATTN_SPLIT_KEYS);
+      const int c = block * w.side + w.head, j0 = it.y, j1 = min(found ? keys_seen(a, e, it.x) : 0, j0 + ATTN_SPLIT_KEYS);
       const bool in = w.in_d && c < a.kv_heads;
       const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
       const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
@@ -392,7 +396,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
         forward_keys<T, DP, R, SPLIT_U>(k, a.k.row, v, a.v.row, j0 + warp * w.keys * SPLIT_U, j1, ROW_WARPS * w.keys * SPLIT_U, w, in, q, m, l, acc);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          join_keys<VEC>(a.side * G, m[r], l[r], acc[r]);
+          join_keys<VEC>(w.side * G, m[r], l[r], acc[r]);
           if (r >= heads) continue;  // (the same for all threads)
           __syncthreads();           // `shared` may be written again
           if (w.key == 0) {
@@ -403,8 +407,8 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
           }
           __syncthreads();
           // the warps' parts, an element a thread
-          for (int i = threadIdx.x; i < a.side * (a.d + 1); i += ROW_WARPS * 32) {
-            const int hs = i / (a.d + 1), x = i - hs * (a.d + 1), at = x < a.d ? x : DP + 1, kv = block * a.side + hs;
+          for (int i = threadIdx.x; i < w.side * (a.d + 1); i += ROW_WARPS * 32) {
+            const int hs = i / (a.d + 1), x = i - hs * (a.d + 1), at = x < a.d ? x : DP + 1, kv = block * w.side + hs;
             if (kv >= a.kv_heads) continue;
             float top = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -419,7 +423,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
         }
       }
       if (last_part(a, it, block, &flag) && found) {
-        const int lane = threadIdx.x & 31, first = block * a.side * group, all = min(a.heads - first, a.side * group);
+        const int lane = threadIdx.x & 31, first = block * w.side * group, all = min(a.heads - first, w.side * group);
         for (int h = warp; h < all; h += ROW_WARPS) {
           const int head = first + h;
           const float* part = a.parts + (static_cast<int64_t>(it.z) * a.heads + head) * floats;
@@ -457,7 +461,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
       a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
       [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e)); },
       [&](int row, int block, const AttnSeq& e) {
-        const int seen = keys_seen(a, e, row), c = block * a.side + w.head;
+        const int seen = keys_seen(a, e, row), c = block * w.side + w.head;
         const bool in = w.in_d && c < a.kv_heads;
         const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
         const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
@@ -475,7 +479,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
           forward_keys<T, DP, R, U>(k, a.k.row, v, a.v.row, 0, seen, w.keys * U, w, in, q, m, l, acc);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            join_keys<VEC>(a.side * G, m[r], l[r], acc[r]);
+            join_keys<VEC>(w.side * G, m[r], l[r], acc[r]);
             if (!(w.key == 0 && in && r < heads)) continue;
             const int head = c * group + h0 + r;
             const float inv = l[r] > 0.0f ? 1.0f / l[r] : (l[r] == 0.0f ? 0.0f : l[r]);
@@ -504,12 +508,12 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_single_backward_kernel
   pdl_enter();
   if ((a.counts[ATTN_KINDS] >> ATTN_HAS_SINGLE & 1) == 0) return;
   const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
-  const Lanes<T, DP> w(a);
+  const Lanes<T, DP> w(a, a.side);
   each_row(
       a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
       [&](const AttnSeq& e, bool found) { return found && !attn_in_tiles(a, e) && attn_is_single(a, e); },
       [&](int row, int block, const AttnSeq& e) {
-        const int seen = e.k_len, c = block * a.side + w.head;  // (the one query sees all keys, causal or not)
+        const int seen = e.k_len, c = block * w.side + w.head;  // (the one query sees all keys, causal or not)
         const bool in = w.in_d && c < a.kv_heads;
         const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
         const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
@@ -566,7 +570,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_single_backward_kernel
         if (a.dq == nullptr) return;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          add_keys<VEC>(a.side * G, dq[r]);
+          add_keys<VEC>(w.side * G, dq[r]);
           if (w.key == 0 && in && r < group)
             store_vec<T, VEC>(static_cast<T*>(a.dq) + (static_cast<int64_t>(row) * a.heads + c * group + r) * a.d + w.vec * VEC, dq[r]);
         }
@@ -619,8 +623,10 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
   __shared__ Shared<T, DP, 2 * DP + 1> shared;
   __shared__ bool flag;
   pdl_enter();
-  const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
-  const Lanes<T, DP> w(a);
+  const bool splits = static_cast<int>(blockIdx.x) < split_ctas;
+  const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
+  const Lanes<T, DP> w(a, splits ? a.split_side : a.side);
+  const int blocks = w.blocks;
   float q[R][VEC], g[R][VEC], ref[R], pek[R][VEC], pk[R][VEC], delta[R];
   const auto begin = [&](int row, int head, int heads, bool in) {
     load_heads<T, R>(a.q, row, head, heads, w.vec, in, a.scale * LOG2E, q);
@@ -634,20 +640,20 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
     }
   };
   const auto add = [&](int r) {
-    add_keys<VEC>(a.side * G, pek[r]);
-    add_keys<VEC>(a.side * G, pk[r]);
+    add_keys<VEC>(w.side * G, pek[r]);
+    add_keys<VEC>(w.side * G, pk[r]);
     float one[1] = {delta[r]};
-    add_keys<1>(a.side * G, one);
+    add_keys<1>(w.side * G, one);
     delta[r] = one[0];
   };
-  if (static_cast<int>(blockIdx.x) < split_ctas) {
+  if (splits) {
     const int floats = 2 * a.d + 1, n = min(a.counts[ATTN_N_SPLITS], a.split_bound);
     for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * blocks; t += split_ctas) {
       const int item = static_cast<int>(t / blocks), block = static_cast<int>(t - static_cast<int64_t>(item) * blocks);
       const int4 it = a.splits[item];
       bool found;
       const AttnSeq e = sequence_of(a, a.q_seq, it.x, false, &found);
-      const int c = block * a.side + w.head, j0 = it.y, j1 = min(found ? keys_seen(a, e, it.x) : 0, j0 + ATTN_SPLIT_KEYS);
+      const int c = block * w.side + w.head, j0 = it.y, j1 = min(found ? keys_seen(a, e, it.x) : 0, j0 + ATTN_SPLIT_KEYS);
       const bool in = w.in_d && c < a.kv_heads;
       const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
       const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
@@ -670,8 +676,8 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
             if (w.vec == 0) to[2 * DP] = delta[r];
           }
           __syncthreads();
-          for (int i = threadIdx.x; i < a.side * floats; i += ROW_WARPS * 32) {
-            const int hs = i / floats, x = i - hs * floats, at = x < a.d ? x : x < 2 * a.d ? DP + x - a.d : 2 * DP, kv = block * a.side + hs;
+          for (int i = threadIdx.x; i < w.side * floats; i += ROW_WARPS * 32) {
+            const int hs = i / floats, x = i - hs * floats, at = x < a.d ? x : x < 2 * a.d ? DP + x - a.d : 2 * DP, kv = block * w.side + hs;
             if (kv >= a.kv_heads) continue;
             float sum = 0.0f;
 #pragma unroll
@@ -681,7 +687,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
         }
       }
       if (last_part(a, it, block, &flag) && found) {
-        const int lane = threadIdx.x & 31, first = block * a.side * group, all = min(a.heads - first, a.side * group);
+        const int lane = threadIdx.x & 31, first = block * w.side * group, all = min(a.heads - first, w.side * group);
         for (int h = warp; h < all; h += ROW_WARPS) {
           const int head = first + h;
           const float* part = a.parts + (static_cast<int64_t>(it.z) * a.heads + head) * floats;
@@ -716,7 +722,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
       a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
       [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e) || attn_is_single(a, e)); },
       [&](int row, int block, const AttnSeq& e) {
-        const int seen = keys_seen(a, e, row), c = block * a.side + w.head;
+        const int seen = keys_seen(a, e, row), c = block * w.side + w.head;
         const bool in = w.in_d && c < a.kv_heads;
         const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
         const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
@@ -746,7 +752,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dkv_kernel(const 
   constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>();
   pdl_enter();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
-  const Lanes<T, DP> w(a);
+  const Lanes<T, DP> w(a, a.side);
   const int64_t all = static_cast<int64_t>((a.n_k + a.rows_at_once - 1) / a.rows_at_once) * blocks;
   for (int64_t task = static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp; task < all; task += static_cast<int64_t>(gridDim.x) * ROW_WARPS) {
     const int batch = static_cast<int>(task / blocks), block = static_cast<int>(task - static_cast<int64_t>(batch) * blocks);
@@ -764,7 +770,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dkv_kernel(const 
       int n = -1;
       for (int i = 0; i < w.keys && todo != 0; ++i, todo &= todo - 1)
         if (i == w.key) n = __ffs(todo) - 1;
-      const int from = n < 0 ? 0 : n, row = begin + from, c = block * a.side + w.head;
+      const int from = n < 0 ? 0 : n, row = begin + from, c = block * w.side + w.head;
       const AttnSeq e{__shfl_sync(FULL_MASK, own.q0, from), __shfl_sync(FULL_MASK, own.q_len, from), __shfl_sync(FULL_MASK, own.k0, from),
                       __shfl_sync(FULL_MASK, own.k_len, from)};
       const bool here = n >= 0 && c < a.kv_heads, in = here && w.in_d;
@@ -949,9 +955,9 @@ unsigned row_ctas(const AttnArgs& a, int64_t rows) {
 // how the lanes of a warp are shared out, and how many rows a warp looks up at once: more where there are rows enough for all warps
 template <typename T, int DP>
 AttnArgs with_lanes(AttnArgs a, int64_t rows) {
-  a.side = 1;
-  if (a.n_k <= static_cast<int64_t>(ATTN_FEW_KEYS) * a.seqs)
-    while (a.side < a.kv_heads && a.side < 32 / lanes_of<T, DP>()) a.side *= 2;
+  a.split_side = 1;
+  while (a.split_side < a.kv_heads && a.split_side < 32 / lanes_of<T, DP>()) a.split_side *= 2;
+  a.side = a.n_k <= static_cast<int64_t>(ATTN_FEW_KEYS) * a.seqs ? a.split_side : 1;
   const int64_t warps = static_cast<int64_t>(sm_count()) * 32;
   a.rows_at_once = 1;
   while (a.rows_at_once < 8 && rows >= warps * 2 * a.rows_at_once) a.rows_at_once *= 2;

@@ -47,7 +47,8 @@ struct AttnArgs {
   float* norms;                 // [2] the largest row norms of dout and v (as they are ordered, through unsigned words)
   int32_t* status;
   int32_t split_bound, q_tile_bound, k_tile_bound, q_tile_rows, head_pairs;
-  int32_t side, rows_at_once;  // rows on the CUDA cores: key heads side by side in a warp, rows that it looks up at once
+  // rows on the CUDA cores: key heads side by side in a warp (and in those of a split row), rows that it looks up at once
+  int32_t side, split_side, rows_at_once;
 };
 
 enum { ATTN_N_SPLITS = 0, ATTN_N_Q_TILES = 1, ATTN_N_K_TILES = 2, ATTN_KINDS = 3, ATTN_COUNTS = 8 };
