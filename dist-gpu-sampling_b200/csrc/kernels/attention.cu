@@ -79,7 +79,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
       if (q0 >= 0 && q0 <= q1 && q1 <= a.n_q && k0 >= 0 && k0 <= k1 && k1 <= a.n_k)
         own = {static_cast<int32_t>(q0), static_cast<int32_t>(q1 - q0), static_cast<int32_t>(k0), static_cast<int32_t>(k1 - k0)};
       else
-        raise_status(a.status, DGS_ERR_RANGE);
+        raise_status(a.status, DGS_ERR_RANGE), several = 1;
       a.seq[mine] = own;
       if (attn_in_tiles(a, own)) tiles = 1;
       else if (attn_is_single(a, own)) single = 1;
@@ -141,19 +141,24 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
     if (lane == 0) a.counts[warp ? ATTN_N_K_TILES : ATTN_N_Q_TILES] = carry;
   }
   __syncthreads();
-  for (int s = warp; s < a.seqs; s += PLAN_THREADS / 32) {
-    const AttnSeq e = a.seq[s];
-    if (!attn_in_tiles(a, e)) continue;
-    for (int i = lane; i < tiles_of(e.q_len, a.q_tile_rows); i += 32) {
-      const AttnTile t = query_tile(a, e, i);
-      const int at = atomicAdd(&bucket[0][bucket_of(t.steps)], 1);
-      if (at < a.q_tile_bound) a.q_tiles[at] = t;
-    }
-    if (!backward) continue;
-    for (int i = lane; i < tiles_of(e.k_len, ATTN_TILE); i += 32) {
-      const AttnTile t = key_tile(a, e, i);
-      const int at = atomicAdd(&bucket[1][bucket_of(t.steps)], 1);
-      if (at < a.k_tile_bound) a.k_tiles[at] = t;
+  for (int s0 = warp * batch; s0 < a.seqs; s0 += warps * batch) {
+    AttnSeq own{0, 0, 0, 0};
+    if (lane < batch && s0 + lane < a.seqs) own = a.seq[s0 + lane];
+    for (unsigned todo = __ballot_sync(FULL_MASK, attn_in_tiles(a, own)); todo != 0; todo &= todo - 1) {
+      const int n = __ffs(todo) - 1;
+      const AttnSeq e{__shfl_sync(FULL_MASK, own.q0, n), __shfl_sync(FULL_MASK, own.q_len, n), __shfl_sync(FULL_MASK, own.k0, n),
+                      __shfl_sync(FULL_MASK, own.k_len, n)};
+      for (int i = lane; i < tiles_of(e.q_len, a.q_tile_rows); i += 32) {
+        const AttnTile t = query_tile(a, e, i);
+        const int at = atomicAdd(&bucket[0][bucket_of(t.steps)], 1);
+        if (at < a.q_tile_bound) a.q_tiles[at] = t;
+      }
+      if (!backward) continue;
+      for (int i = lane; i < tiles_of(e.k_len, ATTN_TILE); i += 32) {
+        const AttnTile t = key_tile(a, e, i);
+        const int at = atomicAdd(&bucket[1][bucket_of(t.steps)], 1);
+        if (at < a.k_tile_bound) a.k_tiles[at] = t;
+      }
     }
   }
 }
@@ -315,19 +320,33 @@ __device__ __forceinline__ void load_heads(const AttnView& x, int row, int head0
   }
 }
 
+// Rows that a kernel looks at: all, or, where every sequence is another kernel's, those outside of all sequences.
+struct Range {
+  int rows, skip_at, skip;
+  __device__ __forceinline__ int row(int i) const { return i < skip_at ? i : i + skip; }
+};
+__device__ __forceinline__ Range range_of(const AttnArgs& a, bool key) {
+  const int n = key ? a.n_k : a.n_q;
+  if (a.seqs == 0 || (a.counts[ATTN_KINDS] >> ATTN_HAS_SEVERAL & 1) != 0) return {n, n, 0};
+  // (the plan found all offsets in order)
+  const void* p = key ? a.k_offsets : a.q_offsets;
+  const int first = static_cast<int>(offset_at(p, a.offsets64, 0)), skip = static_cast<int>(offset_at(p, a.offsets64, a.seqs)) - first;
+  return {n - skip, first, skip};
+}
+
 // Rows a.rows_at_once at a time: whose they are is looked up side by side, a lane a row; `f` gets those that `mine` names, one after another.
 template <typename Mine, typename F>
-__device__ __forceinline__ void each_row(const AttnArgs& a, int64_t task, int64_t tasks_step, int rows, int blocks, const int32_t* map, bool key,
-                                         const Mine& mine, const F& f) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void each_row(const AttnArgs& a, int64_t task, int64_t tasks_step, const Range& range, int blocks, const int32_t* map,
+                                         bool key, const Mine& mine, const F& f) {
+  const int lane = threadIdx.x & 31, rows = range.rows;
   const int64_t all = static_cast<int64_t>((rows + a.rows_at_once - 1) / a.rows_at_once) * blocks;
   for (; task < all; task += tasks_step) {
     const int batch = static_cast<int>(task / blocks), block = static_cast<int>(task - static_cast<int64_t>(batch) * blocks);
-    const int row = batch * a.rows_at_once + lane;
+    const int at = batch * a.rows_at_once + lane;
     bool found = false, take = false;
     AttnSeq e{0, 0, 0, 0};
-    if (lane < a.rows_at_once && row < rows) {
-      e = sequence_of(a, map, row, key, &found);
+    if (lane < a.rows_at_once && at < rows) {
+      e = sequence_of(a, map, range.row(at), key, &found);
       take = mine(e, found);
     }
     if (!found) e = AttnSeq{0, 0, 0, 0};
@@ -335,7 +354,7 @@ __device__ __forceinline__ void each_row(const AttnArgs& a, int64_t task, int64_
       const int n = __ffs(todo) - 1;
       const AttnSeq x{__shfl_sync(FULL_MASK, e.q0, n), __shfl_sync(FULL_MASK, e.q_len, n), __shfl_sync(FULL_MASK, e.k0, n),
                       __shfl_sync(FULL_MASK, e.k_len, n)};
-      f(batch * a.rows_at_once + n, block, x);
+      f(range.row(batch * a.rows_at_once + n), block, x);
     }
   }
 }
@@ -458,7 +477,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
   }
   const int64_t ctas = gridDim.x - split_ctas;
   each_row(
-      a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
+      a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, Range{a.n_q, a.n_q, 0}, blocks, a.q_seq, false,
       [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e)); },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = keys_seen(a, e, row), c = block * w.side + w.head;
@@ -510,7 +529,8 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_single_backward_kernel
   const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
   const Lanes<T, DP> w(a, a.side);
   each_row(
-      a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
+      a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, Range{a.n_q, a.n_q, 0}, blocks,
+      a.q_seq, false,
       [&](const AttnSeq& e, bool found) { return found && !attn_in_tiles(a, e) && attn_is_single(a, e); },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = e.k_len, c = block * w.side + w.head;  // (the one query sees all keys, causal or not)
@@ -719,7 +739,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
   }
   const int64_t ctas = gridDim.x - split_ctas;
   each_row(
-      a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, a.n_q, blocks, a.q_seq, false,
+      a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, range_of(a, false), blocks, a.q_seq, false,
       [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e) || attn_is_single(a, e)); },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = keys_seen(a, e, row), c = block * w.side + w.head;
@@ -753,14 +773,15 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dkv_kernel(const 
   pdl_enter();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
   const Lanes<T, DP> w(a, a.side);
-  const int64_t all = static_cast<int64_t>((a.n_k + a.rows_at_once - 1) / a.rows_at_once) * blocks;
+  const Range range = range_of(a, true);
+  const int64_t all = static_cast<int64_t>((range.rows + a.rows_at_once - 1) / a.rows_at_once) * blocks;
   for (int64_t task = static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp; task < all; task += static_cast<int64_t>(gridDim.x) * ROW_WARPS) {
     const int batch = static_cast<int>(task / blocks), block = static_cast<int>(task - static_cast<int64_t>(batch) * blocks);
     const int begin = batch * a.rows_at_once, mine = begin + lane;
     bool found = false, take = false;
     AttnSeq own{0, 0, 0, 0};
-    if (lane < a.rows_at_once && mine < a.n_k) {
-      own = sequence_of(a, a.k_seq, mine, true, &found);
+    if (lane < a.rows_at_once && mine < range.rows) {
+      own = sequence_of(a, a.k_seq, range.row(mine), true, &found);
       take = !found || !(attn_in_tiles(a, own) || attn_is_single(a, own));
       if (!found) own = AttnSeq{0, 0, 0, 0};
     }
@@ -770,7 +791,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dkv_kernel(const 
       int n = -1;
       for (int i = 0; i < w.keys && todo != 0; ++i, todo &= todo - 1)
         if (i == w.key) n = __ffs(todo) - 1;
-      const int from = n < 0 ? 0 : n, row = begin + from, c = block * w.side + w.head;
+      const int from = n < 0 ? 0 : n, row = range.row(begin + from), c = block * w.side + w.head;
       const AttnSeq e{__shfl_sync(FULL_MASK, own.q0, from), __shfl_sync(FULL_MASK, own.q_len, from), __shfl_sync(FULL_MASK, own.k0, from),
                       __shfl_sync(FULL_MASK, own.k_len, from)};
       const bool here = n >= 0 && c < a.kv_heads, in = here && w.in_d;
@@ -906,6 +927,7 @@ AttnArgs arguments(const dgs_attention& p) {
   a.kv_heads = p.kv_heads;
   a.d = p.d;
   a.causal = p.causal != 0;
+  a.singles = p.n_q <= 2 * static_cast<int64_t>(p.seqs) && p.heads <= ATTN_SINGLE_GROUP * p.kv_heads;
   a.scale = p.scale;
   return a;
 }
@@ -954,13 +976,15 @@ unsigned row_ctas(const AttnArgs& a, int64_t rows) {
 }
 // how the lanes of a warp are shared out, and how many rows a warp looks up at once: more where there are rows enough for all warps
 template <typename T, int DP>
-AttnArgs with_lanes(AttnArgs a, int64_t rows) {
+AttnArgs with_lanes(AttnArgs a, int64_t rows, bool keys = false) {
   a.split_side = 1;
   while (a.split_side < a.kv_heads && a.split_side < 32 / lanes_of<T, DP>()) a.split_side *= 2;
   a.side = a.n_k <= static_cast<int64_t>(ATTN_FEW_KEYS) * a.seqs ? a.split_side : 1;
+  // (eight where rows are short; two, or a key for each slot of a warp, where they may take long)
   const int64_t warps = static_cast<int64_t>(sm_count()) * 32;
-  a.rows_at_once = 1;
-  while (a.rows_at_once < 8 && rows >= warps * 2 * a.rows_at_once) a.rows_at_once *= 2;
+  const int most = a.side > 1 ? 8 : keys ? 32 / lanes_of<T, DP>() : 2;
+  a.rows_at_once = keys && a.side == 1 ? most : 1;
+  while (a.rows_at_once < most && rows >= warps * 2 * a.rows_at_once) a.rows_at_once *= 2;
   return a;
 }
 
@@ -990,11 +1014,18 @@ struct RowsBackward {
   cudaStream_t s;
   template <typename T, int DP, int R>
   int run() const {
-    AttnArgs b = with_lanes<T, DP>(a, a.n_q);
+    const AttnArgs b = with_lanes<T, DP>(a, a.n_q);
     const int splits = split_ctas(b);
     DGS_CUDA_TRY(launch_training(attn_rows_dq_kernel<T, DP, R>, dim3(splits + row_ctas(b, b.n_q)), ROW_WARPS * 32, 0, s, b, splits));
-    if (b.dk == nullptr || b.n_k == 0) return DGS_OK;
-    b = with_lanes<T, DP>(a, a.n_k);
+    return DGS_OK;
+  }
+};
+struct KeysBackward {
+  const AttnArgs& a;
+  cudaStream_t s;
+  template <typename T, int DP, int R>
+  int run() const {
+    const AttnArgs b = with_lanes<T, DP>(a, a.n_k, true);
     DGS_CUDA_TRY(launch_training(attn_rows_dkv_kernel<T, DP, R>, dim3(row_ctas(b, b.n_k)), ROW_WARPS * 32, 0, s, b));
     return DGS_OK;
   }
@@ -1066,7 +1097,8 @@ extern "C" int dgs_attention_backward(const dgs_attention* p, const void* dout, 
   if (int rc = launch_plan(a, true, s)) return rc;
   if (a.tiles)
     if (int rc = attn_tiles_backward(a, p->dtype, s)) return rc;
-  if (a.heads / a.kv_heads <= ATTN_SINGLE_GROUP)
+  if (a.singles)
     if (int rc = with_type<4>(p->dtype, a, RowsSingle{a, s})) return rc;
-  return with_type<2>(p->dtype, a, RowsBackward{a, s});
+  if (int rc = with_type<2>(p->dtype, a, RowsBackward{a, s})) return rc;
+  return a.dk == nullptr || a.n_k == 0 ? DGS_OK : with_type<4>(p->dtype, a, KeysBackward{a, s});
 }

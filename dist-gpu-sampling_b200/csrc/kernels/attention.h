@@ -29,7 +29,8 @@ struct AttnArgs {
   AttnView q, k, v, dout;
   const void *q_offsets, *k_offsets;
   int32_t offsets64;
-  int32_t seqs, n_q, n_k, heads, kv_heads, d, causal, tiles;  // tiles: long sequences go to the tensor cores
+  int32_t seqs, n_q, n_k, heads, kv_heads, d, causal;
+  int32_t tiles, singles;  // whether long sequences go to the tensor cores, single queries to a kernel of their own
   float scale;
   // results: contiguous rows of `heads` (`kv_heads`) times d elements; lse and delta [heads, n_q]
   void* out;
@@ -74,10 +75,10 @@ __host__ __device__ inline bool attn_in_tiles(const AttnArgs& a, const AttnSeq& 
 __host__ __device__ inline bool attn_is_split(const AttnArgs& a, const AttnSeq& s) {
   return s.k_len > ATTN_SPLIT_FROM && s.q_len <= ATTN_SPLIT_QUERIES && !attn_in_tiles(a, s);
 }
-// one query over a few keys: its backward pass is one kernel (whose registers hold so many heads of a group)
+// one query over a few keys: its backward pass is one kernel (whose registers hold so many heads of a group), where most sequences are so
 constexpr int ATTN_SINGLE_GROUP = 4;
 __host__ __device__ inline bool attn_is_single(const AttnArgs& a, const AttnSeq& s) {
-  return s.q_len == 1 && s.k_len <= ATTN_SPLIT_FROM && a.heads <= ATTN_SINGLE_GROUP * a.kv_heads;
+  return a.singles && s.q_len == 1 && s.k_len <= ATTN_SPLIT_FROM;
 }
 
 // attention_mma.cu: the sequences that attn_in_tiles names, after the plan

@@ -491,38 +491,49 @@ __device__ __forceinline__ void largest_of_cta(float v, float* to) {
   if (threadIdx.x == 0 && top != 0) atomicMax(reinterpret_cast<unsigned*>(to), top);
 }
 
-// Rows of the tiles' sequences: delta = do.o, lse in powers of two (less the lift), the largest norm of do.  16 lanes a row and head.
-template <typename T>
+// Rows of the tiles' sequences: delta = do.o, lse in powers of two (less the lift), the largest norm of do.  A warp looks eight rows up side by
+// side and takes each of them with all its heads, LANES lanes a head.
+constexpr int DELTA_ROWS = 8;
+template <typename T, int LANES>
 __global__ __launch_bounds__(DELTA_THREADS) void attn_delta_kernel(const __grid_constant__ AttnArgs a, float down, int32_t norm) {
   pdl_enter();
   if ((a.counts[ATTN_KINDS] >> ATTN_HAS_TILES & 1) == 0) return;
-  const int lane = threadIdx.x % 16, head = blockIdx.y;
+  const int lane = threadIdx.x & 31, vec = lane % LANES, warps = gridDim.x * (DELTA_THREADS / 32);
+  constexpr int SIDE = 32 / LANES;
   float top = 0.0f;
-  for (int row0 = blockIdx.x * (DELTA_THREADS / 16); row0 < a.n_q; row0 += gridDim.x * (DELTA_THREADS / 16)) {
-    const int row = row0 + threadIdx.x / 16;
-    const bool mine = row < a.n_q && in_a_tile(a, a.q_seq, row, false);
-    float sum = 0.0f, square = 0.0f;
-    if (mine && lane * 8 < a.d) {
-      float x[8], y[8];
-      load_vec<T, 8>(static_cast<const T*>(a.dout.p) + row * a.dout.row + head * a.dout.head + lane * 8, x);
-      load_vec<T, 8>(static_cast<const T*>(a.out) + (static_cast<int64_t>(row) * a.heads + head) * a.d + lane * 8, y);
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x * (DELTA_THREADS / 32) + threadIdx.x / 32) * DELTA_ROWS; row0 < a.n_q;
+       row0 += static_cast<int64_t>(warps) * DELTA_ROWS) {
+    const bool mine = lane < DELTA_ROWS && row0 + lane < a.n_q && in_a_tile(a, a.q_seq, static_cast<int>(row0) + lane, false);
+    for (unsigned todo = __ballot_sync(FULL_MASK, mine); todo != 0; todo &= todo - 1) {
+      const int row = static_cast<int>(row0) + __ffs(todo) - 1;
+#pragma unroll 4
+      for (int h0 = 0; h0 < a.heads; h0 += SIDE) {
+        const int head = h0 + lane / LANES;
+        const bool in = head < a.heads;
+        float sum = 0.0f, square = 0.0f;
+        if (in && vec * 8 < a.d) {
+          float x[8], y[8];
+          load_vec<T, 8>(static_cast<const T*>(a.dout.p) + row * a.dout.row + head * a.dout.head + vec * 8, x);
+          load_vec<T, 8>(static_cast<const T*>(a.out) + (static_cast<int64_t>(row) * a.heads + head) * a.d + vec * 8, y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum = fmaf(x[i], y[i], sum);
-        square = fmaf(x[i], x[i], square);
+          for (int i = 0; i < 8; ++i) {
+            sum = fmaf(x[i], y[i], sum);
+            square = fmaf(x[i], x[i], square);
+          }
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+          sum += __shfl_xor_sync(FULL_MASK, sum, o);
+          square += __shfl_xor_sync(FULL_MASK, square, o);
+        }
+        if (in && vec == 0) {
+          const int64_t at = static_cast<int64_t>(head) * a.n_q + row;
+          const float lse = a.lse[at];
+          a.delta[at] = sum;
+          a.lse2[at] = lse == -INFINITY ? INFINITY : lse * LOG2E - down;  // (a row that sees no key has no weights)
+          top = fmaxf(top, sqrtf(square));
+        }
       }
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      sum += __shfl_xor_sync(FULL_MASK, sum, o);
-      square += __shfl_xor_sync(FULL_MASK, square, o);
-    }
-    if (mine && lane == 0) {
-      const int64_t at = static_cast<int64_t>(head) * a.n_q + row;
-      const float lse = a.lse[at];
-      a.delta[at] = sum;
-      a.lse2[at] = lse == -INFINITY ? INFINITY : lse * LOG2E - down;  // (a row that sees no key has no weights)
-      top = fmaxf(top, sqrtf(square));
     }
   }
   if (norm) largest_of_cta(top, a.norms);
@@ -554,8 +565,9 @@ __global__ __launch_bounds__(DELTA_THREADS) void attn_norm_kernel(const __grid_c
 template <int DP>
 struct BackwardShape {
   static constexpr int STAGES = DP == 128 ? 5 : 8;
-  static constexpr uint32_t RING = 2 * tile_bytes<DP>(), STATS = RING + STAGES * tile_bytes<DP>(), BARS = STATS + 2 * 2 * ATTN_TILE * 4,
-                            SMEM = BARS + 256;
+  static constexpr int ITEMS = DP == 128 ? 1 : 2;  // items whose own tiles fit: the next one's come while this one is worked on
+  static constexpr uint32_t OWN_BYTES = 2 * tile_bytes<DP>(), RING = ITEMS * OWN_BYTES, STATS = RING + STAGES * tile_bytes<DP>(),
+                            BARS = STATS + 2 * 2 * ATTN_TILE * 4, SMEM = BARS + 256;
 };
 
 // a row of DP values out of TMEM, times `by`, into contiguous rows of d elements
@@ -590,20 +602,21 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
   const AttnArgs& a = args.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t smem = smem_addr(smem_raw), bars = smem + Shape::BARS;
-  const uint32_t kv_full = bars, kv_empty = bars + 8, s_full = bars + 16, e_full = bars + 24, p_full = bars + 32, ds_full = bars + 40,
-                 done = bars + 48, stats_full = bars + 56, stats_empty = bars + 72, full = bars + 88, empty = full + 8 * STAGES,
+  constexpr int ITEMS = Shape::ITEMS;
+  const uint32_t kv_full = bars, kv_empty = bars + 16, s_full = bars + 32, e_full = bars + 40, p_full = bars + 48, ds_full = bars + 56,
+                 done = bars + 64, stats_full = bars + 72, stats_empty = bars + 88, full = bars + 104, empty = full + 8 * STAGES,
                  tmem_word = empty + 8 * STAGES;
   volatile int* dead = reinterpret_cast<volatile int*>(smem_raw + (tmem_word + 4 - smem));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    bar_init(kv_full, LOAD_THREADS);
-    bar_init(kv_empty, 1);
     bar_init(s_full, 1);
     bar_init(e_full, 1);
     bar_init(p_full, SOFTMAX_WARPS * 32);
     bar_init(ds_full, SOFTMAX_WARPS * 32);
     bar_init(done, 1);
     for (int i = 0; i < 2; ++i) {
+      bar_init(kv_full + 8 * i, LOAD_THREADS);
+      bar_init(kv_empty + 8 * i, 1);
       bar_init(stats_full + 8 * i, LOAD_THREADS);
       bar_init(stats_empty + 8 * i, SOFTMAX_WARPS * 32);
     }
@@ -637,8 +650,9 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
         const int index = static_cast<int>(item / a.kv_heads), kv = static_cast<int>(item - static_cast<int64_t>(index) * a.kv_heads);
         const AttnTile x = tile_at(a.k_tiles + index);
         if (x.steps == 0) continue;
-        if (!(ok = !*dead && bar_wait(kv_empty, (n & 1) ^ 1))) break;
-        load.boxes(smem, &args.k, kv, x.row, &args.v, kv, x.row, true, kv_full);
+        const int own = n % ITEMS;
+        if (!(ok = !*dead && bar_wait(kv_empty + 8 * own, ((n / ITEMS) & 1) ^ 1))) break;
+        load.boxes(smem + own * Shape::OWN_BYTES, &args.k, kv, x.row, &args.v, kv, x.row, true, kv_full + 8 * own);
         for (int u = 0; ok && u < x.steps * group; ++u, ++step) {
           const int head = kv * group + u / x.steps, at = u % x.steps * ATTN_TILE, row = x.other + at, left = x.others - at;
           if (!(ok = load.free_stage())) break;
@@ -671,14 +685,15 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
     if (lane == 0) {
       const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
       const uint32_t s = tmem, e = tmem + 128, dv = tmem + 256, dk = tmem + 256 + DP;
-      const uint32_t k = smem, v = smem + tile_bytes<DP>();
       Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
       int n = 0;
       uint32_t at = 0;
       for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
         const AttnTile x = tile_at(a.k_tiles + item / a.kv_heads);
         if (x.steps == 0) continue;
-        if (!(ok = !*dead && bar_wait(kv_full, n & 1) && st.ready(0))) break;
+        const int own = n % ITEMS;
+        const uint32_t k = smem + own * Shape::OWN_BYTES, v = k + tile_bytes<DP>();
+        if (!(ok = !*dead && bar_wait(kv_full + 8 * own, (n / ITEMS) & 1) && st.ready(0))) break;
         fence_after();
         product_rows<DP>(s, k, st.tile(0), by_rows);
         mma_commit_one(s_full);
@@ -708,7 +723,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
         }
         if (!ok) break;
         mma_commit_one(done);
-        mma_commit_one(kv_empty);
+        mma_commit_one(kv_empty + 8 * own);
         ++n;
       }
     }
@@ -811,15 +826,17 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
   const AttnArgs& a = args.a;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t smem = smem_addr(smem_raw), bars = smem + Shape::BARS;
-  const uint32_t q_full = bars, q_empty = bars + 8, s_full = bars + 16, e_full = bars + 32, e_read = bars + 40, ds_full = bars + 48,
-                 done = bars + 64, full = bars + 72, empty = full + 8 * STAGES, tmem_word = empty + 8 * STAGES;
+  constexpr int ITEMS = Shape::ITEMS;
+  const uint32_t q_full = bars, q_empty = bars + 16, s_full = bars + 32, e_full = bars + 48, e_read = bars + 56, ds_full = bars + 64,
+                 done = bars + 80, full = bars + 88, empty = full + 8 * STAGES, tmem_word = empty + 8 * STAGES;
   volatile int* dead = reinterpret_cast<volatile int*>(smem_raw + (tmem_word + 4 - smem));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    bar_init(q_full, LOAD_THREADS);
-    bar_init(q_empty, 1);
-    bar_init(s_full, 1);
-    bar_init(s_full + 8, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(q_full + 8 * i, LOAD_THREADS);
+      bar_init(q_empty + 8 * i, 1);
+      bar_init(s_full + 8 * i, 1);
+    }
     bar_init(e_full, 1);
     bar_init(e_read, SOFTMAX_WARPS * 32);
     // (two: the slopes of a step may be there before the products' thread has looked for those of the step before)
@@ -855,8 +872,9 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
         const int index = static_cast<int>(item / a.heads), head = static_cast<int>(item - static_cast<int64_t>(index) * a.heads);
         const AttnTile x = tile_at(a.q_tiles + index);
         if (x.steps == 0) continue;
-        if (!(ok = !*dead && bar_wait(q_empty, (n & 1) ^ 1))) break;
-        load.boxes(smem, &args.q, head, x.row, &args.dout, head, x.row, true, q_full);
+        const int own = n % ITEMS;
+        if (!(ok = !*dead && bar_wait(q_empty + 8 * own, ((n / ITEMS) & 1) ^ 1))) break;
+        load.boxes(smem + own * Shape::OWN_BYTES, &args.q, head, x.row, &args.dout, head, x.row, true, q_full + 8 * own);
         // K0, V0, K1, V1, ..  (K's rows are summed over)
         for (int j = 0; ok && j < x.steps; ++j) {
           const int at = j * ATTN_TILE;
@@ -874,14 +892,16 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
     fewer_registers<FEW_REGISTERS>();
     if (lane == 0) {
       const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
-      const uint32_t e = tmem + 256, dq = tmem + 384, q = smem, g = smem + tile_bytes<DP>();
+      const uint32_t e = tmem + 256, dq = tmem + 384;
       Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
       int n = 0;
       uint32_t at = 0;
       for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
         const AttnTile x = tile_at(a.q_tiles + item / a.heads);
         if (x.steps == 0) continue;
-        if (!(ok = !*dead && bar_wait(q_full, n & 1) && st.ready(0))) break;
+        const int own = n % ITEMS;
+        const uint32_t q = smem + own * Shape::OWN_BYTES, g = q + tile_bytes<DP>();
+        if (!(ok = !*dead && bar_wait(q_full + 8 * own, (n / ITEMS) & 1) && st.ready(0))) break;
         fence_after();
         product_rows<DP>(tmem + (at & 1) * 128, q, st.tile(0), by_rows);
         mma_commit_one(s_full + 8 * (at & 1));
@@ -908,7 +928,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
         }
         if (!ok) break;
         mma_commit_one(done);
-        mma_commit_one(q_empty);
+        mma_commit_one(q_empty + 8 * own);
         ++n;
       }
     }
@@ -1026,7 +1046,8 @@ int backward(const TileArgs& t, cudaStream_t s) {
     const int need = (rows + DELTA_THREADS / 16 - 1) / (DELTA_THREADS / 16), most = (sm_count() * 8 + heads - 1) / heads;
     return static_cast<unsigned>(need < most ? need : most);
   };
-  DGS_CUDA_TRY(launch_training(attn_delta_kernel<T>, dim3(ctas(a.n_q, a.heads), a.heads), DELTA_THREADS, 0, s, a, lift<BF16>(), static_cast<int32_t>(!BF16)));
+  DGS_CUDA_TRY(launch_training(attn_delta_kernel<T, DP / 8>, dim3(ctas((a.n_q + DELTA_ROWS - 1) / DELTA_ROWS * 2, 1)), DELTA_THREADS, 0, s, a,
+                               lift<BF16>(), static_cast<int32_t>(!BF16)));
   if (!BF16) DGS_CUDA_TRY(launch_training(attn_norm_kernel<T>, dim3(ctas(a.n_k, a.kv_heads), a.kv_heads), DELTA_THREADS, 0, s, a));
   if (a.dk != nullptr)
     if (int rc = launch_tiles(attn_dkv_kernel<DP, BF16>, t, static_cast<int64_t>(a.k_tile_bound) * a.kv_heads, BackwardShape<DP>::SMEM, known[0], s))
