@@ -61,16 +61,19 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
   __shared__ int bucket[2][PLAN_BUCKETS];
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (alone) {
+  if (alone && blockIdx.x == 0) {
     if (threadIdx.x < ATTN_COUNTS) a.counts[threadIdx.x] = 0;
     if (threadIdx.x < 2) a.norms[threadIdx.x] = 0.0f;
     if (threadIdx.x < 2 * PLAN_BUCKETS) bucket[threadIdx.x / PLAN_BUCKETS][threadIdx.x % PLAN_BUCKETS] = 0;
     __syncthreads();
   }
-  // each warp reads the offsets of up to 32 sequences at once and then takes them in turn
-  const int warps = gridDim.x * (PLAN_THREADS / 32), batch = min(32, (a.seqs + warps - 1) / warps);
+  // Where one CTA makes the lists, the others write whose the rows are.  Each warp reads the offsets of up to 32 sequences at once and then
+  // takes them in turn.
+  const bool lists = !alone || blockIdx.x == 0, maps = !alone || blockIdx.x > 0;
+  const int ctas = alone ? (lists ? 1 : gridDim.x - 1) : gridDim.x, cta = alone && !lists ? blockIdx.x - 1 : blockIdx.x;
+  const int warps = ctas * (PLAN_THREADS / 32), batch = min(32, (a.seqs + warps - 1) / warps);
   int tiles = 0, single = 0, several = 0;  // sequences of each kind
-  for (int s0 = (blockIdx.x * (PLAN_THREADS / 32) + warp) * batch; s0 < a.seqs; s0 += warps * batch) {
+  for (int s0 = (cta * (PLAN_THREADS / 32) + warp) * batch; s0 < a.seqs; s0 += warps * batch) {
     const int mine = s0 + lane;
     AttnSeq own{0, 0, 0, 0};
     if (lane < batch && mine < a.seqs) {
@@ -80,7 +83,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
         own = {static_cast<int32_t>(q0), static_cast<int32_t>(q1 - q0), static_cast<int32_t>(k0), static_cast<int32_t>(k1 - k0)};
       else
         raise_status(a.status, DGS_ERR_RANGE), several = 1;
-      a.seq[mine] = own;
+      if (lists) a.seq[mine] = own;
       if (attn_in_tiles(a, own)) tiles = 1;
       else if (attn_is_single(a, own)) single = 1;
       else several = 1;
@@ -89,9 +92,12 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
       const int s = s0 + n;
       const AttnSeq e{__shfl_sync(FULL_MASK, own.q0, n), __shfl_sync(FULL_MASK, own.q_len, n), __shfl_sync(FULL_MASK, own.k0, n),
                       __shfl_sync(FULL_MASK, own.k_len, n)};
-      for (int i = lane; i < e.q_len; i += 32) a.q_seq[e.q0 + i] = s;
-      if (backward)
-        for (int i = lane; i < e.k_len; i += 32) a.k_seq[e.k0 + i] = s;
+      if (maps) {
+        for (int i = lane; i < e.q_len; i += 32) a.q_seq[e.q0 + i] = s;
+        if (backward)
+          for (int i = lane; i < e.k_len; i += 32) a.k_seq[e.k0 + i] = s;
+        if (!lists) continue;
+      }
       if (attn_in_tiles(a, e)) {
         const int nq = tiles_of(e.q_len, a.q_tile_rows), nk = backward ? tiles_of(e.k_len, ATTN_TILE) : 0;
         if (alone) {  // counted first, placed below
@@ -120,6 +126,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
       }
     }
   }
+  if (!lists) return;
   // which kinds there are: kernels for the others leave at once
   const unsigned kinds = __reduce_or_sync(FULL_MASK, (tiles ? 1u << ATTN_HAS_TILES : 0u) | (single ? 1u << ATTN_HAS_SINGLE : 0u) | (several ? 1u << ATTN_HAS_SEVERAL : 0u));
   if (lane == 0 && kinds != 0) atomicOr(&a.counts[ATTN_KINDS], static_cast<int>(kinds));
@@ -938,8 +945,9 @@ int launch_plan(const AttnArgs& a, bool backward, cudaStream_t s) {
     DGS_CUDA_TRY(cudaMemsetAsync(a.counts, 0, ATTN_COUNTS * 4, s));
     DGS_CUDA_TRY(cudaMemsetAsync(a.norms, 0, 8, s));
   }
-  const int64_t ctas = one ? 1 : (static_cast<int64_t>(a.seqs) + PLAN_THREADS / 32 - 1) / (PLAN_THREADS / 32);
-  const int64_t most = 2 * static_cast<int64_t>(sm_count());
+  // (one CTA: and others for the maps, a warp for every sequence or two)
+  const int64_t each = (static_cast<int64_t>(a.seqs) + PLAN_THREADS / 32 - 1) / (PLAN_THREADS / 32);
+  const int64_t ctas = one ? 1 + (each < 32 ? each < 1 ? 1 : each : 32) : each, most = 2 * static_cast<int64_t>(sm_count());
   DGS_CUDA_TRY(launch_training(attn_plan_kernel, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), PLAN_THREADS, 0, s, a,
                                static_cast<int32_t>(backward), static_cast<int32_t>(one)));
   return DGS_OK;

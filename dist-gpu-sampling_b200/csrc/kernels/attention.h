@@ -60,9 +60,9 @@ constexpr int ATTN_SPLIT_FROM = 256;   // keys from which a CTA takes a row inst
 constexpr int ATTN_SPLIT_KEYS = 1024;  // ... so many at a time
 constexpr int ATTN_SPLIT_QUERIES = 16; // (with more queries there are warps enough)
 constexpr int ATTN_TILE = 128;         // rows of a tile of keys, and of queries
-constexpr int ATTN_TILE_QUERIES = 48;  // queries from which a sequence goes to the tensor cores whatever its keys, ...
+constexpr int ATTN_TILE_QUERIES = 24;  // queries from which a sequence goes to the tensor cores whatever its keys, ...
 constexpr int ATTN_FEW_QUERIES = 8;    // ... or from which it does with so many pairs, unless there are keys enough to be split
-constexpr int ATTN_TILE_PAIRS = 2048, ATTN_MANY_KEYS = 4096;
+constexpr int ATTN_TILE_PAIRS = 576, ATTN_MANY_KEYS = 4096;
 constexpr int ATTN_FEW_KEYS = 24;      // keys a sequence on average up to which a warp takes key heads side by side, beyond it takes keys
 
 __host__ __device__ inline bool attn_many_keys(const AttnSeq& s) {

@@ -159,8 +159,8 @@ def attention(q, k, v, q_offsets, k_offsets=None, causal=False, scale=None, retu
 
     causal: query i of Lq sees the keys j <= i + Lk - Lq (the last query sees all of them).  scale: 1 / sqrt(d) by default.  A query that
     sees no key gives zeros, and so do rows outside of all sequences.  return_lse: also the logarithm of the sum of exponentials
-    [heads, n_q] (float32, without a gradient; -inf where no key is seen).  Sequences of 48 queries and more run on the tensor cores in
-    16 bits; float32 runs on the CUDA cores.  Gradients are added in a fixed order."""
+    [heads, n_q] (float32, without a gradient; -inf where no key is seen).  Sequences of 24 queries and more (8 over
+    many keys) run on the tensor cores in 16 bits; float32 runs on the CUDA cores.  Gradients are added in a fixed order."""
     if k_offsets is None:
         k_offsets = q_offsets
     if not _functions:
