@@ -171,15 +171,40 @@ __device__ __forceinline__ void product_columns(uint32_t d, uint32_t a, uint32_t
     mma_one_tmem(d, a + (k / 4) * half + (k % 4) * 8, db + k * (2048 >> 4), idesc, accumulate || k > 0);
 }
 
-__device__ __forceinline__ void take(int4* to, const AttnTile* p) {
-  to[0] = reinterpret_cast<const int4*>(p)[0];
-  to[1] = reinterpret_cast<const int4*>(p)[1];
-}
 __device__ __forceinline__ AttnTile tile_at(const AttnTile* p) {
   AttnTile t;
-  take(reinterpret_cast<int4*>(&t), p);
+  reinterpret_cast<int4*>(&t)[0] = reinterpret_cast<const int4*>(p)[0];
+  reinterpret_cast<int4*>(&t)[1] = reinterpret_cast<const int4*>(p)[1];
   return t;
 }
+// The items of a CTA: every gridDim.x-th (tile, head), the next tile's words on their way.
+struct Items {
+  const AttnTile* list;
+  int tiles, heads, index, head;
+  AttnTile x, next;
+  __device__ __forceinline__ Items(const AttnTile* tiles_list, int n_tiles, int n_heads) : list(tiles_list), tiles(n_tiles), heads(n_heads) {
+    index = blockIdx.x / heads;
+    head = blockIdx.x % heads;
+    if (index < tiles) x = tile_at(list + index);
+    ask();
+  }
+  __device__ __forceinline__ bool more() const { return index < tiles; }
+  __device__ __forceinline__ void step(int* to_index, int* to_head) const {
+    *to_index = index + static_cast<int>(gridDim.x) / heads;
+    *to_head = head + static_cast<int>(gridDim.x) % heads;
+    if (*to_head >= heads) *to_head -= heads, ++*to_index;
+  }
+  __device__ __forceinline__ void ask() {
+    int i, h;
+    step(&i, &h);
+    if (i < tiles) next = tile_at(list + i);
+  }
+  __device__ __forceinline__ void advance() {
+    step(&index, &head);
+    x = next;
+    ask();
+  }
+};
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 template <int DP>
@@ -495,7 +520,7 @@ __device__ __forceinline__ void largest_of_cta(float v, float* to) {
 // side and takes each of them with all its heads, LANES lanes a head.
 constexpr int DELTA_ROWS = 8;
 template <typename T, int LANES>
-__global__ __launch_bounds__(DELTA_THREADS) void attn_delta_kernel(const __grid_constant__ AttnArgs a, float down, int32_t norm) {
+__global__ __launch_bounds__(DELTA_THREADS, 4) void attn_delta_kernel(const __grid_constant__ AttnArgs a, float down, int32_t norm) {
   pdl_enter();
   if ((a.counts[ATTN_KINDS] >> ATTN_HAS_TILES & 1) == 0) return;
   const int lane = threadIdx.x & 31, vec = lane % LANES, warps = gridDim.x * (DELTA_THREADS / 32);
@@ -506,7 +531,7 @@ __global__ __launch_bounds__(DELTA_THREADS) void attn_delta_kernel(const __grid_
     const bool mine = lane < DELTA_ROWS && row0 + lane < a.n_q && in_a_tile(a, a.q_seq, static_cast<int>(row0) + lane, false);
     for (unsigned todo = __ballot_sync(FULL_MASK, mine); todo != 0; todo &= todo - 1) {
       const int row = static_cast<int>(row0) + __ffs(todo) - 1;
-#pragma unroll 4
+#pragma unroll 2
       for (int h0 = 0; h0 < a.heads; h0 += SIDE) {
         const int head = h0 + lane / LANES;
         const bool in = head < a.heads;
@@ -634,7 +659,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_word) : "memory");
   pdl_enter();
-  const int64_t items = static_cast<int64_t>(min(a.counts[ATTN_N_K_TILES], a.k_tile_bound)) * a.kv_heads;
+  Items items(a.k_tiles, min(a.counts[ATTN_N_K_TILES], a.k_tile_bound), a.kv_heads);
   const int group = a.heads / a.kv_heads;
   bool ok = true;
 
@@ -646,9 +671,9 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
       const int t = static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32;
       Loader<DP, STAGES> load{smem + Shape::RING, full, empty, t, dead};
       int n = 0, step = 0;
-      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-        const int index = static_cast<int>(item / a.kv_heads), kv = static_cast<int>(item - static_cast<int64_t>(index) * a.kv_heads);
-        const AttnTile x = tile_at(a.k_tiles + index);
+      for (; ok && items.more(); items.advance()) {
+        const int kv = items.head;
+        const AttnTile& x = items.x;
         if (x.steps == 0) continue;
         const int own = n % ITEMS;
         if (!(ok = !*dead && bar_wait(kv_empty + 8 * own, ((n / ITEMS) & 1) ^ 1))) break;
@@ -688,8 +713,8 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
       Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
       int n = 0;
       uint32_t at = 0;
-      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-        const AttnTile x = tile_at(a.k_tiles + item / a.kv_heads);
+      for (; ok && items.more(); items.advance()) {
+        const AttnTile& x = items.x;
         if (x.steps == 0) continue;
         const int own = n % ITEMS;
         const uint32_t k = smem + own * Shape::OWN_BYTES, v = k + tile_bytes<DP>();
@@ -736,9 +761,9 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
     const uint32_t s = tmem + half * 64 + lanes, e = tmem + 128 + half * 64 + lanes;
     const float c = a.scale * LOG2E, by = slope_scale<BF16>(a);
     int at = 0, items_done = 0;
-    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const int index = static_cast<int>(item / a.kv_heads), kv = static_cast<int>(item - static_cast<int64_t>(index) * a.kv_heads);
-      const AttnTile x = tile_at(a.k_tiles + index);
+    for (; ok && items.more(); items.advance()) {
+      const int kv = items.head;
+      const AttnTile& x = items.x;
       const bool there = mine < x.rows;
       char* to = static_cast<char*>(half ? a.dk : a.dv) + (static_cast<int64_t>(x.row + mine) * a.kv_heads + kv) * a.d * 2;
       if (x.steps == 0) {
@@ -857,7 +882,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_word) : "memory");
   pdl_enter();
-  const int64_t items = static_cast<int64_t>(min(a.counts[ATTN_N_Q_TILES], a.q_tile_bound)) * a.heads;
+  Items items(a.q_tiles, min(a.counts[ATTN_N_Q_TILES], a.q_tile_bound), a.heads);
   const int group = a.heads / a.kv_heads;
   bool ok = true;
 
@@ -868,9 +893,9 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
       fence_async_global();
       Loader<DP, STAGES> load{smem + Shape::RING, full, empty, static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32, dead};
       int n = 0;
-      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-        const int index = static_cast<int>(item / a.heads), head = static_cast<int>(item - static_cast<int64_t>(index) * a.heads);
-        const AttnTile x = tile_at(a.q_tiles + index);
+      for (; ok && items.more(); items.advance()) {
+        const int head = items.head;
+        const AttnTile& x = items.x;
         if (x.steps == 0) continue;
         const int own = n % ITEMS;
         if (!(ok = !*dead && bar_wait(q_empty + 8 * own, ((n / ITEMS) & 1) ^ 1))) break;
@@ -896,8 +921,8 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
       Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
       int n = 0;
       uint32_t at = 0;
-      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-        const AttnTile x = tile_at(a.q_tiles + item / a.heads);
+      for (; ok && items.more(); items.advance()) {
+        const AttnTile& x = items.x;
         if (x.steps == 0) continue;
         const int own = n % ITEMS;
         const uint32_t q = smem + own * Shape::OWN_BYTES, g = q + tile_bytes<DP>();
@@ -941,9 +966,9 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
     const uint32_t e = tmem + 256 + half * 64 + lanes;
     const float c = a.scale * LOG2E, by = slope_scale<BF16>(a);
     int at = 0, items_done = 0;
-    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const int index = static_cast<int>(item / a.heads), head = static_cast<int>(item - static_cast<int64_t>(index) * a.heads);
-      const AttnTile x = tile_at(a.q_tiles + index);
+    for (; ok && items.more(); items.advance()) {
+      const int head = items.head;
+      const AttnTile& x = items.x;
       const bool there = mine < x.rows;
       char* to = static_cast<char*>(a.dq) + (static_cast<int64_t>(x.row + mine) * a.heads + head) * a.d * 2;
       if (x.steps == 0) {
