@@ -170,6 +170,12 @@ __global__ __launch_bounds__(PLAN_THREADS) void attn_plan_kernel(const __grid_co
   }
 }
 
+__device__ __forceinline__ float ex2(float x) {  // exp2 within two units in the last place, results below 2^-126 flushed to 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // ---- rows ------------------------------------------------------------------------------------------------------------
 // A row of DP elements lies in G lanes, VEC elements each.  A warp holds 32 / G of them side by side: `side` key heads of one key (which
 // lie side by side in memory too), and where there are fewer heads than that, several keys.
@@ -208,12 +214,21 @@ __device__ __forceinline__ void load_row(const T* p, bool there, float (&v)[VEC]
     for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
   }
 }
+// two elements an instruction
 template <int VEC>
 __device__ __forceinline__ float dot(const float (&a)[VEC], const float (&b)[VEC]) {
-  float s = a[0] * b[0];
+  uint64_t s = mul2(two(a[0], a[1]), two(b[0], b[1]));
 #pragma unroll
-  for (int e = 1; e < VEC; ++e) s = fmaf(a[e], b[e], s);
-  return s;
+  for (int e = 2; e < VEC; e += 2) s = fma2(two(a[e], a[e + 1]), two(b[e], b[e + 1]), s);
+  float lo, hi;
+  split2(s, &lo, &hi);
+  return lo + hi;
+}
+template <int VEC>
+__device__ __forceinline__ void add_scaled(float by, const float (&x)[VEC], float (&sum)[VEC]) {
+  const uint64_t by2 = two(by, by);
+#pragma unroll
+  for (int e = 0; e < VEC; e += 2) split2(fma2(by2, two(x[e], x[e + 1]), two(sum[e], sum[e + 1])), &sum[e], &sum[e + 1]);
 }
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -254,25 +269,25 @@ __device__ __forceinline__ void forward_keys(const T* k, int64_t k_row, const T*
         if (j + u * w.keys + w.key >= j1) x[r][u] = -INFINITY;
         top = fmaxf(top, x[r][u]);
       }
-      const float ref = top == -INFINITY ? 0.0f : top, scale = exp2f(m[r] - ref);
+      const float ref = top == -INFINITY ? 0.0f : top, scale = ex2(m[r] - ref);
       m[r] = top;
       l[r] *= scale;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        x[r][u] = exp2f(x[r][u] - ref);
+        x[r][u] = ex2(x[r][u] - ref);
         l[r] += x[r][u];
       }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) acc[r][e] *= scale;
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      float vf[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float f = to_float<T>(vr[u].v[e]);
+      for (int e = 0; e < VEC; ++e) vf[e] = to_float<T>(vr[u].v[e]);
 #pragma unroll
-        for (int r = 0; r < R; ++r) acc[r][e] = fmaf(x[r][u], f, acc[r][e]);
-      }
+      for (int r = 0; r < R; ++r) add_scaled<VEC>(x[r][u], vf, acc[r]);
+    }
   }
 }
 
@@ -282,7 +297,7 @@ __device__ __forceinline__ void join_keys(int first, float& m, float& l, float (
   for (int o = first; o < 32; o <<= 1) {
     const float m2 = __shfl_xor_sync(FULL_MASK, m, o), l2 = __shfl_xor_sync(FULL_MASK, l, o);
     const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
-    const float s1 = exp2f(m - ref), s2 = exp2f(m2 - ref);
+    const float s1 = ex2(m - ref), s2 = ex2(m2 - ref);
     l = l * s1 + l2 * s2;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = acc[e] * s1 + __shfl_xor_sync(FULL_MASK, acc[e], o) * s2;
@@ -384,20 +399,21 @@ __device__ __forceinline__ bool last_part(const AttnArgs& a, const int4& it, int
   return last;
 }
 
-// Forward.  Rows with up to ATTN_SPLIT_FROM keys: a warp each, for all the key heads side by side.  The first `split_ctas` CTAs take the
-// parts of rows with many keys; the last part of a row to be there joins them in their order.  Bound by HBM where every query has keys
-// of its own.
-template <typename T, int DP, int R>
-__global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __grid_constant__ AttnArgs a, int32_t split_ctas) {
-  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = R == 4 ? 2 : 4, SPLIT_U = R == 1 ? 4 : 2;
-  __shared__ Shared<T, DP, DP + 2> shared;
-  __shared__ bool flag;
+// Forward.  Rows with up to ATTN_SPLIT_FROM keys: a warp each, for all the key heads side by side.  SPLIT: CTAs take the parts of rows with
+// many keys; the last part of a row to be there joins them in their order.  Bound by HBM where every query has keys of its own: what is
+// under way is many warps with few keys each for short rows (60 000 seeds of 7.5 keys: 144 us with 32 warps an SM and two keys, 169 with
+// 16 and four), more keys a warp for long ones.
+template <typename T, int DP, int R, bool SPLIT>
+__global__ __launch_bounds__(ROW_WARPS * 32, R == 1 && !SPLIT ? 4 : 2) void attn_rows_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = R == 2 ? 4 : 2, SPLIT_U = R == 1 ? 4 : 2;
   pdl_enter();
-  const bool splits = static_cast<int>(blockIdx.x) < split_ctas;
   const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
-  const Lanes<T, DP> w(a, splits ? a.split_side : a.side);
+  const Lanes<T, DP> w(a, SPLIT ? a.split_side : a.side);
   const int blocks = w.blocks;
-  if (splits) {
+  if constexpr (SPLIT) {
+    __shared__ Shared<T, DP, DP + 2> shared;
+    __shared__ bool flag;
+    const int split_ctas = gridDim.x;
     const int floats = a.d + 2, n = min(a.counts[ATTN_N_SPLITS], a.split_bound);
     for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * blocks; t += split_ctas) {
       const int item = static_cast<int>(t / blocks), block = static_cast<int>(t - static_cast<int64_t>(item) * blocks);
@@ -441,7 +457,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
             for (int y = 0; y < ROW_WARPS; ++y) top = fmaxf(top, shared.v[y][hs][DP]);
             const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int y = 0; y < ROW_WARPS; ++y) sum += shared.v[y][hs][at] * exp2f(shared.v[y][hs][DP] - ref);
+            for (int y = 0; y < ROW_WARPS; ++y) sum += shared.v[y][hs][at] * ex2(shared.v[y][hs][DP] - ref);
             float* part = a.parts + (static_cast<int64_t>(item) * a.heads + kv * group + h0 + r) * floats;
             part[x < a.d ? x : a.d + 1] = sum;
             if (x == 0) part[a.d] = top;
@@ -464,7 +480,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
           for (int x = 0; x < DP / 32; ++x) acc[x] = 0.0f;
 #pragma unroll 4
           for (int p = 0; p < it.w; ++p) {
-            const float by = exp2f(__ldcg(part + p * apart + a.d) - ref);
+            const float by = ex2(__ldcg(part + p * apart + a.d) - ref);
             l += __ldcg(part + p * apart + a.d + 1) * by;
 #pragma unroll
             for (int x = 0; x < DP / 32; ++x)
@@ -482,9 +498,8 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_kernel(const __gr
     }
     return;
   }
-  const int64_t ctas = gridDim.x - split_ctas;
   each_row(
-      a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, Range{a.n_q, a.n_q, 0}, blocks, a.q_seq, false,
+      a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, Range{a.n_q, a.n_q, 0}, blocks, a.q_seq, false,
       [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e)); },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = keys_seen(a, e, row), c = block * w.side + w.head;
@@ -529,8 +544,8 @@ __device__ __forceinline__ float reference_of(const AttnArgs& a, int head, int r
 // Sequences of one query and few keys (a seed over its neighbours): nobody else reads these keys, so one pass over them gives all
 // three gradients.  A warp a query, delta = do.o from the stored result.  Bound by HBM: K and V read, dK and dV written.
 template <typename T, int DP, int R>
-__global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_single_backward_kernel(const __grid_constant__ AttnArgs a) {
-  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = R == 1 ? 4 : 2;
+__global__ __launch_bounds__(ROW_WARPS * 32, R == 1 ? 4 : 2) void attn_single_backward_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = 2;
   pdl_enter();
   if ((a.counts[ATTN_KINDS] >> ATTN_HAS_SINGLE & 1) == 0) return;
   const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
@@ -580,13 +595,10 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_single_backward_kernel
 #pragma unroll
             for (int r = 0; r < R; ++r) {
               const float x = group_sum<G>(dot<VEC>(q[r], kf)) * (a.scale * LOG2E), y = group_sum<G>(dot<VEC>(g[r], vf));
-              const float p = at < seen && r < group ? exp2f(x - ref[r]) : 0.0f, ds = p * (y - delta[r]) * a.scale;
-#pragma unroll
-              for (int n = 0; n < VEC; ++n) {
-                dv[n] = fmaf(p, g[r][n], dv[n]);
-                dk[n] = fmaf(ds, q[r][n], dk[n]);
-                dq[r][n] = fmaf(ds, kf[n], dq[r][n]);
-              }
+              const float p = at < seen && r < group ? ex2(x - ref[r]) : 0.0f, ds = p * (y - delta[r]) * a.scale;
+              add_scaled<VEC>(p, g[r], dv);
+              add_scaled<VEC>(ds, q[r], dk);
+              add_scaled<VEC>(ds, kf, dq[r]);
             }
             if (a.dk != nullptr && at < seen && in) {
               store_vec<T, VEC>(static_cast<T*>(a.dk) + to + at * to_row, dk);
@@ -631,28 +643,22 @@ __device__ __forceinline__ void backward_keys(const T* k, int64_t k_row, const T
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float x = group_sum<G>(dot<VEC>(q[r], kf)), e = group_sum<G>(dot<VEC>(g[r], vf));
-        const float p = j + u * w.keys + w.key < j1 ? exp2f(x - ref[r]) : 0.0f;
+        const float p = j + u * w.keys + w.key < j1 ? ex2(x - ref[r]) : 0.0f;
         delta[r] = fmaf(p, e, delta[r]);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          pek[r][i] = fmaf(p * e, kf[i], pek[r][i]);
-          pk[r][i] = fmaf(p, kf[i], pk[r][i]);
-        }
+        add_scaled<VEC>(p * e, kf, pek[r]);
+        add_scaled<VEC>(p, kf, pk[r]);
       }
     }
   }
 }
 
 // dq and delta of the rows of other sequences, in the shape of attn_rows_kernel
-template <typename T, int DP, int R>
-__global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const __grid_constant__ AttnArgs a, int32_t split_ctas) {
+template <typename T, int DP, int R, bool SPLIT>
+__global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = 2;
-  __shared__ Shared<T, DP, 2 * DP + 1> shared;
-  __shared__ bool flag;
   pdl_enter();
-  const bool splits = static_cast<int>(blockIdx.x) < split_ctas;
   const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
-  const Lanes<T, DP> w(a, splits ? a.split_side : a.side);
+  const Lanes<T, DP> w(a, SPLIT ? a.split_side : a.side);
   const int blocks = w.blocks;
   float q[R][VEC], g[R][VEC], ref[R], pek[R][VEC], pk[R][VEC], delta[R];
   const auto begin = [&](int row, int head, int heads, bool in) {
@@ -673,7 +679,10 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
     add_keys<1>(w.side * G, one);
     delta[r] = one[0];
   };
-  if (splits) {
+  if constexpr (SPLIT) {
+    __shared__ Shared<T, DP, 2 * DP + 1> shared;
+    __shared__ bool flag;
+    const int split_ctas = gridDim.x;
     const int floats = 2 * a.d + 1, n = min(a.counts[ATTN_N_SPLITS], a.split_bound);
     for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * blocks; t += split_ctas) {
       const int item = static_cast<int>(t / blocks), block = static_cast<int>(t - static_cast<int64_t>(item) * blocks);
@@ -744,9 +753,8 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
     }
     return;
   }
-  const int64_t ctas = gridDim.x - split_ctas;
   each_row(
-      a, static_cast<int64_t>(blockIdx.x - split_ctas) * ROW_WARPS + warp, ctas * ROW_WARPS, range_of(a, false), blocks, a.q_seq, false,
+      a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, range_of(a, false), blocks, a.q_seq, false,
       [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e) || attn_is_single(a, e)); },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = keys_seen(a, e, row), c = block * w.side + w.head;
@@ -826,12 +834,9 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dkv_kernel(const 
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const float x = group_sum<G>(dot<VEC>(q[r], k)) * (a.scale * LOG2E), y = group_sum<G>(dot<VEC>(g[r], v));
-            const float p = on && r < heads ? exp2f(x - ref[r]) : 0.0f, ds = p * (y - delta[r]);
-#pragma unroll
-            for (int x2 = 0; x2 < VEC; ++x2) {
-              dv[x2] = fmaf(p, g[r][x2], dv[x2]);
-              dk[x2] = fmaf(ds, q[r][x2], dk[x2]);
-            }
+            const float p = on && r < heads ? ex2(x - ref[r]) : 0.0f, ds = p * (y - delta[r]);
+            add_scaled<VEC>(p, g[r], dv);
+            add_scaled<VEC>(ds, q[r], dk);
           }
         }
       }
@@ -856,6 +861,8 @@ struct Layout {
 };
 
 // Parts that rows with many keys can have, whatever the offsets: parts <= k_len / ATTN_SPLIT_KEYS + 1 for each of a sequence's queries
+// (none, and no launch for them, where all keys together are too few for one: whether a row is split is a matter of its own keys alone, so
+// that it has the same bits in every batch)
 int64_t split_bound(int64_t n_q, int64_t n_k, int64_t seqs) {
   if (n_k <= ATTN_SPLIT_FROM) return 0;
   const int64_t queries = n_q < ATTN_SPLIT_QUERIES ? n_q : ATTN_SPLIT_QUERIES;
@@ -1002,8 +1009,8 @@ struct RowsForward {
   template <typename T, int DP, int R>
   int run() const {
     const AttnArgs b = with_lanes<T, DP>(a, a.n_q);
-    const int splits = split_ctas(b);
-    DGS_CUDA_TRY(launch_training(attn_rows_kernel<T, DP, R>, dim3(splits + row_ctas(b, b.n_q)), ROW_WARPS * 32, 0, s, b, splits));
+    if (const int ctas = split_ctas(b)) DGS_CUDA_TRY(launch_training(attn_rows_kernel<T, DP, R, true>, dim3(ctas), ROW_WARPS * 32, 0, s, b));
+    DGS_CUDA_TRY(launch_training(attn_rows_kernel<T, DP, R, false>, dim3(row_ctas(b, b.n_q)), ROW_WARPS * 32, 0, s, b));
     return DGS_OK;
   }
 };
@@ -1023,8 +1030,8 @@ struct RowsBackward {
   template <typename T, int DP, int R>
   int run() const {
     const AttnArgs b = with_lanes<T, DP>(a, a.n_q);
-    const int splits = split_ctas(b);
-    DGS_CUDA_TRY(launch_training(attn_rows_dq_kernel<T, DP, R>, dim3(splits + row_ctas(b, b.n_q)), ROW_WARPS * 32, 0, s, b, splits));
+    if (const int ctas = split_ctas(b)) DGS_CUDA_TRY(launch_training(attn_rows_dq_kernel<T, DP, R, true>, dim3(ctas), ROW_WARPS * 32, 0, s, b));
+    DGS_CUDA_TRY(launch_training(attn_rows_dq_kernel<T, DP, R, false>, dim3(row_ctas(b, b.n_q)), ROW_WARPS * 32, 0, s, b));
     return DGS_OK;
   }
 };

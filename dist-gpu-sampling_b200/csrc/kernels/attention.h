@@ -56,8 +56,10 @@ enum { ATTN_N_SPLITS = 0, ATTN_N_Q_TILES = 1, ATTN_N_K_TILES = 2, ATTN_KINDS = 3
 enum { ATTN_HAS_TILES = 0, ATTN_HAS_SINGLE = 1, ATTN_HAS_SEVERAL = 2 };  // bits of the word ATTN_KINDS
 
 constexpr int ATTN_MAX_D = 128;
-constexpr int ATTN_SPLIT_FROM = 256;   // keys from which a CTA takes a row instead of a warp, ...
-constexpr int ATTN_SPLIT_KEYS = 1024;  // ... so many at a time
+// keys from which a CTA takes a row instead of a warp.  8 heads on 2, width 64, bf16, us forward / backward with 256 and with 512 here: 2 000
+// rows of 500 keys 287 / 1 650 and 185 / 559, one row of 500 keys 25 / 38 and 38 / 81; with 1 024: one row of 1 000 keys 36 / 54 and 68 / 153
+constexpr int ATTN_SPLIT_FROM = 512;
+constexpr int ATTN_SPLIT_KEYS = 1024;  // so many of them at a time
 constexpr int ATTN_SPLIT_QUERIES = 16; // (with more queries there are warps enough)
 constexpr int ATTN_TILE = 128;         // rows of a tile of keys, and of queries
 constexpr int ATTN_TILE_QUERIES = 24;  // queries from which a sequence goes to the tensor cores whatever its keys, ...

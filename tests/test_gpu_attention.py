@@ -267,6 +267,21 @@ def test_many_sequences(ops):
             assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("n", [255, 256, 257, 300, 511, 513, 1000, 1024, 1025, 2500])
+def test_a_row_does_not_depend_on_its_batch(ops, n):
+    """Whether a row is split is a matter of its own keys: alone, and among many short ones, it has the same bits."""
+    q_lens, k_lens = [1] * 3001, [i % 7 for i in range(3001)]
+    k_lens[1500] = n
+    q, k, v, do = make(q_lens, k_lens, 4, 2, 32, torch.bfloat16)
+    qo, ko = offsets(q_lens), offsets(k_lens)
+    out, lse = ops._CAPI_attention(q, k, v, qo, ko, False, 0.2)
+    dq, dk, dv = ops._CAPI_attention_backward(do, q, k, v, out, lse, qo, ko, False, 0.2, True, True)
+    A, C = slice(1500, 1501), slice(sum(k_lens[:1500]), sum(k_lens[:1500]) + n)
+    got = check(ops, q[A], k[C], v[C], do[A], [1], [n], False, scale=0.2)
+    for x, y in zip(got, (out[A], lse[:, A], dq[A], dk[C], dv[C])):
+        assert torch.equal(x, y)
+
+
 def test_nothing_to_do(ops):
     q, k, v, do = make([3, 2], [4, 1], 2, 1, 16, torch.float32)
     none = torch.zeros(1, dtype=torch.int64, device="cuda")
