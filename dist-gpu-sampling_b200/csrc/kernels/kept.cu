@@ -410,7 +410,9 @@ extern "C" int dgs_kept_8bit_weight_grad(const void* grad, int64_t grad_stride, 
                                          const float* scales, int64_t n, int64_t O, int64_t D, void* dweight, void* dbias,
                                          void* workspace, size_t workspace_bytes, dgs_stream_t stream) {
   if (int rc = check("kept_8bit_weight_grad", n, D, dtype)) return rc;
-  DGS_REQUIRE(O >= 1 && O <= KEPT_MAX_SIDE, DGS_ERR_INVALID, "kept_8bit_weight_grad: %lld rows of the weight", static_cast<long long>(O));
+  // (tiles of the weight's rows are the grid's second extent, below 2^16; the join's CTAs its first, below 2^31)
+  DGS_REQUIRE(O >= 1 && O < KEPT_MAX_SIDE / 2 && O * D < (int64_t(1) << 35), DGS_ERR_INVALID, "kept_8bit_weight_grad: a weight of %lld rows of %lld",
+              static_cast<long long>(O), static_cast<long long>(D));
   DGS_REQUIRE((grad_stride >= O && codes_stride >= D) || n <= 1, DGS_ERR_INVALID, "kept_8bit_weight_grad: rows that overlap");
   DGS_REQUIRE(dweight != nullptr, DGS_ERR_INVALID, "kept_8bit_weight_grad: null argument");
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -147,6 +147,10 @@ def test_kept_argument_errors(abi):
     assert keep(x=None) == INVALID and values(out=None) == INVALID
     assert grad(O=0) == INVALID and grad(g=None) == INVALID and grad(dw=None) == INVALID and grad(g_stride=46) == INVALID
     assert grad(ws=None) == INVALID and grad(wb=8) == INVALID and grad(ws=A + 8) == INVALID and b"workspace" in abi.dgs_last_error()
+    # weights whose tiles a grid cannot have
+    for dtype in (0, 1, 2):
+        assert grad(O=1 << 22, g_stride=1 << 22, dtype=dtype) == INVALID and grad(O=1 << 20, D=1 << 20, g_stride=1 << 20, stride=1 << 20, dtype=dtype) == INVALID
+        assert b"a weight of" in abi.dgs_last_error()
     assert keep(n=0, x=None) == 0 and values(n=0, out=None) == 0
     size = abi.dgs_kept_8bit_weight_grad_workspace_bytes
     assert size(0, 4, 4, 0) == 0 and size(4, 4, 4, 7) == 0 and 0 < size(1, 4, 4, 1) and size(430_000, 47, 256, 1) < 64 << 20
