@@ -1,10 +1,11 @@
 """A small node classifier trained on sampled mini-batches, from the sampler to the optimizer:
 
-    python dist-gpu-sampling_b200/train_nodes.py [--nodes 200000] [--steps 100] [--bits 8]
+    python dist-gpu-sampling_b200/train_nodes.py [--nodes 200000] [--steps 100] [--bits 8] [--model attention]
 
 PipelinedSampler delivers blocks and feature rows with several batches in flight; the rows go through layer_norm, two
 mean-aggregation layers (plain torch), and linear_cross_entropy against the classes; AdamW steps 32-bit masters and writes the
-16-bit parameters that the model reads.  The role of the reference's training loop (oppo_bench/single_node/chunktensor.py:120-172)
+16-bit parameters that the model reads.  --model attention: the layers are attention over the sampled neighbours, between linear_8bit
+projections and residual_norm.  The role of the reference's training loop (oppo_bench/single_node/chunktensor.py:120-172)
 without DGL.  The graph is synthetic: nodes of one class are linked more often, and their features lean one way.
 """
 import argparse
@@ -67,6 +68,45 @@ class Sage:
         return h
 
 
+class Attend:
+    """Blocks h' = norm(h_dst + gate * W_out attention(W_query h_dst, the sampled neighbours' W_key_value h)) and a row per class.  Query
+    heads share key heads in pairs, and the projections keep their inputs for the backward pass in 8 bits."""
+
+    def __init__(self, dim, hidden, classes, hops, heads=4, seed=0):
+        import torch
+        if heads % 2 or hidden % heads or hidden // heads > 128:
+            raise ValueError("Attend: hidden %d does not make an even number of %d heads of up to 128" % (hidden, heads))
+        g = torch.Generator().manual_seed(seed)
+
+        def weight(rows, cols):
+            return torch.randn(rows, cols, generator=g) / cols ** 0.5
+
+        masters = {"norm_in": torch.ones(dim), "bias_in": torch.zeros(dim), "into": weight(hidden, dim), "norm": torch.ones(hidden),
+                   "bias": torch.zeros(hidden), "head": weight(classes, hidden)}
+        for i in range(hops):
+            masters.update({"query%d" % i: weight(hidden, hidden), "key_value%d" % i: weight(hidden, hidden), "out%d" % i: weight(hidden, hidden),
+                            "gate%d" % i: torch.full((hidden,), 0.5), "norm%d" % i: torch.ones(hidden)})
+        self.masters = {k: v.cuda() for k, v in masters.items()}
+        self.p = {k: v.bfloat16().requires_grad_() for k, v in self.masters.items()}
+        self.hops, self.heads, self.width = hops, heads, hidden // heads
+
+    def hidden(self, pkg, x, blocks):
+        import torch
+        p, heads, width = self.p, self.heads, self.width
+        x = pkg.layer_norm(x, p["norm_in"], p["bias_in"]).bfloat16()
+        rows = pkg.linear_8bit(x, p["into"])  # the residual rows; h: their norm, which a block reads
+        h = pkg.layer_norm(rows, p["norm"], p["bias"])
+        for i, (row, col, n_src, n_dst) in enumerate(blocks):
+            indptr, indices = pkg.block_csc(row, col, n_dst)
+            query = pkg.linear_8bit(h[:n_dst], p["query%d" % i]).view(n_dst, heads, width)
+            key_value = pkg.linear_8bit(h, p["key_value%d" % i])[indices].view(-1, heads, width)
+            key, value = key_value[:, :heads // 2], key_value[:, heads // 2:]
+            seen = pkg.attention(query, key, value, torch.arange(n_dst + 1, device=x.device), indptr)
+            rows, h = pkg.residual_norm(rows[:n_dst], pkg.linear_8bit(seen.reshape(n_dst, heads * width), p["out%d" % i]), p["gate%d" % i],
+                                        weight=p["norm%d" % i])
+        return h
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--nodes", type=int, default=200_000)
@@ -79,6 +119,7 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=100)
     ap.add_argument("--lr", type=float, default=3e-3)
     ap.add_argument("--bits", type=int, default=32, choices=(8, 32))
+    ap.add_argument("--model", default="sage", choices=("sage", "attention"), help="mean aggregation, or attention over the neighbours")
     ap.add_argument("--unlabelled", type=float, default=0.1, help="share of the training nodes without a label")
     a = ap.parse_args(argv)
 
@@ -98,7 +139,7 @@ def main(argv=None):
     c_indptr, c_indices, c_feats = chunk(indptr), chunk(indices), chunk(feats)
     fanouts = [int(k) for k in a.fanouts.split(",")]
     sampler = pkg.PipelinedSampler(c_indptr, c_indices, fanouts, features=c_feats, max_seeds=a.batch, depth=3)
-    model = Sage(a.dim, a.hidden, a.classes, len(fanouts))
+    model = (Attend if a.model == "attention" else Sage)(a.dim, a.hidden, a.classes, len(fanouts))
     names = sorted(model.masters)
     optimizer = pkg.AdamW([model.masters[k] for k in names], lr=a.lr, bits=a.bits, copies=[model.p[k] for k in names])
     torch.manual_seed(3)

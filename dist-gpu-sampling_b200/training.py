@@ -103,7 +103,8 @@ def _define():
             rows = x.reshape(-1, x.shape[-1])
             ctx.shape = x.shape
             ctx.save_for_backward(weight, *ops._CAPI_keep_8bit(rows) if ctx.needs_input_grad[1] else ())
-            return torch.nn.functional.linear(x, weight, bias)
+            with torch.autocast("cuda", enabled=False):  # (the caller's types, here and in the backward pass)
+                return torch.nn.functional.linear(x, weight, bias)
 
         @staticmethod
         @torch.autograd.function.once_differentiable
@@ -116,7 +117,9 @@ def _define():
                 dw, db = ops._CAPI_kept_8bit_weight_grad(rows, *kept, want_b)
             elif want_b:
                 db = rows.sum(0, dtype=torch.float32).to(grad.dtype)
-            return (rows @ weight).view(ctx.shape) if want_x else None, dw, db if want_b else None
+            with torch.autocast("cuda", enabled=False):
+                dx = (rows @ weight).view(ctx.shape) if want_x else None
+            return dx, dw, db if want_b else None
 
     _functions.update(norm=LayerNorm, loss=LinearCrossEntropy, attention=Attention, residual=ResidualNorm, linear=Linear8bit)
 
