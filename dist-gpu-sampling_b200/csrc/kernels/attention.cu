@@ -6,8 +6,9 @@
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i   (over all queries and heads that read j)
 //
 // This file: the plan of a call, and the rows of sequences with few queries (a seed over its sampled neighbours, a read-out over
-// a graph) and of 32-bit operands, on the CUDA cores; sequences of at least ATTN_TILE_QUERIES queries in 16 bits are tiles on the
-// tensor cores (attention_mma.cu).  Nothing is added by atomics: the same inputs give the same bits.
+// a graph) and of 32-bit operands, on the CUDA cores; sequences of ATTN_TILE_QUERIES queries and more in 16 bits (of fewer over many pairs,
+// attn_in_tiles) are tiles on the tensor cores (attention_mma.cu).  Nothing is added by atomics: the same call gives the same bits.  How the
+// lanes of a warp share a row follows from the call's keys a sequence on average, so in another batch a row's sums may have another order.
 #include "attention.h"
 
 namespace dgs {
@@ -861,8 +862,7 @@ struct Layout {
 };
 
 // Parts that rows with many keys can have, whatever the offsets: parts <= k_len / ATTN_SPLIT_KEYS + 1 for each of a sequence's queries
-// (none, and no launch for them, where all keys together are too few for one: whether a row is split is a matter of its own keys alone, so
-// that it has the same bits in every batch)
+// (none, and no launch for them, where all keys together are too few for one: whether a row is split is a matter of its own keys alone)
 int64_t split_bound(int64_t n_q, int64_t n_k, int64_t seqs) {
   if (n_k <= ATTN_SPLIT_FROM) return 0;
   const int64_t queries = n_q < ATTN_SPLIT_QUERIES ? n_q : ATTN_SPLIT_QUERIES;
