@@ -15,6 +15,8 @@
 //   dpost_weight = gate S2,  dpost_bias = gate S3,  dgate = post_weight S2 + post_bias S3
 // At 12 bytes an element the issue slots allow some 60 instructions: weights lie in shared memory in 32 bits (a quarter of a load each, no
 // conversion), arithmetic is two elements an instruction, and with 16 elements a thread a row's sums over the CTA cost a twentieth.
+// Measured, 16 384 x 4 096 bfloat16, both norms and a gate of the columns: forward 131 us (3.5 TB/s of DRAM, 62 % of the issue slots), backward
+// 244 us (3.2 TB/s).
 #include <initializer_list>
 
 #include "train_common.cuh"
