@@ -208,6 +208,7 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
       }
     }
     if (ok && blocks > 0) ok = !*dead && bar_wait(done, 0);
+    ok = __all_sync(FULL_MASK, ok);  // (the loads below are the whole warp's)
     if (ok) {
       // ---- results: a row of the weight a thread
       fence_after();
@@ -224,35 +225,37 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0;
           }
-          if (o >= outs) continue;
-          const int64_t at = static_cast<int64_t>(o0 + o) * a.D + d0 + q * 32;
-          const int left = cols - q * 32;
-          if (a.splits == 1) {
-            uint16_t* to = static_cast<uint16_t*>(a.dweight) + at;
-            if (left >= 32 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+          if (o < outs) {
+            const int64_t at = static_cast<int64_t>(o0 + o) * a.D + d0 + q * 32;
+            const int left = cols - q * 32;
+            if (a.splits == 1) {
+              uint16_t* to = static_cast<uint16_t*>(a.dweight) + at;
+              if (left >= 32 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t y[4];
+                for (int i = 0; i < 4; ++i) {
+                  uint32_t y[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = pack2<BF16>(__uint_as_float(v[i * 8 + e * 2]), __uint_as_float(v[i * 8 + e * 2 + 1]));
-                reinterpret_cast<uint4*>(to)[i] = make_uint4(y[0], y[1], y[2], y[3]);
+                  for (int e = 0; e < 4; ++e) y[e] = pack2<BF16>(__uint_as_float(v[i * 8 + e * 2]), __uint_as_float(v[i * 8 + e * 2 + 1]));
+                  reinterpret_cast<uint4*>(to)[i] = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (i < left) to[i] = static_cast<uint16_t>(pack2<BF16>(__uint_as_float(v[i]), 0.0f));
               }
             } else {
+              float* to = a.parts + static_cast<int64_t>(split) * a.O * a.D + at;
+              if (left >= 32 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i < left) to[i] = static_cast<uint16_t>(pack2<BF16>(__uint_as_float(v[i]), 0.0f));
-            }
-          } else {
-            float* to = a.parts + static_cast<int64_t>(split) * a.O * a.D + at;
-            if (left >= 32 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+                for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+              } else {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i < left) to[i] = __uint_as_float(v[i]);
+                for (int i = 0; i < 32; ++i)
+                  if (i < left) to[i] = __uint_as_float(v[i]);
+              }
             }
           }
+          __syncwarp();
         }
       }
       if (sums) {
