@@ -174,6 +174,7 @@ ABI_SIGNATURES = {
     "dgs_adamw_step_8bit": (ctypes.c_int, [_AP, _I32, _VP, _VP, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _VP]),
     "dgs_adamw_step_8bit_unbiased": (ctypes.c_int, [_AP, _I32, _VP, _VP, _VP, _VP, _F64, _F64, _F64, _F64, _F64, _I64, _U64, _VP]),
     "dgs_adamw_state_values": (ctypes.c_int, [_VP, _I32, _VP, _I64, _VP, _VP]),
+    "dgs_set_wait_limit": (_I64, [_I64]),
     "dgs_attention_workspace_bytes": (_SZ, [_TP, _I32]),
     "dgs_attention_forward": (ctypes.c_int, [_TP, _VP, _VP, _VP, _SZ, _VP, _VP]),
     "dgs_attention_backward": (ctypes.c_int, [_TP, _VP, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP]),

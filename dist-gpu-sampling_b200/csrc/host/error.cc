@@ -1,6 +1,7 @@
 // Thread-local error text behind dgs_last_error(); replaces the reference's
 // print-and-exit macros (CUDA_CALL / NCCL_CALL / SHM_CHECK,
 // src/dgs_headers.h:11-45): failures are returned to the caller as codes.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -10,6 +11,7 @@
 namespace dgs {
 namespace {
 thread_local char g_err[512] = "";
+std::atomic<int64_t> g_wait_limit{2000000000};
 }
 
 void set_error(const char* fmt, ...) {
@@ -31,6 +33,8 @@ bool chained_launches_enabled(int site) {
   return ((off >> site) & 1ul) == 0;
 }
 
+uint64_t wait_limit() { return static_cast<uint64_t>(g_wait_limit.load(std::memory_order_relaxed)); }
+
 int cuda_fail(cudaError_t e, const char* what, const char* file, int line) {
   set_error("%s:%d: %s failed: %s (%d)", file, line, what, cudaGetErrorString(e), static_cast<int>(e));
   return DGS_ERR_CUDA;
@@ -38,6 +42,8 @@ int cuda_fail(cudaError_t e, const char* what, const char* file, int line) {
 }  // namespace dgs
 
 extern "C" const char* dgs_last_error(void) { return dgs::g_err; }
+
+extern "C" int64_t dgs_set_wait_limit(int64_t nanoseconds) { return dgs::g_wait_limit.exchange(nanoseconds < 0 ? 0 : nanoseconds); }
 
 extern "C" int dgs_device_check(void) {
   int dev = 0;

@@ -943,6 +943,7 @@ AttnArgs arguments(const dgs_attention& p) {
   a.causal = p.causal != 0;
   a.singles = p.n_q <= 2 * static_cast<int64_t>(p.seqs) && p.heads <= ATTN_SINGLE_GROUP * p.kv_heads;
   a.scale = p.scale;
+  a.wait_limit = wait_limit();
   return a;
 }
 

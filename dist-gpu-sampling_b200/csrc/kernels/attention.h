@@ -47,6 +47,7 @@ struct AttnArgs {
   float *delta, *lse2;  // [heads, n_q]; lse in powers of two, as the tiles' backward pass takes it
   float* norms;                 // [2] the largest row norms of dout and v (as they are ordered, through unsigned words)
   int32_t* status;
+  uint64_t wait_limit;  // of a wait, in nanoseconds
   int32_t split_bound, q_tile_bound, k_tile_bound, q_tile_rows, head_pairs;
   // rows on the CUDA cores: key heads side by side in a warp (and in those of a split row), rows that it looks up at once
   int32_t side, split_side, rows_at_once;

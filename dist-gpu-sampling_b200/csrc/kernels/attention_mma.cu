@@ -86,7 +86,7 @@ template <int DP, int STAGES>
 struct Loader {
   uint32_t tiles, full, empty;  // shared memory of the stages, their barriers
   int t;
-  const volatile int* dead;
+  Waits wait;
   int at = 0;        // stages filled
   int waiting = 0;   // the newest of them that came by cp.async and are not handed over
 
@@ -114,7 +114,7 @@ struct Loader {
       bar_arrive(bar);
     }
   }
-  __device__ __forceinline__ bool free_stage() const { return !*dead && bar_wait(empty + 8 * (at % STAGES), ((at / STAGES) & 1) ^ 1); }
+  __device__ __forceinline__ bool free_stage() const { return wait(empty + 8 * (at % STAGES), ((at / STAGES) & 1) ^ 1); }
   // the next stage: rows row.. of a head, `there` of them; zeros: whether those behind them must be zeros
   __device__ __forceinline__ void fill(const CUtensorMap* map, const AttnView& view, int32_t head, int32_t row, int there, bool zeros, int d) {
     const uint32_t dst = tiles + (at % STAGES) * tile_bytes<DP>();
@@ -140,13 +140,13 @@ struct Loader {
 template <int DP, int STAGES>
 struct Stage {
   uint32_t tiles, full, empty;
-  const volatile int* dead;
+  Waits wait;
   int slot = 0;
   uint32_t phase = 0;
   __device__ __forceinline__ int slot_of(int ahead) const { return slot + ahead < STAGES ? slot + ahead : slot + ahead - STAGES; }
   __device__ __forceinline__ uint32_t tile(int ahead) const { return tiles + slot_of(ahead) * tile_bytes<DP>(); }
   __device__ __forceinline__ bool ready(int ahead) const {
-    return !*dead && bar_wait(full + 8 * slot_of(ahead), slot + ahead < STAGES ? phase : phase ^ 1);
+    return wait(full + 8 * slot_of(ahead), slot + ahead < STAGES ? phase : phase ^ 1);
   }
   __device__ __forceinline__ void release(int ahead) const { mma_commit_one(empty + 8 * slot_of(ahead)); }
   __device__ __forceinline__ void advance(int by) {
@@ -305,6 +305,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
   pdl_enter();
   const int group = a.heads / a.kv_heads, heads = a.head_pairs ? a.heads / 2 : a.heads;  // an item is a tile of queries and a head, or two of them
   const int64_t items = static_cast<int64_t>(min(a.counts[ATTN_N_Q_TILES], a.q_tile_bound)) * heads;
+  const Waits wait{dead, a.wait_limit};
   bool ok = true;
 
   if (warp > SOFTMAX_WARPS) {
@@ -312,14 +313,14 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
     fewer_registers<FEW_REGISTERS>();
     if (warp <= SOFTMAX_WARPS + LOAD_WARPS) {  // (the last warp fills the warpgroup)
       fence_async_global();  // rows that ordinary stores of an earlier launch wrote
-      Loader<DP, STAGES> load{smem + Shape::RING, full, empty, static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32, dead};
+      Loader<DP, STAGES> load{smem + Shape::RING, full, empty, static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32, wait};
       int n = 0;  // items with keys so far
       for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
         const int index = static_cast<int>(item / heads), head = static_cast<int>(item - static_cast<int64_t>(index) * heads) << a.head_pairs;
         const AttnTile x = tile_at(a.q_tiles + index);
         if (x.steps == 0) continue;
         const int slot = n % QUERIES;
-        if (!(ok = !*dead && bar_wait(q_empty + 8 * slot, ((n / QUERIES) & 1) ^ 1))) break;
+        if (!(ok = wait(q_empty + 8 * slot, ((n / QUERIES) & 1) ^ 1))) break;
         load.boxes(smem + slot * Shape::QUERY_BYTES, &args.q, head, x.row, &args.q, head + a.head_pairs, a.head_pairs ? x.row : x.row + ATTN_TILE,
                    a.head_pairs || x.rows > ATTN_TILE, q_full + 8 * slot);
         // K0, V0, K1, V1, ..  (only V's rows are summed over)
@@ -339,14 +340,14 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
     fewer_registers<FEW_REGISTERS>();
     if (lane == 0) {
       const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
-      Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
+      Stage<DP, STAGES> st{smem + Shape::RING, full, empty, wait};
       uint32_t p_phase[2] = {0, 0};
       int n = 0;
       // O += P V of the tile of queries w, then S of the next keys
       const auto step = [&](auto which, uint32_t q, bool first, bool more) {
         constexpr uint32_t w = decltype(which)::value;
         const uint32_t s = tmem + w * 128;
-        if (*dead || !bar_wait(p_full + 8 * w, p_phase[w])) return false;
+        if (!wait(p_full + 8 * w, p_phase[w])) return false;
         p_phase[w] ^= 1;
         fence_after();
         product_columns<DP>(tmem + 256 + w * DP, s, 32, st.tile(1), by_columns, !first);
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
         const bool two = a.head_pairs || x.rows > ATTN_TILE;
         const int slot = n % QUERIES;
         const uint32_t q = smem + slot * Shape::QUERY_BYTES;
-        if (!(ok = !*dead && bar_wait(q_full + 8 * slot, (n / QUERIES) & 1) && st.ready(0))) break;
+        if (!(ok = wait(q_full + 8 * slot, (n / QUERIES) & 1) && st.ready(0))) break;
         fence_after();
         product_rows<DP>(tmem, q, st.tile(0), by_rows);
         mma_commit_one(s_full);
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
         const int first = a.causal ? x.seen + below : x.others;  // keys that the first row of this tile sees
         const int seen = a.causal ? min(x.others, x.seen + mine) : x.others;
         for (int j = 0; j < x.steps; ++j) {
-          if (!(ok = !*dead && bar_wait(s_full + 8 * w, at++ & 1))) break;
+          if (!(ok = wait.warp(s_full + 8 * w, at++ & 1))) break;
           fence_after();
           const int left = seen - j * ATTN_TILE;
           const bool whole = first >= (j + 1) * ATTN_TILE && x.others >= (j + 1) * ATTN_TILE;
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
           bar_arrive(p_full + 8 * w);
         }
         if (!ok) break;
-        if (!(ok = !*dead && bar_wait(o_full + 8 * w, o_at++ & 1))) break;
+        if (!(ok = wait.warp(o_full + 8 * w, o_at++ & 1))) break;
         fence_after();
       }
       if (below >= x.rows) continue;
@@ -664,6 +665,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
   pdl_enter();
   Items items(a.k_tiles, min(a.counts[ATTN_N_K_TILES], a.k_tile_bound), a.kv_heads);
   const int group = a.heads / a.kv_heads;
+  const Waits wait{dead, a.wait_limit};
   bool ok = true;
 
   if (warp > SOFTMAX_WARPS) {
@@ -672,21 +674,21 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
     if (warp <= SOFTMAX_WARPS + LOAD_WARPS) {
       fence_async_global();
       const int t = static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32;
-      Loader<DP, STAGES> load{smem + Shape::RING, full, empty, t, dead};
+      Loader<DP, STAGES> load{smem + Shape::RING, full, empty, t, wait};
       int n = 0, step = 0;
       for (; ok && items.more(); items.advance()) {
         const int kv = items.head;
         const AttnTile& x = items.x;
         if (x.steps == 0) continue;
         const int own = n % ITEMS;
-        if (!(ok = !*dead && bar_wait(kv_empty + 8 * own, ((n / ITEMS) & 1) ^ 1))) break;
+        if (!(ok = wait(kv_empty + 8 * own, ((n / ITEMS) & 1) ^ 1))) break;
         load.boxes(smem + own * Shape::OWN_BYTES, &args.k, kv, x.row, &args.v, kv, x.row, true, kv_full + 8 * own);
         for (int u = 0; ok && u < x.steps * group; ++u, ++step) {
           const int head = kv * group + u / x.steps, at = u % x.steps * ATTN_TILE, row = x.other + at, left = x.others - at;
           if (!(ok = load.free_stage())) break;
           load.fill(&args.q, a.q, head, row, left, true, a.d);
           const int slot = step & 1;
-          if (!(ok = !*dead && bar_wait(stats_empty + 8 * slot, ((step >> 1) & 1) ^ 1))) break;
+          if (!(ok = wait(stats_empty + 8 * slot, ((step >> 1) & 1) ^ 1))) break;
           const uint32_t to = smem + Shape::STATS + slot * 2 * ATTN_TILE * 4;
           const int64_t from = static_cast<int64_t>(head) * a.n_q + row;
 #pragma unroll
@@ -713,7 +715,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
     if (lane == 0) {
       const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
       const uint32_t s = tmem, e = tmem + 128, dv = tmem + 256, dk = tmem + 256 + DP;
-      Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
+      Stage<DP, STAGES> st{smem + Shape::RING, full, empty, wait};
       int n = 0;
       uint32_t at = 0;
       for (; ok && items.more(); items.advance()) {
@@ -721,7 +723,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
         if (x.steps == 0) continue;
         const int own = n % ITEMS;
         const uint32_t k = smem + own * Shape::OWN_BYTES, v = k + tile_bytes<DP>();
-        if (!(ok = !*dead && bar_wait(kv_full + 8 * own, (n / ITEMS) & 1) && st.ready(0))) break;
+        if (!(ok = wait(kv_full + 8 * own, (n / ITEMS) & 1) && st.ready(0))) break;
         fence_after();
         product_rows<DP>(s, k, st.tile(0), by_rows);
         mma_commit_one(s_full);
@@ -731,7 +733,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
         const int steps = x.steps * group;
         for (int u = 0; ok && u < steps; ++u, at ^= 1) {
           const bool more = u + 1 < steps;
-          if (!(ok = (!more || st.ready(2)) && !*dead && bar_wait(p_full, at))) break;
+          if (!(ok = (!more || st.ready(2)) && wait(p_full, at))) break;
           fence_after();
           product_columns<DP>(dv, s, 64, st.tile(1), by_columns, u > 0);
           if (more) {
@@ -739,7 +741,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
             mma_commit_one(s_full);
           }
           st.release(1);
-          if (!(ok = (!more || st.ready(3)) && !*dead && bar_wait(ds_full, at))) break;
+          if (!(ok = (!more || st.ready(3)) && wait(ds_full, at))) break;
           fence_after();
           product_columns<DP>(dk, e, 64, st.tile(0), by_columns, u > 0);
           if (more) {
@@ -776,7 +778,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
       for (int u = 0; u < x.steps * group; ++u, ++at) {
         const int slot = at & 1, q0 = u % x.steps * ATTN_TILE + half * 64;
         const float4* stats = reinterpret_cast<const float4*>(smem_raw + Shape::STATS + slot * 2 * ATTN_TILE * 4 + half * 64 * 4);
-        if (!(ok = !*dead && bar_wait(stats_full + 8 * slot, (at >> 1) & 1) && bar_wait(s_full, at & 1))) break;
+        if (!(ok = wait.warp(stats_full + 8 * slot, (at >> 1) & 1) && wait.warp(s_full, at & 1))) break;
         fence_after();
         uint32_t r[2][32];
         float p[64];
@@ -803,7 +805,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
         tmem_store_wait();
         fence_before();
         bar_arrive(p_full);
-        if (!(ok = !*dead && bar_wait(e_full, at & 1))) break;
+        if (!(ok = wait.warp(e_full, at & 1))) break;
         fence_after();
         tmem_load32(e, r[0]);
         tmem_load32(e + 32, r[1]);
@@ -826,7 +828,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
         bar_arrive(ds_full);
       }
       if (!ok) break;
-      if (!(ok = !*dead && bar_wait(done, items_done++ & 1))) break;
+      if (!(ok = wait.warp(done, items_done++ & 1))) break;
       fence_after();
       const float last = half ? a.scale / (by * exp2f(lift<BF16>())) : exp2f(-lift<BF16>());
       store_row<0, DP, BF16>(tmem + 256 + half * DP + lanes, there, last, to, a.d);
@@ -898,6 +900,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
   pdl_enter();
   Items items(a.q_tiles, min(a.counts[ATTN_N_Q_TILES], a.q_tile_bound), a.heads);
   const int group = a.heads / a.kv_heads;
+  const Waits wait{dead, a.wait_limit};
   bool ok = true;
 
   if (warp > SOFTMAX_WARPS) {
@@ -905,7 +908,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
     fewer_registers<FEW_REGISTERS>();
     if (warp <= SOFTMAX_WARPS + LOAD_WARPS) {
       fence_async_global();
-      Loader<DP, STAGES> load{smem + Shape::RING, full, empty, static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32, dead};
+      Loader<DP, STAGES> load{smem + Shape::RING, full, empty, static_cast<int>(threadIdx.x) - (SOFTMAX_WARPS + 1) * 32, wait};
       int n = 0;
       for (; ok && items.more(); items.advance()) {
         const int head = items.head;
@@ -913,7 +916,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
         const int steps = query_steps(a, x);
         if (steps == 0) continue;
         const int own = n % ITEMS;
-        if (!(ok = !*dead && bar_wait(q_empty + 8 * own, ((n / ITEMS) & 1) ^ 1))) break;
+        if (!(ok = wait(q_empty + 8 * own, ((n / ITEMS) & 1) ^ 1))) break;
         load.boxes(smem + own * Shape::OWN_BYTES, &args.q, head, x.row, &args.dout, head, x.row, true, q_full + 8 * own);
         // K0, V0, K1, V1, ..  (K's rows are summed over)
         for (int j = 0; ok && j < steps; ++j) {
@@ -933,7 +936,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
     if (lane == 0) {
       const uint32_t by_rows = mma_desc(BF16, false, false, ATTN_TILE, ATTN_TILE), by_columns = mma_desc(BF16, false, true, ATTN_TILE, DP);
       const uint32_t e = tmem + 256, dq = tmem + 384;
-      Stage<DP, STAGES> st{smem + Shape::RING, full, empty, dead};
+      Stage<DP, STAGES> st{smem + Shape::RING, full, empty, wait};
       int n = 0;
       uint32_t at = 0;
       for (; ok && items.more(); items.advance()) {
@@ -942,7 +945,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
         if (steps == 0) continue;
         const int own = n % ITEMS;
         const uint32_t q = smem + own * Shape::OWN_BYTES, g = q + tile_bytes<DP>();
-        if (!(ok = !*dead && bar_wait(q_full + 8 * own, (n / ITEMS) & 1) && st.ready(0))) break;
+        if (!(ok = wait(q_full + 8 * own, (n / ITEMS) & 1) && st.ready(0))) break;
         fence_after();
         product_rows<DP>(tmem + (at & 1) * 128, q, st.tile(0), by_rows);
         mma_commit_one(s_full + 8 * (at & 1));
@@ -955,13 +958,13 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
             if (!(ok = st.ready(2))) break;
             product_rows<DP>(tmem + ((at + 1) & 1) * 128, q, st.tile(2), by_rows);
             mma_commit_one(s_full + 8 * ((at + 1) & 1));
-            if (!(ok = st.ready(3) && !*dead && bar_wait(e_read, at & 1))) break;
+            if (!(ok = st.ready(3) && wait(e_read, at & 1))) break;
             fence_after();
             product_rows<DP>(e, g, st.tile(3), by_rows);
             mma_commit_one(e_full);
             st.release(3);
           }
-          if (!(ok = !*dead && bar_wait(ds_full + 8 * (at & 1), (at >> 1) & 1))) break;
+          if (!(ok = wait(ds_full + 8 * (at & 1), (at >> 1) & 1))) break;
           fence_after();
           product_columns<DP>(dq, tmem + (at & 1) * 128, 64, st.tile(0), by_columns, j > 0);
           st.release(0);
@@ -1001,7 +1004,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
       const int seen = a.causal ? min(x.others, x.seen + mine) : x.others, first = first_seen(a, x);
       for (int j = 0; j < steps; ++j, ++at) {
         const uint32_t s = tmem + (at & 1) * 128 + half * 64 + lanes;
-        if (!(ok = !*dead && bar_wait(s_full + 8 * (at & 1), (at >> 1) & 1))) break;
+        if (!(ok = wait.warp(s_full + 8 * (at & 1), (at >> 1) & 1))) break;
         fence_after();
         uint32_t r[2][32];
         float p[64];
@@ -1011,7 +1014,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
         tmem_wait(r[1]);
 #pragma unroll
         for (int i = 0; i < 64; ++i) p[i] = ex2(fmaf(__uint_as_float(r[i / 32][i % 32]), c, -lse));
-        if (!(ok = !*dead && bar_wait(e_full, at & 1))) break;
+        if (!(ok = wait.warp(e_full, at & 1))) break;
         fence_after();
         tmem_load32(e, r[0]);
         tmem_load32(e + 32, r[1]);
@@ -1028,7 +1031,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
           float* slot = near + (joined & 1) * 2 * ATTN_TILE;
           slot[half * ATTN_TILE + mine] = sum;
           bar_arrive(near_full);
-          if (!(ok = !*dead && bar_wait(near_full, joined++ & 1))) break;
+          if (!(ok = wait.warp(near_full, joined++ & 1))) break;
           if (seen <= ATTN_TILE) {
             delta = (slot[mine] + slot[ATTN_TILE + mine]) * exp2f(-lift<BF16>());
             if (half == 0 && there) a.delta[stat] = delta;
@@ -1049,7 +1052,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
         bar_arrive(ds_full + 8 * (at & 1));
       }
       if (!ok) break;
-      if (!(ok = !*dead && bar_wait(done, items_done++ & 1))) break;
+      if (!(ok = wait.warp(done, items_done++ & 1))) break;
       fence_after();
       const float last = a.scale / (by * exp2f(lift<BF16>()));
       const bool wanted = there && a.dq != nullptr;

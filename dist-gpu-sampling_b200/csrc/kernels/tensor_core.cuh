@@ -73,15 +73,40 @@ __device__ __forceinline__ uint64_t nanoseconds() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint64_t limit = kWaitNanoseconds) {
   if (bar_try(bar, parity)) return true;
   const uint64_t began = nanoseconds();
   for (uint32_t polls = 1; polls < kWaitPolls; ++polls) {
     if (bar_try(bar, parity)) return true;
-    if ((polls & 255) == 0 && nanoseconds() - began > kWaitNanoseconds) return false;
+    if ((polls & 255) == 0 && nanoseconds() - began > limit) return false;
   }
   return false;
 }
+// whether the phase is over, without a wait
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// The waits of a CTA whose roles give up together: none once one of them has, or beyond `limit` nanoseconds (0: none that would have to
+// wait).
+struct Waits {
+  const volatile int* dead;
+  uint64_t limit;
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
+    if (*dead) return false;
+    if (limit == 0) return bar_test(bar, parity);
+    return bar_wait(bar, parity, limit);
+  }
+  // all lanes of a warp go on, or none does: what follows may be an instruction of the whole warp
+  __device__ __forceinline__ bool warp(uint32_t bar, uint32_t parity) const { return __all_sync(FULL_MASK, (*this)(bar, parity)); }
+};
 
 // ---- TMA ----------------------------------------------------------------------------------------------------------
 // One box into this CTA's shared memory; `cluster_bar` may be the other CTA's barrier.

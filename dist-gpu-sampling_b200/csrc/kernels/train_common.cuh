@@ -29,6 +29,9 @@ static inline int sm_count() {
   return sms;
 }
 
+// how long a wait of a kernel may take, in nanoseconds (host/error.cc)
+uint64_t wait_limit();
+
 #ifdef __CUDACC__
 
 template <typename T>

@@ -481,6 +481,13 @@ DGS_API int dgs_adamw_step_8bit_unbiased(const dgs_adamw_tensor* tensors, int32_
 DGS_API int dgs_adamw_state_values(const void* codes, int32_t second, const float* scales, int64_t n, float* out,
                                    dgs_stream_t stream);
 
+/* How long the tensor-core kernels of attention let one of their waits (for tiles, for
+ * products) take before they raise DGS_ERR_CUDA in the status word and leave: 2 s
+ * unless it is set, in nanoseconds; 0 (and less): a wait that would have to wait is
+ * given up.  For the whole process, for calls made or recorded from then on; returns
+ * the limit before. */
+DGS_API int64_t dgs_set_wait_limit(int64_t nanoseconds);
+
 /* Softmax attention of packed sequences: sequence s holds the query rows
  * [q_offsets[s], q_offsets[s + 1]) and the key and value rows of k_offsets (for a
  * sampled block the queries are its seeds and k_offsets is its indptr).  Query head a
