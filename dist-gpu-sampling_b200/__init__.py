@@ -185,6 +185,7 @@ ABI_SIGNATURES = {
     "dgs_kept_8bit_values": (ctypes.c_int, [_VP, _I64, _VP, _I64, _I64, _I32, _VP, _VP]),
     "dgs_kept_8bit_weight_grad_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
     "dgs_kept_8bit_weight_grad": (ctypes.c_int, [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _I64, _I64, _VP, _VP, _VP, _SZ, _VP]),
+    "dgs_kept_8bit_weight_grad_reported": (ctypes.c_int, [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _I64, _I64, _VP, _VP, _VP, _SZ, _VP, _VP]),
 }
 
 

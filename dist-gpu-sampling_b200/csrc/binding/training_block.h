@@ -383,8 +383,11 @@ inline std::tuple<torch::Tensor, torch::Tensor> Kept8bitWeightGradCUDA(torch::Te
   torch::Tensor db = device_empty({want_bias ? O : 0}, grad.scalar_type(), grad.device());
   const size_t wb = dgs_kept_8bit_weight_grad_workspace_bytes(n, O, D, dtype);
   torch::Tensor ws = byte_scratch(wb, grad.device());
-  DGS_CHECK_RC(dgs_kept_8bit_weight_grad(g.t.data_ptr(), g.stride, dtype, c.t.data_ptr<int8_t>(), c.stride, scales.data_ptr<float>(), n, O, D,
-                                         dw.data_ptr(), want_bias ? db.data_ptr() : nullptr, ws.data_ptr(), wb, current_stream()));
+  const CallStatus w(op, grad.device().index(), current_stream());
+  DGS_CHECK_RC(dgs_kept_8bit_weight_grad_reported(g.t.data_ptr(), g.stride, dtype, c.t.data_ptr<int8_t>(), c.stride, scales.data_ptr<float>(), n,
+                                                  O, D, dw.data_ptr(), want_bias ? db.data_ptr() : nullptr, ws.data_ptr(), wb, w.status(),
+                                                  current_stream()));
+  w.finish();
   return std::make_tuple(dw, db);
 }
 

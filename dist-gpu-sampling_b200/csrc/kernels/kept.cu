@@ -410,6 +410,14 @@ extern "C" size_t dgs_kept_8bit_weight_grad_workspace_bytes(int64_t n, int64_t O
 extern "C" int dgs_kept_8bit_weight_grad(const void* grad, int64_t grad_stride, int32_t dtype, const int8_t* codes, int64_t codes_stride,
                                          const float* scales, int64_t n, int64_t O, int64_t D, void* dweight, void* dbias,
                                          void* workspace, size_t workspace_bytes, dgs_stream_t stream) {
+  return dgs_kept_8bit_weight_grad_reported(grad, grad_stride, dtype, codes, codes_stride, scales, n, O, D, dweight, dbias, workspace,
+                                            workspace_bytes, nullptr, stream);
+}
+
+extern "C" int dgs_kept_8bit_weight_grad_reported(const void* grad, int64_t grad_stride, int32_t dtype, const int8_t* codes,
+                                                  int64_t codes_stride, const float* scales, int64_t n, int64_t O, int64_t D, void* dweight,
+                                                  void* dbias, void* workspace, size_t workspace_bytes, int32_t* status,
+                                                  dgs_stream_t stream) {
   if (int rc = check("kept_8bit_weight_grad", n, D, dtype)) return rc;
   // (tiles of the weight's rows are the grid's second extent, below 2^16; the join's CTAs its first, below 2^31)
   DGS_REQUIRE(O >= 1 && O < KEPT_MAX_SIDE / 2 && O * D < (int64_t(1) << 35), DGS_ERR_INVALID, "kept_8bit_weight_grad: a weight of %lld rows of %lld",
@@ -441,5 +449,7 @@ extern "C" int dgs_kept_8bit_weight_grad(const void* grad, int64_t grad_stride, 
   a.bias_parts = a.parts + static_cast<int64_t>(a.splits) * O * D;
   a.dweight = dweight;
   a.dbias = dbias;
+  a.status = status;
+  a.wait_limit = wait_limit();
   return weight_grad(a, dtype, s);
 }

@@ -16,6 +16,8 @@ struct KeptGradArgs {
   int32_t O, D, groups, splits;
   float *parts, *bias_parts;  // [splits][O][D], [splits][O]
   void *dweight, *dbias;
+  int32_t* status;
+  uint64_t wait_limit;  // of a wait, in nanoseconds
 };
 
 // kept_mma.cu: 16-bit gradients on the tensor cores; one share writes the results, several leave parts to be added

@@ -5,6 +5,7 @@
 // values and leave both in shared memory as they lie (the sum's index outermost: MN-major tiles), a thread of a seventeenth issues the
 // products (cta_group::1, two accumulators of 128 x 256 in TMEM).  The next blocks are on their way in registers.
 // With few results the rows are cut into shares that fill the SMs; shares are added in their order by a second launch.
+// Every wait is bounded; one that runs out raises DGS_ERR_CUDA in the status word, leaves no number among the CTA's results, and all roles leave.
 // Bound by turning codes into operands: 430 000 rows of 256 against 47 (358 bytes a row) 57 us = 2.7 TB/s, 16 384 x 4 096 against 1 024 168 us =
 // 820 TFLOP/s with the tensor pipe 40 % active, each with 9 to 10 us of joins behind it.
 #include "kept.h"
@@ -120,6 +121,7 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
   const int64_t r0 = a.n * split / a.splits, r1 = a.n * (split + 1) / a.splits;
   const int blocks = static_cast<int>((r1 - r0 + ROWS - 1) / ROWS);
   const int cols = min(TILE, a.D - d0), outs = min(TILE, a.O - o0);
+  const Waits wait{dead, a.wait_limit};
   bool ok = true;
 
   if (warp < FETCH_WARPS) {
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
 #pragma unroll
       for (int w = 0; w < DEPTH; ++w) {
         if (!ok || b0 + w >= blocks) continue;
-        if (!(ok = !*dead && bar_wait(empty + 8 * slot, phase ^ 1))) continue;
+        if (!(ok = wait(empty + 8 * slot, phase ^ 1))) continue;
         store(on_way[w]);
         fence_async_smem();
         bar_arrive(full + 8 * slot);
@@ -207,8 +209,7 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
         if (++slot == STAGES) slot = 0, phase ^= 1;
       }
     }
-    if (ok && blocks > 0) ok = !*dead && bar_wait(done, 0);
-    ok = __all_sync(FULL_MASK, ok);  // (the loads below are the whole warp's)
+    ok = __all_sync(FULL_MASK, ok && (blocks == 0 || wait(done, 0)));  // (the loads below are the whole warp's)
     if (ok) {
       // ---- results: a row of the weight a thread
       fence_after();
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
 #pragma unroll
         for (int e = 0; e < 8; ++e) part[g_row * G_CHUNKS * 8 + g_chunk * 8 + e] = db[e];
         bar_arrive(summed);
-        ok = !*dead && bar_wait(summed, 0);
+        ok = wait(summed, 0);
         if (ok && static_cast<int>(threadIdx.x) < outs) {
           float s = 0.0f;
 #pragma unroll 8
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
       int slot = 0;
       uint32_t phase = 0;
       for (int b = 0; b < blocks; ++b) {
-        if (!(ok = !*dead && bar_wait(full + 8 * slot, phase))) break;
+        if (!(ok = wait(full + 8 * slot, phase))) break;
         fence_after();
         const uint64_t da = smem_desc(smem + slot * STAGE, PANEL, 1024), dv = smem_desc(smem + slot * STAGE + OPERAND, PANEL, 1024);
 #pragma unroll
@@ -298,14 +299,26 @@ __global__ __launch_bounds__(THREADS, 1) void kept_mma_kernel(const __grid_const
     }
   }
   __syncwarp();
-  if (!ok) *dead = 1;
+  if (!ok) {
+    *dead = 1;
+    raise_status(a.status, DGS_ERR_CUDA);
+  }
   __syncthreads();
   if (*dead) {
-    // (no status word here: an error leaves the results not a number)
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-    if (threadIdx.x == 0) {
-      if (a.splits > 1) a.parts[static_cast<int64_t>(split) * a.O * a.D + static_cast<int64_t>(o0) * a.D + d0] = __uint_as_float(0x7fffffffu);
-      else static_cast<uint16_t*>(a.dweight)[static_cast<int64_t>(o0) * a.D + d0] = 0x7fffu;
+    // (found anew, so that nothing of it is held all the way here)
+    const int d0 = blockIdx.x * TILE, o0 = blockIdx.y * TILE, split = blockIdx.z, cols = min(TILE, a.D - d0), outs = min(TILE, a.O - o0);
+    // a call without a status word shows it too: none of this CTA's results is a number
+    for (int i = threadIdx.x; i < outs * cols; i += THREADS) {
+      const int64_t at = static_cast<int64_t>(o0 + i / cols) * a.D + d0 + i % cols;
+      if (a.splits > 1) a.parts[static_cast<int64_t>(split) * a.O * a.D + at] = __uint_as_float(0x7fffffffu);
+      else static_cast<uint16_t*>(a.dweight)[at] = 0x7fffu;
+    }
+    if (a.dbias != nullptr && blockIdx.x == 0) {
+      for (int i = threadIdx.x; i < outs; i += THREADS) {
+        if (a.splits > 1) a.bias_parts[static_cast<int64_t>(split) * a.O + o0 + i] = __uint_as_float(0x7fffffffu);
+        else static_cast<uint16_t*>(a.dbias)[o0 + i] = 0x7fffu;
+      }
     }
   }
   if (warp == 0) {

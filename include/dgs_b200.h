@@ -481,11 +481,11 @@ DGS_API int dgs_adamw_step_8bit_unbiased(const dgs_adamw_tensor* tensors, int32_
 DGS_API int dgs_adamw_state_values(const void* codes, int32_t second, const float* scales, int64_t n, float* out,
                                    dgs_stream_t stream);
 
-/* How long the tensor-core kernels of attention let one of their waits (for tiles, for
- * products) take before they raise DGS_ERR_CUDA in the status word and leave: 2 s
- * unless it is set, in nanoseconds; 0 (and less): a wait that would have to wait is
- * given up.  For the whole process, for calls made or recorded from then on; returns
- * the limit before. */
+/* How long the tensor-core kernels of attention, and of weight gradients from rows
+ * kept in 8 bits, let one of their waits (for tiles, for products) take before they
+ * raise DGS_ERR_CUDA in the status word and leave: 2 s unless it is set, in
+ * nanoseconds; 0 (and less): a wait that would have to wait is given up.  For the
+ * whole process, for calls made or recorded from then on; returns the limit before. */
 DGS_API int64_t dgs_set_wait_limit(int64_t nanoseconds);
 
 /* Softmax attention of packed sequences: sequence s holds the query rows
@@ -575,6 +575,12 @@ DGS_API size_t dgs_kept_8bit_weight_grad_workspace_bytes(int64_t n, int64_t O, i
 DGS_API int dgs_kept_8bit_weight_grad(const void* grad, int64_t grad_stride, int32_t dtype, const int8_t* codes, int64_t codes_stride,
                                       const float* scales, int64_t n, int64_t O, int64_t D, void* dweight, void* dbias,
                                       void* workspace, size_t workspace_bytes, dgs_stream_t stream);
+/* ... which raises DGS_ERR_CUDA in *status (may be NULL, as above) where a wait of the
+ * kernel ran out; results of a part that gave up are not numbers. */
+DGS_API int dgs_kept_8bit_weight_grad_reported(const void* grad, int64_t grad_stride, int32_t dtype, const int8_t* codes,
+                                               int64_t codes_stride, const float* scales, int64_t n, int64_t O, int64_t D,
+                                               void* dweight, void* dbias, void* workspace, size_t workspace_bytes, int32_t* status,
+                                               dgs_stream_t stream);
 
 #ifdef __cplusplus
 }
