@@ -9,6 +9,8 @@
 // a graph) and of 32-bit operands, on the CUDA cores; sequences of ATTN_TILE_QUERIES queries and more in 16 bits (of fewer over many pairs,
 // attn_in_tiles) are tiles on the tensor cores (attention_mma.cu).  Nothing is added by atomics: the same call gives the same bits.  How the
 // lanes of a warp share a row follows from the call's keys a sequence on average, so in another batch a row's sums may have another order.
+#include <type_traits>
+
 #include "attention.h"
 
 namespace dgs {
@@ -542,15 +544,25 @@ __device__ __forceinline__ float reference_of(const AttnArgs& a, int head, int r
   return lse == -INFINITY ? INFINITY : lse;
 }
 
-// Sequences of one query and few keys (a seed over its neighbours): nobody else reads these keys, so one pass over them gives all
-// three gradients.  A warp a query, delta = do.o from the stored result.  Bound by HBM: K and V read, dK and dV written.
+// Sequences of one query and few keys (a seed over its neighbours): nobody else reads these keys, so a warp a query gives all three
+// gradients.  delta = sum_j p_j e_j of values in 32 bits has to be there before the first slope, so the keys are gone over twice: for dv and
+// delta, then for dk.  (do.o of an `out` rounded to 16 bits, which would be there at once, is off most where few keys are averaged: it left dq of two
+// keys 1.95 times as far off as rounding the exact one does, 2 to 6 times where v and do have a common mean.)  Weights and e are held in
+// shared memory in between, HELD / side / R keys of them, all that most rows have; others, and those of three and four heads (which a bound of 128
+// registers leaves little room), are made again.  ONCE: dq = scale (sum p e k - delta sum p k) out of the first pass, else out of the second, which
+// reads K again.  Bound by HBM and by what is under way.  Backward calls, us, 60 000 seeds of up to 15 keys, 4 heads of 64: bfloat16 299, float16 308,
+// float32 416; 2 key heads 240; 5 000 of 100 to 400 keys, 8 heads: bfloat16 1 042 (1 302 without ONCE), float32 2 217.
 template <typename T, int DP, int R>
-__global__ __launch_bounds__(ROW_WARPS * 32, R == 1 ? 4 : 2) void attn_single_backward_kernel(const __grid_constant__ AttnArgs a) {
-  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = 2;
+__global__ __launch_bounds__(ROW_WARPS * 32, R == 1 ? 3 : 2) void attn_single_backward_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = 2, SLOTS = Lanes<T, DP>::SLOTS;
+  constexpr bool ONCE = R == 2 || (R == 1 && sizeof(T) == 2);
+  constexpr int HELD = R <= 2 ? 512 : 1, HELD_STEPS = R <= 2 ? HELD / (U * SLOTS * R) : 0;
+  __shared__ float2 held[ROW_WARPS][HELD];
   pdl_enter();
   if ((a.counts[ATTN_KINDS] >> ATTN_HAS_SINGLE & 1) == 0) return;
   const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads, blocks = (a.kv_heads + a.side - 1) / a.side;
   const Lanes<T, DP> w(a, a.side);
+  float2* const mine = held[warp] + (threadIdx.x & 31) / G * R;
   each_row(
       a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, Range{a.n_q, a.n_q, 0}, blocks,
       a.q_seq, false,
@@ -561,55 +573,123 @@ __global__ __launch_bounds__(ROW_WARPS * 32, R == 1 ? 4 : 2) void attn_single_ba
         const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
         const T* v = static_cast<const T*>(a.v.p) + e.k0 * a.v.row + c * a.v.head + w.vec * VEC;
         const int64_t to = (static_cast<int64_t>(e.k0) * a.kv_heads + c) * a.d + w.vec * VEC, to_row = static_cast<int64_t>(a.kv_heads) * a.d;
-        float q[R][VEC], g[R][VEC], dq[R][VEC], ref[R], delta[R];
+        float q[R][VEC], g[R][VEC], ref[R], delta[R], dq[R][VEC], pk[ONCE ? R : 1][VEC];
         load_heads<T, R>(a.q, row, c * group, group, w.vec, in && seen > 0, 1.0f, q);
         load_heads<T, R>(a.dout, row, c * group, group, w.vec, in && seen > 0, 1.0f, g);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          float o[VEC];
-          const bool there = in && seen > 0 && r < group;
-          load_row<T, VEC>(static_cast<const T*>(a.out) + (static_cast<int64_t>(row) * a.heads + c * group + r) * a.d + w.vec * VEC, there, o);
-          delta[r] = group_sum<G>(dot<VEC>(g[r], o));
-          ref[r] = reference_of(a, c * group + r, row, there);
+          ref[r] = reference_of(a, c * group + r, row, in && seen > 0 && r < group);
+          delta[r] = 0.0f;
 #pragma unroll
-          for (int x = 0; x < VEC; ++x) dq[r][x] = 0.0f;
-        }
-        for (int j = 0; j < seen; j += w.keys * U) {
-          Vec<T, VEC> kr[U], vr[U];
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int at = j + u * w.keys + w.key;
-            const bool there = at < seen && in;
-            kr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(k + at * a.k.row) : Vec<T, VEC>{};
-            vr[u] = there ? *reinterpret_cast<const Vec<T, VEC>*>(v + at * a.v.row) : Vec<T, VEC>{};
+          for (int x = 0; x < VEC; ++x) {
+            dq[r][x] = 0.0f;
+            if (ONCE) pk[r][x] = 0.0f;
           }
+        }
+        const auto rows_of = [&](const T* p, int64_t p_row, int j, Vec<T, VEC> (&x)[U]) {
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const int at = j + u * w.keys + w.key;
-            float kf[VEC], vf[VEC], dk[VEC], dv[VEC];
+            x[u] = at < seen && in ? *reinterpret_cast<const Vec<T, VEC>*>(p + at * p_row) : Vec<T, VEC>{};
+          }
+        };
+        const auto floats_of = [&](const Vec<T, VEC>& x, float (&f)[VEC]) {
+          if constexpr (R == 1 && sizeof(T) == 2) {  // (kept in their place: moved ahead of one another they take more registers than there are)
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) {
-              kf[x] = to_float<T>(kr[u].v[x]);
-              vf[x] = to_float<T>(vr[u].v[x]);
-              dk[x] = dv[x] = 0.0f;
+            for (int i = 0; i < VEC; i += 2) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(&x.v[i]);
+              if constexpr (std::is_same_v<T, __half>) {
+                asm volatile("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}"
+                             : "=f"(f[i]), "=f"(f[i + 1])
+                             : "r"(w));
+              } else {
+                uint32_t lo, hi;
+                asm volatile("shl.b32 %0, %2, 16;\n\tand.b32 %1, %2, 0xffff0000;" : "=r"(lo), "=r"(hi) : "r"(w));
+                f[i] = __uint_as_float(lo), f[i + 1] = __uint_as_float(hi);
+              }
             }
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = to_float<T>(x.v[i]);
+          }
+        };
+        // a weight and e = do.v
+        const auto pair = [&](int r, int at, const float (&kf)[VEC], const float (&vf)[VEC]) {
+          const float x = group_sum<G>(dot<VEC>(q[r], kf)) * (a.scale * LOG2E), y = group_sum<G>(dot<VEC>(g[r], vf));
+          return make_float2(at < seen && r < group ? ex2(x - ref[r]) : 0.0f, y);
+        };
+        __syncwarp();  // (the row before has read what it held)
+        for (int j = 0, step = 0; j < seen; j += w.keys * U, ++step) {
+          Vec<T, VEC> kr[U], vr[U];
+          rows_of(k, a.k.row, j, kr);
+          rows_of(v, a.v.row, j, vr);
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int at = j + u * w.keys + w.key;
+            float kf[VEC], vf[VEC], dv[VEC];
+            floats_of(kr[u], kf);
+            floats_of(vr[u], vf);
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) dv[x] = 0.0f;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-              const float x = group_sum<G>(dot<VEC>(q[r], kf)) * (a.scale * LOG2E), y = group_sum<G>(dot<VEC>(g[r], vf));
-              const float p = at < seen && r < group ? ex2(x - ref[r]) : 0.0f, ds = p * (y - delta[r]) * a.scale;
-              add_scaled<VEC>(p, g[r], dv);
-              add_scaled<VEC>(ds, q[r], dk);
-              add_scaled<VEC>(ds, kf, dq[r]);
+              const float2 pe = pair(r, at, kf, vf);
+              delta[r] = fmaf(pe.x, pe.y, delta[r]);
+              add_scaled<VEC>(pe.x, g[r], dv);
+              if constexpr (ONCE) {
+                add_scaled<VEC>(pe.x * pe.y, kf, dq[r]);
+                add_scaled<VEC>(pe.x, kf, pk[r]);
+              }
+              if (HELD_STEPS > 0 && w.vec == 0 && step < HELD_STEPS) mine[(step * U + u) * SLOTS * R + r] = pe;
             }
-            if (a.dk != nullptr && at < seen && in) {
-              store_vec<T, VEC>(static_cast<T*>(a.dk) + to + at * to_row, dk);
-              store_vec<T, VEC>(static_cast<T*>(a.dv) + to + at * to_row, dv);
+            if (a.dk != nullptr && at < seen && in) store_vec<T, VEC>(static_cast<T*>(a.dv) + to + at * to_row, dv);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float one[1] = {delta[r]};
+          add_keys<1>(w.side * G, one);
+          delta[r] = one[0];
+        }
+        __syncwarp();
+        if (!ONCE || a.dk != nullptr) {
+          for (int j = 0, step = 0; j < seen; j += w.keys * U, ++step) {
+            Vec<T, VEC> kr[U], vr[U];
+            const bool again = HELD_STEPS == 0 || step >= HELD_STEPS;
+            if (!ONCE || again) rows_of(k, a.k.row, j, kr);
+            if (again) rows_of(v, a.v.row, j, vr);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int at = j + u * w.keys + w.key;
+              float kf[VEC], dk[VEC];
+              if (!ONCE || again) floats_of(kr[u], kf);
+#pragma unroll
+              for (int x = 0; x < VEC; ++x) dk[x] = 0.0f;
+#pragma unroll
+              for (int r = 0; r < R; ++r) {
+                float2 pe;
+                if (again) {
+                  float vf[VEC];
+                  floats_of(vr[u], vf);
+                  pe = pair(r, at, kf, vf);
+                } else {
+                  pe = mine[(step * U + u) * SLOTS * R + r];
+                }
+                const float ds = pe.x * (pe.y - delta[r]) * a.scale;
+                add_scaled<VEC>(ds, q[r], dk);
+                if constexpr (!ONCE) add_scaled<VEC>(ds, kf, dq[r]);
+              }
+              if (a.dk != nullptr && at < seen && in) store_vec<T, VEC>(static_cast<T*>(a.dk) + to + at * to_row, dk);
             }
           }
         }
         if (a.dq == nullptr) return;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
+          if constexpr (ONCE) {
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) dq[r][x] = a.scale * fmaf(-delta[r], pk[r][x], dq[r][x]);
+          }
           add_keys<VEC>(w.side * G, dq[r]);
           if (w.key == 0 && in && r < group)
             store_vec<T, VEC>(static_cast<T*>(a.dq) + (static_cast<int64_t>(row) * a.heads + c * group + r) * a.d + w.vec * VEC, dq[r]);
