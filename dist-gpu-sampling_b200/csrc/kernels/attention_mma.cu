@@ -416,7 +416,8 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
           const int left = seen - j * ATTN_TILE;
           const bool whole = first >= (j + 1) * ATTN_TILE && x.others >= (j + 1) * ATTN_TILE;
           const float top = c * (whole ? largest<false>(s, ATTN_TILE) : largest<true>(s, left));
-          if (__any_sync(FULL_MASK, top > ref + LAZY)) {
+          // (rows behind the sequence's end, which may hold anything, have no say in how those of the sequence are rounded)
+          if (__any_sync(FULL_MASK, there && top > ref + LAZY)) {
             const float next = fmaxf(top, ref), by = next == -INFINITY ? 1.0f : ex2(ref - next);
             ref = next;
             l *= by;
