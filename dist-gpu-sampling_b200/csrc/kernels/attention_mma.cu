@@ -494,7 +494,7 @@ template <bool BF16>
 __device__ __forceinline__ float slope_scale(const AttnArgs& a) {
   if constexpr (BF16) return 1.0f;
   const float b = a.norms[0] * a.norms[1];
-  if (!(b > 0.0f) || b - b != 0.0f) return 1.0f / 4096.0f;
+  if (!(b > 0.0f)) return 1.0f / 4096.0f;
   int e;
   frexpf(b, &e);
   return ldexpf(1.0f, max(-100, min(100, 4 - e)));
@@ -520,6 +520,10 @@ __device__ __forceinline__ void largest_of_cta(float v, float* to) {
   __syncthreads();
   if (threadIdx.x == 0 && top != 0) atomicMax(reinterpret_cast<unsigned*>(to), top);
 }
+
+// The norm of a row for the bound of the slopes.  A row that is not finite has none: its own gradients are not numbers whatever the scale, and
+// the other sequences of the call keep theirs (squares of float16 numbers are far from the largest of 32 bits).
+__device__ __forceinline__ float finite_norm(float square) { return square < INFINITY ? sqrtf(square) : 0.0f; }
 
 // Rows of the tiles' sequences: delta = do.o, lse in powers of two (less the lift), the largest norm of do.  A warp looks eight rows up side by
 // side and takes each of them with all its heads, LANES lanes a head.
@@ -561,7 +565,7 @@ __global__ __launch_bounds__(DELTA_THREADS, 4) void attn_delta_kernel(const __gr
           const float lse = a.lse[at];
           a.delta[at] = sum;
           a.lse2[at] = lse == -INFINITY ? INFINITY : lse * LOG2E - down;  // (a row that sees no key has no weights)
-          top = fmaxf(top, sqrtf(square));
+          top = fmaxf(top, finite_norm(square));
         }
       }
     }
@@ -587,7 +591,7 @@ __global__ __launch_bounds__(DELTA_THREADS) void attn_norm_kernel(const __grid_c
     }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) square += __shfl_xor_sync(FULL_MASK, square, o);
-    top = fmaxf(top, sqrtf(square));
+    top = fmaxf(top, finite_norm(square));
   }
   largest_of_cta(top, a.norms + 1);
 }
