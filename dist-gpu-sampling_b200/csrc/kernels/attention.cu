@@ -314,12 +314,13 @@ __device__ __forceinline__ void add_keys(int first, float (&v)[VEC]) {
     for (int e = 0; e < VEC; ++e) v[e] += __shfl_xor_sync(FULL_MASK, v[e], o);
 }
 
-// The sequence of a row, or none (a row outside of all of them)
-__device__ __forceinline__ AttnSeq sequence_of(const AttnArgs& a, const int32_t* map, int row, bool key, bool* found) {
-  const int s = map[row];
+// The sequence of a row, or none (a row outside of all of them); again: the tiles left the row to be made again
+__device__ __forceinline__ AttnSeq sequence_of(const AttnArgs& a, const int32_t* map, int row, bool key, bool* found, bool* again) {
+  const int word = map[row], s = word & ~ATTN_AGAIN;
   AttnSeq e{0, 0, 0, 0};
   *found = false;
-  if (s >= 0 && s < a.seqs) {
+  *again = (word & ATTN_AGAIN) != 0;
+  if (s < a.seqs) {
     e = a.seq[s];
     const int at = row - (key ? e.k0 : e.q0);
     *found = at >= 0 && at < (key ? e.k_len : e.q_len);
@@ -352,7 +353,7 @@ struct Range {
 };
 __device__ __forceinline__ Range range_of(const AttnArgs& a, bool key) {
   const int n = key ? a.n_k : a.n_q;
-  if (a.seqs == 0 || (a.counts[ATTN_KINDS] >> ATTN_HAS_SEVERAL & 1) != 0) return {n, n, 0};
+  if (a.seqs == 0 || (a.counts[ATTN_KINDS] & (1 << ATTN_HAS_SEVERAL | 1 << ATTN_HAS_AGAIN)) != 0) return {n, n, 0};
   // (the plan found all offsets in order)
   const void* p = key ? a.k_offsets : a.q_offsets;
   const int first = static_cast<int>(offset_at(p, a.offsets64, 0)), skip = static_cast<int>(offset_at(p, a.offsets64, a.seqs)) - first;
@@ -368,11 +369,11 @@ __device__ __forceinline__ void each_row(const AttnArgs& a, int64_t task, int64_
   for (; task < all; task += tasks_step) {
     const int batch = static_cast<int>(task / blocks), block = static_cast<int>(task - static_cast<int64_t>(batch) * blocks);
     const int at = batch * a.rows_at_once + lane;
-    bool found = false, take = false;
+    bool found = false, take = false, again;
     AttnSeq e{0, 0, 0, 0};
     if (lane < a.rows_at_once && at < rows) {
-      e = sequence_of(a, map, range.row(at), key, &found);
-      take = mine(e, found);
+      e = sequence_of(a, map, range.row(at), key, &found, &again);
+      take = mine(e, found, again);
     }
     if (!found) e = AttnSeq{0, 0, 0, 0};
     for (unsigned todo = __ballot_sync(FULL_MASK, take); todo != 0; todo &= todo - 1) {
@@ -421,8 +422,8 @@ __global__ __launch_bounds__(ROW_WARPS * 32, R == 1 && !SPLIT ? 4 : 2) void attn
     for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * blocks; t += split_ctas) {
       const int item = static_cast<int>(t / blocks), block = static_cast<int>(t - static_cast<int64_t>(item) * blocks);
       const int4 it = a.splits[item];
-      bool found;
-      const AttnSeq e = sequence_of(a, a.q_seq, it.x, false, &found);
+      bool found, again;
+      const AttnSeq e = sequence_of(a, a.q_seq, it.x, false, &found, &again);
       const int c = block * w.side + w.head, j0 = it.y, j1 = min(found ? keys_seen(a, e, it.x) : 0, j0 + ATTN_SPLIT_KEYS);
       const bool in = w.in_d && c < a.kv_heads;
       const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
@@ -503,7 +504,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, R == 1 && !SPLIT ? 4 : 2) void attn
   }
   each_row(
       a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, Range{a.n_q, a.n_q, 0}, blocks, a.q_seq, false,
-      [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e)); },
+      [&](const AttnSeq& e, bool found, bool again) { return !found || again || !(attn_in_tiles(a, e) || attn_is_split(a, e)); },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = keys_seen(a, e, row), c = block * w.side + w.head;
         const bool in = w.in_d && c < a.kv_heads;
@@ -566,7 +567,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32, R == 1 ? 3 : 2) void attn_single_ba
   each_row(
       a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, Range{a.n_q, a.n_q, 0}, blocks,
       a.q_seq, false,
-      [&](const AttnSeq& e, bool found) { return found && !attn_in_tiles(a, e) && attn_is_single(a, e); },
+      [&](const AttnSeq& e, bool found, bool) { return found && !attn_in_tiles(a, e) && attn_is_single(a, e); },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = e.k_len, c = block * w.side + w.head;  // (the one query sees all keys, causal or not)
         const bool in = w.in_d && c < a.kv_heads;
@@ -768,8 +769,8 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
     for (int64_t t = blockIdx.x; t < static_cast<int64_t>(n) * blocks; t += split_ctas) {
       const int item = static_cast<int>(t / blocks), block = static_cast<int>(t - static_cast<int64_t>(item) * blocks);
       const int4 it = a.splits[item];
-      bool found;
-      const AttnSeq e = sequence_of(a, a.q_seq, it.x, false, &found);
+      bool found, again;
+      const AttnSeq e = sequence_of(a, a.q_seq, it.x, false, &found, &again);
       const int c = block * w.side + w.head, j0 = it.y, j1 = min(found ? keys_seen(a, e, it.x) : 0, j0 + ATTN_SPLIT_KEYS);
       const bool in = w.in_d && c < a.kv_heads;
       const T* k = static_cast<const T*>(a.k.p) + e.k0 * a.k.row + c * a.k.head + w.vec * VEC;
@@ -836,7 +837,9 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dq_kernel(const _
   }
   each_row(
       a, static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp, static_cast<int64_t>(gridDim.x) * ROW_WARPS, range_of(a, false), blocks, a.q_seq, false,
-      [&](const AttnSeq& e, bool found) { return !found || !(attn_in_tiles(a, e) || attn_is_split(a, e) || attn_is_single(a, e)); },
+      [&](const AttnSeq& e, bool found, bool again) {
+        return !found || again || !(attn_in_tiles(a, e) || attn_is_split(a, e) || attn_is_single(a, e));
+      },
       [&](int row, int block, const AttnSeq& e) {
         const int seen = keys_seen(a, e, row), c = block * w.side + w.head;
         const bool in = w.in_d && c < a.kv_heads;
@@ -874,11 +877,11 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dkv_kernel(const 
   for (int64_t task = static_cast<int64_t>(blockIdx.x) * ROW_WARPS + warp; task < all; task += static_cast<int64_t>(gridDim.x) * ROW_WARPS) {
     const int batch = static_cast<int>(task / blocks), block = static_cast<int>(task - static_cast<int64_t>(batch) * blocks);
     const int begin = batch * a.rows_at_once, mine = begin + lane;
-    bool found = false, take = false;
+    bool found = false, take = false, again;
     AttnSeq own{0, 0, 0, 0};
     if (lane < a.rows_at_once && mine < range.rows) {
-      own = sequence_of(a, a.k_seq, range.row(mine), true, &found);
-      take = !found || !(attn_in_tiles(a, own) || attn_is_single(a, own));
+      own = sequence_of(a, a.k_seq, range.row(mine), true, &found, &again);
+      take = !found || again || !(attn_in_tiles(a, own) || attn_is_single(a, own));
       if (!found) own = AttnSeq{0, 0, 0, 0};
     }
     unsigned todo = __ballot_sync(FULL_MASK, take);

@@ -38,7 +38,7 @@ struct AttnArgs {
   void *dq, *dk, *dv;
   // workspace
   AttnSeq* seq;                 // [seqs]
-  int32_t *q_seq, *k_seq;       // the sequence of a row; only entries whose sequence holds the row mean anything
+  int32_t *q_seq, *k_seq;       // the sequence of a row (ATTN_AGAIN beside it); only entries whose sequence holds the row mean anything
   int32_t* counts;              // ATTN_COUNTS words
   int4* splits;                 // {row, first key, index of the row's first part, parts}
   uint32_t* arrived;            // parts that are there, one word for each part (the first of a row's is used) and key head
@@ -54,7 +54,11 @@ struct AttnArgs {
 };
 
 enum { ATTN_N_SPLITS = 0, ATTN_N_Q_TILES = 1, ATTN_N_K_TILES = 2, ATTN_KINDS = 3, ATTN_COUNTS = 8 };
-enum { ATTN_HAS_TILES = 0, ATTN_HAS_SINGLE = 1, ATTN_HAS_SEVERAL = 2 };  // bits of the word ATTN_KINDS
+enum { ATTN_HAS_TILES = 0, ATTN_HAS_SINGLE = 1, ATTN_HAS_SEVERAL = 2, ATTN_HAS_AGAIN = 3 };  // bits of the word ATTN_KINDS
+
+// A row of a causal tile whose result is not a number although it may have to be one: a pair that is masked has the weight 0, and 0 times what is
+// not finite is not a number.  The rows' kernels, which come after the tiles' and read what a row sees alone, make it again.
+constexpr int32_t ATTN_AGAIN = INT32_MIN;
 
 constexpr int ATTN_MAX_D = 128;
 // keys from which a CTA takes a row instead of a warp.  8 heads on 2, width 64, bf16, us forward / backward with 256 and with 512 here: 2 000

@@ -209,6 +209,12 @@ struct Items {
   }
 };
 
+// a row that the rows' kernels have to make again (ATTN_AGAIN)
+__device__ __forceinline__ void leave_row(const AttnArgs& a, int32_t* map, int row) {
+  atomicOr(&map[row], ATTN_AGAIN);
+  atomicOr(&a.counts[ATTN_KINDS], 1 << ATTN_HAS_AGAIN);
+}
+
 // ---- forward ----------------------------------------------------------------------------------------------------------
 template <int DP>
 struct ForwardShape {
@@ -446,6 +452,7 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
       if (below >= x.rows) continue;
       const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (nan stays nan)
       char* to = static_cast<char*>(a.out) + ((static_cast<int64_t>(x.row + mine) * a.heads + head) * a.d) * 2;
+      bool nan = false;
 #pragma unroll
       for (int q = 0; q < DP / 32; ++q) {
         uint32_t r[32];
@@ -460,11 +467,14 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_forward_kernel(const __g
           for (int e = 0; e < 4; ++e) {
             const float lo = __uint_as_float(r[i * 8 + e * 2]) * inv, hi = __uint_as_float(r[i * 8 + e * 2 + 1]) * inv;
             y[e] = l == 0.0f ? 0u : pack2<BF16>(lo, hi);
+            nan |= lo != lo || hi != hi;
           }
           if (there && q * 32 + i * 8 < a.d) *reinterpret_cast<uint4*>(to + (q * 32 + i * 8) * 2) = make_uint4(y[0], y[1], y[2], y[3]);
         }
       }
       fence_before();
+      // (a sum of the weights that is not a number: neither is the row, by its own scores)
+      if (a.causal && there && nan && l > 0.0f) leave_row(a, a.q_seq, x.row + mine);
       if (there) a.lse[static_cast<int64_t>(head) * a.n_q + x.row + mine] = l == 0.0f ? -INFINITY : (ref - LIFT + log2f(l)) * LN2;
     }
   }
@@ -504,8 +514,8 @@ constexpr int DELTA_THREADS = 256;
 
 // the sequence of a row is one of the tiles'
 __device__ __forceinline__ bool in_a_tile(const AttnArgs& a, const int32_t* map, int row, bool key) {
-  const int s = map[row];
-  if (s < 0 || s >= a.seqs) return false;
+  const int s = map[row] & ~ATTN_AGAIN;
+  if (s >= a.seqs) return false;
   const AttnSeq e = a.seq[s];
   const int at = row - (key ? e.k0 : e.q0);
   return at >= 0 && at < (key ? e.k_len : e.q_len) && attn_in_tiles(a, e);
@@ -604,9 +614,10 @@ struct BackwardShape {
                             BARS = STATS + 2 * 2 * ATTN_TILE * 4, SMEM = BARS + 256;
 };
 
-// a row of DP values out of TMEM, times `by`, into contiguous rows of d elements
+// a row of DP values out of TMEM, times `by`, into contiguous rows of d elements; whether one of them is not a number
 template <int FROM, int TO, bool BF16>
-__device__ __forceinline__ void store_row(uint32_t tmem, bool there, float by, char* to, int d) {
+__device__ __forceinline__ bool store_row(uint32_t tmem, bool there, float by, char* to, int d) {
+  bool nan = false;
 #pragma unroll
   for (int q = FROM / 32; q < TO / 32; ++q) {
     uint32_t r[32];
@@ -616,10 +627,15 @@ __device__ __forceinline__ void store_row(uint32_t tmem, bool there, float by, c
     for (int i = 0; i < 4; ++i) {
       uint32_t y[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = pack2<BF16>(__uint_as_float(r[i * 8 + e * 2]) * by, __uint_as_float(r[i * 8 + e * 2 + 1]) * by);
+      for (int e = 0; e < 4; ++e) {
+        const float lo = __uint_as_float(r[i * 8 + e * 2]) * by, hi = __uint_as_float(r[i * 8 + e * 2 + 1]) * by;
+        y[e] = pack2<BF16>(lo, hi);
+        nan |= lo != lo || hi != hi;
+      }
       if (there && q * 32 + i * 8 < d) *reinterpret_cast<uint4*>(to + (q * 32 + i * 8) * 2) = make_uint4(y[0], y[1], y[2], y[3]);
     }
   }
+  return nan;
 }
 template <int FROM, int TO>
 __device__ __forceinline__ void store_zeros(bool there, char* to, int d) {
@@ -836,7 +852,8 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
       if (!(ok = wait.warp(done, items_done++ & 1))) break;
       fence_after();
       const float last = half ? a.scale / (by * exp2f(lift<BF16>())) : exp2f(-lift<BF16>());
-      store_row<0, DP, BF16>(tmem + 256 + half * DP + lanes, there, last, to, a.d);
+      const bool nan = store_row<0, DP, BF16>(tmem + 256 + half * DP + lanes, there, last, to, a.d);
+      if (a.causal && there && nan) leave_row(a, a.k_seq, x.row + mine);
       fence_before();
     }
   }
@@ -1061,8 +1078,10 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dq_kernel(const __grid_c
       fence_after();
       const float last = a.scale / (by * exp2f(lift<BF16>()));
       const bool wanted = there && a.dq != nullptr;
-      if (half) store_row<DP / 2, DP, BF16>(tmem + 384 + lanes, wanted, last, to, a.d);
-      else store_row<0, DP / 2, BF16>(tmem + 384 + lanes, wanted, last, to, a.d);
+      const bool nan = half ? store_row<DP / 2, DP, BF16>(tmem + 384 + lanes, wanted, last, to, a.d)
+                            : store_row<0, DP / 2, BF16>(tmem + 384 + lanes, wanted, last, to, a.d);
+      // (a delta or lse that is not a number: neither is the row, if it sees a key)
+      if (a.causal && wanted && nan && !(seen > 0 && (delta != delta || lse != lse))) leave_row(a, a.q_seq, x.row + mine);
       fence_before();
     }
   }
