@@ -99,10 +99,11 @@ def _define():
 
     class Linear8bit(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, x, weight, bias):
-            rows = x.reshape(-1, x.shape[-1])
+        def forward(ctx, x, weight, bias, recorded):
             ctx.shape = x.shape
-            ctx.save_for_backward(weight, *ops._CAPI_keep_8bit(rows) if ctx.needs_input_grad[1] else ())
+            # (needs_input_grad is true of a trainable weight where nothing is recorded, too)
+            keep = recorded and ctx.needs_input_grad[1]
+            ctx.save_for_backward(weight, *ops._CAPI_keep_8bit(x.reshape(-1, x.shape[-1])) if keep else ())
             with torch.autocast("cuda", enabled=False):  # (the caller's types, here and in the backward pass)
                 return torch.nn.functional.linear(x, weight, bias)
 
@@ -110,7 +111,7 @@ def _define():
         @torch.autograd.function.once_differentiable
         def backward(ctx, grad):
             weight, *kept = ctx.saved_tensors
-            want_x, want_w, want_b = ctx.needs_input_grad
+            want_x, want_w, want_b, _ = ctx.needs_input_grad
             rows = grad.reshape(-1, grad.shape[-1])
             dw = db = None
             if want_w:
@@ -119,7 +120,7 @@ def _define():
                 db = rows.sum(0, dtype=torch.float32).to(grad.dtype)
             with torch.autocast("cuda", enabled=False):
                 dx = (rows @ weight).view(ctx.shape) if want_x else None
-            return dx, dw, db if want_b else None
+            return dx, dw, db if want_b else None, None
 
     _functions.update(norm=LayerNorm, loss=LinearCrossEntropy, attention=Attention, residual=ResidualNorm, linear=Linear8bit)
 
@@ -207,12 +208,13 @@ def linear_8bit(x, weight, bias=None):
     """x @ weight.T + bias whose input is kept for the backward pass in 8 bits (keep_8bit) instead of its own type: half the memory of
     16-bit activations, a quarter of 32-bit ones.  The result and the gradient of x are those of torch's linear; the weight's gradient is
     taken from the kept rows, in one pass over their codes.  x [..., D], weight [O, D] and bias [O] of one type (16 bits run on the tensor
-    cores)."""
+    cores).  Nothing is kept without gradients (torch.no_grad, a weight that needs none)."""
+    import torch
     if not _functions:
         _define()
     if x.dtype != weight.dtype or (bias is not None and bias.dtype != weight.dtype):
         raise ValueError("linear_8bit: x, weight and bias must share one type")
-    return _functions["linear"].apply(x, weight, bias)
+    return _functions["linear"].apply(x, weight, bias, torch.is_grad_enabled())
 
 
 class AdamW:
