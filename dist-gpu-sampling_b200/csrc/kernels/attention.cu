@@ -944,19 +944,33 @@ struct Layout {
   }
 };
 
-// Parts that rows with many keys can have, whatever the offsets: parts <= k_len / ATTN_SPLIT_KEYS + 1 for each of a sequence's queries
+// whether sequences may go to the tensor cores (a scale that is not positive, which no model has, stays on the CUDA cores: the tiles take the largest
+// score for the largest weight)
+bool has_tiles(const dgs_attention& p) {
+  return p.dtype != DGS_F32 && p.n_q >= ATTN_FEW_QUERIES && p.n_k > 0 && p.seqs > 0 && p.scale > 1e-30f;
+}
+
+// Parts that rows with many keys can have, whatever the offsets: k keys are ceil(k / ATTN_SPLIT_KEYS) <= k / ATTN_SPLIT_KEYS + 1 parts for each of a
+// sequence's queries.  Where many sequences are just long enough, keys are the bound: 2 parts for ATTN_SPLIT_KEYS + 1 of them is the most (as
+// 1 for ATTN_SPLIT_FROM + 1 nearly is), and with tiles, which take ATTN_FEW_QUERIES and more over up to ATTN_MANY_KEYS, 5 for ATTN_MANY_KEYS + 1.
 // (none, and no launch for them, where all keys together are too few for one: whether a row is split is a matter of its own keys alone)
-int64_t split_bound(int64_t n_q, int64_t n_k, int64_t seqs) {
-  if (n_k <= ATTN_SPLIT_FROM) return 0;
-  const int64_t queries = n_q < ATTN_SPLIT_QUERIES ? n_q : ATTN_SPLIT_QUERIES;
-  const int64_t longest = n_k / (ATTN_SPLIT_FROM + 1), some = ATTN_SPLIT_QUERIES * (longest < seqs ? longest : seqs);
-  return queries * (n_k / ATTN_SPLIT_KEYS) + (n_q < some ? n_q : some);
+int64_t split_bound(const dgs_attention& p) {
+  if (p.n_k <= ATTN_SPLIT_FROM) return 0;
+  static_assert(2 * (ATTN_SPLIT_FROM + 1) >= ATTN_SPLIT_KEYS + 1 && ATTN_MANY_KEYS == 4 * ATTN_SPLIT_KEYS, "parts of a key");
+  const int64_t queries = p.n_q < ATTN_SPLIT_QUERIES ? p.n_q : ATTN_SPLIT_QUERIES;
+  const int64_t longest = p.n_k / (ATTN_SPLIT_FROM + 1), some = ATTN_SPLIT_QUERIES * (longest < p.seqs ? longest : p.seqs);
+  const int64_t by_rows = queries * (p.n_k / ATTN_SPLIT_KEYS) + (p.n_q < some ? p.n_q : some);
+  const bool tiles = has_tiles(p);
+  const int64_t few = tiles && queries >= ATTN_FEW_QUERIES ? ATTN_FEW_QUERIES - 1 : queries;
+  int64_t by_keys = few * 2 * p.n_k / (ATTN_SPLIT_KEYS + 1);
+  if (tiles && by_keys < queries * 5 * p.n_k / (ATTN_MANY_KEYS + 1)) by_keys = queries * 5 * p.n_k / (ATTN_MANY_KEYS + 1);
+  return by_rows < by_keys ? by_rows : by_keys;
 }
 
 // Workspace of a call; `base` == nullptr: its size alone
 int64_t lay_out(const dgs_attention& p, bool backward, char* base, AttnArgs* a) {
   Layout l;
-  a->split_bound = static_cast<int32_t>(split_bound(p.n_q, p.n_k, p.seqs));
+  a->split_bound = static_cast<int32_t>(split_bound(p));
   const int64_t floats = backward ? 2 * p.d + 1 : p.d + 2;
   auto at = [&](int64_t bytes) { return base + l.take(bytes); };
   a->counts = reinterpret_cast<int32_t*>(at(ATTN_COUNTS * 4));
@@ -968,8 +982,7 @@ int64_t lay_out(const dgs_attention& p, bool backward, char* base, AttnArgs* a) 
   a->arrived = reinterpret_cast<uint32_t*>(at(int64_t(4) * a->split_bound * p.kv_heads));
   a->parts = reinterpret_cast<float*>(at(int64_t(4) * a->split_bound * p.heads * floats));
   a->delta = reinterpret_cast<float*>(at(backward ? int64_t(4) * p.heads * p.n_q : 0));
-  // (a scale that is not positive, which no model has, stays on the CUDA cores: the tiles take the largest score for the largest weight)
-  a->tiles = p.dtype != DGS_F32 && p.n_q >= ATTN_FEW_QUERIES && p.n_k > 0 && p.seqs > 0 && p.scale > 1e-30f;
+  a->tiles = has_tiles(p);
   // forward, a CTA's two tiles of queries: the same rows of two heads that share their keys, or neighbouring rows
   a->head_pairs = p.heads / p.kv_heads % 2 == 0;
   a->q_tile_rows = backward || a->head_pairs ? ATTN_TILE : 2 * ATTN_TILE;
@@ -1005,7 +1018,7 @@ int check(const char* who, const dgs_attention* p) {
   DGS_REQUIRE((p->n_q == 0 || p->q != nullptr) && (p->n_k == 0 || (p->k != nullptr && p->v != nullptr)) &&
                   p->q_offsets != nullptr && p->k_offsets != nullptr,
               DGS_ERR_INVALID, "%s: null argument", who);
-  DGS_REQUIRE(split_bound(p->n_q, p->n_k, p->seqs) < (int64_t(1) << 27), DGS_ERR_INVALID, "%s: too many rows", who);
+  DGS_REQUIRE(split_bound(*p) < (int64_t(1) << 27), DGS_ERR_INVALID, "%s: too many rows", who);
   return DGS_OK;
 }
 
