@@ -923,6 +923,14 @@ __global__ __launch_bounds__(ROW_WARPS * 32, 2) void attn_rows_dkv_kernel(const 
             add_scaled<VEC>(ds, q[r], dk);
           }
         }
+        // what is not a number stays so: long sequences made again after a step that went wrong altogether end here (4 causal ones of 8 192 tokens,
+        // forward and backward: 5.1 ms of numbers, 7.7 with q and v all nan, 370 without this; 95 with one nan, in the first value)
+        if ((i & 31) == 31) {
+          bool gone = true;
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) gone &= dk[x] != dk[x] && dv[x] != dv[x];
+          if (__all_sync(FULL_MASK, gone || !in)) break;
+        }
       }
       if (!in) continue;
 #pragma unroll

@@ -84,3 +84,28 @@ def test_queries_that_see_no_key(ops, dtype):
         dq = ops._CAPI_attention_backward(do, *t[:3], out, lse, qo, ko, True, 0.125, True, True)[0]
         assert (out[:lq - lk] == 0).all() and (lse[:, :lq - lk] == -math.inf).all() and (dq[:lq - lk] == 0).all()
         assert out[lq - lk:].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_step_that_went_wrong_altogether(ops, dtype):
+    """Nothing but nan in one of the sequences: its results are nan, the others' bits are what they were."""
+    lens = [100, 600, 40]
+    q, k, v, do = make(lens, lens, 4, 2, 64, dtype)
+    o = offsets(lens)
+
+    def both(q, k, v, do):
+        out, lse = ops._CAPI_attention(q, k, v, o, o, True, 0.125)
+        return (out, *ops._CAPI_attention_backward(do, q, k, v, out, lse, o, o, True, 0.125, True, True))
+
+    v[:100] *= 2.0  # (the bound by which float16 slopes are scaled is the first sequence's)
+    do[:100] *= 2.0
+    base = both(q, k, v, do)
+    for which in ((0, 1, 2, 3), (0, 2), (2,), (3,)):
+        t = [x.clone() for x in (q, k, v, do)]
+        for i in which:
+            t[i][100:700] = math.nan
+        got = both(*t)
+        for a, b in zip(got, base):
+            assert torch.equal(a[:100], b[:100]) and torch.equal(a[700:], b[700:])
+        assert got[1][100:700].isnan().all() and got[2][100:700].isnan().all()
+        assert got[0][100:700].isnan().all() == (which != (3,)) and got[3][100:700].isnan().all() == (which != (2,))
