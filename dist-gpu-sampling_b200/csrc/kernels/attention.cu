@@ -405,8 +405,8 @@ __device__ __forceinline__ bool last_part(const AttnArgs& a, const int4& it, int
 
 // Forward.  Rows with up to ATTN_SPLIT_FROM keys: a warp each, for all the key heads side by side.  SPLIT: CTAs take the parts of rows with
 // many keys; the last part of a row to be there joins them in their order.  Bound by HBM where every query has keys of its own: what is
-// under way is many warps with few keys each for short rows (60 000 seeds of 7.5 keys: 144 us with 32 warps an SM and two keys, 169 with
-// 16 and four), more keys a warp for long ones.
+// under way is many warps with few keys each for short rows (60 000 seeds of 7.5 keys: 144 us with 32 warps an SM and two keys against 169 with
+// 16 and four when that was chosen, 127 now), more keys a warp for long ones.
 template <typename T, int DP, int R, bool SPLIT>
 __global__ __launch_bounds__(ROW_WARPS * 32, R == 1 && !SPLIT ? 4 : 2) void attn_rows_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int VEC = vec_of<T>(), G = lanes_of<T, DP>(), U = R == 2 ? 4 : 2, SPLIT_U = R == 1 ? 4 : 2;

@@ -62,7 +62,8 @@ constexpr int32_t ATTN_AGAIN = INT32_MIN;
 
 constexpr int ATTN_MAX_D = 128;
 // keys from which a CTA takes a row instead of a warp.  8 heads on 2, width 64, bf16, us forward / backward with 256 and with 512 here: 2 000
-// rows of 500 keys 287 / 1 650 and 185 / 559, one row of 500 keys 25 / 38 and 38 / 81; with 1 024: one row of 1 000 keys 36 / 54 and 68 / 153
+// rows of 500 keys 287 / 1 650 and 185 / 702, one row of 500 keys 25 / 38 and 38 / 114; with 1 024, when a warp took its keys once backward: one
+// row of 1 000 keys 36 / 54 and 68 / 153
 constexpr int ATTN_SPLIT_FROM = 512;
 constexpr int ATTN_SPLIT_KEYS = 1024;  // so many of them at a time
 constexpr int ATTN_SPLIT_QUERIES = 16; // (with more queries there are warps enough)

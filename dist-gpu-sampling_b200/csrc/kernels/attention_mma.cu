@@ -15,9 +15,9 @@
 // Whole tiles travel by TMA.  Where a product's sum runs over a tile's rows, rows behind a sequence's end have to be zeros, not the next
 // sequence's: such last tiles come row by row through cp.async.
 // Every wait is bounded; a wait that runs out raises DGS_ERR_CUDA in the status word and all roles leave.
-// Measured, bfloat16: 4 causal sequences of 8 192 tokens, 16 heads of 128 on 4, forward 1 086 us = 1 013 TFLOP/s, backward 4 192 us = 656 of
-// the 5 products that are needed; bound by the exponentials and slopes beside the products.  320 of 100 tokens, 8 heads of 64 on 2: 78 and
-// 178 us, bound by launches and half-filled tiles (tensor pipe 17 to 24 % active on ragged lengths).
+// Measured, bfloat16: 4 causal sequences of 8 192 tokens, 16 heads of 128 on 4, forward 1 053 us = 1 044 TFLOP/s, backward 4 310 us = 638 of
+// the 5 products that are needed; bound by the exponentials and slopes beside the products.  320 of 100 tokens, 8 heads of 64 on 2: 86 and
+// 185 us, bound by launches and half-filled tiles (tensor pipe 17 to 23 % active on ragged lengths).
 #include <type_traits>
 
 #include "attention.h"
@@ -871,9 +871,11 @@ __global__ __launch_bounds__(TILE_THREADS, 1) void attn_dkv_kernel(const __grid_
 }
 
 // dQ of 128 queries of one head.  A query that sees a tile's keys at the most has delta = sum_j p_j e_j of values that its two threads hold
-// anyway, in 32 bits, and leaves it for the gradients of the keys, which follow: do.o of an `out` rounded to 16 bits is off most where few
-// keys were averaged.  Errors of dq and dk, causal, against rounding the exact ones: 40 tokens 1.57 -> 1.41 times, 100 tokens 1.51 -> 1.41
-// (what is left is the rounding of dS to 16 bits, which its products ask for).
+// anyway, in 32 bits, and leaves it for the gradients of the keys, which follow.  Errors of dq and dk, causal, against rounding the exact ones:
+// 40 tokens 1.57 -> 1.41 times, 100 tokens 1.51 -> 1.41 (what is left is the rounding of dS to 16 bits, which its products ask for).  A query
+// over more keys has delta = do.o from `out` as it is stored: both products and the exponentials twice would be the price of the other (7 products
+// a pair of tiles -> 9).  Its rounding goes with the size of out: 1.45 times for v and do around 0, whatever the keys, but with a mean of 1 in both (of
+// 3) dq is off by 2.3 (5.7) times over 200 keys, 3.2 (7.8) over 1 000, dk by 1.6 (2.9) and 1.3 (1.7).
 __device__ __forceinline__ int first_seen(const AttnArgs& a, const AttnTile& x) { return a.causal ? min(x.seen, x.others) : x.others; }
 // (without dq: only what the deltas need, so that the gradients of the keys are the same bits whether dq is wanted or not)
 __device__ __forceinline__ int query_steps(const AttnArgs& a, const AttnTile& x) {

@@ -6,8 +6,8 @@
 // products (cta_group::1, two accumulators of 128 x 256 in TMEM).  The next blocks are on their way in registers.
 // With few results the rows are cut into shares that fill the SMs; shares are added in their order by a second launch.
 // Every wait is bounded; one that runs out raises DGS_ERR_CUDA in the status word, leaves no number among the CTA's results, and all roles leave.
-// Bound by turning codes into operands: 430 000 rows of 256 against 47 (358 bytes a row) 57 us = 2.7 TB/s, 16 384 x 4 096 against 1 024 168 us =
-// 820 TFLOP/s with the tensor pipe 40 % active, each with 9 to 10 us of joins behind it.
+// Bound by turning codes into operands: 430 000 rows of 256 against 47 (358 bytes a row) 55 us = 2.8 TB/s, 16 384 x 4 096 against 1 024 165 us =
+// 833 TFLOP/s with the tensor pipe 41 % active, each with 9 to 10 us of joins behind it.
 #include "kept.h"
 #include "tensor_core.cuh"
 

@@ -164,7 +164,9 @@ def attention(q, k, v, q_offsets, k_offsets=None, causal=False, scale=None, retu
     causal: query i of Lq sees the keys j <= i + Lk - Lq (the last query sees all of them).  scale: 1 / sqrt(d) by default.  A query that
     sees no key gives zeros, and so do rows outside of all sequences.  return_lse: also the logarithm of the sum of exponentials
     [heads, n_q] (float32, without a gradient; -inf where no key is seen).  Sequences of 24 queries and more (8 over
-    many keys) run on the tensor cores in 16 bits; float32 runs on the CUDA cores.  Gradients are added in a fixed order."""
+    many keys) run on the tensor cores in 16 bits; float32 runs on the CUDA cores.  Gradients are added in a fixed order (those of `k[indices]`
+    back into k are torch's, by atomics).  A number that is not finite reaches what depends on it: other sequences, and causal queries
+    that do not see it, keep their results."""
     if k_offsets is None:
         k_offsets = q_offsets
     if not _functions:
@@ -208,7 +210,8 @@ def linear_8bit(x, weight, bias=None):
     """x @ weight.T + bias whose input is kept for the backward pass in 8 bits (keep_8bit) instead of its own type: half the memory of
     16-bit activations, a quarter of 32-bit ones.  The result and the gradient of x are those of torch's linear; the weight's gradient is
     taken from the kept rows, in one pass over their codes.  x [..., D], weight [O, D] and bias [O] of one type (16 bits run on the tensor
-    cores).  Nothing is kept without gradients (torch.no_grad, a weight that needs none)."""
+    cores).  Nothing is kept without gradients (torch.no_grad, a weight that needs none).  Where another operator keeps x anyway (attention
+    keeps its result), or two layers read it, the codes come on top, once for each layer."""
     import torch
     if not _functions:
         _define()
